@@ -245,7 +245,7 @@ def _plain_layout(s):
     j = torch.searchsorted(b_upto, b, right=True)
     first = (b - (b_upto - nb)[j]) * block
     out = {"positions": pos, "slots": slots, "rb_req": req[j], "rb_qstart": row0[j] + first, "rb_qcount": torch.minimum(count[j] - first, torch.full_like(first, block)),
-           "rb_ctx": start[j] + first + 1, "row0": row0, "logit_rows": rows - 1}
+           "rb_ctx": start[j] + first + 1, "row0": row0, "logit_rows": torch.where(count > 0, rows - 1, -1)}
     if pad > T:
         tail = torch.arange(T, pad, device=dev)
         zero = torch.zeros_like(tail)
