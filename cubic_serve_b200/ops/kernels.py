@@ -717,6 +717,240 @@ def verify_sampled(q_val: torch.Tensor, q_id: torch.Tensor, p_val: torch.Tensor,
     native.check(code, "cb_verify_sampled")
 
 
+# ------------------------------------------------------------------ what a step does for each of its requests
+def _require(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _device_of(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
+    """The one GPU of an operator's tensors."""
+    dev = first.device
+    _require(dev.type == "cuda", "tensors must be on a GPU")
+    for t in others:
+        _require(t is None or t.device == dev, "tensors must be on one GPU")
+    return dev
+
+
+def _call(dev: torch.device, entry: str, *args) -> None:
+    """Launch on the current stream of the tensors' own GPU, whichever is the current one."""
+    if dev.index == torch.cuda.current_device():
+        code = getattr(native.lib(), entry)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            code = getattr(native.lib(), entry)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    native.check(code, entry)
+
+
+def _vector(t: torch.Tensor | None, dtype: torch.dtype, n: int, name: str) -> int | None:
+    """Address of an optional contiguous vector of at least ``n`` elements."""
+    if t is None:
+        return None
+    _require(t.dtype == dtype and t.dim() == 1 and t.numel() >= n and (t.numel() <= 1 or t.stride(0) == 1), f"{name}: a contiguous {dtype} vector of {n} elements")
+    return t.data_ptr()
+
+
+class StepLayout:
+    """Fixed-address outputs of ``step_layout`` for up to ``max_tokens`` rows, ``max_requests`` requests and ``max_blocks`` row
+    blocks: what the cache write and the attention of a step read (``positions``, ``slots``, ``rb_*``), the first row of every
+    request (``row0``), its last (``logit_rows``, int64, -1: no new tokens) and ``totals``: rows, row blocks and pages taken,
+    and what went wrong (``WRONG``).  ``into``: buffers to use in place of new ones, by name."""
+
+    WRONG = {1: "not enough pages", 2: "a request is longer than the block table is wide", 4: "a row that the block table does not have",
+             8: "more rows or row blocks than there is room for"}
+
+    def __init__(self, max_tokens: int, max_requests: int, max_blocks: int, device, into: dict | None = None) -> None:
+        _require(max_tokens >= 0 and max_blocks >= 0 and 0 <= max_requests <= 4096, "a layout holds up to 4096 requests")
+        sizes = {"positions": max_tokens, "slots": max_tokens, "rb_req": max_blocks, "rb_qstart": max_blocks, "rb_qcount": max_blocks,
+                 "rb_ctx": max_blocks, "row0": max_requests, "logit_rows": max_requests, "totals": 4}
+        self.max_tokens, self.max_requests, self.max_blocks = max_tokens, max_requests, max_blocks
+        into = into or {}
+        _require(set(into) <= set(sizes), f"unknown buffers {sorted(set(into) - set(sizes))}")
+        s = self._struct = native.StepLayoutStruct()
+        for name, n in sizes.items():
+            dt = torch.int64 if name == "logit_rows" else torch.int32
+            t = into[name] if name in into else torch.zeros(n, dtype=dt, device=device)
+            setattr(s, name, _vector(t, dt, n, name))
+            setattr(self, name, t)
+        self.device = self.totals.device
+
+    def check(self) -> None:
+        """Raise if the last layout met a request that it could not place (reads ``totals``: waits for the GPU)."""
+        wrong = int(self.totals[3].item())
+        if wrong:
+            raise RuntimeError("step layout: " + ", ".join(w for bit, w in self.WRONG.items() if wrong & bit))
+
+
+def step_layout(request: torch.Tensor, start: torch.Tensor, count: torch.Tensor, held: torch.Tensor | None, pages: torch.Tensor,
+                table: torch.Tensor, out: StepLayout, block: int, tokens: int, blocks: int, pad: int = 0) -> StepLayout:
+    """Lay a step out from the lengths of its requests (``csrc/step_layout.cu``).
+
+    ``request`` int32 ``[n]``: rows of the block table, none of them twice; ``start`` / ``count``: tokens in the cache and new
+    tokens; ``held``: pages in the row already (None: those of ``start`` tokens).  Requests take their missing pages from
+    ``pages`` (int32, in their order) into ``table`` (int32 ``[rows, width]``, written in place).  ``block``: positions of a
+    row block.  ``tokens`` / ``blocks``: rows and row blocks to write at most; rows and row blocks behind the last one up to
+    ``pad`` become padding (slot -1, nothing to attend to), what is behind them stays.  A request that cannot be placed gets
+    no slots and attends to nothing; ``out.totals[3]`` says why."""
+    n = start.numel()
+    _require(n <= out.max_requests and 0 <= tokens <= out.max_tokens and 0 <= blocks <= out.max_blocks and pad <= min(out.max_tokens, out.max_blocks),
+             "more rows, row blocks or requests than the layout holds")
+    _require(1 <= block <= 1 << 20, "a row block holds at least one position")
+    _require(table.dtype == torch.int32 and table.dim() == 2 and table.stride(1) == 1 and table.stride(0) >= table.shape[1], "the block table is int32 with rows of neighbouring entries")
+    s = native.StepLayoutStruct.from_buffer_copy(out._struct)
+    i32 = torch.int32
+    s.request, s.start, s.count = _vector(request, i32, n, "request"), _vector(start, i32, n, "start"), _vector(count, i32, n, "count")
+    s.held, s.pages = _vector(held, i32, n, "held"), _vector(pages, i32, 0, "pages")
+    s.table, s.table_rows, s.width, s.ld = table.data_ptr(), table.shape[0], table.shape[1], table.stride(0)
+    s.n, s.num_pages, s.block, s.cap_tokens, s.cap_blocks, s.pad = n, pages.numel(), block, max(tokens, pad), max(blocks, pad), max(0, pad)
+    _call(_device_of(start, request, count, held, pages, table, out.totals), "cb_step_layout", ctypes.byref(s))
+    return out
+
+
+class AdapterBank:
+    """The low-rank adapters of one projection: ``a`` bf16 ``[slots, sections * rank, k]``, ``b`` bf16 ``[slots, n, rank]``,
+    ``scale`` fp32 ``[slots]``.  ``widths``: columns of the projection's sections (q | k | v), each with its own ranks of
+    ``a``; all but the last a multiple of 32.  ``ranks`` int32 ``[slots]``: ranks in use of every adapter (0: an empty slot).
+
+    Ranks up to 128; one that is not 16, 32, 64 or 128 is stored with zeros up to the next.  Tensors that need none are kept as
+    they are: what is copied into them later takes effect (``load`` writes one slot)."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, widths: tuple[int, ...] | None = None, ranks: torch.Tensor | None = None) -> None:
+        _require(a.dtype == b.dtype == torch.bfloat16 and a.dim() == b.dim() == 3 and a.shape[0] == b.shape[0], "adapters are bf16 [slots, ranks, k] and [slots, n, rank]")
+        slots, n, rank = b.shape
+        self.widths = tuple(int(w) for w in (widths or (n,)))
+        S = len(self.widths)
+        _require(1 <= slots <= 1023, "a bank holds up to 1023 adapters")
+        _require(1 <= S <= 4 and sum(self.widths) == n and all(w > 0 for w in self.widths) and all(w % 32 == 0 for w in self.widths[:-1]), "one to four sections that cover the columns, all but the last of a multiple of 32")
+        _require(1 <= rank <= 128 and a.shape[1] == S * rank, "ranks up to 128, the same for every section")
+        _require(n % 8 == 0 and a.shape[2] % 8 == 0 and a.shape[2] > 0, "inputs and outputs are multiples of 8")
+        _require(scale.dtype == torch.float32 and scale.shape == (slots,) and scale.is_contiguous(), "one fp32 scale an adapter")
+        _require(ranks is None or (ranks.dtype == torch.int32 and ranks.shape == (slots,) and ranks.is_contiguous()), "ranks: one int32 an adapter")
+        for t in (b, scale, ranks):
+            _require(t is None or t.device == a.device, "tensors must be on one device")
+        full = next(r for r in (16, 32, 64, 128) if r >= rank)
+        self.max_rank = rank
+        if full != rank:
+            a = torch.nn.functional.pad(a.view(slots, S, rank, -1) if a.is_contiguous() else a.reshape(slots, S, rank, -1), (0, 0, 0, full - rank)).reshape(slots, S * full, -1)
+            b = torch.nn.functional.pad(b, (0, full - rank))
+            if ranks is None:
+                ranks = torch.full((slots,), rank, dtype=torch.int32, device=a.device)
+        a, b = a.contiguous(), b.contiguous()
+        _require(a.data_ptr() % 16 == 0 and b.data_ptr() % 16 == 0, "adapters start on a 16-byte boundary")
+        self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
+        self.slots, self.k, self.n, self.rank, self.sections = slots, a.shape[2], n, full, S
+        s = self._struct = native.AdapterStruct()
+        s.a, s.b, s.scale, s.ranks = a.data_ptr(), b.data_ptr(), scale.data_ptr(), _ptr(ranks)
+        s.slots, s.k, s.n, s.rank, s.sections = slots, self.k, n, full, S
+        for i, w in enumerate(self.widths):
+            s.width[i] = w
+
+    def load(self, slot: int, a, b, scale: float) -> None:
+        """Write one adapter: ``a`` / ``b`` a matrix ``[rank, k]`` / ``[width, rank]`` for every section (None: the section has
+        none); ranks below the bank's leave the rest zero."""
+        _require(0 <= slot < self.slots and len(a) == len(b) == self.sections, "no such slot, or not a matrix for every section")
+        col, most = 0, 0
+        for i, (ai, bi) in enumerate(zip(a, b)):
+            at, width = i * self.rank, self.widths[i]
+            _require((ai is None) == (bi is None), "a section has both matrices or none")
+            r = 0 if ai is None else ai.shape[0]
+            _require(r <= self.max_rank and (r == 0 or (tuple(ai.shape) == (r, self.k) and tuple(bi.shape) == (width, r))), f"section {i}: [rank <= {self.max_rank}, {self.k}] and [{width}, rank]")
+            self.a[slot, at:at + self.rank].zero_()
+            self.b[slot, col:col + width].zero_()
+            if r:
+                self.a[slot, at:at + r].copy_(ai)
+                self.b[slot, col:col + width, :r].copy_(bi)
+            col += width
+            most = max(most, r)
+        self.scale[slot] = float(scale)
+        if self.ranks is not None:
+            self.ranks[slot] = most
+
+
+class AdapterRows:
+    """A step's rows sorted by adapter, for all its projections: fixed-address buffers for up to ``max_rows`` rows over
+    ``slots`` adapters.  ``max_ranks``: ranks of the widest projection, summed over its sections.  Steps that may run at the
+    same time (two captured graphs on two streams) need one each."""
+
+    def __init__(self, max_rows: int, slots: int, max_ranks: int, device) -> None:
+        _require(0 < max_rows <= 65535 and 1 <= slots <= 1023 and max_ranks > 0, "up to 65535 rows over up to 1023 adapters")
+        self.max_rows, self.slots, self.rows = max_rows, slots, 0
+        self.max_ranks = max(64, 2 * max_ranks)                     # ranks are stored as 16, 32, 64 or 128
+        self.order = torch.zeros(max_rows, dtype=torch.int32, device=device)
+        self.items = torch.zeros(1 + 3 * (max_rows // 64 + min(slots + 1, max_rows)), dtype=torch.int32, device=device)
+        self.h = torch.zeros(2, max_rows * self.max_ranks, dtype=torch.bfloat16, device=device)
+        self._at = (self.order.data_ptr(), self.items.data_ptr(), self.h[0].data_ptr(), self.h[1].data_ptr())
+
+
+def adapter_rows(ids: torch.Tensor, out: AdapterRows) -> AdapterRows:
+    """Sort the rows of a step by adapter: ``ids`` int32 ``[rows]``, the slot of every row's adapter (below 0, or a slot that
+    there is not: none)."""
+    rows = ids.numel()
+    _require(rows <= out.max_rows, f"{rows} rows, room for {out.max_rows}")
+    at = _vector(ids, torch.int32, rows, "ids")
+    _call(_device_of(ids, out.order), "cb_adapter_rows", at, rows, out.slots, out._at[0], out._at[1])
+    out.rows = rows
+    return out
+
+
+def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, rows: AdapterRows, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[t] = y[t] + scale (x[t] A^T) B^T`` with the adapter of row ``t`` (``csrc/adapters.cu``); rows without one are ``y``.
+
+    ``x`` bf16 ``[rows, k]``, ``y`` bf16 ``[rows, n]``, rows of neighbouring elements at a stride of a multiple of 8;
+    ``out`` None: into ``y``.  Sums are fp32, the result is rounded once."""
+    out = y if out is None else out
+    t, bf = x.shape[0], torch.bfloat16
+    _require(x.dim() == y.dim() == out.dim() == 2 and x.dtype == y.dtype == out.dtype == bf, "x, y and out are bf16 matrices")
+    _require(t == rows.rows and rows.slots == bank.slots, "the rows were sorted for another step or another number of adapters")
+    _require(x.shape[1] == bank.k and y.shape == out.shape == (t, bank.n), f"x [{t}, {bank.k}], y and out [{t}, {bank.n}]")
+    _require(bank.sections * bank.rank <= rows.max_ranks, "more ranks than the sorted rows have room for")
+    s = native.AdapterStruct.from_buffer_copy(bank._struct)
+    s.x, s.y, s.out, s.ldx, s.ldy, s.ldo = x.data_ptr(), y.data_ptr(), out.data_ptr(), x.stride(0), y.stride(0), out.stride(0)
+    if t > 1:
+        _require(x.stride(1) == y.stride(1) == out.stride(1) == 1 and s.ldx >= bank.k and min(s.ldy, s.ldo) >= bank.n and (s.ldx | s.ldy | s.ldo) % 8 == 0, "rows of neighbouring elements at a stride of a multiple of 8")
+    else:
+        s.ldx, s.ldy, s.ldo = bank.k, bank.n, bank.n
+    _require((s.x | s.y | s.out) % 16 == 0, "x, y and out start on a 16-byte boundary")
+    s.rows, (s.order, s.items, s.hi, s.lo) = t, rows._at
+    _call(_device_of(x, y, out, bank.a, rows.order), "cb_adapter_add", ctypes.byref(s))
+    return out
+
+
+def sample_vocabulary(logits: torch.Tensor, out_ids: torch.Tensor, temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
+                      top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None, uniforms: torch.Tensor | None = None,
+                      seeds: torch.Tensor | None = None, counters: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                      out_logprob: torch.Tensor | None = None, out_kept: torch.Tensor | None = None, vocab: int | None = None,
+                      rows: torch.Tensor | None = None) -> torch.Tensor:
+    """Draw every row's token from the whole vocabulary (``csrc/sample_vocabulary.cu``); ``sample`` draws from the 20 best.
+
+    Tokens in order of (value, lowest id first) have weights ``exp((x - max) / temperature)``.  A row keeps the first ``top_k``
+    of them (0: all), of those the shortest prefix with at least ``top_p`` of their mass (1: all), of those the tokens with
+    at least ``min_p`` of the largest weight (less than 2^-60: all); the draw is the first whose running mass is above
+    ``u`` times the mass kept.  ``u``: ``uniforms`` fp32 in [0, 1), or the stream of ``seeds`` and ``counters`` that ``sample``
+    uses.  ``temperature`` 0: the largest value.  NaN, -inf and what ``mask`` (bit i: token i is allowed) leaves out are never
+    drawn; a row that nothing is left of gets id 0 and log-probability -inf.  ``out_logprob``: of the token among those kept;
+    ``out_kept``: how many those are.  ``rows`` int32: draw for these rows only (below 0: none), each at its own place of every
+    other tensor."""
+    _require(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32), "logits are a bf16 or fp32 matrix")
+    n, f32 = logits.shape[0], torch.float32
+    vocab = logits.shape[1] if vocab is None else vocab
+    _require(1 <= vocab <= min(logits.shape[1], 1 << 20) and (logits.stride(1) == 1 or vocab == 1), "rows of one to 2^20 neighbouring logits")
+    ld = logits.stride(0) if n > 1 else max(logits.stride(0), vocab)
+    _require(ld >= vocab, "rows of logits do not overlap")
+    ld_mask = 0
+    if mask is not None:
+        _require(mask.dtype == torch.int32 and mask.dim() == 2 and mask.shape[0] >= n and mask.shape[1] * 32 >= vocab and mask.stride(1) == 1, "mask: int32 words of 32 tokens for every row")
+        ld_mask = max(mask.stride(0), mask.shape[1])
+    s = native.VocabularyStruct(
+        logits.data_ptr(), ld, _ptr(mask), ld_mask, _vector(temperature, f32, n, "temperature"),
+        _vector(top_k, torch.int32, n, "top_k"), _vector(top_p, f32, n, "top_p"), _vector(min_p, f32, n, "min_p"), _vector(uniforms, f32, n, "uniforms"),
+        _vector(seeds, torch.int64, n, "seeds"), _vector(counters, torch.int64, n, "counters"), _vector(rows, torch.int32, 0, "rows"),
+        _vector(out_ids, torch.int32, n, "out_ids"), _vector(out_logprob, f32, n, "out_logprob"), _vector(out_kept, torch.int32, n, "out_kept"),
+        n if rows is None else rows.numel(), vocab, int(logits.dtype == f32))
+    dev = _device_of(logits, out_ids, temperature, top_k, top_p, min_p, uniforms, seeds, counters, mask, out_logprob, out_kept, rows)
+    _call(dev, "cb_sample_vocabulary", ctypes.byref(s))
+    return out_ids
+
+
 # ------------------------------------------------------------------ mixture of experts
 class MoeScratch:
     """Fixed-address routing buffers for up to ``max_tokens`` tokens (graph-capturable)."""

@@ -329,6 +329,13 @@ def _declare(l: ctypes.CDLL) -> None:
     l.cb_canary_fill.restype = i
     l.cb_canary_check.argtypes = [vp, ll, ctypes.c_uint, i, vp, vp]
     l.cb_canary_check.restype = i
+    # what a step does for each of its requests: layout, adapters, draws from a whole vocabulary
+    l.cb_adapter_items.argtypes = [i, i]
+    l.cb_adapter_rows.argtypes = [vp, i, i, vp, vp, vp]
+    for name in ("step_layout", "adapter_add", "sample_vocabulary"):
+        getattr(l, f"cb_{name}").argtypes = [vp, vp]
+    for name in ("step_layout", "adapter_items", "adapter_rows", "adapter_add", "sample_vocabulary"):
+        getattr(l, f"cb_{name}").restype = i
     # layered decoders: fp32 residual stream, delta rule of any head size, latent attention
     l.cb_bf16_gemm_wide.argtypes = [vp, vp, ll, vp, vp, vp]
     l.cb_f32_gemm.argtypes = [vp, vp]
@@ -554,6 +561,36 @@ class ScoredMoeStruct(ctypes.Structure):
                 ("top", ctypes.c_int), ("mb", ctypes.c_int), ("ids", ctypes.c_void_p), ("pos", ctypes.c_void_p),
                 ("weight", ctypes.c_void_p), ("self_w", ctypes.c_void_p), ("counts", ctypes.c_void_p),
                 ("tiles", ctypes.c_void_p)]
+
+
+class StepLayoutStruct(ctypes.Structure):
+    """Mirror of ``CbStepLayout`` in ``csrc/step_layout.cu``."""
+    _fields_ = [("request", ctypes.c_void_p), ("start", ctypes.c_void_p), ("count", ctypes.c_void_p), ("held", ctypes.c_void_p),
+                ("pages", ctypes.c_void_p), ("table", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+                ("rb_req", ctypes.c_void_p), ("rb_qstart", ctypes.c_void_p), ("rb_qcount", ctypes.c_void_p),
+                ("rb_ctx", ctypes.c_void_p), ("row0", ctypes.c_void_p), ("logit_rows", ctypes.c_void_p),
+                ("totals", ctypes.c_void_p), ("n", ctypes.c_int), ("num_pages", ctypes.c_int), ("table_rows", ctypes.c_int),
+                ("width", ctypes.c_int), ("ld", ctypes.c_int), ("block", ctypes.c_int), ("cap_tokens", ctypes.c_int),
+                ("cap_blocks", ctypes.c_int), ("pad", ctypes.c_int)]
+
+
+class AdapterStruct(ctypes.Structure):
+    """Mirror of ``CbAdapter`` in ``csrc/adapters.cu``."""
+    _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_longlong), ("y", ctypes.c_void_p), ("ldy", ctypes.c_longlong),
+                ("out", ctypes.c_void_p), ("ldo", ctypes.c_longlong), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
+                ("scale", ctypes.c_void_p), ("ranks", ctypes.c_void_p), ("order", ctypes.c_void_p), ("items", ctypes.c_void_p),
+                ("hi", ctypes.c_void_p), ("lo", ctypes.c_void_p), ("rows", ctypes.c_int), ("slots", ctypes.c_int),
+                ("k", ctypes.c_int), ("n", ctypes.c_int), ("rank", ctypes.c_int), ("sections", ctypes.c_int),
+                ("width", ctypes.c_int * 4)]
+
+
+class VocabularyStruct(ctypes.Structure):
+    """Mirror of ``CbVocabulary`` in ``csrc/sample_vocabulary.cu``."""
+    _fields_ = [("logits", ctypes.c_void_p), ("ld", ctypes.c_longlong), ("mask", ctypes.c_void_p), ("ld_mask", ctypes.c_longlong),
+                ("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p),
+                ("uniforms", ctypes.c_void_p), ("seeds", ctypes.c_void_p), ("counters", ctypes.c_void_p),
+                ("rows_of", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("logprob", ctypes.c_void_p), ("kept", ctypes.c_void_p),
+                ("rows", ctypes.c_int), ("vocab", ctypes.c_int), ("f32", ctypes.c_int)]
 
 
 class ReduceNormStruct(ctypes.Structure):
