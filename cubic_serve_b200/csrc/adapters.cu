@@ -92,7 +92,7 @@ adapter_rows_kernel(const int* __restrict__ ids, int rows, int slots, int* __res
 
 }  // namespace cb
 
-// Mirrored by ops/native.py::AdapterStruct.
+// Packed by ops/native.py::ADAPTER.
 struct CbAdapter {
   const void* x; long long ldx;          // bf16 [rows, k]
   const void* y; long long ldy;          // bf16 [rows, n]

@@ -21,7 +21,7 @@ static constexpr int kLayoutMost = 1 << 29;
 
 }  // namespace cb
 
-// Mirrored by ops/native.py::StepLayoutStruct.
+// Packed by ops/native.py::STEP_LAYOUT.
 struct CbStepLayout {
   const int* request;        // [n] row of the block table
   const int* start;          // [n] tokens before the step

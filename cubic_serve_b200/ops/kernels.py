@@ -723,30 +723,28 @@ def _require(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _device_of(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    """The one GPU of an operator's tensors."""
-    dev = first.device
-    _require(dev.type == "cuda", "tensors must be on a GPU")
-    for t in others:
-        _require(t is None or t.device == dev, "tensors must be on one GPU")
-    return dev
-
-
-def _call(dev: torch.device, entry: str, *args) -> None:
+def _call(entry: str, args: tuple, tensors: tuple) -> None:
     """Launch on the current stream of the tensors' own GPU, whichever is the current one."""
-    if dev.index == torch.cuda.current_device():
-        code = getattr(native.lib(), entry)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    dev = tensors[0].get_device()
+    _require(dev >= 0, "tensors must be on a GPU")
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError("tensors must be on one GPU")
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch._C._cuda_getDevice():
+        code = getattr(native.lib(), entry)(*args, stream)
     else:
         with torch.cuda.device(dev):
-            code = getattr(native.lib(), entry)(*args, torch.cuda.current_stream(dev).cuda_stream)
+            code = getattr(native.lib(), entry)(*args, stream)
     native.check(code, entry)
 
 
-def _vector(t: torch.Tensor | None, dtype: torch.dtype, n: int, name: str) -> int | None:
+def _vector(t: torch.Tensor | None, dtype: torch.dtype, n: int, name: str) -> int:
     """Address of an optional contiguous vector of at least ``n`` elements."""
     if t is None:
-        return None
-    _require(t.dtype == dtype and t.dim() == 1 and t.numel() >= n and (t.numel() <= 1 or t.stride(0) == 1), f"{name}: a contiguous {dtype} vector of {n} elements")
+        return 0
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous {dtype} vector of {n} elements")
     return t.data_ptr()
 
 
@@ -766,13 +764,13 @@ class StepLayout:
         self.max_tokens, self.max_requests, self.max_blocks = max_tokens, max_requests, max_blocks
         into = into or {}
         _require(set(into) <= set(sizes), f"unknown buffers {sorted(set(into) - set(sizes))}")
-        s = self._struct = native.StepLayoutStruct()
+        at = []
         for name, n in sizes.items():
             dt = torch.int64 if name == "logit_rows" else torch.int32
             t = into[name] if name in into else torch.zeros(n, dtype=dt, device=device)
-            setattr(s, name, _vector(t, dt, n, name))
+            at.append(_vector(t, dt, n, name))
             setattr(self, name, t)
-        self.device = self.totals.device
+        self._at = tuple(at)
 
     def check(self) -> None:
         """Raise if the last layout met a request that it could not place (reads ``totals``: waits for the GPU)."""
@@ -791,18 +789,16 @@ def step_layout(request: torch.Tensor, start: torch.Tensor, count: torch.Tensor,
     row block.  ``tokens`` / ``blocks``: rows and row blocks to write at most; rows and row blocks behind the last one up to
     ``pad`` become padding (slot -1, nothing to attend to), what is behind them stays.  A request that cannot be placed gets
     no slots and attends to nothing; ``out.totals[3]`` says why."""
-    n = start.numel()
-    _require(n <= out.max_requests and 0 <= tokens <= out.max_tokens and 0 <= blocks <= out.max_blocks and pad <= min(out.max_tokens, out.max_blocks),
+    n, i32 = start.numel(), torch.int32
+    _require(n <= out.max_requests and 0 <= tokens <= out.max_tokens and 0 <= blocks <= out.max_blocks and pad <= out.max_tokens and pad <= out.max_blocks,
              "more rows, row blocks or requests than the layout holds")
     _require(1 <= block <= 1 << 20, "a row block holds at least one position")
-    _require(table.dtype == torch.int32 and table.dim() == 2 and table.stride(1) == 1 and table.stride(0) >= table.shape[1], "the block table is int32 with rows of neighbouring entries")
-    s = native.StepLayoutStruct.from_buffer_copy(out._struct)
-    i32 = torch.int32
-    s.request, s.start, s.count = _vector(request, i32, n, "request"), _vector(start, i32, n, "start"), _vector(count, i32, n, "count")
-    s.held, s.pages = _vector(held, i32, n, "held"), _vector(pages, i32, 0, "pages")
-    s.table, s.table_rows, s.width, s.ld = table.data_ptr(), table.shape[0], table.shape[1], table.stride(0)
-    s.n, s.num_pages, s.block, s.cap_tokens, s.cap_blocks, s.pad = n, pages.numel(), block, max(tokens, pad), max(blocks, pad), max(0, pad)
-    _call(_device_of(start, request, count, held, pages, table, out.totals), "cb_step_layout", ctypes.byref(s))
+    rows, width = table.shape if table.dim() == 2 else (0, 0)
+    _require(table.dtype is i32 and table.dim() == 2 and table.stride(1) == 1 and table.stride(0) >= width, "the block table is int32 with rows of neighbouring entries")
+    packed = native.STEP_LAYOUT.pack(
+        _vector(request, i32, n, "request"), _vector(start, i32, n, "start"), _vector(count, i32, n, "count"), _vector(held, i32, n, "held"), _vector(pages, i32, 0, "pages"),
+        table.data_ptr(), *out._at, n, pages.numel(), rows, width, table.stride(0), block, max(tokens, pad), max(blocks, pad), max(0, pad))
+    _call("cb_step_layout", (packed,), (start, request, count, held, pages, table, out.totals))
     return out
 
 
@@ -838,11 +834,8 @@ class AdapterBank:
         _require(a.data_ptr() % 16 == 0 and b.data_ptr() % 16 == 0, "adapters start on a 16-byte boundary")
         self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
         self.slots, self.k, self.n, self.rank, self.sections = slots, a.shape[2], n, full, S
-        s = self._struct = native.AdapterStruct()
-        s.a, s.b, s.scale, s.ranks = a.data_ptr(), b.data_ptr(), scale.data_ptr(), _ptr(ranks)
-        s.slots, s.k, s.n, s.rank, s.sections = slots, self.k, n, full, S
-        for i, w in enumerate(self.widths):
-            s.width[i] = w
+        self._at = (a.data_ptr(), b.data_ptr(), scale.data_ptr(), 0 if ranks is None else ranks.data_ptr())
+        self._shape = (slots, self.k, n, full, S, *self.widths, *(0,) * (4 - S))
 
     def load(self, slot: int, a, b, scale: float) -> None:
         """Write one adapter: ``a`` / ``b`` a matrix ``[rank, k]`` / ``[width, rank]`` for every section (None: the section has
@@ -885,9 +878,8 @@ def adapter_rows(ids: torch.Tensor, out: AdapterRows) -> AdapterRows:
     """Sort the rows of a step by adapter: ``ids`` int32 ``[rows]``, the slot of every row's adapter (below 0, or a slot that
     there is not: none)."""
     rows = ids.numel()
-    _require(rows <= out.max_rows, f"{rows} rows, room for {out.max_rows}")
-    at = _vector(ids, torch.int32, rows, "ids")
-    _call(_device_of(ids, out.order), "cb_adapter_rows", at, rows, out.slots, out._at[0], out._at[1])
+    _require(rows <= out.max_rows, "more rows than there is room for")
+    _call("cb_adapter_rows", (_vector(ids, torch.int32, rows, "ids"), rows, out.slots, out._at[0], out._at[1]), (ids, out.order))
     out.rows = rows
     return out
 
@@ -898,20 +890,17 @@ def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, rows: Adapt
     ``x`` bf16 ``[rows, k]``, ``y`` bf16 ``[rows, n]``, rows of neighbouring elements at a stride of a multiple of 8;
     ``out`` None: into ``y``.  Sums are fp32, the result is rounded once."""
     out = y if out is None else out
-    t, bf = x.shape[0], torch.bfloat16
-    _require(x.dim() == y.dim() == out.dim() == 2 and x.dtype == y.dtype == out.dtype == bf, "x, y and out are bf16 matrices")
-    _require(t == rows.rows and rows.slots == bank.slots, "the rows were sorted for another step or another number of adapters")
-    _require(x.shape[1] == bank.k and y.shape == out.shape == (t, bank.n), f"x [{t}, {bank.k}], y and out [{t}, {bank.n}]")
+    t, bf = rows.rows, torch.bfloat16
+    _require(x.dtype is bf and y.dtype is bf and out.dtype is bf, "x, y and out are bf16 matrices")
+    _require(rows.slots == bank.slots, "the rows were sorted for another number of adapters")
+    _require(x.shape == (t, bank.k) and y.shape == (t, bank.n) and out.shape == (t, bank.n), "x is [sorted rows, k], y and out are [sorted rows, n]")
     _require(bank.sections * bank.rank <= rows.max_ranks, "more ranks than the sorted rows have room for")
-    s = native.AdapterStruct.from_buffer_copy(bank._struct)
-    s.x, s.y, s.out, s.ldx, s.ldy, s.ldo = x.data_ptr(), y.data_ptr(), out.data_ptr(), x.stride(0), y.stride(0), out.stride(0)
-    if t > 1:
-        _require(x.stride(1) == y.stride(1) == out.stride(1) == 1 and s.ldx >= bank.k and min(s.ldy, s.ldo) >= bank.n and (s.ldx | s.ldy | s.ldo) % 8 == 0, "rows of neighbouring elements at a stride of a multiple of 8")
-    else:
-        s.ldx, s.ldy, s.ldo = bank.k, bank.n, bank.n
-    _require((s.x | s.y | s.out) % 16 == 0, "x, y and out start on a 16-byte boundary")
-    s.rows, (s.order, s.items, s.hi, s.lo) = t, rows._at
-    _call(_device_of(x, y, out, bank.a, rows.order), "cb_adapter_add", ctypes.byref(s))
+    ldx, ldy, ldo = (x.stride(0), y.stride(0), out.stride(0)) if t > 1 else (bank.k, bank.n, bank.n)
+    px, py, po = x.data_ptr(), y.data_ptr(), out.data_ptr()
+    _require(x.stride(1) == 1 and y.stride(1) == 1 and out.stride(1) == 1 and ldx >= bank.k and ldy >= bank.n and ldo >= bank.n and (ldx | ldy | ldo) % 8 == 0 and (px | py | po) % 16 == 0,
+             "rows of neighbouring elements at a stride of a multiple of 8, from a 16-byte boundary")
+    packed = native.ADAPTER.pack(px, ldx, py, ldy, po, ldo, *bank._at, *rows._at, t, *bank._shape)
+    _call("cb_adapter_add", (packed,), (x, y, out, bank.a, rows.order))
     return out
 
 
@@ -940,14 +929,14 @@ def sample_vocabulary(logits: torch.Tensor, out_ids: torch.Tensor, temperature: 
     if mask is not None:
         _require(mask.dtype == torch.int32 and mask.dim() == 2 and mask.shape[0] >= n and mask.shape[1] * 32 >= vocab and mask.stride(1) == 1, "mask: int32 words of 32 tokens for every row")
         ld_mask = max(mask.stride(0), mask.shape[1])
-    s = native.VocabularyStruct(
-        logits.data_ptr(), ld, _ptr(mask), ld_mask, _vector(temperature, f32, n, "temperature"),
-        _vector(top_k, torch.int32, n, "top_k"), _vector(top_p, f32, n, "top_p"), _vector(min_p, f32, n, "min_p"), _vector(uniforms, f32, n, "uniforms"),
-        _vector(seeds, torch.int64, n, "seeds"), _vector(counters, torch.int64, n, "counters"), _vector(rows, torch.int32, 0, "rows"),
-        _vector(out_ids, torch.int32, n, "out_ids"), _vector(out_logprob, f32, n, "out_logprob"), _vector(out_kept, torch.int32, n, "out_kept"),
-        n if rows is None else rows.numel(), vocab, int(logits.dtype == f32))
-    dev = _device_of(logits, out_ids, temperature, top_k, top_p, min_p, uniforms, seeds, counters, mask, out_logprob, out_kept, rows)
-    _call(dev, "cb_sample_vocabulary", ctypes.byref(s))
+    i32, i64 = torch.int32, torch.int64
+    packed = native.VOCABULARY.pack(
+        logits.data_ptr(), ld, 0 if mask is None else mask.data_ptr(), ld_mask, _vector(temperature, f32, n, "temperature"),
+        _vector(top_k, i32, n, "top_k"), _vector(top_p, f32, n, "top_p"), _vector(min_p, f32, n, "min_p"), _vector(uniforms, f32, n, "uniforms"),
+        _vector(seeds, i64, n, "seeds"), _vector(counters, i64, n, "counters"), _vector(rows, i32, 0, "rows"),
+        _vector(out_ids, i32, n, "out_ids"), _vector(out_logprob, f32, n, "out_logprob"), _vector(out_kept, i32, n, "out_kept"),
+        n if rows is None else rows.numel(), vocab, logits.dtype is f32)
+    _call("cb_sample_vocabulary", (packed,), (logits, out_ids, temperature, top_k, top_p, min_p, uniforms, seeds, counters, mask, out_logprob, out_kept, rows))
     return out_ids
 
 

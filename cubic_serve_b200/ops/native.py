@@ -14,6 +14,7 @@ import ctypes
 import hashlib
 import json
 import os
+import struct
 import subprocess
 import threading
 from pathlib import Path
@@ -563,34 +564,10 @@ class ScoredMoeStruct(ctypes.Structure):
                 ("tiles", ctypes.c_void_p)]
 
 
-class StepLayoutStruct(ctypes.Structure):
-    """Mirror of ``CbStepLayout`` in ``csrc/step_layout.cu``."""
-    _fields_ = [("request", ctypes.c_void_p), ("start", ctypes.c_void_p), ("count", ctypes.c_void_p), ("held", ctypes.c_void_p),
-                ("pages", ctypes.c_void_p), ("table", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("slots", ctypes.c_void_p),
-                ("rb_req", ctypes.c_void_p), ("rb_qstart", ctypes.c_void_p), ("rb_qcount", ctypes.c_void_p),
-                ("rb_ctx", ctypes.c_void_p), ("row0", ctypes.c_void_p), ("logit_rows", ctypes.c_void_p),
-                ("totals", ctypes.c_void_p), ("n", ctypes.c_int), ("num_pages", ctypes.c_int), ("table_rows", ctypes.c_int),
-                ("width", ctypes.c_int), ("ld", ctypes.c_int), ("block", ctypes.c_int), ("cap_tokens", ctypes.c_int),
-                ("cap_blocks", ctypes.c_int), ("pad", ctypes.c_int)]
-
-
-class AdapterStruct(ctypes.Structure):
-    """Mirror of ``CbAdapter`` in ``csrc/adapters.cu``."""
-    _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_longlong), ("y", ctypes.c_void_p), ("ldy", ctypes.c_longlong),
-                ("out", ctypes.c_void_p), ("ldo", ctypes.c_longlong), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
-                ("scale", ctypes.c_void_p), ("ranks", ctypes.c_void_p), ("order", ctypes.c_void_p), ("items", ctypes.c_void_p),
-                ("hi", ctypes.c_void_p), ("lo", ctypes.c_void_p), ("rows", ctypes.c_int), ("slots", ctypes.c_int),
-                ("k", ctypes.c_int), ("n", ctypes.c_int), ("rank", ctypes.c_int), ("sections", ctypes.c_int),
-                ("width", ctypes.c_int * 4)]
-
-
-class VocabularyStruct(ctypes.Structure):
-    """Mirror of ``CbVocabulary`` in ``csrc/sample_vocabulary.cu``."""
-    _fields_ = [("logits", ctypes.c_void_p), ("ld", ctypes.c_longlong), ("mask", ctypes.c_void_p), ("ld_mask", ctypes.c_longlong),
-                ("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p),
-                ("uniforms", ctypes.c_void_p), ("seeds", ctypes.c_void_p), ("counters", ctypes.c_void_p),
-                ("rows_of", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("logprob", ctypes.c_void_p), ("kept", ctypes.c_void_p),
-                ("rows", ctypes.c_int), ("vocab", ctypes.c_int), ("f32", ctypes.c_int)]
+# Arguments of the operators around a step's shared layers, packed in one call: an operator of 2 us has no time for a field at a time.
+STEP_LAYOUT = struct.Struct("@15P9i4x")                      # CbStepLayout, csrc/step_layout.cu
+ADAPTER = struct.Struct("@PqPqPq8P10i")                      # CbAdapter, csrc/adapters.cu
+VOCABULARY = struct.Struct("@PqPq11P3i4x")                     # CbVocabulary, csrc/sample_vocabulary.cu
 
 
 class ReduceNormStruct(ctypes.Structure):
