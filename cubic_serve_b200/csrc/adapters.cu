@@ -21,6 +21,7 @@ static constexpr int kAdapterMaxRows = 65535;
 static constexpr int kAdapterSections = 4;
 static constexpr int kSortThreads = 1024;
 static constexpr int kAdapterThreads = 256;
+static constexpr int kAdapterFewRows = 256;                           // up to here A is streamed through registers
 
 // ------------------------------------------------------------------ rows by adapter
 // order[]: the step's rows by adapter, a row's place among its adapter's by its index; rows without one last.
@@ -33,7 +34,8 @@ adapter_rows_kernel(const int* __restrict__ ids, int rows, int slots, int* __res
   __shared__ int warp_rows[32], warp_items[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, buckets = slots + 1;
   const int share = (((rows + 31) >> 5) + 31) & ~31, lo = min(rows, warp * share), hi = min(rows, lo + share);
-  for (int i = tid; i < 32 * buckets; i += kSortThreads) cnt[i] = 0;
+  const int warps = rows ? (rows + share - 1) / share : 0;               // that have any rows
+  for (int i = tid; i < warps * buckets; i += kSortThreads) cnt[i] = 0;
   pdl_wait();
   pdl_launch_dependents();
   __syncthreads();
@@ -50,7 +52,7 @@ adapter_rows_kernel(const int* __restrict__ ids, int rows, int slots, int* __res
   // counts of the warps before, rows and items of the buckets before
   int n = 0;
   if (tid < buckets)
-    for (int w = 0; w < 32; ++w) {
+    for (int w = 0; w < warps; ++w) {
       const int c = cnt[w * buckets + tid];
       cnt[w * buckets + tid] = static_cast<unsigned short>(n);
       n += c;
@@ -67,7 +69,7 @@ adapter_rows_kernel(const int* __restrict__ ids, int rows, int slots, int* __res
   for (int w = 0; w < warp; ++w) { at += warp_rows[w]; it += warp_items[w]; }
   at -= n;
   if (tid < buckets) {
-    for (int w = 0; w < 32; ++w) cnt[w * buckets + tid] = static_cast<unsigned short>(cnt[w * buckets + tid] + at);
+    for (int w = 0; w < warps; ++w) cnt[w * buckets + tid] = static_cast<unsigned short>(cnt[w * buckets + tid] + at);
     for (int i = 0; i < nt; ++i) {
       int* e = items + 1 + 3 * (it - nt + i);
       e[0] = tid < slots ? tid : -1;
@@ -124,82 +126,104 @@ __device__ __forceinline__ void split_h(float v, __nv_bfloat16& hi, __nv_bfloat1
   lo = __float2bfloat16(v - __uint_as_float(u & 0xffff0000u));
 }
 
-// h of one item, one section and sixteen rows at a time: the eight warps take turns of 64 along k, the CTAs of a cluster a share of it each; sums are
-// joined in their order.  The order of k inside a product is free: a lane's 16 bytes of x and of A are its operands of two products as they lie.
-template <int R16>
+// What is left to do with a sum: scale it, and write its two parts.
+__device__ __forceinline__ void put_h(const CbAdapter& p, float v, float scale, bool in_use, size_t at) {
+  __nv_bfloat16 hi, lo;
+  split_h(in_use ? v * scale : 0.f, hi, lo);                          // ranks that are not in use may meet what is not finite in x
+  static_cast<__nv_bfloat16*>(p.hi)[at] = hi;
+  static_cast<__nv_bfloat16*>(p.lo)[at] = lo;
+}
+
+// h of few rows: one item, one section, sixteen rows at a time.  A is the operand of sixteen, rows of x those of eight, for most adapters of a decode step have
+// no more.  The eight warps and the CTAs of a cluster take turns of 32 along k; sums are joined in their order.  The order of k inside a product is free: a
+// lane's 16 bytes of x and of A are its operands of two products as they lie.  J turns of a warp are on their way at once.
+template <int R16, int J>
 __global__ void __launch_bounds__(kAdapterThreads)
 adapter_down_kernel(const CbAdapter p, int splits) {
-  constexpr int R = R16 * 16, NT = R16 * 2;
-  extern __shared__ float sh[];                                       // [8][16][R], then the cluster's part [16][R]
-  float* part = sh + 8 * 16 * R;
+  constexpr int R = R16 * 16, RP = R + 4;
+  extern __shared__ float sh[];                                       // [8][16][RP], then the cluster's part [16][R]
+  float* part = sh + 8 * 16 * RP;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const int rank_in = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0, team = blockIdx.x / splits, teams = gridDim.x / splits;
   pdl_launch_dependents();
   pdl_wait();
-  const int count = p.items[0], units = count * p.sections;
-  const int chunk = (((p.k + 63) / 64 + splits - 1) / splits) * 64, k0 = rank_in * chunk, k1 = min(p.k, k0 + chunk);
-  const int rt = p.sections * R;
+  const int units = p.items[0] * p.sections, rt = p.sections * R, turns = (p.k + 31) >> 5;
   for (int u = team; u < units; u += teams) {
     const int item = u / p.sections, sec = u - item * p.sections;
     const int slot = p.items[1 + 3 * item], first = p.items[2 + 3 * item], rows = p.items[3 + 3 * item];
     if (slot < 0) continue;
     const float scale = p.scale[slot];
     const int used = p.ranks ? min(R, max(0, p.ranks[slot])) : R;
-    const __nv_bfloat16* A = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * rt + sec * R) * p.k;
+    const __nv_bfloat16* A = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * rt + sec * R + g) * p.k + c * 8;
     for (int m0 = 0; m0 < rows; m0 += 16) {
-      const bool in0 = m0 + g < rows, in1 = m0 + g + 8 < rows;
-      const __nv_bfloat16* x0 = static_cast<const __nv_bfloat16*>(p.x) + (in0 ? p.order[first + m0 + g] * p.ldx : 0);
-      const __nv_bfloat16* x1 = static_cast<const __nv_bfloat16*>(p.x) + (in1 ? p.order[first + m0 + g + 8] * p.ldx : 0);
-      float acc[NT][4];
+      const int left = min(16, rows - m0);
+      const bool in0 = g < left, in1 = g + 8 < left, both = left > 8;
+      const __nv_bfloat16* x0 = static_cast<const __nv_bfloat16*>(p.x) + (in0 ? p.order[first + m0 + g] * p.ldx : 0) + c * 8;
+      const __nv_bfloat16* x1 = static_cast<const __nv_bfloat16*>(p.x) + (in1 ? p.order[first + m0 + g + 8] * p.ldx : 0) + c * 8;
+      float acc[R16][2][4];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-      for (int kk = k0 + warp * 64; kk < k1; kk += 8 * 64) {
+      for (int t = 0; t < R16; ++t)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int k = kk + j * 32 + c * 8;
-          const bool in = k < k1;
-          const uint4 zero = make_uint4(0, 0, 0, 0);
-          const uint4 xa = in && in0 ? ldg16(x0 + k) : zero, xb = in && in1 ? ldg16(x1 + k) : zero;
-          const uint32_t f0[4] = {xa.x, xb.x, xa.y, xb.y}, f1[4] = {xa.z, xb.z, xa.w, xb.w};
+        for (int h = 0; h < 2; ++h) acc[t][h][0] = acc[t][h][1] = acc[t][h][2] = acc[t][h][3] = 0.f;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      for (int t0 = rank_in * 8 + warp; t0 < turns; t0 += 8 * J * splits) {
+        uint4 w[J][R16][2], xa[J], xb[J];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if (t * 8 >= used) break;
-            const uint4 w = in ? ldg16(A + static_cast<size_t>(t * 8 + g) * p.k + k) : zero;
-            mma_bf16(acc[t], f0, w.x, w.y);
-            mma_bf16(acc[t], f1, w.z, w.w);
-          }
+        for (int j = 0; j < J; ++j) {
+          const int k = (t0 + j * 8 * splits) * 32;
+          const bool in = k + c * 8 < p.k;
+          xa[j] = in && in0 ? ldg16(x0 + k) : zero;
+          xb[j] = in && in1 ? ldg16(x1 + k) : zero;
+#pragma unroll
+          for (int t = 0; t < R16; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[j][t][h] = in && t * 16 + h * 8 < used ? ldg16(A + static_cast<size_t>(t * 16 + h * 8) * p.k + k) : zero;
         }
-      }
-      float* mine = sh + warp * 16 * R;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        *reinterpret_cast<float2*>(mine + g * R + t * 8 + c * 2) = make_float2(acc[t][0], acc[t][1]);
-        *reinterpret_cast<float2*>(mine + (g + 8) * R + t * 8 + c * 2) = make_float2(acc[t][2], acc[t][3]);
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int t = 0; t < R16; ++t) {
+            const uint32_t f0[4] = {w[j][t][0].x, w[j][t][1].x, w[j][t][0].y, w[j][t][1].y}, f1[4] = {w[j][t][0].z, w[j][t][1].z, w[j][t][0].w, w[j][t][1].w};
+            mma_bf16(acc[t][0], f0, xa[j].x, xa[j].y);
+            mma_bf16(acc[t][0], f1, xa[j].z, xa[j].w);
+            if (both) {
+              mma_bf16(acc[t][1], f0, xb[j].x, xb[j].y);
+              mma_bf16(acc[t][1], f1, xb[j].z, xb[j].w);
+            }
+          }
       }
+      float* mine = sh + warp * 16 * RP;
+#pragma unroll
+      for (int t = 0; t < R16; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h && !both) break;
+          float* at = mine + (h * 8 + c * 2) * RP + t * 16 + g;
+          at[0] = acc[t][h][0];
+          at[RP] = acc[t][h][1];
+          at[8] = acc[t][h][2];
+          at[RP + 8] = acc[t][h][3];
+        }
       __syncthreads();
-      auto put = [&](int e, float v) {
-        const int r = e / R;
-        if (m0 + r >= rows) return;
-        __nv_bfloat16 hi, lo;
-        split_h(e - r * R < used ? v * scale : 0.f, hi, lo);          // ranks that are not in use may meet what is not finite in x
-        const size_t o = static_cast<size_t>(first + m0 + r) * rt + sec * R + (e - r * R);
-        static_cast<__nv_bfloat16*>(p.hi)[o] = hi;
-        static_cast<__nv_bfloat16*>(p.lo)[o] = lo;
-      };
-      for (int e = tid; e < 16 * R; e += kAdapterThreads) {
+      const size_t out = static_cast<size_t>(first + m0) * rt + sec * R;
+      for (int e = tid; e < left * R; e += kAdapterThreads) {
+        const int r = e / R, k = e % R;
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) v += sh[w * 16 * R + e];
-        if (splits == 1) put(e, v);
+        for (int w = 0; w < 8; ++w) v += sh[(w * 16 + r) * RP + k];
+        if (splits == 1) put_h(p, v, scale, k < used, out + static_cast<size_t>(r) * rt + k);
         else part[e] = v;
       }
       if (splits > 1) {
         cluster_sync_all();
         const uint32_t base = smem_u32(part);
-        for (int e = rank_in * kAdapterThreads + tid; e < 16 * R; e += splits * kAdapterThreads) {
-          float v = 0.f;
-          for (int s = 0; s < splits; ++s) v += ld_cluster_f32(cluster_map(base + e * 4, s));
-          put(e, v);
+        for (int e = rank_in * kAdapterThreads + tid; e < left * R; e += splits * kAdapterThreads) {
+          float q[8], v = 0.f;
+#pragma unroll
+          for (int s = 0; s < 8; ++s) q[s] = s < splits ? ld_cluster_f32(cluster_map(base + e * 4, s)) : 0.f;
+#pragma unroll
+          for (int s = 0; s < 8; ++s) v += q[s];
+          put_h(p, v, scale, e % R < used, out + static_cast<size_t>(e / R) * rt + e % R);
         }
         cluster_sync_all();
       } else {
@@ -209,105 +233,299 @@ adapter_down_kernel(const CbAdapter p, int splits) {
   }
 }
 
-// out = y + h B^T of one item and 256 columns, 32 a warp.  The eight columns of a product are chosen so that a lane ends up with eight neighbours
-// of a row: y and out are 16 bytes a lane.  B's operands stay in registers for all rows of the item.
-template <int R16>
+// h of many rows: a CTA makes 64 rows x (16 NT) ranks, whatever sections these belong to, so that x is read once; stages of 64 along k come by asynchronous
+// copies.  Four warps by two: 16 rows and half of the ranks each.  The CTAs of a cluster take turns of a stage.
+template <int NT>
 __global__ void __launch_bounds__(kAdapterThreads)
+adapter_down_tile_kernel(const CbAdapter p, int splits) {
+  constexpr int NR = NT * 16, kStages = 4, kStageBytes = (64 + NR) * 128, SP = NR + 2;
+  extern __shared__ __align__(128) unsigned char st[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp & 3, wn = warp >> 2;
+  const int rank_in = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0, team = blockIdx.x / splits, teams = gridDim.x / splits;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int rt = p.sections * p.rank, parts = (rt + NR - 1) / NR, units = p.items[0] * parts, stages = (p.k + 63) >> 6;
+  const uint32_t base = smem_u32(st);
+  for (int u = team; u < units; u += teams) {
+    const int item = u / parts, r0 = (u - item * parts) * NR;
+    const int slot = p.items[1 + 3 * item], first = p.items[2 + 3 * item], rows = p.items[3 + 3 * item];
+    if (slot < 0) continue;
+    const int used = p.ranks ? min(p.rank, max(0, p.ranks[slot])) : p.rank;
+    const int row = tid >> 3, ch = tid & 7;                           // a thread's 16 bytes of rows row, row + 32, ...
+    const __nv_bfloat16* xr[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) xr[i] = static_cast<const __nv_bfloat16*>(p.x) + (row + 32 * i < rows ? p.order[first + row + 32 * i] * p.ldx : 0) + ch * 8;
+    const __nv_bfloat16* A = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * rt + r0 + row) * p.k + ch * 8;
+    auto fetch = [&](int s, int buf) {
+      const int k = s * 64;
+      const bool in = s < stages && k + ch * 8 < p.k;
+      const uint32_t to = base + buf * kStageBytes + row * 128 + ((ch ^ (row & 7)) << 4);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) cp_async16(to + i * 32 * 128, in && row + 32 * i < rows ? xr[i] + k : p.x, in && row + 32 * i < rows);
+#pragma unroll
+      for (int i = 0; i < (NR + 31) / 32; ++i)
+        if (row + 32 * i < NR) {
+          const bool ok = in && r0 + row + 32 * i < rt && (r0 + row + 32 * i) % p.rank < used;
+          cp_async16(to + (64 + i * 32) * 128, ok ? static_cast<const void*>(A + static_cast<size_t>(32 * i) * p.k + k) : p.a, ok);
+        }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float acc[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) fetch(rank_in + i * splits, i);
+    int buf = 0;
+    for (int s = rank_in; s < stages; s += splits) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncthreads();
+      fetch(s + (kStages - 1) * splits, (buf + kStages - 1) % kStages);
+      const uint32_t xs = base + buf * kStageBytes, as = xs + 64 * 128;
+      if (wm * 16 < rows) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t a[4];
+          const int r = wm * 16 + (lane & 15), kc = k * 2 + (lane >> 4);
+          ldsm4(a, xs + r * 128 + ((kc ^ (r & 7)) << 4));
+#pragma unroll
+          for (int t = 0; t < NT; t += 2) {
+            uint32_t b[4];
+            const int n = (wn * NT + t) * 8 + (lane & 7) + (t + 1 < NT ? (lane >> 4) * 8 : 0), bc = k * 2 + (lane >> 3 & 1);
+            ldsm4(b, as + n * 128 + ((bc ^ (n & 7)) << 4));
+            mma_bf16(acc[t], a, b[0], b[1]);
+            if (t + 1 < NT) mma_bf16(acc[t + 1], a, b[2], b[3]);
+          }
+        }
+      }
+      buf = (buf + 1) % kStages;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    const float scale = p.scale[slot];
+    float* part = reinterpret_cast<float*>(st);                       // [64][SP]
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float* at = part + (wm * 16 + (lane >> 2)) * SP + (wn * NT + t) * 8 + (lane & 3) * 2;
+      *reinterpret_cast<float2*>(at) = make_float2(acc[t][0], acc[t][1]);
+      *reinterpret_cast<float2*>(at + 8 * SP) = make_float2(acc[t][2], acc[t][3]);
+    }
+    if (splits > 1) cluster_sync_all(); else __syncthreads();
+    const int width = min(NR, rt - r0);
+    for (int e = rank_in * kAdapterThreads + tid; e < rows * NR; e += splits * kAdapterThreads) {
+      const int r = e / NR, k = e % NR;
+      if (k >= width) continue;
+      float v = 0.f;
+      if (splits > 1) {
+        float q[8];
+        const uint32_t at = smem_u32(part + r * SP + k);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) q[s] = s < splits ? ld_cluster_f32(cluster_map(at, s)) : 0.f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) v += q[s];
+      } else {
+        v = part[r * SP + k];
+      }
+      put_h(p, v, scale, (r0 + k) % p.rank < used, static_cast<size_t>(first + r) * rt + r0 + k);
+    }
+    if (splits > 1) cluster_sync_all(); else __syncthreads();
+  }
+}
+
+// out = y + h B^T of one item and 16 MT columns a warp.  B is the operand of sixteen, rows of h those of eight.  Which columns a product has is free: they are
+// chosen so that a lane ends up with 2 MT neighbours of two rows, and eight lanes with a row of 16 MT: whole lines of y and out.  B's operands stay in
+// registers for all rows of the item; y of the next sixteen rows is on its way while eight are added to.
+template <int R16, int MT>
+__global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_up_kernel(const CbAdapter p) {
-  constexpr int R = R16 * 16;
+  constexpr int R = R16 * 16, W = 16 * MT, V = MT / 2;                // V 8-byte words a lane and row
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   pdl_launch_dependents();
   pdl_wait();
-  const int blocks = (p.n + 255) / 256, units = p.items[0] * blocks, rt = p.sections * R;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const int item = u / blocks, col0 = (u - item * blocks) * 256 + warp * 32;
-    if (col0 >= p.n) continue;
+  const int blocks = (p.n + W - 1) / W, units = p.items[0] * blocks, rt = p.sections * R;
+  const bool in_place = p.out == p.y;
+  for (int u = blockIdx.x * 8 + warp; u < units; u += gridDim.x * 8) {
+    const int item = u / blocks, col0 = (u - item * blocks) * W, col = col0 + g * 2 * MT;
     const int slot = p.items[1 + 3 * item], first = p.items[2 + 3 * item], rows = p.items[3 + 3 * item];
-    const int col = col0 + c * 8;
     const bool in = col < p.n;
-    if (slot < 0) {
-      if (p.out == p.y) continue;
-      for (int r = g; r < rows; r += 8) {
-        const size_t row = p.order[first + r];
-        if (in) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + col) = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.y) + row * p.ldy + col);
-      }
-      continue;
-    }
+    if (slot < 0 && in_place) continue;
     int sec = 0;
     for (int at = p.width[0]; sec + 1 < p.sections && col0 >= at; at += p.width[sec]) ++sec;
-    const int used = p.ranks ? min(R, max(0, p.ranks[slot])) : R;
-    // product j, column g is column 8 (g / 2) + 2 j + g % 2 of the 32
-    uint32_t b[4][R16][2];
-    const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + static_cast<size_t>(slot) * p.n * R;
+    const int used = slot < 0 ? 0 : p.ranks ? min(R, max(0, p.ranks[slot])) : R;
+    // product t, places g and g + 8: columns 2 t and 2 t + 1 of the lane's
+    uint32_t b[MT][R16][4];
+    const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(max(slot, 0)) * p.n + col) * R;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = col0 + 8 * (g >> 1) + 2 * j + (g & 1);
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int s = 0; s < R16; ++s) {
-        const uint2 w = n < p.n && s * 16 < used ? __ldg(reinterpret_cast<const uint2*>(B + static_cast<size_t>(n) * R + s * 16 + c * 4)) : make_uint2(0, 0);
-        b[j][s][0] = w.x;
-        b[j][s][1] = w.y;
+      for (int h = 0; h < 2; ++h) {
+        const __nv_bfloat16* at = B + (2 * t + h) * R;
+        if (R16 == 1) {
+          const uint2 w = in && used ? __ldg(reinterpret_cast<const uint2*>(at + c * 4)) : make_uint2(0, 0);
+          b[t][0][h] = w.x;
+          b[t][0][2 + h] = w.y;
+        } else {
+#pragma unroll
+          for (int s = 0; s < R16 / 2; ++s) {
+            const uint4 w = in && s * 32 < used ? ldg16(at + s * 32 + c * 8) : make_uint4(0, 0, 0, 0);
+            b[t][2 * s][h] = w.x;
+            b[t][2 * s][2 + h] = w.y;
+            b[t][2 * s + 1][h] = w.z;
+            b[t][2 * s + 1][2 + h] = w.w;
+          }
+        }
       }
-    }
+    // y of the rows 2 c and 2 c + 1 of an eight
+    auto row_of = [&](int r) { return r < rows ? p.order[first + r] : -1; };
+    auto load = [&](int row, uint2 (&v)[V]) {
+      if (row < 0 || !in) return;
+      const __nv_bfloat16* at = static_cast<const __nv_bfloat16*>(p.y) + row * p.ldy + col;
+      if (V == 2) {
+        const uint4 w = *reinterpret_cast<const uint4*>(at);
+        v[0] = make_uint2(w.x, w.y);
+        v[V - 1] = make_uint2(w.z, w.w);
+      } else {
+        v[0] = *reinterpret_cast<const uint2*>(at);
+      }
+    };
+    constexpr bool AHEAD = R16 * MT <= 8;                             // registers for the next rows
+    int next_row[2][2];
+    uint2 next[2][2][V];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) next_row[e][i] = row_of(e * 8 + 2 * c + i);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) load(next_row[e][i], next[e][i]);
     for (int m0 = 0; m0 < rows; m0 += 16) {
-      const int r0 = m0 + g, r1 = r0 + 8;
-      const bool in0 = in && r0 < rows, in1 = in && r1 < rows;
-      const size_t row0 = r0 < rows ? p.order[first + r0] : 0, row1 = r1 < rows ? p.order[first + r1] : 0;
-      uint4 y0 = make_uint4(0, 0, 0, 0), y1 = y0;
-      if (in0) y0 = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.y) + row0 * p.ldy + col);
-      if (in1) y1 = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.y) + row1 * p.ldy + col);
-      float acc[4][4];
+      int row[2][2];
+      uint2 y[2][2][V];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-      const size_t h0 = static_cast<size_t>(first + min(r0, rows - 1)) * rt + sec * R + c * 4, h1 = static_cast<size_t>(first + min(r1, rows - 1)) * rt + sec * R + c * 4;
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int s = 0; s < R16; ++s) {
-        if (s * 16 >= used) break;
+        for (int i = 0; i < 2; ++i) {
+          row[e][i] = next_row[e][i];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(half ? p.lo : p.hi);
-          const uint2 a0 = *reinterpret_cast<const uint2*>(h + h0 + s * 16), a1 = *reinterpret_cast<const uint2*>(h + h1 + s * 16);
-          const uint32_t f[4] = {a0.x, a1.x, a0.y, a1.y};
+          for (int v = 0; v < V; ++v) y[e][i][v] = next[e][i][v];
+        }
+      auto ahead = [&]() {
+        if (m0 + 16 >= rows) return;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mma_bf16(acc[j], f, b[j][s][0], b[j][s][1]);
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) next_row[e][i] = row_of(m0 + 16 + e * 8 + 2 * c + i);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) load(next_row[e][i], next[e][i]);
+      };
+      if (AHEAD) ahead();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (m0 + e * 8 >= rows) break;
+        float acc[MT][4];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+        if (used) {
+          const size_t at = static_cast<size_t>(first + min(m0 + e * 8 + g, rows - 1)) * rt + sec * R;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(half ? p.lo : p.hi) + at;
+            if (R16 == 1) {
+              const uint2 w = *reinterpret_cast<const uint2*>(h + c * 4);
+#pragma unroll
+              for (int t = 0; t < MT; ++t) mma_bf16(acc[t], b[t][0], w.x, w.y);
+            } else {
+#pragma unroll
+              for (int s = 0; s < R16 / 2; ++s) {
+                if (s * 32 >= used) break;
+                const uint4 w = *reinterpret_cast<const uint4*>(h + s * 32 + c * 8);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                  mma_bf16(acc[t], b[t][2 * s], w.x, w.y);
+                  mma_bf16(acc[t], b[t][2 * s + 1], w.z, w.w);
+                }
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (row[e][i] < 0 || !in) continue;
+          uint32_t q[MT];
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            const uint32_t v = t & 1 ? y[e][i][t / 2].y : y[e][i][t / 2].x;
+            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+            q[t] = used ? pack_bf16x2(f.x + acc[t][i], f.y + acc[t][2 + i]) : v;
+          }
+          __nv_bfloat16* at = static_cast<__nv_bfloat16*>(p.out) + row[e][i] * p.ldo + col;
+          if (MT == 4) *reinterpret_cast<uint4*>(at) = make_uint4(q[0], q[1], q[MT - 2], q[MT - 1]);
+          else *reinterpret_cast<uint2*>(at) = make_uint2(q[0], q[1]);
         }
       }
-      auto add = [](uint4 v, const float (&f)[4][4], int o) {
-        uint32_t* q = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 w = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(q + j));
-          q[j] = pack_bf16x2(w.x + f[j][o], w.y + f[j][o + 1]);
-        }
-        return v;
-      };
-      if (in0) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row0 * p.ldo + col) = add(y0, acc, 0);
-      if (in1) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row1 * p.ldo + col) = add(y1, acc, 2);
+      if (!AHEAD) ahead();
     }
   }
 }
 
-template <int R16>
-static int adapter_launch(const CbAdapter& p, int items, cudaStream_t stream) {
-  constexpr int R = R16 * 16;
-  constexpr int smem = 9 * 16 * R * sizeof(float);
-  static bool ready[64] = {};
+template <typename Kernel>
+static cudaError_t adapter_smem(Kernel kernel, int smem, bool (&ready)[64]) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  if (smem > 48 * 1024 && (dev >= 64 || !ready[dev])) {
-    e = cudaFuncSetAttribute(adapter_down_kernel<R16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    if (dev < 64) ready[dev] = true;
-  }
+  if (e != cudaSuccess || smem <= 48 * 1024 || (dev < 64 && ready[dev])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && dev < 64) ready[dev] = true;
+  return e;
+}
+
+template <int R16>
+static cudaError_t adapter_down(const CbAdapter& p, int items, cudaStream_t stream) {
+  constexpr int R = R16 * 16, J = R16 == 1 ? 4 : R16 == 2 ? 3 : R16 == 4 ? 2 : 1;
+  constexpr int smem = (8 * 16 * (R + 4) + 16 * R) * sizeof(float);
+  static bool ready[64] = {};
+  const cudaError_t e = adapter_smem(adapter_down_kernel<R16, J>, smem, ready);
+  if (e != cudaSuccess) return e;
   const int units = items * p.sections;
   int splits = 1;
-  while (splits < 8 && units * splits * 2 <= 592 && p.k / (splits * 2) >= 256) splits *= 2;
-  const int teams = min(units, 592 / splits);
-  e = launch(adapter_down_kernel<R16>, dim3(teams * splits), dim3(kAdapterThreads), smem, stream, dim3(splits, 1, 1), p, splits);
+  while (splits < 8 && units * splits * 2 <= 296 && p.k / (splits * 2) >= 256) splits *= 2;
+  return launch(adapter_down_kernel<R16, J>, dim3(min(units, 592 / splits) * splits), dim3(kAdapterThreads), smem, stream, dim3(splits, 1, 1), p, splits);
+}
+
+template <int NT>
+static cudaError_t adapter_down_tile(const CbAdapter& p, int items, cudaStream_t stream) {
+  constexpr int NR = NT * 16, smem = 4 * (64 + NR) * 128;
+  static_assert(64 * (NR + 2) * 4 <= smem, "the sums fit where the stages were");
+  static bool ready[64] = {};
+  const cudaError_t e = adapter_smem(adapter_down_tile_kernel<NT>, smem, ready);
+  if (e != cudaSuccess) return e;
+  const int units = items * ((p.sections * p.rank + NR - 1) / NR);
+  int splits = 1;
+  while (splits < 8 && units * splits * 2 <= 296 && p.k / (splits * 2) >= 256) splits *= 2;
+  return launch(adapter_down_tile_kernel<NT>, dim3(min(units, 592 / splits) * splits), dim3(kAdapterThreads), smem, stream, dim3(splits, 1, 1), p, splits);
+}
+
+template <int R16, int MT>
+static cudaError_t adapter_up(const CbAdapter& p, int items, cudaStream_t stream) {
+  const int warps = items * ((p.n + 16 * MT - 1) / (16 * MT));
+  return launch(adapter_up_kernel<R16, MT>, dim3(min((warps + 7) / 8, 148 * 8)), dim3(kAdapterThreads), 0, stream, p);
+}
+
+template <int R16>
+static int adapter_launch(const CbAdapter& p, int items, cudaStream_t stream) {
+  cudaError_t e;
+  if (p.rows <= kAdapterFewRows) {
+    e = adapter_down<R16>(p, items, stream);
+  } else {
+    const int n = p.sections * R16;                                   // sixteens of ranks
+    e = n == 1 ? adapter_down_tile<1>(p, items, stream) : n == 2 ? adapter_down_tile<2>(p, items, stream) : n == 3 ? adapter_down_tile<3>(p, items, stream)
+      : n == 4 ? adapter_down_tile<4>(p, items, stream) : n % 8 == 0 ? adapter_down_tile<8>(p, items, stream) : adapter_down_tile<6>(p, items, stream);
+  }
   if (e != cudaSuccess) return static_cast<int>(e);
-  const int blocks = (p.n + 255) / 256;
-  return static_cast<int>(launch(adapter_up_kernel<R16>, dim3(min(items * blocks, 148 * 4)), dim3(kAdapterThreads), 0, stream, p));
+  bool wide = R16 < 8;                                                // a warp's columns belong to one section
+  for (int i = 0; i + 1 < p.sections; ++i) wide = wide && p.width[i] % 64 == 0;
+  return static_cast<int>(wide ? adapter_up<R16, R16 < 8 ? 4 : 2>(p, items, stream) : adapter_up<R16, 2>(p, items, stream));
 }
 
 static int adapter_items(int rows, int slots) { return rows / kAdapterItemRows + min(slots + 1, rows); }
