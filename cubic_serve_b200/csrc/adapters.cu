@@ -233,18 +233,25 @@ adapter_down_kernel(const CbAdapter p, int splits) {
   }
 }
 
-// h of many rows: a CTA makes 64 rows x (16 NT) ranks, whatever sections these belong to, so that x is read once; stages of 64 along k come by asynchronous
-// copies.  Four warps by two: 16 rows and half of the ranks each.  The CTAs of a cluster take turns of a stage.
+// h of many rows: a CTA makes 64 rows x (16 NT) ranks, whatever sections these belong to, so that x is read once; stages of 64 H along k come by asynchronous
+// copies.  Four warps by two: 16 rows and half of the ranks each.  The CTAs of a cluster have a share of k each.
 template <int NT>
-__global__ void __launch_bounds__(kAdapterThreads)
+struct DownTile {
+  static constexpr int NR = NT * 16, H = NT <= 4 ? 2 : 1, kStages = NT <= 4 ? 3 : 4;
+  static constexpr int kHalfBytes = (64 + NR) * 128, kStageBytes = H * kHalfBytes, kBytes = kStages * kStageBytes, SP = NR + 2;
+};
+template <int NT>
+__global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_down_tile_kernel(const CbAdapter p, int splits) {
-  constexpr int NR = NT * 16, kStages = 4, kStageBytes = (64 + NR) * 128, SP = NR + 2;
+  using T = DownTile<NT>;
+  constexpr int NR = T::NR, H = T::H, kStages = T::kStages, SP = T::SP, AR = (NR + 31) / 32;
   extern __shared__ __align__(128) unsigned char st[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp & 3, wn = warp >> 2;
   const int rank_in = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0, team = blockIdx.x / splits, teams = gridDim.x / splits;
   pdl_launch_dependents();
   pdl_wait();
-  const int rt = p.sections * p.rank, parts = (rt + NR - 1) / NR, units = p.items[0] * parts, stages = (p.k + 63) >> 6;
+  const int rt = p.sections * p.rank, parts = (rt + NR - 1) / NR, units = p.items[0] * parts, stages = (p.k + 64 * H - 1) / (64 * H);
+  const int share = (stages + splits - 1) / splits, s0 = rank_in * share, s1 = min(stages, s0 + share);
   const uint32_t base = smem_u32(st);
   for (int u = team; u < units; u += teams) {
     const int item = u / parts, r0 = (u - item * parts) * NR;
@@ -252,38 +259,49 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
     if (slot < 0) continue;
     const int used = p.ranks ? min(p.rank, max(0, p.ranks[slot])) : p.rank;
     const int row = tid >> 3, ch = tid & 7;                           // a thread's 16 bytes of rows row, row + 32, ...
-    const __nv_bfloat16* xr[2];
+    const __nv_bfloat16 *xr[2], *ar[AR];
+    bool xin[2], ain[AR];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) xr[i] = static_cast<const __nv_bfloat16*>(p.x) + (row + 32 * i < rows ? p.order[first + row + 32 * i] * p.ldx : 0) + ch * 8;
-    const __nv_bfloat16* A = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * rt + r0 + row) * p.k + ch * 8;
+    for (int i = 0; i < 2; ++i) {
+      xin[i] = row + 32 * i < rows;
+      xr[i] = static_cast<const __nv_bfloat16*>(p.x) + (xin[i] ? p.order[first + row + 32 * i] * p.ldx : 0) + ch * 8;
+    }
+#pragma unroll
+    for (int i = 0; i < AR; ++i) {
+      const int r = r0 + row + 32 * i;
+      ain[i] = row + 32 * i < NR && r < rt && r % p.rank < used;
+      ar[i] = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * rt + (ain[i] ? r : 0)) * p.k + ch * 8;
+    }
+    const uint32_t to0 = base + row * 128 + ((ch ^ (row & 7)) << 4);
     auto fetch = [&](int s, int buf) {
-      const int k = s * 64;
-      const bool in = s < stages && k + ch * 8 < p.k;
-      const uint32_t to = base + buf * kStageBytes + row * 128 + ((ch ^ (row & 7)) << 4);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) cp_async16(to + i * 32 * 128, in && row + 32 * i < rows ? xr[i] + k : p.x, in && row + 32 * i < rows);
+      for (int h = 0; h < H; ++h) {
+        const int k = (s * H + h) * 64;
+        const bool in = s < s1 && k + ch * 8 < p.k;
+        const uint32_t to = to0 + buf * T::kStageBytes + h * T::kHalfBytes;
 #pragma unroll
-      for (int i = 0; i < (NR + 31) / 32; ++i)
-        if (row + 32 * i < NR) {
-          const bool ok = in && r0 + row + 32 * i < rt && (r0 + row + 32 * i) % p.rank < used;
-          cp_async16(to + (64 + i * 32) * 128, ok ? static_cast<const void*>(A + static_cast<size_t>(32 * i) * p.k + k) : p.a, ok);
-        }
+        for (int i = 0; i < 2; ++i) cp_async16(to + i * 32 * 128, in && xin[i] ? xr[i] + k : p.x, in && xin[i]);
+#pragma unroll
+        for (int i = 0; i < AR; ++i)
+          if (row + 32 * i < NR) cp_async16(to + (64 + i * 32) * 128, in && ain[i] ? static_cast<const void*>(ar[i] + k) : p.a, in && ain[i]);
+      }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     float acc[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch(rank_in + i * splits, i);
+    for (int i = 0; i < kStages - 1; ++i) fetch(s0 + i, i);
     int buf = 0;
-    for (int s = rank_in; s < stages; s += splits) {
+    for (int s = s0; s < s1; ++s) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
       __syncthreads();
-      fetch(s + (kStages - 1) * splits, (buf + kStages - 1) % kStages);
-      const uint32_t xs = base + buf * kStageBytes, as = xs + 64 * 128;
+      fetch(s + kStages - 1, (buf + kStages - 1) % kStages);
       if (wm * 16 < rows) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int kk = 0; kk < 4 * H; ++kk) {
+          const uint32_t xs = base + buf * T::kStageBytes + (kk / 4) * T::kHalfBytes, as = xs + 64 * 128;
+          const int k = kk & 3;
           uint32_t a[4];
           const int r = wm * 16 + (lane & 15), kc = k * 2 + (lane >> 4);
           ldsm4(a, xs + r * 128 + ((kc ^ (r & 7)) << 4));
@@ -333,141 +351,174 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
 
 // out = y + h B^T of one item and 16 MT columns a warp.  B is the operand of sixteen, rows of h those of eight.  Which columns a product has is free: they are
 // chosen so that a lane ends up with 2 MT neighbours of two rows, and eight lanes with a row of 16 MT: whole lines of y and out.  B's operands stay in
-// registers for all rows of the item; y of the next sixteen rows is on its way while eight are added to.
+// registers for all rows of the item.  y comes through a ring of the warp's own, seven eights of rows ahead and on into the next items, and goes back through it:
+// eight lanes copy a line of y, and a line of out.  A lane's own columns straight from global memory were four lines a quarter of a warp: 71 % of the load and
+// store unit's cycles, and 3.7 TB/s.
 template <int R16, int MT>
-__global__ void __launch_bounds__(kAdapterThreads, 2)
+__global__ void __launch_bounds__(kAdapterThreads, R16 * MT <= 4 ? 3 : 2)
 adapter_up_kernel(const CbAdapter p) {
-  constexpr int R = R16 * 16, W = 16 * MT, V = MT / 2;                // V 8-byte words a lane and row
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+  constexpr int R = R16 * 16, W = 16 * MT, kRing = 8, CH = 2 * MT, RP = 32 / CH, I = 8 / RP;      // 16-byte chunks of a row, rows of a copy, copies
+  extern __shared__ __align__(16) unsigned char ring[];                        // [8 warps][kRing][8 rows][CH chunks]
+  __shared__ int ring_row[8][kRing][8];                                        // which rows they are
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3, rr = lane / CH, rc = lane % CH;
+  unsigned char* mine = ring + warp * kRing * 128 * CH;
+  auto place = [](int row, int chunk) { return (row * CH + (chunk ^ (MT == 4 ? row & 7 : row >> 1 & 3))) * 16; };
   pdl_launch_dependents();
   pdl_wait();
-  const int blocks = (p.n + W - 1) / W, units = p.items[0] * blocks, rt = p.sections * R;
+  const int blocks = (p.n + W - 1) / W, units = p.items[0] * blocks, stride = gridDim.x * 8, rt = p.sections * R;
   const bool in_place = p.out == p.y;
-  for (int u = blockIdx.x * 8 + warp; u < units; u += gridDim.x * 8) {
-    const int item = u / blocks, col0 = (u - item * blocks) * W, col = col0 + g * 2 * MT;
-    const int slot = p.items[1 + 3 * item], first = p.items[2 + 3 * item], rows = p.items[3 + 3 * item];
+  struct Walk {                                                                // through the eights of rows of the warp's units
+    int u, m0, slot, first, rows, col0;
+  };
+  auto enter = [&](Walk& w) {
+    for (;; w.u += stride) {
+      if (w.u >= units) return;
+      const int item = w.u / blocks;
+      w.col0 = (w.u - item * blocks) * W;
+      w.slot = p.items[1 + 3 * item];
+      w.first = p.items[2 + 3 * item];
+      w.rows = p.items[3 + 3 * item];
+      w.m0 = 0;
+      if (w.slot >= 0 || !in_place) return;
+    }
+  };
+  auto advance = [&](Walk& w) {
+    w.m0 += 8;
+    if (w.m0 < w.rows) return;
+    w.u += stride;
+    enter(w);
+  };
+  // what is fetched next: its rows are looked up a step before
+  Walk f{static_cast<int>(blockIdx.x) * 8 + warp, 0, 0, 0, 0, 0};
+  enter(f);
+  Walk w = f;
+  int ahead[I];
+  auto look_up = [&]() {
+#pragma unroll
+    for (int i = 0; i < I; ++i) ahead[i] = f.u < units && f.m0 + rr + i * RP < f.rows && f.col0 + rc * 8 < p.n ? p.order[f.first + f.m0 + rr + i * RP] : -1;
+  };
+  look_up();
+  int put = 0, get = 0;
+  auto fetch = [&]() {
+    if (f.u < units) {
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+        if (ahead[i] >= 0)
+          cp_async16(smem_u32(mine + put * 128 * CH + place(rr + i * RP, rc)), static_cast<const __nv_bfloat16*>(p.y) + ahead[i] * p.ldy + f.col0 + rc * 8, true);
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+        if (rc == 0) ring_row[warp][put][rr + i * RP] = ahead[i];
+      advance(f);
+      look_up();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    put = (put + 1) % kRing;
+  };
+#pragma unroll 1
+  for (int i = 0; i < kRing - 1; ++i) fetch();
+  while (w.u < units) {
+    const int col = w.col0 + g * 2 * MT;
     const bool in = col < p.n;
-    if (slot < 0 && in_place) continue;
     int sec = 0;
-    for (int at = p.width[0]; sec + 1 < p.sections && col0 >= at; at += p.width[sec]) ++sec;
-    const int used = slot < 0 ? 0 : p.ranks ? min(R, max(0, p.ranks[slot])) : R;
+    for (int at = p.width[0]; sec + 1 < p.sections && w.col0 >= at; at += p.width[sec]) ++sec;
+    const int used = w.slot < 0 ? 0 : p.ranks ? min(R, max(0, p.ranks[w.slot])) : R;
     // product t, places g and g + 8: columns 2 t and 2 t + 1 of the lane's
     uint32_t b[MT][R16][4];
-    const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(max(slot, 0)) * p.n + col) * R;
+    const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(max(w.slot, 0)) * p.n + col) * R;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const __nv_bfloat16* at = B + (2 * t + h) * R;
         if (R16 == 1) {
-          const uint2 w = in && used ? __ldg(reinterpret_cast<const uint2*>(at + c * 4)) : make_uint2(0, 0);
-          b[t][0][h] = w.x;
-          b[t][0][2 + h] = w.y;
+          const uint2 v = in && used ? __ldg(reinterpret_cast<const uint2*>(at + c * 4)) : make_uint2(0, 0);
+          b[t][0][h] = v.x;
+          b[t][0][2 + h] = v.y;
         } else {
 #pragma unroll
           for (int s = 0; s < R16 / 2; ++s) {
-            const uint4 w = in && s * 32 < used ? ldg16(at + s * 32 + c * 8) : make_uint4(0, 0, 0, 0);
-            b[t][2 * s][h] = w.x;
-            b[t][2 * s][2 + h] = w.y;
-            b[t][2 * s + 1][h] = w.z;
-            b[t][2 * s + 1][2 + h] = w.w;
+            const uint4 v = in && s * 32 < used ? ldg16(at + s * 32 + c * 8) : make_uint4(0, 0, 0, 0);
+            b[t][2 * s][h] = v.x;
+            b[t][2 * s][2 + h] = v.y;
+            b[t][2 * s + 1][h] = v.z;
+            b[t][2 * s + 1][2 + h] = v.w;
           }
         }
       }
-    // y of the rows 2 c and 2 c + 1 of an eight
-    auto row_of = [&](int r) { return r < rows ? p.order[first + r] : -1; };
-    auto load = [&](int row, uint2 (&v)[V]) {
-      if (row < 0 || !in) return;
-      const __nv_bfloat16* at = static_cast<const __nv_bfloat16*>(p.y) + row * p.ldy + col;
-      if (V == 2) {
-        const uint4 w = *reinterpret_cast<const uint4*>(at);
-        v[0] = make_uint2(w.x, w.y);
-        v[V - 1] = make_uint2(w.z, w.w);
-      } else {
-        v[0] = *reinterpret_cast<const uint2*>(at);
+    const int first = w.first, rows = w.rows;
+    uint2 h[2][R16];                                                           // of the next eight rows
+    auto load_h = [&](int m0) {
+      const size_t at = static_cast<size_t>(first + min(m0 + g, rows - 1)) * rt + sec * R;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(half ? p.lo : p.hi) + at;
+        if (R16 == 1) {
+          h[half][0] = *reinterpret_cast<const uint2*>(from + c * 4);
+        } else {
+#pragma unroll
+          for (int s = 0; s < R16 / 2; ++s) {
+            if (s * 32 >= used) break;
+            const uint4 v = *reinterpret_cast<const uint4*>(from + s * 32 + c * 8);
+            h[half][2 * s] = make_uint2(v.x, v.y);
+            h[half][2 * s + 1] = make_uint2(v.z, v.w);
+          }
+        }
       }
     };
-    constexpr bool AHEAD = R16 * MT <= 8;                             // registers for the next rows
-    int next_row[2][2];
-    uint2 next[2][2][V];
+    if (used) load_h(0);
+    for (int m0 = 0; m0 < rows; m0 += 8) {
+      float acc[MT][4];
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+      for (int t = 0; t < MT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+      if (used) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) next_row[e][i] = row_of(e * 8 + 2 * c + i);
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+          for (int k = 0; k < R16; ++k) {
+            if (k / 2 * 32 >= used) break;                                     // two products share the ranks of 32
 #pragma unroll
-      for (int i = 0; i < 2; ++i) load(next_row[e][i], next[e][i]);
-    for (int m0 = 0; m0 < rows; m0 += 16) {
-      int row[2][2];
-      uint2 y[2][2][V];
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          row[e][i] = next_row[e][i];
-#pragma unroll
-          for (int v = 0; v < V; ++v) y[e][i][v] = next[e][i][v];
-        }
-      auto ahead = [&]() {
-        if (m0 + 16 >= rows) return;
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) next_row[e][i] = row_of(m0 + 16 + e * 8 + 2 * c + i);
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) load(next_row[e][i], next[e][i]);
-      };
-      if (AHEAD) ahead();
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (m0 + e * 8 >= rows) break;
-        float acc[MT][4];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-        if (used) {
-          const size_t at = static_cast<size_t>(first + min(m0 + e * 8 + g, rows - 1)) * rt + sec * R;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(half ? p.lo : p.hi) + at;
-            if (R16 == 1) {
-              const uint2 w = *reinterpret_cast<const uint2*>(h + c * 4);
-#pragma unroll
-              for (int t = 0; t < MT; ++t) mma_bf16(acc[t], b[t][0], w.x, w.y);
-            } else {
-#pragma unroll
-              for (int s = 0; s < R16 / 2; ++s) {
-                if (s * 32 >= used) break;
-                const uint4 w = *reinterpret_cast<const uint4*>(h + s * 32 + c * 8);
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                  mma_bf16(acc[t], b[t][2 * s], w.x, w.y);
-                  mma_bf16(acc[t], b[t][2 * s + 1], w.z, w.w);
-                }
-              }
-            }
+            for (int t = 0; t < MT; ++t) mma_bf16(acc[t], b[t][k], h[half][k].x, h[half][k].y);
           }
         }
+        if (m0 + 8 < rows) load_h(m0 + 8);
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+      __syncwarp();
+      unsigned char* slot = mine + get * 128 * CH;
+      if (used) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if (row[e][i] < 0 || !in) continue;
-          uint32_t q[MT];
+          unsigned char* at = slot + (MT == 4 ? place(2 * c + i, g) : place(2 * c + i, g >> 1) + (g & 1) * 8);
+          uint32_t y[MT];
+          if (MT == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(at);
+            y[0] = v.x; y[1] = v.y; y[MT - 2] = v.z; y[MT - 1] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(at);
+            y[0] = v.x; y[1] = v.y;
+          }
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
-            const uint32_t v = t & 1 ? y[e][i][t / 2].y : y[e][i][t / 2].x;
-            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
-            q[t] = used ? pack_bf16x2(f.x + acc[t][i], f.y + acc[t][2 + i]) : v;
+            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y[t]));
+            y[t] = pack_bf16x2(v.x + acc[t][i], v.y + acc[t][2 + i]);
           }
-          __nv_bfloat16* at = static_cast<__nv_bfloat16*>(p.out) + row[e][i] * p.ldo + col;
-          if (MT == 4) *reinterpret_cast<uint4*>(at) = make_uint4(q[0], q[1], q[MT - 2], q[MT - 1]);
-          else *reinterpret_cast<uint2*>(at) = make_uint2(q[0], q[1]);
+          if (MT == 4) *reinterpret_cast<uint4*>(at) = make_uint4(y[0], y[1], y[MT - 2], y[MT - 1]);
+          else *reinterpret_cast<uint2*>(at) = make_uint2(y[0], y[1]);
         }
+        __syncwarp();
       }
-      if (!AHEAD) ahead();
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+        if (m0 + rr + i * RP < rows && w.col0 + rc * 8 < p.n)
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + ring_row[warp][get][rr + i * RP] * p.ldo + w.col0 + rc * 8) = *reinterpret_cast<const uint4*>(slot + place(rr + i * RP, rc));
+      __syncwarp();
+      get = (get + 1) % kRing;
+      fetch();
     }
+    w.u += stride;
+    enter(w);
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 template <typename Kernel>
@@ -495,8 +546,8 @@ static cudaError_t adapter_down(const CbAdapter& p, int items, cudaStream_t stre
 
 template <int NT>
 static cudaError_t adapter_down_tile(const CbAdapter& p, int items, cudaStream_t stream) {
-  constexpr int NR = NT * 16, smem = 4 * (64 + NR) * 128;
-  static_assert(64 * (NR + 2) * 4 <= smem, "the sums fit where the stages were");
+  constexpr int NR = NT * 16, smem = DownTile<NT>::kBytes;
+  static_assert(64 * DownTile<NT>::SP * 4 <= smem, "the sums fit where the stages were");
   static bool ready[64] = {};
   const cudaError_t e = adapter_smem(adapter_down_tile_kernel<NT>, smem, ready);
   if (e != cudaSuccess) return e;
@@ -508,8 +559,12 @@ static cudaError_t adapter_down_tile(const CbAdapter& p, int items, cudaStream_t
 
 template <int R16, int MT>
 static cudaError_t adapter_up(const CbAdapter& p, int items, cudaStream_t stream) {
+  constexpr int smem = 8 * 8 * 256 * MT, resident = R16 * MT <= 4 ? 3 : 2;
+  static bool ready[64] = {};
+  const cudaError_t e = adapter_smem(adapter_up_kernel<R16, MT>, smem, ready);
+  if (e != cudaSuccess) return e;
   const int warps = items * ((p.n + 16 * MT - 1) / (16 * MT));
-  return launch(adapter_up_kernel<R16, MT>, dim3(min((warps + 7) / 8, 148 * 8)), dim3(kAdapterThreads), 0, stream, p);
+  return launch(adapter_up_kernel<R16, MT>, dim3(min((warps + 7) / 8, 148 * resident)), dim3(kAdapterThreads), smem, stream, p);
 }
 
 template <int R16>
