@@ -19,6 +19,7 @@ static constexpr int kAdapterItemRows = 64;
 static constexpr int kAdapterMaxSlots = 1023;
 static constexpr int kAdapterMaxRows = 65535;
 static constexpr int kAdapterSections = 4;
+static constexpr long long kAdapterMaxStride = 1 << 30;               // in bytes a row fits in 32 bits
 static constexpr int kSortThreads = 1024;
 static constexpr int kAdapterThreads = 256;
 static constexpr int kAdapterFewRows = 256;                           // up to here A is streamed through registers
@@ -350,29 +351,38 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
 }
 
 // out = y + h B^T of one item and 16 MT columns a warp.  B is the operand of sixteen, rows of h those of eight.  Which columns a product has is free: they are
-// chosen so that a lane ends up with 2 MT neighbours of two rows, and eight lanes with a row of 16 MT: whole lines of y and out.  B's operands stay in
-// registers for all rows of the item.  y comes through a ring of the warp's own, seven eights of rows ahead and on into the next items, and goes back through it:
-// eight lanes copy a line of y, and a line of out.  A lane's own columns straight from global memory were four lines a quarter of a warp: 71 % of the load and
-// store unit's cycles, and 3.7 TB/s.
+// chosen so that a lane ends up with 2 MT neighbours of two rows, and eight lanes with a row of 16 MT.  B's operands stay in registers for all rows of the
+// item; the products add to y, which is rounded once.  y comes through a ring of the warp's own, three sixteens of rows ahead and on into the next items, and
+// goes back through it: eight lanes copy a line of y, and a line of out.  (A lane's own columns straight from global memory were four lines a quarter of a
+// warp: 71 % of the load and store unit's cycles.)
 template <int R16, int MT>
 __global__ void __launch_bounds__(kAdapterThreads, R16 * MT <= 4 ? 3 : 2)
 adapter_up_kernel(const CbAdapter p) {
-  constexpr int R = R16 * 16, W = 16 * MT, kRing = 8, CH = 2 * MT, RP = 32 / CH, I = 8 / RP;      // 16-byte chunks of a row, rows of a copy, copies
-  extern __shared__ __align__(16) unsigned char ring[];                        // [8 warps][kRing][8 rows][CH chunks]
-  __shared__ int ring_row[8][kRing][8];                                        // which rows they are
+  constexpr int R = R16 * 16, W = 16 * MT, kRing = 4, CH = 2 * MT, RP = 32 / CH, I = 16 / RP;     // 16-byte chunks of a row, rows of a copy, copies
+  constexpr bool AHEAD = R16 <= 2;                                             // registers for the next rows of h
+  extern __shared__ __align__(16) unsigned char ring[];                        // [8 warps][kRing][16 rows][CH chunks]
+  __shared__ int ring_row[8][kRing][16];                                       // which rows they are
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3, rr = lane / CH, rc = lane % CH;
-  unsigned char* mine = ring + warp * kRing * 128 * CH;
-  auto place = [](int row, int chunk) { return (row * CH + (chunk ^ (MT == 4 ? row & 7 : row >> 1 & 3))) * 16; };
+  unsigned char* mine = ring + warp * kRing * 256 * CH;
+  const uint32_t mine_at = smem_u32(mine);
+  // rows of eight fall on all banks: MT 4 by their number, MT 2 (64 bytes a row) by that of their pair
+  auto place = [](int row, int chunk) { return static_cast<uint32_t>((row * CH + (chunk ^ (MT == 4 ? row & 7 : row >> 1 & 3))) * 16); };
+  uint32_t own[2], copy[I > 1 ? 2 : 1];                                        // places of the lane: its products' rows 2 c + i, the rows it copies; the next eight 128 CH on
+#pragma unroll
+  for (int i = 0; i < 2; ++i) own[i] = MT == 4 ? place(2 * c + i, g) : place(2 * c + i, g >> 1) + (g & 1) * 8;
+#pragma unroll
+  for (int i = 0; i < 8 / RP; ++i) copy[i] = place(rr + i * RP, rc);
+  auto copy_at = [&](int i) { return copy[i % (8 / RP)] + i / (8 / RP) * 128 * CH; };
   pdl_launch_dependents();
   pdl_wait();
-  const int blocks = (p.n + W - 1) / W, units = p.items[0] * blocks, stride = gridDim.x * 8, rt = p.sections * R;
+  const int n = p.n, blocks = (n + W - 1) / W, units = p.items[0] * blocks, stride = gridDim.x * 8, rt = p.sections * R;
+  const uint32_t ldy = static_cast<uint32_t>(p.ldy) * 2, ldo = static_cast<uint32_t>(p.ldo) * 2;
   const bool in_place = p.out == p.y;
-  struct Walk {                                                                // through the eights of rows of the warp's units
+  struct Walk {                                                                // through the sixteens of rows of the warp's units
     int u, m0, slot, first, rows, col0;
   };
   auto enter = [&](Walk& w) {
-    for (;; w.u += stride) {
-      if (w.u >= units) return;
+    for (; w.u < units; w.u += stride) {
       const int item = w.u / blocks;
       w.col0 = (w.u - item * blocks) * W;
       w.slot = p.items[1 + 3 * item];
@@ -381,34 +391,30 @@ adapter_up_kernel(const CbAdapter p) {
       w.m0 = 0;
       if (w.slot >= 0 || !in_place) return;
     }
+    w.rows = 0;
   };
-  auto advance = [&](Walk& w) {
-    w.m0 += 8;
-    if (w.m0 < w.rows) return;
-    w.u += stride;
-    enter(w);
-  };
-  // what is fetched next: its rows are looked up a step before
   Walk f{static_cast<int>(blockIdx.x) * 8 + warp, 0, 0, 0, 0, 0};
   enter(f);
   Walk w = f;
-  int ahead[I];
-  auto look_up = [&]() {
-#pragma unroll
-    for (int i = 0; i < I; ++i) ahead[i] = f.u < units && f.m0 + rr + i * RP < f.rows && f.col0 + rc * 8 < p.n ? p.order[f.first + f.m0 + rr + i * RP] : -1;
-  };
+  // what is fetched next: its rows are looked up a step before, one a lane
+  int ahead = 0;
+  auto look_up = [&]() { if (lane < 16 && f.m0 + lane < f.rows) ahead = p.order[f.first + f.m0 + lane]; };
   look_up();
   int put = 0, get = 0;
   auto fetch = [&]() {
-    if (f.u < units) {
+    if (f.rows) {
+      if (lane < 16) ring_row[warp][put][lane] = ahead;
+      const int left = f.col0 + rc * 8 < n ? f.rows - f.m0 - rr : 0;
+      const char* from = static_cast<const char*>(p.y) + (f.col0 + rc * 8) * 2;
+      const uint32_t to = mine_at + put * 256 * CH;
 #pragma unroll
       for (int i = 0; i < I; ++i)
-        if (ahead[i] >= 0)
-          cp_async16(smem_u32(mine + put * 128 * CH + place(rr + i * RP, rc)), static_cast<const __nv_bfloat16*>(p.y) + ahead[i] * p.ldy + f.col0 + rc * 8, true);
-#pragma unroll
-      for (int i = 0; i < I; ++i)
-        if (rc == 0) ring_row[warp][put][rr + i * RP] = ahead[i];
-      advance(f);
+        cp_async16(to + copy_at(i), from + static_cast<size_t>(ldy) * static_cast<uint32_t>(__shfl_sync(0xffffffffu, ahead, rr + i * RP)), i * RP < left);
+      f.m0 += 16;
+      if (f.m0 >= f.rows) {
+        f.u += stride;
+        enter(f);
+      }
       look_up();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -416,101 +422,115 @@ adapter_up_kernel(const CbAdapter p) {
   };
 #pragma unroll 1
   for (int i = 0; i < kRing - 1; ++i) fetch();
-  while (w.u < units) {
-    const int col = w.col0 + g * 2 * MT;
-    const bool in = col < p.n;
+  while (w.rows) {
+    const int col = w.col0 + g * 2 * MT, first = w.first, rows = w.rows;
+    const bool in = col < n, in_copy = w.col0 + rc * 8 < n;
     int sec = 0;
     for (int at = p.width[0]; sec + 1 < p.sections && w.col0 >= at; at += p.width[sec]) ++sec;
     const int used = w.slot < 0 ? 0 : p.ranks ? min(R, max(0, p.ranks[w.slot])) : R;
-    // product t, places g and g + 8: columns 2 t and 2 t + 1 of the lane's
-    uint32_t b[MT][R16][4];
-    const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(max(w.slot, 0)) * p.n + col) * R;
+    char* to = static_cast<char*>(p.out) + (w.col0 + rc * 8) * 2;
+    uint2 h[AHEAD ? 2 : 1][2][R16];                                            // of eight rows, both parts
+    auto load_h = [&](int e_, int m0) {
+      if (m0 + e_ * 8 < rows) {
+        const size_t at = static_cast<size_t>(first + min(m0 + e_ * 8 + g, rows - 1)) * rt + sec * R;
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+        for (int half = 0; half < 2; ++half) {
+          const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(half ? p.lo : p.hi) + at;
+          const int e = AHEAD ? e_ : 0;
+          if (R16 == 1) {
+            h[e][half][0] = *reinterpret_cast<const uint2*>(from + c * 4);
+          } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const __nv_bfloat16* at = B + (2 * t + h) * R;
-        if (R16 == 1) {
-          const uint2 v = in && used ? __ldg(reinterpret_cast<const uint2*>(at + c * 4)) : make_uint2(0, 0);
-          b[t][0][h] = v.x;
-          b[t][0][2 + h] = v.y;
-        } else {
-#pragma unroll
-          for (int s = 0; s < R16 / 2; ++s) {
-            const uint4 v = in && s * 32 < used ? ldg16(at + s * 32 + c * 8) : make_uint4(0, 0, 0, 0);
-            b[t][2 * s][h] = v.x;
-            b[t][2 * s][2 + h] = v.y;
-            b[t][2 * s + 1][h] = v.z;
-            b[t][2 * s + 1][2 + h] = v.w;
-          }
-        }
-      }
-    const int first = w.first, rows = w.rows;
-    uint2 h[2][R16];                                                           // of the next eight rows
-    auto load_h = [&](int m0) {
-      const size_t at = static_cast<size_t>(first + min(m0 + g, rows - 1)) * rt + sec * R;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(half ? p.lo : p.hi) + at;
-        if (R16 == 1) {
-          h[half][0] = *reinterpret_cast<const uint2*>(from + c * 4);
-        } else {
-#pragma unroll
-          for (int s = 0; s < R16 / 2; ++s) {
-            if (s * 32 >= used) break;
-            const uint4 v = *reinterpret_cast<const uint4*>(from + s * 32 + c * 8);
-            h[half][2 * s] = make_uint2(v.x, v.y);
-            h[half][2 * s + 1] = make_uint2(v.z, v.w);
+            for (int s = 0; s < R16 / 2; ++s) {
+              if (s * 32 >= used) break;
+              const uint4 v = *reinterpret_cast<const uint4*>(from + s * 32 + c * 8);
+              h[e][half][2 * s] = make_uint2(v.x, v.y);
+              h[e][half][2 * s + 1] = make_uint2(v.z, v.w);
+            }
           }
         }
       }
     };
-    if (used) load_h(0);
-    for (int m0 = 0; m0 < rows; m0 += 8) {
-      float acc[MT][4];
+    if (AHEAD && used) { load_h(0, 0); load_h(1, 0); }
+    // product t, places g and g + 8: columns 2 t and 2 t + 1 of the lane's
+    uint32_t b[MT][R16][4];
+    const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(max(w.slot, 0)) * n + col) * R;
 #pragma unroll
-      for (int t = 0; t < MT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-      if (used) {
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+      for (int k = 0; k < 2; ++k) {
+        const __nv_bfloat16* at = B + (2 * t + k) * R;
+        if (R16 == 1) {
+          const uint2 v = in && used ? __ldg(reinterpret_cast<const uint2*>(at + c * 4)) : make_uint2(0, 0);
+          b[t][0][k] = v.x;
+          b[t][0][2 + k] = v.y;
+        } else {
 #pragma unroll
-          for (int k = 0; k < R16; ++k) {
-            if (k / 2 * 32 >= used) break;                                     // two products share the ranks of 32
-#pragma unroll
-            for (int t = 0; t < MT; ++t) mma_bf16(acc[t], b[t][k], h[half][k].x, h[half][k].y);
+          for (int s = 0; s < R16 / 2; ++s) {
+            const uint4 v = in && s * 32 < used ? ldg16(at + s * 32 + c * 8) : make_uint4(0, 0, 0, 0);
+            b[t][2 * s][k] = v.x;
+            b[t][2 * s][2 + k] = v.y;
+            b[t][2 * s + 1][k] = v.z;
+            b[t][2 * s + 1][2 + k] = v.w;
           }
         }
-        if (m0 + 8 < rows) load_h(m0 + 8);
       }
+#pragma unroll 1
+    for (int m0 = 0; m0 < rows; m0 += 16) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
       __syncwarp();
-      unsigned char* slot = mine + get * 128 * CH;
+      unsigned char* slot = mine + get * 256 * CH;
+      const int left = in_copy ? rows - m0 - rr : 0;
       if (used) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          unsigned char* at = slot + (MT == 4 ? place(2 * c + i, g) : place(2 * c + i, g >> 1) + (g & 1) * 8);
-          uint32_t y[MT];
-          if (MT == 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(at);
-            y[0] = v.x; y[1] = v.y; y[MT - 2] = v.z; y[MT - 1] = v.w;
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(at);
-            y[0] = v.x; y[1] = v.y;
+        for (int e = 0; e < 2; ++e) {
+          if (m0 + e * 8 >= rows) break;
+          if (!AHEAD) load_h(e, m0);
+          float acc[MT][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const unsigned char* at = slot + own[i] + e * 128 * CH;
+            uint32_t y[MT];
+            if (MT == 4) {
+              const uint4 v = *reinterpret_cast<const uint4*>(at);
+              y[0] = v.x; y[1] = v.y; y[MT - 2] = v.z; y[MT - 1] = v.w;
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2*>(at);
+              y[0] = v.x; y[1] = v.y;
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              acc[t][i] = __uint_as_float(y[t] << 16);
+              acc[t][2 + i] = __uint_as_float(y[t] & 0xffff0000u);
+            }
           }
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y[t]));
-            y[t] = pack_bf16x2(v.x + acc[t][i], v.y + acc[t][2 + i]);
+          for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int k = 0; k < R16; ++k) {
+              if (k / 2 * 32 >= used) break;                                   // two products share the ranks of 32
+#pragma unroll
+              for (int t = 0; t < MT; ++t) mma_bf16(acc[t], b[t][k], h[AHEAD ? e : 0][half][k].x, h[AHEAD ? e : 0][half][k].y);
+            }
           }
-          if (MT == 4) *reinterpret_cast<uint4*>(at) = make_uint4(y[0], y[1], y[MT - 2], y[MT - 1]);
-          else *reinterpret_cast<uint2*>(at) = make_uint2(y[0], y[1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            unsigned char* at = slot + own[i] + e * 128 * CH;
+            if (MT == 4) {
+              *reinterpret_cast<uint4*>(at) = make_uint4(pack_bf16x2(acc[0][i], acc[0][2 + i]), pack_bf16x2(acc[1][i], acc[1][2 + i]),
+                                                         pack_bf16x2(acc[MT - 2][i], acc[MT - 2][2 + i]), pack_bf16x2(acc[MT - 1][i], acc[MT - 1][2 + i]));
+            } else {
+              *reinterpret_cast<uint2*>(at) = make_uint2(pack_bf16x2(acc[0][i], acc[0][2 + i]), pack_bf16x2(acc[1][i], acc[1][2 + i]));
+            }
+          }
         }
+        if (AHEAD) { load_h(0, m0 + 16); load_h(1, m0 + 16); }
         __syncwarp();
       }
 #pragma unroll
       for (int i = 0; i < I; ++i)
-        if (m0 + rr + i * RP < rows && w.col0 + rc * 8 < p.n)
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + ring_row[warp][get][rr + i * RP] * p.ldo + w.col0 + rc * 8) = *reinterpret_cast<const uint4*>(slot + place(rr + i * RP, rc));
+        if (i * RP < left)
+          *reinterpret_cast<uint4*>(to + static_cast<size_t>(ldo) * static_cast<uint32_t>(ring_row[warp][get][rr + i * RP])) = *reinterpret_cast<const uint4*>(slot + copy_at(i));
       __syncwarp();
       get = (get + 1) % kRing;
       fetch();
@@ -559,7 +579,7 @@ static cudaError_t adapter_down_tile(const CbAdapter& p, int items, cudaStream_t
 
 template <int R16, int MT>
 static cudaError_t adapter_up(const CbAdapter& p, int items, cudaStream_t stream) {
-  constexpr int smem = 8 * 8 * 256 * MT, resident = R16 * MT <= 4 ? 3 : 2;
+  constexpr int smem = 8 * 4 * 512 * MT, resident = R16 * MT <= 4 ? 3 : 2;
   static bool ready[64] = {};
   const cudaError_t e = adapter_smem(adapter_up_kernel<R16, MT>, smem, ready);
   if (e != cudaSuccess) return e;
@@ -607,7 +627,7 @@ int cb_adapter_rows(const void* ids, int rows, int slots, void* order, void* ite
 int cb_adapter_add(const CbAdapter* p, void* stream) {
   using namespace cb;
   if (p->rows < 0 || p->rows > kAdapterMaxRows || p->slots < 1 || p->slots > kAdapterMaxSlots || p->k < 8 || p->k % 8 || p->n < 8 || p->n % 8) return -10;
-  if (p->sections < 1 || p->sections > kAdapterSections || p->ldx % 8 || p->ldy % 8 || p->ldo % 8) return -11;
+  if (p->sections < 1 || p->sections > kAdapterSections || p->ldx % 8 || p->ldy % 8 || p->ldo % 8 || p->ldy > kAdapterMaxStride || p->ldo > kAdapterMaxStride) return -11;
   int n = 0;
   for (int i = 0; i < p->sections; ++i) {
     if (p->width[i] < 8 || (i + 1 < p->sections && p->width[i] % 32)) return -12;

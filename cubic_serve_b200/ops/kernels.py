@@ -897,7 +897,7 @@ def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, rows: Adapt
     _require(bank.sections * bank.rank <= rows.max_ranks, "more ranks than the sorted rows have room for")
     ldx, ldy, ldo = (x.stride(0), y.stride(0), out.stride(0)) if t > 1 else (bank.k, bank.n, bank.n)
     px, py, po = x.data_ptr(), y.data_ptr(), out.data_ptr()
-    _require(x.stride(1) == 1 and y.stride(1) == 1 and out.stride(1) == 1 and ldx >= bank.k and ldy >= bank.n and ldo >= bank.n and (ldx | ldy | ldo) % 8 == 0 and (px | py | po) % 16 == 0,
+    _require(x.stride(1) == 1 and y.stride(1) == 1 and out.stride(1) == 1 and ldx >= bank.k and ldy >= bank.n and ldo >= bank.n and (ldx | ldy | ldo) % 8 == 0 and max(ldy, ldo) <= 1 << 30 and (px | py | po) % 16 == 0,
              "rows of neighbouring elements at a stride of a multiple of 8, from a 16-byte boundary")
     packed = native.ADAPTER.pack(px, ldx, py, ldy, po, ldo, *bank._at, *rows._at, t, *bank._shape)
     _call("cb_adapter_add", (packed,), (x, y, out, bank.a, rows.order))
