@@ -4,7 +4,7 @@
 // ranks [j rank, (j + 1) rank).
 //
 // Three kernels.  `adapter_rows_kernel` sorts a step's rows by adapter, once for all projections of all layers.  `adapter_down_kernel`
-// makes h = scale x A^T of the sorted rows, `adapter_up_kernel` adds h B^T.  A work item is up to 64 rows of one adapter.
+// makes h = scale x A^T of the sorted rows, `adapter_up_kernel` adds h B^T.  A work item is up to 16 rows of one adapter in small steps, 64 in large.
 //
 // Bound by memory: with few rows by A and B of the adapters in use, with many by y and out.  The products run on
 // mma.sync m16n8k16 with operands that go from global memory to registers: rank 16 makes 16 products of every byte of x, far from
@@ -15,14 +15,16 @@
 
 namespace cb {
 
-static constexpr int kAdapterItemRows = 64;
+// Up to here a work item is sixteen rows and A is streamed through registers, from here on it is 64 and A and x come by tiles.  331 rows over two adapters, a
+// layer: 82 us by tiles, 56 by sixteens.
+static constexpr int kAdapterFewRows = 512;
+static constexpr int adapter_item_rows(int rows) { return rows <= kAdapterFewRows ? 16 : 64; }
 static constexpr int kAdapterMaxSlots = 1023;
 static constexpr int kAdapterMaxRows = 65535;
 static constexpr int kAdapterSections = 4;
 static constexpr long long kAdapterMaxStride = 1 << 30;               // in bytes a row fits in 32 bits
 static constexpr int kSortThreads = 1024;
 static constexpr int kAdapterThreads = 256;
-static constexpr int kAdapterFewRows = 256;                           // up to here A is streamed through registers
 
 // ------------------------------------------------------------------ rows by adapter
 // order[]: the step's rows by adapter, a row's place among its adapter's by its index; rows without one last.
@@ -58,7 +60,7 @@ adapter_rows_kernel(const int* __restrict__ ids, int rows, int slots, int* __res
       cnt[w * buckets + tid] = static_cast<unsigned short>(n);
       n += c;
     }
-  const int nt = (n + kAdapterItemRows - 1) / kAdapterItemRows;
+  const int per = adapter_item_rows(rows), nt = (n + per - 1) / per;
   int at = n, it = nt;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -74,8 +76,8 @@ adapter_rows_kernel(const int* __restrict__ ids, int rows, int slots, int* __res
     for (int i = 0; i < nt; ++i) {
       int* e = items + 1 + 3 * (it - nt + i);
       e[0] = tid < slots ? tid : -1;
-      e[1] = at + i * kAdapterItemRows;
-      e[2] = min(kAdapterItemRows, n - i * kAdapterItemRows);
+      e[1] = at + i * per;
+      e[2] = min(per, n - i * per);
     }
   }
   if (tid == kSortThreads - 1) items[0] = it;
@@ -100,7 +102,7 @@ struct CbAdapter {
   const void* x; long long ldx;          // bf16 [rows, k]
   const void* y; long long ldy;          // bf16 [rows, n]
   void* out; long long ldo;              // bf16 [rows, n], may be y
-  const void* a;                         // bf16 [slots, sections * rank, k]
+  const void* a;                         // bf16 [slots, ceil(k / 32), sections * rank, 32]: what is read together lies together
   const void* b;                         // bf16 [slots, n, rank]
   const float* scale;                    // [slots]
   const int* ranks;                      // [slots] ranks in use, or null: all
@@ -137,25 +139,25 @@ __device__ __forceinline__ void put_h(const CbAdapter& p, float v, float scale, 
 
 // h of few rows: one item, one section, sixteen rows at a time.  A is the operand of sixteen, rows of x those of eight, for most adapters of a decode step have
 // no more.  The eight warps and the CTAs of a cluster take turns of 32 along k; sums are joined in their order.  The order of k inside a product is free: a
-// lane's 16 bytes of x and of A are its operands of two products as they lie.  J turns of a warp are on their way at once.
-template <int R16, int J>
-__global__ void __launch_bounds__(kAdapterThreads)
+// lane's 16 bytes of x and of A are its operands of two products as they lie.  J turns of a warp are on their way while J others are multiplied.
+template <int R16>
+__global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_down_kernel(const CbAdapter p, int splits) {
-  constexpr int R = R16 * 16, RP = R + 4;
+  constexpr int R = R16 * 16, RP = R + 4, J = R16 == 1 ? 2 : 1, kBuffers = R16 == 8 ? 1 : 2;
   extern __shared__ float sh[];                                       // [8][16][RP], then the cluster's part [16][R]
   float* part = sh + 8 * 16 * RP;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const int rank_in = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0, team = blockIdx.x / splits, teams = gridDim.x / splits;
   pdl_launch_dependents();
   pdl_wait();
-  const int units = p.items[0] * p.sections, rt = p.sections * R, turns = (p.k + 31) >> 5;
+  const int units = p.items[0] * p.sections, rt = p.sections * R, turns = (p.k + 31) >> 5, step = 8 * splits;
   for (int u = team; u < units; u += teams) {
     const int item = u / p.sections, sec = u - item * p.sections;
     const int slot = p.items[1 + 3 * item], first = p.items[2 + 3 * item], rows = p.items[3 + 3 * item];
     if (slot < 0) continue;
     const float scale = p.scale[slot];
     const int used = p.ranks ? min(R, max(0, p.ranks[slot])) : R;
-    const __nv_bfloat16* A = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * rt + sec * R + g) * p.k + c * 8;
+    const __nv_bfloat16* A = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * turns * rt + sec * R) * 32 + lane * 8;
     for (int m0 = 0; m0 < rows; m0 += 16) {
       const int left = min(16, rows - m0);
       const bool in0 = g < left, in1 = g + 8 < left, both = left > 8;
@@ -166,32 +168,51 @@ adapter_down_kernel(const CbAdapter p, int splits) {
       for (int t = 0; t < R16; ++t)
 #pragma unroll
         for (int h = 0; h < 2; ++h) acc[t][h][0] = acc[t][h][1] = acc[t][h][2] = acc[t][h][3] = 0.f;
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      for (int t0 = rank_in * 8 + warp; t0 < turns; t0 += 8 * J * splits) {
-        uint4 w[J][R16][2], xa[J], xb[J];
+      uint4 w[kBuffers][J][R16][2], xa[kBuffers][J], xb[kBuffers][J];
+      auto load = [&](int b, int t0) {
+        const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          const int k = (t0 + j * 8 * splits) * 32;
-          const bool in = k + c * 8 < p.k;
-          xa[j] = in && in0 ? ldg16(x0 + k) : zero;
-          xb[j] = in && in1 ? ldg16(x1 + k) : zero;
+          const int at = t0 + j * step;
+          const bool in = at < turns, in_x = at * 32 + c * 8 < p.k;
+          xa[b][j] = in_x && in0 ? ldg16(x0 + at * 32) : zero;
+          xb[b][j] = in_x && in1 ? ldg16(x1 + at * 32) : zero;
+          const __nv_bfloat16* from = A + static_cast<size_t>(at) * rt * 32;
 #pragma unroll
           for (int t = 0; t < R16; ++t)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) w[j][t][h] = in && t * 16 + h * 8 < used ? ldg16(A + static_cast<size_t>(t * 16 + h * 8) * p.k + k) : zero;
+            for (int h = 0; h < 2; ++h) w[b][j][t][h] = in && t * 16 + h * 8 < used ? ldg16(from + (t * 16 + h * 8) * 32) : zero;
         }
+      };
+      auto multiply = [&](int b) {
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
           for (int t = 0; t < R16; ++t) {
-            const uint32_t f0[4] = {w[j][t][0].x, w[j][t][1].x, w[j][t][0].y, w[j][t][1].y}, f1[4] = {w[j][t][0].z, w[j][t][1].z, w[j][t][0].w, w[j][t][1].w};
-            mma_bf16(acc[t][0], f0, xa[j].x, xa[j].y);
-            mma_bf16(acc[t][0], f1, xa[j].z, xa[j].w);
+            const uint4 &lo = w[b][j][t][0], &hi = w[b][j][t][1];
+            const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
+            mma_bf16(acc[t][0], f0, xa[b][j].x, xa[b][j].y);
+            mma_bf16(acc[t][0], f1, xa[b][j].z, xa[b][j].w);
             if (both) {
-              mma_bf16(acc[t][1], f0, xb[j].x, xb[j].y);
-              mma_bf16(acc[t][1], f1, xb[j].z, xb[j].w);
+              mma_bf16(acc[t][1], f0, xb[b][j].x, xb[b][j].y);
+              mma_bf16(acc[t][1], f1, xb[b][j].z, xb[b][j].w);
             }
           }
+      };
+      const int t0 = rank_in * 8 + warp;
+      if (kBuffers == 1) {
+        for (int t = t0; t < turns; t += J * step) {
+          load(0, t);
+          multiply(0);
+        }
+      } else {
+        load(0, t0);
+        for (int t = t0; t < turns; t += 2 * J * step) {
+          load(kBuffers - 1, t + J * step);
+          multiply(0);
+          load(0, t + 2 * J * step);
+          multiply(kBuffers - 1);
+        }
       }
       float* mine = sh + warp * 16 * RP;
 #pragma unroll
@@ -252,7 +273,7 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
   pdl_launch_dependents();
   pdl_wait();
   const int rt = p.sections * p.rank, parts = (rt + NR - 1) / NR, units = p.items[0] * parts, stages = (p.k + 64 * H - 1) / (64 * H);
-  const int share = (stages + splits - 1) / splits, s0 = rank_in * share, s1 = min(stages, s0 + share);
+  const int turns = (p.k + 31) >> 5, share = (stages + splits - 1) / splits, s0 = rank_in * share, s1 = min(stages, s0 + share);
   const uint32_t base = smem_u32(st);
   for (int u = team; u < units; u += teams) {
     const int item = u / parts, r0 = (u - item * parts) * NR;
@@ -271,7 +292,7 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
     for (int i = 0; i < AR; ++i) {
       const int r = r0 + row + 32 * i;
       ain[i] = row + 32 * i < NR && r < rt && r % p.rank < used;
-      ar[i] = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * rt + (ain[i] ? r : 0)) * p.k + ch * 8;
+      ar[i] = static_cast<const __nv_bfloat16*>(p.a) + ((static_cast<size_t>(slot) * turns + ch / 4) * rt + (ain[i] ? r : 0)) * 32 + ch % 4 * 8;
     }
     const uint32_t to0 = base + row * 128 + ((ch ^ (row & 7)) << 4);
     auto fetch = [&](int s, int buf) {
@@ -284,7 +305,7 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
         for (int i = 0; i < 2; ++i) cp_async16(to + i * 32 * 128, in && xin[i] ? xr[i] + k : p.x, in && xin[i]);
 #pragma unroll
         for (int i = 0; i < AR; ++i)
-          if (row + 32 * i < NR) cp_async16(to + (64 + i * 32) * 128, in && ain[i] ? static_cast<const void*>(ar[i] + k) : p.a, in && ain[i]);
+          if (row + 32 * i < NR) cp_async16(to + (64 + i * 32) * 128, in && ain[i] ? static_cast<const void*>(ar[i] + static_cast<size_t>(k) * rt) : p.a, in && ain[i]);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -551,17 +572,24 @@ static cudaError_t adapter_smem(Kernel kernel, int smem, bool (&ready)[64]) {
   return e;
 }
 
+// CTAs that share k: as long as two find room on every SM.  Layers of 256 rows over 64 adapters of rank 64 and of 8192 rows of rank 16 by the most CTAs: 148
+// 178 and 456 us, 320 164 and 408, 592 180 and 426.
+static int adapter_splits(int units, int k) {
+  int splits = 1;
+  while (splits < 8 && units * splits * 2 <= 320 && k / (splits * 2) >= 256) splits *= 2;
+  return splits;
+}
+
 template <int R16>
 static cudaError_t adapter_down(const CbAdapter& p, int items, cudaStream_t stream) {
-  constexpr int R = R16 * 16, J = R16 == 1 ? 4 : R16 == 2 ? 3 : R16 == 4 ? 2 : 1;
+  constexpr int R = R16 * 16;
   constexpr int smem = (8 * 16 * (R + 4) + 16 * R) * sizeof(float);
   static bool ready[64] = {};
-  const cudaError_t e = adapter_smem(adapter_down_kernel<R16, J>, smem, ready);
+  const cudaError_t e = adapter_smem(adapter_down_kernel<R16>, smem, ready);
   if (e != cudaSuccess) return e;
   const int units = items * p.sections;
-  int splits = 1;
-  while (splits < 8 && units * splits * 2 <= 296 && p.k / (splits * 2) >= 256) splits *= 2;
-  return launch(adapter_down_kernel<R16, J>, dim3(min(units, 592 / splits) * splits), dim3(kAdapterThreads), smem, stream, dim3(splits, 1, 1), p, splits);
+  const int splits = adapter_splits(units, p.k);
+  return launch(adapter_down_kernel<R16>, dim3(min(units, 592 / splits) * splits), dim3(kAdapterThreads), smem, stream, dim3(splits, 1, 1), p, splits);
 }
 
 template <int NT>
@@ -572,8 +600,7 @@ static cudaError_t adapter_down_tile(const CbAdapter& p, int items, cudaStream_t
   const cudaError_t e = adapter_smem(adapter_down_tile_kernel<NT>, smem, ready);
   if (e != cudaSuccess) return e;
   const int units = items * ((p.sections * p.rank + NR - 1) / NR);
-  int splits = 1;
-  while (splits < 8 && units * splits * 2 <= 296 && p.k / (splits * 2) >= 256) splits *= 2;
+  const int splits = adapter_splits(units, p.k);
   return launch(adapter_down_tile_kernel<NT>, dim3(min(units, 592 / splits) * splits), dim3(kAdapterThreads), smem, stream, dim3(splits, 1, 1), p, splits);
 }
 
@@ -598,12 +625,15 @@ static int adapter_launch(const CbAdapter& p, int items, cudaStream_t stream) {
       : n == 4 ? adapter_down_tile<4>(p, items, stream) : n % 8 == 0 ? adapter_down_tile<8>(p, items, stream) : adapter_down_tile<6>(p, items, stream);
   }
   if (e != cudaSuccess) return static_cast<int>(e);
-  bool wide = R16 < 8;                                                // a warp's columns belong to one section
+  bool wide = R16 < 4;                                                // a warp's columns belong to one section
   for (int i = 0; i + 1 < p.sections; ++i) wide = wide && p.width[i] % 64 == 0;
-  return static_cast<int>(wide ? adapter_up<R16, R16 < 8 ? 4 : 2>(p, items, stream) : adapter_up<R16, 2>(p, items, stream));
+  return static_cast<int>(wide ? adapter_up<R16, R16 < 4 ? 4 : 2>(p, items, stream) : adapter_up<R16, 2>(p, items, stream));
 }
 
-static int adapter_items(int rows, int slots) { return rows / kAdapterItemRows + min(slots + 1, rows); }
+static int adapter_items(int rows, int slots) {
+  const int used = min(slots + 1, rows);                              // adapters with a row, each with one item and what its other rows fill
+  return used + (rows - used) / adapter_item_rows(rows);
+}
 
 }  // namespace cb
 

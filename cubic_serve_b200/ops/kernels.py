@@ -803,12 +803,13 @@ def step_layout(request: torch.Tensor, start: torch.Tensor, count: torch.Tensor,
 
 
 class AdapterBank:
-    """The low-rank adapters of one projection: ``a`` bf16 ``[slots, sections * rank, k]``, ``b`` bf16 ``[slots, n, rank]``,
-    ``scale`` fp32 ``[slots]``.  ``widths``: columns of the projection's sections (q | k | v), each with its own ranks of
-    ``a``; all but the last a multiple of 32.  ``ranks`` int32 ``[slots]``: ranks in use of every adapter (0: an empty slot).
+    """The low-rank adapters of one projection, in the kernels' layout: made from ``a`` bf16 ``[slots, sections * rank, k]``,
+    ``b`` bf16 ``[slots, n, rank]``, ``scale`` fp32 ``[slots]``.  ``widths``: columns of the projection's sections (q | k | v),
+    each with its own ranks of ``a``; all but the last a multiple of 32.  ``ranks`` int32 ``[slots]``: ranks in use of every
+    adapter (None: all; 0: an empty slot).
 
-    Ranks up to 128; one that is not 16, 32, 64 or 128 is stored with zeros up to the next.  Tensors that need none are kept as
-    they are: what is copied into them later takes effect (``load`` writes one slot)."""
+    ``a`` becomes ``[slots, ceil(k / 32), sections * rank, 32]``; ranks up to 128 are stored as 16, 32, 64 or 128, with zeros.
+    ``load`` writes one slot, at the same addresses: captured graphs follow."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, widths: tuple[int, ...] | None = None, ranks: torch.Tensor | None = None) -> None:
         _require(a.dtype == b.dtype == torch.bfloat16 and a.dim() == b.dim() == 3 and a.shape[0] == b.shape[0], "adapters are bf16 [slots, ranks, k] and [slots, n, rank]")
@@ -824,17 +825,16 @@ class AdapterBank:
         for t in (b, scale, ranks):
             _require(t is None or t.device == a.device, "tensors must be on one device")
         full = next(r for r in (16, 32, 64, 128) if r >= rank)
-        self.max_rank = rank
-        if full != rank:
-            a = torch.nn.functional.pad(a.view(slots, S, rank, -1) if a.is_contiguous() else a.reshape(slots, S, rank, -1), (0, 0, 0, full - rank)).reshape(slots, S * full, -1)
-            b = torch.nn.functional.pad(b, (0, full - rank))
-            if ranks is None:
-                ranks = torch.full((slots,), rank, dtype=torch.int32, device=a.device)
-        a, b = a.contiguous(), b.contiguous()
-        _require(a.data_ptr() % 16 == 0 and b.data_ptr() % 16 == 0, "adapters start on a 16-byte boundary")
+        self.max_rank, k = rank, a.shape[2]
+        blocks = -(-k // 32)
+        pad = torch.nn.functional.pad
+        a = pad(a.reshape(slots, S, rank, k), (0, blocks * 32 - k, 0, full - rank)).view(slots, S * full, blocks, 32).transpose(1, 2).contiguous()
+        b = pad(b, (0, full - rank)) if full != rank else b.clone(memory_format=torch.contiguous_format)
+        scale = scale.clone()
+        ranks = torch.full((slots,), rank, dtype=torch.int32, device=a.device) if ranks is None else ranks.clone()
         self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
-        self.slots, self.k, self.n, self.rank, self.sections = slots, a.shape[2], n, full, S
-        self._at = (a.data_ptr(), b.data_ptr(), scale.data_ptr(), 0 if ranks is None else ranks.data_ptr())
+        self.slots, self.k, self.n, self.rank, self.sections = slots, k, n, full, S
+        self._at = (a.data_ptr(), b.data_ptr(), scale.data_ptr(), ranks.data_ptr())
         self._shape = (slots, self.k, n, full, S, *self.widths, *(0,) * (4 - S))
 
     def load(self, slot: int, a, b, scale: float) -> None:
@@ -847,16 +847,16 @@ class AdapterBank:
             _require((ai is None) == (bi is None), "a section has both matrices or none")
             r = 0 if ai is None else ai.shape[0]
             _require(r <= self.max_rank and (r == 0 or (tuple(ai.shape) == (r, self.k) and tuple(bi.shape) == (width, r))), f"section {i}: [rank <= {self.max_rank}, {self.k}] and [{width}, rank]")
-            self.a[slot, at:at + self.rank].zero_()
+            self.a[slot, :, at:at + self.rank].zero_()
             self.b[slot, col:col + width].zero_()
             if r:
-                self.a[slot, at:at + r].copy_(ai)
+                rows = torch.nn.functional.pad(ai.to(self.a.device, self.a.dtype), (0, self.a.shape[1] * 32 - self.k))
+                self.a[slot, :, at:at + r].copy_(rows.view(r, -1, 32).transpose(0, 1))
                 self.b[slot, col:col + width, :r].copy_(bi)
             col += width
             most = max(most, r)
         self.scale[slot] = float(scale)
-        if self.ranks is not None:
-            self.ranks[slot] = most
+        self.ranks[slot] = most
 
 
 class AdapterRows:
@@ -869,7 +869,7 @@ class AdapterRows:
         self.max_rows, self.slots, self.rows = max_rows, slots, 0
         self.max_ranks = max(64, 2 * max_ranks)                     # ranks are stored as 16, 32, 64 or 128
         self.order = torch.zeros(max_rows, dtype=torch.int32, device=device)
-        self.items = torch.zeros(1 + 3 * (max_rows // 64 + min(slots + 1, max_rows)), dtype=torch.int32, device=device)
+        self.items = torch.zeros(1 + 3 * (max(max_rows // 64, min(max_rows, 512) // 16) + min(slots + 1, max_rows)), dtype=torch.int32, device=device)
         self.h = torch.zeros(2, max_rows * self.max_ranks, dtype=torch.bfloat16, device=device)
         self._at = (self.order.data_ptr(), self.items.data_ptr(), self.h[0].data_ptr(), self.h[1].data_ptr())
 

@@ -249,7 +249,9 @@ def test_adapters_in_a_graph_follow_the_ids_and_the_weights():
                 K.adapter_add(x, y, bank, K.adapter_rows(ids, plan), out=out)
         graphs.append((g, ids, out, st))
     for trial in range(3):
-        bank.load(trial % 3, [torch.randn(16, k, device=DEV) * 0.05] * 2, [torch.randn(w, 16, device=DEV) * 0.1 for w in widths], 0.5 + trial)
+        new_a, new_b = [torch.randn(16, k, device=DEV).bfloat16() * 0.05 for _ in widths], [torch.randn(n, 16, device=DEV).bfloat16() * 0.1 for n in widths]
+        bank.load(trial % 3, new_a, new_b, 0.5 + trial)
+        a[trial % 3], b[trial % 3], scale[trial % 3] = torch.cat(new_a), torch.cat(new_b), 0.5 + trial
         for i, (g, ids, out, st) in enumerate(graphs):
             ids.copy_(torch.from_numpy(np.random.default_rng(10 * trial + i).integers(-1, 3, rows).astype(np.int32)))
         torch.cuda.synchronize()
@@ -258,7 +260,7 @@ def test_adapters_in_a_graph_follow_the_ids_and_the_weights():
                 g.replay()
         torch.cuda.synchronize()
         for g, ids, out, _ in graphs:
-            want, err = _adapter_truth(x, y, bank.a, bank.b, bank.scale, widths, ids)
+            want, err = _adapter_truth(x, y, a, b, scale, widths, ids)
             assert bool(((out.double() - want).abs() <= err).all())
 
 

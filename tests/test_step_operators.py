@@ -57,15 +57,23 @@ def test_adapter_banks_refuse(make):
         make()
 
 
+def _stored(bank):
+    """[slots, sections, stored ranks, k stored] of a bank's A."""
+    return bank.a.transpose(1, 2).reshape(bank.slots, bank.sections, bank.rank, -1)
+
+
 def test_bank_ranks_are_stored_as_the_next_width():
     b = _bank(rank=20, sections=3, n=96, widths=(32, 32, 32))
-    assert b.rank == 32 and b.a.shape == (2, 96, 64) and b.b.shape == (2, 96, 32) and b.ranks.tolist() == [20, 20]
-    a = torch.randn(2, 3 * 20, 64).bfloat16()
+    assert b.rank == 32 and b.a.shape == (2, 2, 96, 32) and b.b.shape == (2, 96, 32) and b.ranks.tolist() == [20, 20]
+    a = torch.randn(2, 3 * 20, 72).bfloat16()
     b = K.AdapterBank(a, torch.randn(2, 96, 20).bfloat16(), torch.ones(2), (32, 32, 32))
-    assert torch.equal(b.a.view(2, 3, 32, 64)[:, :, :20].reshape(2, 60, 64), a) and not b.a.view(2, 3, 32, 64)[:, :, 20:].any()
-    b.load(1, [torch.ones(4, 64), None, torch.full((20, 64), 2.0)], [torch.ones(32, 4), None, torch.ones(32, 20)], 0.5)
-    assert b.ranks.tolist() == [20, 20] and b.scale.tolist() == [1.0, 0.5] and not b.a[1, 32:64].any() and b.a[1, :4].eq(1).all() and not b.a[1, 4:32].any()
-    for bad in (dict(slot=2), dict(a=[torch.ones(21, 64), None, None], b=[torch.ones(32, 21), None, None]), dict(a=[torch.ones(4, 60)] * 3, b=[torch.ones(32, 4)] * 3), dict(a=[None] * 2, b=[None] * 2)):
+    assert torch.equal(_stored(b)[:, :, :20, :72].reshape(2, 60, 72), a) and not _stored(b)[:, :, 20:].any() and not _stored(b)[..., 72:].any()
+    b.load(1, [torch.ones(4, 72), None, torch.full((20, 72), 2.0)], [torch.ones(32, 4), None, torch.ones(32, 20)], 0.5)
+    s = _stored(b)[1]
+    assert b.ranks.tolist() == [20, 20] and b.scale.tolist() == [1.0, 0.5] and not s[1].any() and s[0, :4, :72].eq(1).all() and not s[0, 4:].any() and s[2, :20, :72].eq(2).all()
+    b.load(0, [torch.ones(3, 72)] * 3, [torch.ones(32, 3)] * 3, 1.0)
+    assert b.ranks.tolist() == [3, 20]
+    for bad in (dict(slot=2), dict(a=[torch.ones(21, 72), None, None], b=[torch.ones(32, 21), None, None]), dict(a=[torch.ones(4, 64)] * 3, b=[torch.ones(32, 4)] * 3), dict(a=[None] * 2, b=[None] * 2)):
         with pytest.raises(ValueError):
             b.load(**{"slot": 0, "a": [None] * 3, "b": [None] * 3, "scale": 1.0, **bad})
 
