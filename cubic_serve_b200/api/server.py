@@ -157,7 +157,8 @@ class CubicASGIApp:
                 return
             if path == "/v1/models" and method == "GET":
                 await self._json(send, 200, {"object": "list", "data": [
-                    {"id": self.served_model_name, "object": "model", "created": self.created, "owned_by": "cubic-serve-b200"}]})
+                    {"id": name, "object": "model", "created": self.created, "owned_by": "cubic-serve-b200"}
+                    for name in (self.served_model_name, *self._adapter_names())]})
                 return
             if path in ("/v1/chat/completions", "/v1/messages"):
                 if method != "POST":
@@ -222,6 +223,9 @@ class CubicASGIApp:
             if not msg.get("more_body", False):
                 return b"".join(chunks)
 
+    def _adapter_names(self) -> tuple[str, ...]:
+        return tuple(getattr(self.backend, "adapter_names", ()))
+
     async def _chat(self, protocol: str, receive, send) -> None:
         try:
             raw = await self._read_body(receive)
@@ -232,10 +236,12 @@ class CubicASGIApp:
                 req = normalize_openai_chat_completions(body, self.served_model_name, self.sampling_defaults)
             else:
                 req = normalize_anthropic_messages(body, self.served_model_name, self.sampling_defaults)
-            if req.model not in self.accepted_names:
+            if req.model in self._adapter_names() and req.model not in self.accepted_names:
+                pass                                 # a low-rank adapter beside the model: responses carry its name
+            elif req.model not in self.accepted_names:
                 raise RequestError(f"model {req.model!r} is not served here", param="model", status=404,
                                    code="model_not_found")
-            if req.model != self.served_model_name:
+            elif req.model != self.served_model_name:
                 import dataclasses
                 req = dataclasses.replace(req, model=self.served_model_name)      # responses carry the first public name
             if not getattr(self.backend, "ready", True):

@@ -154,6 +154,11 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--dtype", choices=("bfloat16", "float32"), default="bfloat16",
                    help="activations and products; float32 is available for the layered decoders")
     g.add_argument("--max-model-len", type=int)
+    g.add_argument("--low-rank-adapter", action="append", default=[], metavar="NAME=DIR",
+                   help="serve the low-rank adapter of this directory beside the model: requests whose `model` is NAME are "
+                        "computed with it (repeatable; one GPU, native mode)")
+    g.add_argument("--low-rank-slots", type=int, default=None, help="adapters that can be loaded at once (default: those given)")
+    g.add_argument("--low-rank-max-rank", type=int, default=64, help="largest rank of a low-rank adapter")
     g.add_argument("--chat-template")
     g.add_argument("--reasoning-parser", default="auto")
     g.add_argument("--tool-call-parser", default="hermes")

@@ -83,7 +83,9 @@ class StructuredOutput:
 
 @dataclass(frozen=True)
 class SamplingMeta:
-    """Sampling controls; ranges follow the reference (T in [0, 2], top_k <= 20)."""
+    """Sampling controls; ranges follow the reference (T in [0, 2], top_k <= 20).  Beyond it: ``whole_vocabulary`` draws from
+    all tokens instead of the 20 best (``top_k`` is then any number, 0 = all), and so does ``min_p`` above 0, which keeps the
+    tokens with at least this share of the best one's probability."""
     temperature: float = 1.0
     top_p: float = 1.0
     top_k: int = 0
@@ -95,13 +97,17 @@ class SamplingMeta:
     frequency_penalty: float = 0.0
     logprobs: bool = False
     top_logprobs: int = 0
+    whole_vocabulary: bool = False
+    min_p: float = 0.0
 
     def __post_init__(self) -> None:
         if not 0.0 <= self.temperature <= 2.0:
             raise RequestError("temperature must be between 0 and 2", param="temperature")
         if not 0.0 < self.top_p <= 1.0:
             raise RequestError("top_p must be in (0, 1]", param="top_p")
-        if not 0 <= self.top_k <= 20:
+        if not 0.0 <= self.min_p <= 1.0:
+            raise RequestError("min_p must be in [0, 1]", param="min_p")
+        if not 0 <= self.top_k <= (2 ** 31 - 1 if self.whole_vocabulary or self.min_p > 0 else 20):
             raise RequestError("top_k must be between 0 and 20", param="top_k")
         if self.max_tokens is not None and self.max_tokens < 1:
             raise RequestError("max_tokens must be at least 1", param="max_tokens")

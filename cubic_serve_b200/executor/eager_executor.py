@@ -27,6 +27,8 @@ def sample_row(logits: torch.Tensor, s: Segment) -> int:
         logits = logits.masked_fill(~allowed, float("-inf"))
     if s.temperature <= 0:
         return int(logits.argmax())
+    if getattr(s, "whole", False):
+        return _draw_whole(logits, s)
     k = s.top_k if 0 < s.top_k <= 20 else 20
     vals, idx = logits.topk(k)
     p = torch.softmax(vals / s.temperature, -1)
@@ -37,7 +39,24 @@ def sample_row(logits: torch.Tensor, s: Segment) -> int:
     return int(idx[torch.multinomial(p, 1, generator=g)])
 
 
+def _draw_whole(logits: torch.Tensor, s: Segment) -> int:
+    """A draw from the whole vocabulary: the first ``top_k`` tokens (0: all), of those the shortest prefix with ``top_p`` of
+    their mass, of those the ones with at least ``min_p`` of the best one's probability."""
+    vals, idx = logits.double().masked_fill(logits.isnan(), float("-inf")).sort(descending=True, stable=True)
+    w = torch.where(vals == vals[0], 1.0, torch.exp((vals - vals[0]) / s.temperature))
+    n = min(s.top_k, w.numel()) if s.top_k > 0 else w.numel()
+    if s.top_p < 1:
+        upto = w[:n].cumsum(0)
+        n = int((upto < s.top_p * upto[-1]).sum()) + 1
+    if s.min_p > 0:
+        n = min(n, max(1, int((w >= s.min_p).sum())))
+    g = torch.Generator().manual_seed((s.seed * 1000003 + s.draw) & 0x7FFFFFFF)
+    upto = w[:n].cumsum(0)
+    return int(idx[min(int((upto <= float(torch.rand((), generator=g, dtype=torch.float64)) * upto[-1]).sum()), n - 1)])
+
+
 class EagerPagedExecutor:
+    accepts_vocabulary_draws = True
     accepts_features = True          # segments may carry encoder feature rows and three-axis positions
     accepts_deepstack = True         # ... and additions after the first decoder layers
 

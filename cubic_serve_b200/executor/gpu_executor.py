@@ -55,6 +55,11 @@ class Segment:
     deep_embeds: object = None
     # offsets of this segment's tokens whose logits are wanted (``GpuExecutor.execute_logits``)
     logit_offsets: list = field(default_factory=list)
+    # draw from the whole vocabulary (``top_k`` is then any number, 0 = all) and keep the tokens with at least ``min_p`` of
+    # the best one's probability
+    whole: bool = False
+    min_p: float = 0.0
+    adapter: int = -1            # slot of the request's low-rank adapter, -1 = none
 
 
 class _Staging:
@@ -73,7 +78,10 @@ class _Staging:
             ("seg_pos0", np.int32, max_rows),
             # per sampled row: the request's slot and its thinking-budget command (device-side budget state machine)
             ("row_slot", np.int32, max_rows), ("budget_init", np.int32, max_rows),
+            # the sampled rows that draw from the whole vocabulary, and the min-p of every sampled row
+            ("whole_rows", np.int32, max_rows), ("min_p", np.float32, max_rows),
             ("page_table", np.int32, max_rows * max_pages),
+            ("row_adapter", np.int32, max_tokens),        # slot of every row's low-rank adapter, -1 = none
             # row- and column-axis rotary positions of multimodal prefill steps (``positions`` is the temporal axis)
             ("positions_h", np.int32, max_tokens), ("positions_w", np.int32, max_tokens),
         ]
@@ -120,7 +128,9 @@ def capturing(graph: "torch.cuda.CUDAGraph", stream: "torch.cuda.Stream"):
 class BatchBuilder:
     """Host side of a step: turns segments into the staged metadata arrays (no CUDA calls except the upload)."""
 
-    def __init__(self, max_rows: int, max_tokens: int, max_model_len: int, group: int, kv_heads: int, device) -> None:
+    def __init__(self, max_rows: int, max_tokens: int, max_model_len: int, group: int, kv_heads: int, device, adapters: bool = False) -> None:
+        """``adapters``: rows carry the slots of low-rank adapters (``Segment.adapter``)."""
+        self.adapters = adapters
         self.qb = 16 // group                                   # query positions per attention row block
         self.kv_heads = kv_heads
         self.max_rows = max_rows
@@ -247,6 +257,8 @@ class BatchBuilder:
             h["seg_count"][:n] = 1
             h["seg_slot"][:n] = h["rb_req"][:n]
             h["seg_pos0"][:n] = starts
+            if self.adapters:
+                h["row_adapter"][:n] = [s.adapter for s in segs]
             t = rb = nseg = n
             rows = 0
             decode = self.qb >= 2                                 # one position of at most eight heads per row block
@@ -278,6 +290,8 @@ class BatchBuilder:
                 n = len(s.token_ids)
                 h["seg_row0"][i], h["seg_count"][i], h["seg_slot"][i], h["seg_pos0"][i] = t, n, s.request_slot, s.start
                 h["token_ids"][t:t + n] = s.token_ids
+                if self.adapters:
+                    h["row_adapter"][t:t + n] = s.adapter
                 pos = np.arange(s.start, s.start + n, dtype=np.int32)
                 if s.positions3 is None:
                     h["positions"][t:t + n] = pos
@@ -312,6 +326,7 @@ class BatchBuilder:
             h["token_ids"][t:p] = 0
             h["positions"][t:p] = 0
             h["slots"][t:p] = -1
+            h["row_adapter"][t:p] = -1
             h["rb_req"][rb:p] = 0
             h["rb_qstart"][rb:p] = np.arange(rb, p, dtype=np.int32)
             h["rb_qcount"][rb:p] = 0
@@ -336,6 +351,7 @@ class BatchBuilder:
                          attn_decode=decode, attn_prompts=prompts,
                          segments=K.GdnSegments(d["seg_row0"], d["seg_count"], d["seg_slot"], d["seg_pos0"], nseg, max((len(s.token_ids) for s in segs), default=1)),
                          positions_hw=(d["positions_h"], d["positions_w"]) if axes else None,
+                         row_adapters=d["row_adapter"] if self.adapters else None,
                          embeds=[(first, feat.to(self.device, torch.bfloat16, non_blocking=True))
                                  for first, feat in embeds] or None), rows
 
@@ -349,6 +365,9 @@ class GpuExecutor:
         # executors and the tensor-parallel embedding path do not carry them)
         self.accepts_features = type(self) is GpuExecutor and runner.tp is None and getattr(runner, "pp", None) is None \
             and runner.cfg.mrope_section is not None
+        # draws from the whole vocabulary read a row's logits where one GPU has all of them; speculative rounds verify against
+        # the 20 best
+        self.accepts_vocabulary_draws = type(self) is GpuExecutor and runner.tp is None and getattr(runner, "pp", None) is None
         self.cfg = runner.cfg
         self.device = runner.device
         self.max_rows = max_rows
@@ -356,8 +375,10 @@ class GpuExecutor:
         assert self.max_tokens <= runner.max_tokens
         if runner.cfg.is_hybrid and max_rows > runner.max_requests:
             raise ValueError("the runner's recurrent state has fewer rows than the executor has request slots")
+        # the low-rank adapters that requests may name (speculative rounds compute and verify without)
+        self.low_rank = getattr(runner, "low_rank", None) if type(self) is GpuExecutor else None
         self.builder = BatchBuilder(max_rows * rows_per_request, self.max_tokens, max_model_len,
-                                    runner.hq // runner.hkv, runner.hkv, self.device)
+                                    runner.hq // runner.hkv, runner.hkv, self.device, adapters=self.low_rank is not None)
         self.stage = self.builder.stage
         self._fill = self.builder._fill
         self.invalidate_page_rows = self.builder.invalidate_page_rows
@@ -444,6 +465,18 @@ class GpuExecutor:
         self.h2d_mask_bytes_last = n * words * 4
         return True
 
+    def _stage_whole(self, segs: list[Segment]) -> int:
+        """Stage which sampled rows draw from the whole vocabulary; returns how many."""
+        rows = [(i, s.min_p) for i, s in enumerate(s for s in segs if s.sample) if s.whole and s.temperature > 0]
+        self.stage.d.pop("whole", None)
+        if rows:
+            h = self.stage.h
+            h["whole_rows"][:len(rows)] = [i for i, _ in rows]
+            for i, m in rows:
+                h["min_p"][i] = m
+            self.stage.d["whole"] = self.stage.d["whole_rows"][:len(rows)]
+        return len(rows)
+
     def capture_decode_graphs(self, capacities: list[int] | None = None) -> list[int]:
         """Capture one graph per decode row capacity (largest first, like the reference)."""
         caps = capacities or [c for c in (1, 2, 4, 8, 16, 32, 64, 128, 256, 512) if c <= self.max_rows]
@@ -452,6 +485,7 @@ class GpuExecutor:
         self._mask_buffers()
         self.graph_masks = True
         self.stage.d["mask"] = self._mask_dev
+        self.stage.d.pop("whole", None)
         rt = CudaGraphRuntime(resources=(0, 1))
         if isinstance(getattr(self.runner, "attn", None), torch.Tensor):
             with torch.cuda.stream(self.stream):
@@ -559,6 +593,17 @@ class GpuExecutor:
         for t in (src, dst):
             t.record_stream(self.stream)       # read there after this call has returned
 
+    def load_adapter(self, name: str, path):
+        """Load a low-rank adapter in stream order with the steps."""
+        with torch.cuda.stream(self.stream):
+            got = self.low_rank.load(name, path)
+        self.stream.synchronize()              # the host copies of its matrices may go
+        return got
+
+    def unload_adapter(self, name: str) -> None:
+        with torch.cuda.stream(self.stream):
+            self.low_rank.unload(name)
+
     def execute(self, segs: list[Segment]) -> np.ndarray:
         """Run one step and return the sampled token id of every sampling segment (host array)."""
         return self.collect(self.launch(segs))
@@ -611,13 +656,17 @@ class GpuExecutor:
         """
         total = sum(len(s.token_ids) for s in segs)
         masked = self._stage_masks(segs)
+        whole = any(s.whole for s in segs)
         decode = (all(len(s.token_ids) == 1 for s in segs) and self.use_graphs and (self.graph_masks or not masked))
+        # the budgets' state machine runs on the ids of the draw, inside the step
+        decode = decode and not (whole and self.runner.reasoning is not None)
         cap = self.graph_rt.dispatch(total) if decode else None
         if self._upload_pending:
             # the pinned staging buffer is rewritten below: the previous launch's upload must have left it
             self._uploaded.synchronize()
             self._upload_pending = False
         b, rows = self._fill(segs, pad_rows_to=cap)
+        whole = self._stage_whole(segs) if whole or "whole" in self.stage.d else 0
         if cap is not None and getattr(self, "audit_poison_padding", False):
             self._poison_padding(total, cap)
         k = self._launches & 1
@@ -634,6 +683,9 @@ class GpuExecutor:
                 self._ev[k][0].record(self.stream)
             if cap is not None:
                 launches = self.graph_rt.replay(cap, self._leases[k]).launches
+                if whole:                      # behind the graph, whose sampler drew these rows from the 20 best
+                    self.runner.draw_whole(self.stage.d, self.logits, self.out_ids, rows)
+                    launches += 1
             else:
                 self._body(b)
                 launches = self.runner.launches_per_step

@@ -41,6 +41,7 @@ class StatefulEagerExecutor:
         if speculative_depth and not getattr(model, "has_draft_head", False):
             raise ValueError("speculative rounds need the checkpoint's draft head (mtp.* tensors)")
         self.speculative_depth = int(speculative_depth)
+        self.accepts_vocabulary_draws = not self.speculative_depth
         self._slots: dict[int, RequestSlot] = {}
         self.last_round: dict | None = None
         self.h2d_bytes_last = self.d2h_bytes_last = self.kernel_launches_last = 0

@@ -26,7 +26,8 @@ from pathlib import Path
 
 from ..runtime.scheduler import SamplingParams
 
-_SAMPLING_FIELDS = ("temperature", "top_p", "top_k", "seed", "max_tokens", "stop_token_ids", "ignore_eos", "thinking_budget")
+_SAMPLING_FIELDS = ("temperature", "top_p", "top_k", "seed", "max_tokens", "stop_token_ids", "ignore_eos", "thinking_budget",
+                    "whole_vocabulary", "min_p", "adapter")
 
 
 @dataclass

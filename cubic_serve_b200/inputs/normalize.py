@@ -199,6 +199,7 @@ def normalize_openai_chat_completions(body: Any, default_model: str | None = Non
     _require(not so or stream, "stream_options requires stream = true", "stream_options")
     seed = body.get("seed")
     _require(seed is None or (isinstance(seed, int) and not isinstance(seed, bool)), "seed must be an integer", "seed")
+    _require(isinstance(body.get("whole_vocabulary", False), bool), "whole_vocabulary must be true or false", "whole_vocabulary")
     tlp = body.get("top_logprobs") or 0
     _require(isinstance(tlp, int) and 0 <= tlp <= 20, "top_logprobs must be in [0, 20]", "top_logprobs")
     sampling = SamplingMeta(
@@ -209,7 +210,8 @@ def normalize_openai_chat_completions(body: Any, default_model: str | None = Non
         stop_token_ids=tuple(int(t) for t in (body.get("stop_token_ids") or [])),
         presence_penalty=float(_as_number(body, "presence_penalty", 0.0, -2.0, 2.0)),
         frequency_penalty=float(_as_number(body, "frequency_penalty", 0.0, -2.0, 2.0)),
-        logprobs=bool(body.get("logprobs", False)), top_logprobs=tlp)
+        logprobs=bool(body.get("logprobs", False)), top_logprobs=tlp,
+        whole_vocabulary=body.get("whole_vocabulary", False), min_p=float(_as_number(body, "min_p", 0.0)))
     tools, choice = _openai_tools(body)
     structured = _openai_structured(body)
     _require(not (structured.kind != StructuredKind.NONE and choice.mode in ("required", "named")),

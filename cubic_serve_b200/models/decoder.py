@@ -274,16 +274,18 @@ class StepBatch:
     # the temporal axis) and encoder feature rows ``[(first row, bf16 [n, H])]`` that replace token embeddings
     positions_hw: tuple | None = None
     embeds: list | None = None
+    row_adapters: torch.Tensor | None = None     # int32 [T] adapter slot of every row, -1 = none (decoders with low-rank adapters)
 
 
 class DecoderRunner(StepRunner):
     def __init__(self, cfg: ModelConfig, weights: DecoderWeights, num_pages: int, max_tokens: int,
                  k_bits: int = 8, v_bits: int = 8, tp=None, device=None, pp=None, max_requests: int = 256,
                  state_checkpoints: int = 0,
-                 kv_rotation: bool = False) -> None:
+                 kv_rotation: bool = False, low_rank: tuple[int, int] | None = None) -> None:
         """``max_requests``: rows of the per-request recurrent state of Gated DeltaNet layers (= page-table rows).
         ``kv_rotation``: q / k / v head vectors are Walsh-Hadamard transformed before the cache write (smoother
-        channels for INT4 / INT6 codes); the attention output is transformed back."""
+        channels for INT4 / INT6 codes); the attention output is transformed back.
+        ``low_rank``: (slots, largest rank) of the low-rank adapters that requests may name (``models/low_rank.py``; one GPU)."""
         self.cfg = cfg
         self.w = weights            # ``weights.layers`` holds only the layers of this pipeline stage
         self.device = device or weights.embed.device
@@ -354,12 +356,18 @@ class DecoderRunner(StepRunner):
         self.ws = K.workspace(dev)
         self.launches_per_step = 0
         from ..ops.strategies import active
+        self.low_rank = None
+        if low_rank is not None:
+            if tp is not None or pp is not None:
+                raise ValueError("low-rank adapters are served on one GPU")
+            from .low_rank import LowRankAdapters
+            self.low_rank = LowRankAdapters(cfg, weights.layers, *low_rank, max_tokens, dev)
         if active().gemm.fuse_swiglu and torch.device(dev).type == "cuda":
             # gate / up rows interleaved once, so that the GEMM epilogue applies the activation (no [T, 2I] round trip)
             for lw in weights.layers:
                 if lw.moe is not None:
                     lw.moe.fuse_activation()
-                elif lw.gate_up is not None and (lw.gate_up.n // 2) % 16 == 0:
+                elif low_rank is None and lw.gate_up is not None and (lw.gate_up.n // 2) % 16 == 0:
                     lw.gate_up = wq_pack.swiglu_interleave(lw.gate_up)
         self.ep = None
         if cfg.is_moe and tp is not None and tp.fused is not None:
@@ -507,13 +515,17 @@ class DecoderRunner(StepRunner):
                 lo, hi = max(first, t0), min(first + rows.shape[0], t1)
                 if lo < hi:
                     h[lo - t0:hi - t0].copy_(rows[lo - first:hi - first])
+        ad = self.low_rank if b.row_adapters is not None else None
+        if ad is not None:
+            ad.begin(b.row_adapters[:T])
+            n += 1
         pending = None  # partial sum waiting to be folded into h by the next norm (TP > 1)
         fp8s = (wq_pack.FMT_FP8, wq_pack.FMT_FP8_BLOCK)
 
         def norm(src, weight, residual, consumers):
             """RMSNorm into ``x``; when every consumer of the result is an fp8 GEMM the norm kernel quantizes its own
             output per token and the e4m3 operand is returned instead (no bf16 round trip, no extra launch)."""
-            if consumers and all(c is not None and c.fmt in fp8s for c in consumers):
+            if ad is None and consumers and all(c is not None and c.fmt in fp8s for c in consumers):
                 return K.rmsnorm_fp8(src, weight, cfg.rms_eps, residual=residual, zero_centered=cfg.zero_centered_norm,
                                      ws=self.ws)
             return K.rmsnorm(src, weight, cfg.rms_eps, out=x, residual=residual, zero_centered=cfg.zero_centered_norm)
@@ -534,6 +546,8 @@ class DecoderRunner(StepRunner):
                 n += 5
             else:
                 K.wq_gemm(xin, lw.qkv, out=qkv, ws=self.ws)
+                if ad is not None:
+                    n += ad.add(li, "qkv", xin, qkv)
                 hw = None if b.positions_hw is None else (b.positions_hw[0][t0:t1], b.positions_hw[1][t0:t1])
                 K.rope_kv_write(qkv, q, self.kv[li], b.positions[t0:t1], b.slots[t0:t1], self.inv_freq, self.hq, self.hkv,
                                 self.D, self.k_bits, self.v_bits, q_norm=lw.q_norm, k_norm=lw.k_norm, eps=cfg.rms_eps,
@@ -552,6 +566,8 @@ class DecoderRunner(StepRunner):
             ffn_in = [] if lw.moe is not None else [lw.gate_up]
             if self.tp is None:
                 K.wq_gemm(mixed, o_w, out=h, residual=h, ws=self.ws)
+                if ad is not None and lw.gdn is None:
+                    n += ad.add(li, "o", mixed, h)
                 xin = norm(h, lw.ln2, None, ffn_in)
             else:
                 part = self.part[t0:t1]
@@ -572,9 +588,16 @@ class DecoderRunner(StepRunner):
                     pending = out
             else:
                 gu, act = self.gu[t0:t1], self.act[t0:t1]
-                n += 1 + K.gate_up_act(xin, lw.gate_up, gu, act, ws=self.ws)
+                if ad is None:
+                    n += 1 + K.gate_up_act(xin, lw.gate_up, gu, act, ws=self.ws)
+                else:
+                    K.wq_gemm(xin, lw.gate_up, out=gu, ws=self.ws)
+                    n += 3 + ad.add(li, "gate_up", xin, gu)
+                    K.swiglu(gu, out=act)
                 if self.tp is None:
                     K.wq_gemm(act, lw.down, out=h, residual=h, ws=self.ws)
+                    if ad is not None:
+                        n += ad.add(li, "down", act, h)
                 else:
                     part = self.part[t0:t1]
                     K.wq_gemm(row_in(act, lw.down), lw.down, out=part, ws=self.ws)

@@ -20,6 +20,8 @@ Optional capabilities (attribute -> meaning):
 * ``invalidate_page_rows(slots)``: a cached device page table exists and must forget these request slots;
 * ``accepts_features``: segments may carry encoder feature rows and three-axis positions;
 * ``keeps_request_state``: the executor holds a request's context itself (no pages): the engine keeps prefix sharing off;
+* ``accepts_vocabulary_draws``: segments may draw from the whole vocabulary (``Segment.whole``, any ``top_k``, ``min_p``);
+* ``low_rank`` + ``load_adapter(name, directory) / unload_adapter(name)``: segments may name a low-rank adapter's slot;
 * ``reasoning_end_id``: thinking budgets are enforced by the executor.
 
 Reference counterpart: ``models/protocol.py:28-251`` there (``ModelSegment``, ``ModelStepResult``, the semantic-op

@@ -40,9 +40,18 @@ class StepRunner:
         """Whole step: layers, final norm, lm_head, sampling (and the cross-rank token agreement under TP), then the
         thinking-budget state machine on the sampled ids when it is enabled."""
         self._run_step(b, d, logits_buf, out_ids)
+        if d.get("whole") is not None and b.num_logit_rows:
+            self.draw_whole(d, logits_buf, out_ids, b.num_logit_rows)
+            self.launches_per_step += 1
         if self.reasoning is not None and b.num_logit_rows:
             self.reasoning.apply(out_ids, d["row_slot"], d["budget_init"], b.num_logit_rows)
             self.launches_per_step += 1
+
+    def draw_whole(self, d: dict, logits_buf: torch.Tensor, out_ids: torch.Tensor, rows: int) -> None:
+        """Draw the rows ``d["whole"]`` again, from the whole vocabulary, by the stream that the sampler drew them with."""
+        mask = d.get("mask")
+        K.sample_vocabulary(logits_buf[:rows], out_ids, d["temperature"], d["top_k"], d["top_p"], d["min_p"], seeds=d["seeds"], counters=d["draws"],
+                            mask=None if mask is None else mask[:rows], rows=d["whole"])
 
     def _run_step(self, b, d: dict, logits_buf: torch.Tensor, out_ids: torch.Tensor) -> None:
         R = b.num_logit_rows

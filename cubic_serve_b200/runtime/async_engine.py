@@ -96,6 +96,11 @@ class TokenChatBackend:
         self._thread.start()
         self.stats = {"requests": 0, "tokens": 0, "started": time.time()}
 
+    @property
+    def adapter_names(self) -> tuple[str, ...]:
+        """Low-rank adapters that a request may name as its model."""
+        return tuple(getattr(self.engine, "adapter_names", ()))
+
     # ------------------------------------------------------------ front side
     def start(self, req: CanonicalChatRequest):
         if self.engine.poisoned or not self.ready:
@@ -137,7 +142,7 @@ class TokenChatBackend:
                     matcher = DelayedMatcher(matcher, end)
         sp = SamplingParams(temperature=s.temperature, top_p=s.top_p, top_k=s.top_k, seed=s.seed, max_tokens=max_tokens,
                             stop_token_ids=tuple(s.stop_token_ids) + ((eos,) if eos is not None else ()),
-                            matcher=matcher,
+                            matcher=matcher, adapter=req.model if req.model in self.adapter_names else None, whole_vocabulary=s.whole_vocabulary, min_p=s.min_p,
                             thinking_budget=req.reasoning.budget_tokens if prepared.starts_in_reasoning else None)
         with self._lock:
             self._live[req.request_id] = live

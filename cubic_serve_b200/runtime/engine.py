@@ -90,15 +90,47 @@ class LLMEngine:
                 raise AdmissionError("this executor does not consume the vision tower's intermediate outputs", status=400)
             if multimodal.prompt_length != len(prompt_token_ids):
                 raise AdmissionError("the media positions do not cover the prompt", status=400)
+        if sampling is not None and sampling.draws_whole and not getattr(self.executor, "accepts_vocabulary_draws", False):
+            raise AdmissionError("this executor draws from the 20 best tokens only; whole_vocabulary and min_p are not accepted", status=400)
         rid = request_id or f"req-{next(self._ids)}"
         if rid in self.requests:
             raise AdmissionError(f"duplicate request id {rid}")
         if len(self.scheduler.waiting) + len(self.scheduler.running) >= 4 * self.cfg.max_running_requests:
             raise AdmissionError("too many queued requests", status=429)
         req = Request(rid, list(prompt_token_ids), sampling or SamplingParams(), multimodal=multimodal)
+        if req.sampling.adapter is not None:
+            known = self._adapters().loaded.get(req.sampling.adapter)
+            if known is None:
+                raise AdmissionError(f"no adapter named {req.sampling.adapter!r} is loaded", status=404)
+            req.adapter_slot, req.adapter_key = known.slot, known.key
         self.scheduler.add(req)
         self.requests[rid] = req
         return rid
+
+    def _adapters(self):
+        low_rank = getattr(self.executor, "low_rank", None)
+        if low_rank is None:
+            raise AdmissionError("this executor serves no low-rank adapters", status=400)
+        return low_rank
+
+    @property
+    def adapter_names(self) -> tuple[str, ...]:
+        """The low-rank adapters that requests may name."""
+        low_rank = getattr(self.executor, "low_rank", None)
+        return () if low_rank is None else tuple(low_rank.loaded)
+
+    def load_adapter(self, name: str, path) -> None:
+        """Make the low-rank adapter of a directory available under ``name``; call it between steps."""
+        self._adapters()
+        self.executor.load_adapter(name, path)
+
+    def unload_adapter(self, name: str) -> None:
+        """Free an adapter's slot; refused while a request names it."""
+        self._adapters()
+        if any(r.sampling.adapter == name for r in self.requests.values()) or self._ahead is not None and any(
+                s.request.sampling.adapter == name for s in self._ahead[0].segments):
+            raise AdmissionError(f"requests still use the adapter {name!r}", status=409)
+        self.executor.unload_adapter(name)
 
     def abort(self, request_id: str) -> bool:
         r = self.scheduler.abort(request_id)
@@ -192,6 +224,9 @@ class LLMEngine:
                                 sp.seed if sp.seed is not None else hash(r.request_id) & 0x7FFFFFFF,
                                 r.draws + (1 if ahead else 0), (r.arrival << 16) | (r.preemptions & 0xFFFF), mask,
                                 self._budget_init(r) if s.sample and end_id is not None else -2, mask_fn))
+            segs[-1].adapter = r.adapter_slot
+            if sp.draws_whole:
+                segs[-1].whole, segs[-1].min_p = True, sp.min_p
             if r.multimodal is not None:
                 segs[-1].embeds, segs[-1].positions3 = r.multimodal.segment_inputs(s.start, s.count)
                 if getattr(r.multimodal, "deep_layers", 0):

@@ -47,14 +47,26 @@ class SamplingParams:
     # thinking-token budget of a request that starts inside a reasoning block: after this many tokens the executor
     # forces the end of the block (enforced on the device, see ``csrc/sampling.cu``); None = unlimited
     thinking_budget: int | None = None
+    # draw from the whole vocabulary instead of the 20 best tokens: ``top_k`` is then any number (0 = all); ``min_p``: only
+    # tokens with at least this share of the best one's probability (above 0 it implies the whole vocabulary)
+    whole_vocabulary: bool = False
+    min_p: float = 0.0
+    # the low-rank adapter that the request's tokens are computed with (``models/low_rank.py``); None = the model alone
+    adapter: str | None = None
+
+    @property
+    def draws_whole(self) -> bool:
+        return self.temperature > 0 and (self.whole_vocabulary or self.min_p > 0)
 
     def validate(self) -> None:
         if not 0.0 <= self.temperature <= 2.0:
             raise ValueError("temperature must be in [0, 2]")
         if not 0.0 < self.top_p <= 1.0:
             raise ValueError("top_p must be in (0, 1]")
-        if not 0 <= self.top_k <= 20:
-            raise ValueError("top_k must be in [0, 20]")
+        if not 0.0 <= self.min_p <= 1.0:
+            raise ValueError("min_p must be in [0, 1]")
+        if not 0 <= self.top_k <= (2 ** 31 - 1 if self.whole_vocabulary or self.min_p > 0 else 20):
+            raise ValueError("top_k must be in [0, 20], or any number with whole_vocabulary")
         if self.max_tokens < 1:
             raise ValueError("max_tokens must be >= 1")
         if self.thinking_budget is not None and self.thinking_budget < 0:
@@ -82,6 +94,9 @@ class Request:
     # multimodal prompt (``runtime/multimodal.py::MultimodalInput``): encoder feature rows that replace the embedding
     # of placeholder tokens, three-axis positions, and per-row content keys for the prefix cache
     multimodal: object | None = None
+    # slot and cache key of the request's low-rank adapter (``SamplingParams.adapter``), resolved at admission
+    adapter_slot: int = -1
+    adapter_key: bytes = b""
 
     def __post_init__(self) -> None:
         if not self.tokens:
@@ -232,7 +247,7 @@ class ContinuousScheduler:
         if not self._free_slots:
             return False
         # restore the longest cached prefix, always leaving >= 1 prompt token to compute
-        pages = self.prefix.match(_keys(req, req.prompt), max_tokens=len(req.prompt) - 1) if not req.pages else []
+        pages = self.prefix.match(_keys(req, req.prompt), req.adapter_key, max_tokens=len(req.prompt) - 1) if not req.pages else []
         if pages:
             req.pages = list(pages)
             req.num_computed = len(pages) * BLOCK
@@ -422,11 +437,11 @@ class ContinuousScheduler:
             r.num_computed += seg.count
             full = r.num_computed // BLOCK
             if full > r.num_published and self.prefix.enabled:
-                self.prefix.publish(_keys(r, r.tokens[:full * BLOCK]), r.pages[:full])
+                self.prefix.publish(_keys(r, r.tokens[:full * BLOCK]), r.pages[:full], r.adapter_key)
                 r.num_published = full
                 if self.prefix.needs_checkpoint and r.num_computed == full * BLOCK and not seg.sample:
                     # the step ended on a page boundary inside the prompt: its recurrent state is a valid snapshot
-                    slot = self.prefix.publish_checkpoint(_keys(r, r.tokens[:full * BLOCK]))
+                    slot = self.prefix.publish_checkpoint(_keys(r, r.tokens[:full * BLOCK]), r.adapter_key)
                     if slot is not None:
                         self.state_saves.append((r.slot, slot))
             if seg.sample:

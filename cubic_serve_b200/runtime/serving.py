@@ -79,6 +79,8 @@ def build_backend(args, devices: list[int], tp: int, spec, k_bits: int, v_bits: 
     if tp != 1 or args.pp_size != 1:
         if _is_layered(args.model):
             raise SystemExit("layered decoders are served on one GPU")
+        if _low_rank_adapters(args) is not None:
+            raise SystemExit("low-rank adapters are served on one GPU")
         from ..executor.multiproc import build_multiproc_backend
         for flag in ("startup_numerical_audit", "tune_launch_plans"):
             if getattr(args, flag, False):
@@ -94,6 +96,9 @@ def build_backend(args, devices: list[int], tp: int, spec, k_bits: int, v_bits: 
         raise SystemExit("--dtype float32 is available for the layered decoders; use --execution-mode eager for fp32 arithmetic "
                          "of the other families")
     eager = args.execution_mode != "cuda" or not torch.cuda.is_available()
+    adapters = _low_rank_adapters(args)
+    if adapters is not None and (eager or layered or spec is not None and getattr(spec, "method", "none") != "none"):
+        raise SystemExit("low-rank adapters are served by the native decoder runner, without --speculative-config")
     gguf_weights = None
     if model.startswith("random:"):
         cfg = NAMED_CONFIGS[model.split(":", 1)[1]]()
@@ -177,7 +182,8 @@ def build_backend(args, devices: list[int], tp: int, spec, k_bits: int, v_bits: 
                               args.max_running_requests, state_snapshots=snapshots)
         runner = defn.build_runner(cfg, weights, num_pages=pages, max_tokens=args.token_budget, k_bits=k_bits, v_bits=v_bits,
                                    max_requests=args.max_running_requests, state_checkpoints=snapshots,
-                                   kv_rotation=bool(getattr(args, "enable_kv_cache_rotation", False)))
+                                   kv_rotation=bool(getattr(args, "enable_kv_cache_rotation", False)),
+                                   **({} if adapters is None else {"low_rank": adapters[0]}))
         depth = getattr(spec, "num_speculative_tokens", 0) if spec is not None else 0
         if depth and getattr(spec, "method", "mtp") == "ngram":
             # prompt-lookup drafts: no draft model; steps without a draft replay the decode graphs
@@ -220,6 +226,9 @@ def build_backend(args, devices: list[int], tp: int, spec, k_bits: int, v_bits: 
                 rows = [c for c in (1, 2, 4, 8, 16, 32, 64, 128, 256, 512) if c <= args.max_running_requests]
                 n = autotune.install(autotune.prepare(cfg, rows, dev, prep))
                 log.info("launch plans: %d measured entries replace the rules (%s)", n, "cached" if prep.hits else "measured now")
+            for name, path in (adapters[1] if adapters is not None else ()):
+                got = executor.load_adapter(name, path)
+                log.info("low-rank adapter %s in slot %d", name, got.slot)
             caps = executor.capture_decode_graphs()
             log.info("captured decode graphs for capacities %s; %d KV pages", caps, pages)
     tok = _tokenizer_for(model, cfg.vocab_size)
@@ -234,6 +243,22 @@ def build_backend(args, devices: list[int], tp: int, spec, k_bits: int, v_bits: 
         processor = build_media_processor(args, ck, tok, executor, max_len)
     backend = TokenChatBackend(engine, tok, default_thinking=args.thinking, processor=processor)
     return backend, (_first_name(args.served_model_name) or cfg.name)
+
+
+def _low_rank_adapters(args):
+    """``((slots, largest rank), [(name, directory)])`` of ``--low-rank-*``, None without any."""
+    given = []
+    for item in getattr(args, "low_rank_adapter", None) or ():
+        name, eq, path = item.partition("=")
+        if not (name and eq and path) or name in dict(given):
+            raise SystemExit(f"--low-rank-adapter wants NAME=DIR with names of their own, got {item!r}")
+        given.append((name, path))
+    slots = getattr(args, "low_rank_slots", None) or len(given)
+    if not slots:
+        return None
+    if slots < len(given):
+        raise SystemExit(f"{len(given)} low-rank adapters do not fit {slots} slots")
+    return (slots, args.low_rank_max_rank), given
 
 
 def _first_name(names):
