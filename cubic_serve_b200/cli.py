@@ -183,6 +183,9 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--token-budget", type=int, default=8192)
     g.add_argument("--cuda-graph-max-tokens", default="auto")
     g.add_argument("--prefill-chunk-tokens", type=int, default=4096)
+    g.add_argument("--device-layout", action="store_true",
+                   help="make positions, cache slots and the block table of a step on the GPU from the lengths of its requests; only "
+                        "those and the new pages are uploaded (one GPU, without --speculative-config)")
     g = s.add_argument_group("Multimodal input")
     g.add_argument("--encoder-memory-gib", "--multimodal-memory-gib", dest="encoder_memory_gib", type=float, default=2.0,
                    help="transient memory one call of the vision tower may use; larger items are cut at frame boundaries "

@@ -68,9 +68,7 @@ class _Staging:
     def __init__(self, max_tokens: int, max_rows: int, max_row_blocks: int, max_pages: int, device) -> None:
         self.max_tokens, self.max_rows, self.max_row_blocks, self.max_pages = max_tokens, max_rows, max_row_blocks, max_pages
         fields = [
-            ("token_ids", np.int32, max_tokens), ("positions", np.int32, max_tokens), ("slots", np.int32, max_tokens),
-            ("rb_req", np.int32, max_row_blocks), ("rb_qstart", np.int32, max_row_blocks),
-            ("rb_qcount", np.int32, max_row_blocks), ("rb_ctx", np.int32, max_row_blocks),
+            ("token_ids", np.int32, max_tokens),
             ("top_k", np.int32, max_rows), ("temperature", np.float32, max_rows), ("top_p", np.float32, max_rows),
             ("logit_rows", np.int64, max_rows), ("seeds", np.int64, max_rows), ("draws", np.int64, max_rows),
             # the step's rows grouped by request (recurrent layers walk a request's rows in order)
@@ -80,8 +78,14 @@ class _Staging:
             ("row_slot", np.int32, max_rows), ("budget_init", np.int32, max_rows),
             # the sampled rows that draw from the whole vocabulary, and the min-p of every sampled row
             ("whole_rows", np.int32, max_rows), ("min_p", np.float32, max_rows),
-            ("page_table", np.int32, max_rows * max_pages),
             ("row_adapter", np.int32, max_tokens),        # slot of every row's low-rank adapter, -1 = none
+            # what a layout on the device is made from besides: pages that a request's row holds, pages that rows are given.  A step
+            # laid out there uploads up to the last page given, what follows is written by ``K.step_layout``
+            ("held", np.int32, max_rows), ("new_pages", np.int32, max_rows * max_pages),
+            ("positions", np.int32, max_tokens), ("slots", np.int32, max_tokens),
+            ("rb_req", np.int32, max_row_blocks), ("rb_qstart", np.int32, max_row_blocks),
+            ("rb_qcount", np.int32, max_row_blocks), ("rb_ctx", np.int32, max_row_blocks),
+            ("page_table", np.int32, max_rows * max_pages),
             # row- and column-axis rotary positions of multimodal prefill steps (``positions`` is the temporal axis)
             ("positions_h", np.int32, max_tokens), ("positions_w", np.int32, max_tokens),
         ]
@@ -140,6 +144,7 @@ class BatchBuilder:
         self.stage = _Staging(max_tokens, max_rows, max_rb, self.max_pages, device)
         self.device = device
         self._page_rows: list[tuple[int, int]] = [(-2, 0)] * max_rows
+        self._device_rows: list[tuple[int, int]] = [(-2, 0)] * max_rows      # the same of the device's table, in steps laid out there
 
     def _splits(self, row_blocks: int, decode: bool = False) -> int:
         """KV splits of a step.  Four CTAs of the decode form run on an SM where the general kernel has two, so from one
@@ -226,7 +231,23 @@ class BatchBuilder:
     def invalidate_page_rows(self, slots) -> None:
         """Force a full rewrite of these page-table rows (used after copy-on-write replaced a page)."""
         for slot in slots:
-            self._page_rows[slot] = (-2, 0)
+            self._page_rows[slot] = self._device_rows[slot] = (-2, 0)
+
+    def stage_layout(self, segs: list[Segment]) -> tuple[int, int]:
+        """Stage what ``K.step_layout`` needs of a filled step besides its segments: the pages that the device's rows hold and those
+        that they are given.  Returns (pages given, bytes to upload)."""
+        h, given = self.stage.h, 0
+        for i, s in enumerate(segs):
+            uid, held = self._device_rows[s.request_slot]
+            need = -(-(s.start + len(s.token_ids)) // K.PAGE_TOKENS)
+            if uid != s.uid or s.uid < 0 or len(s.pages) < held:
+                held = 0
+            h["held"][i] = held
+            if need > held:
+                h["new_pages"][given:given + need - held] = s.pages[held:need]
+                given += need - held
+            self._device_rows[s.request_slot] = (s.uid, max(held, need))
+        return given, self.stage.offsets["new_pages"][0] + 4 * given
 
     def _fill(self, segs: list[Segment], pad_rows_to: int | None = None, review: bool = False) -> StepBatch:
         """``review``: the segments are drafts to be verified.  Their pass is captured once for a number of requests and replayed behind
@@ -358,8 +379,11 @@ class BatchBuilder:
 
 class GpuExecutor:
     def __init__(self, runner: DecoderRunner, max_rows: int = 256, max_prefill_tokens: int = 8192,
-                 max_model_len: int = 4096, use_graphs: bool = True, rows_per_request: int = 1) -> None:
-        """``rows_per_request`` > 1 sizes the sampled-row staging for speculative review (K + 1 rows per request)."""
+                 max_model_len: int = 4096, use_graphs: bool = True, rows_per_request: int = 1, device_layout: bool = False) -> None:
+        """``rows_per_request`` > 1 sizes the sampled-row staging for speculative review (K + 1 rows per request).
+        ``device_layout``: positions, cache slots, row blocks and the block table of a step are made on the GPU from the lengths of its
+        requests (``K.step_layout``) and only the lengths, the new pages and the sampling parameters are uploaded; steps with media
+        positions and speculative rounds keep the host's."""
         self.runner = runner
         # encoder feature rows and three-axis positions are taken on one GPU by the plain executor (the speculative
         # executors and the tensor-parallel embedding path do not carry them)
@@ -382,6 +406,11 @@ class GpuExecutor:
         self.stage = self.builder.stage
         self._fill = self.builder._fill
         self.invalidate_page_rows = self.builder.invalidate_page_rows
+        self.layout = None
+        if device_layout and type(self) is GpuExecutor:
+            st = self.stage
+            self.layout = K.StepLayout(st.max_tokens, st.max_rows, st.max_row_blocks, self.device, into={
+                **{name: st.d[name] for name in ("positions", "slots", "rb_req", "rb_qstart", "rb_qcount", "rb_ctx")}, "row0": st.d["seg_row0"]})
         v_local = runner.w.lm_head.n
         self.logits = torch.empty(max_rows, v_local, dtype=getattr(runner, "logits_dtype", torch.bfloat16), device=self.device)
         self.out_ids = torch.zeros(max_rows * rows_per_request, dtype=torch.int32, device=self.device)
@@ -667,6 +696,8 @@ class GpuExecutor:
             self._upload_pending = False
         b, rows = self._fill(segs, pad_rows_to=cap)
         whole = self._stage_whole(segs) if whole or "whole" in self.stage.d else 0
+        laid_out = self.layout is not None and all(s.positions3 is None for s in segs)
+        given, upload = self.builder.stage_layout(segs) if laid_out else (0, None)
         if cap is not None and getattr(self, "audit_poison_padding", False):
             self._poison_padding(total, cap)
         k = self._launches & 1
@@ -674,9 +705,13 @@ class GpuExecutor:
         self._leases[k] = self.graph_rt.leases.acquire(k, f"launch {self._launches}")
         self._launches += 1
         with torch.cuda.stream(self.stream):
-            h2d = self.stage.upload()
+            h2d = self.stage.upload(upload)
             self._uploaded.record(self.stream)
             self._upload_pending = True
+            if laid_out:
+                d, n = self.stage.d, len(segs)
+                K.step_layout(d["seg_slot"][:n], d["seg_pos0"][:n], d["seg_count"][:n], d["held"][:n], d["new_pages"][:given], d["page_table"], self.layout,
+                              self.builder.qb, tokens=total, blocks=sum(-(-len(s.token_ids) // self.builder.qb) for s in segs), pad=cap or 0)
             if feedback_rows:
                 self.stage.d["token_ids"][:feedback_rows].copy_(self.out_ids[:feedback_rows], non_blocking=True)
             if self.timing:

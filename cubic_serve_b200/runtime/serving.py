@@ -213,7 +213,7 @@ def build_backend(args, devices: list[int], tp: int, spec, k_bits: int, v_bits: 
             if think is not None:
                 runner.enable_reasoning_budget(*think)       # thinking-token budgets are enforced on the device
             executor = GpuExecutor(runner, max_rows=args.max_running_requests, max_prefill_tokens=args.token_budget,
-                                   max_model_len=max_len)
+                                   max_model_len=max_len, device_layout=bool(getattr(args, "device_layout", False)))
             if getattr(args, "tune_launch_plans", False) and layered:
                 log.warning("--tune-launch-plans measures the quantized projections; layered decoders use the built-in rules")
             elif getattr(args, "tune_launch_plans", False):
