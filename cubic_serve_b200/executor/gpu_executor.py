@@ -65,7 +65,7 @@ class Segment:
 class _Staging:
     """Typed views over one pinned host buffer and its device mirror."""
 
-    def __init__(self, max_tokens: int, max_rows: int, max_row_blocks: int, max_pages: int, device) -> None:
+    def __init__(self, max_tokens: int, max_rows: int, max_row_blocks: int, max_pages: int, device, adapters: bool = False) -> None:
         self.max_tokens, self.max_rows, self.max_row_blocks, self.max_pages = max_tokens, max_rows, max_row_blocks, max_pages
         fields = [
             ("token_ids", np.int32, max_tokens),
@@ -78,10 +78,8 @@ class _Staging:
             ("row_slot", np.int32, max_rows), ("budget_init", np.int32, max_rows),
             # the sampled rows that draw from the whole vocabulary, and the min-p of every sampled row
             ("whole_rows", np.int32, max_rows), ("min_p", np.float32, max_rows),
-            ("row_adapter", np.int32, max_tokens),        # slot of every row's low-rank adapter, -1 = none
-            # what a layout on the device is made from besides: pages that a request's row holds, pages that rows are given.  A step
-            # laid out there uploads up to the last page given, what follows is written by ``K.step_layout``
-            ("held", np.int32, max_rows), ("new_pages", np.int32, max_rows * max_pages),
+            *([("row_adapter", np.int32, max_tokens)] if adapters else []),     # slot of every row's low-rank adapter, -1 = none
+            # from here on a layout on the device (``K.step_layout``) writes: such a step uploads what is before
             ("positions", np.int32, max_tokens), ("slots", np.int32, max_tokens),
             ("rb_req", np.int32, max_row_blocks), ("rb_qstart", np.int32, max_row_blocks),
             ("rb_qcount", np.int32, max_row_blocks), ("rb_ctx", np.int32, max_row_blocks),
@@ -108,6 +106,11 @@ class _Staging:
             self.d[name] = self.dev[o:o + size].view(tmap[dt])
         self.d["page_table"] = self.d["page_table"].view(max_rows, max_pages)
         self.h["page_table"] = self.h["page_table"].reshape(max_rows, max_pages)
+
+    @property
+    def lengths_bytes(self) -> int:
+        """What a step that is laid out on the device uploads of this buffer."""
+        return self.offsets["positions"][0]
 
     def upload(self, nbytes: int | None = None) -> int:
         n = self.nbytes if nbytes is None else nbytes
@@ -141,10 +144,12 @@ class BatchBuilder:
         self.max_tokens = max_tokens
         self.max_pages = -(-max_model_len // K.PAGE_TOKENS)
         max_rb = max(max_rows, max_tokens // self.qb + max_rows)
-        self.stage = _Staging(max_tokens, max_rows, max_rb, self.max_pages, device)
+        self.stage = _Staging(max_tokens, max_rows, max_rb, self.max_pages, device, adapters)
         self.device = device
         self._page_rows: list[tuple[int, int]] = [(-2, 0)] * max_rows
-        self._device_rows: list[tuple[int, int]] = [(-2, 0)] * max_rows      # the same of the device's table, in steps laid out there
+        # steps that are laid out on the device: whose pages its table holds, and how many; what it is given, as [pages held | new pages]
+        self._device_uid, self._device_held = np.full(max_rows, -2, dtype=np.int64), np.zeros(max_rows, dtype=np.int32)
+        self.given_host = self.given = None
 
     def _splits(self, row_blocks: int, decode: bool = False) -> int:
         """KV splits of a step.  Four CTAs of the decode form run on an SM where the general kernel has two, so from one
@@ -231,52 +236,68 @@ class BatchBuilder:
     def invalidate_page_rows(self, slots) -> None:
         """Force a full rewrite of these page-table rows (used after copy-on-write replaced a page)."""
         for slot in slots:
-            self._page_rows[slot] = self._device_rows[slot] = (-2, 0)
+            self._page_rows[slot] = (-2, 0)
+            self._device_uid[slot] = -2
 
-    def stage_layout(self, segs: list[Segment]) -> tuple[int, int]:
-        """Stage what ``K.step_layout`` needs of a filled step besides its segments: the pages that the device's rows hold and those
-        that they are given.  Returns (pages given, bytes to upload)."""
-        h, given = self.stage.h, 0
-        for i, s in enumerate(segs):
-            uid, held = self._device_rows[s.request_slot]
-            need = -(-(s.start + len(s.token_ids)) // K.PAGE_TOKENS)
-            if uid != s.uid or s.uid < 0 or len(s.pages) < held:
-                held = 0
-            h["held"][i] = held
-            if need > held:
-                h["new_pages"][given:given + need - held] = s.pages[held:need]
-                given += need - held
-            self._device_rows[s.request_slot] = (s.uid, max(held, need))
-        return given, self.stage.offsets["new_pages"][0] + 4 * given
+    def forget_device_rows(self) -> None:
+        """The device's table was overwritten by the host's: the next layout there starts every row anew."""
+        self._device_uid[:] = -2
 
-    def _fill(self, segs: list[Segment], pad_rows_to: int | None = None, review: bool = False) -> StepBatch:
-        """``review``: the segments are drafts to be verified.  Their pass is captured once for a number of requests and replayed behind
+    def stage_layout(self, segs: list[Segment]) -> int:
+        """Stage what ``K.step_layout`` needs of a step besides the lengths that ``_fill`` staged: the pages that the device's rows hold
+        and those that they are given.  Returns how many these are."""
+        if self.given is None:
+            n = self.max_rows * (self.max_pages + 1)
+            self.given_host = torch.empty(n, dtype=torch.int32, pin_memory=torch.cuda.is_available())
+            self.given = torch.empty(n, dtype=torch.int32, device=self.device)
+        n, h, out = len(segs), self.stage.h, self.given_host.numpy()
+        slots, uids = h["seg_slot"][:n], np.array([s.uid for s in segs], dtype=np.int64)
+        need = (h["seg_pos0"][:n] + h["seg_count"][:n] + K.PAGE_TOKENS - 1) // K.PAGE_TOKENS
+        held = self._device_held[slots]
+        known = (self._device_uid[slots] == uids) & (uids >= 0) & (np.array([len(s.pages) for s in segs]) >= held)
+        held = np.where(known, held, 0)
+        out[:n] = held
+        at = n
+        for i in np.flatnonzero(need > held):
+            m = int(need[i] - held[i])
+            out[at:at + m] = segs[i].pages[held[i]:need[i]]
+            at += m
+        self._device_uid[slots], self._device_held[slots] = uids, np.maximum(held, need)
+        return at - n
+
+    def _fill(self, segs: list[Segment], pad_rows_to: int | None = None, review: bool = False, lengths: bool = False) -> StepBatch:
+        """``lengths``: the step is laid out on the device (``K.step_layout``): positions, slots, row blocks and block table are left to it,
+        but for what ``_prompts`` looks at.
+
+        ``review``: the segments are drafts to be verified.  Their pass is captured once for a number of requests and replayed behind
         any contexts, so nothing that its launches depend on may follow the contexts of this step: the general kernel takes them.
         (64 requests of four rows, 64 over 4 heads: 29 us behind 100 tokens against 25 of the prompt kernel, but 268 against 390 behind 4000.)"""
         st = self.stage
         h = st.h
         qb = self.qb
         axes, embeds, decode, blocks = False, [], False, []
-        for s in segs:
-            self._sync_page_row(s)
+        if not lengths:
+            for s in segs:
+                self._sync_page_row(s)
         if all(len(s.token_ids) == 1 for s in segs):
             # decode fast path: one token, one row block and one sampled row per segment
             n = len(segs)
             h["token_ids"][:n] = [s.token_ids[0] for s in segs]
             starts = np.fromiter((s.start for s in segs), dtype=np.int32, count=n)
-            h["positions"][:n] = starts
-            for i, s in enumerate(segs):
-                if s.positions3 is not None:               # a request with media decodes at sequence index + its offset
-                    h["positions"][i] = int(np.asarray(s.positions3)[0, 0])
-            h["slots"][:n] = [s.pages[s.start >> 4] * 16 + (s.start & 15) for s in segs]
-            h["rb_req"][:n] = [s.request_slot for s in segs]
+            h["seg_slot"][:n] = [s.request_slot for s in segs]
             ar = np.arange(n, dtype=np.int32)
-            h["rb_qstart"][:n] = ar
-            h["rb_qcount"][:n] = 1
-            h["rb_ctx"][:n] = starts + 1
+            if not lengths:
+                h["positions"][:n] = starts
+                for i, s in enumerate(segs):
+                    if s.positions3 is not None:               # a request with media decodes at sequence index + its offset
+                        h["positions"][i] = int(np.asarray(s.positions3)[0, 0])
+                h["slots"][:n] = [s.pages[s.start >> 4] * 16 + (s.start & 15) for s in segs]
+                h["rb_req"][:n] = h["seg_slot"][:n]
+                h["rb_qstart"][:n] = ar
+                h["rb_qcount"][:n] = 1
+                h["rb_ctx"][:n] = starts + 1
             h["seg_row0"][:n] = ar
             h["seg_count"][:n] = 1
-            h["seg_slot"][:n] = h["rb_req"][:n]
             h["seg_pos0"][:n] = starts
             if self.adapters:
                 h["row_adapter"][:n] = [s.adapter for s in segs]
@@ -284,7 +305,7 @@ class BatchBuilder:
             rows = 0
             decode = self.qb >= 2                                 # one position of at most eight heads per row block
             if all(s.sample for s in segs):
-                h["row_slot"][:n] = h["rb_req"][:n]
+                h["row_slot"][:n] = h["seg_slot"][:n]
                 h["budget_init"][:n] = [s.budget_init for s in segs]
                 h["logit_rows"][:n] = ar
                 h["temperature"][:n] = [s.temperature for s in segs]
@@ -313,8 +334,10 @@ class BatchBuilder:
                 h["token_ids"][t:t + n] = s.token_ids
                 if self.adapters:
                     h["row_adapter"][t:t + n] = s.adapter
-                pos = np.arange(s.start, s.start + n, dtype=np.int32)
-                if s.positions3 is None:
+                pos = np.arange(s.start, s.start + (0 if lengths else n), dtype=np.int32)
+                if lengths:
+                    pass
+                elif s.positions3 is None:
                     h["positions"][t:t + n] = pos
                     if axes:
                         h["positions_h"][t:t + n] = pos
@@ -324,12 +347,13 @@ class BatchBuilder:
                     h["positions"][t:t + n], h["positions_h"][t:t + n], h["positions_w"][t:t + n] = p3[0], p3[1], p3[2]
                 for off, feat in (s.embeds or ()):
                     embeds.append((t + off, feat))
-                pages = np.asarray(s.pages, dtype=np.int32)
-                h["slots"][t:t + n] = pages[pos >> 4] * 16 + (pos & 15)
                 nb = -(-n // qb)
                 starts = np.arange(nb, dtype=np.int32) * qb
-                h["rb_req"][rb:rb + nb] = s.request_slot
-                h["rb_qstart"][rb:rb + nb] = t + starts
+                if not lengths:
+                    pages = np.asarray(s.pages, dtype=np.int32)
+                    h["slots"][t:t + n] = pages[pos >> 4] * 16 + (pos & 15)
+                    h["rb_req"][rb:rb + nb] = s.request_slot
+                    h["rb_qstart"][rb:rb + nb] = t + starts
                 h["rb_qcount"][rb:rb + nb] = np.minimum(n - starts, qb)
                 h["rb_ctx"][rb:rb + nb] = s.start + starts + 1
                 rb += nb
@@ -345,13 +369,15 @@ class BatchBuilder:
             # decode bucket padding: rows that write nothing and attend to nothing
             p = pad_rows_to
             h["token_ids"][t:p] = 0
-            h["positions"][t:p] = 0
-            h["slots"][t:p] = -1
-            h["row_adapter"][t:p] = -1
-            h["rb_req"][rb:p] = 0
-            h["rb_qstart"][rb:p] = np.arange(rb, p, dtype=np.int32)
-            h["rb_qcount"][rb:p] = 0
-            h["rb_ctx"][rb:p] = 0
+            if self.adapters:
+                h["row_adapter"][t:p] = -1
+            if not lengths:
+                h["positions"][t:p] = 0
+                h["slots"][t:p] = -1
+                h["rb_req"][rb:p] = 0
+                h["rb_qstart"][rb:p] = np.arange(rb, p, dtype=np.int32)
+                h["rb_qcount"][rb:p] = 0
+                h["rb_ctx"][rb:p] = 0
             h["logit_rows"][rows:p] = np.arange(rows, p)
             h["row_slot"][rows:p] = -1
             h["temperature"][rows:p] = 0
@@ -526,6 +552,7 @@ class GpuExecutor:
             # the warm-up run below must not touch real cache pages: the single real row is turned into padding too
             self.stage.h["slots"][:cap] = -1
             self.stage.h["rb_qcount"][:cap] = 0
+            self.builder.forget_device_rows()
             with torch.cuda.stream(self.stream):
                 self.stage.upload()                # on the steps' stream: the step below reads it
                 for _ in range(2):
@@ -657,6 +684,7 @@ class GpuExecutor:
             rows += [base + int(o) for o in s.logit_offsets]
             base += len(s.token_ids)
         out = np.empty((len(rows), self.logits.shape[1]), dtype=np.float32)
+        self.builder.forget_device_rows()
         with torch.cuda.stream(self.stream):
             self.h2d_bytes_last = self.stage.upload()
             hidden = self.runner.forward_hidden(b)
@@ -694,10 +722,10 @@ class GpuExecutor:
             # the pinned staging buffer is rewritten below: the previous launch's upload must have left it
             self._uploaded.synchronize()
             self._upload_pending = False
-        b, rows = self._fill(segs, pad_rows_to=cap)
-        whole = self._stage_whole(segs) if whole or "whole" in self.stage.d else 0
         laid_out = self.layout is not None and all(s.positions3 is None for s in segs)
-        given, upload = self.builder.stage_layout(segs) if laid_out else (0, None)
+        b, rows = self._fill(segs, pad_rows_to=cap, lengths=True) if laid_out else self._fill(segs, pad_rows_to=cap)
+        given = self.builder.stage_layout(segs) if laid_out else 0
+        whole = self._stage_whole(segs) if whole or "whole" in self.stage.d else 0
         if cap is not None and getattr(self, "audit_poison_padding", False):
             self._poison_padding(total, cap)
         k = self._launches & 1
@@ -705,13 +733,19 @@ class GpuExecutor:
         self._leases[k] = self.graph_rt.leases.acquire(k, f"launch {self._launches}")
         self._launches += 1
         with torch.cuda.stream(self.stream):
-            h2d = self.stage.upload(upload)
+            n = len(segs)
+            if laid_out:
+                h2d = self.stage.upload(self.stage.lengths_bytes) + 4 * (n + given)
+                self.builder.given[:n + given].copy_(self.builder.given_host[:n + given], non_blocking=True)
+            else:
+                h2d = self.stage.upload()
+                self.builder.forget_device_rows()
             self._uploaded.record(self.stream)
             self._upload_pending = True
             if laid_out:
-                d, n = self.stage.d, len(segs)
-                K.step_layout(d["seg_slot"][:n], d["seg_pos0"][:n], d["seg_count"][:n], d["held"][:n], d["new_pages"][:given], d["page_table"], self.layout,
-                              self.builder.qb, tokens=total, blocks=sum(-(-len(s.token_ids) // self.builder.qb) for s in segs), pad=cap or 0)
+                d = self.stage.d
+                K.step_layout(d["seg_slot"][:n], d["seg_pos0"][:n], d["seg_count"][:n], self.builder.given[:n], self.builder.given[n:n + given], d["page_table"],
+                              self.layout, self.builder.qb, tokens=total, blocks=b.num_row_blocks if cap is None else total, pad=cap or 0)
             if feedback_rows:
                 self.stage.d["token_ids"][:feedback_rows].copy_(self.out_ids[:feedback_rows], non_blocking=True)
             if self.timing:

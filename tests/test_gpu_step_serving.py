@@ -233,23 +233,25 @@ def test_adapters_beside_fp8_and_packed_weights(tmp_path):
 
 # ------------------------------------------------------------------------------------------------- layout
 def _compare_layout(ex, seen):
-    """After every launch what the device made is what the host filled in."""
-    launch = ex.launch
+    """After every launch what the device made is what the host would have filled in."""
+    from cubic_serve_b200.executor.gpu_executor import BatchBuilder
+    launch, n = ex.launch, ex.builder
+    host = BatchBuilder(n.max_rows, n.max_tokens, 256, 16 // n.qb, n.kv_heads, "cpu")
 
     def checked(segs, feedback_rows=0):
         handle = launch(segs, feedback_rows)
         torch.cuda.synchronize()
-        h, d = ex.stage.h, ex.stage.d
         t = sum(len(s.token_ids) for s in segs)
-        rb = sum(-(-len(s.token_ids) // ex.builder.qb) for s in segs)
-        decode = all(len(s.token_ids) == 1 for s in segs)
-        cap = (ex.graph_rt.dispatch(t) if decode and ex.use_graphs else None) or 0
-        for name, n in (("positions", max(t, cap)), ("slots", max(t, cap)), ("rb_req", max(rb, cap)), ("rb_qstart", max(rb, cap)), ("rb_qcount", max(rb, cap)),
-                        ("rb_ctx", max(rb, cap)), ("seg_row0", len(segs))):
-            assert d[name][:n].cpu().numpy().tolist() == h[name][:n].tolist(), name
+        cap = ex.graph_rt.dispatch(t) if all(len(s.token_ids) == 1 for s in segs) and ex.use_graphs else None
+        host.invalidate_page_rows([s.request_slot for s in segs])
+        b, _ = host._fill(segs, pad_rows_to=cap)
+        h, d = host.stage.h, ex.stage.d
+        for name, k in (("positions", b.num_tokens), ("slots", b.num_tokens), ("rb_req", b.num_row_blocks), ("rb_qstart", b.num_row_blocks), ("rb_qcount", b.num_row_blocks),
+                        ("rb_ctx", b.num_row_blocks), ("seg_row0", len(segs)), ("logit_rows", b.num_logit_rows)):
+            assert d[name][:k].cpu().numpy().tolist() == h[name][:k].tolist(), name
         for s in segs:
-            n = -(-(s.start + len(s.token_ids)) // 16)
-            assert d["page_table"][s.request_slot, :n].tolist() == list(s.pages[:n])
+            k = -(-(s.start + len(s.token_ids)) // 16)
+            assert d["page_table"][s.request_slot, :k].tolist() == list(s.pages[:k])
         assert ex.layout.totals.tolist()[3] == 0
         seen.append((t, handle["h2d"]))
         return handle
