@@ -254,11 +254,10 @@ class BatchBuilder:
         slots, uids = h["seg_slot"][:n], np.array([s.uid for s in segs], dtype=np.int64)
         need = (h["seg_pos0"][:n] + h["seg_count"][:n] + K.PAGE_TOKENS - 1) // K.PAGE_TOKENS
         held = self._device_held[slots]
-        known = (self._device_uid[slots] == uids) & (uids >= 0) & (np.array([len(s.pages) for s in segs]) >= held)
-        held = np.where(known, held, 0)
+        held = np.where((self._device_uid[slots] == uids) & (uids >= 0) & (np.array([len(s.pages) for s in segs]) >= held), held, 0)
         out[:n] = held
         at = n
-        for i in np.flatnonzero(need > held):
+        for i in np.flatnonzero(need > held).tolist():
             m = int(need[i] - held[i])
             out[at:at + m] = segs[i].pages[held[i]:need[i]]
             at += m
@@ -713,7 +712,7 @@ class GpuExecutor:
         """
         total = sum(len(s.token_ids) for s in segs)
         masked = self._stage_masks(segs)
-        whole = any(s.whole for s in segs)
+        whole = True in [s.whole for s in segs]
         decode = (all(len(s.token_ids) == 1 for s in segs) and self.use_graphs and (self.graph_masks or not masked))
         # the budgets' state machine runs on the ids of the draw, inside the step
         decode = decode and not (whole and self.runner.reasoning is not None)
@@ -722,7 +721,7 @@ class GpuExecutor:
             # the pinned staging buffer is rewritten below: the previous launch's upload must have left it
             self._uploaded.synchronize()
             self._upload_pending = False
-        laid_out = self.layout is not None and all(s.positions3 is None for s in segs)
+        laid_out = self.layout is not None and [s.positions3 for s in segs].count(None) == len(segs)
         b, rows = self._fill(segs, pad_rows_to=cap, lengths=True) if laid_out else self._fill(segs, pad_rows_to=cap)
         given = self.builder.stage_layout(segs) if laid_out else 0
         whole = self._stage_whole(segs) if whole or "whole" in self.stage.d else 0
