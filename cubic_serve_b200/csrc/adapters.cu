@@ -451,28 +451,27 @@ adapter_up_kernel(const CbAdapter p) {
     const int used = w.slot < 0 ? 0 : p.ranks ? min(R, max(0, p.ranks[w.slot])) : R;
     char* to = static_cast<char*>(p.out) + (w.col0 + rc * 8) * 2;
     uint2 h[AHEAD ? 2 : 1][2][R16];                                            // of eight rows, both parts
-    auto load_h = [&](int e_, int m0) {
-      if (m0 + e_ * 8 < rows) {
-        const size_t at = static_cast<size_t>(first + min(m0 + e_ * 8 + g, rows - 1)) * rt + sec * R;
+    const __nv_bfloat16* hi_at = static_cast<const __nv_bfloat16*>(p.hi) + static_cast<size_t>(first + g) * rt + sec * R + c * (R16 == 1 ? 4 : 8);
+    const ptrdiff_t lo_off = static_cast<const __nv_bfloat16*>(p.lo) - static_cast<const __nv_bfloat16*>(p.hi);
+    // rows behind the item's last are another's, or the spare ones behind the buffer's: what comes of them is not written
+    auto load_h = [&](int e_, const __nv_bfloat16* at) {
+      const int e = AHEAD ? e_ : 0;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(half ? p.lo : p.hi) + at;
-          const int e = AHEAD ? e_ : 0;
-          if (R16 == 1) {
-            h[e][half][0] = *reinterpret_cast<const uint2*>(from + c * 4);
-          } else {
+      for (int half = 0; half < 2; ++half) {
+        const __nv_bfloat16* from = at + e_ * 8 * rt + (half ? lo_off : 0);
+        if (R16 == 1) {
+          h[e][half][0] = *reinterpret_cast<const uint2*>(from);
+        } else {
 #pragma unroll
-            for (int s = 0; s < R16 / 2; ++s) {
-              if (s * 32 >= used) break;
-              const uint4 v = *reinterpret_cast<const uint4*>(from + s * 32 + c * 8);
-              h[e][half][2 * s] = make_uint2(v.x, v.y);
-              h[e][half][2 * s + 1] = make_uint2(v.z, v.w);
-            }
+          for (int s = 0; s < R16 / 2; ++s) {
+            const uint4 v = *reinterpret_cast<const uint4*>(from + s * 32);
+            h[e][half][2 * s] = make_uint2(v.x, v.y);
+            h[e][half][2 * s + 1] = make_uint2(v.z, v.w);
           }
         }
       }
     };
-    if (AHEAD && used) { load_h(0, 0); load_h(1, 0); }
+    if (AHEAD && used) { load_h(0, hi_at); load_h(1, hi_at); }
     // product t, places g and g + 8: columns 2 t and 2 t + 1 of the lane's
     uint32_t b[MT][R16][4];
     const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(max(w.slot, 0)) * n + col) * R;
@@ -505,8 +504,8 @@ adapter_up_kernel(const CbAdapter p) {
       if (used) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          if (m0 + e * 8 >= rows) break;
-          if (!AHEAD) load_h(e, m0);
+          if (R16 > 1 && m0 + e * 8 >= rows) break;
+          if (!AHEAD) load_h(e, hi_at);
           float acc[MT][4];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -529,7 +528,6 @@ adapter_up_kernel(const CbAdapter p) {
           for (int half = 0; half < 2; ++half) {
 #pragma unroll
             for (int k = 0; k < R16; ++k) {
-              if (k / 2 * 32 >= used) break;                                   // two products share the ranks of 32
 #pragma unroll
               for (int t = 0; t < MT; ++t) mma_bf16(acc[t], b[t][k], h[AHEAD ? e : 0][half][k].x, h[AHEAD ? e : 0][half][k].y);
             }
@@ -545,7 +543,8 @@ adapter_up_kernel(const CbAdapter p) {
             }
           }
         }
-        if (AHEAD) { load_h(0, m0 + 16); load_h(1, m0 + 16); }
+        hi_at += 16 * rt;
+        if (AHEAD && m0 + 16 < rows) { load_h(0, hi_at); load_h(1, hi_at); }
         __syncwarp();
       }
 #pragma unroll

@@ -870,7 +870,7 @@ class AdapterRows:
         self.max_ranks = max(64, 2 * max_ranks)                     # ranks are stored as 16, 32, 64 or 128
         self.order = torch.zeros(max_rows, dtype=torch.int32, device=device)
         self.items = torch.zeros(1 + 3 * (max(max_rows // 64, min(max_rows, 512) // 16) + min(slots + 1, max_rows)), dtype=torch.int32, device=device)
-        self.h = torch.zeros(2, max_rows * self.max_ranks, dtype=torch.bfloat16, device=device)
+        self.h = torch.zeros(2, (max_rows + 16) * self.max_ranks, dtype=torch.bfloat16, device=device)      # sixteen spare rows: they are read
         self._at = (self.order.data_ptr(), self.items.data_ptr(), self.h[0].data_ptr(), self.h[1].data_ptr())
 
 
