@@ -28,16 +28,17 @@ static constexpr int kAdapterThreads = 256;
 
 // ------------------------------------------------------------------ rows by adapter
 // order[]: the step's rows by adapter, a row's place among its adapter's by its index; rows without one last.
-// items[]: [0] = count, then {adapter (-1: none), first place, rows}.
+// items[]: [0] = count, then {adapter (-1: none), first place, rows} of up to 16 or 64 rows.
+// strips[]: [0] = count, from [4] on {adapter, first place, rows, 0} of up to 16.
 // One CTA: a warp counts the adapters of its share of the rows, the counts become places, a second look at the ids fills them.  8192 rows
 // are two rounds of 8 steps a warp.
 __global__ void __launch_bounds__(kSortThreads)
-adapter_rows_kernel(const int* __restrict__ ids, int rows, int slots, int* __restrict__ order, int* __restrict__ items) {
-  extern __shared__ unsigned short cnt[];                             // [32 warps][buckets]
-  __shared__ int warp_rows[32], warp_items[32];
+adapter_rows_kernel(const int* __restrict__ ids, int rows, int slots, int* __restrict__ order, int* __restrict__ items, int* __restrict__ strips) {
+  extern __shared__ unsigned short cnt[];                             // [warps][buckets]
+  __shared__ int warp_sum[3][32], base[3][kAdapterMaxSlots + 2];      // rows, items and strips of the buckets before
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, buckets = slots + 1;
   const int share = (((rows + 31) >> 5) + 31) & ~31, lo = min(rows, warp * share), hi = min(rows, lo + share);
-  const int warps = rows ? (rows + share - 1) / share : 0;               // that have any rows
+  const int warps = rows ? (rows + share - 1) / share : 0;            // that have any rows
   for (int i = tid; i < warps * buckets; i += kSortThreads) cnt[i] = 0;
   pdl_wait();
   pdl_launch_dependents();
@@ -52,36 +53,70 @@ adapter_rows_kernel(const int* __restrict__ ids, int rows, int slots, int* __res
     __syncwarp();
   }
   __syncthreads();
-  // counts of the warps before, rows and items of the buckets before
+  // counts of the warps before, then of the buckets before
   int n = 0;
-  if (tid < buckets)
+  if (tid < buckets) {
+#pragma unroll 8
     for (int w = 0; w < warps; ++w) {
       const int c = cnt[w * buckets + tid];
       cnt[w * buckets + tid] = static_cast<unsigned short>(n);
       n += c;
     }
-  const int per = adapter_item_rows(rows), nt = (n + per - 1) / per;
-  int at = n, it = nt;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, at, o), b = __shfl_up_sync(0xffffffffu, it, o);
-    if (lane >= o) { at += a; it += b; }
   }
-  if (lane == 31) { warp_rows[warp] = at; warp_items[warp] = it; }
+  const int per = adapter_item_rows(rows);
+  int sum[3] = {n, (n + per - 1) / per, (n + 15) / 16};
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const int a = __shfl_up_sync(0xffffffffu, sum[i], o);
+      if (lane >= o) sum[i] += a;
+    }
+  if (lane == 31) for (int i = 0; i < 3; ++i) warp_sum[i][warp] = sum[i];
   __syncthreads();
-  for (int w = 0; w < warp; ++w) { at += warp_rows[w]; it += warp_items[w]; }
-  at -= n;
-  if (tid < buckets) {
-    for (int w = 0; w < warps; ++w) cnt[w * buckets + tid] = static_cast<unsigned short>(cnt[w * buckets + tid] + at);
-    for (int i = 0; i < nt; ++i) {
-      int* e = items + 1 + 3 * (it - nt + i);
-      e[0] = tid < slots ? tid : -1;
-      e[1] = at + i * per;
-      e[2] = min(per, n - i * per);
+  if (warp == 0) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      int v = warp_sum[i][lane];
+      const int own = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += a;
+      }
+      warp_sum[i][lane] = v - own;
     }
   }
-  if (tid == kSortThreads - 1) items[0] = it;
+  if (tid == 0) base[0][0] = base[1][0] = base[2][0] = 0;
   __syncthreads();
+  if (tid < buckets) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) base[i][tid + 1] = sum[i] + warp_sum[i][warp];
+    const int at = base[0][tid + 1] - n;
+#pragma unroll 8
+    for (int w = 0; w < warps; ++w) cnt[w * buckets + tid] = static_cast<unsigned short>(cnt[w * buckets + tid] + at);
+  }
+  __syncthreads();
+  // both lists, an entry a thread
+  auto bucket_of = [&](const int* upto, int e) {                      // the last that starts at or before e
+    int a = 0, b = buckets;
+    while (b - a > 1) {
+      const int mid = (a + b) >> 1;
+      if (upto[mid] <= e) a = mid; else b = mid;
+    }
+    return a;
+  };
+  for (int e = tid; e < base[1][buckets]; e += kSortThreads) {
+    const int b = bucket_of(base[1], e), off = (e - base[1][b]) * per;
+    items[1 + 3 * e] = b < slots ? b : -1;
+    items[2 + 3 * e] = base[0][b] + off;
+    items[3 + 3 * e] = min(per, base[0][b + 1] - base[0][b] - off);
+  }
+  for (int e = tid; e < base[2][buckets]; e += kSortThreads) {
+    const int b = bucket_of(base[2], e), off = (e - base[2][b]) * 16;
+    reinterpret_cast<int4*>(strips)[1 + e] = make_int4(b < slots ? b : -1, base[0][b] + off, min(16, base[0][b + 1] - base[0][b] - off), 0);
+  }
+  if (tid == 0) { items[0] = base[1][buckets]; strips[0] = base[2][buckets]; }
   for (int r = lo; r < hi; r += 32) {
     const int row = r + lane;
     int b = -1;
@@ -106,7 +141,7 @@ struct CbAdapter {
   const void* b;                         // bf16 [slots, n, rank]
   const float* scale;                    // [slots]
   const int* ranks;                      // [slots] ranks in use, or null: all
-  const int* order; const int* items;    // adapter_rows_kernel's
+  const int* order; const int* items; const int* strips;         // adapter_rows_kernel's
   void* hi; void* lo;                    // bf16 [rows, sections * rank]: h as a sum of two
   int rows, slots, k, n, rank, sections;
   int width[4];                          // columns of the sections
@@ -114,6 +149,7 @@ struct CbAdapter {
 
 namespace cb {
 
+// For A and B alone: what another kernel of the stream writes may change after this one has started, which the read-only path does not allow.
 __device__ __forceinline__ uint4 ldg16(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
 // h is kept as two bf16: the leading 8 bits of its mantissa cut off, and what is left, rounded: 2^-16 of the value, where one bf16 would
@@ -175,8 +211,8 @@ adapter_down_kernel(const CbAdapter p, int splits) {
         for (int j = 0; j < J; ++j) {
           const int at = t0 + j * step;
           const bool in = at < turns, in_x = at * 32 + c * 8 < p.k;
-          xa[b][j] = in_x && in0 ? ldg16(x0 + at * 32) : zero;
-          xb[b][j] = in_x && in1 ? ldg16(x1 + at * 32) : zero;
+          xa[b][j] = in_x && in0 ? *reinterpret_cast<const uint4*>(x0 + at * 32) : zero;
+          xb[b][j] = in_x && in1 ? *reinterpret_cast<const uint4*>(x1 + at * 32) : zero;
           const __nv_bfloat16* from = A + static_cast<size_t>(at) * rt * 32;
 #pragma unroll
           for (int t = 0; t < R16; ++t)
@@ -371,16 +407,16 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
   }
 }
 
-// out = y + h B^T of one item and 16 MT columns a warp.  B is the operand of sixteen, rows of h those of eight.  Which columns a product has is free: they are
-// chosen so that a lane ends up with 2 MT neighbours of two rows, and eight lanes with a row of 16 MT.  B's operands stay in registers for all rows of the
-// item; the products add to y, which is rounded once.  y comes through a ring of the warp's own, three sixteens of rows ahead and on into the next items, and
-// goes back through it: eight lanes copy a line of y, and a line of out.  (A lane's own columns straight from global memory were four lines a quarter of a
-// warp: 71 % of the load and store unit's cycles.)
+// out = y + h B^T of strips of sixteen rows, 16 MT columns a warp.  B is the operand of sixteen, rows of h those of eight.  Which columns a product has is
+// free: they are chosen so that a lane ends up with 2 MT neighbours of two rows, and eight lanes with a row of 16 MT.  A warp keeps its columns for a run of
+// strips and B's operands in registers as long as these are of one adapter; the products add to y, which is rounded once.  y comes through a ring of the
+// warp's own, three strips ahead, and goes back through it: eight lanes copy a line of y, and a line of out.  (A lane's own columns straight from global
+// memory were four lines a quarter of a warp: 71 % of the load and store unit's cycles.)
 template <int R16, int MT>
 __global__ void __launch_bounds__(kAdapterThreads, R16 * MT <= 4 ? 3 : 2)
 adapter_up_kernel(const CbAdapter p) {
   constexpr int R = R16 * 16, W = 16 * MT, kRing = 4, CH = 2 * MT, RP = 32 / CH, I = 16 / RP;     // 16-byte chunks of a row, rows of a copy, copies
-  constexpr bool AHEAD = R16 <= 2;                                             // registers for the next rows of h
+  constexpr bool AHEAD = R16 <= 2;                                             // registers for the next strip's h
   extern __shared__ __align__(16) unsigned char ring[];                        // [8 warps][kRing][16 rows][CH chunks]
   __shared__ int ring_row[8][kRing][16];                                       // which rows they are
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3, rr = lane / CH, rc = lane % CH;
@@ -396,116 +432,107 @@ adapter_up_kernel(const CbAdapter p) {
   auto copy_at = [&](int i) { return copy[i % (8 / RP)] + i / (8 / RP) * 128 * CH; };
   pdl_launch_dependents();
   pdl_wait();
-  const int n = p.n, blocks = (n + W - 1) / W, units = p.items[0] * blocks, stride = gridDim.x * 8, rt = p.sections * R;
+  const int n = p.n, blocks = (n + W - 1) / W, strips = p.strips[0], rt = p.sections * R, warps = gridDim.x * 8;
+  const int runs = min(strips, max(1, warps / blocks)), tasks = runs * blocks;         // runs of strips, of about the same length
   const uint32_t ldy = static_cast<uint32_t>(p.ldy) * 2, ldo = static_cast<uint32_t>(p.ldo) * 2;
   const bool in_place = p.out == p.y;
-  struct Walk {                                                                // through the sixteens of rows of the warp's units
-    int u, m0, slot, first, rows, col0;
-  };
-  auto enter = [&](Walk& w) {
-    for (; w.u < units; w.u += stride) {
-      const int item = w.u / blocks;
-      w.col0 = (w.u - item * blocks) * W;
-      w.slot = p.items[1 + 3 * item];
-      w.first = p.items[2 + 3 * item];
-      w.rows = p.items[3 + 3 * item];
-      w.m0 = 0;
-      if (w.slot >= 0 || !in_place) return;
-    }
-    w.rows = 0;
-  };
-  Walk f{static_cast<int>(blockIdx.x) * 8 + warp, 0, 0, 0, 0, 0};
-  enter(f);
-  Walk w = f;
-  // what is fetched next: its rows are looked up a step before, one a lane
-  int ahead = 0;
-  auto look_up = [&]() { if (lane < 16 && f.m0 + lane < f.rows) ahead = p.order[f.first + f.m0 + lane]; };
-  look_up();
-  int put = 0, get = 0;
-  auto fetch = [&]() {
-    if (f.rows) {
-      if (lane < 16) ring_row[warp][put][lane] = ahead;
-      const int left = f.col0 + rc * 8 < n ? f.rows - f.m0 - rr : 0;
-      const char* from = static_cast<const char*>(p.y) + (f.col0 + rc * 8) * 2;
-      const uint32_t to = mine_at + put * 256 * CH;
-#pragma unroll
-      for (int i = 0; i < I; ++i)
-        cp_async16(to + copy_at(i), from + static_cast<size_t>(ldy) * static_cast<uint32_t>(__shfl_sync(0xffffffffu, ahead, rr + i * RP)), i * RP < left);
-      f.m0 += 16;
-      if (f.m0 >= f.rows) {
-        f.u += stride;
-        enter(f);
-      }
-      look_up();
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    put = (put + 1) % kRing;
-  };
-#pragma unroll 1
-  for (int i = 0; i < kRing - 1; ++i) fetch();
-  while (w.rows) {
-    const int col = w.col0 + g * 2 * MT, first = w.first, rows = w.rows;
-    const bool in = col < n, in_copy = w.col0 + rc * 8 < n;
+  const int4* list = reinterpret_cast<const int4*>(p.strips) + 1;              // adapter, first place, rows
+  const ptrdiff_t lo_off = static_cast<const __nv_bfloat16*>(p.lo) - static_cast<const __nv_bfloat16*>(p.hi);
+  for (int task = blockIdx.x * 8 + warp; task < tasks; task += warps) {
+    const int run = task / blocks, col0 = (task - run * blocks) * W, col = col0 + g * 2 * MT;
+    const int s0 = static_cast<int>(static_cast<long long>(strips) * run / runs), s1 = static_cast<int>(static_cast<long long>(strips) * (run + 1) / runs);
+    const bool in = col < n, in_copy = col0 + rc * 8 < n;
     int sec = 0;
-    for (int at = p.width[0]; sec + 1 < p.sections && w.col0 >= at; at += p.width[sec]) ++sec;
-    const int used = w.slot < 0 ? 0 : p.ranks ? min(R, max(0, p.ranks[w.slot])) : R;
-    char* to = static_cast<char*>(p.out) + (w.col0 + rc * 8) * 2;
+    for (int at = p.width[0]; sec + 1 < p.sections && col0 >= at; at += p.width[sec]) ++sec;
+    const char* from = static_cast<const char*>(p.y) + (col0 + rc * 8) * 2;
+    char* to = static_cast<char*>(p.out) + (col0 + rc * 8) * 2;
+    const __nv_bfloat16* h0 = static_cast<const __nv_bfloat16*>(p.hi) + static_cast<size_t>(g) * rt + sec * R + c * (R16 == 1 ? 4 : 8);
+    // what is fetched next: its strip and rows (one a lane) are looked up a step before
+    int f = s0, put = 0, get = 0, ahead = 0;
+    int4 f_strip = make_int4(-1, 0, 0, 0);
+    auto look_up = [&]() {
+      if (f >= s1) return;
+      f_strip = list[f];
+      if (lane < f_strip.z) ahead = p.order[f_strip.y + lane];
+    };
+    auto fetch = [&]() {
+      if (f < s1) {
+        const bool skip = in_place && f_strip.x < 0;
+        if (lane < 16) ring_row[warp][put][lane] = ahead;
+        const int left = in_copy && !skip ? f_strip.z - rr : 0;
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+          cp_async16(mine_at + put * 256 * CH + copy_at(i), from + static_cast<size_t>(ldy) * static_cast<uint32_t>(__shfl_sync(0xffffffffu, ahead, rr + i * RP)), i * RP < left);
+        ++f;
+        look_up();
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      put = (put + 1) % kRing;
+    };
+    look_up();
+#pragma unroll 1
+    for (int i = 0; i < kRing - 1; ++i) fetch();
     uint2 h[AHEAD ? 2 : 1][2][R16];                                            // of eight rows, both parts
-    const __nv_bfloat16* hi_at = static_cast<const __nv_bfloat16*>(p.hi) + static_cast<size_t>(first + g) * rt + sec * R + c * (R16 == 1 ? 4 : 8);
-    const ptrdiff_t lo_off = static_cast<const __nv_bfloat16*>(p.lo) - static_cast<const __nv_bfloat16*>(p.hi);
-    // rows behind the item's last are another's, or the spare ones behind the buffer's: what comes of them is not written
-    auto load_h = [&](int e_, const __nv_bfloat16* at) {
+    // rows behind the strip's last are another's, or the spare ones behind the buffer's: what comes of them is not written
+    auto load_h = [&](int e_, int first) {
       const int e = AHEAD ? e_ : 0;
+      const __nv_bfloat16* at = h0 + static_cast<size_t>(first + e_ * 8) * rt;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const __nv_bfloat16* from = at + e_ * 8 * rt + (half ? lo_off : 0);
         if (R16 == 1) {
-          h[e][half][0] = *reinterpret_cast<const uint2*>(from);
+          h[e][half][0] = *reinterpret_cast<const uint2*>(at + (half ? lo_off : 0));
         } else {
 #pragma unroll
           for (int s = 0; s < R16 / 2; ++s) {
-            const uint4 v = *reinterpret_cast<const uint4*>(from + s * 32);
+            const uint4 v = *reinterpret_cast<const uint4*>(at + (half ? lo_off : 0) + s * 32);
             h[e][half][2 * s] = make_uint2(v.x, v.y);
             h[e][half][2 * s + 1] = make_uint2(v.z, v.w);
           }
         }
       }
     };
-    if (AHEAD && used) { load_h(0, hi_at); load_h(1, hi_at); }
-    // product t, places g and g + 8: columns 2 t and 2 t + 1 of the lane's
+    int4 strip = list[s0];
+    if (AHEAD) { load_h(0, strip.y); load_h(1, strip.y); }
     uint32_t b[MT][R16][4];
-    const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(max(w.slot, 0)) * n + col) * R;
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const __nv_bfloat16* at = B + (2 * t + k) * R;
-        if (R16 == 1) {
-          const uint2 v = in && used ? __ldg(reinterpret_cast<const uint2*>(at + c * 4)) : make_uint2(0, 0);
-          b[t][0][k] = v.x;
-          b[t][0][2 + k] = v.y;
-        } else {
-#pragma unroll
-          for (int s = 0; s < R16 / 2; ++s) {
-            const uint4 v = in && s * 32 < used ? ldg16(at + s * 32 + c * 8) : make_uint4(0, 0, 0, 0);
-            b[t][2 * s][k] = v.x;
-            b[t][2 * s][2 + k] = v.y;
-            b[t][2 * s + 1][k] = v.z;
-            b[t][2 * s + 1][2 + k] = v.w;
-          }
-        }
-      }
+    int held = -2, used = 0;                                                   // the adapter whose B is in registers
 #pragma unroll 1
-    for (int m0 = 0; m0 < rows; m0 += 16) {
+    for (int s = s0; s < s1; ++s) {
+      if (strip.x != held) {
+        held = strip.x;
+        used = held < 0 ? 0 : p.ranks ? min(R, max(0, p.ranks[held])) : R;
+        // product t, places g and g + 8: columns 2 t and 2 t + 1 of the lane's
+        const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(max(held, 0)) * n + col) * R;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const __nv_bfloat16* at = B + (2 * t + k) * R;
+            if (R16 == 1) {
+              const uint2 v = in && used ? __ldg(reinterpret_cast<const uint2*>(at + c * 4)) : make_uint2(0, 0);
+              b[t][0][k] = v.x;
+              b[t][0][2 + k] = v.y;
+            } else {
+#pragma unroll
+              for (int q = 0; q < R16 / 2; ++q) {
+                const uint4 v = in && q * 32 < used ? ldg16(at + q * 32 + c * 8) : make_uint4(0, 0, 0, 0);
+                b[t][2 * q][k] = v.x;
+                b[t][2 * q][2 + k] = v.y;
+                b[t][2 * q + 1][k] = v.z;
+                b[t][2 * q + 1][2 + k] = v.w;
+              }
+            }
+          }
+      }
+      const int first = strip.y, left = in_copy && !(in_place && held < 0) ? strip.z - rr : 0, rows = strip.z;
+      if (s + 1 < s1) strip = list[s + 1];
       asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
       __syncwarp();
       unsigned char* slot = mine + get * 256 * CH;
-      const int left = in_copy ? rows - m0 - rr : 0;
       if (used) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          if (R16 > 1 && m0 + e * 8 >= rows) break;
-          if (!AHEAD) load_h(e, hi_at);
+          if (R16 > 1 && e * 8 >= rows) break;
+          if (!AHEAD) load_h(e, first);
           float acc[MT][4];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -525,13 +552,11 @@ adapter_up_kernel(const CbAdapter p) {
             }
           }
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int k = 0; k < R16; ++k) {
+            for (int k = 0; k < R16; ++k)
 #pragma unroll
               for (int t = 0; t < MT; ++t) mma_bf16(acc[t], b[t][k], h[AHEAD ? e : 0][half][k].x, h[AHEAD ? e : 0][half][k].y);
-            }
-          }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             unsigned char* at = slot + own[i] + e * 128 * CH;
@@ -543,10 +568,9 @@ adapter_up_kernel(const CbAdapter p) {
             }
           }
         }
-        hi_at += 16 * rt;
-        if (AHEAD && m0 + 16 < rows) { load_h(0, hi_at); load_h(1, hi_at); }
         __syncwarp();
       }
+      if (AHEAD && s + 1 < s1) { load_h(0, strip.y); load_h(1, strip.y); }
 #pragma unroll
       for (int i = 0; i < I; ++i)
         if (i * RP < left)
@@ -555,10 +579,9 @@ adapter_up_kernel(const CbAdapter p) {
       get = (get + 1) % kRing;
       fetch();
     }
-    w.u += stride;
-    enter(w);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 template <typename Kernel>
@@ -570,6 +593,14 @@ static cudaError_t adapter_smem(Kernel kernel, int smem, bool (&ready)[64]) {
   if (e == cudaSuccess && dev < 64) ready[dev] = true;
   return e;
 }
+
+// Most entries of a list of `per` rows each: every adapter with a row has one, and what its other rows fill.
+static int adapter_entries(int rows, int slots, int per) {
+  const int used = min(slots + 1, rows);
+  return used + (rows - used) / per;
+}
+static int adapter_items(int rows, int slots) { return adapter_entries(rows, slots, adapter_item_rows(rows)); }
+static int adapter_strips(int rows, int slots) { return adapter_entries(rows, slots, 16); }
 
 // CTAs that share k: as long as two find room on every SM.  Layers of 256 rows over 64 adapters of rank 64 and of 8192 rows of rank 16 by the most CTAs: 148
 // 178 and 456 us, 320 164 and 408, 592 180 and 426.
@@ -604,12 +635,12 @@ static cudaError_t adapter_down_tile(const CbAdapter& p, int items, cudaStream_t
 }
 
 template <int R16, int MT>
-static cudaError_t adapter_up(const CbAdapter& p, int items, cudaStream_t stream) {
+static cudaError_t adapter_up(const CbAdapter& p, cudaStream_t stream) {
   constexpr int smem = 8 * 4 * 512 * MT, resident = R16 * MT <= 4 ? 3 : 2;
   static bool ready[64] = {};
   const cudaError_t e = adapter_smem(adapter_up_kernel<R16, MT>, smem, ready);
   if (e != cudaSuccess) return e;
-  const int warps = items * ((p.n + 16 * MT - 1) / (16 * MT));
+  const int warps = adapter_strips(p.rows, p.slots) * ((p.n + 16 * MT - 1) / (16 * MT));
   return launch(adapter_up_kernel<R16, MT>, dim3(min((warps + 7) / 8, 148 * resident)), dim3(kAdapterThreads), smem, stream, p);
 }
 
@@ -626,22 +657,14 @@ static int adapter_launch(const CbAdapter& p, int items, cudaStream_t stream) {
   if (e != cudaSuccess) return static_cast<int>(e);
   bool wide = R16 < 4;                                                // a warp's columns belong to one section
   for (int i = 0; i + 1 < p.sections; ++i) wide = wide && p.width[i] % 64 == 0;
-  return static_cast<int>(wide ? adapter_up<R16, R16 < 4 ? 4 : 2>(p, items, stream) : adapter_up<R16, 2>(p, items, stream));
-}
-
-static int adapter_items(int rows, int slots) {
-  const int used = min(slots + 1, rows);                              // adapters with a row, each with one item and what its other rows fill
-  return used + (rows - used) / adapter_item_rows(rows);
+  return static_cast<int>(wide ? adapter_up<R16, R16 < 4 ? 4 : 2>(p, stream) : adapter_up<R16, 2>(p, stream));
 }
 
 }  // namespace cb
 
 extern "C" {
 
-// Most work items that `rows` rows over `slots` adapters can make: `items` of cb_adapter_rows holds 1 + 3 times as many.
-int cb_adapter_items(int rows, int slots) { return rows <= 0 || slots <= 0 ? 0 : cb::adapter_items(rows, slots); }
-
-int cb_adapter_rows(const void* ids, int rows, int slots, void* order, void* items, void* stream) {
+int cb_adapter_rows(const void* ids, int rows, int slots, void* order, void* items, void* strips, void* stream) {
   using namespace cb;
   if (rows < 0 || rows > kAdapterMaxRows || slots < 1 || slots > kAdapterMaxSlots) return -10;
   const int smem = 32 * (slots + 1) * static_cast<int>(sizeof(unsigned short));
@@ -650,7 +673,7 @@ int cb_adapter_rows(const void* ids, int rows, int slots, void* order, void* ite
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   return static_cast<int>(launch(adapter_rows_kernel, dim3(1), dim3(kSortThreads), smem, static_cast<cudaStream_t>(stream), static_cast<const int*>(ids), rows, slots,
-                                 static_cast<int*>(order), static_cast<int*>(items)));
+                                 static_cast<int*>(order), static_cast<int*>(items), static_cast<int*>(strips)));
 }
 
 int cb_adapter_add(const CbAdapter* p, void* stream) {

@@ -26,6 +26,7 @@ struct CbVocabulary {
   const int* rows_of;                        // [rows] row r is row rows_of[r] of everything (below 0: none), or null: r
   int* ids; float* logprob; int* kept;       // [rows]; the last two or null
   int rows, vocab, f32;
+  int limit;                                 // rows of every tensor: one of rows_of that is not below it is none
 };
 
 namespace cb {
@@ -112,7 +113,7 @@ struct VocabRow {
   }
   __device__ __forceinline__ int first(int v) const { return v * 8 - shift; }
   __device__ __forceinline__ bool whole(int v) const { return first(v) >= 0 && first(v) + 8 <= vocab; }
-  __device__ __forceinline__ uint32_t word(int w) const { return w >= 0 && w < words ? __ldg(mask + w) : 0u; }
+  __device__ __forceinline__ uint32_t word(int w) const { return w >= 0 && w < words ? mask[w] : 0u; }
   __device__ __forceinline__ uint32_t allowed(int v) const {                 // by the mask
     if (!mask) return 0xffu;
     const int i = first(v), w = i >> 5;
@@ -129,10 +130,10 @@ struct VocabRow {
     }
     if (i >= 0 && i + 8 <= vocab) {
       if (F32) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(base) + v * 2), b = __ldg(reinterpret_cast<const uint4*>(base) + v * 2 + 1);
+        const uint4 a = reinterpret_cast<const uint4*>(base)[v * 2], b = reinterpret_cast<const uint4*>(base)[v * 2 + 1];
         u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w; u[4] = b.x; u[5] = b.y; u[6] = b.z; u[7] = b.w;
       } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(base) + v);
+        const uint4 a = reinterpret_cast<const uint4*>(base)[v];
         u[0] = a.x << 16; u[1] = a.x & 0xffff0000u; u[2] = a.y << 16; u[3] = a.y & 0xffff0000u;
         u[4] = a.z << 16; u[5] = a.z & 0xffff0000u; u[6] = a.w << 16; u[7] = a.w & 0xffff0000u;
       }
@@ -141,7 +142,7 @@ struct VocabRow {
       for (int j = 0; j < 8; ++j) {
         const bool in = i + j >= 0 && i + j < vocab;
         if (!in) ok &= ~(1u << j);
-        u[j] = !in ? 0u : F32 ? __ldg(reinterpret_cast<const uint32_t*>(base) + v * 8 + j) : static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(base) + v * 8 + j)) << 16;
+        u[j] = !in ? 0u : F32 ? reinterpret_cast<const uint32_t*>(base)[v * 8 + j] : static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(base)[v * 8 + j]) << 16;
       }
     }
 #pragma unroll
@@ -551,7 +552,7 @@ struct Vocab {
       }
 #pragma unroll
       for (int k = 0; k < U; ++k)
-        if (ok[k]) q[k] = __ldg(vec + row.from + (i0 + k * kVocabWarps) * 32 + lane);
+        if (ok[k]) q[k] = vec[row.from + (i0 + k * kVocabWarps) * 32 + lane];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const int i = i0 + k * kVocabWarps;
@@ -573,7 +574,7 @@ struct Vocab {
       if ((e ? last == row.to : first == row.from) || i % kVocabWarps != tid >> 5) continue;
       int t = -32768;
       if (lane < 8 && row.first(end) + lane >= 0 && row.first(end) + lane < row.vocab && (row.allowed(end) >> lane & 1)) {
-        const uint32_t h = __ldg(reinterpret_cast<const unsigned short*>(row.base) + end * 8 + lane);
+        const uint32_t h = reinterpret_cast<const unsigned short*>(row.base)[end * 8 + lane];
         if (FILL) atomicAdd(&count[place_of(h << 16, kUsualBase)], 1);
         t = static_cast<int>(static_cast<short>(h));
       }
@@ -621,7 +622,7 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
   pdl_wait();
   pdl_launch_dependents();
   const int r = p.rows_of ? p.rows_of[n_row] : n_row;
-  if (r < 0) return;
+  if (r < 0 || r >= p.limit) return;
   const float temp = p.temperature ? p.temperature[r] : 0.f;
   const bool greedy = !(temp > 0.f);
   const double t = greedy ? 1.0 : static_cast<double>(temp);
@@ -805,7 +806,7 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
     const int v = f.row.from + i * 32 + lane;
     if (v >= f.row.to) return 0;
     if (plain && f.row.whole(v)) {
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(f.row.base) + v);
+      const uint4 q = reinterpret_cast<const uint4*>(f.row.base)[v];
       return (__popc(__vcmpeq2(q.x, twice)) + __popc(__vcmpeq2(q.y, twice)) + __popc(__vcmpeq2(q.z, twice)) + __popc(__vcmpeq2(q.w, twice))) >> 4;
     }
     uint32_t u[8];

@@ -764,6 +764,7 @@ class StepLayout:
         self.max_tokens, self.max_requests, self.max_blocks = max_tokens, max_requests, max_blocks
         into = into or {}
         _require(set(into) <= set(sizes), f"unknown buffers {sorted(set(into) - set(sizes))}")
+        _require(len({t.device for t in into.values()} | {torch.empty(0, device=device).device}) == 1, "buffers must be on the layout's device")
         at = []
         for name, n in sizes.items():
             dt = torch.int64 if name == "logit_rows" else torch.int32
@@ -869,9 +870,12 @@ class AdapterRows:
         self.max_rows, self.slots, self.rows = max_rows, slots, 0
         self.max_ranks = max(64, 2 * max_ranks)                     # ranks are stored as 16, 32, 64 or 128
         self.order = torch.zeros(max_rows, dtype=torch.int32, device=device)
-        self.items = torch.zeros(1 + 3 * (max(max_rows // 64, min(max_rows, 512) // 16) + min(slots + 1, max_rows)), dtype=torch.int32, device=device)
+        used = min(slots + 1, max_rows)
+        strips = used + (max_rows - used) // 16 + 1
+        i32 = dict(dtype=torch.int32, device=device)
+        self.items, self.strips = torch.zeros(1 + 3 * strips, **i32), torch.zeros(4 + 4 * strips, **i32)
         self.h = torch.zeros(2, (max_rows + 16) * self.max_ranks, dtype=torch.bfloat16, device=device)      # sixteen spare rows: they are read
-        self._at = (self.order.data_ptr(), self.items.data_ptr(), self.h[0].data_ptr(), self.h[1].data_ptr())
+        self._at = (self.order.data_ptr(), self.items.data_ptr(), self.strips.data_ptr(), self.h[0].data_ptr(), self.h[1].data_ptr())
 
 
 def adapter_rows(ids: torch.Tensor, out: AdapterRows) -> AdapterRows:
@@ -879,7 +883,7 @@ def adapter_rows(ids: torch.Tensor, out: AdapterRows) -> AdapterRows:
     there is not: none)."""
     rows = ids.numel()
     _require(rows <= out.max_rows, "more rows than there is room for")
-    _call("cb_adapter_rows", (_vector(ids, torch.int32, rows, "ids"), rows, out.slots, out._at[0], out._at[1]), (ids, out.order))
+    _call("cb_adapter_rows", (_vector(ids, torch.int32, rows, "ids"), rows, out.slots, *out._at[:3]), (ids, out.order))
     out.rows = rows
     return out
 
@@ -897,6 +901,7 @@ def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, rows: Adapt
     _require(bank.sections * bank.rank <= rows.max_ranks, "more ranks than the sorted rows have room for")
     ldx, ldy, ldo = (x.stride(0), y.stride(0), out.stride(0)) if t > 1 else (bank.k, bank.n, bank.n)
     px, py, po = x.data_ptr(), y.data_ptr(), out.data_ptr()
+    _require(py != po or ldy == ldo, "y and out are the same rows or other memory")
     _require(x.stride(1) == 1 and y.stride(1) == 1 and out.stride(1) == 1 and ldx >= bank.k and ldy >= bank.n and ldo >= bank.n and (ldx | ldy | ldo) % 8 == 0 and max(ldy, ldo) <= 1 << 30 and (px | py | po) % 16 == 0,
              "rows of neighbouring elements at a stride of a multiple of 8, from a 16-byte boundary")
     packed = native.ADAPTER.pack(px, ldx, py, ldy, po, ldo, *bank._at, *rows._at, t, *bank._shape)
@@ -917,8 +922,8 @@ def sample_vocabulary(logits: torch.Tensor, out_ids: torch.Tensor, temperature: 
     ``u`` times the mass kept.  ``u``: ``uniforms`` fp32 in [0, 1), or the stream of ``seeds`` and ``counters`` that ``sample``
     uses.  ``temperature`` 0: the largest value.  NaN, -inf and what ``mask`` (bit i: token i is allowed) leaves out are never
     drawn; a row that nothing is left of gets id 0 and log-probability -inf.  ``out_logprob``: of the token among those kept;
-    ``out_kept``: how many those are.  ``rows`` int32: draw for these rows only (below 0: none), each at its own place of every
-    other tensor."""
+    ``out_kept``: how many those are.  ``rows`` int32: draw for these rows only (below 0, or a row that there is not: none), each at its own
+    place of every other tensor."""
     _require(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32), "logits are a bf16 or fp32 matrix")
     n, f32 = logits.shape[0], torch.float32
     vocab = logits.shape[1] if vocab is None else vocab
@@ -935,7 +940,7 @@ def sample_vocabulary(logits: torch.Tensor, out_ids: torch.Tensor, temperature: 
         _vector(top_k, i32, n, "top_k"), _vector(top_p, f32, n, "top_p"), _vector(min_p, f32, n, "min_p"), _vector(uniforms, f32, n, "uniforms"),
         _vector(seeds, i64, n, "seeds"), _vector(counters, i64, n, "counters"), _vector(rows, i32, 0, "rows"),
         _vector(out_ids, i32, n, "out_ids"), _vector(out_logprob, f32, n, "out_logprob"), _vector(out_kept, i32, n, "out_kept"),
-        n if rows is None else rows.numel(), vocab, logits.dtype is f32)
+        n if rows is None else rows.numel(), vocab, logits.dtype is f32, n)
     _call("cb_sample_vocabulary", (packed,), (logits, out_ids, temperature, top_k, top_p, min_p, uniforms, seeds, counters, mask, out_logprob, out_kept, rows))
     return out_ids
 

@@ -331,11 +331,10 @@ def _declare(l: ctypes.CDLL) -> None:
     l.cb_canary_check.argtypes = [vp, ll, ctypes.c_uint, i, vp, vp]
     l.cb_canary_check.restype = i
     # what a step does for each of its requests: layout, adapters, draws from a whole vocabulary
-    l.cb_adapter_items.argtypes = [i, i]
-    l.cb_adapter_rows.argtypes = [vp, i, i, vp, vp, vp]
+    l.cb_adapter_rows.argtypes = [vp, i, i, vp, vp, vp, vp]
     for name in ("step_layout", "adapter_add", "sample_vocabulary"):
         getattr(l, f"cb_{name}").argtypes = [vp, vp]
-    for name in ("step_layout", "adapter_items", "adapter_rows", "adapter_add", "sample_vocabulary"):
+    for name in ("step_layout", "adapter_rows", "adapter_add", "sample_vocabulary"):
         getattr(l, f"cb_{name}").restype = i
     # layered decoders: fp32 residual stream, delta rule of any head size, latent attention
     l.cb_bf16_gemm_wide.argtypes = [vp, vp, ll, vp, vp, vp]
@@ -566,8 +565,8 @@ class ScoredMoeStruct(ctypes.Structure):
 
 # Arguments of the operators around a step's shared layers, packed in one call: an operator of 2 us has no time for a field at a time.
 STEP_LAYOUT = struct.Struct("@15P9i4x")                      # CbStepLayout, csrc/step_layout.cu
-ADAPTER = struct.Struct("@PqPqPq8P10i")                      # CbAdapter, csrc/adapters.cu
-VOCABULARY = struct.Struct("@PqPq11P3i4x")                     # CbVocabulary, csrc/sample_vocabulary.cu
+ADAPTER = struct.Struct("@PqPqPq9P10i")                      # CbAdapter, csrc/adapters.cu
+VOCABULARY = struct.Struct("@PqPq11P4i")                     # CbVocabulary, csrc/sample_vocabulary.cu
 
 
 class ReduceNormStruct(ctypes.Structure):

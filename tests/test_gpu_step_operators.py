@@ -420,7 +420,7 @@ def test_draws_of_chosen_rows_leave_the_others():
     one = torch.ones(10, device=DEV)
     want, ids = torch.zeros(10, dtype=I32, device=DEV), torch.full((10,), -3, dtype=I32, device=DEV)
     K.sample_vocabulary(x, want, one, uniforms=u)
-    K.sample_vocabulary(x, ids, one, uniforms=u, rows=torch.tensor([7, -1, 2, 9], dtype=I32, device=DEV))
+    K.sample_vocabulary(x, ids, one, uniforms=u, rows=torch.tensor([7, -1, 2, 10, 9, 2, 2 ** 31 - 1], dtype=I32, device=DEV))
     assert [int(v) for v in ids] == [int(want[i]) if i in (2, 7, 9) else -3 for i in range(10)]
 
 
