@@ -33,7 +33,7 @@ static constexpr int kAdapterThreads = 256;
 // One CTA: a warp counts the adapters of its share of the rows, the counts become places, a second look at the ids fills them.  8192 rows
 // are two rounds of 8 steps a warp.
 __global__ void __launch_bounds__(kSortThreads)
-adapter_rows_kernel(const int* __restrict__ ids, int rows, int slots, int* __restrict__ order, int* __restrict__ items, int* __restrict__ strips) {
+adapter_rows_kernel(const int* ids, int rows, int slots, int* order, int* items, int* strips) {
   extern __shared__ unsigned short cnt[];                             // [warps][buckets]
   __shared__ int warp_sum[3][32], base[3][kAdapterMaxSlots + 2];      // rows, items and strips of the buckets before
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, buckets = slots + 1;
@@ -173,86 +173,94 @@ __device__ __forceinline__ void put_h(const CbAdapter& p, float v, float scale, 
   static_cast<__nv_bfloat16*>(p.lo)[at] = lo;
 }
 
-// h of few rows: one item, one section, sixteen rows at a time.  A is the operand of sixteen, rows of x those of eight, for most adapters of a decode step have
-// no more.  The eight warps and the CTAs of a cluster take turns of 32 along k; sums are joined in their order.  The order of k inside a product is free: a
-// lane's 16 bytes of x and of A are its operands of two products as they lie.  J turns of a warp are on their way while J others are multiplied.
-template <int R16>
+// Few rows: both products of an item of up to sixteen rows by a cluster, in one launch.  The CTAs have a share of k each, make their part of h for all sections,
+// add the parts up from one another's shared memory, tell all of them the sums, and go on with a share of the columns each.
+//
+// First product: A is the operand of sixteen, rows of x those of eight, for most adapters of a decode step have no more.  The eight warps of all CTAs take turns
+// of 32 along k.  The order of k inside a product is free: a lane's 16 bytes of x and of A are its operands of two products as they lie.  64 ranks
+// at a time, one turn of a warp on its way while another is multiplied.
+// Second product: as in adapter_up_kernel, with h from shared memory and sixteen rows at most.
+template <int R16, int MT>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
-adapter_down_kernel(const CbAdapter p, int splits) {
-  constexpr int R = R16 * 16, RP = R + 4, J = R16 == 1 ? 2 : 1, kBuffers = R16 == 8 ? 1 : 2;
-  extern __shared__ float sh[];                                       // [8][16][RP], then the cluster's part [16][R]
-  float* part = sh + 8 * 16 * RP;
+adapter_few_kernel(const CbAdapter p, int splits) {
+  constexpr int R = R16 * 16, RP = 68, W = 16 * MT;
+  extern __shared__ __align__(16) unsigned char few[];
+  const int rt = p.sections * R, tiles = rt / 16, hp = rt + 8;        // row pitch of h
+  float* red = reinterpret_cast<float*>(few);                         // [8 warps][16 rows][RP]
+  float* part = red + 8 * 16 * RP;                                    // [16][rt]
+  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(part + 16 * rt);                  // [2 parts][16][hp]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const int rank_in = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0, team = blockIdx.x / splits, teams = gridDim.x / splits;
   pdl_launch_dependents();
   pdl_wait();
-  const int units = p.items[0] * p.sections, rt = p.sections * R, turns = (p.k + 31) >> 5, step = 8 * splits;
-  for (int u = team; u < units; u += teams) {
-    const int item = u / p.sections, sec = u - item * p.sections;
-    const int slot = p.items[1 + 3 * item], first = p.items[2 + 3 * item], rows = p.items[3 + 3 * item];
-    if (slot < 0) continue;
-    const float scale = p.scale[slot];
+  const int4* list = reinterpret_cast<const int4*>(p.strips) + 1;     // adapter, first place, rows
+  const int items = p.strips[0], turns = (p.k + 31) >> 5, step = 8 * splits, n = p.n;
+  const bool in_place = p.out == p.y;
+  int4 next = list[team];                                             // on its way with their number
+  for (int item = team; item < items; item += teams) {
+    const int slot = next.x, first = next.y, rows = next.z;
+    if (item + teams < items) next = list[item + teams];
+    if (slot < 0) {                                                   // rows without an adapter
+      if (in_place) continue;
+      const int chunks = n / 8;
+      for (int e = rank_in * kAdapterThreads + tid; e < rows * chunks; e += splits * kAdapterThreads) {
+        const size_t row = p.order[first + e / chunks];
+        const int col = e % chunks * 8;
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + col) = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.y) + row * p.ldy + col);
+      }
+      continue;
+    }
     const int used = p.ranks ? min(R, max(0, p.ranks[slot])) : R;
-    const __nv_bfloat16* A = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * turns * rt + sec * R) * 32 + lane * 8;
-    for (int m0 = 0; m0 < rows; m0 += 16) {
-      const int left = min(16, rows - m0);
-      const bool in0 = g < left, in1 = g + 8 < left, both = left > 8;
-      const __nv_bfloat16* x0 = static_cast<const __nv_bfloat16*>(p.x) + (in0 ? p.order[first + m0 + g] * p.ldx : 0) + c * 8;
-      const __nv_bfloat16* x1 = static_cast<const __nv_bfloat16*>(p.x) + (in1 ? p.order[first + m0 + g + 8] * p.ldx : 0) + c * 8;
-      float acc[R16][2][4];
+    const float scale = p.scale[slot];
+    const bool in0 = g < rows, in1 = g + 8 < rows, both = rows > 8;
+    const __nv_bfloat16* x0 = static_cast<const __nv_bfloat16*>(p.x) + (in0 ? p.order[first + g] * p.ldx : 0) + c * 8;
+    const __nv_bfloat16* x1 = static_cast<const __nv_bfloat16*>(p.x) + (in1 ? p.order[first + g + 8] * p.ldx : 0) + c * 8;
+    for (int q0 = 0; q0 < tiles; q0 += 4) {
+      const __nv_bfloat16* A = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * turns * rt + q0 * 16) * 32 + lane * 8;
+      bool on[4];                                                     // tiles of sixteen that hold ranks in use
 #pragma unroll
-      for (int t = 0; t < R16; ++t)
+      for (int t = 0; t < 4; ++t) on[t] = q0 + t < tiles && (q0 + t) % R16 * 16 < used;
+      float acc[4][2][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int h = 0; h < 2; ++h) acc[t][h][0] = acc[t][h][1] = acc[t][h][2] = acc[t][h][3] = 0.f;
-      uint4 w[kBuffers][J][R16][2], xa[kBuffers][J], xb[kBuffers][J];
-      auto load = [&](int b, int t0) {
+      uint4 w[2][4][2], xa[2], xb[2];
+      auto load = [&](int b, int at) {
         const uint4 zero = make_uint4(0, 0, 0, 0);
+        const bool in = at < turns, in_x = at * 32 + c * 8 < p.k;
+        xa[b] = in_x && in0 ? *reinterpret_cast<const uint4*>(x0 + at * 32) : zero;
+        xb[b] = in_x && in1 ? *reinterpret_cast<const uint4*>(x1 + at * 32) : zero;
+        const __nv_bfloat16* from = A + static_cast<size_t>(at) * rt * 32;
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const int at = t0 + j * step;
-          const bool in = at < turns, in_x = at * 32 + c * 8 < p.k;
-          xa[b][j] = in_x && in0 ? *reinterpret_cast<const uint4*>(x0 + at * 32) : zero;
-          xb[b][j] = in_x && in1 ? *reinterpret_cast<const uint4*>(x1 + at * 32) : zero;
-          const __nv_bfloat16* from = A + static_cast<size_t>(at) * rt * 32;
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int t = 0; t < R16; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) w[b][j][t][h] = in && t * 16 + h * 8 < used ? ldg16(from + (t * 16 + h * 8) * 32) : zero;
-        }
+          for (int h = 0; h < 2; ++h) w[b][t][h] = in && on[t] ? ldg16(from + (t * 16 + h * 8) * 32) : zero;
       };
       auto multiply = [&](int b) {
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-          for (int t = 0; t < R16; ++t) {
-            const uint4 &lo = w[b][j][t][0], &hi = w[b][j][t][1];
-            const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
-            mma_bf16(acc[t][0], f0, xa[b][j].x, xa[b][j].y);
-            mma_bf16(acc[t][0], f1, xa[b][j].z, xa[b][j].w);
-            if (both) {
-              mma_bf16(acc[t][1], f0, xb[b][j].x, xb[b][j].y);
-              mma_bf16(acc[t][1], f1, xb[b][j].z, xb[b][j].w);
-            }
+        for (int t = 0; t < 4; ++t) {
+          const uint4 &lo = w[b][t][0], &hi = w[b][t][1];
+          const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
+          mma_bf16(acc[t][0], f0, xa[b].x, xa[b].y);
+          mma_bf16(acc[t][0], f1, xa[b].z, xa[b].w);
+          if (both) {
+            mma_bf16(acc[t][1], f0, xb[b].x, xb[b].y);
+            mma_bf16(acc[t][1], f1, xb[b].z, xb[b].w);
           }
+        }
       };
       const int t0 = rank_in * 8 + warp;
-      if (kBuffers == 1) {
-        for (int t = t0; t < turns; t += J * step) {
-          load(0, t);
-          multiply(0);
-        }
-      } else {
-        load(0, t0);
-        for (int t = t0; t < turns; t += 2 * J * step) {
-          load(kBuffers - 1, t + J * step);
-          multiply(0);
-          load(0, t + 2 * J * step);
-          multiply(kBuffers - 1);
-        }
+      load(0, t0);
+      for (int t = t0; t < turns; t += 2 * step) {
+        load(1, t + step);
+        multiply(0);
+        load(0, t + 2 * step);
+        multiply(1);
       }
-      float* mine = sh + warp * 16 * RP;
+      float* mine = red + warp * 16 * RP;
 #pragma unroll
-      for (int t = 0; t < R16; ++t)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (h && !both) break;
@@ -263,31 +271,160 @@ adapter_down_kernel(const CbAdapter p, int splits) {
           at[RP + 8] = acc[t][h][3];
         }
       __syncthreads();
-      const size_t out = static_cast<size_t>(first + m0) * rt + sec * R;
-      for (int e = tid; e < left * R; e += kAdapterThreads) {
-        const int r = e / R, k = e % R;
+      const int width = min(64, rt - q0 * 16);
+      for (int e = tid; e < rows * 64; e += kAdapterThreads) {
+        const int r = e >> 6, k = e & 63;
+        if (k >= width) continue;
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) v += sh[(w * 16 + r) * RP + k];
-        if (splits == 1) put_h(p, v, scale, k < used, out + static_cast<size_t>(r) * rt + k);
-        else part[e] = v;
+        for (int q = 0; q < 8; ++q) v += red[(q * 16 + r) * RP + k];
+        part[r * rt + q0 * 16 + k] = v;
       }
-      if (splits > 1) {
-        cluster_sync_all();
-        const uint32_t base = smem_u32(part);
-        for (int e = rank_in * kAdapterThreads + tid; e < left * R; e += splits * kAdapterThreads) {
-          float q[8], v = 0.f;
+      __syncthreads();
+    }
+    // B and y of the warp's first columns come while the sums are exchanged
+    int row[2][2];
 #pragma unroll
-          for (int s = 0; s < 8; ++s) q[s] = s < splits ? ld_cluster_f32(cluster_map(base + e * 4, s)) : 0.f;
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int s = 0; s < 8; ++s) v += q[s];
-          put_h(p, v, scale, e % R < used, out + static_cast<size_t>(e / R) * rt + e % R);
+      for (int i = 0; i < 2; ++i) row[e][i] = e * 8 + 2 * c + i < rows ? p.order[first + e * 8 + 2 * c + i] : -1;
+    // product t, places g and g + 8: columns 2 t and 2 t + 1 of the lane's
+    uint32_t b[MT][R16][4], y[2][2][MT];
+    auto load_columns = [&](int u) {
+      const int col = u * W + g * 2 * MT;
+      const bool in = col < n;
+      const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(slot) * n + col) * R;
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const __nv_bfloat16* at = B + (2 * t + k) * R;
+          if (R16 == 1) {
+            const uint2 v = in && used ? __ldg(reinterpret_cast<const uint2*>(at + c * 4)) : make_uint2(0, 0);
+            b[t][0][k] = v.x;
+            b[t][0][2 + k] = v.y;
+          } else {
+#pragma unroll
+            for (int s = 0; s < R16 / 2; ++s) {
+              const uint4 v = in && s * 32 < used ? ldg16(at + s * 32 + c * 8) : make_uint4(0, 0, 0, 0);
+              b[t][2 * s][k] = v.x;
+              b[t][2 * s][2 + k] = v.y;
+              b[t][2 * s + 1][k] = v.z;
+              b[t][2 * s + 1][2 + k] = v.w;
+            }
+          }
         }
-        cluster_sync_all();
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t) y[e][i][t] = 0;
+          if (!in || row[e][i] < 0) continue;
+          const __nv_bfloat16* at = static_cast<const __nv_bfloat16*>(p.y) + row[e][i] * p.ldy + col;
+          if (MT == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(at);
+            y[e][i][0] = v.x; y[e][i][1] = v.y; y[e][i][MT - 2] = v.z; y[e][i][MT - 1] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(at);
+            y[e][i][0] = v.x; y[e][i][1] = v.y;
+          }
+        }
+    };
+    load_columns(rank_in * 8 + warp);
+    // two ranks a thread: the sum over the CTAs in their order, and its two parts to all of them
+    if (splits > 1) cluster_sync_all();
+    const uint32_t part_at = smem_u32(part), hs_at = smem_u32(hs);
+    for (int e = rank_in * kAdapterThreads + tid; e < 8 * rt; e += splits * kAdapterThreads) {
+      const int r = e / (rt / 2), k = e % (rt / 2) * 2;
+      float v[2] = {0.f, 0.f};
+      if (r < rows) {
+        if (splits > 1) {
+          float2 q[8];
+#pragma unroll
+          for (int s = 0; s < 8; ++s) {
+            q[s] = make_float2(0.f, 0.f);
+            if (s < splits) {
+              asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(q[s].x), "=f"(q[s].y) : "r"(cluster_map(part_at + (r * rt + k) * 4, s)) : "memory");
+            }
+          }
+#pragma unroll
+          for (int s = 0; s < 8; ++s) { v[0] += q[s].x; v[1] += q[s].y; }
+        } else {
+          v[0] = part[r * rt + k];
+          v[1] = part[r * rt + k + 1];
+        }
+      }
+      uint32_t hi = 0, lo = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        __nv_bfloat16 a, b;
+        split_h((k + i) % R < used ? v[i] * scale : 0.f, a, b);       // ranks that are not in use may have met what is not finite in x
+        hi |= static_cast<uint32_t>(__bfloat16_as_ushort(a)) << 16 * i;
+        lo |= static_cast<uint32_t>(__bfloat16_as_ushort(b)) << 16 * i;
+      }
+      const uint32_t to = hs_at + (r * hp + k) * 2;
+      if (splits > 1) {
+        for (int s = 0; s < splits; ++s) {
+          st_cluster_u32(cluster_map(to, s), hi);
+          st_cluster_u32(cluster_map(to + 16 * hp * 2, s), lo);
+        }
       } else {
-        __syncthreads();
+        *reinterpret_cast<uint32_t*>(hs + r * hp + k) = hi;
+        *reinterpret_cast<uint32_t*>(hs + (16 + r) * hp + k) = lo;
       }
     }
+    if (splits > 1) cluster_sync_all(); else __syncthreads();
+    for (int u = rank_in * 8 + warp; u * W < n; u += step) {
+      const int col0 = u * W, col = col0 + g * 2 * MT;
+      const bool in = col < n;
+      int sec = 0;
+      for (int at = p.width[0]; sec + 1 < p.sections && col0 >= at; at += p.width[sec]) ++sec;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (e * 8 >= rows) break;
+        float acc[MT][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            acc[t][i] = __uint_as_float(y[e][i][t] << 16);
+            acc[t][2 + i] = __uint_as_float(y[e][i][t] & 0xffff0000u);
+          }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const __nv_bfloat16* h = hs + (half * 16 + e * 8 + g) * hp + sec * R;
+          if (R16 == 1) {
+            const uint2 v = *reinterpret_cast<const uint2*>(h + c * 4);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) mma_bf16(acc[t], b[t][0], v.x, v.y);
+          } else {
+#pragma unroll
+            for (int s = 0; s < R16 / 2; ++s) {
+              const uint4 v = *reinterpret_cast<const uint4*>(h + s * 32 + c * 8);
+#pragma unroll
+              for (int t = 0; t < MT; ++t) {
+                mma_bf16(acc[t], b[t][2 * s], v.x, v.y);
+                mma_bf16(acc[t], b[t][2 * s + 1], v.z, v.w);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!in || row[e][i] < 0) continue;
+          __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.out) + row[e][i] * p.ldo + col;
+          if (MT == 4) {
+            *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16x2(acc[0][i], acc[0][2 + i]), pack_bf16x2(acc[1][i], acc[1][2 + i]),
+                                                       pack_bf16x2(acc[MT - 2][i], acc[MT - 2][2 + i]), pack_bf16x2(acc[MT - 1][i], acc[MT - 1][2 + i]));
+          } else {
+            *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc[0][i], acc[0][2 + i]), pack_bf16x2(acc[1][i], acc[1][2 + i]));
+          }
+        }
+      }
+      if ((u + step) * W < n) load_columns(u + step);
+    }
+    if (splits == 1) __syncthreads();                                 // h is read until here
   }
 }
 
@@ -610,16 +747,21 @@ static int adapter_splits(int units, int k) {
   return splits;
 }
 
-template <int R16>
-static cudaError_t adapter_down(const CbAdapter& p, int items, cudaStream_t stream) {
-  constexpr int R = R16 * 16;
-  constexpr int smem = (8 * 16 * (R + 4) + 16 * R) * sizeof(float);
-  static bool ready[64] = {};
-  const cudaError_t e = adapter_smem(adapter_down_kernel<R16>, smem, ready);
+template <int R16, int MT>
+static cudaError_t adapter_few(const CbAdapter& p, int items, cudaStream_t stream) {
+  const int rt = p.sections * R16 * 16, smem = (8 * 16 * 68 + 16 * rt) * 4 + 2 * 16 * (rt + 8) * 2;
+  static_assert((8 * 16 * 68 + 16 * 512) * 4 + 2 * 16 * 520 * 2 <= 113 * 1024, "two of the largest on an SM");
+  static int ready[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  const int units = items * p.sections;
-  const int splits = adapter_splits(units, p.k);
-  return launch(adapter_down_kernel<R16>, dim3(min(units, 592 / splits) * splits), dim3(kAdapterThreads), smem, stream, dim3(splits, 1, 1), p, splits);
+  if (smem > 48 * 1024 && (dev >= 64 || ready[dev] < smem)) {
+    e = cudaFuncSetAttribute(adapter_few_kernel<R16, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready[dev] = smem;
+  }
+  const int splits = adapter_splits(items, p.k);
+  return launch(adapter_few_kernel<R16, MT>, dim3(min(items, 592 / splits) * splits), dim3(kAdapterThreads), smem, stream, dim3(splits, 1, 1), p, splits);
 }
 
 template <int NT>
@@ -645,19 +787,17 @@ static cudaError_t adapter_up(const CbAdapter& p, cudaStream_t stream) {
 }
 
 template <int R16>
-static int adapter_launch(const CbAdapter& p, int items, cudaStream_t stream) {
-  cudaError_t e;
-  if (p.rows <= kAdapterFewRows) {
-    e = adapter_down<R16>(p, items, stream);
-  } else {
-    const int n = p.sections * R16;                                   // sixteens of ranks
-    e = n == 1 ? adapter_down_tile<1>(p, items, stream) : n == 2 ? adapter_down_tile<2>(p, items, stream) : n == 3 ? adapter_down_tile<3>(p, items, stream)
-      : n == 4 ? adapter_down_tile<4>(p, items, stream) : n % 8 == 0 ? adapter_down_tile<8>(p, items, stream) : adapter_down_tile<6>(p, items, stream);
-  }
-  if (e != cudaSuccess) return static_cast<int>(e);
+static int adapter_launch(const CbAdapter& p, cudaStream_t stream) {
   bool wide = R16 < 4;                                                // a warp's columns belong to one section
   for (int i = 0; i + 1 < p.sections; ++i) wide = wide && p.width[i] % 64 == 0;
-  return static_cast<int>(wide ? adapter_up<R16, R16 < 4 ? 4 : 2>(p, stream) : adapter_up<R16, 2>(p, stream));
+  constexpr int kWide = R16 < 4 ? 4 : 2;
+  const int items = adapter_items(p.rows, p.slots);
+  if (p.rows <= kAdapterFewRows) return static_cast<int>(wide ? adapter_few<R16, kWide>(p, items, stream) : adapter_few<R16, 2>(p, items, stream));
+  const int n = p.sections * R16;                                     // sixteens of ranks
+  const cudaError_t e = n == 1 ? adapter_down_tile<1>(p, items, stream) : n == 2 ? adapter_down_tile<2>(p, items, stream) : n == 3 ? adapter_down_tile<3>(p, items, stream)
+                      : n == 4 ? adapter_down_tile<4>(p, items, stream) : n % 8 == 0 ? adapter_down_tile<8>(p, items, stream) : adapter_down_tile<6>(p, items, stream);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  return static_cast<int>(wide ? adapter_up<R16, kWide>(p, stream) : adapter_up<R16, 2>(p, stream));
 }
 
 }  // namespace cb
@@ -690,13 +830,12 @@ int cb_adapter_add(const CbAdapter* p, void* stream) {
         reinterpret_cast<uintptr_t>(p->hi) | reinterpret_cast<uintptr_t>(p->lo)) & 15) != 0)
     return -13;
   if (p->rows == 0) return 0;
-  const int items = adapter_items(p->rows, p->slots);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (p->rank) {
-    case 16: return adapter_launch<1>(*p, items, s);
-    case 32: return adapter_launch<2>(*p, items, s);
-    case 64: return adapter_launch<4>(*p, items, s);
-    case 128: return adapter_launch<8>(*p, items, s);
+    case 16: return adapter_launch<1>(*p, s);
+    case 32: return adapter_launch<2>(*p, s);
+    case 64: return adapter_launch<4>(*p, s);
+    case 128: return adapter_launch<8>(*p, s);
   }
   return -14;
 }

@@ -231,6 +231,30 @@ def test_adapters_beside_fp8_and_packed_weights(tmp_path):
         assert bool((((mixed - none).norm(dim=1) / none.norm(dim=1))[[0, 2]] > 0.3).all())
 
 
+@pytest.mark.parametrize("kind", ["experts", "hybrid"])
+def test_adapters_of_attention_layers_beside_experts_and_recurrent_mixers(tmp_path, kind):
+    from dataclasses import replace
+
+    from cubic_serve_b200.models.low_rank import AdapterError
+    if kind == "experts":
+        cfg = replace(CFG, family="gqa_moe", num_experts=8, experts_per_token=2, moe_intermediate_size=256, intermediate_size=0)
+    else:
+        cfg = replace(CFG, family="qwen3_5", num_layers=4, gdn_interval=4, gdn_k_heads=2, gdn_v_heads=4, attn_output_gate=True, rotary_dim=64)
+    full = [i for i in range(cfg.num_layers) if not cfg.layer_is_gdn(i)]
+    _adapter(tmp_path / "a", 1, modules=("q_proj", "v_proj", "o_proj"), layers=full)
+    _adapter(tmp_path / "no", 1, modules=("gate_proj",) if kind == "experts" else ("q_proj",), layers=range(cfg.num_layers))
+    ex = _executor(cfg, low_rank=(2, 8))
+    with pytest.raises(AdapterError):
+        ex.load_adapter("no", tmp_path / "no")
+    eng = _engine(ex, [("a", tmp_path / "a")], enable_prefix_cache=False)
+    p = _prompts(4, 7)
+    none = _run(eng, [(q, _sampling()) for q in p])
+    mixed = _run(eng, [(q, _sampling(adapter="a" if i % 2 else None)) for i, q in enumerate(p)])
+    assert [mixed[0], mixed[2]] == [none[0], none[2]] and mixed[1] != none[1] and mixed[3] != none[3]
+    if kind == "experts":
+        assert none == _run(_engine(_executor(cfg), enable_prefix_cache=False), [(q, _sampling()) for q in p]), "without an adapter the model is what it was"
+
+
 # ------------------------------------------------------------------------------------------------- layout
 def _compare_layout(ex, seen):
     """After every launch what the device made is what the host would have filled in."""
