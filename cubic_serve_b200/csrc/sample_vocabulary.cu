@@ -18,7 +18,7 @@
 // Packed by ops/native.py::VOCABULARY.
 struct CbVocabulary {
   const void* logits; long long ld;          // [rows, vocab], bf16 or fp32
-  const uint32_t* mask; long long ld_mask;   // [rows, words] allowed tokens, or null
+  const uint32_t* mask; long long ld_mask;   // [rows, words] allowed tokens, or null; a stride of 0: of all rows
   const float* temperature;                  // [rows], 0: greedy
   const int* top_k; const float* top_p; const float* min_p;      // [rows] or null; 0, 1, 0: none
   const float* uniforms;                     // [rows], or null: seeds and counters
@@ -47,6 +47,9 @@ static constexpr double kUnit = 4398046511104.0;           // 2^42
 static constexpr float kLeastMinP = 8.6736174e-19f;        // 2^-60: less is as good as none
 static constexpr int kUsualBase = ((127 - 32) << 7) - 1;
 static_assert(kSegments <= kVocabThreads, "a thread holds the sums before a segment");
+
+// Segments of a CTA of several that are added up at a time: all of its own, but no more than find room beside a table with masses.
+__host__ __device__ constexpr int team_room(int team, bool f32) { return f32 && team < 4 ? (kSegments + 3) / 4 : (kSegments + team - 1) / team; }
 
 __device__ __forceinline__ uint32_t sort_key(uint32_t u) {                 // order of the values; both zeros are one
   if ((u << 1) == 0) return 0x80000000u;
@@ -179,7 +182,7 @@ struct Vocab {
   int* count; u64* mass;                        // the table of the CTA's own tokens
   int* all_count; u64* all_mass;                // TEAM: of the row, the CTA's share of the segments
   short* tile_max;                              // bf16: largest of every 256 tokens as a signed 16-bit number: exact where it is not negative
-  int rank, team, base;
+  int rank, team, room, base;
   bool mixed;                                   // bf16: the bin of zero holds other values
   u64 zero_mass;
   float best;
@@ -286,70 +289,76 @@ struct Vocab {
     return c ? static_cast<u64>(__double2ll_rn(c * (w * kUnit))) : 0ull;
   }
 
-  // Sums of the segments, then those before each.  A thread takes a segment, from the bin of its lane on, so that 32 threads are at 32 banks; a CTA of several
-  // takes every team-th segment, once the bins of all have been added up.
-  __device__ void sums(int& total_c, u64& total_m) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (TEAM) {
-#pragma unroll 2
-      for (int i = warp; i * team + rank < kSegments; i += kVocabWarps) {
-        const int d = bin_in(i * team + rank, lane);
-        all_count[i * 32 + lane] = bin_count(d);
-        if (F32) all_mass[i * 32 + lane] = d >= kBins ? 0ull : at(mass, place_of_bin(d)) + (d == kZero ? at(mass, kNegative) : 0ull);
+  // A thread's segment; TEAM: its bins added up from `bins` on.
+  __device__ __forceinline__ void segment_sum(int g, int bins) {
+    const int lane = threadIdx.x & 31;
+    const bool one = bin_in(g, 1) >= kBins;                      // a segment of one bin
+    int from = 0, n = 0;
+    double w0 = 0.0, q = 0.0, w = 0.0;
+    u64 m = 0;
+    if (!F32 && !one) {
+      w0 = s.seg_w[g];
+      q = s.ratio[segment_step(g)];
+      if (w0 < 0.0) {                                            // up to the best value, whose weight is one; what is above it is empty
+        const int off = static_cast<int>(__float_as_uint(best) >> 16 & 0x7fffu) - static_cast<int>(segment_mag(g));
+        from = (best < 0.f) == (g > kZeroSegment) ? (g < kZeroSegment ? -off : off) : 32;
+        w0 = from >= 0 && from < 32 ? 1.0 : 0.0;
+      }
+      if (lane >= from) {
+        w = w0;
+        double power = q;
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          if ((lane - from) >> i & 1) w *= power;
+          power *= power;
+        }
       }
     }
-    weigh_segments();
-    __syncthreads();
-    const int g = tid * team + rank;
-    if (g < kSegments) {
-      const bool one = bin_in(g, 1) >= kBins;                      // a segment of one bin
-      int from = 0, n = 0;
-      double w0 = 0.0, q = 0.0, w = 0.0;
-      u64 m = 0;
-      if (!F32 && !one) {
-        w0 = s.seg_w[g];
-        q = s.ratio[segment_step(g)];
-        if (w0 < 0.0) {                                            // up to the best value, whose weight is one; what is above it is empty
-          const int off = static_cast<int>(__float_as_uint(best) >> 16 & 0x7fffu) - static_cast<int>(segment_mag(g));
-          from = (best < 0.f) == (g > kZeroSegment) ? (g < kZeroSegment ? -off : off) : 32;
-          w0 = from >= 0 && from < 32 ? 1.0 : 0.0;
-        }
-        if (lane >= from) {
-          w = w0;
-          double power = q;
-#pragma unroll
-          for (int i = 0; i < 5; ++i) {
-            if ((lane - from) >> i & 1) w *= power;
-            power *= power;
-          }
-        }
-      }
-      const int d0 = bin_in(g, 0), place = place_of_bin(d0), step = d0 < kZero ? -1 : 1;
-      if (one) {
-        n = TEAM ? all_count[tid * 32] : bin_count(d0);
-        m = F32 ? (TEAM ? all_mass[tid * 32] : lane_mass(g, 0, n)) : lane_mass(g, 0, n);
-      } else {
+    const int d0 = bin_in(g, 0), place = place_of_bin(d0), step = d0 < kZero ? -1 : 1;
+    if (one) {
+      n = TEAM ? all_count[bins] : bin_count(d0);
+      m = F32 ? (TEAM ? all_mass[bins] : lane_mass(g, 0, n)) : lane_mass(g, 0, n);
+    } else {
 #pragma unroll 8
-        for (int i = 0; i < 32; ++i) {
-          const int l = (i + lane) & 31, c = TEAM ? all_count[tid * 32 + l] : count[place + step * l];
-          n += c;
-          if (F32) {
-            m += TEAM ? all_mass[tid * 32 + l] : mass[place + step * l];
-          } else {
-            if (c) m += static_cast<u64>(__double2ll_rn(c * (w * kUnit)));
-            w = ((l + 1) & 31) == from ? w0 : l == 31 ? 0.0 : w * q;
-          }
+      for (int i = 0; i < 32; ++i) {
+        const int l = (i + lane) & 31, c = TEAM ? all_count[bins + l] : count[place + step * l];
+        n += c;
+        if (F32) {
+          m += TEAM ? all_mass[bins + l] : mass[place + step * l];
+        } else {
+          if (c) m += static_cast<u64>(__double2ll_rn(c * (w * kUnit)));
+          w = ((l + 1) & 31) == from ? w0 : l == 31 ? 0.0 : w * q;
         }
       }
-      if (!TEAM) {
-        s.seg_c[g] = n;
-        s.seg_m[g] = m;
-      } else {
-        for (int r = 0; r < team; ++r) {
-          st_cluster_u32(cluster_map(smem_u32(s.seg_c + g), r), n);
-          st_peer64(cluster_map(smem_u32(s.seg_m + g), r), m);
-        }
+    }
+    if (!TEAM) {
+      s.seg_c[g] = n;
+      s.seg_m[g] = m;
+    } else {
+      for (int r = 0; r < team; ++r) {
+        st_cluster_u32(cluster_map(smem_u32(s.seg_c + g), r), n);
+        st_peer64(cluster_map(smem_u32(s.seg_m + g), r), m);
       }
+    }
+  }
+
+  // Sums of the segments, then those before each.  A thread takes a segment, from the bin of its lane on, so that 32 threads are at 32 banks; a CTA of several
+  // takes every team-th segment, `room` of them at a time, once the bins of all have been added up.
+  __device__ void sums(int& total_c, u64& total_m) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    weigh_segments();
+    for (int from_i = 0; from_i * team + rank < kSegments; from_i += room) {
+      if (TEAM) {
+        if (from_i) __syncthreads();
+#pragma unroll 2
+        for (int i = from_i + warp; i < from_i + room && i * team + rank < kSegments; i += kVocabWarps) {
+          const int d = bin_in(i * team + rank, lane), to = (i - from_i) * 32 + lane;
+          all_count[to] = bin_count(d);
+          if (F32) all_mass[to] = d >= kBins ? 0ull : at(mass, place_of_bin(d)) + (d == kZero ? at(mass, kNegative) : 0ull);
+        }
+        __syncthreads();
+      }
+      if (tid >= from_i && tid < from_i + room && tid * team + rank < kSegments) segment_sum(tid * team + rank, (tid - from_i) * 32);
     }
     meet();
     const int own_c = tid < kSegments ? s.seg_c[tid] : 0;
@@ -412,18 +421,19 @@ struct Vocab {
     if (lane == l) { s.found_c = c - own_c; s.found_m = m - own_m; s.found_ties = own_c; s.found_at = l; }
     __syncwarp();
   }
+  // At least e^far of the best one's weight: without the exponential.
+  __device__ __forceinline__ bool heavy_one(float v, double far) const { return v >= best || (best < INFINITY && (static_cast<double>(v) - best) * inv_t >= far); }
   // Tokens of a bf16 row that have at least `least` of the best one's weight: all in the segments before the last one whose first value has it, and
   // those of that one.
   __device__ int heavy(double least) {
     const int tid = threadIdx.x, lane = tid & 31;
     const double far = log(least);
-    auto heavy_one = [&](float v) { return v >= best || (best < INFINITY && (static_cast<double>(v) - best) * inv_t >= far); };
     __syncthreads();
-    if (tid < kSegments && heavy_one(segment_top(tid)) && (tid + 1 == kSegments || !heavy_one(segment_top(tid + 1)))) s.owner = tid;
+    if (tid < kSegments && heavy_one(segment_top(tid), far) && (tid + 1 == kSegments || !heavy_one(segment_top(tid + 1), far))) s.owner = tid;
     __syncthreads();
     if (tid < 32) {
       const int g = s.owner, d = bin_in(g, lane), c = bin_count(d);
-      const int n = __reduce_add_sync(0xffffffffu, c && d < kBins - 1 && heavy_one(key_value(value_of(d))) ? c : 0);
+      const int n = __reduce_add_sync(0xffffffffu, c && d < kBins - 1 && heavy_one(key_value(value_of(d)), far) ? c : 0);
       if (lane == 0) s.found_c = s.seg_c[g] + n;
     }
     __syncthreads();
@@ -616,7 +626,7 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
   u64* mass = reinterpret_cast<u64*>(dyn);
   int* count = reinterpret_cast<int*>(dyn + (F32 ? kTable * sizeof(u64) : 0));
   int* all_count = count + (kTable + 3) / 4 * 4;
-  const int share = TEAM ? (kSegments + team - 1) / team * 32 : 0;
+  const int room = TEAM ? team_room(team, F32) : kSegments, share = TEAM ? room * 32 : 0;
   u64* all_mass = reinterpret_cast<u64*>(all_count + share);
   short* tile_max = reinterpret_cast<short*>(all_count + share + (F32 ? 2 * share : 0));
   pdl_wait();
@@ -626,7 +636,7 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
   const float temp = p.temperature ? p.temperature[r] : 0.f;
   const bool greedy = !(temp > 0.f);
   const double t = greedy ? 1.0 : static_cast<double>(temp);
-  Vocab<F32, TEAM> f{VocabRow<F32>(p, r, rank, team), s, count, mass, all_count, all_mass, tile_max, rank, team, kUsualBase, false, 0ull, 0.f, 1.0 / t};
+  Vocab<F32, TEAM> f{VocabRow<F32>(p, r, rank, team), s, count, mass, all_count, all_mass, tile_max, rank, team, room, kUsualBase, false, 0ull, 0.f, 1.0 / t};
   f.turn = 0;
   if (tid == 0) s.owner = 0;
   if (!greedy) f.clear();
@@ -752,12 +762,13 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
       const double least = fmin(static_cast<double>(mp), 1.0);
       int c = 0;
       if (F32 || f.mixed) {
+        const double far = log(least);
         for (int v = f.row.from + tid; v < f.row.to; v += kVocabThreads) {
           uint32_t u[8];
           const uint32_t ok = f.row.load(v, u);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (ok >> j & 1) c += f.weight(sort_key(u[j])) >= least;
+            if (ok >> j & 1) c += f.heavy_one(__uint_as_float(u[j]), far);
         }
         c = f.block_sum(c);
         f.meet();
@@ -894,7 +905,7 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
 
 template <bool F32, bool TEAM>
 static cudaError_t vocabulary_launch(const CbVocabulary& p, int team, cudaStream_t stream) {
-  const int share = TEAM ? (kSegments + team - 1) / team * 32 : 0, tiles = p.vocab / (256 * team) + 3;
+  const int share = TEAM ? team_room(team, F32) * 32 : 0, tiles = p.vocab / (256 * team) + 3;
   const int smem = ((kTable + 3) / 4 * 4 + share) * 4 + (F32 ? (kTable + share) * 8 : tiles * 2);
   static int ready[64] = {};
   int dev = 0;
@@ -912,7 +923,7 @@ static cudaError_t vocabulary_launch(const CbVocabulary& p, int team, cudaStream
 
 extern "C" int cb_sample_vocabulary(const CbVocabulary* p, void* stream) {
   using namespace cb;
-  if (p->rows < 0 || p->vocab < 1 || p->vocab > kVocabMax || p->ld < p->vocab || (p->mask && p->ld_mask * 32 < p->vocab)) return -10;
+  if (p->rows < 0 || p->vocab < 1 || p->vocab > kVocabMax || p->ld < p->vocab || (p->mask && p->ld_mask < 0)) return -10;
   if (reinterpret_cast<uintptr_t>(p->logits) % (p->f32 ? 4 : 2)) return -11;
   if (p->rows == 0) return 0;
   // CTAs of a row: as many as find room at once, with work for each

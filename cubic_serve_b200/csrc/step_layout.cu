@@ -188,7 +188,6 @@ extern "C" int cb_step_layout(const CbStepLayout* p, void* stream) {
   using namespace cb;
   if (p->cap_tokens > kLayoutMost / 2 || p->cap_blocks > kLayoutMost / 2 || p->num_pages > kLayoutMost / 2) return -11;
   if (p->n < 0 || p->n > kLayoutMaxRequests || p->block < 1 || p->pad > p->cap_tokens || p->pad > p->cap_blocks || p->ld < p->width) return -10;
-  if (p->n == 0 && p->pad <= 0) return 0;
   const size_t smem = static_cast<size_t>(6 * p->n + 3) * sizeof(int);
   static bool wide[64] = {};
   int dev = 0;

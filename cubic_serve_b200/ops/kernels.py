@@ -901,7 +901,7 @@ def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, rows: Adapt
     _require(bank.sections * bank.rank <= rows.max_ranks, "more ranks than the sorted rows have room for")
     ldx, ldy, ldo = (x.stride(0), y.stride(0), out.stride(0)) if t > 1 else (bank.k, bank.n, bank.n)
     px, py, po = x.data_ptr(), y.data_ptr(), out.data_ptr()
-    _require(py != po or ldy == ldo, "y and out are the same rows or other memory")
+    _require((py != po or ldy == ldo) and (px != po or t == 0), "y and out are the same rows or other memory, x and out other memory")
     _require(x.stride(1) == 1 and y.stride(1) == 1 and out.stride(1) == 1 and ldx >= bank.k and ldy >= bank.n and ldo >= bank.n and (ldx | ldy | ldo) % 8 == 0 and max(ldy, ldo) <= 1 << 30 and (px | py | po) % 16 == 0,
              "rows of neighbouring elements at a stride of a multiple of 8, from a 16-byte boundary")
     packed = native.ADAPTER.pack(px, ldx, py, ldy, po, ldo, *bank._at, *rows._at, t, *bank._shape)
@@ -933,7 +933,8 @@ def sample_vocabulary(logits: torch.Tensor, out_ids: torch.Tensor, temperature: 
     ld_mask = 0
     if mask is not None:
         _require(mask.dtype == torch.int32 and mask.dim() == 2 and mask.shape[0] >= n and mask.shape[1] * 32 >= vocab and mask.stride(1) == 1, "mask: int32 words of 32 tokens for every row")
-        ld_mask = max(mask.stride(0), mask.shape[1])
+        ld_mask = mask.stride(0)                                    # 0: one mask for all rows
+    _require(temperature is None or uniforms is not None or seeds is not None, "a draw needs uniforms, or seeds")
     i32, i64 = torch.int32, torch.int64
     packed = native.VOCABULARY.pack(
         logits.data_ptr(), ld, 0 if mask is None else mask.data_ptr(), ld_mask, _vector(temperature, f32, n, "temperature"),

@@ -60,6 +60,7 @@ def _lay(n, most_start, most_count, block, pad=0, seed=0, width_extra=0, extra_p
     wide = torch.full((rows, width + 5), -7, dtype=I32, device=DEV)                          # a table inside a wider one
     wide[:, :width] = cu(table)
     lay = K.StepLayout(max(t, pad) + 11, min(n + 2, 4096), max(b, pad) + 11, DEV)
+    lay.totals.fill_(-77)
     for k in want:
         getattr(lay, k).fill_(-77)
     K.step_layout(cu(req), cu(start), cu(count), cu(held) if known else None, cu(pages), wide[:, :width], lay, block, tokens=t, blocks=b, pad=pad)
@@ -83,6 +84,7 @@ def test_layout_equals_the_plain_form(n, start, count, block, pad):
 def test_layout_takes_held_from_the_lengths_and_leaves_pages_over():
     _lay(9, 200, 90, 4, seed=5, known=False, extra_pages=4, width_extra=2)
     _lay(0, 0, 0, 4, pad=4)
+    _lay(0, 0, 0, 4, pad=0)
 
 
 def test_layout_refuses_on_the_device_what_it_cannot_place():
@@ -394,6 +396,7 @@ def test_draws_under_masks(dtype, vocab):
     wide = torch.zeros(rows, words + 3, dtype=I32, device=DEV)
     wide[:, 2:2 + words] = mask
     _check_draw(x, u=0.61, mask=wide[:, 2:2 + words], p=0.9)
+    _check_draw(x, u=0.61, mask=mask[5:].expand(rows, words), p=0.9)         # one mask for all rows
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -405,6 +408,22 @@ def test_draws_of_rows_at_any_address(dtype):
         view.copy_(_logits(5, 3001, dtype, off))
         _check_draw(view, u=[0.1, 0.3, 0.5, 0.7, 0.9], k=[0, 40, 0, 0, 7], p=[1.0, 1.0, 0.8, 0.99, 1.0])
         wide.fill_(90.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 18, 37, 38, 74, 75, 149])
+@pytest.mark.parametrize("vocab", [8192, 16400, 32801])
+def test_draws_of_any_number_of_rows(dtype, rows, vocab):
+    """Rows are shared by one, two, four and eight blocks, by how many there are and how long: every way draws the same."""
+    x = _logits(rows, vocab, dtype, rows + vocab)
+    x[1:] = x[:1]                                                              # equal rows draw the same for the same number
+    one = torch.ones(rows, device=DEV)
+    ids, alone = torch.full((rows,), -1, dtype=I32, device=DEV), torch.full((1,), -1, dtype=I32, device=DEV)
+    for u in (0.03, 0.4, 0.97):
+        K.sample_vocabulary(x, ids, one, top_p=one * 0.97, min_p=one * 1e-4, uniforms=one * u)
+        K.sample_vocabulary(x[:1], alone, one, top_p=one * 0.97, min_p=one * 1e-4, uniforms=one * u)
+        assert ids.eq(alone).all()
+    _check_draw(x[:2], k=300, p=0.9, m=0.01, u=0.37)
 
 
 def test_draws_with_narrow_bins():

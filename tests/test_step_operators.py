@@ -112,3 +112,17 @@ def test_sample_vocabulary_refuses(change):
     a.update(change)
     with pytest.raises(ValueError):
         K.sample_vocabulary(**a)
+
+
+def test_calls_that_would_mean_something_else_are_refused():
+    """A product that reads what it has written already; a draw without a number to draw with."""
+    square = K.AdapterBank(torch.zeros(2, 16, 64).bfloat16(), torch.zeros(2, 64, 16).bfloat16(), torch.ones(2))
+    rows = K.AdapterRows(4, 2, 16, "cpu")
+    rows.rows = 4
+    x, y = torch.zeros(4, 64).bfloat16(), torch.zeros(4, 64).bfloat16()
+    with pytest.raises(ValueError, match="other memory"):
+        K.adapter_add(x, x, square, rows)
+    with pytest.raises(ValueError, match="other memory"):
+        K.adapter_add(x, y, square, rows, out=x)
+    with pytest.raises(ValueError, match="needs uniforms, or seeds"):
+        K.sample_vocabulary(torch.zeros(2, 9), _ints(2), torch.ones(2))
