@@ -48,8 +48,9 @@ static constexpr float kLeastMinP = 8.6736174e-19f;        // 2^-60: less is as 
 static constexpr int kUsualBase = ((127 - 32) << 7) - 1;
 static_assert(kSegments <= kVocabThreads, "a thread holds the sums before a segment");
 
-// Segments of a CTA of several that are added up at a time: all of its own, but no more than find room beside a table with masses.
-__host__ __device__ constexpr int team_room(int team, bool f32) { return f32 && team < 4 ? (kSegments + 3) / 4 : (kSegments + team - 1) / team; }
+// Places 1 to 32, 33 to 64, ... of either side are a segment: they start on 16 bytes.
+static constexpr int kCountAt = 3, kMassAt = 1, kCountRoom = (kCountAt + kTable + 3) / 4 * 4, kMassRoom = (kMassAt + kTable + 1) / 2 * 2;
+static constexpr int kFew = 256;                           // tokens of a bin that are ranked one against the other
 
 __device__ __forceinline__ uint32_t sort_key(uint32_t u) {                 // order of the values; both zeros are one
   if ((u << 1) == 0) return 0x80000000u;
@@ -83,6 +84,11 @@ __device__ __forceinline__ uint32_t ld_peer(uint32_t addr) {
 __device__ __forceinline__ u64 ld_peer64(uint32_t addr) {
   u64 v;
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 ld_peer128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
 __device__ __forceinline__ void st_peer64(uint32_t addr, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory"); }
@@ -170,7 +176,8 @@ struct VocabScratch {
   u64 sum_m[kVocabWarps]; int sum_c[kVocabWarps];
   uint32_t warp_top[kVocabWarps];
   int owner;
-  u64 sub_m[2][256]; int sub_c[2][256];             // a bin divided; two, for the peers may still read one
+  u64 sub_m[2][256]; __align__(16) int sub_c[2][256];            // a bin divided, or its tokens; two, for the peers may still read one
+  int few[2];
   u64 part_m[256]; int part_c[256];                 // the same of all CTAs
   u64 found_m; int found_c, found_ties, found_at;
 };
@@ -179,10 +186,9 @@ template <bool F32, bool TEAM>
 struct Vocab {
   VocabRow<F32> row;
   VocabScratch& s;
-  int* count; u64* mass;                        // the table of the CTA's own tokens
-  int* all_count; u64* all_mass;                // TEAM: of the row, the CTA's share of the segments
+  int* count; u64* mass;                        // the table of the CTA's own tokens; in the segments that are its, once they are merged, of the row's
   short* tile_max;                              // bf16: largest of every 256 tokens as a signed 16-bit number: exact where it is not negative
-  int rank, team, room, base;
+  int rank, team, base;
   bool mixed;                                   // bf16: the bin of zero holds other values
   u64 zero_mass;
   float best;
@@ -233,9 +239,12 @@ struct Vocab {
     for (int r = 0; r < kTeamMax; ++r) m += v[r];
     return m;
   }
-  __device__ __forceinline__ int bin_count(int d) const {
+  // What the table holds of a segment's bin, once merged: TEAM: at the CTA that the segment belongs to.
+  __device__ __forceinline__ int merged(const int* t, int g, int i) const { return TEAM ? static_cast<int>(ld_peer(cluster_map(smem_u32(t + i), g % team))) : t[i]; }
+  __device__ __forceinline__ u64 merged(const u64* t, int g, int i) const { return TEAM ? ld_peer64(cluster_map(smem_u32(t + i), g % team)) : t[i]; }
+  __device__ __forceinline__ int bin_count(int g, int d) const {
     if (d >= kBins) return 0;
-    return at(count, place_of_bin(d)) + (d == kZero ? at(count, kNegative) : 0);
+    return merged(count, g, place_of_bin(d)) + (d == kZero ? merged(count, g, kNegative) : 0);
   }
   // The values of a segment's bins fall by the same step of 2^(exponent - 7): their weights are the first one's times powers of one ratio.  387 + 49 exponentials
   // a row, a thread each, in place of one a bin.  In the segment of the best value the weights start from it.
@@ -267,7 +276,7 @@ struct Vocab {
   // mass of the bin of a segment's lane that holds c tokens
   __device__ __forceinline__ u64 lane_mass(int g, int lane, int c) const {
     const int d = bin_in(g, lane);
-    if (F32) return c == 0 ? 0ull : at(mass, place_of_bin(d)) + (d == kZero ? at(mass, kNegative) : 0ull);
+    if (F32) return d >= kBins ? 0ull : merged(mass, g, place_of_bin(d)) + (d == kZero ? merged(mass, g, kNegative) : 0ull);
     if (g == kSegments - 1) return 0;
     if (g == kZeroSegment && mixed) return c ? zero_mass : 0ull;
     double w = s.seg_w[g];
@@ -289,8 +298,8 @@ struct Vocab {
     return c ? static_cast<u64>(__double2ll_rn(c * (w * kUnit))) : 0ull;
   }
 
-  // A thread's segment; TEAM: its bins added up from `bins` on.
-  __device__ __forceinline__ void segment_sum(int g, int bins) {
+  // A thread's segment.
+  __device__ __forceinline__ void segment_sum(int g) {
     const int lane = threadIdx.x & 31;
     const bool one = bin_in(g, 1) >= kBins;                      // a segment of one bin
     int from = 0, n = 0;
@@ -316,15 +325,15 @@ struct Vocab {
     }
     const int d0 = bin_in(g, 0), place = place_of_bin(d0), step = d0 < kZero ? -1 : 1;
     if (one) {
-      n = TEAM ? all_count[bins] : bin_count(d0);
-      m = F32 ? (TEAM ? all_mass[bins] : lane_mass(g, 0, n)) : lane_mass(g, 0, n);
+      n = bin_count(g, d0);
+      m = lane_mass(g, 0, n);
     } else {
 #pragma unroll 8
       for (int i = 0; i < 32; ++i) {
-        const int l = (i + lane) & 31, c = TEAM ? all_count[bins + l] : count[place + step * l];
+        const int l = (i + lane) & 31, c = count[place + step * l];
         n += c;
         if (F32) {
-          m += TEAM ? all_mass[bins + l] : mass[place + step * l];
+          m += mass[place + step * l];
         } else {
           if (c) m += static_cast<u64>(__double2ll_rn(c * (w * kUnit)));
           w = ((l + 1) & 31) == from ? w0 : l == 31 ? 0.0 : w * q;
@@ -342,24 +351,49 @@ struct Vocab {
     }
   }
 
+  // TEAM: the CTA adds the peers' tables to its own in every team-th segment, 16 bytes a load; the peers read nothing of these.
+  template <typename V>
+  __device__ __forceinline__ void merge(V* table) {
+    constexpr int E = 16 / sizeof(V), L = 32 / E, P = 32 / L;                  // entries of a load, lanes of a segment, segments of a warp
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i0 = warp * P; i0 * team + rank < kSegments; i0 += kVocabWarps * P) {
+      const int g = (i0 + lane / L) * team + rank;
+      if (g >= kSegments) continue;
+      const int d0 = bin_in(g, 0);
+      if (bin_in(g, 1) < kBins) {
+        V* own = table + (d0 < kZero ? place_of_bin(d0) - 31 : place_of_bin(d0)) + lane % L * E;
+        uint4 q[kTeamMax - 1];
+#pragma unroll
+        for (int r = 1; r < kTeamMax; ++r) {
+          q[r - 1] = make_uint4(0, 0, 0, 0);
+          if (r < team) q[r - 1] = ld_peer128(cluster_map(smem_u32(own), (rank + r) & (team - 1)));
+        }
+        V v[E];
+        *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(own);
+#pragma unroll
+        for (int r = 1; r < kTeamMax; ++r) {
+          const V* o = reinterpret_cast<const V*>(&q[r - 1]);
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[e] += o[e];
+        }
+        *reinterpret_cast<uint4*>(own) = *reinterpret_cast<const uint4*>(v);
+      } else if (lane % L < (d0 == kZero ? 2 : 1)) {                           // a segment of one bin, two places for that of zero
+        V* own = table + (lane % L ? kNegative : place_of_bin(d0));
+        *own = at(own, 0);
+      }
+    }
+  }
   // Sums of the segments, then those before each.  A thread takes a segment, from the bin of its lane on, so that 32 threads are at 32 banks; a CTA of several
-  // takes every team-th segment, `room` of them at a time, once the bins of all have been added up.
+  // takes every team-th segment.
   __device__ void sums(int& total_c, u64& total_m) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    weigh_segments();
-    for (int from_i = 0; from_i * team + rank < kSegments; from_i += room) {
-      if (TEAM) {
-        if (from_i) __syncthreads();
-#pragma unroll 2
-        for (int i = from_i + warp; i < from_i + room && i * team + rank < kSegments; i += kVocabWarps) {
-          const int d = bin_in(i * team + rank, lane), to = (i - from_i) * 32 + lane;
-          all_count[to] = bin_count(d);
-          if (F32) all_mass[to] = d >= kBins ? 0ull : at(mass, place_of_bin(d)) + (d == kZero ? at(mass, kNegative) : 0ull);
-        }
-        __syncthreads();
-      }
-      if (tid >= from_i && tid < from_i + room && tid * team + rank < kSegments) segment_sum(tid * team + rank, (tid - from_i) * 32);
+    if (TEAM) {
+      merge(count);
+      if (F32) merge(mass);
+      __syncthreads();
     }
+    weigh_segments();
+    if (tid * team + rank < kSegments) segment_sum(tid * team + rank);
     meet();
     const int own_c = tid < kSegments ? s.seg_c[tid] : 0;
     const u64 own_m = tid < kSegments ? s.seg_m[tid] : 0ull;
@@ -394,7 +428,7 @@ struct Vocab {
     if (by_mass ? pre_m < want && want <= end_m : static_cast<u64>(pre_c) < want && want <= static_cast<u64>(end_c)) s.owner = tid;
     __syncthreads();
     if (tid < 32) {
-      const int g = s.owner, own_c = bin_count(bin_in(g, lane));
+      const int g = s.owner, own_c = bin_count(g, bin_in(g, lane));
       settle(by_mass, want, own_c, lane_mass(g, lane, own_c), s.seg_c[g], s.seg_m[g]);
       if (lane == 0) s.found_at = bin_in(g, s.found_at);
     }
@@ -432,17 +466,78 @@ struct Vocab {
     if (tid < kSegments && heavy_one(segment_top(tid), far) && (tid + 1 == kSegments || !heavy_one(segment_top(tid + 1), far))) s.owner = tid;
     __syncthreads();
     if (tid < 32) {
-      const int g = s.owner, d = bin_in(g, lane), c = bin_count(d);
+      const int g = s.owner, d = bin_in(g, lane), c = bin_count(g, d);
       const int n = __reduce_add_sync(0xffffffffu, c && d < kBins - 1 && heavy_one(key_value(value_of(d)), far) ? c : 0);
       if (lane == 0) s.found_c = s.seg_c[g] + n;
     }
     __syncthreads();
     return s.found_c;
   }
+  // Up to kFew tokens from lo to hi: every CTA gets them all, a thread each, and adds up those that come before its own.
+  __device__ void settle_few(bool by_mass, u64 want) {
+    const int tid = threadIdx.x;
+    int* few = &s.few[turn];
+    uint32_t* list = reinterpret_cast<uint32_t*>(s.sub_c[turn]);
+    turn ^= 1;
+    __syncthreads();
+    if (tid == 0) *few = 0;
+    __syncthreads();
+    for (int v = row.from + tid; v < row.to; v += kVocabThreads) {
+      uint32_t u[8];
+      const uint32_t ok = row.load(v, u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t k = sort_key(u[j]);
+        if (!(ok >> j & 1) || k < lo || k > hi) continue;
+        const int at = atomicAdd(few, 1);
+        if (at < kFew) list[at] = k;
+      }
+    }
+    meet();
+    uint32_t key = 0;
+    u64 own = 0;
+    if (tid < ties) {
+      int r = 0, i = tid;
+      if (TEAM) {
+        uint32_t n[kTeamMax];
+#pragma unroll
+        for (int q = 0; q < kTeamMax; ++q) n[q] = q < team ? ld_peer(cluster_map(smem_u32(few), q)) : 0u;
+#pragma unroll
+        for (int q = 0; q + 1 < kTeamMax; ++q)
+          if (r == q && i >= static_cast<int>(n[q])) { i -= n[q]; ++r; }
+      }
+      key = TEAM ? ld_peer(cluster_map(smem_u32(list + i), min(r, team - 1))) : list[i];
+      own = units(key);
+      s.part_c[tid] = static_cast<int>(key);
+      s.part_m[tid] = own;
+    }
+    __syncthreads();
+    if (tid < ties) {
+      int c = 0, same = 0;
+      u64 m = 0;
+#pragma unroll 4
+      for (int j = 0; j < ties; ++j) {
+        const uint32_t o = static_cast<uint32_t>(s.part_c[j]);
+        const u64 w = s.part_m[j];
+        if (o > key) { ++c; m += w; }
+        same += o == key;
+      }
+      const bool last = c + same == ties;
+      c += before_c;
+      m += before_m;
+      if (by_mass ? m < want && (last || want <= m + same * own) : static_cast<u64>(c) < want && (last || want <= static_cast<u64>(c + same))) {
+        s.found_c = c; s.found_m = m; s.found_ties = same; s.found_at = static_cast<int>(key);
+      }
+    }
+    __syncthreads();
+    before_c = s.found_c; before_m = s.found_m; ties = s.found_ties;
+    lo = hi = static_cast<uint32_t>(s.found_at);
+  }
   // Divides what a search ended in until it is one value.
   __device__ void divide(bool by_mass, u64 want) {
     const int tid = threadIdx.x, lane = tid & 31;
     while (lo != hi) {
+      if (ties <= kFew) return settle_few(by_mass, want);
       const int shift = max(0, 24 - __clz(hi - lo));
       u64* sub_m = s.sub_m[turn];
       int* sub_c = s.sub_c[turn];
@@ -491,10 +586,12 @@ struct Vocab {
   __device__ __forceinline__ u64 mass_of(int prefix) const { return before_m + static_cast<u64>(__double2ll_rn((prefix - before_c) * found_weight())); }
 
   __device__ __forceinline__ void clear() {
-    uint4* t = reinterpret_cast<uint4*>(count);
-    for (int i = threadIdx.x; i < (kTable + 3) / 4; i += kVocabThreads) t[i] = make_uint4(0, 0, 0, 0);
-    if (F32)
-      for (int i = threadIdx.x; i < kTable; i += kVocabThreads) mass[i] = 0;
+    uint4* t = reinterpret_cast<uint4*>(count - kCountAt);
+    for (int i = threadIdx.x; i < kCountRoom / 4; i += kVocabThreads) t[i] = make_uint4(0, 0, 0, 0);
+    if (F32) {
+      t = reinterpret_cast<uint4*>(mass - kMassAt);
+      for (int i = threadIdx.x; i < kMassRoom / 2; i += kVocabThreads) t[i] = make_uint4(0, 0, 0, 0);
+    }
   }
   __device__ __forceinline__ uint32_t block_max(uint32_t v) {
     v = __reduce_max_sync(0xffffffffu, v);
@@ -622,13 +719,10 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (!TEAM) team = 1;
   const int rank = TEAM ? static_cast<int>(cluster_ctarank()) : 0, n_row = blockIdx.x / team;
-  // the masses, the counts, a share of the row's of both, the tiles
-  u64* mass = reinterpret_cast<u64*>(dyn);
-  int* count = reinterpret_cast<int*>(dyn + (F32 ? kTable * sizeof(u64) : 0));
-  int* all_count = count + (kTable + 3) / 4 * 4;
-  const int room = TEAM ? team_room(team, F32) : kSegments, share = TEAM ? room * 32 : 0;
-  u64* all_mass = reinterpret_cast<u64*>(all_count + share);
-  short* tile_max = reinterpret_cast<short*>(all_count + share + (F32 ? 2 * share : 0));
+  // the masses, the counts, the tiles
+  u64* mass = reinterpret_cast<u64*>(dyn) + kMassAt;
+  int* count = reinterpret_cast<int*>(dyn + (F32 ? kMassRoom * sizeof(u64) : 0)) + kCountAt;
+  short* tile_max = reinterpret_cast<short*>(count - kCountAt + kCountRoom);
   pdl_wait();
   pdl_launch_dependents();
   const int r = p.rows_of ? p.rows_of[n_row] : n_row;
@@ -636,7 +730,7 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
   const float temp = p.temperature ? p.temperature[r] : 0.f;
   const bool greedy = !(temp > 0.f);
   const double t = greedy ? 1.0 : static_cast<double>(temp);
-  Vocab<F32, TEAM> f{VocabRow<F32>(p, r, rank, team), s, count, mass, all_count, all_mass, tile_max, rank, team, room, kUsualBase, false, 0ull, 0.f, 1.0 / t};
+  Vocab<F32, TEAM> f{VocabRow<F32>(p, r, rank, team), s, count, mass, tile_max, rank, team, kUsualBase, false, 0ull, 0.f, 1.0 / t};
   f.turn = 0;
   if (tid == 0) s.owner = 0;
   if (!greedy) f.clear();
@@ -707,7 +801,7 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
   uint32_t pick_key = best_key;
   int pick = 0;                                  // which of the tokens of that value, by id
   if (!greedy) {
-    if (f.mixed && f.bin_count(kZero) == 0) f.mixed = false;
+    if (f.mixed && f.at(count, 0) + f.at(count, kNegative) == 0) f.mixed = false;
     if (f.mixed) {
       u64 m = 0;
       int other = 0;
@@ -905,8 +999,7 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
 
 template <bool F32, bool TEAM>
 static cudaError_t vocabulary_launch(const CbVocabulary& p, int team, cudaStream_t stream) {
-  const int share = TEAM ? team_room(team, F32) * 32 : 0, tiles = p.vocab / (256 * team) + 3;
-  const int smem = ((kTable + 3) / 4 * 4 + share) * 4 + (F32 ? (kTable + share) * 8 : tiles * 2);
+  const int smem = kCountRoom * 4 + (F32 ? kMassRoom * 8 : (p.vocab / (256 * team) + 3) * 2);
   static int ready[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
