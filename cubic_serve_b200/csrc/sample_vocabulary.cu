@@ -33,7 +33,8 @@ namespace cb {
 
 typedef unsigned long long u64;
 
-static constexpr int kVocabThreads = 512, kVocabWarps = kVocabThreads / 32;
+template <bool F32> constexpr int kThreadsOf = F32 ? 1024 : 512;
+static constexpr int kVocabMostWarps = 32;
 static constexpr int kVocabMax = 1 << 20;
 static constexpr int kTeamMax = 8;                         // CTAs of a row
 static constexpr int kSpan = 48 * 128;                     // bins of a sign; one more at the end for what is larger
@@ -46,7 +47,7 @@ static constexpr int kSideSegments = kSpan / 32, kZeroSegment = kSideSegments + 
 static constexpr double kUnit = 4398046511104.0;           // 2^42
 static constexpr float kLeastMinP = 8.6736174e-19f;        // 2^-60: less is as good as none
 static constexpr int kUsualBase = ((127 - 32) << 7) - 1;
-static_assert(kSegments <= kVocabThreads, "a thread holds the sums before a segment");
+static_assert(kSegments <= kThreadsOf<false>, "a thread holds the sums before a segment");
 
 // Places 1 to 32, 33 to 64, ... of either side are a segment: they start on 16 bytes.
 static constexpr int kCountAt = 3, kMassAt = 1, kCountRoom = (kCountAt + kTable + 3) / 4 * 4, kMassRoom = (kMassAt + kTable + 1) / 2 * 2;
@@ -100,6 +101,9 @@ __device__ __forceinline__ void add_shared(u64* at, u64 v) {
   if (hi) atomicAdd(half + 1, hi);
 }
 
+// Can be drawn: more than -inf.
+__device__ __forceinline__ bool is_more(uint32_t u) { return __uint_as_float(u) > -INFINITY; }
+
 // A CTA's share of a row's tokens, eight neighbours at a time from a 16-byte boundary.
 template <bool F32>
 struct VocabRow {
@@ -128,21 +132,19 @@ struct VocabRow {
     const int i = first(v), w = i >> 5;
     return __funnelshift_r(word(w), (i & 31) > 24 ? word(w + 1) : 0u, i & 31) & 0xffu;
   }
-  // the bits of the values, and which of them count: tokens of the row that the mask allows and that are more than -inf
-  __device__ __forceinline__ uint32_t load(int v, uint32_t (&u)[8]) const {
+  // a vector in two steps, so that several are on their way: its bytes, if it has any that count and lies in the row, then
+  // the bits of the values, and which of them are tokens of the row that the mask allows
+  __device__ __forceinline__ void fetch(int v, uint32_t ok, uint4& a, uint4& b) const {
+    if (ok == 0 || !whole(v)) return;
+    a = reinterpret_cast<const uint4*>(base)[F32 ? v * 2 : v];
+    if (F32) b = reinterpret_cast<const uint4*>(base)[v * 2 + 1];
+  }
+  __device__ __forceinline__ uint32_t values(int v, uint32_t ok, const uint4& a, const uint4& b, uint32_t (&u)[8]) const {
     const int i = first(v);
-    uint32_t ok = allowed(v);
-    if (ok == 0) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = 0u;
-      return 0u;
-    }
-    if (i >= 0 && i + 8 <= vocab) {
+    if (whole(v)) {
       if (F32) {
-        const uint4 a = reinterpret_cast<const uint4*>(base)[v * 2], b = reinterpret_cast<const uint4*>(base)[v * 2 + 1];
         u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w; u[4] = b.x; u[5] = b.y; u[6] = b.z; u[7] = b.w;
       } else {
-        const uint4 a = reinterpret_cast<const uint4*>(base)[v];
         u[0] = a.x << 16; u[1] = a.x & 0xffff0000u; u[2] = a.y << 16; u[3] = a.y & 0xffff0000u;
         u[4] = a.z << 16; u[5] = a.z & 0xffff0000u; u[6] = a.w << 16; u[7] = a.w & 0xffff0000u;
       }
@@ -154,10 +156,27 @@ struct VocabRow {
         u[j] = !in ? 0u : F32 ? reinterpret_cast<const uint32_t*>(base)[v * 8 + j] : static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(base)[v * 8 + j]) << 16;
       }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if ((u[j] & 0x7fffffffu) > 0x7f800000u || u[j] == 0xff800000u) ok &= ~(1u << j);
     return ok;
+  }
+  // fn(values, which of them are allowed) of the CTA's vectors, U of a thread on their way at a time
+  template <int U, typename Fn>
+  __device__ __forceinline__ void each(Fn fn) const {
+    constexpr int T = kThreadsOf<F32>;
+    for (int v0 = from + threadIdx.x; v0 < to; v0 += U * T) {
+      uint4 a[U], b[U];
+      uint32_t ok[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) ok[k] = v0 + k * T < to ? allowed(v0 + k * T) : 0u;
+#pragma unroll
+      for (int k = 0; k < U; ++k) fetch(v0 + k * T, ok[k], a[k], b[k]);
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (ok[k] == 0) continue;
+        uint32_t u[8];
+        const uint32_t in = values(v0 + k * T, ok[k], a[k], b[k], u);
+        fn(u, in);
+      }
+    }
   }
 };
 
@@ -173,8 +192,8 @@ struct VocabScratch {
   VocabTold told;
   u64 seg_m[kSegments]; int seg_c[kSegments];       // of the row: sums of a segment, then those before it
   double seg_w[kSegments], ratio[49];               // weight of a segment's first bin; of neighbouring bins of an exponent, one to the other
-  u64 sum_m[kVocabWarps]; int sum_c[kVocabWarps];
-  uint32_t warp_top[kVocabWarps];
+  u64 sum_m[kVocabMostWarps]; int sum_c[kVocabMostWarps];
+  uint32_t warp_top[kVocabMostWarps];
   int owner;
   u64 sub_m[2][256]; __align__(16) int sub_c[2][256];            // a bin divided, or its tokens; two, for the peers may still read one
   int few[2];
@@ -184,6 +203,7 @@ struct VocabScratch {
 
 template <bool F32, bool TEAM>
 struct Vocab {
+  static constexpr int kVocabThreads = kThreadsOf<F32>, kVocabWarps = kVocabThreads / 32, kAhead = F32 ? 2 : 4;      // vectors of a thread on their way
   VocabRow<F32> row;
   VocabScratch& s;
   int* count; u64* mass;                        // the table of the CTA's own tokens; in the segments that are its, once they are merged, of the row's
@@ -482,17 +502,18 @@ struct Vocab {
     __syncthreads();
     if (tid == 0) *few = 0;
     __syncthreads();
-    for (int v = row.from + tid; v < row.to; v += kVocabThreads) {
-      uint32_t u[8];
-      const uint32_t ok = row.load(v, u);
+    const float least = key_value(max(lo, 0x007fffffu)), most = key_value(min(hi, 0xff800000u));       // the bin of an infinity reaches behind it
+    row.template each<kAhead>([&](const uint32_t (&u)[8], uint32_t ok) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t k = sort_key(u[j]);
-        if (!(ok >> j & 1) || k < lo || k > hi) continue;
+        const float v = __uint_as_float(u[j]);
+        if (!(v >= least && v <= most)) continue;
+        const uint32_t k = sort_key(u[j]);                                     // the keys tell a range that ends below zero from one with it
+        if (!(ok >> j & 1) || !is_more(u[j]) || k < lo || k > hi) continue;
         const int at = atomicAdd(few, 1);
         if (at < kFew) list[at] = k;
       }
-    }
+    });
     meet();
     uint32_t key = 0;
     u64 own = 0;
@@ -545,17 +566,15 @@ struct Vocab {
       __syncthreads();
       for (int i = tid; i < 256; i += kVocabThreads) { sub_c[i] = 0; sub_m[i] = 0; }
       __syncthreads();
-      for (int v = row.from + tid; v < row.to; v += kVocabThreads) {
-        uint32_t u[8];
-        const uint32_t ok = row.load(v, u);
+      row.template each<2>([&](const uint32_t (&u)[8], uint32_t ok) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const uint32_t k = sort_key(u[j]);
-          if (!(ok >> j & 1) || k < lo || k > hi) continue;
+          if (!(ok >> j & 1) || !is_more(u[j]) || k < lo || k > hi) continue;
           atomicAdd(&sub_c[(k - lo) >> shift], 1);
           add_shared(&sub_m[(k - lo) >> shift], units(k));
         }
-      }
+      });
       meet();
       if (tid < 256) { s.part_c[tid] = at(sub_c, 255 - tid); s.part_m[tid] = at(sub_m, 255 - tid); }
       __syncthreads();
@@ -692,28 +711,28 @@ struct Vocab {
     }
     return most;
   }
-  // Any row: the largest key, and the table if `fill`.
-  __device__ __forceinline__ uint32_t look(bool fill, bool with_mass) {
-    uint32_t top = 0;
-#pragma unroll 2
-    for (int v = row.from + threadIdx.x; v < row.to; v += kVocabThreads) {
-      uint32_t u[8];
-      const uint32_t ok = row.load(v, u);
+  // Any row: the largest key, and the table if FILL.
+  template <bool FILL>
+  __device__ __forceinline__ uint32_t look() {
+    float top = -INFINITY;                       // NaN is no maximum
+    row.template each<FILL ? (F32 ? 1 : 2) : kAhead>([&](const uint32_t (&u)[8], uint32_t ok) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (!(ok >> j & 1)) continue;
-        top = max(top, sort_key(u[j]));
-        if (fill) atomicAdd(&count[place_of(u[j], base)], 1);
-        if (fill && with_mass) add_shared(&mass[place_of(u[j], base)], units(sort_key(u[j])));
+        const float v = ok >> j & 1 ? __uint_as_float(u[j]) : -INFINITY;
+        top = fmaxf(top, v);
+        if (!FILL || !(v > -INFINITY)) continue;
+        atomicAdd(&count[place_of(u[j], base)], 1);
+        if (F32) add_shared(&mass[place_of(u[j], base)], units(sort_key(u[j])));
       }
-    }
-    return top;
+    });
+    return top > -INFINITY ? sort_key(__float_as_uint(top)) : 0u;
   }
 };
 
 template <bool F32, bool TEAM>
-__global__ void __launch_bounds__(kVocabThreads, F32 ? 1 : 2)
+__global__ void __launch_bounds__(kThreadsOf<F32>, F32 ? 1 : 2)
 sample_vocabulary_kernel(const CbVocabulary p, int team) {
+  constexpr int kVocabThreads = kThreadsOf<F32>, kVocabWarps = kVocabThreads / 32;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ VocabScratch s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -769,7 +788,7 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
     // a look that knows what counts; in the usual bins at first, which most rows keep
     bool fill = !F32 && !greedy && best_key == 0;
     if (best_key == 0) {
-      const uint32_t top = f.block_max(f.look(fill, false));
+      const uint32_t top = f.block_max(!F32 && fill ? f.template look<!F32>() : f.template look<false>());
       if (tid == 0) f.tell(s.told.zero_m, top);
       f.meet();
       for (int c = 0; c < team; ++c) best_key = max(best_key, static_cast<uint32_t>(s.told.zero_m[c]));
@@ -790,7 +809,7 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
         f.meet();
         if (fill) { f.clear(); __syncthreads(); }
         f.base = base;
-        f.look(true, F32);
+        f.template look<true>();
       }
       f.mixed = !F32;
       f.meet();
@@ -805,17 +824,15 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
     if (f.mixed) {
       u64 m = 0;
       int other = 0;
-      for (int v = f.row.from + tid; v < f.row.to; v += kVocabThreads) {
-        uint32_t u[8];
-        const uint32_t ok = f.row.load(v, u);
+      f.row.template each<2>([&](const uint32_t (&u)[8], uint32_t ok) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int d = place_of(u[j], f.base);
-          if (!(ok >> j & 1) || (d != 0 && d != kNegative)) continue;
+          if (!(ok >> j & 1) || !is_more(u[j]) || (d != 0 && d != kNegative)) continue;
           m += f.units(sort_key(u[j]));
           other |= (u[j] << 1) != 0;
         }
-      }
+      });
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
       const int others = f.block_sum(other);
@@ -856,14 +873,14 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
       const double least = fmin(static_cast<double>(mp), 1.0);
       int c = 0;
       if (F32 || f.mixed) {
-        const double far = log(least);
-        for (int v = f.row.from + tid; v < f.row.to; v += kVocabThreads) {
-          uint32_t u[8];
-          const uint32_t ok = f.row.load(v, u);
+        // most tokens are told by one comparison with a little less than the smallest value that is heavy enough
+        const double far = log(least), edge = f.best + far * t;
+        const float cut = isfinite(edge) ? static_cast<float>(edge - 1e-5 * (fabs(static_cast<double>(f.best)) + fabs(far * t)) - 1e-37) : f.best == INFINITY ? INFINITY : -INFINITY;
+        f.row.template each<f.kAhead>([&](const uint32_t (&u)[8], uint32_t ok) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (ok >> j & 1) c += f.heavy_one(__uint_as_float(u[j]), far);
-        }
+            if ((ok >> j & 1) && __uint_as_float(u[j]) >= cut) c += f.heavy_one(__uint_as_float(u[j]), far);
+        });
         c = f.block_sum(c);
         f.meet();
         if (tid == 0) f.tell(s.told.least, static_cast<u64>(c));
@@ -907,18 +924,14 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
   const int least = static_cast<int>(__float_as_uint(pick_value) >> 16);
   const bool plain = !F32 && !f.row.mask && pick_value != 0.f;
   const uint32_t twice = (__float_as_uint(pick_value) >> 16) * 0x10001u;
-  auto of_tile = [&](int i) {
-    const int v = f.row.from + i * 32 + lane;
-    if (v >= f.row.to) return 0;
-    if (plain && f.row.whole(v)) {
-      const uint4 q = reinterpret_cast<const uint4*>(f.row.base)[v];
-      return (__popc(__vcmpeq2(q.x, twice)) + __popc(__vcmpeq2(q.y, twice)) + __popc(__vcmpeq2(q.z, twice)) + __popc(__vcmpeq2(q.w, twice))) >> 4;
-    }
+  auto of_tile = [&](int v, uint32_t ok, const uint4& a, const uint4& b) {
+    if (ok == 0) return 0;
+    if (plain && f.row.whole(v)) return (__popc(__vcmpeq2(a.x, twice)) + __popc(__vcmpeq2(a.y, twice)) + __popc(__vcmpeq2(a.z, twice)) + __popc(__vcmpeq2(a.w, twice))) >> 4;
     uint32_t u[8];
-    const uint32_t ok = f.row.load(v, u);
+    ok = f.row.values(v, ok, a, b, u);
     int c = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) c += (ok >> j & 1) && sort_key(u[j]) == pick_key;
+    for (int j = 0; j < 8; ++j) c += (ok >> j & 1) && __uint_as_float(u[j]) == pick_value;       // zeros are one
     return c;
   };
   int found = 0;
@@ -928,15 +941,23 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
     uint32_t todo = __ballot_sync(0xffffffffu, mine < tiles && (!some || f.tile_max[mine] >= least));
     __syncwarp();
     while (todo) {
-      constexpr int U = 4;
+      constexpr int U = f.kAhead;
       int i[U], c[U];
+      uint32_t ok[U];
+      uint4 a[U], b[U];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         i[k] = todo ? i0 + (__ffs(todo) - 1) * kVocabWarps : -1;
         todo &= todo - 1;
       }
 #pragma unroll
-      for (int k = 0; k < U; ++k) c[k] = i[k] >= 0 ? of_tile(i[k]) : 0;
+      for (int k = 0; k < U; ++k) {
+        const int v = f.row.from + i[k] * 32 + lane;
+        ok[k] = i[k] >= 0 && v < f.row.to ? f.row.allowed(v) : 0u;
+        f.row.fetch(v, ok[k], a[k], b[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) c[k] = of_tile(f.row.from + i[k] * 32 + lane, ok[k], a[k], b[k]);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         if (!__any_sync(0xffffffffu, c[k])) continue;
@@ -978,11 +999,13 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
   const int v = f.row.from + tile * 32 + lane;
   uint32_t hit = 0;
   if (v < f.row.to) {
-    uint32_t u[8];
-    const uint32_t ok = f.row.load(v, u);
+    uint32_t u[8], ok = f.row.allowed(v);
+    uint4 a, b;
+    f.row.fetch(v, ok, a, b);
+    ok = f.row.values(v, ok, a, b, u);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if ((ok >> j & 1) && sort_key(u[j]) == pick_key) hit |= 1u << j;
+      if ((ok >> j & 1) && __uint_as_float(u[j]) == pick_value) hit |= 1u << j;
   }
   int upto = __popc(hit);
 #pragma unroll
@@ -1009,7 +1032,7 @@ static cudaError_t vocabulary_launch(const CbVocabulary& p, int team, cudaStream
     if (e != cudaSuccess) return e;
     if (dev < 64) ready[dev] = smem;
   }
-  return launch(sample_vocabulary_kernel<F32, TEAM>, dim3(p.rows * team), dim3(kVocabThreads), smem, stream, dim3(team, 1, 1), p, team);
+  return launch(sample_vocabulary_kernel<F32, TEAM>, dim3(p.rows * team), dim3(kThreadsOf<F32>), smem, stream, dim3(team, 1, 1), p, team);
 }
 
 }  // namespace cb
