@@ -371,7 +371,8 @@ struct Vocab {
     }
   }
 
-  // TEAM: the CTA adds the peers' tables to its own in every team-th segment, 16 bytes a load; the peers read nothing of these.
+  // TEAM: the CTA adds the peers' tables to its own in every team-th segment, 16 bytes a load; the peers read nothing of these.  Masses come after the
+  // counts, of bins that hold a token: most do not.
   template <typename V>
   __device__ __forceinline__ void merge(V* table) {
     constexpr int E = 16 / sizeof(V), L = 32 / E, P = 32 / L;                  // entries of a load, lanes of a segment, segments of a warp
@@ -381,7 +382,9 @@ struct Vocab {
       if (g >= kSegments) continue;
       const int d0 = bin_in(g, 0);
       if (bin_in(g, 1) < kBins) {
-        V* own = table + (d0 < kZero ? place_of_bin(d0) - 31 : place_of_bin(d0)) + lane % L * E;
+        const int at0 = (d0 < kZero ? place_of_bin(d0) - 31 : place_of_bin(d0)) + lane % L * E;
+        if (sizeof(V) == 8 && (count[at0] | count[at0 + 1]) == 0) continue;
+        V* own = table + at0;
         uint4 q[kTeamMax - 1];
 #pragma unroll
         for (int r = 1; r < kTeamMax; ++r) {
@@ -409,8 +412,11 @@ struct Vocab {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (TEAM) {
       merge(count);
-      if (F32) merge(mass);
       __syncthreads();
+      if (F32) {
+        merge(mass);
+        __syncthreads();
+      }
     }
     weigh_segments();
     if (tid * team + rank < kSegments) segment_sum(tid * team + rank);
