@@ -3,12 +3,13 @@
 // A projection made of sections (q | k | v, gate | up) has an A of its own for each: A[s] stacks them, and the columns of section j see
 // ranks [j rank, (j + 1) rank).
 //
-// Three kernels.  `adapter_rows_kernel` sorts a step's rows by adapter, once for all projections of all layers.  `adapter_down_kernel`
-// makes h = scale x A^T of the sorted rows, `adapter_up_kernel` adds h B^T.  A work item is up to 16 rows of one adapter in small steps, 64 in large.
+// `adapter_rows_kernel` sorts a step's rows by adapter, once for all projections of all layers.  Up to 512 rows `adapter_few_kernel` makes
+// h = scale x A^T of up to sixteen rows of an adapter and adds h B^T, in one launch.  From there on `adapter_down_tile_kernel` makes h of up to 64 rows and
+// `adapter_up_kernel` adds h B^T to strips of sixteen.
 //
 // Bound by memory: with few rows by A and B of the adapters in use, with many by y and out.  The products run on
 // mma.sync m16n8k16 with operands that go from global memory to registers: rank 16 makes 16 products of every byte of x, far from
-// what would keep tensor memory busy, and a stage of shared memory would add a round trip to a chain of two short kernels.
+// what would keep tensor memory busy.
 #include "ptx.cuh"
 #include "mma.cuh"
 #include "launch.cuh"
@@ -16,7 +17,7 @@
 namespace cb {
 
 // Up to here a work item is sixteen rows and A is streamed through registers, from here on it is 64 and A and x come by tiles.  331 rows over two adapters, a
-// layer: 82 us by tiles, 56 by sixteens.
+// layer: 82 us by tiles, 57 by sixteens.
 static constexpr int kAdapterFewRows = 512;
 static constexpr int adapter_item_rows(int rows) { return rows <= kAdapterFewRows ? 16 : 64; }
 static constexpr int kAdapterMaxSlots = 1023;
@@ -180,6 +181,10 @@ __device__ __forceinline__ void put_h(const CbAdapter& p, float v, float scale, 
 // of 32 along k.  The order of k inside a product is free: a lane's 16 bytes of x and of A are its operands of two products as they lie.  64 ranks
 // at a time, one turn of a warp on its way while another is multiplied.
 // Second product: as in adapter_up_kernel, with h from shared memory and sixteen rows at most.
+//
+// A layer's four projections (4096 -> 6144 of three sections, 4096 -> 4096, 4096 -> 24576 of two, 12288 -> 4096) one after the other: one row of rank 16 takes
+// 27 us (a launch's start, two waits for the cluster and four trips to memory, 6.7 us each), 48 rows over 12 adapters of rank 32 46 us, 256 rows over 64 of rank
+// 64 133 us (634 MB: 4.8 TB/s; with a launch for each product 27, 50 and 150).
 template <int R16, int MT>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_few_kernel(const CbAdapter p, int splits) {
@@ -430,6 +435,7 @@ adapter_few_kernel(const CbAdapter p, int splits) {
 
 // h of many rows: a CTA makes 64 rows x (16 NT) ranks, whatever sections these belong to, so that x is read once; stages of 64 H along k come by asynchronous
 // copies.  Four warps by two: 16 rows and half of the ranks each.  The CTAs of a cluster have a share of k each.
+// 8192 rows of rank 16, a layer: 127 us for 402 MB of x (3.2 TB/s) and as much again of A out of L2 at 64 rows a tile; two more stages in flight change nothing.
 template <int NT>
 struct DownTile {
   static constexpr int NR = NT * 16, H = NT <= 4 ? 2 : 1, kStages = NT <= 4 ? 3 : 4;
@@ -549,6 +555,7 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
 // strips and B's operands in registers as long as these are of one adapter; the products add to y, which is rounded once.  y comes through a ring of the
 // warp's own, three strips ahead, and goes back through it: eight lanes copy a line of y, and a line of out.  (A lane's own columns straight from global
 // memory were four lines a quarter of a warp: 71 % of the load and store unit's cycles.)
+// 8192 rows of rank 16, 24576 columns: 160 us for 805 MB of y and out (5.0 TB/s); a bare copy in the same pattern takes 133 to 143.
 template <int R16, int MT>
 __global__ void __launch_bounds__(kAdapterThreads, R16 * MT <= 4 ? 3 : 2)
 adapter_up_kernel(const CbAdapter p) {
@@ -739,8 +746,8 @@ static int adapter_entries(int rows, int slots, int per) {
 static int adapter_items(int rows, int slots) { return adapter_entries(rows, slots, adapter_item_rows(rows)); }
 static int adapter_strips(int rows, int slots) { return adapter_entries(rows, slots, 16); }
 
-// CTAs that share k: as long as two find room on every SM.  Layers of 256 rows over 64 adapters of rank 64 and of 8192 rows of rank 16 by the most CTAs: 148
-// 178 and 456 us, 320 164 and 408, 592 180 and 426.
+// CTAs that share k: as long as two find room on every SM.  A layer by the most CTAs: 256 rows over 64 adapters of rank 64 (one launch) 160 185 us, 320 133,
+// 640 154; 48 rows over 12 80 63 us, 160 and more 46; 8192 rows of rank 16 (tiles) 148 456 us, 320 408, 592 426.  Clusters of sixteen change nothing.
 static int adapter_splits(int units, int k) {
   int splits = 1;
   while (splits < 8 && units * splits * 2 <= 320 && k / (splits * 2) >= 256) splits *= 2;

@@ -10,7 +10,12 @@
 // anything else.  Masses are whole multiples of 2^-42 of the largest weight: sums of 64-bit integers do not depend on their order, and two equal rows draw
 // the same whatever the shape of the launch.
 //
-// A row belongs to one CTA or to a cluster of up to eight, each with a share of its tokens: histograms and sums are read from the peers' shared memory.
+// A row belongs to one CTA or to a cluster of up to eight, each with a share of its tokens: tables are added up through the peers' shared memory.
+//
+// Few rows are bound by latency, many by additions to shared memory: one a token, about 5 cycles a warp of 32.  One row of 151936 bf16 values takes 15.7 us: the look
+// 4, its tables and their sums 5, the search and the id 3, the launch 3.  256 rows with top-p take 50 us, 1.6 TB/s: an SM with one row is through its look after 12 us, one
+// with two after 27; sums 5, each search 1 to 2, the id 1.  Nine fp32 rows with all filters take 39 us: a look for the largest, one with masses 4,
+// sums 7, each of four searches 5.  (Exponentials are no burden: without them the look takes 2.5.)
 #include "ptx.cuh"
 #include "launch.cuh"
 #include "philox.cuh"
@@ -33,6 +38,7 @@ namespace cb {
 
 typedef unsigned long long u64;
 
+// A table with masses leaves room for one CTA on an SM, so it has all the threads: 48 rows of 151936 tokens with all filters take 136 us, with 512 threads 162.
 template <bool F32> constexpr int kThreadsOf = F32 ? 1024 : 512;
 static constexpr int kVocabMostWarps = 32;
 static constexpr int kVocabMax = 1 << 20;
@@ -51,7 +57,7 @@ static_assert(kSegments <= kThreadsOf<false>, "a thread holds the sums before a 
 
 // Places 1 to 32, 33 to 64, ... of either side are a segment: they start on 16 bytes.
 static constexpr int kCountAt = 3, kMassAt = 1, kCountRoom = (kCountAt + kTable + 3) / 4 * 4, kMassRoom = (kMassAt + kTable + 1) / 2 * 2;
-static constexpr int kFew = 256;                           // tokens of a bin that are ranked one against the other
+static constexpr int kFew = 256;                           // tokens of a bin that are ranked one against the other: a search takes 5 us, with two divisions 11
 
 __device__ __forceinline__ uint32_t sort_key(uint32_t u) {                 // order of the values; both zeros are one
   if ((u << 1) == 0) return 0x80000000u;

@@ -9,6 +9,8 @@
 // Bound by latency: 256 decoding requests are 4 KB in and 6 KB out.  One launch; every CTA makes the three sums of all requests for itself (a few per
 // thread) and keeps them in shared memory, so that no CTA waits for another; a page that is taken in this step is read from the list
 // and not from the table, which another CTA may be writing.  Owners are found by bisection, four outputs a thread in one 16-byte store.
+// 256 decoding requests take 4.6 us, 37 portions of up to 220 tokens 4.3, 300 of up to 700 5.6 (their 3.5 MB would take 0.5): a launch, four trips to memory in
+// a row (ids and lengths; table or page; store) and the scan.
 #include "ptx.cuh"
 #include "launch.cuh"
 
