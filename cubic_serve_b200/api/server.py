@@ -130,6 +130,8 @@ class CubicASGIApp:
         names = [served_model_name] if isinstance(served_model_name, str) else list(served_model_name or ())
         self.served_model_name = names[0] if names else model_id
         self.accepted_names = tuple(dict.fromkeys([*names, model_id]))
+        if hasattr(backend, "model_names"):
+            backend.model_names = frozenset(self.accepted_names)
         self._key_digest = hashlib.sha256(api_key.encode()).digest() if api_key else None
         self.created = int(time.time())
 

@@ -150,4 +150,4 @@ class LowRankAdapters:
         if bank is None:
             return 0
         K.adapter_add(x, y, bank, self.rows)
-        return 2
+        return 1 if self.rows.rows <= K.ADAPTER_FEW_ROWS else 2

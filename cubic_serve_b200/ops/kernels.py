@@ -803,6 +803,9 @@ def step_layout(request: torch.Tensor, start: torch.Tensor, count: torch.Tensor,
     return out
 
 
+ADAPTER_FEW_ROWS = 512          # up to here both products of ``adapter_add`` are one launch (``csrc/adapters.cu``)
+
+
 class AdapterBank:
     """The low-rank adapters of one projection, in the kernels' layout: made from ``a`` bf16 ``[slots, sections * rank, k]``,
     ``b`` bf16 ``[slots, n, rank]``, ``scale`` fp32 ``[slots]``.  ``widths``: columns of the projection's sections (q | k | v),

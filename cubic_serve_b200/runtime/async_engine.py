@@ -86,6 +86,7 @@ class TokenChatBackend:
         self.processor = processor or ChatInputProcessor(tokenizer, default_thinking, engine.cfg.max_model_len)
         self.reasoning_parser = reasoning_parser
         self.default_max_tokens = default_max_tokens
+        self.model_names: frozenset[str] = frozenset()       # what the model itself is called: no adapter's name
         self.ready = True
         self._lock = threading.Lock()
         self._inbox: deque = deque()
@@ -99,7 +100,7 @@ class TokenChatBackend:
     @property
     def adapter_names(self) -> tuple[str, ...]:
         """Low-rank adapters that a request may name as its model."""
-        return tuple(getattr(self.engine, "adapter_names", ()))
+        return tuple(n for n in getattr(self.engine, "adapter_names", ()) if n not in self.model_names)
 
     # ------------------------------------------------------------ front side
     def start(self, req: CanonicalChatRequest):

@@ -226,7 +226,10 @@ def build_backend(args, devices: list[int], tp: int, spec, k_bits: int, v_bits: 
                 rows = [c for c in (1, 2, 4, 8, 16, 32, 64, 128, 256, 512) if c <= args.max_running_requests]
                 n = autotune.install(autotune.prepare(cfg, rows, dev, prep))
                 log.info("launch plans: %d measured entries replace the rules (%s)", n, "cached" if prep.hits else "measured now")
+            own = args.served_model_name or cfg.name
             for name, path in (adapters[1] if adapters is not None else ()):
+                if name in ([own] if isinstance(own, str) else own):
+                    raise SystemExit(f"the model itself is called {name!r}: a low-rank adapter needs another name")
                 got = executor.load_adapter(name, path)
                 log.info("low-rank adapter %s in slot %d", name, got.slot)
             caps = executor.capture_decode_graphs()

@@ -158,3 +158,15 @@ def test_requests_name_adapters_as_models():
     for model, seen in (("legal", "legal"), ("other", "public"), ("base", "public")):
         assert ask(model)[0] == 418 and backend.seen == seen
     assert ask("unknown")[0] == 404
+
+
+def test_a_name_of_the_model_reaches_no_adapter():
+    from types import SimpleNamespace
+
+    from cubic_serve_b200.api.server import CubicASGIApp
+    from cubic_serve_b200.runtime.async_engine import TokenChatBackend
+    backend = TokenChatBackend.__new__(TokenChatBackend)              # without its thread
+    backend.engine, backend.model_names = SimpleNamespace(adapter_names=("public", "legal", "base")), frozenset()
+    assert backend.adapter_names == ("public", "legal", "base")
+    CubicASGIApp(backend, "base", ["public", "other"])
+    assert backend.adapter_names == ("legal",)
