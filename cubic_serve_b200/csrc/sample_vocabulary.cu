@@ -12,10 +12,10 @@
 //
 // A row belongs to one CTA or to a cluster of up to eight, each with a share of its tokens: tables are added up through the peers' shared memory.
 //
-// Few rows are bound by latency, many by additions to shared memory: one a token, about 5 cycles a warp of 32.  One row of 151936 bf16 values takes 15.7 us: the look
-// 4, its tables and their sums 5, the search and the id 3, the launch 3.  256 rows with top-p take 50 us, 1.6 TB/s: an SM with one row is through its look after 12 us, one
-// with two after 27; sums 5, each search 1 to 2, the id 1.  Nine fp32 rows with all filters take 39 us: a look for the largest, one with masses 4,
-// sums 7, each of four searches 5.  (Exponentials are no burden: without them the look takes 2.5.)
+// Few rows are bound by latency, many by additions to shared memory: one a token, about 5 cycles a warp of 32.  One row of 151936 bf16 values takes 16 us: the look
+// 4, its tables and their sums 5, the search and the id 3, the launch 3.  48 rows with masks and all filters 28: the look 10.  256 rows with top-p 50, 1.6 TB/s: an
+// SM with one row is through its look after 12 us, one with two after 27; sums 5, each search 1 to 2, the id 1.  Nine fp32 rows of 50257 with all filters 39: a look
+// for the largest 2, one with masses 4, sums 7, each of four searches 5.  (Exponentials are no burden: without them the look takes 2.5.)
 #include "ptx.cuh"
 #include "launch.cuh"
 #include "philox.cuh"
@@ -135,13 +135,14 @@ struct VocabRow {
   __device__ __forceinline__ uint32_t word(int w) const { return w >= 0 && w < words ? mask[w] : 0u; }
   __device__ __forceinline__ uint32_t allowed(int v) const {                 // by the mask
     if (!mask) return 0xffu;
+    if (shift == 0) return reinterpret_cast<const unsigned char*>(mask)[v];     // eight neighbours are a byte
     const int i = first(v), w = i >> 5;
     return __funnelshift_r(word(w), (i & 31) > 24 ? word(w + 1) : 0u, i & 31) & 0xffu;
   }
-  // a vector in two steps, so that several are on their way: its bytes, if it has any that count and lies in the row, then
+  // a vector in two steps, so that several are on their way, and do not wait for their mask: its bytes, if it lies in the row, then
   // the bits of the values, and which of them are tokens of the row that the mask allows
-  __device__ __forceinline__ void fetch(int v, uint32_t ok, uint4& a, uint4& b) const {
-    if (ok == 0 || !whole(v)) return;
+  __device__ __forceinline__ void fetch(int v, bool in, uint4& a, uint4& b) const {
+    if (!in || !whole(v)) return;
     a = reinterpret_cast<const uint4*>(base)[F32 ? v * 2 : v];
     if (F32) b = reinterpret_cast<const uint4*>(base)[v * 2 + 1];
   }
@@ -172,9 +173,11 @@ struct VocabRow {
       uint4 a[U], b[U];
       uint32_t ok[U];
 #pragma unroll
-      for (int k = 0; k < U; ++k) ok[k] = v0 + k * T < to ? allowed(v0 + k * T) : 0u;
-#pragma unroll
-      for (int k = 0; k < U; ++k) fetch(v0 + k * T, ok[k], a[k], b[k]);
+      for (int k = 0; k < U; ++k) {
+        const bool in = v0 + k * T < to;
+        fetch(v0 + k * T, in, a[k], b[k]);
+        ok[k] = in ? allowed(v0 + k * T) : 0u;
+      }
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         if (ok[k] == 0) continue;
@@ -215,7 +218,7 @@ struct Vocab {
   int* count; u64* mass;                        // the table of the CTA's own tokens; in the segments that are its, once they are merged, of the row's
   short* tile_max;                              // bf16: largest of every 256 tokens as a signed 16-bit number: exact where it is not negative
   int rank, team, base;
-  bool mixed;                                   // bf16: the bin of zero holds other values
+  bool mixed;                                   // bf16: the bin of zero holds other values, or may
   u64 zero_mass;
   float best;
   double inv_t;
@@ -654,12 +657,17 @@ struct Vocab {
 
   // One look at a bf16 row, two tokens in a word: places in the table with one clamped addition, one shift and one merge for both.  NaN and -inf
   // are counted with what is too large to have a bin.  Returns the largest value as a signed 16-bit number: the largest value if that is not negative.
+  // `tiny`: whether the bin of zero holds another value of the thread's: the smallest magnitude less one, which takes zeros to the top.
   template <bool FILL>
-  __device__ __forceinline__ int quick_look() {
+  __device__ __forceinline__ int quick_look(bool& tiny) {
     constexpr uint32_t down = static_cast<uint32_t>(0x10000 - kUsualBase) * 0x10001u, limit = static_cast<uint32_t>(kSpan + 1) * 0x10001u;
-    uint32_t top = 0x80008000u;
+    uint32_t top = 0x80008000u, least = 0xffffffffu;
     char* table = reinterpret_cast<char*>(count);
-    auto places = [&](uint32_t w) { return (__viaddmin_s16x2_relu(w & 0x7fff7fffu, down, limit) << 2) | (w & 0x80008000u); };
+    auto places = [&](uint32_t w) {
+      const uint32_t mag = w & 0x7fff7fffu;
+      least = __viaddmin_u16x2(mag, 0xffffffffu, least);
+      return (__viaddmin_s16x2_relu(mag, down, limit) << 2) | (w & 0x80008000u);
+    };
     auto pair = [&](uint32_t w) {
       top = __vmaxs2(top, w);
       if (!FILL) return;
@@ -671,9 +679,18 @@ struct Vocab {
       const uint32_t sel = (ok & 1 ? 0xffffu : 0u) | (ok & 2 ? 0xffff0000u : 0u);
       top = __vmaxs2(top, (w & sel) | (0x80008000u & ~sel));
       if (!FILL) return;
-      const uint32_t place = places(w);
+      const uint32_t place = places(w & sel);
       if (ok & 1) atomicAdd(reinterpret_cast<int*>(table + (place & 0xffffu)), 1);
       if (ok & 2) atomicAdd(reinterpret_cast<int*>(table + (place >> 16)), 1);
+    };
+    auto few = [&](const uint4& q, uint32_t ok) {                            // an allowed token at a time
+      do {
+        const int j = __ffs(ok) - 1;
+        const uint32_t w = j & 4 ? (j & 2 ? q.w : q.z) : (j & 2 ? q.y : q.x), h = j & 1 ? w >> 16 : w & 0xffffu;
+        top = __vmaxs2(top, h | 0x80000000u);
+        if (FILL) atomicAdd(reinterpret_cast<int*>(table + (places(h) & 0xffffu)), 1);
+        ok &= ok - 1;
+      } while (ok);
     };
     const uint4* vec = reinterpret_cast<const uint4*>(row.base);
     const int tid = threadIdx.x, lane = tid & 31, first = row.from + (row.from < row.to && !row.whole(row.from)), last = row.to - (row.to > first && !row.whole(row.to - 1));
@@ -684,13 +701,12 @@ struct Vocab {
       uint4 q[U];
       uint32_t ok[U];
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
+      for (int k = 0; k < U; ++k) {                  // values do not wait for their mask
         const int v = row.from + (i0 + k * kVocabWarps) * 32 + lane;
-        ok[k] = v >= first && v < last ? row.allowed(v) : 0u;
+        const bool in = v >= first && v < last;
+        if (in) q[k] = vec[v];
+        ok[k] = in ? row.allowed(v) : 0u;
       }
-#pragma unroll
-      for (int k = 0; k < U; ++k)
-        if (ok[k]) q[k] = vec[row.from + (i0 + k * kVocabWarps) * 32 + lane];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const int i = i0 + k * kVocabWarps;
@@ -698,6 +714,8 @@ struct Vocab {
         top = 0x80008000u;
         if (ok[k] == 0xffu) {
           pair(q[k].x); pair(q[k].y); pair(q[k].z); pair(q[k].w);
+        } else if (ok[k] && __popc(ok[k]) <= 3) {
+          few(q[k], ok[k]);
         } else if (ok[k]) {
           some(q[k].x, ok[k]); some(q[k].y, ok[k] >> 2); some(q[k].z, ok[k] >> 4); some(q[k].w, ok[k] >> 6);
         }
@@ -713,7 +731,10 @@ struct Vocab {
       int t = -32768;
       if (lane < 8 && row.first(end) + lane >= 0 && row.first(end) + lane < row.vocab && (row.allowed(end) >> lane & 1)) {
         const uint32_t h = reinterpret_cast<const unsigned short*>(row.base)[end * 8 + lane];
-        if (FILL) atomicAdd(&count[place_of(h << 16, kUsualBase)], 1);
+        if (FILL) {
+          places(h);
+          atomicAdd(&count[place_of(h << 16, kUsualBase)], 1);
+        }
         t = static_cast<int>(static_cast<short>(h));
       }
       t = __reduce_max_sync(0xffffffffu, t);
@@ -721,6 +742,7 @@ struct Vocab {
       if (lane == 0) tile_max[i] = static_cast<short>(max(t, static_cast<int>(tile_max[i])));
       most = max(most, t);
     }
+    tiny = min(least & 0xffffu, least >> 16) < static_cast<uint32_t>(kUsualBase);
     return most;
   }
   // Any row: the largest key, and the table if FILL.
@@ -771,23 +793,24 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
   uint32_t best_key = 0;
   bool filled = false;
   if (!F32) {
-    const int most = static_cast<int>(f.block_max(static_cast<uint32_t>((greedy ? f.template quick_look<false>() : f.template quick_look<true>()) + 32768))) - 32768;
-    // what the peers have to know: the largest, tokens at zero, tokens too large below zero (among them -inf and NaN)
-    if (tid == 0)
-      f.tell(s.told.top, static_cast<u64>(most + 32768) << 48 | (greedy ? 0ull : static_cast<u64>(count[0] + count[kNegative]) << 24 | static_cast<u64>(count[kNegative + kSpan + 1])));
+    bool tiny = false;
+    const int most = static_cast<int>(f.block_max(static_cast<uint32_t>((greedy ? f.template quick_look<false>(tiny) : f.template quick_look<true>(tiny)) + 32768))) - 32768;
+    tiny = __syncthreads_or(tiny);
+    // what the peers have to know: the largest, whether there are tiny values, tokens too large below zero (among them -inf and NaN)
+    if (tid == 0) f.tell(s.told.top, static_cast<u64>(most + 32768) << 48 | static_cast<u64>(tiny) << 32 | (greedy ? 0ull : static_cast<u64>(count[kNegative + kSpan + 1])));
     f.meet();
-    u64 top = 0, zeros = 0, low = 0;
+    u64 top = 0, tinies = 0, low = 0;
     for (int c = 0; c < team; ++c) {
       const u64 v = s.told.top[c];
       top = max(top, v >> 48);
-      zeros += v >> 24 & 0xffffff;
+      tinies += v >> 32 & 1;
       low += v & 0xffffff;
     }
     const int value = static_cast<int>(top) - 32768;
     if (value >= 0 && value < 0x7f80 && low == 0) {
       best_key = sort_key(static_cast<uint32_t>(value) << 16);
       filled = greedy || f.base_for(key_value(best_key), t) == kUsualBase;
-      f.mixed = zeros != 0;                      // to be seen
+      f.mixed = tinies != 0;
     }
     if (!filled && !greedy) {
       f.meet();                                  // the peers may still read the table
@@ -965,8 +988,9 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const int v = f.row.from + i[k] * 32 + lane;
-        ok[k] = i[k] >= 0 && v < f.row.to ? f.row.allowed(v) : 0u;
-        f.row.fetch(v, ok[k], a[k], b[k]);
+        const bool in = i[k] >= 0 && v < f.row.to;
+        f.row.fetch(v, in, a[k], b[k]);
+        ok[k] = in ? f.row.allowed(v) : 0u;
       }
 #pragma unroll
       for (int k = 0; k < U; ++k) c[k] = of_tile(f.row.from + i[k] * 32 + lane, ok[k], a[k], b[k]);
@@ -1013,7 +1037,7 @@ sample_vocabulary_kernel(const CbVocabulary p, int team) {
   if (v < f.row.to) {
     uint32_t u[8], ok = f.row.allowed(v);
     uint4 a, b;
-    f.row.fetch(v, ok, a, b);
+    f.row.fetch(v, true, a, b);
     ok = f.row.values(v, ok, a, b, u);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -1054,9 +1078,10 @@ extern "C" int cb_sample_vocabulary(const CbVocabulary* p, void* stream) {
   if (p->rows < 0 || p->vocab < 1 || p->vocab > kVocabMax || p->ld < p->vocab || (p->mask && p->ld_mask < 0)) return -10;
   if (reinterpret_cast<uintptr_t>(p->logits) % (p->f32 ? 4 : 2)) return -11;
   if (p->rows == 0) return 0;
-  // CTAs of a row: as many as find room at once, with work for each
+  // CTAs of a row: as many as find an SM each, with work for each.  bf16 rows of 151936 tokens with top-k, limit 296 -> 148: 20 rows 21.5 -> 18.7 us,
+  // 48 23.8 -> 22.4, 74 38 -> 22.6 (clusters that do not fit at once), 100 30.8 -> 25.6.
   int team = 1;
-  while (team < kTeamMax && static_cast<long long>(p->rows) * team * 2 <= (p->f32 ? 148 : 296) && p->vocab / (team * 2) >= 4096) team *= 2;
+  while (team < kTeamMax && static_cast<long long>(p->rows) * team * 2 <= 148 && p->vocab / (team * 2) >= 4096) team *= 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = p->f32 ? (team > 1 ? vocabulary_launch<true, true>(*p, team, st) : vocabulary_launch<true, false>(*p, 1, st))
                                : (team > 1 ? vocabulary_launch<false, true>(*p, team, st) : vocabulary_launch<false, false>(*p, 1, st));
