@@ -726,10 +726,10 @@ def _require(ok: bool, what: str) -> None:
 def _call(entry: str, args: tuple, tensors: tuple) -> None:
     """Launch on the current stream of the tensors' own GPU, whichever is the current one."""
     dev = tensors[0].get_device()
-    _require(dev >= 0, "tensors must be on a GPU")
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError("tensors must be on one GPU")
+    _require(dev >= 0, "tensors must be on a GPU")
     stream = torch._C._cuda_getCurrentRawStream(dev)
     if dev == torch._C._cuda_getDevice():
         code = getattr(native.lib(), entry)(*args, stream)
@@ -794,11 +794,12 @@ def step_layout(request: torch.Tensor, start: torch.Tensor, count: torch.Tensor,
     _require(n <= out.max_requests and 0 <= tokens <= out.max_tokens and 0 <= blocks <= out.max_blocks and pad <= out.max_tokens and pad <= out.max_blocks,
              "more rows, row blocks or requests than the layout holds")
     _require(1 <= block <= 1 << 20, "a row block holds at least one position")
-    rows, width = table.shape if table.dim() == 2 else (0, 0)
-    _require(table.dtype is i32 and table.dim() == 2 and table.stride(1) == 1 and table.stride(0) >= width, "the block table is int32 with rows of neighbouring entries")
+    _require(table.dtype is i32 and table.dim() == 2, "the block table is an int32 matrix")
+    (rows, width), (ld, one) = table.shape, table.stride()
+    _require(one == 1 and ld >= width, "rows of the block table are neighbouring entries")
     packed = native.STEP_LAYOUT.pack(
         _vector(request, i32, n, "request"), _vector(start, i32, n, "start"), _vector(count, i32, n, "count"), _vector(held, i32, n, "held"), _vector(pages, i32, 0, "pages"),
-        table.data_ptr(), *out._at, n, pages.numel(), rows, width, table.stride(0), block, max(tokens, pad), max(blocks, pad), max(0, pad))
+        table.data_ptr(), *out._at, n, pages.numel(), rows, width, ld, block, max(tokens, pad), max(blocks, pad), max(0, pad))
     _call("cb_step_layout", (packed,), (start, request, count, held, pages, table, out.totals))
     return out
 
@@ -896,17 +897,24 @@ def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, rows: Adapt
 
     ``x`` bf16 ``[rows, k]``, ``y`` bf16 ``[rows, n]``, rows of neighbouring elements at a stride of a multiple of 8;
     ``out`` None: into ``y``.  Sums are fp32, the result is rounded once."""
-    out = y if out is None else out
     t, bf = rows.rows, torch.bfloat16
-    _require(x.dtype is bf and y.dtype is bf and out.dtype is bf, "x, y and out are bf16 matrices")
     _require(rows.slots == bank.slots, "the rows were sorted for another number of adapters")
-    _require(x.shape == (t, bank.k) and y.shape == (t, bank.n) and out.shape == (t, bank.n), "x is [sorted rows, k], y and out are [sorted rows, n]")
     _require(bank.sections * bank.rank <= rows.max_ranks, "more ranks than the sorted rows have room for")
-    ldx, ldy, ldo = (x.stride(0), y.stride(0), out.stride(0)) if t > 1 else (bank.k, bank.n, bank.n)
-    px, py, po = x.data_ptr(), y.data_ptr(), out.data_ptr()
-    _require((py != po or ldy == ldo) and (px != po or t == 0), "y and out are the same rows or other memory, x and out other memory")
-    _require(x.stride(1) == 1 and y.stride(1) == 1 and out.stride(1) == 1 and ldx >= bank.k and ldy >= bank.n and ldo >= bank.n and (ldx | ldy | ldo) % 8 == 0 and max(ldy, ldo) <= 1 << 30 and (px | py | po) % 16 == 0,
-             "rows of neighbouring elements at a stride of a multiple of 8, from a 16-byte boundary")
+    px, py = x.data_ptr(), y.data_ptr()
+    if x.dtype is not bf or y.dtype is not bf or x.shape != (t, bank.k) or y.shape != (t, bank.n):
+        raise ValueError("x is bf16 [sorted rows, k], y bf16 [sorted rows, n]")
+    (ldx, x1), (ldy, y1) = x.stride(), y.stride()
+    if out is None or out is y:
+        out, po, ldo, o1 = y, py, ldy, y1
+    else:
+        _require(out.dtype is bf and out.shape == (t, bank.n), "out is bf16 [sorted rows, n]")
+        po, (ldo, o1) = out.data_ptr(), out.stride()
+    if t <= 1:
+        ldx, ldy, ldo = bank.k, bank.n, bank.n
+    if (py == po and ldy != ldo) or (px == po and t):
+        raise ValueError("y and out are the same rows or other memory, x and out other memory")
+    if x1 != 1 or y1 != 1 or o1 != 1 or ldx < bank.k or ldy < bank.n or ldo < bank.n or (ldx | ldy | ldo) % 8 or ldy > 1 << 30 or ldo > 1 << 30 or (px | py | po) % 16:
+        raise ValueError("rows of neighbouring elements at a stride of a multiple of 8, from a 16-byte boundary")
     packed = native.ADAPTER.pack(px, ldx, py, ldy, po, ldo, *bank._at, *rows._at, t, *bank._shape)
     _call("cb_adapter_add", (packed,), (x, y, out, bank.a, rows.order))
     return out
@@ -928,10 +936,10 @@ def sample_vocabulary(logits: torch.Tensor, out_ids: torch.Tensor, temperature: 
     ``out_kept``: how many those are.  ``rows`` int32: draw for these rows only (below 0, or a row that there is not: none), each at its own
     place of every other tensor."""
     _require(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32), "logits are a bf16 or fp32 matrix")
-    n, f32 = logits.shape[0], torch.float32
-    vocab = logits.shape[1] if vocab is None else vocab
-    _require(1 <= vocab <= min(logits.shape[1], 1 << 20) and (logits.stride(1) == 1 or vocab == 1), "rows of one to 2^20 neighbouring logits")
-    ld = logits.stride(0) if n > 1 else max(logits.stride(0), vocab)
+    (n, width), (ld, one), f32 = logits.shape, logits.stride(), torch.float32
+    vocab = width if vocab is None else vocab
+    _require(1 <= vocab <= min(width, 1 << 20) and (one == 1 or vocab == 1), "rows of one to 2^20 neighbouring logits")
+    ld = ld if n > 1 else max(ld, vocab)
     _require(ld >= vocab, "rows of logits do not overlap")
     ld_mask = 0
     if mask is not None:
