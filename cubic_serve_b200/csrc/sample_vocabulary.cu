@@ -7,8 +7,8 @@
 // A row's values fall into bins of one sign, exponent and seven bits of mantissa: for bf16 a bin IS a value.  48 exponents have bins (2^-32 to 2^16, or those
 // below the row's largest magnitude that matters); smaller magnitudes share the bin of zero.  bf16: counts alone are gathered, a weight is computed once a
 // bin, in 64 bits.  fp32: counts and masses, and the bin that holds the end of a prefix is divided again by the bits below, as is the bin of zero if it holds
-// anything else.  Masses are whole multiples of 2^-42 of the largest weight: sums of 64-bit integers do not depend on their order, and two equal rows draw
-// the same whatever the shape of the launch.
+// anything else.  Masses are whole multiples of 2^-42 of the largest weight: sums of 64-bit integers do not depend on their order, so
+// that a launch repeats itself bit for bit.
 //
 // A row belongs to one CTA or to a cluster of up to eight, each with a share of its tokens: tables are added up through the peers' shared memory.
 //
@@ -302,6 +302,11 @@ struct Vocab {
     }
     __syncthreads();
   }
+  // Of a segment that begins at the best value or above it: the best one's bin, 32 or more if that is in another segment.
+  __device__ __forceinline__ int best_lane(int g) const {
+    const int off = static_cast<int>(__float_as_uint(best) >> 16 & 0x7fffu) - static_cast<int>(segment_mag(g)), at = g < kZeroSegment ? -off : off;
+    return (best < 0.f) != (g > kZeroSegment) || at < 0 ? 32 : at;
+  }
   // mass of the bin of a segment's lane that holds c tokens
   __device__ __forceinline__ u64 lane_mass(int g, int lane, int c) const {
     const int d = bin_in(g, lane);
@@ -314,7 +319,7 @@ struct Vocab {
     } else {
       int n = lane;
       if (w < 0.0) {
-        n = (best < 0.f) == (g > kZeroSegment) ? n - abs(static_cast<int>(__float_as_uint(best) >> 16 & 0x7fffu) - static_cast<int>(segment_mag(g))) : -1;
+        n -= best_lane(g);
         w = n >= 0 ? 1.0 : 0.0;
       }
       double q = s.ratio[segment_step(g)];
@@ -338,9 +343,8 @@ struct Vocab {
       w0 = s.seg_w[g];
       q = s.ratio[segment_step(g)];
       if (w0 < 0.0) {                                            // up to the best value, whose weight is one; what is above it is empty
-        const int off = static_cast<int>(__float_as_uint(best) >> 16 & 0x7fffu) - static_cast<int>(segment_mag(g));
-        from = (best < 0.f) == (g > kZeroSegment) ? (g < kZeroSegment ? -off : off) : 32;
-        w0 = from >= 0 && from < 32 ? 1.0 : 0.0;
+        from = best_lane(g);
+        w0 = from < 32 ? 1.0 : 0.0;
       }
       if (lane >= from) {
         w = w0;
