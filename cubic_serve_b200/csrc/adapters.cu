@@ -16,8 +16,8 @@
 
 namespace cb {
 
-// Up to here a work item is sixteen rows and A is streamed through registers, from here on it is 64 and A and x come by tiles.  331 rows over two adapters, a
-// layer: 82 us by tiles, 57 by sixteens.
+// Up to here a work item is sixteen rows and A is streamed through registers, from here on it is 64 and A and x come by tiles.  A layer of rank 16, by tiles and
+// by sixteens: 331 rows over 2 adapters 82 and 57 us; 640 over 2, 16 and 64 76, 86, 112 and 82, 87, 128; 1024 98, 103, 122 and 90, 93, 147; 2048 143, 153, 184 and 151, 154, 251.
 static constexpr int kAdapterFewRows = 512;
 static constexpr int adapter_item_rows(int rows) { return rows <= kAdapterFewRows ? 16 : 64; }
 static constexpr int kAdapterMaxSlots = 1023;
