@@ -814,11 +814,14 @@ extern "C" {
 int cb_adapter_rows(const void* ids, int rows, int slots, void* order, void* items, void* strips, void* stream) {
   using namespace cb;
   if (rows < 0 || rows > kAdapterMaxRows || slots < 1 || slots > kAdapterMaxSlots) return -10;
+  constexpr int most = 32 * (kAdapterMaxSlots + 1) * sizeof(unsigned short);
   const int smem = 32 * (slots + 1) * static_cast<int>(sizeof(unsigned short));
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(adapter_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * (kAdapterMaxSlots + 1) * sizeof(unsigned short));
-    if (e != cudaSuccess) return static_cast<int>(e);
-  }
+  static bool ready[64] = {};                                         // once a device, whatever the size: the kernel's own arrays (12.5 KB) count towards the usual 48 KB too
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !ready[dev])) e = cudaFuncSetAttribute(adapter_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 64) ready[dev] = true;
   return static_cast<int>(launch(adapter_rows_kernel, dim3(1), dim3(kSortThreads), smem, static_cast<cudaStream_t>(stream), static_cast<const int*>(ids), rows, slots,
                                  static_cast<int*>(order), static_cast<int*>(items), static_cast<int*>(strips)));
 }
