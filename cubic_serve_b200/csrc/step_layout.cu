@@ -191,15 +191,13 @@ extern "C" int cb_step_layout(const CbStepLayout* p, void* stream) {
   if (p->cap_tokens > kLayoutMost / 2 || p->cap_blocks > kLayoutMost / 2 || p->num_pages > kLayoutMost / 2) return -11;
   if (p->n < 0 || p->n > kLayoutMaxRequests || p->block < 1 || p->pad > p->cap_tokens || p->pad > p->cap_blocks || p->ld < p->width) return -10;
   const size_t smem = static_cast<size_t>(6 * p->n + 3) * sizeof(int);
-  static bool wide[64] = {};
+  static bool ready[64] = {};            // once a device, whatever the size: the kernel's own arrays count towards the usual 48 KB too
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  if (smem > 48 * 1024 && dev < 64 && !wide[dev]) {
+  if (e == cudaSuccess && (dev >= 64 || !ready[dev]))
     e = cudaFuncSetAttribute(step_layout_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (6 * kLayoutMaxRequests + 3) * sizeof(int));
-    if (e != cudaSuccess) return static_cast<int>(e);
-    wide[dev] = true;
-  }
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 64) ready[dev] = true;
   const int units = p->cap_tokens / 4 + p->cap_blocks / 4 + 2 + p->num_pages + p->n, grid = min(296, (units + kLayoutThreads - 1) / kLayoutThreads);
   return static_cast<int>(launch(step_layout_kernel, dim3(grid), dim3(kLayoutThreads), smem, static_cast<cudaStream_t>(stream), *p));
 }

@@ -30,3 +30,20 @@ assert torch.equal(plan.order.long(), torch.sort(key, stable=True).indices), "ro
 def test_rows_are_sorted_over_any_number_of_slots(slots):
     """Tables of 36 to 48 KB: more than 48 KB with the kernel's other shared memory."""
     _alone(_SORT, slots)
+
+
+_LAY = """
+import sys, torch
+from cubic_serve_b200.ops import kernels as K
+n = int(sys.argv[1])
+i = torch.arange(n, dtype=torch.int32, device="cuda")
+table, start, one = (i[:, None] * 3 + torch.arange(3, dtype=torch.int32, device="cuda")).contiguous(), i % 40, torch.ones_like(i)
+lay = K.step_layout(i, start, one, torch.full_like(i, 3), i[:0], table, K.StepLayout(n, n, n, "cuda"), 4, tokens=n, blocks=n)
+assert lay.totals.tolist() == [n, n, 0, 0] and torch.equal(lay.row0, i) and torch.equal(lay.slots, (i * 3 + start // 16) * 16 + start % 16)
+"""
+
+
+@pytest.mark.parametrize("n", [2043, 2047])
+def test_layouts_of_any_number_of_requests(n):
+    """Sums of 48 KB less a little: more than 48 KB with the kernel's other shared memory."""
+    _alone(_LAY, n)
