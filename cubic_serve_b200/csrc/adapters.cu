@@ -141,7 +141,7 @@ struct CbAdapter {
   const void* a;                         // bf16 [slots, ceil(k / 32), sections * rank, 32]: what is read together lies together
   const void* b;                         // bf16 [slots, n, rank]
   const float* scale;                    // [slots]
-  const int* ranks;                      // [slots] ranks in use, or null: all
+  const uint32_t* ranks;                 // [slots] ranks in use, a byte a section, or null: all
   const int* order; const int* items; const int* strips;         // adapter_rows_kernel's
   void* hi; void* lo;                    // bf16 [rows, sections * rank]: h as a sum of two
   int rows, slots, k, n, rank, sections;
@@ -149,6 +149,14 @@ struct CbAdapter {
 };
 
 namespace cb {
+
+// A section has ranks of its own (none, if the adapter leaves it as it is): an infinity in x makes NaN of the zeros behind them, and that must meet no column.
+__device__ __forceinline__ uint32_t ranks_of(const CbAdapter& p, int slot) { return p.ranks ? p.ranks[slot] : 0xffffffffu; }
+__device__ __forceinline__ int ranks_in(uint32_t ranks, int section) { return static_cast<int>(ranks >> 8 * section & 0xffu); }
+__device__ __forceinline__ int most_ranks(uint32_t ranks) {
+  const uint32_t two = __vmaxu4(ranks, ranks >> 16);
+  return static_cast<int>(max(two & 0xffu, two >> 8 & 0xffu));
+}
 
 // For A and B alone: what another kernel of the stream writes may change after this one has started, which the read-only path does not allow.
 __device__ __forceinline__ uint4 ldg16(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
@@ -215,7 +223,7 @@ adapter_few_kernel(const CbAdapter p, int splits) {
       }
       continue;
     }
-    const int used = p.ranks ? min(R, max(0, p.ranks[slot])) : R;
+    const uint32_t used = ranks_of(p, slot);
     const float scale = p.scale[slot];
     const bool in0 = g < rows, in1 = g + 8 < rows, both = rows > 8;
     const __nv_bfloat16* x0 = static_cast<const __nv_bfloat16*>(p.x) + (in0 ? p.order[first + g] * p.ldx : 0) + c * 8;
@@ -224,7 +232,7 @@ adapter_few_kernel(const CbAdapter p, int splits) {
       const __nv_bfloat16* A = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * turns * rt + q0 * 16) * 32 + lane * 8;
       bool on[4];                                                     // tiles of sixteen that hold ranks in use
 #pragma unroll
-      for (int t = 0; t < 4; ++t) on[t] = q0 + t < tiles && (q0 + t) % R16 * 16 < used;
+      for (int t = 0; t < 4; ++t) on[t] = q0 + t < tiles && (q0 + t) % R16 * 16 < ranks_in(used, (q0 + t) / R16);
       float acc[4][2][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -298,6 +306,7 @@ adapter_few_kernel(const CbAdapter p, int splits) {
     auto load_columns = [&](int u) {
       const int col = u * W + g * 2 * MT;
       const bool in = col < n;
+      const int most = most_ranks(used);
       const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(slot) * n + col) * R;
 #pragma unroll
       for (int t = 0; t < MT; ++t)
@@ -311,7 +320,7 @@ adapter_few_kernel(const CbAdapter p, int splits) {
           } else {
 #pragma unroll
             for (int s = 0; s < R16 / 2; ++s) {
-              const uint4 v = in && s * 32 < used ? ldg16(at + s * 32 + c * 8) : make_uint4(0, 0, 0, 0);
+              const uint4 v = in && s * 32 < most ? ldg16(at + s * 32 + c * 8) : make_uint4(0, 0, 0, 0);
               b[t][2 * s][k] = v.x;
               b[t][2 * s][2 + k] = v.y;
               b[t][2 * s + 1][k] = v.z;
@@ -364,7 +373,7 @@ adapter_few_kernel(const CbAdapter p, int splits) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         __nv_bfloat16 a, b;
-        split_h((k + i) % R < used ? v[i] * scale : 0.f, a, b);       // ranks that are not in use may have met what is not finite in x
+        split_h((k + i) % R < ranks_in(used, (k + i) / R) ? v[i] * scale : 0.f, a, b);       // ranks that are not in use may have met what is not finite in x
         hi |= static_cast<uint32_t>(__bfloat16_as_ushort(a)) << 16 * i;
         lo |= static_cast<uint32_t>(__bfloat16_as_ushort(b)) << 16 * i;
       }
@@ -458,7 +467,7 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
     const int item = u / parts, r0 = (u - item * parts) * NR;
     const int slot = p.items[1 + 3 * item], first = p.items[2 + 3 * item], rows = p.items[3 + 3 * item];
     if (slot < 0) continue;
-    const int used = p.ranks ? min(p.rank, max(0, p.ranks[slot])) : p.rank;
+    const uint32_t used = ranks_of(p, slot);
     const int row = tid >> 3, ch = tid & 7;                           // a thread's 16 bytes of rows row, row + 32, ...
     const __nv_bfloat16 *xr[2], *ar[AR];
     bool xin[2], ain[AR];
@@ -470,7 +479,7 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
 #pragma unroll
     for (int i = 0; i < AR; ++i) {
       const int r = r0 + row + 32 * i;
-      ain[i] = row + 32 * i < NR && r < rt && r % p.rank < used;
+      ain[i] = row + 32 * i < NR && r < rt && r % p.rank < ranks_in(used, r / p.rank);
       ar[i] = static_cast<const __nv_bfloat16*>(p.a) + ((static_cast<size_t>(slot) * turns + ch / 4) * rt + (ain[i] ? r : 0)) * 32 + ch % 4 * 8;
     }
     const uint32_t to0 = base + row * 128 + ((ch ^ (row & 7)) << 4);
@@ -544,7 +553,7 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
       } else {
         v = part[r * SP + k];
       }
-      put_h(p, v, scale, (r0 + k) % p.rank < used, static_cast<size_t>(first + r) * rt + r0 + k);
+      put_h(p, v, scale, (r0 + k) % p.rank < ranks_in(used, (r0 + k) / p.rank), static_cast<size_t>(first + r) * rt + r0 + k);
     }
     if (splits > 1) cluster_sync_all(); else __syncthreads();
   }
@@ -643,7 +652,7 @@ adapter_up_kernel(const CbAdapter p) {
     for (int s = s0; s < s1; ++s) {
       if (strip.x != held) {
         held = strip.x;
-        used = held < 0 ? 0 : p.ranks ? min(R, max(0, p.ranks[held])) : R;
+        used = held < 0 ? 0 : ranks_in(ranks_of(p, held), sec);
         // product t, places g and g + 8: columns 2 t and 2 t + 1 of the lane's
         const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(max(held, 0)) * n + col) * R;
 #pragma unroll

@@ -836,17 +836,18 @@ class AdapterBank:
         a = pad(a.reshape(slots, S, rank, k), (0, blocks * 32 - k, 0, full - rank)).view(slots, S * full, blocks, 32).transpose(1, 2).contiguous()
         b = pad(b, (0, full - rank)) if full != rank else b.clone(memory_format=torch.contiguous_format)
         scale = scale.clone()
-        ranks = torch.full((slots,), rank, dtype=torch.int32, device=a.device) if ranks is None else ranks.clone()
+        ranks = torch.full((slots,), rank, dtype=torch.int32, device=a.device) if ranks is None else ranks.clamp(0, rank)
         self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
+        self._section_ranks = ranks.view(slots, 1).to(torch.uint8).repeat(1, 4)        # what the kernels go by: a byte a section
         self.slots, self.k, self.n, self.rank, self.sections = slots, k, n, full, S
-        self._at = (a.data_ptr(), b.data_ptr(), scale.data_ptr(), ranks.data_ptr())
+        self._at = (a.data_ptr(), b.data_ptr(), scale.data_ptr(), self._section_ranks.data_ptr())
         self._shape = (slots, self.k, n, full, S, *self.widths, *(0,) * (4 - S))
 
     def load(self, slot: int, a, b, scale: float) -> None:
         """Write one adapter: ``a`` / ``b`` a matrix ``[rank, k]`` / ``[width, rank]`` for every section (None: the section has
-        none); ranks below the bank's leave the rest zero."""
+        none, and its columns stay as they are); ranks below the bank's leave the rest zero."""
         _require(0 <= slot < self.slots and len(a) == len(b) == self.sections, "no such slot, or not a matrix for every section")
-        col, most = 0, 0
+        col, used = 0, [0] * 4
         for i, (ai, bi) in enumerate(zip(a, b)):
             at, width = i * self.rank, self.widths[i]
             _require((ai is None) == (bi is None), "a section has both matrices or none")
@@ -859,9 +860,10 @@ class AdapterBank:
                 self.a[slot, :, at:at + r].copy_(rows.view(r, -1, 32).transpose(0, 1))
                 self.b[slot, col:col + width, :r].copy_(bi)
             col += width
-            most = max(most, r)
+            used[i] = r
         self.scale[slot] = float(scale)
-        self.ranks[slot] = most
+        self.ranks[slot] = max(used)
+        self._section_ranks[slot].copy_(torch.tensor(used, dtype=torch.uint8))
 
 
 class AdapterRows:

@@ -1,11 +1,19 @@
 """Edges of the operators around a step's shared layers."""
+import math
 import subprocess
 import sys
 from pathlib import Path
 
+import numpy as np
 import pytest
+import torch
+
+from cubic_serve_b200.ops import kernels as K
+from test_gpu_step_operators import _adapter_case, _adapter_truth
 
 pytestmark = pytest.mark.gpu
+DEV = "cuda"
+I32 = torch.int32
 ROOT = Path(__file__).resolve().parent.parent
 
 
@@ -47,3 +55,47 @@ assert lay.totals.tolist() == [n, n, 0, 0] and torch.equal(lay.row0, i) and torc
 def test_layouts_of_any_number_of_requests(n):
     """Sums of 48 KB less a little: more than 48 KB with the kernel's other shared memory."""
     _alone(_LAY, n)
+
+
+# ------------------------------------------------------------------------------------------------- adapters
+@pytest.mark.parametrize("rows", [1, 40, 700])
+@pytest.mark.parametrize("rank,widths", [(16, (96, 32, 64)), (40, (64, 64)), (128, (32, 32, 32))])
+def test_a_section_without_matrices_is_left_alone(rows, rank, widths):
+    """An infinity or NaN in x meets an adapter that has no matrices for a section: that section's columns are y, to the bit."""
+    k, S = 264, len(widths)
+    x, y, a, b, scale = _adapter_case(rows, 2, rank, k, widths, None, seed=6)
+    bank = K.AdapterBank(a, b, scale, widths)
+    cut = lambda i: b[0, sum(widths[:i]):sum(widths[:i + 1])]        # noqa: E731
+    for none in range(S):
+        bank.load(0, [None if i == none else a[0, i * rank:i * rank + rank] for i in range(S)], [None if i == none else cut(i) for i in range(S)], 1.5)
+        x2 = x.clone()
+        x2[0, 7] = math.inf
+        x2[rows // 2, 100] = math.nan
+        x2[rows - 1, 263] = -math.inf
+        ids = torch.zeros(rows, dtype=I32, device=DEV)
+        plan = K.adapter_rows(ids, K.AdapterRows(rows, 2, S * rank, DEV))
+        lo = sum(widths[:none])
+        for in_place in (False, True):
+            got = K.adapter_add(x2, y.clone(), bank, plan) if in_place else K.adapter_add(x2, y, bank, plan, out=torch.empty_like(y))
+            assert torch.equal(got[:, lo:lo + widths[none]], y[:, lo:lo + widths[none]])
+            rest = torch.cat([got[rows // 2, :lo], got[rows // 2, lo + widths[none]:]])
+            assert bool(rest.isnan().all()), "what is not finite reaches the columns of the other sections"
+
+
+@pytest.mark.parametrize("rows", [33, 600])
+def test_sections_of_different_ranks(rows):
+    """Ranks 24, none and 3 of one adapter, all of another: the ranks behind a section's own are nobody's, also where x is not finite."""
+    widths, rank, k = (64, 32, 40), 24, 136
+    x, y, a, b, scale = _adapter_case(rows, 2, rank, k, widths, None, seed=8)
+    bank = K.AdapterBank(a, b, scale, widths)
+    bank.load(1, [a[1, :24], None, a[1, 48:51]], [b[1, :64], None, b[1, 96:, :3]], float(scale[1]))
+    a[1, 24:48], a[1, 51:], b[1, 64:96], b[1, 96:, 3:] = 0, 0, 0, 0
+    ids = np.arange(rows) % 3 - 1
+    plan = K.adapter_rows(torch.tensor(ids.tolist(), dtype=I32, device=DEV), K.AdapterRows(rows, 2, 72, DEV))
+    want, err = _adapter_truth(x, y, a, b, scale, widths, ids)
+    got = K.adapter_add(x, y, bank, plan, out=torch.empty_like(y))
+    assert bool(((got.double() - want).abs() <= err).all())
+    x[2, 5], b[1, 96:, :3] = math.inf, b[1, 96:, :3].abs() + 0.1
+    bank.load(1, [a[1, :24], None, a[1, 48:51].abs() + 0.1], [b[1, :64], None, b[1, 96:, :3]], float(scale[1]))
+    got = K.adapter_add(x, y, bank, plan, out=torch.empty_like(y))
+    assert torch.equal(got[2, 64:96], y[2, 64:96]) and bool((got[2, 96:] == math.inf).all())
