@@ -847,12 +847,15 @@ class AdapterBank:
         """Write one adapter: ``a`` / ``b`` a matrix ``[rank, k]`` / ``[width, rank]`` for every section (None: the section has
         none, and its columns stay as they are); ranks below the bank's leave the rest zero."""
         _require(0 <= slot < self.slots and len(a) == len(b) == self.sections, "no such slot, or not a matrix for every section")
-        col, used = 0, [0] * 4
-        for i, (ai, bi) in enumerate(zip(a, b)):
-            at, width = i * self.rank, self.widths[i]
+        used = [0] * 4
+        for i, (ai, bi) in enumerate(zip(a, b)):                     # all of them before the first is written
             _require((ai is None) == (bi is None), "a section has both matrices or none")
-            r = 0 if ai is None else ai.shape[0]
-            _require(r <= self.max_rank and (r == 0 or (tuple(ai.shape) == (r, self.k) and tuple(bi.shape) == (width, r))), f"section {i}: [rank <= {self.max_rank}, {self.k}] and [{width}, rank]")
+            used[i] = r = 0 if ai is None else ai.shape[0]
+            _require(r <= self.max_rank and (r == 0 or (tuple(ai.shape) == (r, self.k) and tuple(bi.shape) == (self.widths[i], r))),
+                     f"section {i}: [rank <= {self.max_rank}, {self.k}] and [{self.widths[i]}, rank]")
+        col, scale = 0, float(scale)
+        for i, (ai, bi) in enumerate(zip(a, b)):
+            at, width, r = i * self.rank, self.widths[i], used[i]
             self.a[slot, :, at:at + self.rank].zero_()
             self.b[slot, col:col + width].zero_()
             if r:
@@ -860,8 +863,7 @@ class AdapterBank:
                 self.a[slot, :, at:at + r].copy_(rows.view(r, -1, 32).transpose(0, 1))
                 self.b[slot, col:col + width, :r].copy_(bi)
             col += width
-            used[i] = r
-        self.scale[slot] = float(scale)
+        self.scale[slot] = scale
         self.ranks[slot] = max(used)
         self._section_ranks[slot].copy_(torch.tensor(used, dtype=torch.uint8))
 
