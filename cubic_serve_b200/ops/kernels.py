@@ -833,7 +833,7 @@ class AdapterBank:
         self.max_rank, k = rank, a.shape[2]
         blocks = -(-k // 32)
         pad = torch.nn.functional.pad
-        a = pad(a.reshape(slots, S, rank, k), (0, blocks * 32 - k, 0, full - rank)).view(slots, S * full, blocks, 32).transpose(1, 2).clone(memory_format=torch.contiguous_format)
+        a = pad(a.reshape(slots, S, rank, k), (0, blocks * 32 - k, 0, full - rank)).view(slots, S * full, blocks, 32).transpose(1, 2).contiguous()
         b = pad(b, (0, full - rank)) if full != rank else b.clone(memory_format=torch.contiguous_format)
         scale = scale.clone()
         ranks = torch.full((slots,), rank, dtype=torch.int32, device=a.device) if ranks is None else ranks.clamp(0, rank)

@@ -16,14 +16,3 @@ def test_a_refused_load_leaves_the_slot_as_it_was():
         with pytest.raises(ValueError):
             bank.load(0, a, b, 3.0)
         assert all(torch.equal(t, h) for t, h in zip((bank.a, bank.b, bank.scale, bank.ranks, bank._section_ranks), held))
-
-
-@pytest.mark.parametrize("k,rank", [(32, 16), (8, 16), (64, 16), (32, 20)])
-def test_a_bank_keeps_copies(k, rank):
-    """Also where a single block of 32 along k has the stored order already."""
-    a, b, scale, ranks = torch.ones(2, rank, k).bfloat16(), torch.ones(2, 64, rank).bfloat16(), torch.ones(2), torch.full((2,), rank, dtype=torch.int32)
-    bank = K.AdapterBank(a, b, scale, ranks=ranks)
-    bank.load(0, [None], [None], 0.0)
-    assert a.eq(1).all() and b.eq(1).all() and scale.eq(1).all() and ranks.eq(rank).all(), "what it was made from is not written"
-    a.fill_(5), b.fill_(5), scale.fill_(5), ranks.fill_(1)
-    assert bank.a[1].max() == 1 and bank.b[1].max() == 1 and bank.scale[1] == 1 and bank.ranks[1] == rank, "and may be written"
