@@ -837,6 +837,7 @@ class AdapterBank:
         b = pad(b, (0, full - rank)) if full != rank else b.clone(memory_format=torch.contiguous_format)
         scale = scale.clone()
         ranks = torch.full((slots,), rank, dtype=torch.int32, device=a.device) if ranks is None else ranks.clamp(0, rank)
+        b.masked_fill_(torch.arange(full, device=b.device) >= ranks.view(slots, 1, 1), 0)       # h is zero there, whatever A and x hold
         self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
         self._section_ranks = ranks.view(slots, 1).to(torch.uint8).repeat(1, 4)        # what the kernels go by: a byte a section
         self.slots, self.k, self.n, self.rank, self.sections = slots, k, n, full, S

@@ -99,3 +99,21 @@ def test_sections_of_different_ranks(rows):
     bank.load(1, [a[1, :24], None, a[1, 48:51].abs() + 0.1], [b[1, :64], None, b[1, 96:, :3]], float(scale[1]))
     got = K.adapter_add(x, y, bank, plan, out=torch.empty_like(y))
     assert torch.equal(got[2, 64:96], y[2, 64:96]) and bool((got[2, 96:] == math.inf).all())
+
+
+@pytest.mark.parametrize("rows", [20, 600])
+@pytest.mark.parametrize("rank", [24, 100])
+def test_ranks_that_are_not_in_use_reach_nothing(rows, rank):
+    """A bank made over buffers with NaN behind the ranks in use, and an empty slot that is NaN throughout."""
+    widths, ranks = (64, 32), (rank, 5, 0)
+    x, y, a, b, scale = _adapter_case(rows, 3, rank, 136, widths, None, seed=2)
+    ids = np.arange(rows) % 4 - 1
+    want, err = _adapter_truth(x, y, a, b, scale, widths, ids, ranks)
+    for s, r in enumerate(ranks):
+        a.view(3, 2, rank, 136)[s, :, r:] = math.nan
+        b[s, :, r:] = math.nan
+    scale[2] = math.nan
+    bank = K.AdapterBank(a, b, scale, widths, ranks=torch.tensor(ranks, dtype=I32, device=DEV))
+    plan = K.adapter_rows(torch.tensor(ids.tolist(), dtype=I32, device=DEV), K.AdapterRows(rows, 3, 2 * rank, DEV))
+    got = K.adapter_add(x, y, bank, plan, out=torch.empty_like(y))
+    assert bool(((got.double() - want).abs() <= err).all()) and torch.equal(got[3::4], y[3::4])
