@@ -75,7 +75,8 @@ class LowRankAdapters:
 
     def __init__(self, cfg, layers: list, slots: int, max_rank: int, max_tokens: int, device) -> None:
         """``layers``: the decoder's ``LayerWeights``.  Full-attention layers take adapters on q, k, v and o, dense MLPs on gate, up and
-        down; experts and recurrent mixers have none."""
+        down; experts and recurrent mixers have none.  ``nbytes``: memory that all of it holds (a server plans with that of one on
+        the device ``meta``)."""
         if not 1 <= slots <= 1023 or not 1 <= max_rank <= 128:
             raise AdapterError("up to 1023 adapters of ranks up to 128")
         self.slots, self.max_rank = slots, max_rank
@@ -89,12 +90,13 @@ class LowRankAdapters:
             banks = {}
             for name in names:
                 k, widths = shapes[name]
-                bf = dict(dtype=torch.bfloat16, device=device)
-                banks[name] = K.AdapterBank(torch.zeros(slots, len(widths) * max_rank, k, **bf), torch.zeros(slots, sum(widths), max_rank, **bf),
+                zero = torch.zeros((), dtype=torch.bfloat16, device=device)
+                banks[name] = K.AdapterBank(zero.expand(slots, len(widths) * max_rank, k), zero.expand(slots, sum(widths), max_rank),
                                             torch.zeros(slots, device=device), widths, ranks=torch.zeros(slots, dtype=torch.int32, device=device))
                 most = max(most, len(widths) * max_rank)
             self.banks.append(banks)
         self.rows = K.AdapterRows(max_tokens, slots, max(most, 1), device)
+        self.nbytes = self.rows.nbytes + sum(bank.nbytes for banks in self.banks for bank in banks.values())
         self.loaded: dict[str, LoadedAdapter] = {}
         self._loads = 0
 

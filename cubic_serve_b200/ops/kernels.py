@@ -831,10 +831,15 @@ class AdapterBank:
             _require(t is None or t.device == a.device, "tensors must be on one device")
         full = next(r for r in (16, 32, 64, 128) if r >= rank)
         self.max_rank, k = rank, a.shape[2]
-        blocks = -(-k // 32)
-        pad = torch.nn.functional.pad
-        a = pad(a.reshape(slots, S, rank, k), (0, blocks * 32 - k, 0, full - rank)).view(slots, S * full, blocks, 32).transpose(1, 2).contiguous()
-        b = pad(b, (0, full - rank)) if full != rank else b.clone(memory_format=torch.contiguous_format)
+        # into their places at once: a large bank has no room for copies on the way
+        whole, given = k // 32, a.reshape(slots, S, rank, k)
+        a = torch.zeros(slots, -(-k // 32), S, full, 32, dtype=torch.bfloat16, device=b.device)
+        a[:, :whole, :, :rank].copy_(given[..., :whole * 32].unflatten(-1, (whole, 32)).permute(0, 3, 1, 2, 4))
+        if k % 32:
+            a[:, whole, :, :rank, :k % 32].copy_(given[..., whole * 32:])
+        a, given = a.view(slots, -1, S * full, 32), b
+        b = torch.zeros(slots, n, full, dtype=torch.bfloat16, device=b.device)
+        b[..., :rank].copy_(given)
         scale = scale.clone()
         ranks = torch.full((slots,), rank, dtype=torch.int32, device=a.device) if ranks is None else ranks.clamp(0, rank)
         b.masked_fill_(torch.arange(full, device=b.device) >= ranks.view(slots, 1, 1), 0)       # h is zero there, whatever A and x hold
@@ -843,6 +848,11 @@ class AdapterBank:
         self.slots, self.k, self.n, self.rank, self.sections = slots, k, n, full, S
         self._at = (a.data_ptr(), b.data_ptr(), scale.data_ptr(), self._section_ranks.data_ptr())
         self._shape = (slots, self.k, n, full, S, *self.widths, *(0,) * (4 - S))
+
+    @property
+    def nbytes(self) -> int:
+        """Memory that the bank holds."""
+        return sum(t.nbytes for t in (self.a, self.b, self.scale, self.ranks, self._section_ranks))
 
     def load(self, slot: int, a, b, scale: float) -> None:
         """Write one adapter: ``a`` / ``b`` a matrix ``[rank, k]`` / ``[width, rank]`` for every section (None: the section has
@@ -885,6 +895,7 @@ class AdapterRows:
         self.items, self.strips = torch.zeros(1 + 3 * strips, **i32), torch.zeros(4 + 4 * strips, **i32)
         self.h = torch.zeros(2, (max_rows + 16) * self.max_ranks, dtype=torch.bfloat16, device=device)      # sixteen spare rows: they are read
         self._at = (self.order.data_ptr(), self.items.data_ptr(), self.strips.data_ptr(), self.h[0].data_ptr(), self.h[1].data_ptr())
+        self.nbytes = sum(t.nbytes for t in (self.order, self.items, self.strips, self.h))
 
 
 def adapter_rows(ids: torch.Tensor, out: AdapterRows) -> AdapterRows:

@@ -178,7 +178,16 @@ def build_backend(args, devices: list[int], tp: int, spec, k_bits: int, v_bits: 
         # models with recurrent layers resume a cached prefix from a snapshot of the state taken at its last page
         # boundary: as many snapshot rows as request rows
         snapshots = args.max_running_requests if cfg.is_hybrid and args.prefix_cache else 0
-        pages = plan_kv_pages(free, int(args.gpu_reserve_gib * 2 ** 30) + (2 << 30), cfg, 1, k_bits, v_bits, max_len,
+        reserve = int(args.gpu_reserve_gib * 2 ** 30) + (2 << 30)
+        if adapters is not None:
+            # every slot's matrices are allocated at start, behind the cache
+            from ..models.low_rank import LowRankAdapters
+            held = LowRankAdapters(cfg, weights.layers, *adapters[0], args.token_budget, "meta").nbytes
+            if reserve + held >= free:
+                raise SystemExit(f"{adapters[0][0]} low-rank adapters of ranks up to {adapters[0][1]} take {held / 2 ** 30:.1f} GiB; "
+                                 f"{max(0, free - reserve) / 2 ** 30:.1f} GiB are left beside weights and reserve (--low-rank-slots, --low-rank-max-rank)")
+            reserve += held
+        pages = plan_kv_pages(free, reserve, cfg, 1, k_bits, v_bits, max_len,
                               args.max_running_requests, state_snapshots=snapshots)
         runner = defn.build_runner(cfg, weights, num_pages=pages, max_tokens=args.token_budget, k_bits=k_bits, v_bits=v_bits,
                                    max_requests=args.max_running_requests, state_checkpoints=snapshots,

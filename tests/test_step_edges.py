@@ -25,3 +25,71 @@ def test_ranks_that_are_not_in_use_may_hold_anything():
     bank = K.AdapterBank(torch.full((3, 24, 64), float("nan")).bfloat16(), b, torch.full((3,), float("nan")), ranks=torch.tensor([24, 5, 0], dtype=torch.int32))
     assert bank.b[0, :, :24].eq(1).all() and bank.b[1, :, :5].eq(2).all() and not bank.b[0, :, 24:].any() and not bank.b[1, :, 5:].any() and not bank.b[2].any()
     assert b[2].isnan().all(), "the caller's is as it was"
+
+
+# ------------------------------------------------------------------------------------------------- memory of a deployment with adapters
+def _planned_pages(monkeypatch, model, free, *flags):
+    """KV pages that a server would plan with so many bytes free, and the layers it would serve."""
+    from types import SimpleNamespace
+
+    from cubic_serve_b200.cli import build_parser, parse_speculative_config
+    from cubic_serve_b200.models import registry
+    from cubic_serve_b200.models.config import NAMED_CONFIGS
+    from cubic_serve_b200.runtime.serving import build_backend
+
+    cfg = NAMED_CONFIGS[model]()
+    layers = [SimpleNamespace(gdn=object() if cfg.layer_is_gdn(i) else None, moe=object() if cfg.is_moe else None) for i in range(cfg.num_layers)]
+
+    class Planned(Exception):
+        pass
+
+    def runner(*_, num_pages, **kw):
+        raise Planned(num_pages)
+
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "set_device", lambda d: None)
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda d: (free, free))
+    monkeypatch.setattr(registry, "get", lambda family: SimpleNamespace(random_weights=lambda *a: SimpleNamespace(layers=layers), build_runner=runner))
+    args = build_parser().parse_args(["serve", f"random:{model}", "--max-running-requests", "256", "--max-model-len", "32768", "--token-budget", "8192", *flags])
+    with pytest.raises(Planned) as got:
+        build_backend(args, [0], 1, parse_speculative_config(None), 8, 8)
+    return got.value.args[0], cfg, layers
+
+
+@pytest.mark.parametrize("model,slots,rank", [("dense-8b", 16, 64), ("dense-8b", 64, 64), ("moe-30b-a3b", 5, 20), ("hybrid-8b", 3, 128)])
+def test_the_kv_cache_leaves_room_for_the_adapters(monkeypatch, model, slots, rank):
+    from cubic_serve_b200.contracts.model import CacheSpec
+    flags = ("--low-rank-slots", str(slots), "--low-rank-max-rank", str(rank))
+    without, cfg, layers = _planned_pages(monkeypatch, model, 60 << 30)
+    with_them, _, _ = _planned_pages(monkeypatch, model, 60 << 30, *flags)
+    # every slot has A and B of each projection, ranks stored as 16, 32, 64 or 128; h of a step's rows
+    stored, D = next(r for r in (16, 32, 64, 128) if r >= rank), cfg.head_dim
+    q, kv, h, i = cfg.num_q_heads * D, cfg.num_kv_heads * D, cfg.hidden_size, cfg.intermediate_size
+    need = 0
+    for lw in layers:
+        if lw.gdn is None:
+            need += (3 * h + q + 2 * kv) + (q + h)
+        if lw.moe is None:
+            need += (2 * h + 2 * i) + (i + h)
+    need = need * slots * stored * 2 + 2 * 2 * 8192 * 3 * stored
+    page = CacheSpec(sum(lw.gdn is None for lw in layers), cfg.num_kv_heads, D, 8, 8).page_bytes
+    assert need / page <= without - with_them <= need / page * 1.02 + 2, "pages given up are the adapters' bytes, and their rows' lists"
+
+
+def test_adapters_that_leave_no_room_are_refused(monkeypatch):
+    with pytest.raises(SystemExit, match="GiB"):
+        _planned_pages(monkeypatch, "dense-8b", 20 << 30, "--low-rank-slots", "64")
+
+
+def test_empty_banks_take_their_own_memory_and_no_more():
+    """The sum that a server plans with is what the banks hold."""
+    from types import SimpleNamespace
+
+    from cubic_serve_b200.models.config import ModelConfig, QuantSpec
+    from cubic_serve_b200.models.low_rank import LowRankAdapters
+    cfg = ModelConfig(name="t", num_layers=2, hidden_size=72, num_q_heads=2, num_kv_heads=1, head_dim=32, intermediate_size=96, vocab_size=128, quant=QuantSpec("none"))
+    layers = [SimpleNamespace(gdn=None, moe=None), SimpleNamespace(gdn=None, moe=object())]
+    real, planned = LowRankAdapters(cfg, layers, 3, 20, 50, "cpu"), LowRankAdapters(cfg, layers, 3, 20, 50, "meta")
+    held = [t for banks in real.banks for b in banks.values() for t in vars(b).values() if isinstance(t, torch.Tensor)] + [t for t in vars(real.rows).values() if isinstance(t, torch.Tensor)]
+    assert planned.nbytes == real.nbytes == sum(t.untyped_storage().nbytes() for t in held)
+    assert not any(t.any() for t in held)
