@@ -318,6 +318,8 @@ def _build_qwen4_exp_backend(args, cfg, path, spec=None):
     from ..runtime.async_engine import TokenChatBackend
     from ..runtime.engine import LLMEngine
     from ..runtime.scheduler import SchedulerConfig
+    if _low_rank_adapters(args) is not None:
+        raise SystemExit("low-rank adapters are served by the native decoder runner, which the qwen4_exp family does not have")
     if args.execution_mode == "cuda":
         log.warning("the qwen4_exp family runs on the eager executor; --execution-mode cuda has no native runner for it")
     store = None

@@ -93,3 +93,13 @@ def test_empty_banks_take_their_own_memory_and_no_more():
     held = [t for banks in real.banks for b in banks.values() for t in vars(b).values() if isinstance(t, torch.Tensor)] + [t for t in vars(real.rows).values() if isinstance(t, torch.Tensor)]
     assert planned.nbytes == real.nbytes == sum(t.untyped_storage().nbytes() for t in held)
     assert not any(t.any() for t in held)
+
+
+def test_adapters_of_a_family_without_a_native_runner_are_refused(monkeypatch):
+    """Not left out in silence: a request that names one would be told that there is no such model."""
+    from cubic_serve_b200.cli import build_parser, parse_speculative_config
+    from cubic_serve_b200.runtime.serving import build_backend
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    args = build_parser().parse_args(["serve", "random:qwen4-exp-tiny", "--low-rank-slots", "2", "--execution-mode", "cuda"])
+    with pytest.raises(SystemExit, match="low-rank adapters"):
+        build_backend(args, [0], 1, parse_speculative_config(None), 8, 8)
