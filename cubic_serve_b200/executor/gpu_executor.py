@@ -245,7 +245,8 @@ class BatchBuilder:
 
     def stage_layout(self, segs: list[Segment]) -> int:
         """Stage what ``K.step_layout`` needs of a step besides the lengths that ``_fill`` staged: the pages that the device's rows hold
-        and those that they are given.  Returns how many these are."""
+        and those that they are given.  Returns how many these are.  A request that has too few pages, or more than a row holds, is an
+        error before anything is staged."""
         if self.given is None:
             n = self.max_rows * (self.max_pages + 1)
             self.given_host = torch.empty(n, dtype=torch.int32, pin_memory=torch.cuda.is_available())
@@ -253,8 +254,11 @@ class BatchBuilder:
         n, h, out = len(segs), self.stage.h, self.given_host.numpy()
         slots, uids = h["seg_slot"][:n], np.array([s.uid for s in segs], dtype=np.int64)
         need = (h["seg_pos0"][:n] + h["seg_count"][:n] + K.PAGE_TOKENS - 1) // K.PAGE_TOKENS
-        held = self._device_held[slots]
-        held = np.where((self._device_uid[slots] == uids) & (uids >= 0) & (np.array([len(s.pages) for s in segs]) >= held), held, 0)
+        has, held = np.array([len(s.pages) for s in segs], dtype=np.int64), self._device_held[slots]
+        if (need > np.minimum(has, self.max_pages)).any():
+            i = int(np.flatnonzero(need > np.minimum(has, self.max_pages))[0])
+            raise IndexError(f"the request in row {slots[i]} needs {need[i]} pages: it has {has[i]}, and a row holds {self.max_pages}")
+        held = np.where((self._device_uid[slots] == uids) & (uids >= 0) & (has >= held), held, 0)
         out[:n] = held
         at = n
         for i in np.flatnonzero(need > held).tolist():

@@ -103,3 +103,25 @@ def test_adapters_of_a_family_without_a_native_runner_are_refused(monkeypatch):
     args = build_parser().parse_args(["serve", "random:qwen4-exp-tiny", "--low-rank-slots", "2", "--execution-mode", "cuda"])
     with pytest.raises(SystemExit, match="low-rank adapters"):
         build_backend(args, [0], 1, parse_speculative_config(None), 8, 8)
+
+
+# ------------------------------------------------------------------------------------------------- steps laid out on the device
+def test_a_step_that_lacks_pages_is_not_staged_for_the_device():
+    """As the host's layout: an error before anything is launched, and what the device's rows hold is still known."""
+    from cubic_serve_b200.executor.gpu_executor import BatchBuilder, Segment
+    b = BatchBuilder(4, 128, 96, 4, 2, "cpu")                         # six pages a row
+    good = Segment(0, [1] * 20, 0, [7, 8], True, uid=5)
+
+    def stage(*segs):
+        b._fill(list(segs), lengths=True)
+        n = b.stage_layout(list(segs))
+        return b.given_host[:len(segs) + n].tolist()
+
+    assert stage(good) == [0, 7, 8]
+    for bad in (Segment(1, [1], 16, [3], True, uid=6), Segment(1, [1] * 40, 0, [3, 4], True, uid=6), Segment(1, [1] * 3, 30, [], True, uid=6),
+                Segment(1, [1], 96, list(range(20, 27)), True, uid=6), Segment(1, [1] * 60, 50, list(range(20, 27)), True, uid=6)):
+        for order in ((bad, good), (good, bad)):
+            with pytest.raises(IndexError, match="pages"):
+                stage(*order)
+    assert stage(Segment(0, [1], 20, [7, 8], True, uid=5)) == [2] and stage(Segment(0, [1] * 13, 21, [7, 8, 9], True, uid=5)) == [2, 9]
+    assert stage(Segment(1, [1], 95, list(range(20, 26)), True, uid=6), Segment(0, [1], 34, [7, 8, 9], True, uid=5)) == [0, 3, *range(20, 26)]
