@@ -435,16 +435,19 @@ class GpuExecutor:
         self.stage = self.builder.stage
         self._fill = self.builder._fill
         self.invalidate_page_rows = self.builder.invalidate_page_rows
+        v_local = runner.w.lm_head.n
+        self.logits = torch.empty(max_rows, v_local, dtype=getattr(runner, "logits_dtype", torch.bfloat16), device=self.device)
+        # a step's sampled ids, behind what its layout on the device says of it: one copy brings both
+        self._result = torch.zeros(4 + max_rows * rows_per_request, dtype=torch.int32, device=self.device)
+        self.out_ids = self._result[4:]
+        # two result buffers: a step may be launched before the previous step's ids have been read (``launch`` / ``collect``)
+        self._result_host = torch.zeros(2, self._result.numel(), dtype=torch.int32, pin_memory=torch.cuda.is_available())
+        self.out_host = self._result_host[:, 4:]
         self.layout = None
         if device_layout and type(self) is GpuExecutor:
             st = self.stage
             self.layout = K.StepLayout(st.max_tokens, st.max_rows, st.max_row_blocks, self.device, into={
-                **{name: st.d[name] for name in ("positions", "slots", "rb_req", "rb_qstart", "rb_qcount", "rb_ctx")}, "row0": st.d["seg_row0"]})
-        v_local = runner.w.lm_head.n
-        self.logits = torch.empty(max_rows, v_local, dtype=getattr(runner, "logits_dtype", torch.bfloat16), device=self.device)
-        self.out_ids = torch.zeros(max_rows * rows_per_request, dtype=torch.int32, device=self.device)
-        # two result buffers: a step may be launched before the previous step's ids have been read (``launch`` / ``collect``)
-        self.out_host = torch.zeros(2, max_rows * rows_per_request, dtype=torch.int32, pin_memory=torch.cuda.is_available())
+                **{name: st.d[name] for name in ("positions", "slots", "rb_req", "rb_qstart", "rb_qcount", "rb_ctx")}, "row0": st.d["seg_row0"], "totals": self._result[:4]})
         self.use_graphs = use_graphs
         self.graph_masks = False         # True once decode graphs were captured with the mask buffer as an input
         self.graph_rt = CudaGraphRuntime(resources=(0, 1))      # capture -> qualify -> seal -> replay; result-buffer leases
@@ -763,10 +766,12 @@ class GpuExecutor:
                 launches = self.runner.launches_per_step
             if self.timing:
                 self._ev[k][1].record(self.stream)
-            if rows:
+            if laid_out:
+                self._result_host[k, :4 + rows].copy_(self._result[:4 + rows], non_blocking=True)
+            elif rows:
                 self.out_host[k, :rows].copy_(self.out_ids[:rows], non_blocking=True)
             self._done[k].record(self.stream)
-        return {"k": k, "rows": rows, "h2d": h2d, "launches": launches}
+        return {"k": k, "rows": rows, "h2d": h2d, "launches": launches, "laid_out": laid_out}
 
     def _poison_padding(self, rows: int, cap: int) -> None:
         """Audit facility (``guardrail/graph_audit.py``): the padding rows ``[rows, cap)`` of a decode bucket get random
@@ -783,14 +788,18 @@ class GpuExecutor:
                 attn[rows:cap].fill_(float("nan"))
 
     def collect(self, handle: dict) -> np.ndarray:
-        """Wait for a launched step and return its sampled ids (host array)."""
+        """Wait for a launched step and return its sampled ids (host array).  A step that its layout on the device could not place is an
+        error: rows without a cache slot attend to nothing, and their ids mean nothing."""
         k, rows = handle["k"], handle["rows"]
         self._done[k].synchronize()
         self.graph_rt.leases.release(self._leases[k])
         self._leases[k] = None
         self.h2d_bytes_last = handle["h2d"]
         self.kernel_launches_last = handle["launches"]
-        self.d2h_bytes_last = rows * 4
+        self.d2h_bytes_last = rows * 4 + (16 if handle["laid_out"] else 0)
         if self.timing:
             self.device_ms.append(self._ev[k][0].elapsed_time(self._ev[k][1]))
+        if handle["laid_out"] and self._result_host[k, 3]:
+            self.builder.forget_device_rows()
+            K.StepLayout.raise_if(int(self._result_host[k, 3]))
         return self.out_host[k, :rows].numpy().copy()

@@ -775,9 +775,13 @@ class StepLayout:
 
     def check(self) -> None:
         """Raise if the last layout met a request that it could not place (reads ``totals``: waits for the GPU)."""
-        wrong = int(self.totals[3].item())
+        self.raise_if(int(self.totals[3].item()))
+
+    @classmethod
+    def raise_if(cls, wrong: int) -> None:
+        """The error that ``totals[3]`` stands for, 0: none."""
         if wrong:
-            raise RuntimeError("step layout: " + ", ".join(w for bit, w in self.WRONG.items() if wrong & bit))
+            raise RuntimeError("step layout: " + ", ".join(w for bit, w in cls.WRONG.items() if wrong & bit))
 
 
 def step_layout(request: torch.Tensor, start: torch.Tensor, count: torch.Tensor, held: torch.Tensor | None, pages: torch.Tensor,

@@ -117,3 +117,38 @@ def test_ranks_that_are_not_in_use_reach_nothing(rows, rank):
     plan = K.adapter_rows(torch.tensor(ids.tolist(), dtype=I32, device=DEV), K.AdapterRows(rows, 3, 2 * rank, DEV))
     got = K.adapter_add(x, y, bank, plan, out=torch.empty_like(y))
     assert bool(((got.double() - want).abs() <= err).all()) and torch.equal(got[3::4], y[3::4])
+
+
+# ------------------------------------------------------------------------------------------------- served steps
+def _laid_out(**kw):
+    from test_gpu_step_serving import _executor
+    return _executor(device_layout=True, **kw)
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_a_step_that_the_device_could_not_place_is_an_error(graphs):
+    """Pages that go missing between staging and layout: the step's ids are not handed out, and the executor serves on."""
+    from cubic_serve_b200.executor.gpu_executor import Segment
+    ex = _laid_out(graphs=graphs)
+    if graphs:
+        ex.capture_decode_graphs([1, 2, 4, 8])
+    seg = lambda start, n, sample=True: Segment(0, list(range(1, n + 1)), start, [5, 6, 7], sample, uid=9)        # noqa: E731
+    first = ex.execute([seg(0, 30)]).tolist()
+    stage = ex.builder.stage_layout
+    for s in (seg(30, 1), seg(30, 10), seg(30, 10, False)):                 # a decode step, a portion with a sampled row, one without
+        ex.builder.forget_device_rows()
+        ex.builder.stage_layout = lambda segs: stage(segs) - 1
+        with pytest.raises(RuntimeError, match="not enough pages"):
+            ex.execute([s])
+        ex.builder.stage_layout = stage
+        assert ex.execute([seg(0, 30)]).tolist() == first
+    # two steps under way: the error belongs to the one that met it
+    a = ex.launch([seg(30, 1)])
+    ex.builder.forget_device_rows()
+    ex.builder.stage_layout = lambda segs: stage(segs) - 1
+    b = ex.launch([seg(31, 1)], feedback_rows=1)
+    ex.builder.stage_layout = stage
+    assert len(ex.collect(a)) == 1
+    with pytest.raises(RuntimeError, match="not enough pages"):
+        ex.collect(b)
+    assert ex.execute([seg(0, 30)]).tolist() == first
