@@ -732,7 +732,8 @@ class GpuExecutor:
         b, rows = self._fill(segs, pad_rows_to=cap, lengths=True) if laid_out else self._fill(segs, pad_rows_to=cap)
         given = self.builder.stage_layout(segs) if laid_out else 0
         whole = self._stage_whole(segs) if whole or "whole" in self.stage.d else 0
-        if cap is not None and getattr(self, "audit_poison_padding", False):
+        poisoned = cap is not None and getattr(self, "audit_poison_padding", False)
+        if poisoned:
             self._poison_padding(total, cap)
         k = self._launches & 1
         # the result buffer of this launch must have been collected: a third outstanding launch is an error, not an overwrite
@@ -752,6 +753,8 @@ class GpuExecutor:
                 d = self.stage.d
                 K.step_layout(d["seg_slot"][:n], d["seg_pos0"][:n], d["seg_count"][:n], self.builder.given[:n], self.builder.given[n:n + given], d["page_table"],
                               self.layout, self.builder.qb, tokens=total, blocks=b.num_row_blocks if cap is None else total, pad=cap or 0)
+                if poisoned:                   # the layout made the padding's positions
+                    d["positions"][total:cap].copy_(torch.from_numpy(self.stage.h["positions"][total:cap].copy()))
             if feedback_rows:
                 self.stage.d["token_ids"][:feedback_rows].copy_(self.out_ids[:feedback_rows], non_blocking=True)
             if self.timing:

@@ -152,3 +152,31 @@ def test_a_step_that_the_device_could_not_place_is_an_error(graphs):
     with pytest.raises(RuntimeError, match="not enough pages"):
         ex.collect(b)
     assert ex.execute([seg(0, 30)]).tolist() == first
+
+
+def test_padding_is_poisoned_in_steps_laid_out_on_the_device_too():
+    """The audit of padding rows: positions and ids of the padding are the poison's when the graph runs, and no real row shows them."""
+    from cubic_serve_b200.executor.gpu_executor import Segment
+    outs = []
+    for poison in (False, True):
+        ex = _laid_out()
+        ex.capture_decode_graphs([4, 8])
+        segs = lambda start, n: [Segment(i, [3 + i] * n, start, [2 * i + 1, 2 * i + 2], True, uid=i) for i in range(5)]        # noqa: E731
+        ex.execute(segs(0, 20))
+        ex.audit_poison_padding = poison
+        outs.append((ex.execute(segs(20, 1)).tolist(), ex.logits[:5].clone()))
+        torch.cuda.synchronize()
+        positions, host = ex.stage.d["positions"][:8].tolist(), ex.stage.h["positions"][5:8].tolist()
+        assert positions[:5] == [20] * 5 and ex.stage.d["slots"][5:8].tolist() == [-1] * 3 and ex.stage.d["rb_qcount"][5:8].tolist() == [0] * 3
+        if poison:
+            assert positions[5:] == host and any(positions[5:]), "the poison reached the device"
+        else:
+            assert positions[5:] == [0] * 3
+    assert outs[0][0] == outs[1][0] and torch.equal(outs[0][1], outs[1][1])
+
+
+def test_the_graph_audit_of_an_executor_with_layout_on_the_device():
+    from cubic_serve_b200.guardrail.graph_audit import audit_decode_graphs
+    r = np.random.default_rng(0)
+    rep = audit_decode_graphs(_laid_out, [r.integers(0, 1000, 12 + 3 * i).tolist() for i in range(3)], (4, 8))
+    assert rep.poisoned_padding_bit_identical and rep.poisoned_padding_finite and rep.permutation_bit_identical
