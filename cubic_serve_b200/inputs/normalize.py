@@ -200,18 +200,20 @@ def normalize_openai_chat_completions(body: Any, default_model: str | None = Non
     seed = body.get("seed")
     _require(seed is None or (isinstance(seed, int) and not isinstance(seed, bool)), "seed must be an integer", "seed")
     _require(isinstance(body.get("whole_vocabulary", False), bool), "whole_vocabulary must be true or false", "whole_vocabulary")
+    whole, min_p = body.get("whole_vocabulary", False), float(_as_number(body, "min_p", 0.0))
     tlp = body.get("top_logprobs") or 0
     _require(isinstance(tlp, int) and 0 <= tlp <= 20, "top_logprobs must be in [0, 20]", "top_logprobs")
     sampling = SamplingMeta(
         temperature=float(_as_number(body, "temperature", _default(sampling_defaults, "temperature", 1.0))),
         top_p=float(_as_number(body, "top_p", _default(sampling_defaults, "top_p", 1.0))),
-        top_k=int(_as_number(body, "top_k", _default(sampling_defaults, "top_k", 0))),
+        # the deployment's top_k is the one of the sampler of 20: a request for all tokens has only its own
+        top_k=int(_as_number(body, "top_k", 0 if whole or min_p > 0 else _default(sampling_defaults, "top_k", 0))),
         seed=seed, max_tokens=max_tokens, stop=_stops(body.get("stop")),
         stop_token_ids=tuple(int(t) for t in (body.get("stop_token_ids") or [])),
         presence_penalty=float(_as_number(body, "presence_penalty", 0.0, -2.0, 2.0)),
         frequency_penalty=float(_as_number(body, "frequency_penalty", 0.0, -2.0, 2.0)),
         logprobs=bool(body.get("logprobs", False)), top_logprobs=tlp,
-        whole_vocabulary=body.get("whole_vocabulary", False), min_p=float(_as_number(body, "min_p", 0.0)))
+        whole_vocabulary=whole, min_p=min_p)
     tools, choice = _openai_tools(body)
     structured = _openai_structured(body)
     _require(not (structured.kind != StructuredKind.NONE and choice.mode in ("required", "named")),

@@ -125,3 +125,16 @@ def test_a_step_that_lacks_pages_is_not_staged_for_the_device():
                 stage(*order)
     assert stage(Segment(0, [1], 20, [7, 8], True, uid=5)) == [2] and stage(Segment(0, [1] * 13, 21, [7, 8, 9], True, uid=5)) == [2, 9]
     assert stage(Segment(1, [1], 95, list(range(20, 26)), True, uid=6), Segment(0, [1], 34, [7, 8, 9], True, uid=5)) == [0, 3, *range(20, 26)]
+
+
+# ------------------------------------------------------------------------------------------------- requests
+def test_whole_vocabulary_requests_are_not_cut_to_the_checkpoints_top_k():
+    """A checkpoint's recommended ``top_k`` (kept as 20 at most, for the sampler of 20) is the default of requests to that sampler alone."""
+    from cubic_serve_b200.inputs.normalize import normalize_openai_chat_completions as n
+    body, defaults = {"model": "m", "messages": [{"role": "user", "content": "x"}]}, {"temperature": 0.6, "top_p": 0.95, "top_k": 20}
+    top_k = lambda **kw: n({**body, **kw}, "m", defaults).sampling.top_k        # noqa: E731
+    assert top_k() == 20 and top_k(min_p=0.0) == 20 and top_k(whole_vocabulary=False) == 20 and top_k(min_p=None) == 20
+    assert top_k(whole_vocabulary=True) == 0 and top_k(min_p=0.05) == 0 and top_k(whole_vocabulary=True, top_k=None) == 0
+    assert top_k(whole_vocabulary=True, top_k=300) == 300 and top_k(min_p=0.05, top_k=7) == 7 and top_k(whole_vocabulary=True, top_k=0) == 0
+    s = n({**body, "whole_vocabulary": True}, "m", defaults).sampling
+    assert (s.temperature, s.top_p) == (0.6, 0.95), "what else the checkpoint recommends holds"
