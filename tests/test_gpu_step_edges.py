@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from cubic_serve_b200.ops import kernels as K
-from test_gpu_step_operators import _adapter_case, _adapter_truth
+from test_gpu_step_operators import _adapter_case, _adapter_truth, _check_adapter
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -119,6 +119,61 @@ def test_ranks_that_are_not_in_use_reach_nothing(rows, rank):
     assert bool(((got.double() - want).abs() <= err).all()) and torch.equal(got[3::4], y[3::4])
 
 
+@pytest.mark.parametrize("rows,slots", [(1, 8), (48, 16), (200, 5), (513, 3), (900, 40)])
+@pytest.mark.parametrize("rank,widths", [(16, (96, 32)), (64, (64, 32, 32))])
+def test_a_row_keeps_its_bits_whatever_its_neighbours_are(rows, slots, rank, widths):
+    """As many rows and slots: a row's result is the same bits wherever it stands, whatever the other rows hold and whichever adapters these name."""
+    k = 1100 // 8 * 8
+    x, y, a, b, scale = _adapter_case(rows, slots, rank, k, widths, None, seed=rows)
+    bank, plan = K.AdapterBank(a, b, scale, widths), K.AdapterRows(rows, slots, len(widths) * rank, DEV)
+    r = np.random.default_rng(rows)
+    mine = x[0].clone(), y[0].clone()
+    seen = []
+    for trial in range(6):
+        at = int(r.integers(0, rows)) if trial else 0
+        ids = r.integers(-1, slots, rows).astype(np.int32) if trial % 2 else np.full(rows, slots // 2, dtype=np.int32)
+        ids[at] = slots // 2
+        x2, y2 = x[torch.from_numpy(r.permutation(rows)).to(DEV)] * (1.0 + trial), y.clone()
+        x2[at], y2[at] = mine
+        K.adapter_rows(torch.from_numpy(ids).to(DEV), plan)
+        seen.append(K.adapter_add(x2, y2, bank, plan, out=torch.empty_like(y) if trial % 3 else None)[at].clone())
+    assert all(torch.equal(seen[0], s) for s in seen[1:])
+
+
+def test_a_row_among_other_numbers_of_rows_is_within_its_bound():
+    """The order of the sums follows the numbers of rows and slots: the same row alone and among 47, 511, 512 and 1200 others is within the bound each time."""
+    k, rank, widths = 2048, 32, (128, 64)
+    for slots in (2, 60):
+        x, y, a, b, scale = _adapter_case(1201, slots, rank, k, widths, None, seed=slots)
+        bank = K.AdapterBank(a, b, scale, widths)
+        want, err = _adapter_truth(x[:1], y[:1], a, b, scale, widths, np.array([1]))
+        for rows in (1, 48, 512, 513, 1201):
+            ids = torch.arange(1, rows + 1, dtype=I32, device=DEV) % slots
+            plan = K.adapter_rows(ids, K.AdapterRows(rows, slots, 2 * rank, DEV))
+            got = K.adapter_add(x[:rows], y[:rows], bank, plan, out=torch.empty(rows, 192, device=DEV, dtype=torch.bfloat16))
+            assert bool(((got[:1].double() - want).abs() <= err).all())
+
+
+@pytest.mark.parametrize("rows,slots,rank,k,widths,ranks", [
+    (513, 3, 16, 520, (96, 32, 32), None), (640, 5, 32, 264, (64, 64, 64), None), (777, 2, 64, 136, (128, 32, 32), None), (600, 4, 128, 264, (64, 32, 32), None), (1025, 9, 20, 72, (32, 40), None),
+    (530, 3, 32, 512, (256,), None), (700, 6, 64, 200, (96, 32), (64, 0, 5, 33, 1, 17)), (640, 4, 128, 136, (96,), (128, 0, 70, 3)), (520, 1, 48, 1032, (64, 64, 32, 32), None),
+    (2000, 600, 16, 64, (64, 64), None), (513, 2, 16, 8, (8,), (16, 9)),
+])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_many_rows_of_every_rank_against_64_bits(rows, slots, rank, k, widths, ranks, in_place):
+    """More rows than the launch for few takes: three and four sections, every stored rank, ranks in use, strides, in place."""
+    ids = np.random.default_rng(rows).integers(-1, slots + 1, rows)
+    _check_adapter(rows, slots, rank, k, widths, ids, seed=rows + rank, ranks=ranks, in_place=in_place, pad_x=16, pad_y=24)
+
+
+def test_many_rows_of_one_adapter_and_of_runs():
+    """Runs that end inside a tile of 64 and a strip of sixteen; one adapter for all rows; rows without one in between."""
+    rows, slots = 1111, 5
+    for ids in (np.full(rows, 2), np.arange(rows) * slots // rows, np.where(np.arange(rows) % 97 < 50, 3, -1), np.arange(rows) % 7 - 1):
+        a = _check_adapter(rows, slots, 32, 136, (64, 32, 32), ids, seed=3, in_place=True, pad_y=8)
+        assert torch.equal(a, _check_adapter(rows, slots, 32, 136, (64, 32, 32), ids, seed=3, pad_y=8))
+
+
 # ------------------------------------------------------------------------------------------------- served steps
 def _laid_out(**kw):
     from test_gpu_step_serving import _executor
@@ -180,3 +235,34 @@ def test_the_graph_audit_of_an_executor_with_layout_on_the_device():
     r = np.random.default_rng(0)
     rep = audit_decode_graphs(_laid_out, [r.integers(0, 1000, 12 + 3 * i).tolist() for i in range(3)], (4, 8))
     assert rep.poisoned_padding_bit_identical and rep.poisoned_padding_finite and rep.permutation_bit_identical
+
+
+def test_prompts_of_many_rows_are_computed_with_their_adapters(tmp_path):
+    """Steps of 700 and 1000 tokens, several adapters and none among them: every prompt's logits are those of a step of its own, within the rounding of
+    bf16 activations (three layers, some ten roundings of 2^-8 in a row), which the adapters move by much more."""
+    from cubic_serve_b200.executor.gpu_executor import GpuExecutor, Segment
+    from cubic_serve_b200.models.decoder import DecoderRunner, random_decoder_weights
+    from test_gpu_step_serving import CFG, _adapter
+    ranks = (4, 16, 40, 64)
+    for i, rank in enumerate(ranks):
+        _adapter(tmp_path / f"a{i}", 30 + i, rank=rank, modules=("q_proj", "v_proj", "o_proj", "gate_proj", "down_proj") if i % 2 else ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj"))
+    runner = DecoderRunner(CFG, random_decoder_weights(CFG, torch.device(DEV), seed=3, std=0.05), num_pages=160, max_tokens=1024, max_requests=8, low_rank=(4, 64))
+    ex = GpuExecutor(runner, max_rows=8, max_prefill_tokens=1024, max_model_len=512, use_graphs=False)
+    for i in range(4):
+        ex.load_adapter(f"a{i}", tmp_path / f"a{i}")
+    r = np.random.default_rng(4)
+    for lengths, slots in (((150, 90, 201, 160, 99), (0, -1, 3, 1, 2)), ((331, 13, 400, 257), (1, 2, 2, -1))):
+        prompts = [r.integers(0, CFG.vocab_size, n).tolist() for n in lengths]
+        segs = [Segment(i, p, 0, list(range(1 + 32 * i, 33 + 32 * i)), logit_offsets=[len(p) - 1], adapter=s) for i, (p, s) in enumerate(zip(prompts, slots))]
+
+        def logits(some):
+            ex.invalidate_page_rows(range(8))
+            return torch.from_numpy(np.concatenate(ex.execute_logits(some)))
+
+        together, alone = logits(segs), torch.cat([logits([s]) for s in segs])
+        for s in segs:
+            s.adapter = -1
+        without = logits(segs)
+        off, moved = (together - alone).norm(dim=1) / alone.norm(dim=1), (without - alone).norm(dim=1) / alone.norm(dim=1)
+        named = torch.tensor(slots) >= 0
+        assert bool((off < 0.1).all()) and bool((moved[named] > 0.3).all()) and bool((moved[~named] < 0.1).all()), (off, moved)
