@@ -141,7 +141,8 @@ struct CbAdapter {
   const void* a;                         // bf16 [slots, ceil(k / 32), sections * rank, 32]: what is read together lies together
   const void* b;                         // bf16 [slots, n, rank]
   const float* scale;                    // [slots]
-  const uint32_t* ranks;                 // [slots] ranks in use, a byte a section, or null: all
+  const int* ranks;                      // [slots] ranks in use by any section
+  const uint32_t* section_ranks;         // [slots] ranks in use, a byte a section; B is zero behind them
   const int* order; const int* items; const int* strips;         // adapter_rows_kernel's
   void* hi; void* lo;                    // bf16 [rows, sections * rank]: h as a sum of two
   int rows, slots, k, n, rank, sections;
@@ -151,10 +152,9 @@ struct CbAdapter {
 namespace cb {
 
 // A section has ranks of its own (none, if the adapter leaves it as it is): an infinity in x makes NaN of the zeros behind them, and that must meet no column.
-__device__ __forceinline__ uint32_t ranks_of(const CbAdapter& p, int slot) { return p.ranks ? p.ranks[slot] : 0xffffffffu; }
-__device__ __forceinline__ int ranks_in(uint32_t ranks, int section) { return static_cast<int>(ranks >> 8 * section & 0xffu); }
-__device__ __forceinline__ int most_ranks(uint32_t ranks) {
-  const uint32_t two = __vmaxu4(ranks, ranks >> 16);
+__device__ __forceinline__ int ranks_in(uint32_t section_ranks, int section) { return static_cast<int>(section_ranks >> 8 * section & 0xffu); }
+__device__ __forceinline__ int most_ranks(uint32_t section_ranks) {
+  const uint32_t two = __vmaxu4(section_ranks, section_ranks >> 16);
   return static_cast<int>(max(two & 0xffu, two >> 8 & 0xffu));
 }
 
@@ -223,7 +223,7 @@ adapter_few_kernel(const CbAdapter p, int splits) {
       }
       continue;
     }
-    const uint32_t used = ranks_of(p, slot);
+    const uint32_t used = p.section_ranks[slot];
     const float scale = p.scale[slot];
     const bool in0 = g < rows, in1 = g + 8 < rows, both = rows > 8;
     const __nv_bfloat16* x0 = static_cast<const __nv_bfloat16*>(p.x) + (in0 ? p.order[first + g] * p.ldx : 0) + c * 8;
@@ -232,7 +232,7 @@ adapter_few_kernel(const CbAdapter p, int splits) {
       const __nv_bfloat16* A = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<size_t>(slot) * turns * rt + q0 * 16) * 32 + lane * 8;
       bool on[4];                                                     // tiles of sixteen that hold ranks in use
 #pragma unroll
-      for (int t = 0; t < 4; ++t) on[t] = q0 + t < tiles && (q0 + t) % R16 * 16 < ranks_in(used, (q0 + t) / R16);
+      for (int t = 0; t < 4; ++t) on[t] = q0 + t < tiles && (R16 == 1 ? used != 0 : (q0 + t) % R16 * 16 < ranks_in(used, (q0 + t) / R16));
       float acc[4][2][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -467,7 +467,7 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
     const int item = u / parts, r0 = (u - item * parts) * NR;
     const int slot = p.items[1 + 3 * item], first = p.items[2 + 3 * item], rows = p.items[3 + 3 * item];
     if (slot < 0) continue;
-    const uint32_t used = ranks_of(p, slot);
+    const int used = min(p.rank, max(0, p.ranks[slot]));
     const int row = tid >> 3, ch = tid & 7;                           // a thread's 16 bytes of rows row, row + 32, ...
     const __nv_bfloat16 *xr[2], *ar[AR];
     bool xin[2], ain[AR];
@@ -479,7 +479,7 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
 #pragma unroll
     for (int i = 0; i < AR; ++i) {
       const int r = r0 + row + 32 * i;
-      ain[i] = row + 32 * i < NR && r < rt && r % p.rank < ranks_in(used, r / p.rank);
+      ain[i] = row + 32 * i < NR && r < rt && r % p.rank < used;
       ar[i] = static_cast<const __nv_bfloat16*>(p.a) + ((static_cast<size_t>(slot) * turns + ch / 4) * rt + (ain[i] ? r : 0)) * 32 + ch % 4 * 8;
     }
     const uint32_t to0 = base + row * 128 + ((ch ^ (row & 7)) << 4);
@@ -530,6 +530,7 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     const float scale = p.scale[slot];
+    const uint32_t by_section = p.section_ranks[slot];
     float* part = reinterpret_cast<float*>(st);                       // [64][SP]
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -553,7 +554,7 @@ adapter_down_tile_kernel(const CbAdapter p, int splits) {
       } else {
         v = part[r * SP + k];
       }
-      put_h(p, v, scale, (r0 + k) % p.rank < ranks_in(used, (r0 + k) / p.rank), static_cast<size_t>(first + r) * rt + r0 + k);
+      put_h(p, v, scale, (r0 + k) % p.rank < ranks_in(by_section, (r0 + k) / p.rank), static_cast<size_t>(first + r) * rt + r0 + k);
     }
     if (splits > 1) cluster_sync_all(); else __syncthreads();
   }
@@ -652,7 +653,7 @@ adapter_up_kernel(const CbAdapter p) {
     for (int s = s0; s < s1; ++s) {
       if (strip.x != held) {
         held = strip.x;
-        used = held < 0 ? 0 : ranks_in(ranks_of(p, held), sec);
+        used = held < 0 ? 0 : min(R, max(0, p.ranks[held]));
         // product t, places g and g + 8: columns 2 t and 2 t + 1 of the lane's
         const __nv_bfloat16* B = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<size_t>(max(held, 0)) * n + col) * R;
 #pragma unroll

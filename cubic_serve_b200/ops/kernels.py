@@ -848,9 +848,9 @@ class AdapterBank:
         ranks = torch.full((slots,), rank, dtype=torch.int32, device=a.device) if ranks is None else ranks.clamp(0, rank)
         b.masked_fill_(torch.arange(full, device=b.device) >= ranks.view(slots, 1, 1), 0)       # h is zero there, whatever A and x hold
         self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
-        self._section_ranks = ranks.view(slots, 1).to(torch.uint8).repeat(1, 4)        # what the kernels go by: a byte a section
+        self._section_ranks = ranks.view(slots, 1).to(torch.uint8).repeat(1, 4)        # a byte a section
         self.slots, self.k, self.n, self.rank, self.sections = slots, k, n, full, S
-        self._at = (a.data_ptr(), b.data_ptr(), scale.data_ptr(), self._section_ranks.data_ptr())
+        self._at = (a.data_ptr(), b.data_ptr(), scale.data_ptr(), ranks.data_ptr(), self._section_ranks.data_ptr())
         self._shape = (slots, self.k, n, full, S, *self.widths, *(0,) * (4 - S))
 
     @property

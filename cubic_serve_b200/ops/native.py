@@ -565,7 +565,7 @@ class ScoredMoeStruct(ctypes.Structure):
 
 # Arguments of the operators around a step's shared layers, packed in one call: an operator of 2 us has no time for a field at a time.
 STEP_LAYOUT = struct.Struct("@15P9i4x")                      # CbStepLayout, csrc/step_layout.cu
-ADAPTER = struct.Struct("@PqPqPq9P10i")                      # CbAdapter, csrc/adapters.cu
+ADAPTER = struct.Struct("@PqPqPq10P10i")                      # CbAdapter, csrc/adapters.cu
 VOCABULARY = struct.Struct("@PqPq11P4i")                     # CbVocabulary, csrc/sample_vocabulary.cu
 
 
