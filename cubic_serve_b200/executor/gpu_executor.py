@@ -243,14 +243,19 @@ class BatchBuilder:
         """The device's table was overwritten by the host's: the next layout there starts every row anew."""
         self._device_uid[:] = -2
 
-    def stage_layout(self, segs: list[Segment]) -> int:
-        """Stage what ``K.step_layout`` needs of a step besides the lengths that ``_fill`` staged: the pages that the device's rows hold
-        and those that they are given.  Returns how many these are.  A request that has too few pages, or more than a row holds, is an
-        error before anything is staged."""
+    def make_layout_buffers(self) -> None:
+        """What ``stage_layout`` fills.  An executor makes it before its first step: memory of the caller's stream, that the steps' stream
+        is to write, has to be free of what the caller's stream still does with it."""
         if self.given is None:
             n = self.max_rows * (self.max_pages + 1)
             self.given_host = torch.empty(n, dtype=torch.int32, pin_memory=torch.cuda.is_available())
             self.given = torch.empty(n, dtype=torch.int32, device=self.device)
+
+    def stage_layout(self, segs: list[Segment]) -> int:
+        """Stage what ``K.step_layout`` needs of a step besides the lengths that ``_fill`` staged: the pages that the device's rows hold
+        and those that they are given.  Returns how many these are.  A request that has too few pages, or more than a row holds, is an
+        error before anything is staged."""
+        self.make_layout_buffers()
         n, h, out = len(segs), self.stage.h, self.given_host.numpy()
         slots, uids = h["seg_slot"][:n], np.array([s.uid for s in segs], dtype=np.int64)
         need = (h["seg_pos0"][:n] + h["seg_count"][:n] + K.PAGE_TOKENS - 1) // K.PAGE_TOKENS
@@ -446,6 +451,7 @@ class GpuExecutor:
         self.layout = None
         if device_layout and type(self) is GpuExecutor:
             st = self.stage
+            self.builder.make_layout_buffers()
             self.layout = K.StepLayout(st.max_tokens, st.max_rows, st.max_row_blocks, self.device, into={
                 **{name: st.d[name] for name in ("positions", "slots", "rb_req", "rb_qstart", "rb_qcount", "rb_ctx")}, "row0": st.d["seg_row0"], "totals": self._result[:4]})
         self.use_graphs = use_graphs

@@ -266,3 +266,9 @@ def test_prompts_of_many_rows_are_computed_with_their_adapters(tmp_path):
         off, moved = (together - alone).norm(dim=1) / alone.norm(dim=1), (without - alone).norm(dim=1) / alone.norm(dim=1)
         named = torch.tensor(slots) >= 0
         assert bool((off < 0.1).all()) and bool((moved[named] > 0.3).all()) and bool((moved[~named] < 0.1).all()), (off, moved)
+
+
+def test_buffers_of_the_layout_are_there_before_the_first_step():
+    """Made in the constructor, which waits for the caller's stream: a step's stream writes no memory that the caller's still uses."""
+    ex = _laid_out(graphs=False)
+    assert ex.builder.given.is_cuda and ex.builder.given.numel() == ex.builder.given_host.numel() >= 8 * (256 // 16 + 1)
