@@ -792,8 +792,9 @@ def step_layout(request: torch.Tensor, start: torch.Tensor, count: torch.Tensor,
     tokens; ``held``: pages in the row already (None: those of ``start`` tokens).  Requests take their missing pages from
     ``pages`` (int32, in their order) into ``table`` (int32 ``[rows, width]``, written in place).  ``block``: positions of a
     row block.  ``tokens`` / ``blocks``: rows and row blocks to write at most; rows and row blocks behind the last one up to
-    ``pad`` become padding (slot -1, nothing to attend to), what is behind them stays.  A request that cannot be placed gets
-    no slots and attends to nothing; ``out.totals[3]`` says why."""
+    ``pad`` become padding (slot -1, nothing to attend to), what is behind them stays.  A request that cannot be placed
+    attends to nothing and ``out.totals[3]`` says why: one that is too long, or of a row that is not there, gets no slots and
+    takes no pages; one that ``pages`` ends in front of has slots on the pages that it got."""
     n, i32 = start.numel(), torch.int32
     _require(n <= out.max_requests and 0 <= tokens <= out.max_tokens and 0 <= blocks <= out.max_blocks and pad <= out.max_tokens and pad <= out.max_blocks,
              "more rows, row blocks or requests than the layout holds")
