@@ -18,6 +18,8 @@ namespace cb {
 
 // Up to here a work item is sixteen rows and A is streamed through registers, from here on it is 64 and A and x come by tiles.  A layer of rank 16, by tiles and
 // by sixteens: 331 rows over 2 adapters 82 and 57 us; 640 over 2, 16 and 64 76, 86, 112 and 82, 87, 128; 1024 98, 103, 122 and 90, 93, 147; 2048 143, 153, 184 and 151, 154, 251.
+// 640 rows of rank 32 89, 98, 130 and 95, 100, 154; of 64 130, 138, 206 and 133, 139, 230; of 128 176, 208, 354 and 219, 229, 398.  1024 rows of rank 32 112, 117, 140 and 102, 106, 171;
+// of 64 162, 174, 215 and 138, 145, 248; of 128 227, 265, 364 and 223, 237, 431: with few adapters the sixteens are ahead beyond the limit, with many they are not.
 static constexpr int kAdapterFewRows = 512;
 static constexpr int adapter_item_rows(int rows) { return rows <= kAdapterFewRows ? 16 : 64; }
 static constexpr int kAdapterMaxSlots = 1023;
@@ -191,7 +193,7 @@ __device__ __forceinline__ void put_h(const CbAdapter& p, float v, float scale, 
 // Second product: as in adapter_up_kernel, with h from shared memory and sixteen rows at most.
 //
 // A layer's four projections (4096 -> 6144 of three sections, 4096 -> 4096, 4096 -> 24576 of two, 12288 -> 4096) one after the other: one row of rank 16 takes
-// 27 us (a launch's start, two waits for the cluster and four trips to memory, 6.7 us each), 48 rows over 12 adapters of rank 32 46 us, 256 rows over 64 of rank
+// 27 us (a launch's start, two waits for the cluster and four trips to memory, 6.7 us each), 48 rows, 36 of them over nine adapters of rank 32, 46 us, 256 rows, 240 over 60 of rank
 // 64 133 us (634 MB: 4.8 TB/s; with a launch for each product 27, 50 and 150).
 template <int R16, int MT>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
@@ -756,8 +758,8 @@ static int adapter_entries(int rows, int slots, int per) {
 static int adapter_items(int rows, int slots) { return adapter_entries(rows, slots, adapter_item_rows(rows)); }
 static int adapter_strips(int rows, int slots) { return adapter_entries(rows, slots, 16); }
 
-// CTAs that share k: as long as two find room on every SM.  A layer by the most CTAs: 256 rows over 64 adapters of rank 64 (one launch) 160 185 us, 320 133,
-// 640 154; 48 rows over 12 80 63 us, 160 and more 46; 8192 rows of rank 16 (tiles) 148 456 us, 320 408, 592 426.  Clusters of sixteen change nothing.
+// CTAs that share k: as long as two find room on every SM.  A layer by the most CTAs: 256 rows, 240 over 60 adapters of rank 64 (one launch), 160 185 us, 320 133,
+// 640 154; 48 rows, 36 over nine, 80 63 us, 160 and more 46; 8192 rows of rank 16 (tiles) 148 456 us, 320 408, 592 426.  Clusters of sixteen change nothing.
 static int adapter_splits(int units, int k) {
   int splits = 1;
   while (splits < 8 && units * splits * 2 <= 320 && k / (splits * 2) >= 256) splits *= 2;

@@ -1083,7 +1083,7 @@ extern "C" int cb_sample_vocabulary(const CbVocabulary* p, void* stream) {
   if (reinterpret_cast<uintptr_t>(p->logits) % (p->f32 ? 4 : 2)) return -11;
   if (p->rows == 0) return 0;
   // CTAs of a row: as many as find an SM each, with work for each.  bf16 rows of 151936 tokens with top-k, limit 296 -> 148: 20 rows 21.5 -> 18.7 us,
-  // 48 23.8 -> 22.4, 74 38 -> 22.6 (clusters that do not fit at once), 100 30.8 -> 25.6.
+  // 48 23.8 -> 22.4, 74 38 -> 22.6 (clusters that do not fit at once), 100 30.8 -> 25.6.  (Other vocabularies were not measured.)
   int team = 1;
   while (team < kTeamMax && static_cast<long long>(p->rows) * team * 2 <= 148 && p->vocab / (team * 2) >= 4096) team *= 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
