@@ -272,3 +272,64 @@ def test_buffers_of_the_layout_are_there_before_the_first_step():
     """Made in the constructor, which waits for the caller's stream: a step's stream writes no memory that the caller's still uses."""
     ex = _laid_out(graphs=False)
     assert ex.builder.given.is_cuda and ex.builder.given.numel() == ex.builder.given_host.numel() >= 8 * (256 // 16 + 1)
+
+
+@pytest.mark.parametrize("model", ["layered-tiny", "layered-seq-tiny", "layered-streams-tiny", "layered-gated-tiny"])
+def test_layered_decoders_are_laid_out_on_the_device_as_on_the_host(model):
+    """Layered decoders through the server's engine: prompts in portions, decode, draws from the whole vocabulary."""
+    from cubic_serve_b200.cli import build_parser, parse_speculative_config
+    from cubic_serve_b200.runtime.scheduler import SamplingParams
+    from cubic_serve_b200.runtime.serving import build_backend
+    outs = []
+    for flags in ((), ("--device-layout",)):
+        args = build_parser().parse_args(["serve", f"random:{model}", "--max-running-requests", "6", "--gpu-memory-gib", "8", "--gpu-reserve-gib", "0.5", "--token-budget", "64",
+                                          "--prefill-chunk-tokens", "48", "--max-model-len", "256", *flags])
+        backend, _ = build_backend(args, [0], 1, parse_speculative_config(None), 8, 8)
+        backend.close()
+        eng = backend.engine
+        assert (eng.executor.layout is not None) == bool(flags)
+        r = np.random.default_rng(3)
+        ids = [eng.add_request(r.integers(0, 200, int(r.integers(3, 90))).tolist(), SamplingParams(max_tokens=9 + i, ignore_eos=True, seed=i, temperature=0.9 * (i % 2), whole_vocabulary=i % 4 == 1, min_p=0.02 if i % 4 == 3 else 0.0))
+               for i in range(9)]
+        reqs = [eng.requests[i] for i in ids]
+        while eng.has_unfinished:
+            eng.step()
+        outs.append([list(q.output) for q in reqs])
+        assert all(len(q.output) == 9 + i for i, q in enumerate(reqs))
+    assert outs[0] == outs[1]
+
+
+@pytest.mark.parametrize("kind", ["experts", "hybrid"])
+def test_decoders_with_experts_and_recurrent_mixers_are_laid_out_on_the_device_as_on_the_host(kind):
+    """Prompts in portions, decode and preemption, with draws from the whole vocabulary."""
+    from dataclasses import replace
+
+    from test_gpu_step_serving import CFG, _engine, _executor, _prompts, _run, _sampling
+    cfg = replace(CFG, family="gqa_moe", num_experts=8, experts_per_token=2, moe_intermediate_size=256, intermediate_size=0) if kind == "experts" else \
+        replace(CFG, family="qwen3_5", num_layers=4, gdn_interval=4, gdn_k_heads=2, gdn_v_heads=4, attn_output_gate=True, rotary_dim=64)
+    outs = []
+    for layout in (False, True):
+        eng = _engine(_executor(cfg, device_layout=layout), pages=48, prefill_chunk_tokens=64, enable_prefix_cache=False)
+        outs.append(_run(eng, [(p, _sampling(max_tokens=10 + i, seed=i, temperature=0.8 * (i % 2), whole_vocabulary=True)) for i, p in enumerate(_prompts(12, 4, 5, 90))]))
+    assert outs[0] == outs[1]
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_steps_laid_out_by_the_host_and_on_the_device_in_turn(graphs):
+    """What happens when requests with media come and go: the block table of either side is whole after steps of the other."""
+    from test_gpu_step_serving import _engine, _executor, _prompts, _run, _sampling
+    requests = [(p, _sampling(max_tokens=14 + i)) for i, p in enumerate(_prompts(12, 14, 5, 90))]
+    outs = []
+    for mixed in (False, True):
+        ex = _executor(graphs=graphs, device_layout=mixed)
+        eng = _engine(ex, pages=44, prefill_chunk_tokens=64)
+        if mixed:
+            launch, layout, turn = ex.launch, ex.layout, np.random.default_rng(2)
+
+            def either(segs, feedback_rows=0):
+                ex.layout = layout if turn.random() < 0.6 else None
+                return launch(segs, feedback_rows)
+
+            ex.launch = either
+        outs.append(_run(eng, requests))
+    assert outs[0] == outs[1]
