@@ -58,6 +58,33 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return r;
 }
 
+// Codes of the channels 4 lane .. 4 lane + 3 of a token of a page, a byte each, with their bias
+template <int BITS>
+__device__ __forceinline__ uint32_t pf_codes_k(const uint8_t* k, int tok, int lane) {
+  if constexpr (BITS == 8) return *reinterpret_cast<const uint32_t*>(k + (lane >> 2) * 256 + tok * 16 + (lane & 3) * 4);
+  const int blk = lane >> 3, high = lane >> 2 & 1, t = lane & 3;
+  uint32_t x = *reinterpret_cast<const uint32_t*>(k + blk * 256 + tok * 16 + t * 4) >> (4 * high) & 0x0F0F0F0Fu;
+  if constexpr (BITS == 6) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(k + kPageTokens * kD / 2 + blk * 128 + (tok & 7) * 16 + t * 4);
+    x |= (tok < 8 ? (high ? w >> 2 : w) : (high ? w << 2 : w << 4)) & 0x30303030u;
+  }
+  return x;
+}
+template <int BITS>
+__device__ __forceinline__ uint32_t pf_codes_v(const uint8_t* v, int tok, int lane) {
+  const int pair = tok >> 1, odd = tok & 1, at = lane ^ ((pair & 3) << 2);
+  if constexpr (BITS == 8) {
+    const uint2 w = *reinterpret_cast<const uint2*>(v + pair * 256 + at * 8);
+    return prmt(w.x, w.y, odd ? 0x7531u : 0x6420u);
+  }
+  uint32_t x = *reinterpret_cast<const uint32_t*>(v + pair * 128 + at * 4) >> (4 * odd) & 0x0F0F0F0Fu;
+  if constexpr (BITS == 6) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(v + kPageTokens * kD / 2 + (pair & 3) * 128 + at * 4);
+    x |= (pair < 4 ? (odd ? w >> 2 : w) : (odd ? w << 2 : w << 4)) & 0x30303030u;
+  }
+  return x;
+}
+
 struct WarpState {
   float m[2];       // running max (log2 domain) for rows g and g+8
   float l[2];       // running partial sum (this lane's columns only)

@@ -978,6 +978,163 @@ def sample_vocabulary(logits: torch.Tensor, out_ids: torch.Tensor, temperature: 
     return out_ids
 
 
+# ------------------------------------------------------------------ drafts in trees, and what requests say about their tokens
+TREE_MAX_REQUESTS, TREE_MAX_NODES, TREE_MAX_GROUP = 1024, 256, 128
+
+
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> int:
+    """Row stride of a matrix of neighbouring elements."""
+    if t.dim() != 2 or (dtype is not None and t.dtype is not dtype) or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{name}: a matrix of neighbouring {'elements' if dtype is None else dtype}")
+    ld = t.stride(0)
+    if t.shape[0] > 1 and ld < t.shape[1]:
+        raise ValueError(f"{name}: rows overlap")
+    return ld
+
+
+def tree_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, request: torch.Tensor, row0: torch.Tensor, count: torch.Tensor,
+                   start: torch.Tensor, masks: torch.Tensor, hq: int, hkv: int, head_dim: int, k_bits: int, v_bits: int, scale: float | None = None,
+                   ws: Workspace | None = None) -> torch.Tensor:
+    """Attention of trees of drafted tokens over the paged quantised cache (``csrc/tree_attn.cu``).
+
+    Request ``i`` of the ``n`` in ``request`` (int32, rows of ``page_table``) has ``start[i]`` tokens in the cache and ``count[i]`` nodes
+    behind them, at the slots ``start[i] + j``, whose queries are the rows ``row0[i] + j`` of ``q`` bf16 ``[rows, hq * 128]``.  A node sees
+    the whole context, and of its tree the nodes whose bits are set in its row of ``masks`` (int32 ``[rows, up to 8]``, bit ``j % 32`` of
+    word ``j / 32``; usually its ancestors and itself: ``runtime.trees.tree_masks``).  A row that sees nothing becomes zeros; rows of no
+    request stay.  ``q`` and ``out`` may be views of wider rows.  A request that is told wrongly (more nodes than ``masks`` has bits, a
+    context that its row of ``page_table`` does not hold) gets zeros, a page that is not there is read as page 0, and
+    ``ws.check_status`` raises in both cases.  Launches that may run at the same time need a ``ws`` of their own each."""
+    n, i32 = request.numel(), torch.int32
+    _require(head_dim == 128, "heads of 128 channels")
+    _require(hkv > 0 and hq % hkv == 0 and hq // hkv <= TREE_MAX_GROUP, "query heads share the key / value heads evenly, up to 128 each")
+    _require(n <= TREE_MAX_REQUESTS, "a launch takes up to 1024 requests")
+    ldq, ldo = _rows(q, "q", torch.bfloat16), _rows(out, "out", torch.bfloat16)
+    (rows, width), at = q.shape, q.data_ptr()
+    _require(width == hq * 128 and out.shape == q.shape, "q and out: a row of all query heads for every node")
+    _require((ldq | ldo) % 8 == 0 and (at | out.data_ptr()) % 16 == 0, "rows of q and out start on 16 bytes")
+    ld, ldm, words = _rows(page_table, "page_table", i32), _rows(masks, "masks", i32), masks.shape[1]
+    _require(masks.shape[0] >= rows and 1 <= words <= TREE_MAX_NODES // 32, "masks: one to eight words for every row")
+    blob = kv_blob_bytes(128, k_bits, v_bits)
+    _require(k_bits in (4, 6, 8) and v_bits in (4, 6, 8) and cache.dtype is torch.uint8 and cache.dim() == 3 and cache.shape[1:] == (hkv, blob) and cache.is_contiguous()
+             and cache.data_ptr() % 16 == 0, "cache: uint8 [pages, hkv, bytes of a page and head]")
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+    _require(0.0 < scale < math.inf, "the scale is above zero")
+    ws = ws or workspace(q.device)
+    packed = native.TREE_ATTN.pack(
+        at, out.data_ptr(), cache.data_ptr(), page_table.data_ptr(), _vector(request, i32, n, "request"), _vector(row0, i32, n, "row0"), _vector(count, i32, n, "count"),
+        _vector(start, i32, n, "start"), masks.data_ptr(), ws.status.data_ptr(), ldq, ldo, ld, ldm, n, rows, page_table.shape[0], page_table.shape[1], cache.shape[0], words,
+        hq, hkv, k_bits, v_bits, scale)
+    if n and rows:
+        _call("cb_tree_attn", (packed,), (q, out, cache, page_table, request, row0, count, start, masks, ws.status))
+    return out
+
+
+def adjust_logits(logits: torch.Tensor, request: torch.Tensor | None, history: torch.Tensor, length: torch.Tensor, prompt: torch.Tensor | None = None,
+                  repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None, presence: torch.Tensor | None = None,
+                  bias: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None, mask: torch.Tensor | None = None,
+                  drafts: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Logits (bf16 or fp32 ``[rows, vocab]``) as the requests want them (``csrc/adjust_logits.cu``); in place without ``out``.
+
+    Row ``r`` belongs to request ``request[r]`` (int32; None: request r; below 0: none, only ``mask`` applies).  ``history`` int32
+    ``[n, most]`` holds the requests' tokens, ``length[n]`` of them, the first ``prompt[n]`` (None: none) the prompt's.  A token of the
+    history has its logit divided (above 0) or multiplied (else) by ``repetition``; one that the output holds ``c`` times is lowered by
+    ``c * frequency + presence``.  ``bias``: ``(first entry of every request int32 [n + 1], tokens int32, values fp32)``; of a token listed
+    twice the later entry counts.  ``mask`` int32 (bit i of a row's words: token i is allowed; one row for all where its row stride is
+    0): the others become -inf.  ``drafts``: ``(tokens int32 [rows], masks int32 [rows, words], row0 int32 [n])`` of trees, as
+    ``tree_attention`` takes them: the tokens of the nodes that a row's mask names count as output, but for node 0, which the
+    history holds.  Tokens outside the vocabulary count for nothing.  fp32 arithmetic, rounded once."""
+    i32, f32 = torch.int32, torch.float32
+    _require(logits.dtype in (torch.bfloat16, f32), "logits are a bf16 or fp32 matrix")
+    ldl = _rows(logits, "logits")
+    rows, vocab = logits.shape
+    _require(1 <= vocab <= 1 << 20 and rows <= 65535, "up to 65535 rows of one to 2^20 logits")
+    ldo = ldl
+    if out is None:
+        out = logits
+    else:
+        ldo = _rows(out, "out", logits.dtype)
+        _require(out.shape == logits.shape, "out: as many logits")
+    ldh = _rows(history, "history", i32)
+    n, most = history.shape
+    _require(most < (1 << 20) - 256, "a history of less than 2^20 tokens")
+    _require(request is not None or n >= rows, "request: whose rows they are")
+    b = (0, 0, 0, 0)
+    if bias is not None:
+        first, ids, values = bias
+        b = (_vector(first, i32, n + 1, "bias"), _vector(ids, i32, 0, "bias"), _vector(values, f32, ids.numel(), "bias"), ids.numel())
+    ldm = lds = words = 0
+    if mask is not None:
+        _require(mask.dtype is i32 and mask.dim() == 2 and mask.shape[0] >= rows and mask.shape[1] * 32 >= vocab and mask.stride(1) == 1, "mask: int32 words of 32 tokens for every row")
+        ldm = mask.stride(0)
+    d = (0, 0, 0)
+    if drafts is not None:
+        tokens, sees, row0 = drafts
+        lds, words = _rows(sees, "drafts", i32), sees.shape[1]
+        _require(sees.shape[0] >= rows and 1 <= words <= TREE_MAX_NODES // 32, "drafts: one to eight words for every row")
+        d = (_vector(tokens, i32, rows, "drafts"), sees.data_ptr(), _vector(row0, i32, n, "drafts"))
+    packed = native.ADJUST.pack(
+        logits.data_ptr(), out.data_ptr(), _vector(request, i32, rows, "request"), history.data_ptr(), _vector(length, i32, n, "length"), _vector(prompt, i32, n, "prompt"),
+        _vector(repetition, f32, n, "repetition"), _vector(frequency, f32, n, "frequency"), _vector(presence, f32, n, "presence"), b[0], b[1], b[2],
+        0 if mask is None else mask.data_ptr(), *d, ldl, ldo, ldh, ldm, lds, rows, vocab, n, most, b[3], words, logits.dtype is f32, 0)
+    if rows:
+        _call("cb_adjust_logits", (packed,), (logits, out, request, history, length, prompt, repetition, frequency, presence, *(bias or ()), mask, *(drafts or ())))
+    return out
+
+
+def verify_tree(target_ids: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, row0: torch.Tensor, count: torch.Tensor, accepted: torch.Tensor,
+                path: torch.Tensor, emitted: torch.Tensor) -> None:
+    """The path through every request's tree of drafts that the target agrees with (``csrc/draft_tree.cu``; chains: ``verify_greedy``).
+
+    ``target_ids`` / ``tokens`` / ``parents`` int32 ``[rows]``: the target's choice behind every node, the nodes' tokens and the node
+    each follows (a lower one; -1 for node 0), request ``i`` having the rows ``row0[i] + j``, ``j < count[i]``.  From node 0 on the
+    target's choice is emitted and the first child that holds it is next.  ``accepted[i]``: drafts on the path; ``path`` /
+    ``emitted`` int32 ``[n, depth]``: its nodes and the ``accepted[i] + 1`` choices along it, -1 behind them; at most ``depth - 1``
+    drafts are accepted."""
+    n, i32 = row0.numel(), torch.int32
+    rows = target_ids.numel()
+    _require(path.dim() == 2 and path.shape == emitted.shape and path.shape[0] >= n and path.shape[1] >= 1 and path.dtype is emitted.dtype is i32 and path.is_contiguous()
+             and emitted.is_contiguous(), "path and emitted: int32, a row of at least one node for every request")
+    packed = native.VERIFY_TREE.pack(
+        _vector(target_ids, i32, rows, "target_ids"), _vector(tokens, i32, rows, "tokens"), _vector(parents, i32, rows, "parents"), _vector(row0, i32, n, "row0"),
+        _vector(count, i32, n, "count"), _vector(accepted, i32, n, "accepted"), path.data_ptr(), emitted.data_ptr(), n, rows, path.shape[1])
+    if n:
+        _call("cb_verify_tree", (packed,), (target_ids, tokens, parents, row0, count, accepted, path, emitted))
+
+
+class LayerCaches:
+    """The layers' caches (uint8 ``[pages, hkv, bytes of a page and head]`` each; layers without pages are left out) for launches
+    that work on all of them."""
+
+    def __init__(self, caches: list[torch.Tensor], hkv: int, head_dim: int, k_bits: int, v_bits: int) -> None:
+        _require(head_dim == 128 and hkv > 0 and k_bits in (4, 6, 8) and v_bits in (4, 6, 8), "heads of 128 channels in 4, 6 or 8 bits")
+        self.caches = [c for c in caches if c.shape[0]]
+        _require(len(self.caches) > 0, "at least one layer with pages")
+        shape, self.device = (self.caches[0].shape[0], hkv, kv_blob_bytes(128, k_bits, v_bits)), self.caches[0].device
+        for c in self.caches:
+            _require(c.dtype is torch.uint8 and tuple(c.shape) == shape and c.is_contiguous() and c.data_ptr() % 16 == 0 and c.device == self.device,
+                     "caches: uint8 [pages, hkv, bytes of a page and head], the same for every layer")
+        self.pages, self.hkv, self.k_bits, self.v_bits = shape[0], hkv, k_bits, v_bits
+        self.at = torch.tensor([c.data_ptr() for c in self.caches], dtype=torch.int64).to(self.device)
+
+
+def keep_tokens(caches: LayerCaches, page_table: torch.Tensor, request: torch.Tensor, start: torch.Tensor, accepted: torch.Tensor, path: torch.Tensor,
+                ws: Workspace | None = None) -> None:
+    """Move the keys and values of accepted nodes up behind their context, in all layers at once (``csrc/draft_tree.cu``).
+
+    Of request ``i`` the line at slot ``start[i] + path[i, k]`` moves to ``start[i] + k``, ``0 < k <= accepted[i]``; ``path`` rises from
+    0, as ``verify_tree`` leaves it.  ``request`` int32: rows of ``page_table``, none of them twice; the pages behind ``start`` are
+    the requests' own.  A path that does not rise and pages that are not there move nothing, and ``ws.check_status`` raises."""
+    n, i32 = request.numel(), torch.int32
+    ld, ldp = _rows(page_table, "page_table", i32), _rows(path, "path", i32)
+    _require(path.shape[0] >= n and path.shape[1] >= 1, "path: a row of at least one node for every request")
+    ws = ws or workspace(caches.device)
+    packed = native.KEEP_TOKENS.pack(
+        caches.at.data_ptr(), page_table.data_ptr(), _vector(request, i32, n, "request"), _vector(start, i32, n, "start"), _vector(accepted, i32, n, "accepted"), path.data_ptr(),
+        ws.status.data_ptr(), ld, ldp, n, len(caches.caches), caches.hkv, caches.pages, page_table.shape[0], page_table.shape[1], path.shape[1], caches.k_bits, caches.v_bits)
+    if n:
+        _call("cb_keep_tokens", (packed,), (caches.at, page_table, request, start, accepted, path, ws.status))
+
+
 # ------------------------------------------------------------------ mixture of experts
 class MoeScratch:
     """Fixed-address routing buffers for up to ``max_tokens`` tokens (graph-capturable)."""

@@ -332,9 +332,10 @@ def _declare(l: ctypes.CDLL) -> None:
     l.cb_canary_check.restype = i
     # what a step does for each of its requests: layout, adapters, draws from a whole vocabulary
     l.cb_adapter_rows.argtypes = [vp, i, i, vp, vp, vp, vp]
-    for name in ("step_layout", "adapter_add", "sample_vocabulary"):
+    # ... and of drafts in trees: their attention, the logits that requests want, the path that is kept
+    for name in ("step_layout", "adapter_add", "sample_vocabulary", "tree_attn", "adjust_logits", "verify_tree", "keep_tokens"):
         getattr(l, f"cb_{name}").argtypes = [vp, vp]
-    for name in ("step_layout", "adapter_rows", "adapter_add", "sample_vocabulary"):
+    for name in ("step_layout", "adapter_rows", "adapter_add", "sample_vocabulary", "tree_attn", "adjust_logits", "verify_tree", "keep_tokens"):
         getattr(l, f"cb_{name}").restype = i
     # layered decoders: fp32 residual stream, delta rule of any head size, latent attention
     l.cb_bf16_gemm_wide.argtypes = [vp, vp, ll, vp, vp, vp]
@@ -567,6 +568,10 @@ class ScoredMoeStruct(ctypes.Structure):
 STEP_LAYOUT = struct.Struct("@15P9i4x")                      # CbStepLayout, csrc/step_layout.cu
 ADAPTER = struct.Struct("@PqPqPq10P10i")                      # CbAdapter, csrc/adapters.cu
 VOCABULARY = struct.Struct("@PqPq11P4i")                     # CbVocabulary, csrc/sample_vocabulary.cu
+TREE_ATTN = struct.Struct("@10P4q10if4x")                    # CbTreeAttn, csrc/tree_attn.cu
+VERIFY_TREE = struct.Struct("@8P3i4x")                       # CbVerifyTree, csrc/draft_tree.cu
+KEEP_TOKENS = struct.Struct("@7P2q9i4x")                     # CbKeepTokens, csrc/draft_tree.cu
+ADJUST = struct.Struct("@16P5q8i")                           # CbAdjust, csrc/adjust_logits.cu
 
 
 class ReduceNormStruct(ctypes.Structure):

@@ -1,0 +1,116 @@
+"""Drafts in trees and what requests say about their tokens: the host's part, and what the operators refuse before anything reaches a GPU."""
+import numpy as np
+import pytest
+import torch
+
+from cubic_serve_b200.ops import kernels as K
+from cubic_serve_b200.runtime.trees import merge_drafts, tree_depths, tree_masks
+
+I32 = torch.int32
+
+
+def _ints(n, v=1):
+    return torch.full((n,), v, dtype=I32)
+
+
+def test_masks_and_depths_of_a_tree():
+    parents = [-1, 0, 0, 1, 1, 2, 5]
+    seen = [{0}, {0, 1}, {0, 2}, {0, 1, 3}, {0, 1, 4}, {0, 2, 5}, {0, 2, 5, 6}]
+    m = tree_masks(parents)
+    assert m.shape == (7, 1) and m.dtype == np.uint32
+    assert [{j for j in range(32) if r[0] >> np.uint32(j) & 1} for r in m] == seen
+    assert tree_depths(parents).tolist() == [len(s) - 1 for s in seen]
+    chain = tree_masks(list(range(-1, 69)))
+    assert chain.shape == (70, 3) and all(sum(int(w).bit_count() for w in r) == j + 1 for j, r in enumerate(chain))
+    assert tree_masks([-1], words=4).shape == (1, 4)
+
+
+@pytest.mark.parametrize("parents,words", [([-1, 1], None), ([-1, 0, 2], None), ([-1, -1], None), (list(range(-1, 40)), 1)])
+def test_masks_of_what_is_no_tree(parents, words):
+    with pytest.raises(ValueError):
+        tree_masks(parents, words)
+
+
+def test_drafts_meet_in_a_tree():
+    tokens, parents = merge_drafts([[5, 6, 7], [5, 8], [9], [5, 6, 7, 1]], 16)
+    assert tokens == [0, 5, 6, 7, 8, 9, 1] and parents == [-1, 0, 1, 2, 1, 0, 3]
+    assert merge_drafts([[5, 6, 7], [5, 8], [9]], 4) == ([0, 5, 6, 7, 8], [-1, 0, 1, 2, 1])
+    assert merge_drafts([], 4) == ([0], [-1]) and merge_drafts([[1, 2]], 0) == ([0], [-1])
+
+
+def _tree_args(**kw):
+    a = dict(q=torch.zeros(6, 512, dtype=torch.bfloat16), out=torch.zeros(6, 512, dtype=torch.bfloat16), cache=torch.zeros(4, 2, K.kv_blob_bytes(128, 8, 8), dtype=torch.uint8),
+             page_table=torch.zeros(3, 2, dtype=I32), request=_ints(2), row0=_ints(2), count=_ints(2), start=_ints(2), masks=torch.zeros(6, 1, dtype=I32), hq=4, hkv=2, head_dim=128,
+             k_bits=8, v_bits=8, ws=K.Workspace(torch.device("cpu"), 16, 16, 16))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=torch.zeros(6, 512)), dict(q=torch.zeros(6, 256, dtype=torch.bfloat16)), dict(out=torch.zeros(5, 512, dtype=torch.bfloat16)), dict(hq=3), dict(head_dim=64), dict(k_bits=5),
+    dict(cache=torch.zeros(4, 2, 100, dtype=torch.uint8)), dict(cache=torch.zeros(4, 4, K.kv_blob_bytes(128, 8, 8), dtype=torch.uint8)[:, ::2]), dict(page_table=torch.zeros(3, 2)),
+    dict(page_table=torch.zeros(3, 4, dtype=I32)[:, ::2]), dict(request=torch.ones(2)), dict(row0=_ints(1)), dict(count=_ints(4)[::2]), dict(start=torch.ones(2, dtype=torch.int64)),
+    dict(masks=torch.zeros(5, 1, dtype=I32)), dict(masks=torch.zeros(6, 9, dtype=I32)), dict(masks=torch.zeros(6, 0, dtype=I32)), dict(masks=torch.zeros(6, 1, dtype=torch.int64)),
+    dict(masks=torch.zeros(1, 1, dtype=I32).expand(6, 1)[:, :1].expand(6, 2)), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(hq=258, hkv=1),
+    dict(q=torch.zeros(6, 516, dtype=torch.bfloat16)[:, :512]), dict(q=torch.zeros(6 * 512 + 4, dtype=torch.bfloat16)[4:].view(6, 512)), dict(request=_ints(1025), row0=_ints(1025)), dict(),
+])
+def test_tree_attention_refuses(change):
+    with pytest.raises(ValueError):
+        K.tree_attention(**_tree_args(**change))
+
+
+def _adjust_args(**kw):
+    a = dict(logits=torch.zeros(4, 100), request=_ints(4), history=torch.zeros(2, 10, dtype=I32), length=_ints(2), prompt=_ints(2), repetition=torch.ones(2), frequency=torch.ones(2),
+             presence=torch.ones(2), bias=(_ints(3), _ints(5), torch.ones(5)), mask=torch.zeros(4, 4, dtype=I32), drafts=(_ints(4), torch.zeros(4, 1, dtype=I32), _ints(2)))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("change", [
+    dict(logits=torch.zeros(4, 100, dtype=torch.float16)), dict(logits=torch.zeros(4, 200)[:, ::2]), dict(logits=torch.zeros(1, 100).expand(4, 100)), dict(out=torch.zeros(4, 99)),
+    dict(out=torch.zeros(4, 100, dtype=torch.bfloat16)), dict(request=_ints(3)), dict(request=None), dict(history=torch.zeros(2, 10)), dict(length=_ints(1)), dict(prompt=_ints(1)),
+    dict(repetition=torch.ones(1)), dict(frequency=torch.ones(2, dtype=torch.float64)), dict(presence=torch.ones(4)[::2]), dict(bias=(_ints(2), _ints(5), torch.ones(5))),
+    dict(bias=(_ints(3), _ints(5), torch.ones(4))), dict(mask=torch.zeros(3, 4, dtype=I32)), dict(mask=torch.zeros(4, 3, dtype=I32)), dict(mask=torch.zeros(4, 4)),
+    dict(drafts=(_ints(3), torch.zeros(4, 1, dtype=I32), _ints(2))), dict(drafts=(_ints(4), torch.zeros(3, 1, dtype=I32), _ints(2))), dict(drafts=(_ints(4), torch.zeros(4, 9, dtype=I32), _ints(2))),
+    dict(drafts=(_ints(4), torch.zeros(4, 1, dtype=I32), _ints(1))), dict(),
+])
+def test_adjust_logits_refuses(change):
+    with pytest.raises(ValueError):
+        K.adjust_logits(**_adjust_args(**change))
+
+
+@pytest.mark.parametrize("change", [
+    dict(tokens=_ints(5)), dict(parents=torch.ones(6)), dict(row0=torch.ones(2)), dict(count=_ints(1)), dict(accepted=_ints(1)), dict(path=torch.zeros(1, 4, dtype=I32)),
+    dict(path=torch.zeros(2, 3, dtype=I32)), dict(path=torch.zeros(2, 8, dtype=I32)[:, ::2]), dict(emitted=torch.zeros(2, 4)), dict(path=torch.zeros(2, 0, dtype=I32), emitted=torch.zeros(2, 0, dtype=I32)), dict(),
+])
+def test_verify_tree_refuses(change):
+    a = dict(target_ids=_ints(6), tokens=_ints(6), parents=_ints(6), row0=_ints(2), count=_ints(2), accepted=_ints(2), path=torch.zeros(2, 4, dtype=I32), emitted=torch.zeros(2, 4, dtype=I32))
+    a.update(change)
+    with pytest.raises(ValueError):
+        K.verify_tree(**a)
+
+
+def _caches(shapes, **kw):
+    a = dict(hkv=2, head_dim=128, k_bits=8, v_bits=8)
+    a.update(kw)
+    return K.LayerCaches([torch.zeros(*s, dtype=torch.uint8) for s in shapes], **a)
+
+
+@pytest.mark.parametrize("shapes,kw", [([(4, 2, 4608), (5, 2, 4608)], {}), ([(4, 2, 4608)], dict(hkv=1)), ([(4, 2, 4608)], dict(k_bits=4)), ([(4, 2, 4608)], dict(v_bits=7)),
+                                       ([(4, 2, 4608)], dict(head_dim=64)), ([(0, 2, 4608)], {}), ([], {})])
+def test_layer_caches_refuse(shapes, kw):
+    with pytest.raises(ValueError):
+        _caches(shapes, **kw)
+
+
+@pytest.mark.parametrize("change", [
+    dict(page_table=torch.zeros(3, 2)), dict(request=torch.ones(2)), dict(start=_ints(1)), dict(accepted=_ints(1)), dict(path=torch.zeros(1, 4, dtype=I32)), dict(path=torch.zeros(2, 4)), dict(),
+])
+def test_keep_tokens_refuses(change):
+    caches = _caches([(4, 2, 4608), (0, 2, 4608), (4, 2, 4608)])
+    assert len(caches.caches) == 2
+    a = dict(caches=caches, page_table=torch.zeros(3, 2, dtype=I32), request=_ints(2), start=_ints(2), accepted=_ints(2), path=torch.zeros(2, 4, dtype=I32),
+             ws=K.Workspace(torch.device("cpu"), 16, 16, 16))
+    a.update(change)
+    with pytest.raises(ValueError):
+        K.keep_tokens(**a)
