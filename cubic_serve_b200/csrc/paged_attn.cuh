@@ -85,6 +85,45 @@ __device__ __forceinline__ uint32_t pf_codes_v(const uint8_t* v, int tok, int la
   return x;
 }
 
+// Shared-memory descriptor of an operand whose rows of 128 bytes run along N (or M), 128-byte swizzle: 8 rows of K are 1024 bytes, blocks of 64 columns
+// `block` bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_sw128_n(uint32_t smem_addr, uint32_t block) {
+  return (umma_desc_sw128(smem_addr) & ~(static_cast<uint64_t>(0x3FFF) << 16)) | static_cast<uint64_t>(block >> 4) << 16;
+}
+__device__ __forceinline__ float pow2f(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
+
+__device__ __forceinline__ uint4 conv8(uint2 w, uint32_t bias) {        // eight codes in order -> eight f16
+  return make_uint4(u8x2_to_f16x2(w.x, 0x5140u, bias), u8x2_to_f16x2(w.x, 0x5342u, bias), u8x2_to_f16x2(w.y, 0x5140u, bias), u8x2_to_f16x2(w.y, 0x5342u, bias));
+}
+
+// an fp32 scale as a pair of f16, each twice
+__device__ __forceinline__ void pf_split(float s, uint32_t& sh, uint32_t& sl) {
+  sh = pack_f16x2(s, s);
+  const float r = s - __low2float(*reinterpret_cast<const __half2*>(&sh));
+  sl = pack_f16x2(r, r);
+}
+
+// The largest magnitude of a token's scales, as bits; FINITE: of those that are
+template <bool FINITE>
+__device__ __forceinline__ uint32_t pf_most(const float4& s) {
+  auto magnitude = [](float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
+    return !FINITE || b < 0x7F800000u ? b : 0u;
+  };
+  return max(max(magnitude(s.x), magnitude(s.y)), max(magnitude(s.z), magnitude(s.w)));
+}
+__device__ __forceinline__ int pf_exponent(uint32_t magnitude) { return max(static_cast<int>(magnitude >> 23) - 127, -100); }
+
+// The scales of a step's tokens `lane` and `lane` + 32, zeros from `visible` on
+__device__ __forceinline__ void pf_scales(const uint8_t* scales, int stride, int visible, int lane, float4 (&of)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int tok = lane + 32 * h;
+    of[h] = *reinterpret_cast<const float4*>(scales + (tok >> 4) * stride + (tok & 15) * 16);
+    if (tok >= visible) of[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+}
+
 struct WarpState {
   float m[2];       // running max (log2 domain) for rows g and g+8
   float l[2];       // running partial sum (this lane's columns only)

@@ -79,13 +79,6 @@ struct __align__(1024) PfSmem {
   uint32_t tmem, abort_word;
 };
 
-// Shared-memory descriptor of an operand whose rows of 128 bytes run along N (or M), 128-byte swizzle: 8 rows of K are 1024 bytes, blocks of 64 columns
-// `block` bytes apart.
-__device__ __forceinline__ uint64_t umma_desc_sw128_n(uint32_t smem_addr, uint32_t block) {
-  return (umma_desc_sw128(smem_addr) & ~(static_cast<uint64_t>(0x3FFF) << 16)) | static_cast<uint64_t>(block >> 4) << 16;
-}
-__device__ __forceinline__ float pow2f(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
-
 // Where a role stands in an item's list of steps: runs one after the other.
 struct PfWalk {
   int run = 0, step = 0;
@@ -93,10 +86,6 @@ struct PfWalk {
     if (++step == l.run[run].steps) { step = 0; ++run; }
   }
 };
-
-__device__ __forceinline__ uint4 conv8(uint2 w, uint32_t bias) {        // eight codes in order -> eight f16
-  return make_uint4(u8x2_to_f16x2(w.x, 0x5140u, bias), u8x2_to_f16x2(w.x, 0x5342u, bias), u8x2_to_f16x2(w.y, 0x5140u, bias), u8x2_to_f16x2(w.y, 0x5342u, bias));
-}
 
 // Two codes times their scales sh + sl: the rounded product with sh, and what it left over with the product with sl.  The residual is exact (a code
 // has 8 bits, sh 11), so hi + lo is off by the rounding of sl and of lo: 2^-22 of the value.
@@ -113,34 +102,6 @@ __device__ __forceinline__ void pf_scaled8(const uint4& c, uint32_t sh, uint32_t
   pf_scaled(c.z, sh, sl, hi.z, lo.z);
   pf_scaled(c.w, sh, sl, hi.w, lo.w);
 }
-// an fp32 scale as a pair of f16, each twice
-__device__ __forceinline__ void pf_split(float s, uint32_t& sh, uint32_t& sl) {
-  sh = pack_f16x2(s, s);
-  const float r = s - __low2float(*reinterpret_cast<const __half2*>(&sh));
-  sl = pack_f16x2(r, r);
-}
-
-// The largest magnitude of a token's scales, as bits; FINITE: of those that are
-template <bool FINITE>
-__device__ __forceinline__ uint32_t pf_most(const float4& s) {
-  auto magnitude = [](float x) {
-    const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
-    return !FINITE || b < 0x7F800000u ? b : 0u;
-  };
-  return max(max(magnitude(s.x), magnitude(s.y)), max(magnitude(s.z), magnitude(s.w)));
-}
-__device__ __forceinline__ int pf_exponent(uint32_t magnitude) { return max(static_cast<int>(magnitude >> 23) - 127, -100); }
-
-// The scales of a step's tokens `lane` and `lane` + 32, zeros from `visible` on
-__device__ __forceinline__ void pf_scales(const uint8_t* scales, int stride, int visible, int lane, float4 (&of)[2]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int tok = lane + 32 * h;
-    of[h] = *reinterpret_cast<const float4*>(scales + (tok >> 4) * stride + (tok & 15) * 16);
-    if (tok >= visible) of[h] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-}
-
 // One step's codes into operands: all of a thread's loads, then its arithmetic (few warps hide nothing).
 // What K holds of tokens that no row sees is masked with their scores.
 template <int KBITS>

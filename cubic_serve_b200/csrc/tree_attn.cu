@@ -18,6 +18,7 @@ struct CbTreeAttn {
   const int* start;          // [n] tokens of the context
   const uint32_t* masks;     // [rows, words], row stride ldm
   uint32_t* status;
+  float* partial;            // cb_tree_attn_floats of them
   long long ldq, ldo, ld, ldm;
   int n, rows, table_rows, width, pages, words;
   int Hq, Hkv, k_bits, v_bits;
@@ -94,32 +95,777 @@ __device__ __forceinline__ void tree_row(const CbTreeAttn& p, const KvLayout& la
   }
 }
 
+// ------------------------------------------------------------------------------------------------- schedule
+// An item is up to 256 rows (node x query head of the group) of a request and key / value head, in steps of 64 tokens.  The steps of all items, one after the
+// other, are dealt out evenly: CTA c takes the steps [c per, (c + 1) per), however uneven the requests are.  An item that several CTAs share leaves a part (its
+// maximum, sum and unnormalised output) of each in the workspace, and tree_merge_kernel joins them in order: no atomics, the same bits every time.
+static constexpr int kTrTiles = 2, kTrRows = 128, kTrItemRows = kTrTiles * kTrRows;
+static constexpr int kTrPages = 4, kTrTok = kTrPages * kPageTokens;
+static constexpr int kTrThreads = 640;
+static constexpr int kTrRegs = 96, kTrRegsSoftmax = 136, kTrRegsConvert = 72, kTrRegsOther = 64;
+static_assert(2 * kTrRegsSoftmax + 2 * kTrRegsConvert + kTrRegsOther <= 5 * kTrRegs, "five warpgroups");
+static constexpr int kTrLists = 4, kTrRaw = 4;
+static constexpr int kTrNotes = kTrRaw + 2;
+static constexpr int kTrLeast = 1;                       // steps of a CTA, at least
+static constexpr float kTrGrowth = 2.f;
+static constexpr int kTrApartK = 18, kTrApartV = 14;
+static constexpr int kTrHalf = kTrTok * 128;             // bytes of 64 channels of a step
+static constexpr uint32_t kTrTmemCols = 512, kTrTmemTile = 256, kTrTmemP = 64, kTrTmemQ = 96, kTrTmemO = 128;
+
+struct TrItem {
+  int kvh;                                               // < 0: no more items
+  int slot, row0, count, start, total;                   // the request
+  int first, rows;                                       // rows [first, first + rows) of its count x group
+  int lo, steps;                                         // steps [lo, lo + steps) of this CTA; none: zeros
+  int part;                                              // place of its part, -1: the whole item
+};
+struct TrDesc { int parts, row0, first, rows, kvh, pad[3]; };
+struct __align__(1024) TrSmem {
+  uint8_t q[kTrTiles][kTrRows * 128];                    // f16, channels 64..127: [row][128 B], 16-byte chunk ^ (row & 7)
+  uint8_t k[2][2 * kTrHalf];                             // f16 [stage][64-channel half][token][128 B]
+  uint8_t v[2][2 * kTrHalf];                             // likewise
+  float k_mul[kTrNotes];                                 // scores are this times what the MMAs give
+  int v_exp[kTrNotes];                                   // output is 2^v_exp times ...
+  uint32_t redo[kTrLists];                               // of an item's steps: some values are beyond what f16 operands hold
+  uint64_t raw_full[kTrRaw], raw_free[kTrRaw], k_full[2], k_free[2], v_full[2], v_free[2], k_note[kTrNotes], v_note[kTrNotes];
+  uint64_t list_full[kTrLists], list_free[kTrLists], q_full[kTrTiles], s_full[kTrTiles], s_free[kTrTiles], p_full[kTrTiles], pv_done[kTrTiles];
+  TrItem list[kTrLists];
+  long long sums[kTrThreads / 32];
+  uint32_t tmem, abort_word;
+  long long upto[kTreeMaxRequests + 1];                  // steps of the requests before
+};
+
+__device__ __forceinline__ int tr_steps(const TreeRequest& r) { return max(1, (r.total + kTrTok - 1) / kTrTok); }
+__device__ __forceinline__ int tr_groups(const TreeRequest& r, int G) { return (r.count * G + kTrItemRows - 1) / kTrItemRows; }
+static inline int tr_rows(int words, int rows, int G) {
+  const long long most = static_cast<long long>(words * 32 < rows ? words * 32 : rows) * G;
+  return most < kTrItemRows ? static_cast<int>(most) : kTrItemRows;
+}
+
+// One step's codes into operands.  A code times its scale sh + sl (f16 each): the product with sl, rounded, is 2^-11 of the whole, so that the
+// multiply-add behind it rounds once what 32-bit arithmetic would.  What K holds of tokens that no row sees is masked with their scores.
+__device__ __forceinline__ uint32_t tr_scaled(uint32_t code, uint32_t sh, uint32_t sl) {
+  uint32_t t, r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(t) : "r"(code), "r"(sl));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(code), "r"(sh), "r"(t));
+  return r;
+}
+__device__ __forceinline__ uint4 tr_scaled8(const uint4& c, uint32_t sh, uint32_t sl) {
+  return make_uint4(tr_scaled(c.x, sh, sl), tr_scaled(c.y, sh, sl), tr_scaled(c.z, sh, sl), tr_scaled(c.w, sh, sl));
+}
+template <int KBITS>
+__device__ __forceinline__ void tr_convert_k(uint8_t (&k)[2 * kTrHalf], const uint8_t* raw, int stride, const KvLayout& lay, float mul, int tid) {
+  constexpr uint32_t kb = KBITS == 8 ? 0x64806480u : KBITS == 6 ? 0x64206420u : 0x64086408u;
+  constexpr int kItems = KBITS == 8 ? kPageTokens * 8 : kPageTokens * 4, kMine = kTrPages * kItems / 128;
+  uint4 x[kMine], xh[kMine];
+  float s[kMine];
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {
+    const int i = tid + j * 128, r = i % kItems, tok = r & 15, blk = r >> 4;
+    const uint8_t* src = raw + i / kItems * stride;
+    x[j] = *reinterpret_cast<const uint4*>(src + blk * 256 + tok * 16);
+    if constexpr (KBITS == 6) xh[j] = *reinterpret_cast<const uint4*>(src + kPageTokens * kD / 2 + blk * 128 + (tok & 7) * 16);
+    s[j] = *reinterpret_cast<const float*>(src + lay.k_scale_off + tok * 16 + (KBITS == 8 ? blk >> 1 : blk) * 4);
+  }
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {
+    const int i = tid + j * 128, r = i % kItems, tok = r & 15, blk = r >> 4, sw = tok & 7;
+    uint4* row = reinterpret_cast<uint4*>(k + (KBITS == 8 ? blk >> 2 : blk >> 1) * kTrHalf + (i / kItems * 16 + tok) * 128);
+    const int c = KBITS == 8 ? (blk & 3) * 2 : (blk & 1) * 4;
+    uint32_t sh, sl;
+    pf_split(s[j] * mul, sh, sl);
+    auto put = [&](int chunk, uint2 codes) { row[chunk ^ sw] = tr_scaled8(conv8(codes, kb), sh, sl); };
+    if constexpr (KBITS == 8) {
+      put(c, make_uint2(x[j].x, x[j].y));
+      put(c + 1, make_uint2(x[j].z, x[j].w));
+    } else {
+      const uint32_t n[4] = {x[j].x, x[j].y, x[j].z, x[j].w}, hw[4] = {xh[j].x, xh[j].y, xh[j].z, xh[j].w};
+      uint32_t lo[4], hi[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        lo[q] = n[q] & 0x0F0F0F0Fu;
+        hi[q] = (n[q] >> 4) & 0x0F0F0F0Fu;
+        if constexpr (KBITS == 6) {
+          lo[q] |= (tok < 8 ? hw[q] : hw[q] << 4) & 0x30303030u;
+          hi[q] |= (tok < 8 ? hw[q] >> 2 : hw[q] << 2) & 0x30303030u;
+        }
+      }
+      put(c, make_uint2(lo[0], lo[1]));
+      put(c + 1, make_uint2(lo[2], lo[3]));
+      put(c + 2, make_uint2(hi[0], hi[1]));
+      put(c + 3, make_uint2(hi[2], hi[3]));
+    }
+  }
+}
+// V from `visible` on becomes zeros: those slots may hold anything, and a probability of zero has to stay zero.
+template <int VBITS>
+__device__ __forceinline__ void tr_convert_v(uint8_t (&v)[2 * kTrHalf], const uint8_t* raw, int stride, const KvLayout& lay, int visible, float mul, int tid) {
+  constexpr uint32_t vb = VBITS == 8 ? 0x64806480u : VBITS == 6 ? 0x64206420u : 0x64086408u;
+  // an item is 8 channels of a token pair of a page
+  const int c = tid & 15, pair = tid >> 4, at = (2 * c) ^ ((pair & 3) << 2);
+  uint4 x[kTrPages];                                     // 8 bit: the codes; else low nibbles, high bits
+  float s[kTrPages][2];
+#pragma unroll
+  for (int j = 0; j < kTrPages; ++j) {
+    const uint8_t* page = raw + j * stride;
+    const uint8_t* src = page + lay.v_code_off;
+    if constexpr (VBITS == 8) {
+      x[j] = *reinterpret_cast<const uint4*>(src + pair * 256 + at * 8);
+    } else {
+      const uint2 n = *reinterpret_cast<const uint2*>(src + pair * 128 + at * 4);
+      uint2 hw = make_uint2(0u, 0u);
+      if constexpr (VBITS == 6) hw = *reinterpret_cast<const uint2*>(src + kPageTokens * kD / 2 + (pair & 3) * 128 + at * 4);
+      x[j] = make_uint4(n.x, n.y, hw.x, hw.y);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) s[j][h] = *reinterpret_cast<const float*>(page + lay.v_scale_off + (2 * pair + h) * 16 + (c >> 2) * 4);
+  }
+#pragma unroll
+  for (int j = 0; j < kTrPages; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int tok = (j * 8 + pair) * 2 + h;
+      uint4 codes;
+      if constexpr (VBITS == 8) {
+        const uint32_t sel = h ? 0x5341u : 0x5240u;
+        codes = make_uint4(u8x2_to_f16x2(x[j].x, sel, vb), u8x2_to_f16x2(x[j].y, sel, vb), u8x2_to_f16x2(x[j].z, sel, vb), u8x2_to_f16x2(x[j].w, sel, vb));
+      } else {
+        uint2 n = h ? make_uint2((x[j].x >> 4) & 0x0F0F0F0Fu, (x[j].y >> 4) & 0x0F0F0F0Fu) : make_uint2(x[j].x & 0x0F0F0F0Fu, x[j].y & 0x0F0F0F0Fu);
+        if constexpr (VBITS == 6) {
+          auto high = [&](uint32_t w) { return (pair < 4 ? (h ? w >> 2 : w) : (h ? w << 2 : w << 4)) & 0x30303030u; };
+          n.x |= high(x[j].z);
+          n.y |= high(x[j].w);
+        }
+        codes = conv8(n, vb);
+      }
+      float f = s[j][h] * mul;
+      if (tok >= visible || !(fabsf(f) < INFINITY)) f = 0.f;
+      uint32_t sh, sl;
+      pf_split(f, sh, sl);
+      *reinterpret_cast<uint4*>(v + (c >> 3) * kTrHalf + tok * 128 + (((c & 7) ^ (tok & 7)) << 4)) = tr_scaled8(codes, sh, sl);
+    }
+}
+// The smallest magnitude of a token's scales that is not zero, as bits
+__device__ __forceinline__ uint32_t tr_least(const float4& s) {
+  auto magnitude = [](float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
+    return b == 0u ? 0x7F800000u : b;
+  };
+  return min(min(magnitude(s.x), magnitude(s.y)), min(magnitude(s.z), magnitude(s.w)));
+}
+
+// 64 bits: which of the tokens [tok0, tok0 + 64) a row sees.  `sees`: its words.
+__device__ __forceinline__ uint2 tr_visible(const uint32_t* sees, int words, int start, int total, int tok0) {
+  auto word = [&](int k) { return k >= 0 && k < words ? sees[k] : 0u; };
+  const int j0 = tok0 - start, w = j0 >> 5, b = j0 & 31;               // (rounded down: the bits before node 0 are the context's)
+  const uint32_t w0 = word(w), w1 = word(w + 1), w2 = word(w + 2);
+  uint2 m = make_uint2(__funnelshift_r(w0, w1, b), __funnelshift_r(w1, w2, b));
+  if (j0 < 0) {
+    m.x |= -j0 >= 32 ? ~0u : (1u << -j0) - 1u;
+    if (j0 < -32) m.y |= -j0 >= 64 ? ~0u : (1u << (-j0 - 32)) - 1u;
+  }
+  const int n = total - tok0;
+  if (n < 64) m.y &= n <= 32 ? 0u : (1u << (n - 32)) - 1u;
+  if (n < 32) m.x &= (1u << max(n, 0)) - 1u;
+  return m;
+}
+
+// Roles: warps 0-7 own a row a thread (softmax needs no exchange: tensor-memory lane = row); warps 8-11 convert raw pages of K to the swizzled operand
+// ([token][channel], f16), warps 12-15 those of V; warps 16 and 18 issue the MMAs of the scores and of the output; warp 17 makes the items and copies pages.
+// Tensor memory of a tile of 128 rows: scores, probabilities (the A operand of their product), output and the first half of Q's channels; the other half of
+// Q is in shared memory.  The scores of step i + 1 are computed while the softmax of step i runs.  The output is rescaled only when a row's maximum has grown by more
+// than a factor of four: until then probabilities relative to the older maximum are at most 4.
+// Powers of two keep operands in the range of f16: a row's for Q (undone with the softmax' scale: its 8 bits stay exact), a step's for K (likewise), one for V that grows
+// with the largest scale (undone with the output).  A request whose scales are further apart than that holds (2^18 in a step of K, 2^14 in a CTA's steps of V), or not finite,
+// is computed in fp32 (tree_row): a hundred times as long, for caches as no model has them.
+// Every wait is bounded; on a timeout the roles leave, the status word is set and tensor memory is freed.
 template <int KBITS, int VBITS>
-__global__ void __launch_bounds__(256)
-tree_simple_kernel(const CbTreeAttn p, const KvLayout lay) {
+__global__ void __launch_bounds__(kTrThreads, 1)
+tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  TrSmem& sm = *reinterpret_cast<TrSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* raw = reinterpret_cast<uint8_t*>(&sm + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv;
+  const int stride = (lay.blob_bytes + 127) & ~127;
+  volatile uint32_t* abort_flag = &sm.abort_word;
+  float* part_o = p.partial;
+  float2* part_ml = reinterpret_cast<float2*>(part_o + static_cast<size_t>(gridDim.x) * 2 * part_rows * kD);
+  TrDesc* desc = reinterpret_cast<TrDesc*>(part_ml + static_cast<size_t>(gridDim.x) * 2 * part_rows);
+  if (tid == 0) {
+    for (int b = 0; b < kTrRaw; ++b) {
+      mbar_init(smem_u32(&sm.raw_full[b]), 1);
+      mbar_init(smem_u32(&sm.raw_free[b]), 8);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&sm.k_full[b]), 4);
+      mbar_init(smem_u32(&sm.k_free[b]), 1);
+      mbar_init(smem_u32(&sm.v_full[b]), 4);
+      mbar_init(smem_u32(&sm.v_free[b]), 1);
+    }
+    for (int b = 0; b < kTrNotes; ++b) {
+      mbar_init(smem_u32(&sm.k_note[b]), 1);
+      mbar_init(smem_u32(&sm.v_note[b]), 1);
+    }
+    for (int b = 0; b < kTrLists; ++b) {
+      mbar_init(smem_u32(&sm.list_full[b]), 1);
+      mbar_init(smem_u32(&sm.list_free[b]), 18);         // all warps but 17 and 19
+    }
+    for (int t = 0; t < kTrTiles; ++t) {
+      mbar_init(smem_u32(&sm.q_full[t]), 4);
+      mbar_init(smem_u32(&sm.s_full[t]), 1);
+      mbar_init(smem_u32(&sm.s_free[t]), 4);
+      mbar_init(smem_u32(&sm.p_full[t]), 4);
+      mbar_init(smem_u32(&sm.pv_done[t]), 1);
+    }
+    sm.abort_word = 0;
+    mbar_fence_init();
+  }
+  if (warp == 16) {
+    tmem_alloc(smem_u32(&sm.tmem), kTrTmemCols);
+    tmem_relinquish();
+  }
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, kvh = blockIdx.y, G = p.Hq / p.Hkv;
   bool bad = false;
-  const TreeRequest r = tree_request(p, blockIdx.x, bad);
-  for (int row = blockIdx.z * 8 + (threadIdx.x >> 5); row < r.count * G; row += gridDim.z * 8) {
-    const int node = row / G, at = (kvh * G + row - node * G) * kD;
-    float m, sum, o[4];
-    tree_row<KBITS, VBITS>(p, lay, r, kvh, 0, r.total, p.masks + (r.row0 + node) * p.ldm, p.q + (r.row0 + node) * p.ldq + at, lane, m, sum, o, bad);
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;                  // NaN stays
-    reinterpret_cast<uint2*>(p.out + (r.row0 + node) * p.ldo + at)[lane] = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+  {
+    // steps of all requests, summed; two neighbouring requests a thread
+    long long mine[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (2 * tid + j < p.n) {
+        const TreeRequest r = tree_request(p, 2 * tid + j, bad);
+        mine[j] = static_cast<long long>(tr_steps(r)) * tr_groups(r, G) * p.Hkv;
+      }
+    long long v = mine[0] + mine[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) sm.sums[warp] = v;
+    __syncthreads();
+    long long before = v - mine[0] - mine[1];
+    for (int w = 0; w < warp; ++w) before += sm.sums[w];
+    if (tid == 0) sm.upto[0] = 0;
+    if (2 * tid < p.n) sm.upto[2 * tid + 1] = before + mine[0];
+    if (2 * tid + 1 < p.n) sm.upto[2 * tid + 2] = before + mine[0] + mine[1];
   }
-  if (bad && lane == 0) atomicExch(p.status, static_cast<uint32_t>(kErrBadArgument));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  const long long all = sm.upto[p.n], per = max(static_cast<long long>(kTrLeast), (all + gridDim.x - 1) / gridDim.x);
+  bool ok = true;
+
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTrRegsOther));
+    if (warp == 17) {
+      // ------------------------------------------------------- items and pages
+      long long u = min(all, per * blockIdx.x);
+      const long long end = min(all, u + per);
+      int i = 0, gs = 0;
+      TreeRequest r = {0, 0, 0, 0, 0};
+      if (u < end) {                                     // the request of the first step
+        int hi = p.n;
+        while (hi - i > 1) {
+          const int mid = (i + hi) >> 1;
+          if (sm.upto[mid] <= u) i = mid; else hi = mid;
+        }
+        r = tree_request(p, i, bad);
+      }
+      TrDesc d = {};
+      int ids_next = 0;                                  // pages of the item made last, 32 from its first on
+      auto ids_of = [&](const TrItem& l, int step) {
+        const int at = (l.lo + step) * kTrPages + lane, pages = (l.total + kPageTokens - 1) / kPageTokens;
+        return at < pages ? tree_page(p, l.slot, at, bad) : 0;
+      };
+      auto publish = [&](int n) {                        // the CTA's n-th item; false: there is none
+        TrItem& to = sm.list[n % kTrLists];
+        if (ok && n >= kTrLists) ok = mbar_wait_park(smem_u32(&sm.list_free[n % kTrLists]), (n / kTrLists - 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return false;
+        TrItem l;
+        l.kvh = -1;
+        if (u < end) {
+          while (u >= sm.upto[i + 1]) {
+            ++i;
+            if (u < sm.upto[i + 1]) r = tree_request(p, i, bad);
+          }
+          const int S = tr_steps(r), groups = tr_groups(r, G);
+          const long long off = u - sm.upto[i];
+          const int k = static_cast<int>(off / S), s = static_cast<int>(off - static_cast<long long>(k) * S);
+          const int n_steps = static_cast<int>(min(static_cast<long long>(S - s), end - u));
+          l.kvh = k / groups;
+          l.slot = r.slot; l.row0 = r.row0; l.count = r.count; l.start = r.start; l.total = r.total;
+          l.first = (k - l.kvh * groups) * kTrItemRows;
+          l.rows = min(kTrItemRows, r.count * G - l.first);
+          l.lo = s;
+          l.steps = r.total > 0 ? n_steps : 0;
+          l.part = n_steps == S ? -1 : 2 * static_cast<int>(blockIdx.x) + (s == 0);
+          if (l.part >= 0 && s == 0) {
+            d.parts = static_cast<int>((u + S - 1) / per) - static_cast<int>(blockIdx.x) + 1;
+            d.row0 = l.row0; d.first = l.first; d.rows = l.rows; d.kvh = l.kvh;
+          }
+          u += n_steps;
+        }
+        if (lane == 0) {
+          to = l;
+          sm.redo[n % kTrLists] = 0;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.list_full[n % kTrLists]));
+        if (l.kvh >= 0) ids_next = ids_of(l, 0);
+        return l.kvh >= 0;
+      };
+      bool more = publish(0);
+      for (int it = 0; more && ok; ++it) {
+        const TrItem l = sm.list[it % kTrLists];
+        const int pages = (l.total + kPageTokens - 1) / kPageTokens;
+        bool next = false;
+        int ids = ids_next, ids_later = 0;
+        for (int s = 0; s < l.steps; ++s, ++gs) {
+          if (s > 0 && s % 8 == 0) ids = ids_later;
+          const int b = gs % kTrRaw;
+          if (ok && gs >= kTrRaw) ok = mbar_wait_park(smem_u32(&sm.raw_free[b]), (gs / kTrRaw - 1) & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int n = min(kTrPages, pages - (l.lo + s) * kTrPages);
+          if (lane == 0) mbar_expect_tx(smem_u32(&sm.raw_full[b]), n * lay.blob_bytes);
+          __syncwarp();
+          const int page = __shfl_sync(0xffffffffu, ids, (s % 8) * kTrPages + (lane & 3));
+          if (lane < n)
+            bulk_g2s(smem_u32(raw + (b * kTrPages + lane) * stride), p.cache + (static_cast<size_t>(page) * p.Hkv + l.kvh) * lay.blob_bytes, lay.blob_bytes, smem_u32(&sm.raw_full[b]));
+          if (s % 8 == 0 && s + 8 < l.steps) ids_later = ids_of(l, s + 8);
+          if (s == min(1, l.steps - 1)) next = publish(it + 1);
+        }
+        if (l.steps == 0) next = publish(it + 1);
+        more = next;
+      }
+      if (lane == 0) desc[blockIdx.x] = d;
+      if (*abort_flag) {                                 // copies in flight land (for a bounded time) before the CTA goes
+        const long long t0 = clock64();
+        for (int g = max(0, gs - kTrRaw); g < gs; ++g)
+          while (!mbar_try_wait(smem_u32(&sm.raw_full[g % kTrRaw]), (g / kTrRaw) & 1) && clock64() - t0 < kWaitBudgetCycles / 8) {
+          }
+      }
+    } else if (warp != 19) {
+      // ---------------------------------------------------------------- MMAs
+      const bool leader = elect_one(), is_s = warp == 16;
+      const uint32_t idesc_s = umma_idesc(kTrRows, kTrTok, 0u, 0u), idesc_o = umma_idesc(kTrRows, kD, 0u, 0u) | 1u << 16;      // V: channels are contiguous
+      const uint64_t dq = umma_desc_sw128(smem_u32(sm.q[0])), dk = umma_desc_sw128(smem_u32(sm.k[0])), dv = umma_desc_sw128_n(smem_u32(sm.v[0]), kTrHalf);
+      int gs = 0;                                        // steps of earlier items
+      int n[kTrTiles] = {0, 0};                          // steps per tile
+      uint32_t q_phase = 0;                              // bit = tile
+      for (int it = 0;; ++it) {
+        const TrItem& l = sm.list[it % kTrLists];
+        if (ok) ok = mbar_wait_park(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok || l.kvh < 0) break;
+        const int steps = l.steps, tiles = l.rows > kTrRows ? 2 : 1;
+        for (int s = 0; s < steps; ++s, ++gs) {
+          const int b = gs & 1;
+          if (ok) ok = mbar_wait_park(smem_u32(is_s ? &sm.k_full[b] : &sm.v_full[b]), (gs >> 1) & 1, abort_flag);
+#pragma unroll
+          for (int t = 0; t < kTrTiles; ++t) {
+            if (t >= tiles) continue;
+            const uint32_t tile = tmem + t * kTrTmemTile;
+            if (is_s) {
+              if (s == 0) {
+                if (ok) ok = mbar_wait_park(smem_u32(&sm.q_full[t]), q_phase >> t & 1, abort_flag);
+                q_phase ^= 1u << t;
+              }
+              if (ok && n[t] > 0) ok = mbar_wait_park(smem_u32(&sm.s_free[t]), (n[t] - 1) & 1, abort_flag);
+            } else {
+              if (ok) ok = mbar_wait_park(smem_u32(&sm.p_full[t]), n[t] & 1, abort_flag);
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            ++n[t];
+            tc_fence_after();
+            if (ok && leader) {
+              if (is_s) {
+                const uint64_t k0 = dk + (b * (2 * kTrHalf) >> 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) umma_f16_ts(tile, tile + kTrTmemQ + k * 8, k0 + k * 2, idesc_s, k > 0);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) umma_f16(tile, dq + (t * (kTrRows * 128) >> 4) + k * 2, k0 + (kTrHalf >> 4) + k * 2, idesc_s, 1);
+                tc_commit(smem_u32(&sm.s_full[t]));
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  umma_f16_ts(tile + kTrTmemO, tile + kTrTmemP + k * 8, dv + (b * (2 * kTrHalf) >> 4) + k * (16 * 128 >> 4), idesc_o, s > 0 || k > 0);
+                tc_commit(smem_u32(&sm.pv_done[t]));
+              }
+            }
+            __syncwarp();
+          }
+          if (ok && leader) tc_commit(smem_u32(is_s ? &sm.k_free[b] : &sm.v_free[b]));
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(smem_u32(&sm.list_free[it % kTrLists]));
+      }
+    }
+  } else if (warp >= 8) {
+    // ------------------------------------------------------------ conversion
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTrRegsConvert));
+    const bool is_v = warp >= 12;
+    const int ct = tid & 127;
+    int gs = 0;
+    for (int it = 0;; ++it) {
+      const TrItem& l = sm.list[it % kTrLists];
+      if (ok) ok = mbar_wait_park(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok || l.kvh < 0) break;
+      const int steps = l.steps;
+      int v_exp = 0;
+      uint32_t v_most = 0, v_least = 0x7F800000u;        // of the item's steps
+      for (int s = 0; s < steps; ++s, ++gs) {
+        const int b = gs & 1, slot = gs % kTrRaw, note = gs % kTrNotes, visible = l.total - (l.lo + s) * kTrTok;
+        if (ok) ok = mbar_wait_park(smem_u32(&sm.raw_full[slot]), (gs / kTrRaw) & 1, abort_flag);
+        if (ok && gs >= 2) ok = mbar_wait_park(smem_u32(is_v ? &sm.v_free[b] : &sm.k_free[b]), ((gs >> 1) - 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint8_t* pages = raw + slot * kTrPages * stride;
+        float4 scale[2];
+        pf_scales(pages + (is_v ? lay.v_scale_off : lay.k_scale_off), stride, visible, lane, scale);
+        uint32_t most = __reduce_max_sync(0xffffffffu, max(pf_most<false>(scale[0]), pf_most<false>(scale[1])));       // (every warp for itself)
+        const bool odd = most >= 0x7F800000u;                            // some are not finite
+        if (odd) most = __reduce_max_sync(0xffffffffu, max(pf_most<true>(scale[0]), pf_most<true>(scale[1])));
+        const int e = pf_exponent(most);
+        uint32_t least = 0x7F800000u;
+        if ((warp & 3) == 0) least = __reduce_min_sync(0xffffffffu, min(tr_least(scale[0]), tr_least(scale[1])));
+        if (!is_v) {
+          // codes times scales below 2^13
+          if (warp == 8 && lane == 0) {
+            if (odd || (least < 0x7F800000u && pf_exponent(least) < e - kTrApartK)) sm.redo[it % kTrLists] = 1;
+            sm.k_mul[note] = pow2f(e - 5);
+            mbar_arrive(smem_u32(&sm.k_note[note]));
+          }
+          tr_convert_k<KBITS>(sm.k[b], pages, stride, lay, pow2f(5 - e), ct);
+        } else {
+          // below 2^11, to be changed when they pass 2^15
+          if (s == 0 || e - 7 > v_exp) v_exp = e - 3;
+          if (warp == 12 && lane == 0) {
+            v_most = max(v_most, most);
+            v_least = min(v_least, least);
+            if (odd || (v_least < 0x7F800000u && pf_exponent(v_least) < pf_exponent(v_most) - kTrApartV)) sm.redo[it % kTrLists] = 1;
+            sm.v_exp[note] = v_exp;
+            mbar_arrive(smem_u32(&sm.v_note[note]));
+          }
+          tr_convert_v<VBITS>(sm.v[b], pages, stride, lay, visible, pow2f(-v_exp), ct);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(is_v ? &sm.v_full[b] : &sm.k_full[b]));
+          mbar_arrive(smem_u32(&sm.raw_free[slot]));
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sm.list_free[it % kTrLists]));
+    }
+  } else {
+    // --------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTrRegsSoftmax));
+    const int t = warp >> 2, row = tid & 127;
+    const uint32_t tile = tmem + t * kTrTmemTile + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    struct Row {
+      long long q, out;                                  // where its query and result are; q < 0: not a row
+      const uint32_t* sees;
+      float mul;                                         // what its scores are multiplied with, but for K's power of two
+    };
+    // the row of the thread in item `it`, and Q of its tile; false: no more items
+    auto begin = [&](int it, Row& r) {
+      const TrItem& l = sm.list[it % kTrLists];
+      if (ok) ok = mbar_wait_park(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      r.q = r.out = -1;
+      r.sees = p.masks;
+      r.mul = 0.f;
+      if (!ok || l.kvh < 0) return false;
+      const int at = t * kTrRows + row;
+      if (at < l.rows) {
+        const int node = (l.first + at) / G, col = (l.kvh * G + (l.first + at - node * G)) * kD;
+        r.q = (l.row0 + node) * p.ldq + col;
+        r.out = (l.row0 + node) * p.ldo + col;
+        r.sees = p.masks + (l.row0 + node) * p.ldm;
+      }
+      if (l.steps > 0 && t * kTrRows < l.rows) {
+        // a power of two brings the row's largest magnitude to 2^10 .. 2^11; what is not finite stays
+        uint32_t most = 0;
+        if (r.q >= 0) {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const uint4 u = reinterpret_cast<const uint4*>(p.q + r.q)[c];
+            const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most = max(most, max(in[j] & 0x7FFFu, in[j] >> 16 & 0x7FFFu));
+          }
+        }
+        const int e = most >= 0x7F80u || most == 0u ? 0 : max(static_cast<int>(most >> 7) - 127 - 10, -126);
+        const float down = pow2f(-e);
+        r.mul = pow2f(e) * p.scale * 1.4426950408889634f;
+        uint32_t x[32];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (r.q >= 0) u = reinterpret_cast<const uint4*>(p.q + r.q)[h * 8 + c];
+            const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&in[j]));
+              x[c * 4 + j] = pack_f16x2(f.x * down, f.y * down);
+            }
+          }
+          if (h == 0) {
+            tmem_st_32x32(tile + kTrTmemQ, x);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<uint4*>(sm.q[t] + row * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+          }
+        }
+        tmem_st_wait();
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.q_full[t]));
+      }
+      return true;
+    };
+    int gs = 0, n = 0;                                   // steps of earlier items; steps that this tile took part in
+    Row cur;
+    bool more = begin(0, cur);
+    for (int it = 0; more; ++it) {
+      const TrItem& l = sm.list[it % kTrLists];
+      const int steps = l.steps, start = l.start, total = l.total;
+      const bool in = t * kTrRows < l.rows, mine = cur.q >= 0;
+      float m = -INFINITY, sum = 0.f;
+      int v_exp = 0;
+      if (!in) {
+        gs += steps;
+      } else {
+        for (int s = 0; s < steps; ++s, ++gs) {
+          const int note = gs % kTrNotes, tok0 = (l.lo + s) * kTrTok;
+          if (ok) ok = mbar_wait_park(smem_u32(&sm.s_full[t]), n & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_after();
+          uint32_t a[2][32];
+          tmem_ld_32x32(tile, a[0]);
+          tmem_ld_32x32(tile + 32, a[1]);
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sm.s_free[t]));
+          // (a note is written again after this step's product, which waits for what follows: kTrNotes)
+          if (ok) ok = mbar_wait_park(smem_u32(&sm.k_note[note]), (gs / kTrNotes) & 1, abort_flag);
+          if (ok) ok = mbar_wait_park(smem_u32(&sm.v_note[note]), (gs / kTrNotes) & 1, abort_flag);
+          if (tok0 + kTrTok > start) {
+            const uint2 see = mine ? tr_visible(cur.sees, p.words, start, total, tok0) : make_uint2(0u, 0u);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (!(see.x >> j & 1u)) a[0][j] = 0xFF800000u;                            // -inf
+              if (!(see.y >> j & 1u)) a[1][j] = 0xFF800000u;
+            }
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < kTrTok; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(a[j >> 5][j & 31]));
+          const float mul = sm.k_mul[note] * cur.mul, top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+          float alpha = 1.f;
+          bool grew = top > m + kTrGrowth || (m == -INFINITY && top > m);
+          if (grew) {
+            alpha = fast_exp2(m - top);
+            m = top;
+            sum *= alpha;
+          }
+          const int e = sm.v_exp[note];
+          if (e != v_exp) {
+            alpha = v_exp - e < -126 ? 0.f : alpha * pow2f(v_exp - e);
+            v_exp = e;
+            grew = true;
+          }
+          const float use = m == -INFINITY ? 0.f : m;
+          const float2 less = make_float2(-use, -use), mul2 = make_float2(mul, mul);
+          float2 part_sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          uint32_t pr[32];
+#pragma unroll
+          for (int j = 0; j < kTrTok / 2; ++j) {
+            const float2 d = __ffma2_rn(make_float2(__uint_as_float(a[j >> 4][2 * j & 31]), __uint_as_float(a[j >> 4][(2 * j + 1) & 31])), mul2, less);
+            const float2 x = make_float2(fast_exp2(d.x), fast_exp2(d.y));
+            part_sum[j & 1] = __fadd2_rn(part_sum[j & 1], x);
+            pr[j] = pack_f16x2(x.x, x.y);
+          }
+          sum += (part_sum[0].x + part_sum[0].y) + (part_sum[1].x + part_sum[1].y);
+          // the previous product has read the probabilities and written the output
+          if (ok && s > 0) ok = mbar_wait_park(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_after();
+          tmem_st_32x32(tile + kTrTmemP, pr);
+          if (s > 0 && __any_sync(0xffffffffu, grew)) {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32(tile + kTrTmemO + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+              tmem_st_32x32(tile + kTrTmemO + c * 32, o);
+            }
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[t]));
+          ++n;
+        }
+      }
+      // the next item's Q while the last product runs (all of this item's scores are there)
+      Row next;
+      more = begin(it + 1, next);
+      if (in) {
+        const int part = l.part;
+        const size_t at = (static_cast<size_t>(max(part, 0)) * part_rows + t * kTrRows + row);
+        if (steps == 0) {                                // a request that is told wrongly
+          if (mine) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) reinterpret_cast<uint4*>(p.out + cur.out)[j] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        } else {
+          if (ok) ok = mbar_wait_park(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_after();
+          const float up = pow2f(v_exp), inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;           // NaN stays
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32(tile + kTrTmemO + c * 32, o);
+            tmem_ld_wait();
+            if (mine) {
+              if (part >= 0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  reinterpret_cast<float4*>(part_o + at * kD + c * 32)[j] =
+                      make_float4(__uint_as_float(o[4 * j]) * up, __uint_as_float(o[4 * j + 1]) * up, __uint_as_float(o[4 * j + 2]) * up, __uint_as_float(o[4 * j + 3]) * up);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  uint32_t x[4];
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) x[k] = pack_bf16x2(__uint_as_float(o[8 * j + 2 * k]) * inv * up, __uint_as_float(o[8 * j + 2 * k + 1]) * inv * up);
+                  *reinterpret_cast<uint4*>(p.out + cur.out + c * 32 + j * 8) = make_uint4(x[0], x[1], x[2], x[3]);
+                }
+              }
+            }
+          }
+          tc_fence_before();
+          if (part >= 0 && mine) part_ml[at] = make_float2(m, sum);
+          if (*const_cast<volatile uint32_t*>(&sm.redo[it % kTrLists]) && ok) {
+            __syncwarp();                                // a row's result is written again by other lanes
+            TreeRequest r;
+            r.slot = l.slot; r.row0 = l.row0; r.count = l.count; r.start = start; r.total = total;
+            const int lo = l.lo * kTrTok, hi = min(total, (l.lo + steps) * kTrTok);
+#pragma unroll 1
+            for (uint32_t rows = __ballot_sync(0xffffffffu, mine); rows; rows &= rows - 1) {
+              const int of = __ffs(rows) - 1;
+              const long long q = __shfl_sync(0xffffffffu, cur.q, of), out = __shfl_sync(0xffffffffu, cur.out, of);
+              const uint32_t* sees = reinterpret_cast<const uint32_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(cur.sees), of));
+              float rm, rs, o[4];
+              tree_row<KBITS, VBITS>(p, lay, r, l.kvh, lo, hi, sees, p.q + q, lane, rm, rs, o, bad);
+              if (part >= 0) {
+                const size_t to = at - lane + of;
+                reinterpret_cast<float4*>(part_o + to * kD)[lane] = make_float4(o[0], o[1], o[2], o[3]);
+                if (lane == 0) part_ml[to] = make_float2(rm, rs);
+              } else {
+                const float f = rs > 0.f ? 1.f / rs : rs == 0.f ? 0.f : rs;
+                reinterpret_cast<uint2*>(p.out + out)[lane] = make_uint2(pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f));
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sm.list_free[it % kTrLists]));
+      cur = next;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 16) tmem_dealloc(tmem, kTrTmemCols);
+  if (bad) atomicExch(p.status, static_cast<uint32_t>(kErrBadArgument));
+  if (tid == 0 && sm.abort_word) atomicExch(p.status, static_cast<uint32_t>(kErrBarrierTimeout));
+}
+
+// Joins the parts of items that several CTAs shared: block x looks after the item that began in CTA x and went on beyond it.  A warp has a row at a time.
+__global__ void __launch_bounds__(256)
+tree_merge_kernel(const CbTreeAttn p, const int part_rows) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const float* part_o = p.partial;
+  const float2* part_ml = reinterpret_cast<const float2*>(part_o + static_cast<size_t>(gridDim.x) * 2 * part_rows * kD);
+  const TrDesc d = reinterpret_cast<const TrDesc*>(part_ml + static_cast<size_t>(gridDim.x) * 2 * part_rows)[blockIdx.x];
+  const int lane = threadIdx.x & 31, G = p.Hq / p.Hkv;
+  for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); d.parts > 0 && row < d.rows; row += gridDim.y * 8) {
+    auto at = [&](int c) { return static_cast<size_t>(2 * (blockIdx.x + c) + (c == 0)) * part_rows + row; };
+    float m = -INFINITY;
+    for (int c = lane; c < d.parts; c += 32) m = fmaxf(m, __ldcg(part_ml + at(c)).x);
+    m = warp_max(m);
+    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < d.parts; ++c) {
+      const float2 ml = __ldcg(part_ml + at(c));
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(part_o + at(c) * kD) + lane);
+      const float f = fast_exp2(ml.x - (m == -INFINITY ? 0.f : m));                    // of a part that saw nothing: zero
+      sum = fmaf(f, ml.y, sum);
+      o[0] = fmaf(f, x.x, o[0]); o[1] = fmaf(f, x.y, o[1]); o[2] = fmaf(f, x.z, o[2]); o[3] = fmaf(f, x.w, o[3]);
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    const int node = (d.first + row) / G, col = (d.kvh * G + (d.first + row - node * G)) * kD;
+    reinterpret_cast<uint2*>(p.out + (d.row0 + node) * p.ldo + col)[lane] = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+  }
+}
+
+template <int KB, int VB>
+static int launch_tree(const CbTreeAttn& p, cudaStream_t st) {
+  const KvLayout lay = make_kv_layout(kD, KB, VB);
+  const int stride = (lay.blob_bytes + 127) & ~127;
+  const size_t smem = sizeof(TrSmem) + 1024 + static_cast<size_t>(kTrRaw) * kTrPages * stride;
+  static int sms[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -18;
+  if (!sms[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(tree_kernel<KB, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    int n = 0;
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    // the warps' new shares come out of the registers that the block was launched with
+    cudaFuncAttributes at;
+    e = cudaFuncGetAttributes(&at, tree_kernel<KB, VB>);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (at.numRegs < kTrRegs) return -19;
+    sms[dev] = n;
+  }
+  const int rows = tr_rows(p.words, p.rows, p.Hq / p.Hkv);
+  cudaError_t e = launch(tree_kernel<KB, VB>, dim3(sms[dev]), dim3(kTrThreads), smem, st, p, lay, rows);
+  if (e == cudaSuccess) e = launch(tree_merge_kernel, dim3(sms[dev], (rows + 15) / 16), dim3(256), 0, st, p, rows);
+  return static_cast<int>(e);
 }
 
 }  // namespace cb
 
-extern "C" int cb_tree_attn(const CbTreeAttn* p, void* stream) {
-  using namespace cb;
-  if (p->n <= 0) return 0;
-  if (p->n > kTreeMaxRequests || p->words < 1 || p->words > kTreeMaxWords || p->Hkv <= 0 || p->Hq % p->Hkv != 0 || p->Hq / p->Hkv > kTreeMaxGroup || p->width > 1 << 26) return -10;
-  const KvLayout lay = make_kv_layout(kD, p->k_bits, p->v_bits);
-  return with_kv_bits(p->k_bits, p->v_bits, [&](auto kb, auto vb) {
-    return static_cast<int>(launch(tree_simple_kernel<decltype(kb)::value, decltype(vb)::value>, dim3(p->n, p->Hkv, 8), dim3(256), 0, static_cast<cudaStream_t>(stream), *p, lay));
-  });
+extern "C" {
+
+// fp32 scratch elements of a launch on a GPU of `sms` multiprocessors
+long long cb_tree_attn_floats(int sms, int words, int rows, int group) {
+  return static_cast<long long>(sms) * (2 * cb::tr_rows(words, rows, group) * (cb::kD + 2) + static_cast<long long>(sizeof(cb::TrDesc) / 4));
 }
+
+int cb_tree_attn(const CbTreeAttn* p, void* stream) {
+  using namespace cb;
+  if (p->n <= 0 || p->rows <= 0) return 0;
+  if (p->n > kTreeMaxRequests || p->words < 1 || p->words > kTreeMaxWords || p->Hkv <= 0 || p->Hq % p->Hkv != 0 || p->Hq / p->Hkv > kTreeMaxGroup || p->width > 1 << 26) return -10;
+  if (!p->partial) return -12;
+  return with_kv_bits(p->k_bits, p->v_bits, [&](auto kb, auto vb) { return launch_tree<decltype(kb)::value, decltype(vb)::value>(*p, static_cast<cudaStream_t>(stream)); });
+}
+
+}  // extern "C"

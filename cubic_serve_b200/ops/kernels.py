@@ -7,6 +7,7 @@ PyTorch fallback on the GPU path: a missing library is an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 
@@ -992,6 +993,11 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> int:
     return ld
 
 
+@functools.lru_cache(maxsize=256)
+def _tree_floats(device: int, words: int, rows: int, group: int) -> int:
+    return native.lib().cb_tree_attn_floats(sm_count(torch.device("cuda", device)), words, rows, group)
+
+
 def tree_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, request: torch.Tensor, row0: torch.Tensor, count: torch.Tensor,
                    start: torch.Tensor, masks: torch.Tensor, hq: int, hkv: int, head_dim: int, k_bits: int, v_bits: int, scale: float | None = None,
                    ws: Workspace | None = None) -> torch.Tensor:
@@ -1019,13 +1025,17 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, page
              and cache.data_ptr() % 16 == 0, "cache: uint8 [pages, hkv, bytes of a page and head]")
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
     _require(0.0 < scale < math.inf, "the scale is above zero")
+    requests = (_vector(request, i32, n, "request"), _vector(row0, i32, n, "row0"), _vector(count, i32, n, "count"), _vector(start, i32, n, "start"))
+    device = q.get_device()
+    _require(device >= 0, "tensors must be on a GPU")
+    if not n or not rows:
+        return out
     ws = ws or workspace(q.device)
+    ws.ensure_attn(_tree_floats(device, words, rows, hq // hkv))
     packed = native.TREE_ATTN.pack(
-        at, out.data_ptr(), cache.data_ptr(), page_table.data_ptr(), _vector(request, i32, n, "request"), _vector(row0, i32, n, "row0"), _vector(count, i32, n, "count"),
-        _vector(start, i32, n, "start"), masks.data_ptr(), ws.status.data_ptr(), ldq, ldo, ld, ldm, n, rows, page_table.shape[0], page_table.shape[1], cache.shape[0], words,
+        at, out.data_ptr(), cache.data_ptr(), page_table.data_ptr(), *requests, masks.data_ptr(), ws.status.data_ptr(), ws.attn.data_ptr(), ldq, ldo, ld, ldm, n, rows, page_table.shape[0], page_table.shape[1], cache.shape[0], words,
         hq, hkv, k_bits, v_bits, scale)
-    if n and rows:
-        _call("cb_tree_attn", (packed,), (q, out, cache, page_table, request, row0, count, start, masks, ws.status))
+    _call("cb_tree_attn", (packed,), (q, out, cache, page_table, request, row0, count, start, masks, ws.status))
     return out
 
 

@@ -333,6 +333,8 @@ def _declare(l: ctypes.CDLL) -> None:
     # what a step does for each of its requests: layout, adapters, draws from a whole vocabulary
     l.cb_adapter_rows.argtypes = [vp, i, i, vp, vp, vp, vp]
     # ... and of drafts in trees: their attention, the logits that requests want, the path that is kept
+    l.cb_tree_attn_floats.argtypes = [i, i, i, i]
+    l.cb_tree_attn_floats.restype = ll
     for name in ("step_layout", "adapter_add", "sample_vocabulary", "tree_attn", "adjust_logits", "verify_tree", "keep_tokens"):
         getattr(l, f"cb_{name}").argtypes = [vp, vp]
     for name in ("step_layout", "adapter_rows", "adapter_add", "sample_vocabulary", "tree_attn", "adjust_logits", "verify_tree", "keep_tokens"):
@@ -568,7 +570,7 @@ class ScoredMoeStruct(ctypes.Structure):
 STEP_LAYOUT = struct.Struct("@15P9i4x")                      # CbStepLayout, csrc/step_layout.cu
 ADAPTER = struct.Struct("@PqPqPq10P10i")                      # CbAdapter, csrc/adapters.cu
 VOCABULARY = struct.Struct("@PqPq11P4i")                     # CbVocabulary, csrc/sample_vocabulary.cu
-TREE_ATTN = struct.Struct("@10P4q10if4x")                    # CbTreeAttn, csrc/tree_attn.cu
+TREE_ATTN = struct.Struct("@11P4q10if4x")                    # CbTreeAttn, csrc/tree_attn.cu
 VERIFY_TREE = struct.Struct("@8P3i4x")                       # CbVerifyTree, csrc/draft_tree.cu
 KEEP_TOKENS = struct.Struct("@7P2q9i4x")                     # CbKeepTokens, csrc/draft_tree.cu
 ADJUST = struct.Struct("@16P5q8i")                           # CbAdjust, csrc/adjust_logits.cu

@@ -75,7 +75,10 @@ class _Round:
 
         Keys, values and probabilities are rounded to f16 (2^-11 of each), the result to bf16 (2^-8); a score is off by 2^-11 of the sum of
         its products' magnitudes at most, which moves a probability and its sum by as much; sums in 32 bits, exponentials and
-        the sums of the matrix units add less than 2^-16."""
+        the sums of the matrix units add less than 2^-16.
+
+        A probability below 2^-14 has the absolute steps of f16's smallest numbers instead: it is off by half of one, 2^-25, at most, relative to a running
+        maximum that is not above the row's own, so that the sum it is divided by is one at least: 2^-25 of the sum of the values' magnitudes."""
         ref, tol = torch.zeros(self.q.shape, dtype=torch.float64), torch.zeros(self.q.shape, dtype=torch.float64)
         cache, table, group = self.cache.cpu(), self.table.cpu(), self.hq // self.hkv
         for i, (s, c) in enumerate(self.sizes):
@@ -97,7 +100,7 @@ class _Round:
                 p = torch.where(sums > 0, p / sums, 0.0)
                 o, a = torch.einsum("cgt,td->cgd", p, v), torch.einsum("cgt,td->cgd", p, v.abs())
                 e = torch.where(sees[:, None], off, 0.0).amax(-1, keepdim=True)
-                t = (torch.expm1(2 * e) + 2 * 2.0 ** -11 + 2.0 ** -16) * a * 1.01 + 2.0 ** -8 * o.abs()
+                t = (torch.expm1(2 * e) + 2 * 2.0 ** -11 + 2.0 ** -16) * a * 1.01 + 2.0 ** -8 * o.abs() + 2.0 ** -25 * torch.einsum("cgt,td->cgd", sees[:, None].double().expand(z.shape), v.abs())
                 ref[rows, h * group * D:(h + 1) * group * D], tol[rows, h * group * D:(h + 1) * group * D] = o.reshape(c, -1), t.reshape(c, -1)
         return ref, tol
 
