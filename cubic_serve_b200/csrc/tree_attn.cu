@@ -105,7 +105,10 @@ static constexpr int kTrThreads = 640;
 static constexpr int kTrRegs = 96, kTrRegsSoftmax = 136, kTrRegsConvert = 72, kTrRegsOther = 64;
 static_assert(2 * kTrRegsSoftmax + 2 * kTrRegsConvert + kTrRegsOther <= 5 * kTrRegs, "five warpgroups");
 static constexpr int kTrLists = 4, kTrRaw = 4;
-static constexpr int kTrNotes = kTrRaw + 2;
+static constexpr int kTrOps = 3;                         // steps of operands
+// Steps whose powers of two are kept: the note of step s is written behind raw_full (s) <- raw_free (s - kTrRaw) <- v_free of step s - kTrRaw - kTrOps <- p_full of the
+// tiles that take part in it, which have read their notes by then.
+static constexpr int kTrNotes = kTrRaw + kTrOps;
 static constexpr int kTrLeast = 1;                       // steps of a CTA, at least
 static constexpr float kTrGrowth = 2.f;
 static constexpr int kTrApartK = 18, kTrApartV = 14;
@@ -122,18 +125,25 @@ struct TrItem {
 struct TrDesc { int parts, row0, first, rows, kvh, pad[3]; };
 struct __align__(1024) TrSmem {
   uint8_t q[kTrTiles][kTrRows * 128];                    // f16, channels 64..127: [row][128 B], 16-byte chunk ^ (row & 7)
-  uint8_t k[2][2 * kTrHalf];                             // f16 [stage][64-channel half][token][128 B]
-  uint8_t v[2][2 * kTrHalf];                             // likewise
+  uint8_t k[kTrOps][2 * kTrHalf];                             // f16 [stage][64-channel half][token][128 B]
+  uint8_t v[kTrOps][2 * kTrHalf];                             // likewise
   float k_mul[kTrNotes];                                 // scores are this times what the MMAs give
   int v_exp[kTrNotes];                                   // output is 2^v_exp times ...
   uint32_t redo[kTrLists];                               // of an item's steps: some values are beyond what f16 operands hold
-  uint64_t raw_full[kTrRaw], raw_free[kTrRaw], k_full[2], k_free[2], v_full[2], v_free[2], k_note[kTrNotes], v_note[kTrNotes];
+  uint64_t raw_full[kTrRaw], raw_free[kTrRaw], k_full[kTrOps], k_free[kTrOps], v_full[kTrOps], v_free[kTrOps], k_note[kTrNotes], v_note[kTrNotes];
   uint64_t list_full[kTrLists], list_free[kTrLists], q_full[kTrTiles], s_full[kTrTiles], s_free[kTrTiles], p_full[kTrTiles], pv_done[kTrTiles];
+  uint64_t exch_full, exch_free;
   TrItem list[kTrLists];
+  float2 exch_ml[kTrTiles][kTrRows];                     // rows in both tiles: maximum and sum, ...
+  int exch_exp[kTrTiles][kTrRows];                       // ... and v_exp
   long long sums[kTrThreads / 32];
   uint32_t tmem, abort_word;
   long long upto[kTreeMaxRequests + 1];                  // steps of the requests before
 };
+
+// Items of one tile's rows have them in both tiles, which take its steps in turn (two warps of a kind on a scheduler where one would wait for itself).
+__device__ __forceinline__ bool tr_split(const TrItem& l) { return l.rows <= kTrRows; }
+__device__ __forceinline__ bool tr_takes_part(const TrItem& l, int t) { return tr_split(l) ? l.steps > t : l.steps > 0; }
 
 __device__ __forceinline__ int tr_steps(const TreeRequest& r) { return max(1, (r.total + kTrTok - 1) / kTrTok); }
 __device__ __forceinline__ int tr_groups(const TreeRequest& r, int G) { return (r.count * G + kTrItemRows - 1) / kTrItemRows; }
@@ -153,47 +163,40 @@ __device__ __forceinline__ uint32_t tr_scaled(uint32_t code, uint32_t sh, uint32
 __device__ __forceinline__ uint4 tr_scaled8(const uint4& c, uint32_t sh, uint32_t sl) {
   return make_uint4(tr_scaled(c.x, sh, sl), tr_scaled(c.y, sh, sl), tr_scaled(c.z, sh, sl), tr_scaled(c.w, sh, sl));
 }
+// (The loops stay loops: four kinds of warps run their code at the same time, and unrolled it does not fit the instruction caches.)
 template <int KBITS>
 __device__ __forceinline__ void tr_convert_k(uint8_t (&k)[2 * kTrHalf], const uint8_t* raw, int stride, const KvLayout& lay, float mul, int tid) {
   constexpr uint32_t kb = KBITS == 8 ? 0x64806480u : KBITS == 6 ? 0x64206420u : 0x64086408u;
-  constexpr int kItems = KBITS == 8 ? kPageTokens * 8 : kPageTokens * 4, kMine = kTrPages * kItems / 128;
-  uint4 x[kMine], xh[kMine];
-  float s[kMine];
-#pragma unroll
-  for (int j = 0; j < kMine; ++j) {
-    const int i = tid + j * 128, r = i % kItems, tok = r & 15, blk = r >> 4;
-    const uint8_t* src = raw + i / kItems * stride;
-    x[j] = *reinterpret_cast<const uint4*>(src + blk * 256 + tok * 16);
-    if constexpr (KBITS == 6) xh[j] = *reinterpret_cast<const uint4*>(src + kPageTokens * kD / 2 + blk * 128 + (tok & 7) * 16);
-    s[j] = *reinterpret_cast<const float*>(src + lay.k_scale_off + tok * 16 + (KBITS == 8 ? blk >> 1 : blk) * 4);
-  }
-#pragma unroll
-  for (int j = 0; j < kMine; ++j) {
-    const int i = tid + j * 128, r = i % kItems, tok = r & 15, blk = r >> 4, sw = tok & 7;
-    uint4* row = reinterpret_cast<uint4*>(k + (KBITS == 8 ? blk >> 2 : blk >> 1) * kTrHalf + (i / kItems * 16 + tok) * 128);
-    const int c = KBITS == 8 ? (blk & 3) * 2 : (blk & 1) * 4;
+  // an item is a scale's 32 channels of a token
+  const int tok = tid & 15, g = tid >> 4 & 3, sw = tok & 7;
+#pragma unroll 1
+  for (int page = tid >> 6; page < kTrPages; page += 2) {
+    const uint8_t* src = raw + page * stride;
+    uint4* row = reinterpret_cast<uint4*>(k + (g >> 1) * kTrHalf + (page * 16 + tok) * 128);
     uint32_t sh, sl;
-    pf_split(s[j] * mul, sh, sl);
-    auto put = [&](int chunk, uint2 codes) { row[chunk ^ sw] = tr_scaled8(conv8(codes, kb), sh, sl); };
-    if constexpr (KBITS == 8) {
-      put(c, make_uint2(x[j].x, x[j].y));
-      put(c + 1, make_uint2(x[j].z, x[j].w));
-    } else {
-      const uint32_t n[4] = {x[j].x, x[j].y, x[j].z, x[j].w}, hw[4] = {xh[j].x, xh[j].y, xh[j].z, xh[j].w};
-      uint32_t lo[4], hi[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        lo[q] = n[q] & 0x0F0F0F0Fu;
-        hi[q] = (n[q] >> 4) & 0x0F0F0F0Fu;
+    pf_split(*reinterpret_cast<const float*>(src + lay.k_scale_off + tok * 16 + g * 4) * mul, sh, sl);
+    uint4 x, w = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (KBITS != 8) x = *reinterpret_cast<const uint4*>(src + g * 256 + tok * 16);
+    if constexpr (KBITS == 6) {
+      w = *reinterpret_cast<const uint4*>(src + kPageTokens * kD / 2 + g * 128 + (tok & 7) * 16);
+      if (tok >= 8) { w.x <<= 4; w.y <<= 4; w.z <<= 4; w.w <<= 4; }                      // (what leaves a byte's bits 4 to 7 is masked)
+    }
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {                        // 16 channels
+      uint4 n;
+      if constexpr (KBITS == 8) {
+        n = *reinterpret_cast<const uint4*>(src + g * 512 + h * 256 + tok * 16);
+      } else {
+        n = make_uint4(x.x & 0x0F0F0F0Fu, x.y & 0x0F0F0F0Fu, x.z & 0x0F0F0F0Fu, x.w & 0x0F0F0F0Fu);
+        x = make_uint4(x.x >> 4, x.y >> 4, x.z >> 4, x.w >> 4);
         if constexpr (KBITS == 6) {
-          lo[q] |= (tok < 8 ? hw[q] : hw[q] << 4) & 0x30303030u;
-          hi[q] |= (tok < 8 ? hw[q] >> 2 : hw[q] << 2) & 0x30303030u;
+          n = make_uint4(n.x | (w.x & 0x30303030u), n.y | (w.y & 0x30303030u), n.z | (w.z & 0x30303030u), n.w | (w.w & 0x30303030u));
+          w = make_uint4(w.x >> 2, w.y >> 2, w.z >> 2, w.w >> 2);
         }
       }
-      put(c, make_uint2(lo[0], lo[1]));
-      put(c + 1, make_uint2(lo[2], lo[3]));
-      put(c + 2, make_uint2(hi[0], hi[1]));
-      put(c + 3, make_uint2(hi[2], hi[3]));
+      const int c = (g & 1) * 4 + h * 2;
+      row[c ^ sw] = tr_scaled8(conv8(make_uint2(n.x, n.y), kb), sh, sl);
+      row[(c + 1) ^ sw] = tr_scaled8(conv8(make_uint2(n.z, n.w), kb), sh, sl);
     }
   }
 }
@@ -201,49 +204,56 @@ __device__ __forceinline__ void tr_convert_k(uint8_t (&k)[2 * kTrHalf], const ui
 template <int VBITS>
 __device__ __forceinline__ void tr_convert_v(uint8_t (&v)[2 * kTrHalf], const uint8_t* raw, int stride, const KvLayout& lay, int visible, float mul, int tid) {
   constexpr uint32_t vb = VBITS == 8 ? 0x64806480u : VBITS == 6 ? 0x64206420u : 0x64086408u;
-  // an item is 8 channels of a token pair of a page
-  const int c = tid & 15, pair = tid >> 4, at = (2 * c) ^ ((pair & 3) << 2);
-  uint4 x[kTrPages];                                     // 8 bit: the codes; else low nibbles, high bits
-  float s[kTrPages][2];
-#pragma unroll
-  for (int j = 0; j < kTrPages; ++j) {
-    const uint8_t* page = raw + j * stride;
-    const uint8_t* src = page + lay.v_code_off;
-    if constexpr (VBITS == 8) {
-      x[j] = *reinterpret_cast<const uint4*>(src + pair * 256 + at * 8);
-    } else {
-      const uint2 n = *reinterpret_cast<const uint2*>(src + pair * 128 + at * 4);
-      uint2 hw = make_uint2(0u, 0u);
-      if constexpr (VBITS == 6) hw = *reinterpret_cast<const uint2*>(src + kPageTokens * kD / 2 + (pair & 3) * 128 + at * 4);
-      x[j] = make_uint4(n.x, n.y, hw.x, hw.y);
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) s[j][h] = *reinterpret_cast<const float*>(page + lay.v_scale_off + (2 * pair + h) * 16 + (c >> 2) * 4);
-  }
-#pragma unroll
-  for (int j = 0; j < kTrPages; ++j)
+  // an item is 16 channels of a token pair, eight at a time: lanes 0-3 of eight take the first eight first, the others the second (no bank twice)
+  const int c = tid & 7, pair = tid >> 3 & 7, first = tid >> 2 & 1;
+  const int at = (4 * c) ^ ((pair & 3) << 2);
+#pragma unroll 1
+  for (int page = tid >> 6; page < kTrPages; page += 2) {
+    const uint8_t* src = raw + page * stride;
+    const uint8_t* codes = src + lay.v_code_off;
+    const int tok = page * 16 + pair * 2;
+    uint32_t sh[2], sl[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int tok = (j * 8 + pair) * 2 + h;
-      uint4 codes;
-      if constexpr (VBITS == 8) {
-        const uint32_t sel = h ? 0x5341u : 0x5240u;
-        codes = make_uint4(u8x2_to_f16x2(x[j].x, sel, vb), u8x2_to_f16x2(x[j].y, sel, vb), u8x2_to_f16x2(x[j].z, sel, vb), u8x2_to_f16x2(x[j].w, sel, vb));
-      } else {
-        uint2 n = h ? make_uint2((x[j].x >> 4) & 0x0F0F0F0Fu, (x[j].y >> 4) & 0x0F0F0F0Fu) : make_uint2(x[j].x & 0x0F0F0F0Fu, x[j].y & 0x0F0F0F0Fu);
-        if constexpr (VBITS == 6) {
-          auto high = [&](uint32_t w) { return (pair < 4 ? (h ? w >> 2 : w) : (h ? w << 2 : w << 4)) & 0x30303030u; };
-          n.x |= high(x[j].z);
-          n.y |= high(x[j].w);
-        }
-        codes = conv8(n, vb);
-      }
-      float f = s[j][h] * mul;
-      if (tok >= visible || !(fabsf(f) < INFINITY)) f = 0.f;
-      uint32_t sh, sl;
-      pf_split(f, sh, sl);
-      *reinterpret_cast<uint4*>(v + (c >> 3) * kTrHalf + tok * 128 + (((c & 7) ^ (tok & 7)) << 4)) = tr_scaled8(codes, sh, sl);
+      float f = *reinterpret_cast<const float*>(src + lay.v_scale_off + (2 * pair + h) * 16 + (c >> 1) * 4) * mul;
+      if (tok + h >= visible || !(fabsf(f) < INFINITY)) f = 0.f;
+      pf_split(f, sh[h], sl[h]);
     }
+#pragma unroll 1
+    for (int e = 0; e < 2; ++e) {
+      const int half = first ^ e;
+      uint4 x;
+      if constexpr (VBITS == 8) {
+        x = *reinterpret_cast<const uint4*>(codes + pair * 256 + (at + 2 * half) * 8);
+      } else {
+        const uint2 n = *reinterpret_cast<const uint2*>(codes + pair * 128 + (at + 2 * half) * 4);
+        uint2 hw = make_uint2(0u, 0u);
+        if constexpr (VBITS == 6) {
+          hw = *reinterpret_cast<const uint2*>(codes + kPageTokens * kD / 2 + (pair & 3) * 128 + (at + 2 * half) * 4);
+          const int up = pair < 4 ? 0 : 4;
+          hw.x <<= up; hw.y <<= up;
+        }
+        x = make_uint4(n.x, n.y, hw.x, hw.y);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 f;
+        if constexpr (VBITS == 8) {
+          const uint32_t sel = h ? 0x5341u : 0x5240u;
+          f = make_uint4(u8x2_to_f16x2(x.x, sel, vb), u8x2_to_f16x2(x.y, sel, vb), u8x2_to_f16x2(x.z, sel, vb), u8x2_to_f16x2(x.w, sel, vb));
+        } else {
+          uint2 n = h ? make_uint2((x.x >> 4) & 0x0F0F0F0Fu, (x.y >> 4) & 0x0F0F0F0Fu) : make_uint2(x.x & 0x0F0F0F0Fu, x.y & 0x0F0F0F0Fu);
+          if constexpr (VBITS == 6) {
+            n.x |= (h ? x.z >> 2 : x.z) & 0x30303030u;
+            n.y |= (h ? x.w >> 2 : x.w) & 0x30303030u;
+          }
+          f = conv8(n, vb);
+        }
+        const int chunk = 2 * c + half;
+        *reinterpret_cast<uint4*>(v + (chunk >> 3) * kTrHalf + (tok + h) * 128 + (((chunk & 7) ^ ((tok + h) & 7)) << 4)) = tr_scaled8(f, sh[h], sl[h]);
+      }
+    }
+  }
 }
 // The smallest magnitude of a token's scales that is not zero, as bits
 __device__ __forceinline__ uint32_t tr_least(const float4& s) {
@@ -252,6 +262,15 @@ __device__ __forceinline__ uint32_t tr_least(const float4& s) {
     return b == 0u ? 0x7F800000u : b;
   };
   return min(min(magnitude(s.x), magnitude(s.y)), min(magnitude(s.z), magnitude(s.w)));
+}
+
+__device__ __forceinline__ void tr_tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void tr_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
 }
 
 // 64 bits: which of the tokens [tok0, tok0 + 64) a row sees.  `sees`: its words.
@@ -296,7 +315,7 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
       mbar_init(smem_u32(&sm.raw_full[b]), 1);
       mbar_init(smem_u32(&sm.raw_free[b]), 8);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kTrOps; ++b) {
       mbar_init(smem_u32(&sm.k_full[b]), 4);
       mbar_init(smem_u32(&sm.k_free[b]), 1);
       mbar_init(smem_u32(&sm.v_full[b]), 4);
@@ -317,6 +336,8 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
       mbar_init(smem_u32(&sm.p_full[t]), 4);
       mbar_init(smem_u32(&sm.pv_done[t]), 1);
     }
+    mbar_init(smem_u32(&sm.exch_full), 8);
+    mbar_init(smem_u32(&sm.exch_free), 8);
     sm.abort_word = 0;
     mbar_fence_init();
   }
@@ -417,29 +438,35 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
         if (l.kvh >= 0) ids_next = ids_of(l, 0);
         return l.kvh >= 0;
       };
-      bool more = publish(0);
-      for (int it = 0; more && ok; ++it) {
-        const TrItem l = sm.list[it % kTrLists];
-        const int pages = (l.total + kPageTokens - 1) / kPageTokens;
-        bool next = false;
-        int ids = ids_next, ids_later = 0;
-        for (int s = 0; s < l.steps; ++s, ++gs) {
-          if (s > 0 && s % 8 == 0) ids = ids_later;
-          const int b = gs % kTrRaw;
-          if (ok && gs >= kTrRaw) ok = mbar_wait_park(smem_u32(&sm.raw_free[b]), (gs / kTrRaw - 1) & 1, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int n = min(kTrPages, pages - (l.lo + s) * kTrPages);
-          if (lane == 0) mbar_expect_tx(smem_u32(&sm.raw_full[b]), n * lay.blob_bytes);
-          __syncwarp();
-          const int page = __shfl_sync(0xffffffffu, ids, (s % 8) * kTrPages + (lane & 3));
-          if (lane < n)
-            bulk_g2s(smem_u32(raw + (b * kTrPages + lane) * stride), p.cache + (static_cast<size_t>(page) * p.Hkv + l.kvh) * lay.blob_bytes, lay.blob_bytes, smem_u32(&sm.raw_full[b]));
-          if (s % 8 == 0 && s + 8 < l.steps) ids_later = ids_of(l, s + 8);
-          if (s == min(1, l.steps - 1)) next = publish(it + 1);
-        }
-        if (l.steps == 0) next = publish(it + 1);
-        more = next;
+      TrItem l = {};
+      int pages = 0, ids = 0, ids_later = 0;
+#pragma unroll 1
+      for (int it = -1;; ++it) {                         // (-1: nothing yet but the first item)
+        bool more = false;
+        int s = 0;
+#pragma unroll 1
+        do {
+          if (s < l.steps) {
+            if (s > 0 && s % 8 == 0) ids = ids_later;
+            const int b = gs % kTrRaw;
+            if (ok && gs >= kTrRaw) ok = mbar_wait_park(smem_u32(&sm.raw_free[b]), (gs / kTrRaw - 1) & 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const int n = min(kTrPages, pages - (l.lo + s) * kTrPages);
+            if (lane == 0) mbar_expect_tx(smem_u32(&sm.raw_full[b]), n * lay.blob_bytes);
+            __syncwarp();
+            const int page = __shfl_sync(0xffffffffu, ids, (s % 8) * kTrPages + (lane & 3));
+            if (lane < n)
+              bulk_g2s(smem_u32(raw + (b * kTrPages + lane) * stride), p.cache + (static_cast<size_t>(page) * p.Hkv + l.kvh) * lay.blob_bytes, lay.blob_bytes, smem_u32(&sm.raw_full[b]));
+            if (s % 8 == 0 && s + 8 < l.steps) ids_later = ids_of(l, s + 8);
+            ++gs;
+          }
+          if (s == max(0, min(1, l.steps - 1))) more = publish(it + 1);
+        } while (++s < l.steps);
+        if (!more || !ok) break;
+        l = sm.list[(it + 1) % kTrLists];
+        pages = (l.total + kPageTokens - 1) / kPageTokens;
+        ids = ids_next;
       }
       if (lane == 0) desc[blockIdx.x] = d;
       if (*abort_flag) {                                 // copies in flight land (for a bounded time) before the CTA goes
@@ -461,16 +488,19 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
         if (ok) ok = mbar_wait_park(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok || l.kvh < 0) break;
-        const int steps = l.steps, tiles = l.rows > kTrRows ? 2 : 1;
+        const int steps = l.steps;
+        const bool split = tr_split(l);
+#pragma unroll 1
         for (int s = 0; s < steps; ++s, ++gs) {
-          const int b = gs & 1;
-          if (ok) ok = mbar_wait_park(smem_u32(is_s ? &sm.k_full[b] : &sm.v_full[b]), (gs >> 1) & 1, abort_flag);
+          const int b = gs % kTrOps;
+          if (ok) ok = mbar_wait_park(smem_u32(is_s ? &sm.k_full[b] : &sm.v_full[b]), (gs / kTrOps) & 1, abort_flag);
 #pragma unroll
           for (int t = 0; t < kTrTiles; ++t) {
-            if (t >= tiles) continue;
+            if (split && (s & 1) != t) continue;
+            const bool first = s == (split ? t : 0);
             const uint32_t tile = tmem + t * kTrTmemTile;
             if (is_s) {
-              if (s == 0) {
+              if (first) {
                 if (ok) ok = mbar_wait_park(smem_u32(&sm.q_full[t]), q_phase >> t & 1, abort_flag);
                 q_phase ^= 1u << t;
               }
@@ -492,7 +522,7 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
               } else {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  umma_f16_ts(tile + kTrTmemO, tile + kTrTmemP + k * 8, dv + (b * (2 * kTrHalf) >> 4) + k * (16 * 128 >> 4), idesc_o, s > 0 || k > 0);
+                  umma_f16_ts(tile + kTrTmemO, tile + kTrTmemP + k * 8, dv + (b * (2 * kTrHalf) >> 4) + k * (16 * 128 >> 4), idesc_o, !first || k > 0);
                 tc_commit(smem_u32(&sm.pv_done[t]));
               }
             }
@@ -518,10 +548,10 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
       const int steps = l.steps;
       int v_exp = 0;
       uint32_t v_most = 0, v_least = 0x7F800000u;        // of the item's steps
+#pragma unroll 1
       for (int s = 0; s < steps; ++s, ++gs) {
-        const int b = gs & 1, slot = gs % kTrRaw, note = gs % kTrNotes, visible = l.total - (l.lo + s) * kTrTok;
+        const int b = gs % kTrOps, slot = gs % kTrRaw, note = gs % kTrNotes, visible = l.total - (l.lo + s) * kTrTok;
         if (ok) ok = mbar_wait_park(smem_u32(&sm.raw_full[slot]), (gs / kTrRaw) & 1, abort_flag);
-        if (ok && gs >= 2) ok = mbar_wait_park(smem_u32(is_v ? &sm.v_free[b] : &sm.k_free[b]), ((gs >> 1) - 1) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint8_t* pages = raw + slot * kTrPages * stride;
@@ -533,16 +563,14 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
         const int e = pf_exponent(most);
         uint32_t least = 0x7F800000u;
         if ((warp & 3) == 0) least = __reduce_min_sync(0xffffffffu, min(tr_least(scale[0]), tr_least(scale[1])));
+        // K: codes times scales below 2^13; V: below 2^11, to be changed when they pass 2^15.  Noted before there is room for the operands: softmax waits for it
         if (!is_v) {
-          // codes times scales below 2^13
           if (warp == 8 && lane == 0) {
             if (odd || (least < 0x7F800000u && pf_exponent(least) < e - kTrApartK)) sm.redo[it % kTrLists] = 1;
             sm.k_mul[note] = pow2f(e - 5);
             mbar_arrive(smem_u32(&sm.k_note[note]));
           }
-          tr_convert_k<KBITS>(sm.k[b], pages, stride, lay, pow2f(5 - e), ct);
         } else {
-          // below 2^11, to be changed when they pass 2^15
           if (s == 0 || e - 7 > v_exp) v_exp = e - 3;
           if (warp == 12 && lane == 0) {
             v_most = max(v_most, most);
@@ -551,8 +579,12 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
             sm.v_exp[note] = v_exp;
             mbar_arrive(smem_u32(&sm.v_note[note]));
           }
-          tr_convert_v<VBITS>(sm.v[b], pages, stride, lay, visible, pow2f(-v_exp), ct);
         }
+        if (gs >= kTrOps) ok = mbar_wait_park(smem_u32(is_v ? &sm.v_free[b] : &sm.k_free[b]), (gs / kTrOps - 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (!is_v) tr_convert_k<KBITS>(sm.k[b], pages, stride, lay, pow2f(5 - e), ct);
+        else tr_convert_v<VBITS>(sm.v[b], pages, stride, lay, visible, pow2f(-v_exp), ct);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -582,20 +614,21 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
       r.sees = p.masks;
       r.mul = 0.f;
       if (!ok || l.kvh < 0) return false;
-      const int at = t * kTrRows + row;
+      const int at = tr_split(l) ? row : t * kTrRows + row;
       if (at < l.rows) {
         const int node = (l.first + at) / G, col = (l.kvh * G + (l.first + at - node * G)) * kD;
         r.q = (l.row0 + node) * p.ldq + col;
         r.out = (l.row0 + node) * p.ldo + col;
         r.sees = p.masks + (l.row0 + node) * p.ldm;
       }
-      if (l.steps > 0 && t * kTrRows < l.rows) {
+      if (tr_takes_part(l, t)) {
         // a power of two brings the row's largest magnitude to 2^10 .. 2^11; what is not finite stays
+        const uint4* q = reinterpret_cast<const uint4*>(p.q + r.q);
         uint32_t most = 0;
         if (r.q >= 0) {
-#pragma unroll
+#pragma unroll 4
           for (int c = 0; c < 16; ++c) {
-            const uint4 u = reinterpret_cast<const uint4*>(p.q + r.q)[c];
+            const uint4 u = q[c];
             const uint32_t in[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) most = max(most, max(in[j] & 0x7FFFu, in[j] >> 16 & 0x7FFFu));
@@ -604,27 +637,19 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
         const int e = most >= 0x7F80u || most == 0u ? 0 : max(static_cast<int>(most >> 7) - 127 - 10, -126);
         const float down = pow2f(-e);
         r.mul = pow2f(e) * p.scale * 1.4426950408889634f;
-        uint32_t x[32];
+#pragma unroll 2
+        for (int c = 0; c < 16; ++c) {                   // eight channels
+          uint4 u = make_uint4(0u, 0u, 0u, 0u);
+          if (r.q >= 0) u = q[c];
+          const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+          uint32_t x[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint4 u = make_uint4(0u, 0u, 0u, 0u);
-            if (r.q >= 0) u = reinterpret_cast<const uint4*>(p.q + r.q)[h * 8 + c];
-            const uint32_t in[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&in[j]));
-              x[c * 4 + j] = pack_f16x2(f.x * down, f.y * down);
-            }
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&in[j]));
+            x[j] = pack_f16x2(f.x * down, f.y * down);
           }
-          if (h == 0) {
-            tmem_st_32x32(tile + kTrTmemQ, x);
-          } else {
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              *reinterpret_cast<uint4*>(sm.q[t] + row * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
-          }
+          if (c < 8) tr_tmem_st4(tile + kTrTmemQ + c * 4, x);
+          else *reinterpret_cast<uint4*>(sm.q[t] + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
         }
         tmem_st_wait();
         fence_proxy_async_smem();
@@ -634,45 +659,59 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
       }
       return true;
     };
-    int gs = 0, n = 0;                                   // steps of earlier items; steps that this tile took part in
-    Row cur;
-    bool more = begin(0, cur);
-    for (int it = 0; more; ++it) {
-      const TrItem& l = sm.list[it % kTrLists];
-      const int steps = l.steps, start = l.start, total = l.total;
-      const bool in = t * kTrRows < l.rows, mine = cur.q >= 0;
+    int gs0 = 0, n = 0, exchanges = 0;                   // steps of earlier items; steps that this tile took part in; items in both tiles
+    bool lent = false;                                   // the other tile may still read this one's output
+    auto wait_lent = [&]() {
+      if (lent && ok) ok = mbar_wait_park(smem_u32(&sm.exch_free), (exchanges - 1) & 1, abort_flag);
+      lent = false;
+    };
+    Row cur = {-1, -1, p.masks, 0.f};
+    bool more = true;
+#pragma unroll 1
+    for (int it = -1; more; ++it) {                      // (-1: nothing yet but the first item's Q)
+      const TrItem& l = sm.list[max(it, 0) % kTrLists];
+      const int steps = it < 0 ? 0 : l.steps, start = l.start, total = l.total;
+      const bool split = it >= 0 && tr_split(l), in = it >= 0 && tr_takes_part(l, t), mine = cur.q >= 0;
       float m = -INFINITY, sum = 0.f;
       int v_exp = 0;
-      if (!in) {
-        gs += steps;
-      } else {
-        for (int s = 0; s < steps; ++s, ++gs) {
-          const int note = gs % kTrNotes, tok0 = (l.lo + s) * kTrTok;
+      {
+        const int first = split ? t : 0;
+#pragma unroll 1
+        for (int s = first; s < steps; s += split ? 2 : 1) {
+          const int gs = gs0 + s, note = gs % kTrNotes, tok0 = (l.lo + s) * kTrTok;
           if (ok) ok = mbar_wait_park(smem_u32(&sm.s_full[t]), n & 1, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
-          uint32_t a[2][32];
-          tmem_ld_32x32(tile, a[0]);
-          tmem_ld_32x32(tile + 32, a[1]);
-          tmem_ld_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sm.s_free[t]));
+          if (tok0 + kTrTok > start) {                   // what a row does not see: -inf in place of its scores
+            const uint2 see = mine ? tr_visible(cur.sees, p.words, start, total, tok0) : make_uint2(0u, 0u);
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+              uint32_t a[32];
+              tmem_ld_32x32(tile + c * 32, a);
+              tmem_ld_wait();
+              const uint32_t bits = c == 0 ? see.x : see.y;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!(bits >> j & 1u)) a[j] = 0xFF800000u;
+              tmem_st_32x32(tile + c * 32, a);
+            }
+            tmem_st_wait();
+          }
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t a[32];
+            tmem_ld_32x32(tile + c * 32, a);
+            tmem_ld_wait();
+            float of[4] = {-INFINITY, -INFINITY, -INFINITY, mx};
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) of[j / 2 & 3] = fmaxf(of[j / 2 & 3], fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
+            mx = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
+          }
           // (a note is written again after this step's product, which waits for what follows: kTrNotes)
           if (ok) ok = mbar_wait_park(smem_u32(&sm.k_note[note]), (gs / kTrNotes) & 1, abort_flag);
           if (ok) ok = mbar_wait_park(smem_u32(&sm.v_note[note]), (gs / kTrNotes) & 1, abort_flag);
-          if (tok0 + kTrTok > start) {
-            const uint2 see = mine ? tr_visible(cur.sees, p.words, start, total, tok0) : make_uint2(0u, 0u);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              if (!(see.x >> j & 1u)) a[0][j] = 0xFF800000u;                            // -inf
-              if (!(see.y >> j & 1u)) a[1][j] = 0xFF800000u;
-            }
-          }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int j = 0; j < kTrTok; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(a[j >> 5][j & 31]));
-          const float mul = sm.k_mul[note] * cur.mul, top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+          const float mul = sm.k_mul[note] * cur.mul, top = mx * mul;
           float alpha = 1.f;
           bool grew = top > m + kTrGrowth || (m == -INFINITY && top > m);
           if (grew) {
@@ -688,22 +727,31 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
           }
           const float use = m == -INFINITY ? 0.f : m;
           const float2 less = make_float2(-use, -use), mul2 = make_float2(mul, mul);
-          float2 part_sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          uint32_t pr[32];
-#pragma unroll
-          for (int j = 0; j < kTrTok / 2; ++j) {
-            const float2 d = __ffma2_rn(make_float2(__uint_as_float(a[j >> 4][2 * j & 31]), __uint_as_float(a[j >> 4][(2 * j + 1) & 31])), mul2, less);
-            const float2 x = make_float2(fast_exp2(d.x), fast_exp2(d.y));
-            part_sum[j & 1] = __fadd2_rn(part_sum[j & 1], x);
-            pr[j] = pack_f16x2(x.x, x.y);
-          }
-          sum += (part_sum[0].x + part_sum[0].y) + (part_sum[1].x + part_sum[1].y);
           // the previous product has read the probabilities and written the output
-          if (ok && s > 0) ok = mbar_wait_park(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
+          if (ok && s > first) ok = mbar_wait_park(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
+          if (s == first) wait_lent();
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
-          tmem_st_32x32(tile + kTrTmemP, pr);
-          if (s > 0 && __any_sync(0xffffffffu, grew)) {
+          float2 part_sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t a[32], pr[16];
+            tmem_ld_32x32(tile + c * 32, a);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 d = __ffma2_rn(make_float2(__uint_as_float(a[2 * j]), __uint_as_float(a[2 * j + 1])), mul2, less);
+              const float2 x = make_float2(fast_exp2(d.x), fast_exp2(d.y));
+              part_sum[j & 1] = __fadd2_rn(part_sum[j & 1], x);
+              pr[j] = pack_f16x2(x.x, x.y);
+            }
+            tr_tmem_st16(tile + kTrTmemP + c * 16, pr);
+          }
+          sum += (part_sum[0].x + part_sum[0].y) + (part_sum[1].x + part_sum[1].y);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sm.s_free[t]));
+          if (s > first && __any_sync(0xffffffffu, grew)) {
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               uint32_t o[32];
@@ -721,72 +769,99 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
           ++n;
         }
       }
+      gs0 += steps;
       // the next item's Q while the last product runs (all of this item's scores are there)
       Row next;
       more = begin(it + 1, next);
-      if (in) {
-        const int part = l.part;
-        const size_t at = (static_cast<size_t>(max(part, 0)) * part_rows + t * kTrRows + row);
-        if (steps == 0) {                                // a request that is told wrongly
-          if (mine) {
+      const int part = it < 0 ? -1 : l.part;
+      const size_t at = static_cast<size_t>(max(part, 0)) * part_rows + (split ? row : t * kTrRows + row);
+      if (steps == 0) {                                  // a request that is told wrongly
+        if (mine) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) reinterpret_cast<uint4*>(p.out + cur.out)[j] = make_uint4(0u, 0u, 0u, 0u);
-          }
-        } else {
-          if (ok) ok = mbar_wait_park(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
+          for (int j = 0; j < 16; ++j) reinterpret_cast<uint4*>(p.out + cur.out)[j] = make_uint4(0u, 0u, 0u, 0u);
+        }
+      } else {
+        if (ok && in) ok = mbar_wait_park(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        // what this tile's output and the other's are multiplied with
+        float mul[2] = {pow2f(v_exp), 0.f};
+        const bool other = split && steps > 1 - t;       // the other tile has an output
+        if (split) {
+          wait_lent();
+          sm.exch_ml[t][row] = make_float2(m, sum);
+          sm.exch_exp[t][row] = v_exp;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sm.exch_full));
+          if (ok) ok = mbar_wait_park(smem_u32(&sm.exch_full), exchanges & 1, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
-          tc_fence_after();
-          const float up = pow2f(v_exp), inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;           // NaN stays
+          ++exchanges;
+          lent = true;
+          const float2 o = sm.exch_ml[1 - t][row];
+          const float top = fmaxf(m, o.x), use = top == -INFINITY ? 0.f : top, f0 = fast_exp2(m - use), f1 = fast_exp2(o.x - use);
+          mul[0] *= f0;
+          mul[1] = f1 * pow2f(sm.exch_exp[1 - t][row]);
+          sum = f0 * sum + f1 * o.y;
+          m = top;
+        }
+        tc_fence_after();
+        if (!*const_cast<volatile uint32_t*>(&sm.redo[it % kTrLists])) {
+          const float inv = part >= 0 ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;            // NaN stays
+          const int c0 = split ? 4 * t : 0, c1 = split ? 4 * t + 4 : 8;                                  // of 16 channels
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32(tile + kTrTmemO + c * 32, o);
+          for (int c = c0; c < c1; ++c) {
+            uint32_t a[16], b[16];
+            const uint32_t from = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kTrTmemO + c * 16;
+            if (in) tmem_ld_32x16(from + t * kTrTmemTile, a);
+            if (other) tmem_ld_32x16(from + (1 - t) * kTrTmemTile, b);
             tmem_ld_wait();
-            if (mine) {
-              if (part >= 0) {
+            float o[16];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  reinterpret_cast<float4*>(part_o + at * kD + c * 32)[j] =
-                      make_float4(__uint_as_float(o[4 * j]) * up, __uint_as_float(o[4 * j + 1]) * up, __uint_as_float(o[4 * j + 2]) * up, __uint_as_float(o[4 * j + 3]) * up);
-              } else {
+            for (int j = 0; j < 16; ++j) {
+              o[j] = in ? __uint_as_float(a[j]) * mul[0] : 0.f;
+              if (other) o[j] = fmaf(__uint_as_float(b[j]), mul[1], o[j]);
+              o[j] *= inv;
+            }
+            if (mine && part >= 0) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  uint32_t x[4];
+              for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(part_o + at * kD + c * 16)[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            } else if (mine) {
 #pragma unroll
-                  for (int k = 0; k < 4; ++k) x[k] = pack_bf16x2(__uint_as_float(o[8 * j + 2 * k]) * inv * up, __uint_as_float(o[8 * j + 2 * k + 1]) * inv * up);
-                  *reinterpret_cast<uint4*>(p.out + cur.out + c * 32 + j * 8) = make_uint4(x[0], x[1], x[2], x[3]);
-                }
-              }
+              for (int j = 0; j < 2; ++j)
+                reinterpret_cast<uint4*>(p.out + cur.out + c * 16)[j] = make_uint4(pack_bf16x2(o[8 * j], o[8 * j + 1]), pack_bf16x2(o[8 * j + 2], o[8 * j + 3]),
+                                                                                  pack_bf16x2(o[8 * j + 4], o[8 * j + 5]), pack_bf16x2(o[8 * j + 6], o[8 * j + 7]));
             }
           }
-          tc_fence_before();
-          if (part >= 0 && mine) part_ml[at] = make_float2(m, sum);
-          if (*const_cast<volatile uint32_t*>(&sm.redo[it % kTrLists]) && ok) {
-            __syncwarp();                                // a row's result is written again by other lanes
-            TreeRequest r;
-            r.slot = l.slot; r.row0 = l.row0; r.count = l.count; r.start = start; r.total = total;
-            const int lo = l.lo * kTrTok, hi = min(total, (l.lo + steps) * kTrTok);
+          if (part >= 0 && mine && c0 == 0) part_ml[at] = make_float2(m, sum);
+        } else if (ok) {
+          TreeRequest r;
+          r.slot = l.slot; r.row0 = l.row0; r.count = l.count; r.start = start; r.total = total;
+          const int lo = l.lo * kTrTok, hi = min(total, (l.lo + steps) * kTrTok);
 #pragma unroll 1
-            for (uint32_t rows = __ballot_sync(0xffffffffu, mine); rows; rows &= rows - 1) {
-              const int of = __ffs(rows) - 1;
-              const long long q = __shfl_sync(0xffffffffu, cur.q, of), out = __shfl_sync(0xffffffffu, cur.out, of);
-              const uint32_t* sees = reinterpret_cast<const uint32_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(cur.sees), of));
-              float rm, rs, o[4];
-              tree_row<KBITS, VBITS>(p, lay, r, l.kvh, lo, hi, sees, p.q + q, lane, rm, rs, o, bad);
-              if (part >= 0) {
-                const size_t to = at - lane + of;
-                reinterpret_cast<float4*>(part_o + to * kD)[lane] = make_float4(o[0], o[1], o[2], o[3]);
-                if (lane == 0) part_ml[to] = make_float2(rm, rs);
-              } else {
-                const float f = rs > 0.f ? 1.f / rs : rs == 0.f ? 0.f : rs;
-                reinterpret_cast<uint2*>(p.out + out)[lane] = make_uint2(pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f));
-              }
+          for (uint32_t rows = __ballot_sync(0xffffffffu, mine && (!split || (lane & 1) == t)); rows; rows &= rows - 1) {
+            const int of = __ffs(rows) - 1;
+            const long long q = __shfl_sync(0xffffffffu, cur.q, of), out = __shfl_sync(0xffffffffu, cur.out, of);
+            const uint32_t* sees = reinterpret_cast<const uint32_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(cur.sees), of));
+            float rm, rs, o[4];
+            tree_row<KBITS, VBITS>(p, lay, r, l.kvh, lo, hi, sees, p.q + q, lane, rm, rs, o, bad);
+            if (part >= 0) {
+              const size_t to = at - lane + of;
+              reinterpret_cast<float4*>(part_o + to * kD)[lane] = make_float4(o[0], o[1], o[2], o[3]);
+              if (lane == 0) part_ml[to] = make_float2(rm, rs);
+            } else {
+              const float f = rs > 0.f ? 1.f / rs : rs == 0.f ? 0.f : rs;
+              reinterpret_cast<uint2*>(p.out + out)[lane] = make_uint2(pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f));
             }
           }
         }
+        tc_fence_before();
+        if (split) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sm.exch_free));
+        }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sm.list_free[it % kTrLists]));
+      if (lane == 0 && it >= 0) mbar_arrive(smem_u32(&sm.list_free[it % kTrLists]));
       cur = next;
     }
   }
