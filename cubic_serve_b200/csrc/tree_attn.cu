@@ -56,10 +56,18 @@ __device__ __forceinline__ int tree_page(const CbTreeAttn& p, int slot, int i, b
   return there ? page : 0;
 }
 
+// The page layout as constants (kv_layout.cuh)
+template <int KBITS, int VBITS>
+struct TreeLay {
+  static constexpr int kScale = kPageTokens * kD * KBITS / 8, kBytesOfScales = kPageTokens * (kD / kKvGroup) * 4, vCode = kScale + kBytesOfScales,
+                       vScale = vCode + kPageTokens * kD * VBITS / 8, bytes = vScale + kBytesOfScales, stride = (bytes + 127) & ~127;
+};
+
 // One row over the tokens [lo, hi) in fp32, by a warp whose lanes have four channels each.  `sees`: the row's words.
 template <int KBITS, int VBITS>
-__device__ __forceinline__ void tree_row(const CbTreeAttn& p, const KvLayout& lay, const TreeRequest& r, int kvh, int lo, int hi, const uint32_t* sees, const __nv_bfloat16* q,
+__device__ __forceinline__ void tree_row(const CbTreeAttn& p, const TreeRequest& r, int kvh, int lo, int hi, const uint32_t* sees, const __nv_bfloat16* q,
                                          int lane, float& m, float& sum, float (&o)[4], bool& bad) {
+  using L = TreeLay<KBITS, VBITS>;
   constexpr float kBias = 1 << (KBITS - 1), vBias = 1 << (VBITS - 1);
   const uint2 qw = reinterpret_cast<const uint2*>(q)[lane];
   const float2 q01 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qw.x)), q23 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qw.y));
@@ -73,10 +81,10 @@ __device__ __forceinline__ void tree_row(const CbTreeAttn& p, const KvLayout& la
     const int j = t - r.start;
     if (j >= 0 && !(sees[j >> 5] >> (j & 31) & 1u)) continue;
     const int page = tree_page(p, r.slot, t / kPageTokens, bad), tok = t % kPageTokens;
-    const uint8_t* blob = p.cache + (static_cast<size_t>(page) * p.Hkv + kvh) * lay.blob_bytes;
-    const uint32_t kc = pf_codes_k<KBITS>(blob, tok, lane), vc = pf_codes_v<VBITS>(blob + lay.v_code_off, tok, lane);
-    const float ks = *reinterpret_cast<const float*>(blob + lay.k_scale_off + tok * 16 + (lane >> 3) * 4);
-    const float vs = *reinterpret_cast<const float*>(blob + lay.v_scale_off + tok * 16 + (lane >> 3) * 4);
+    const uint8_t* blob = p.cache + (static_cast<size_t>(page) * p.Hkv + kvh) * L::bytes;
+    const uint32_t kc = pf_codes_k<KBITS>(blob, tok, lane), vc = pf_codes_v<VBITS>(blob + L::vCode, tok, lane);
+    const float ks = *reinterpret_cast<const float*>(blob + L::kScale + tok * 16 + (lane >> 3) * 4);
+    const float vs = *reinterpret_cast<const float*>(blob + L::vScale + tok * 16 + (lane >> 3) * 4);
     float z = 0.f;
 #pragma unroll
     for (int c = 0; c < 4; ++c) z = fmaf(qf[c], (static_cast<float>(kc >> (8 * c) & 255u) - kBias) * ks, z);
@@ -107,7 +115,7 @@ static_assert(2 * kTrRegsSoftmax + 2 * kTrRegsConvert + kTrRegsOther <= 5 * kTrR
 static constexpr int kTrLists = 4, kTrRaw = 4;
 static constexpr int kTrOps = 3;                         // steps of operands
 // Steps whose powers of two are kept: the note of step s is written behind raw_full (s) <- raw_free (s - kTrRaw) <- v_free of step s - kTrRaw - kTrOps <- p_full of the
-// tiles that take part in it, which have read their notes by then.
+// tiles that take part in it, which have read theirs by then.
 static constexpr int kTrNotes = kTrRaw + kTrOps;
 static constexpr int kTrLeast = 1;                       // steps of a CTA, at least
 static constexpr float kTrGrowth = 2.f;
@@ -115,6 +123,15 @@ static constexpr int kTrApartK = 18, kTrApartV = 14;
 static constexpr int kTrHalf = kTrTok * 128;             // bytes of 64 channels of a step
 static constexpr uint32_t kTrTmemCols = 512, kTrTmemTile = 256, kTrTmemP = 64, kTrTmemQ = 96, kTrTmemO = 128;
 
+// Where a role stands in a ring of n places, and the parity that it waits for there
+struct TrRing {
+  int i, n;
+  uint32_t phase;
+  __device__ __forceinline__ explicit TrRing(int places, uint32_t parity = 0) : i(0), n(places), phase(parity) {}
+  __device__ __forceinline__ void advance() {
+    if (++i == n) { i = 0; phase ^= 1u; }
+  }
+};
 struct TrItem {
   int kvh;                                               // < 0: no more items
   int slot, row0, count, start, total;                   // the request
@@ -127,10 +144,9 @@ struct __align__(1024) TrSmem {
   uint8_t q[kTrTiles][kTrRows * 128];                    // f16, channels 64..127: [row][128 B], 16-byte chunk ^ (row & 7)
   uint8_t k[kTrOps][2 * kTrHalf];                             // f16 [stage][64-channel half][token][128 B]
   uint8_t v[kTrOps][2 * kTrHalf];                             // likewise
-  float k_mul[kTrNotes];                                 // scores are this times what the MMAs give
-  int v_exp[kTrNotes];                                   // output is 2^v_exp times ...
+  float4 note[kTrNotes];                                 // of a step: what K and V are multiplied with, what scores are multiplied with, 2^this is V's unit
   uint32_t redo[kTrLists];                               // of an item's steps: some values are beyond what f16 operands hold
-  uint64_t raw_full[kTrRaw], raw_free[kTrRaw], k_full[kTrOps], k_free[kTrOps], v_full[kTrOps], v_free[kTrOps], k_note[kTrNotes], v_note[kTrNotes];
+  uint64_t raw_full[kTrRaw], raw_free[kTrRaw], k_full[kTrOps], k_free[kTrOps], v_full[kTrOps], v_free[kTrOps], note_full[kTrNotes];
   uint64_t list_full[kTrLists], list_free[kTrLists], q_full[kTrTiles], s_full[kTrTiles], s_free[kTrTiles], p_full[kTrTiles], pv_done[kTrTiles];
   uint64_t exch_full, exch_free;
   TrItem list[kTrLists];
@@ -160,32 +176,42 @@ __device__ __forceinline__ uint32_t tr_scaled(uint32_t code, uint32_t sh, uint32
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(code), "r"(sh), "r"(t));
   return r;
 }
+__device__ __forceinline__ void tr_put(uint32_t to, const uint4& x) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+}
 __device__ __forceinline__ uint4 tr_scaled8(const uint4& c, uint32_t sh, uint32_t sl) {
   return make_uint4(tr_scaled(c.x, sh, sl), tr_scaled(c.y, sh, sl), tr_scaled(c.z, sh, sl), tr_scaled(c.w, sh, sl));
 }
-// (The loops stay loops: four kinds of warps run their code at the same time, and unrolled it does not fit the instruction caches.)
-template <int KBITS>
-__device__ __forceinline__ void tr_convert_k(uint8_t (&k)[2 * kTrHalf], const uint8_t* raw, int stride, const KvLayout& lay, float mul, int tid) {
+// (The loops stay loops: five kinds of warps run their code at the same time, and unrolled it does not fit the instruction caches: 3700 cycles a step.)
+template <int KBITS, int VBITS>
+__device__ __forceinline__ void tr_convert_k(uint8_t* k, const uint8_t* raw, float mul, int tid) {
+  using L = TreeLay<KBITS, VBITS>;
   constexpr uint32_t kb = KBITS == 8 ? 0x64806480u : KBITS == 6 ? 0x64206420u : 0x64086408u;
   // an item is a scale's 32 channels of a token
   const int tok = tid & 15, g = tid >> 4 & 3, sw = tok & 7;
+  raw += (tid >> 6) * L::stride;
+  const uint8_t* codes = raw + tok * 16 + g * (KBITS == 8 ? 512 : 256);
+  const uint8_t* high = raw + kPageTokens * kD / 2 + g * 128 + (tok & 7) * 16;
+  const uint8_t* scale = raw + L::kScale + tok * 16 + g * 4;
+  // chunks 4 (g & 1) + {0, 1, 2, 3} of the token's row, each ^ (row & 7)
+  k += (g >> 1) * kTrHalf + ((tid >> 6) * 16 + tok) * 128 + (((g & 1) * 4 ^ (sw & 6)) << 4);
+  const int one = (sw & 1) << 4;
 #pragma unroll 1
-  for (int page = tid >> 6; page < kTrPages; page += 2) {
-    const uint8_t* src = raw + page * stride;
-    uint4* row = reinterpret_cast<uint4*>(k + (g >> 1) * kTrHalf + (page * 16 + tok) * 128);
+  for (int page = 0; page < kTrPages / 2; ++page) {
     uint32_t sh, sl;
-    pf_split(*reinterpret_cast<const float*>(src + lay.k_scale_off + tok * 16 + g * 4) * mul, sh, sl);
+    pf_split(*reinterpret_cast<const float*>(scale) * mul, sh, sl);
     uint4 x, w = make_uint4(0u, 0u, 0u, 0u);
-    if constexpr (KBITS != 8) x = *reinterpret_cast<const uint4*>(src + g * 256 + tok * 16);
+    if constexpr (KBITS != 8) x = *reinterpret_cast<const uint4*>(codes);
     if constexpr (KBITS == 6) {
-      w = *reinterpret_cast<const uint4*>(src + kPageTokens * kD / 2 + g * 128 + (tok & 7) * 16);
+      w = *reinterpret_cast<const uint4*>(high);
       if (tok >= 8) { w.x <<= 4; w.y <<= 4; w.z <<= 4; w.w <<= 4; }                      // (what leaves a byte's bits 4 to 7 is masked)
     }
+    uint32_t to = smem_u32(k);
 #pragma unroll 1
     for (int h = 0; h < 2; ++h) {                        // 16 channels
       uint4 n;
       if constexpr (KBITS == 8) {
-        n = *reinterpret_cast<const uint4*>(src + g * 512 + h * 256 + tok * 16);
+        n = *reinterpret_cast<const uint4*>(codes + h * 256);
       } else {
         n = make_uint4(x.x & 0x0F0F0F0Fu, x.y & 0x0F0F0F0Fu, x.z & 0x0F0F0F0Fu, x.w & 0x0F0F0F0Fu);
         x = make_uint4(x.x >> 4, x.y >> 4, x.z >> 4, x.w >> 4);
@@ -194,42 +220,50 @@ __device__ __forceinline__ void tr_convert_k(uint8_t (&k)[2 * kTrHalf], const ui
           w = make_uint4(w.x >> 2, w.y >> 2, w.z >> 2, w.w >> 2);
         }
       }
-      const int c = (g & 1) * 4 + h * 2;
-      row[c ^ sw] = tr_scaled8(conv8(make_uint2(n.x, n.y), kb), sh, sl);
-      row[(c + 1) ^ sw] = tr_scaled8(conv8(make_uint2(n.z, n.w), kb), sh, sl);
+      tr_put(to + one, tr_scaled8(conv8(make_uint2(n.x, n.y), kb), sh, sl));
+      tr_put(to + (one ^ 16), tr_scaled8(conv8(make_uint2(n.z, n.w), kb), sh, sl));
+      to ^= 32;
     }
+    codes += 2 * L::stride; high += 2 * L::stride; scale += 2 * L::stride;
+    k += 2 * 16 * 128;
   }
 }
 // V from `visible` on becomes zeros: those slots may hold anything, and a probability of zero has to stay zero.
-template <int VBITS>
-__device__ __forceinline__ void tr_convert_v(uint8_t (&v)[2 * kTrHalf], const uint8_t* raw, int stride, const KvLayout& lay, int visible, float mul, int tid) {
+template <int KBITS, int VBITS>
+__device__ __forceinline__ void tr_convert_v(uint8_t* v, const uint8_t* raw, int visible, float mul, int tid) {
+  using L = TreeLay<KBITS, VBITS>;
   constexpr uint32_t vb = VBITS == 8 ? 0x64806480u : VBITS == 6 ? 0x64206420u : 0x64086408u;
   // an item is 16 channels of a token pair, eight at a time: lanes 0-3 of eight take the first eight first, the others the second (no bank twice)
   const int c = tid & 7, pair = tid >> 3 & 7, first = tid >> 2 & 1;
   const int at = (4 * c) ^ ((pair & 3) << 2);
+  raw += (tid >> 6) * L::stride;
+  const uint8_t* codes = raw + L::vCode + (VBITS == 8 ? pair * 256 + at * 8 : pair * 128 + at * 4);
+  const uint8_t* high = raw + L::vCode + kPageTokens * kD / 2 + (pair & 3) * 128 + at * 4;
+  const uint8_t* scale = raw + L::vScale + pair * 32 + (c >> 1) * 4;
+  // chunk 2 c + half of rows 2 pair and 2 pair + 1, each ^ (row & 7)
+  v += (c >> 2) * kTrHalf + ((tid >> 6) * 16 + pair * 2) * 128 + ((((2 * c) & 7) ^ ((pair & 3) * 2)) << 4);
+  int tok = (tid >> 6) * 16 + pair * 2;
 #pragma unroll 1
-  for (int page = tid >> 6; page < kTrPages; page += 2) {
-    const uint8_t* src = raw + page * stride;
-    const uint8_t* codes = src + lay.v_code_off;
-    const int tok = page * 16 + pair * 2;
+  for (int page = 0; page < kTrPages / 2; ++page, tok += 32) {
     uint32_t sh[2], sl[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float f = *reinterpret_cast<const float*>(src + lay.v_scale_off + (2 * pair + h) * 16 + (c >> 1) * 4) * mul;
+      float f = *reinterpret_cast<const float*>(scale + h * 16) * mul;
       if (tok + h >= visible || !(fabsf(f) < INFINITY)) f = 0.f;
       pf_split(f, sh[h], sl[h]);
     }
+    const uint32_t to = smem_u32(v);
 #pragma unroll 1
     for (int e = 0; e < 2; ++e) {
       const int half = first ^ e;
       uint4 x;
       if constexpr (VBITS == 8) {
-        x = *reinterpret_cast<const uint4*>(codes + pair * 256 + (at + 2 * half) * 8);
+        x = *reinterpret_cast<const uint4*>(codes + half * 16);
       } else {
-        const uint2 n = *reinterpret_cast<const uint2*>(codes + pair * 128 + (at + 2 * half) * 4);
+        const uint2 n = *reinterpret_cast<const uint2*>(codes + half * 8);
         uint2 hw = make_uint2(0u, 0u);
         if constexpr (VBITS == 6) {
-          hw = *reinterpret_cast<const uint2*>(codes + kPageTokens * kD / 2 + (pair & 3) * 128 + (at + 2 * half) * 4);
+          hw = *reinterpret_cast<const uint2*>(high + half * 8);
           const int up = pair < 4 ? 0 : 4;
           hw.x <<= up; hw.y <<= up;
         }
@@ -249,10 +283,11 @@ __device__ __forceinline__ void tr_convert_v(uint8_t (&v)[2 * kTrHalf], const ui
           }
           f = conv8(n, vb);
         }
-        const int chunk = 2 * c + half;
-        *reinterpret_cast<uint4*>(v + (chunk >> 3) * kTrHalf + (tok + h) * 128 + (((chunk & 7) ^ ((tok + h) & 7)) << 4)) = tr_scaled8(f, sh[h], sl[h]);
+        tr_put(to + h * 128 + ((half ^ h) << 4), tr_scaled8(f, sh[h], sl[h]));
       }
     }
+    codes += 2 * L::stride; high += 2 * L::stride; scale += 2 * L::stride;
+    v += 2 * 16 * 128;
   }
 }
 // The smallest magnitude of a token's scales that is not zero, as bits
@@ -290,7 +325,8 @@ __device__ __forceinline__ uint2 tr_visible(const uint32_t* sees, int words, int
 }
 
 // Roles: warps 0-7 own a row a thread (softmax needs no exchange: tensor-memory lane = row); warps 8-11 convert raw pages of K to the swizzled operand
-// ([token][channel], f16), warps 12-15 those of V; warps 16 and 18 issue the MMAs of the scores and of the output; warp 17 makes the items and copies pages.
+// ([token][channel], f16), warps 12-15 those of V; warps 16 and 18 issue the MMAs of the scores and of the output; warp 17 makes the items and copies pages;
+// warp 19 finds the powers of two that bring a step's values into f16's range.
 // Tensor memory of a tile of 128 rows: scores, probabilities (the A operand of their product), output and the first half of Q's channels; the other half of
 // Q is in shared memory.  The scores of step i + 1 are computed while the softmax of step i runs.  The output is rescaled only when a row's maximum has grown by more
 // than a factor of four: until then probabilities relative to the older maximum are at most 4.
@@ -300,12 +336,12 @@ __device__ __forceinline__ uint2 tr_visible(const uint32_t* sees, int words, int
 // Every wait is bounded; on a timeout the roles leave, the status word is set and tensor memory is freed.
 template <int KBITS, int VBITS>
 __global__ void __launch_bounds__(kTrThreads, 1)
-tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
+tree_kernel(const CbTreeAttn p, const int part_rows) {
+  using L = TreeLay<KBITS, VBITS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   TrSmem& sm = *reinterpret_cast<TrSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* raw = reinterpret_cast<uint8_t*>(&sm + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv;
-  const int stride = (lay.blob_bytes + 127) & ~127;
   volatile uint32_t* abort_flag = &sm.abort_word;
   float* part_o = p.partial;
   float2* part_ml = reinterpret_cast<float2*>(part_o + static_cast<size_t>(gridDim.x) * 2 * part_rows * kD);
@@ -322,12 +358,11 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
       mbar_init(smem_u32(&sm.v_free[b]), 1);
     }
     for (int b = 0; b < kTrNotes; ++b) {
-      mbar_init(smem_u32(&sm.k_note[b]), 1);
-      mbar_init(smem_u32(&sm.v_note[b]), 1);
+      mbar_init(smem_u32(&sm.note_full[b]), 1);
     }
     for (int b = 0; b < kTrLists; ++b) {
       mbar_init(smem_u32(&sm.list_full[b]), 1);
-      mbar_init(smem_u32(&sm.list_free[b]), 18);         // all warps but 17 and 19
+      mbar_init(smem_u32(&sm.list_free[b]), 19);         // all warps but 17
     }
     for (int t = 0; t < kTrTiles; ++t) {
       mbar_init(smem_u32(&sm.q_full[t]), 4);
@@ -453,11 +488,11 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int n = min(kTrPages, pages - (l.lo + s) * kTrPages);
-            if (lane == 0) mbar_expect_tx(smem_u32(&sm.raw_full[b]), n * lay.blob_bytes);
+            if (lane == 0) mbar_expect_tx(smem_u32(&sm.raw_full[b]), n * L::bytes);
             __syncwarp();
             const int page = __shfl_sync(0xffffffffu, ids, (s % 8) * kTrPages + (lane & 3));
             if (lane < n)
-              bulk_g2s(smem_u32(raw + (b * kTrPages + lane) * stride), p.cache + (static_cast<size_t>(page) * p.Hkv + l.kvh) * lay.blob_bytes, lay.blob_bytes, smem_u32(&sm.raw_full[b]));
+              bulk_g2s(smem_u32(raw + (b * kTrPages + lane) * L::stride), p.cache + (static_cast<size_t>(page) * p.Hkv + l.kvh) * L::bytes, L::bytes, smem_u32(&sm.raw_full[b]));
             if (s % 8 == 0 && s + 8 < l.steps) ids_later = ids_of(l, s + 8);
             ++gs;
           }
@@ -475,13 +510,62 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
           while (!mbar_try_wait(smem_u32(&sm.raw_full[g % kTrRaw]), (g / kTrRaw) & 1) && clock64() - t0 < kWaitBudgetCycles / 8) {
           }
       }
-    } else if (warp != 19) {
+    } else if (warp == 19) {
+      // ------------------------------------------------------ powers of two
+      TrRing raw_at(kTrRaw), note_at(kTrNotes);
+#pragma unroll 1
+      for (int it = 0;; ++it) {
+        const TrItem& l = sm.list[it % kTrLists];
+        if (ok) ok = mbar_wait_park(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok || l.kvh < 0) break;
+        const int steps = l.steps;
+        int v_exp = 0, visible = l.total - l.lo * kTrTok;
+        uint32_t v_most = 0, v_least = 0x7F800000u;      // of the item's steps
+#pragma unroll 1
+        for (int s = 0; s < steps; ++s, visible -= kTrTok) {
+          if (ok) ok = mbar_wait_park(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint8_t* pages = raw + raw_at.i * kTrPages * L::stride;
+          uint32_t most[2], least[2];
+          bool odd = false;                              // some are not finite
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            float4 scale[2];
+            pf_scales(pages + (w == 0 ? L::kScale : L::vScale), L::stride, visible, lane, scale);
+            most[w] = __reduce_max_sync(0xffffffffu, max(pf_most<false>(scale[0]), pf_most<false>(scale[1])));
+            if (most[w] >= 0x7F800000u) {
+              odd = true;
+              most[w] = __reduce_max_sync(0xffffffffu, max(pf_most<true>(scale[0]), pf_most<true>(scale[1])));
+            }
+            least[w] = __reduce_min_sync(0xffffffffu, min(tr_least(scale[0]), tr_least(scale[1])));
+          }
+          // K: codes times scales below 2^13; V: below 2^11, to be changed when they pass 2^15
+          const int ek = pf_exponent(most[0]), ev = pf_exponent(most[1]);
+          if (s == 0 || ev - 7 > v_exp) v_exp = ev - 3;
+          v_most = max(v_most, most[1]);
+          v_least = min(v_least, least[1]);
+          if (lane == 0) {
+            if (odd || (least[0] < 0x7F800000u && pf_exponent(least[0]) < ek - kTrApartK) || (v_least < 0x7F800000u && pf_exponent(v_least) < pf_exponent(v_most) - kTrApartV))
+              sm.redo[it % kTrLists] = 1;
+            sm.note[note_at.i] = make_float4(pow2f(5 - ek), pow2f(-v_exp), pow2f(ek - 5), __int_as_float(v_exp));
+            mbar_arrive(smem_u32(&sm.note_full[note_at.i]));
+          }
+          __syncwarp();
+          raw_at.advance();
+          note_at.advance();
+        }
+        if (lane == 0) mbar_arrive(smem_u32(&sm.list_free[it % kTrLists]));
+      }
+    } else {
       // ---------------------------------------------------------------- MMAs
       const bool leader = elect_one(), is_s = warp == 16;
       const uint32_t idesc_s = umma_idesc(kTrRows, kTrTok, 0u, 0u), idesc_o = umma_idesc(kTrRows, kD, 0u, 0u) | 1u << 16;      // V: channels are contiguous
       const uint64_t dq = umma_desc_sw128(smem_u32(sm.q[0])), dk = umma_desc_sw128(smem_u32(sm.k[0])), dv = umma_desc_sw128_n(smem_u32(sm.v[0]), kTrHalf);
-      int gs = 0;                                        // steps of earlier items
-      int n[kTrTiles] = {0, 0};                          // steps per tile
+      TrRing op(kTrOps);
+      uint32_t s_phase = 3;                                // of what each tile lets go or brings, bit = tile (a wait for scores that nobody holds is over at once)
+      if (!is_s) s_phase = 0;
       uint32_t q_phase = 0;                              // bit = tile
       for (int it = 0;; ++it) {
         const TrItem& l = sm.list[it % kTrLists];
@@ -491,9 +575,9 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
         const int steps = l.steps;
         const bool split = tr_split(l);
 #pragma unroll 1
-        for (int s = 0; s < steps; ++s, ++gs) {
-          const int b = gs % kTrOps;
-          if (ok) ok = mbar_wait_park(smem_u32(is_s ? &sm.k_full[b] : &sm.v_full[b]), (gs / kTrOps) & 1, abort_flag);
+        for (int s = 0; s < steps; ++s, op.advance()) {
+          const int b = op.i;
+          if (ok) ok = mbar_wait_park(smem_u32(is_s ? &sm.k_full[b] : &sm.v_full[b]), op.phase, abort_flag);
 #pragma unroll
           for (int t = 0; t < kTrTiles; ++t) {
             if (split && (s & 1) != t) continue;
@@ -504,12 +588,12 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
                 if (ok) ok = mbar_wait_park(smem_u32(&sm.q_full[t]), q_phase >> t & 1, abort_flag);
                 q_phase ^= 1u << t;
               }
-              if (ok && n[t] > 0) ok = mbar_wait_park(smem_u32(&sm.s_free[t]), (n[t] - 1) & 1, abort_flag);
+              if (ok) ok = mbar_wait_park(smem_u32(&sm.s_free[t]), s_phase >> t & 1, abort_flag);
             } else {
-              if (ok) ok = mbar_wait_park(smem_u32(&sm.p_full[t]), n[t] & 1, abort_flag);
+              if (ok) ok = mbar_wait_park(smem_u32(&sm.p_full[t]), s_phase >> t & 1, abort_flag);
             }
             ok = __all_sync(0xffffffffu, ok);
-            ++n[t];
+            s_phase ^= 1u << t;
             tc_fence_after();
             if (ok && leader) {
               if (is_s) {
@@ -539,58 +623,36 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTrRegsConvert));
     const bool is_v = warp >= 12;
     const int ct = tid & 127;
-    int gs = 0;
+    TrRing raw_at(kTrRaw), note_at(kTrNotes), op(kTrOps, 1);               // (a wait for operands that nobody reads is over at once)
+    uint64_t* op_free = is_v ? sm.v_free : sm.k_free;
+    uint64_t* op_full = is_v ? sm.v_full : sm.k_full;
+#pragma unroll 1
     for (int it = 0;; ++it) {
       const TrItem& l = sm.list[it % kTrLists];
       if (ok) ok = mbar_wait_park(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok || l.kvh < 0) break;
       const int steps = l.steps;
-      int v_exp = 0;
-      uint32_t v_most = 0, v_least = 0x7F800000u;        // of the item's steps
+      int visible = l.total - l.lo * kTrTok;
 #pragma unroll 1
-      for (int s = 0; s < steps; ++s, ++gs) {
-        const int b = gs % kTrOps, slot = gs % kTrRaw, note = gs % kTrNotes, visible = l.total - (l.lo + s) * kTrTok;
-        if (ok) ok = mbar_wait_park(smem_u32(&sm.raw_full[slot]), (gs / kTrRaw) & 1, abort_flag);
+      for (int s = 0; s < steps; ++s, visible -= kTrTok) {
+        if (ok) ok = mbar_wait_park(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag);
+        if (ok) ok = mbar_wait_park(smem_u32(&sm.note_full[note_at.i]), note_at.phase, abort_flag);
+        if (ok) ok = mbar_wait_park(smem_u32(&op_free[op.i]), op.phase, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const uint8_t* pages = raw + slot * kTrPages * stride;
-        float4 scale[2];
-        pf_scales(pages + (is_v ? lay.v_scale_off : lay.k_scale_off), stride, visible, lane, scale);
-        uint32_t most = __reduce_max_sync(0xffffffffu, max(pf_most<false>(scale[0]), pf_most<false>(scale[1])));       // (every warp for itself)
-        const bool odd = most >= 0x7F800000u;                            // some are not finite
-        if (odd) most = __reduce_max_sync(0xffffffffu, max(pf_most<true>(scale[0]), pf_most<true>(scale[1])));
-        const int e = pf_exponent(most);
-        uint32_t least = 0x7F800000u;
-        if ((warp & 3) == 0) least = __reduce_min_sync(0xffffffffu, min(tr_least(scale[0]), tr_least(scale[1])));
-        // K: codes times scales below 2^13; V: below 2^11, to be changed when they pass 2^15.  Noted before there is room for the operands: softmax waits for it
-        if (!is_v) {
-          if (warp == 8 && lane == 0) {
-            if (odd || (least < 0x7F800000u && pf_exponent(least) < e - kTrApartK)) sm.redo[it % kTrLists] = 1;
-            sm.k_mul[note] = pow2f(e - 5);
-            mbar_arrive(smem_u32(&sm.k_note[note]));
-          }
-        } else {
-          if (s == 0 || e - 7 > v_exp) v_exp = e - 3;
-          if (warp == 12 && lane == 0) {
-            v_most = max(v_most, most);
-            v_least = min(v_least, least);
-            if (odd || (v_least < 0x7F800000u && pf_exponent(v_least) < pf_exponent(v_most) - kTrApartV)) sm.redo[it % kTrLists] = 1;
-            sm.v_exp[note] = v_exp;
-            mbar_arrive(smem_u32(&sm.v_note[note]));
-          }
-        }
-        if (gs >= kTrOps) ok = mbar_wait_park(smem_u32(is_v ? &sm.v_free[b] : &sm.k_free[b]), (gs / kTrOps - 1) & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (!is_v) tr_convert_k<KBITS>(sm.k[b], pages, stride, lay, pow2f(5 - e), ct);
-        else tr_convert_v<VBITS>(sm.v[b], pages, stride, lay, visible, pow2f(-v_exp), ct);
+        const uint8_t* pages = raw + raw_at.i * kTrPages * L::stride;
+        if (!is_v) tr_convert_k<KBITS, VBITS>(sm.k[op.i], pages, sm.note[note_at.i].x, ct);
+        else tr_convert_v<KBITS, VBITS>(sm.v[op.i], pages, visible, sm.note[note_at.i].y, ct);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(smem_u32(is_v ? &sm.v_full[b] : &sm.k_full[b]));
-          mbar_arrive(smem_u32(&sm.raw_free[slot]));
+          mbar_arrive(smem_u32(&op_full[op.i]));
+          mbar_arrive(smem_u32(&sm.raw_free[raw_at.i]));
         }
+        raw_at.advance();
+        note_at.advance();
+        op.advance();
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sm.list_free[it % kTrLists]));
@@ -659,7 +721,7 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
       }
       return true;
     };
-    int gs0 = 0, n = 0, exchanges = 0;                   // steps of earlier items; steps that this tile took part in; items in both tiles
+    int note0 = 0, n = 0, exchanges = 0;                 // note of the item's first step; steps that this tile took part in; items in both tiles
     bool lent = false;                                   // the other tile may still read this one's output
     auto wait_lent = [&]() {
       if (lent && ok) ok = mbar_wait_park(smem_u32(&sm.exch_free), (exchanges - 1) & 1, abort_flag);
@@ -676,9 +738,11 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
       int v_exp = 0;
       {
         const int first = split ? t : 0;
+        int note = note0 + first;
+        if (note >= kTrNotes) note -= kTrNotes;
 #pragma unroll 1
         for (int s = first; s < steps; s += split ? 2 : 1) {
-          const int gs = gs0 + s, note = gs % kTrNotes, tok0 = (l.lo + s) * kTrTok;
+          const int tok0 = (l.lo + s) * kTrTok;
           if (ok) ok = mbar_wait_park(smem_u32(&sm.s_full[t]), n & 1, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
@@ -708,10 +772,11 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
             for (int j = 0; j < 32; j += 2) of[j / 2 & 3] = fmaxf(of[j / 2 & 3], fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
             mx = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
           }
-          // (a note is written again after this step's product, which waits for what follows: kTrNotes)
-          if (ok) ok = mbar_wait_park(smem_u32(&sm.k_note[note]), (gs / kTrNotes) & 1, abort_flag);
-          if (ok) ok = mbar_wait_park(smem_u32(&sm.v_note[note]), (gs / kTrNotes) & 1, abort_flag);
-          const float mul = sm.k_mul[note] * cur.mul, top = mx * mul;
+          // (there before K was converted; written again after this step's product, which waits for what follows: kTrNotes)
+          const float2 told = *reinterpret_cast<const float2*>(&sm.note[note].z);
+          note += split ? 2 : 1;
+          if (note >= kTrNotes) note -= kTrNotes;
+          const float mul = told.x * cur.mul, top = mx * mul;
           float alpha = 1.f;
           bool grew = top > m + kTrGrowth || (m == -INFINITY && top > m);
           if (grew) {
@@ -719,7 +784,7 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
             m = top;
             sum *= alpha;
           }
-          const int e = sm.v_exp[note];
+          const int e = __float_as_int(told.y);
           if (e != v_exp) {
             alpha = v_exp - e < -126 ? 0.f : alpha * pow2f(v_exp - e);
             v_exp = e;
@@ -769,7 +834,7 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
           ++n;
         }
       }
-      gs0 += steps;
+      note0 = (note0 + steps) % kTrNotes;
       // the next item's Q while the last product runs (all of this item's scores are there)
       Row next;
       more = begin(it + 1, next);
@@ -843,7 +908,7 @@ tree_kernel(const CbTreeAttn p, const KvLayout lay, const int part_rows) {
             const long long q = __shfl_sync(0xffffffffu, cur.q, of), out = __shfl_sync(0xffffffffu, cur.out, of);
             const uint32_t* sees = reinterpret_cast<const uint32_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(cur.sees), of));
             float rm, rs, o[4];
-            tree_row<KBITS, VBITS>(p, lay, r, l.kvh, lo, hi, sees, p.q + q, lane, rm, rs, o, bad);
+            tree_row<KBITS, VBITS>(p, r, l.kvh, lo, hi, sees, p.q + q, lane, rm, rs, o, bad);
             if (part >= 0) {
               const size_t to = at - lane + of;
               reinterpret_cast<float4*>(part_o + to * kD)[lane] = make_float4(o[0], o[1], o[2], o[3]);
@@ -902,9 +967,7 @@ tree_merge_kernel(const CbTreeAttn p, const int part_rows) {
 
 template <int KB, int VB>
 static int launch_tree(const CbTreeAttn& p, cudaStream_t st) {
-  const KvLayout lay = make_kv_layout(kD, KB, VB);
-  const int stride = (lay.blob_bytes + 127) & ~127;
-  const size_t smem = sizeof(TrSmem) + 1024 + static_cast<size_t>(kTrRaw) * kTrPages * stride;
+  const size_t smem = sizeof(TrSmem) + 1024 + static_cast<size_t>(kTrRaw) * kTrPages * TreeLay<KB, VB>::stride;
   static int sms[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -18;
@@ -921,7 +984,7 @@ static int launch_tree(const CbTreeAttn& p, cudaStream_t st) {
     sms[dev] = n;
   }
   const int rows = tr_rows(p.words, p.rows, p.Hq / p.Hkv);
-  cudaError_t e = launch(tree_kernel<KB, VB>, dim3(sms[dev]), dim3(kTrThreads), smem, st, p, lay, rows);
+  cudaError_t e = launch(tree_kernel<KB, VB>, dim3(sms[dev]), dim3(kTrThreads), smem, st, p, rows);
   if (e == cudaSuccess) e = launch(tree_merge_kernel, dim3(sms[dev], (rows + 15) / 16), dim3(256), 0, st, p, rows);
   return static_cast<int>(e);
 }
