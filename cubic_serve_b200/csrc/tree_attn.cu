@@ -117,9 +117,10 @@ static constexpr int kTrOps = 3;                         // steps of operands
 // Steps whose powers of two are kept: the note of step s is written behind raw_full (s) <- raw_free (s - kTrRaw) <- v_free of step s - kTrRaw - kTrOps <- p_full of the
 // tiles that take part in it, which have read theirs by then.
 static constexpr int kTrNotes = kTrRaw + kTrOps;
-static constexpr int kTrLeast = 1;                       // steps of a CTA, at least
+static constexpr long long kTrLeast = 1;                       // steps of a CTA, at least
 static constexpr float kTrGrowth = 2.f;
-static constexpr int kTrApartK = 18, kTrApartV = 14;
+static constexpr int kTrApart = 9;                       // powers of two that scales are apart: up to here the short conversion, ...
+static constexpr int kTrApartK = 18, kTrApartV = 14;     // ... and the long one
 static constexpr int kTrHalf = kTrTok * 128;             // bytes of 64 channels of a step
 static constexpr uint32_t kTrTmemCols = 512, kTrTmemTile = 256, kTrTmemP = 64, kTrTmemQ = 96, kTrTmemO = 128;
 
@@ -127,9 +128,10 @@ static constexpr uint32_t kTrTmemCols = 512, kTrTmemTile = 256, kTrTmemP = 64, k
 struct TrRing {
   int i, n;
   uint32_t phase;
-  __device__ __forceinline__ explicit TrRing(int places, uint32_t parity = 0) : i(0), n(places), phase(parity) {}
-  __device__ __forceinline__ void advance() {
-    if (++i == n) { i = 0; phase ^= 1u; }
+  __device__ __forceinline__ explicit TrRing(int places, uint32_t parity = 0, int at = 0) : i(at), n(places), phase(parity) {}
+  __device__ __forceinline__ void advance(int by = 1) {
+    i += by;
+    if (i >= n) { i -= n; phase ^= 1u; }
   }
 };
 struct TrItem {
@@ -144,7 +146,12 @@ struct __align__(1024) TrSmem {
   uint8_t q[kTrTiles][kTrRows * 128];                    // f16, channels 64..127: [row][128 B], 16-byte chunk ^ (row & 7)
   uint8_t k[kTrOps][2 * kTrHalf];                             // f16 [stage][64-channel half][token][128 B]
   uint8_t v[kTrOps][2 * kTrHalf];                             // likewise
-  float4 note[kTrNotes];                                 // of a step: what K and V are multiplied with, what scores are multiplied with, 2^this is V's unit
+  struct Note {
+    float k, v;                                          // of a step: what the scales of K and V are multiplied with, ...
+    int k_wide, v_wide;                                  // ... and whether the long conversion takes them
+    float back;                                          // scores are this times what the MMAs give
+    int v_exp;                                           // output is 2^v_exp times ...
+  } note[kTrNotes];
   uint32_t redo[kTrLists];                               // of an item's steps: some values are beyond what f16 operands hold
   uint64_t raw_full[kTrRaw], raw_free[kTrRaw], k_full[kTrOps], k_free[kTrOps], v_full[kTrOps], v_free[kTrOps], note_full[kTrNotes];
   uint64_t list_full[kTrLists], list_free[kTrLists], q_full[kTrTiles], s_full[kTrTiles], s_free[kTrTiles], p_full[kTrTiles], pv_done[kTrTiles];
@@ -152,7 +159,6 @@ struct __align__(1024) TrSmem {
   TrItem list[kTrLists];
   float2 exch_ml[kTrTiles][kTrRows];                     // rows in both tiles: maximum and sum, ...
   int exch_exp[kTrTiles][kTrRows];                       // ... and v_exp
-  long long sums[kTrThreads / 32];
   uint32_t tmem, abort_word;
   long long upto[kTreeMaxRequests + 1];                  // steps of the requests before
 };
@@ -161,6 +167,9 @@ struct __align__(1024) TrSmem {
 __device__ __forceinline__ bool tr_split(const TrItem& l) { return l.rows <= kTrRows; }
 __device__ __forceinline__ bool tr_takes_part(const TrItem& l, int t) { return tr_split(l) ? l.steps > t : l.steps > 0; }
 
+__device__ __forceinline__ long long tr_divide(long long a, long long b) {       // (most numbers have 32 bits)
+  return (a | b) >> 32 ? a / b : static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+}
 __device__ __forceinline__ int tr_steps(const TreeRequest& r) { return max(1, (r.total + kTrTok - 1) / kTrTok); }
 __device__ __forceinline__ int tr_groups(const TreeRequest& r, int G) { return (r.count * G + kTrItemRows - 1) / kTrItemRows; }
 static inline int tr_rows(int words, int rows, int G) {
@@ -168,25 +177,54 @@ static inline int tr_rows(int words, int rows, int G) {
   return most < kTrItemRows ? static_cast<int>(most) : kTrItemRows;
 }
 
-// One step's codes into operands.  A code times its scale sh + sl (f16 each): the product with sl, rounded, is 2^-11 of the whole, so that the
-// multiply-add behind it rounds once what 32-bit arithmetic would.  What K holds of tokens that no row sees is masked with their scores.
-__device__ __forceinline__ uint32_t tr_scaled(uint32_t code, uint32_t sh, uint32_t sl) {
-  uint32_t t, r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(t) : "r"(code), "r"(sl));
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(code), "r"(sh), "r"(t));
-  return r;
-}
+// One step's codes into operands: code times scale, in f16.  A byte b (the code and its bias) in the low bits of an f16 is the number 2^-24 b, exactly.
+// Short: with the scale as f16 times 2^24 that takes one multiply-add, b S - bias S, of two roundings (the scale's and the product's, 2^-11 each), as long as what the
+// operands hold is below 2^-2 and their scales are no more than 2^9 apart: below 2^-14 f16 has steps of 2^-24.
+// WIDE: the code as f16 (a subtraction) times sh + sl, f16 each: the product with sl, rounded, is 2^-11 of the whole, so that the multiply-add behind it rounds once
+// what 32-bit arithmetic would; values up to 2^15.
+// What K holds of tokens that no row sees is masked with their scores.
 __device__ __forceinline__ void tr_put(uint32_t to, const uint4& x) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
 }
-__device__ __forceinline__ uint4 tr_scaled8(const uint4& c, uint32_t sh, uint32_t sl) {
-  return make_uint4(tr_scaled(c.x, sh, sl), tr_scaled(c.y, sh, sl), tr_scaled(c.z, sh, sl), tr_scaled(c.w, sh, sl));
+__device__ __forceinline__ uint32_t tr_mul(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t tr_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+// the two numbers that a scale times the step's power of two is taken as
+template <int BITS, bool WIDE>
+__device__ __forceinline__ void tr_scale(float s, uint32_t& a, uint32_t& b) {
+  if constexpr (WIDE) {
+    pf_split(s, a, b);
+  } else {
+    constexpr uint32_t bias = BITS == 8 ? 0x80808080u : BITS == 6 ? 0x80208020u : 0x80088008u;           // -bias 2^-24
+    a = pack_f16x2(s, s);
+    b = tr_mul(a, bias);
+  }
+}
+// the bytes that `sel` takes of a word
+template <int BITS, bool WIDE>
+__device__ __forceinline__ uint32_t tr_pair(uint32_t word, uint32_t sel, uint32_t a, uint32_t b) {
+  if constexpr (WIDE) {
+    const uint32_t code = u8x2_to_f16x2(word, sel, BITS == 8 ? 0x64806480u : BITS == 6 ? 0x64206420u : 0x64086408u);
+    return tr_fma(code, a, tr_mul(code, b));
+  } else {
+    return tr_fma(prmt(word, 0u, sel), a, b);
+  }
+}
+template <int BITS, bool WIDE>
+__device__ __forceinline__ uint4 tr_eight(uint32_t x, uint32_t y, uint32_t a, uint32_t b) {              // eight bytes in order
+  return make_uint4(tr_pair<BITS, WIDE>(x, 0x5140u, a, b), tr_pair<BITS, WIDE>(x, 0x5342u, a, b), tr_pair<BITS, WIDE>(y, 0x5140u, a, b), tr_pair<BITS, WIDE>(y, 0x5342u, a, b));
 }
 // (The loops stay loops: five kinds of warps run their code at the same time, and unrolled it does not fit the instruction caches: 3700 cycles a step.)
-template <int KBITS, int VBITS>
+template <int KBITS, int VBITS, bool WIDE>
 __device__ __forceinline__ void tr_convert_k(uint8_t* k, const uint8_t* raw, float mul, int tid) {
   using L = TreeLay<KBITS, VBITS>;
-  constexpr uint32_t kb = KBITS == 8 ? 0x64806480u : KBITS == 6 ? 0x64206420u : 0x64086408u;
   // an item is a scale's 32 channels of a token
   const int tok = tid & 15, g = tid >> 4 & 3, sw = tok & 7;
   raw += (tid >> 6) * L::stride;
@@ -199,7 +237,7 @@ __device__ __forceinline__ void tr_convert_k(uint8_t* k, const uint8_t* raw, flo
 #pragma unroll 1
   for (int page = 0; page < kTrPages / 2; ++page) {
     uint32_t sh, sl;
-    pf_split(*reinterpret_cast<const float*>(scale) * mul, sh, sl);
+    tr_scale<KBITS, WIDE>(*reinterpret_cast<const float*>(scale) * mul, sh, sl);
     uint4 x, w = make_uint4(0u, 0u, 0u, 0u);
     if constexpr (KBITS != 8) x = *reinterpret_cast<const uint4*>(codes);
     if constexpr (KBITS == 6) {
@@ -220,8 +258,8 @@ __device__ __forceinline__ void tr_convert_k(uint8_t* k, const uint8_t* raw, flo
           w = make_uint4(w.x >> 2, w.y >> 2, w.z >> 2, w.w >> 2);
         }
       }
-      tr_put(to + one, tr_scaled8(conv8(make_uint2(n.x, n.y), kb), sh, sl));
-      tr_put(to + (one ^ 16), tr_scaled8(conv8(make_uint2(n.z, n.w), kb), sh, sl));
+      tr_put(to + one, tr_eight<KBITS, WIDE>(n.x, n.y, sh, sl));
+      tr_put(to + (one ^ 16), tr_eight<KBITS, WIDE>(n.z, n.w, sh, sl));
       to ^= 32;
     }
     codes += 2 * L::stride; high += 2 * L::stride; scale += 2 * L::stride;
@@ -229,10 +267,9 @@ __device__ __forceinline__ void tr_convert_k(uint8_t* k, const uint8_t* raw, flo
   }
 }
 // V from `visible` on becomes zeros: those slots may hold anything, and a probability of zero has to stay zero.
-template <int KBITS, int VBITS>
+template <int KBITS, int VBITS, bool WIDE>
 __device__ __forceinline__ void tr_convert_v(uint8_t* v, const uint8_t* raw, int visible, float mul, int tid) {
   using L = TreeLay<KBITS, VBITS>;
-  constexpr uint32_t vb = VBITS == 8 ? 0x64806480u : VBITS == 6 ? 0x64206420u : 0x64086408u;
   // an item is 16 channels of a token pair, eight at a time: lanes 0-3 of eight take the first eight first, the others the second (no bank twice)
   const int c = tid & 7, pair = tid >> 3 & 7, first = tid >> 2 & 1;
   const int at = (4 * c) ^ ((pair & 3) << 2);
@@ -250,7 +287,7 @@ __device__ __forceinline__ void tr_convert_v(uint8_t* v, const uint8_t* raw, int
     for (int h = 0; h < 2; ++h) {
       float f = *reinterpret_cast<const float*>(scale + h * 16) * mul;
       if (tok + h >= visible || !(fabsf(f) < INFINITY)) f = 0.f;
-      pf_split(f, sh[h], sl[h]);
+      tr_scale<VBITS, WIDE>(f, sh[h], sl[h]);
     }
     const uint32_t to = smem_u32(v);
 #pragma unroll 1
@@ -274,16 +311,16 @@ __device__ __forceinline__ void tr_convert_v(uint8_t* v, const uint8_t* raw, int
         uint4 f;
         if constexpr (VBITS == 8) {
           const uint32_t sel = h ? 0x5341u : 0x5240u;
-          f = make_uint4(u8x2_to_f16x2(x.x, sel, vb), u8x2_to_f16x2(x.y, sel, vb), u8x2_to_f16x2(x.z, sel, vb), u8x2_to_f16x2(x.w, sel, vb));
+          f = make_uint4(tr_pair<8, WIDE>(x.x, sel, sh[h], sl[h]), tr_pair<8, WIDE>(x.y, sel, sh[h], sl[h]), tr_pair<8, WIDE>(x.z, sel, sh[h], sl[h]), tr_pair<8, WIDE>(x.w, sel, sh[h], sl[h]));
         } else {
           uint2 n = h ? make_uint2((x.x >> 4) & 0x0F0F0F0Fu, (x.y >> 4) & 0x0F0F0F0Fu) : make_uint2(x.x & 0x0F0F0F0Fu, x.y & 0x0F0F0F0Fu);
           if constexpr (VBITS == 6) {
             n.x |= (h ? x.z >> 2 : x.z) & 0x30303030u;
             n.y |= (h ? x.w >> 2 : x.w) & 0x30303030u;
           }
-          f = conv8(n, vb);
+          f = tr_eight<VBITS, WIDE>(n.x, n.y, sh[h], sl[h]);
         }
-        tr_put(to + h * 128 + ((half ^ h) << 4), tr_scaled8(f, sh[h], sl[h]));
+        tr_put(to + h * 128 + ((half ^ h) << 4), f);
       }
     }
     codes += 2 * L::stride; high += 2 * L::stride; scale += 2 * L::stride;
@@ -324,15 +361,15 @@ __device__ __forceinline__ uint2 tr_visible(const uint32_t* sees, int words, int
   return m;
 }
 
-// Roles: warps 0-7 own a row a thread (softmax needs no exchange: tensor-memory lane = row); warps 8-11 convert raw pages of K to the swizzled operand
-// ([token][channel], f16), warps 12-15 those of V; warps 16 and 18 issue the MMAs of the scores and of the output; warp 17 makes the items and copies pages;
+// Roles: warps 0-7 own a row a thread (softmax needs no exchange: tensor-memory lane = row); warps 8-11 convert raw pages to the swizzled operands of K
+// and V ([token][channel], f16), by turns with warps 12-15; warps 16 and 18 issue the MMAs of the scores and of the output; warp 17 makes the items and copies pages;
 // warp 19 finds the powers of two that bring a step's values into f16's range.
 // Tensor memory of a tile of 128 rows: scores, probabilities (the A operand of their product), output and the first half of Q's channels; the other half of
 // Q is in shared memory.  The scores of step i + 1 are computed while the softmax of step i runs.  The output is rescaled only when a row's maximum has grown by more
 // than a factor of four: until then probabilities relative to the older maximum are at most 4.
 // Powers of two keep operands in the range of f16: a row's for Q (undone with the softmax' scale: its 8 bits stay exact), a step's for K (likewise), one for V that grows
-// with the largest scale (undone with the output).  A request whose scales are further apart than that holds (2^18 in a step of K, 2^14 in a CTA's steps of V), or not finite,
-// is computed in fp32 (tree_row): a hundred times as long, for caches as no model has them.
+// with the largest scale (undone with the output).  Items whose scales are further apart than that holds (2^18 in a step of K, 2^14 in a CTA's steps of V), or not finite,
+// are computed in fp32 (tree_row): a hundred times as long, for caches as no model has them.
 // Every wait is bounded; on a timeout the roles leave, the status word is set and tensor memory is freed.
 template <int KBITS, int VBITS>
 __global__ void __launch_bounds__(kTrThreads, 1)
@@ -349,7 +386,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
   if (tid == 0) {
     for (int b = 0; b < kTrRaw; ++b) {
       mbar_init(smem_u32(&sm.raw_full[b]), 1);
-      mbar_init(smem_u32(&sm.raw_free[b]), 8);
+      mbar_init(smem_u32(&sm.raw_free[b]), 4);
     }
     for (int b = 0; b < kTrOps; ++b) {
       mbar_init(smem_u32(&sm.k_full[b]), 4);
@@ -383,40 +420,36 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
   pdl_wait();
   pdl_launch_dependents();
   bool bad = false;
-  {
-    // steps of all requests, summed; two neighbouring requests a thread
-    long long mine[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      if (2 * tid + j < p.n) {
-        const TreeRequest r = tree_request(p, 2 * tid + j, bad);
-        mine[j] = static_cast<long long>(tr_steps(r)) * tr_groups(r, G) * p.Hkv;
-      }
-    long long v = mine[0] + mine[1];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
-    }
-    if (lane == 31) sm.sums[warp] = v;
-    __syncthreads();
-    long long before = v - mine[0] - mine[1];
-    for (int w = 0; w < warp; ++w) before += sm.sums[w];
-    if (tid == 0) sm.upto[0] = 0;
-    if (2 * tid < p.n) sm.upto[2 * tid + 1] = before + mine[0];
-    if (2 * tid + 1 < p.n) sm.upto[2 * tid + 2] = before + mine[0] + mine[1];
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
-  const long long all = sm.upto[p.n], per = max(static_cast<long long>(kTrLeast), (all + gridDim.x - 1) / gridDim.x);
   bool ok = true;
 
   if (warp >= 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTrRegsOther));
     if (warp == 17) {
       // ------------------------------------------------------- items and pages
+      // steps of all requests, summed
+      long long all = 0;
+      if (lane == 0) sm.upto[0] = 0;
+#pragma unroll 4
+      for (int i0 = 0; i0 < p.n; i0 += 32) {
+        long long v = 0;
+        if (i0 + lane < p.n) {
+          const TreeRequest r = tree_request(p, i0 + lane, bad);
+          v = static_cast<long long>(tr_steps(r)) * (tr_groups(r, G) * p.Hkv);
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long before = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += before;
+        }
+        if (i0 + lane < p.n) sm.upto[i0 + lane + 1] = all + v;
+        all += __shfl_sync(0xffffffffu, v, 31);
+      }
+      __syncwarp();
+      const long long per = max(kTrLeast, tr_divide(all + gridDim.x - 1, gridDim.x));
       long long u = min(all, per * blockIdx.x);
       const long long end = min(all, u + per);
       int i = 0, gs = 0;
@@ -449,7 +482,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           }
           const int S = tr_steps(r), groups = tr_groups(r, G);
           const long long off = u - sm.upto[i];
-          const int k = static_cast<int>(off / S), s = static_cast<int>(off - static_cast<long long>(k) * S);
+          const int k = static_cast<int>(tr_divide(off, S)), s = static_cast<int>(off - static_cast<long long>(k) * S);
           const int n_steps = static_cast<int>(min(static_cast<long long>(S - s), end - u));
           l.kvh = k / groups;
           l.slot = r.slot; l.row0 = r.row0; l.count = r.count; l.start = r.start; l.total = r.total;
@@ -459,7 +492,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           l.steps = r.total > 0 ? n_steps : 0;
           l.part = n_steps == S ? -1 : 2 * static_cast<int>(blockIdx.x) + (s == 0);
           if (l.part >= 0 && s == 0) {
-            d.parts = static_cast<int>((u + S - 1) / per) - static_cast<int>(blockIdx.x) + 1;
+            d.parts = static_cast<int>(tr_divide(u + S - 1, per)) - static_cast<int>(blockIdx.x) + 1;
             d.row0 = l.row0; d.first = l.first; d.rows = l.rows; d.kvh = l.kvh;
           }
           u += n_steps;
@@ -520,8 +553,8 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
         ok = __all_sync(0xffffffffu, ok);
         if (!ok || l.kvh < 0) break;
         const int steps = l.steps;
-        int v_exp = 0, visible = l.total - l.lo * kTrTok;
-        uint32_t v_most = 0, v_least = 0x7F800000u;      // of the item's steps
+        int v_exp = 0, visible = l.total - l.lo * kTrTok, v_most = -200, v_least = 200;              // of the item's steps
+        bool v_wide = false;
 #pragma unroll 1
         for (int s = 0; s < steps; ++s, visible -= kTrTok) {
           if (ok) ok = mbar_wait_park(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag);
@@ -541,15 +574,26 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
             }
             least[w] = __reduce_min_sync(0xffffffffu, min(tr_least(scale[0]), tr_least(scale[1])));
           }
-          // K: codes times scales below 2^13; V: below 2^11, to be changed when they pass 2^15
-          const int ek = pf_exponent(most[0]), ev = pf_exponent(most[1]);
-          if (s == 0 || ev - 7 > v_exp) v_exp = ev - 3;
-          v_most = max(v_most, most[1]);
-          v_least = min(v_least, least[1]);
+          const int ek = pf_exponent(most[0]), ev = pf_exponent(most[1]), lk = pf_exponent(least[0]);
+          const bool k_wide = lk < ek - kTrApart || ek > 100;
+          v_most = max(v_most, ev);
+          v_least = min(v_least, pf_exponent(least[1]));
+          // V: one unit for the item, that follows the largest scale; in the long conversion only when operands pass 2^15
+          if (!v_wide) {
+            v_exp = v_most + 10;
+            if (v_least < v_most - kTrApart || v_most > 100) { v_wide = true; v_exp = v_most - 3; }
+          } else if (ev - 7 > v_exp) {
+            v_exp = ev - 3;
+          }
           if (lane == 0) {
-            if (odd || (least[0] < 0x7F800000u && pf_exponent(least[0]) < ek - kTrApartK) || (v_least < 0x7F800000u && pf_exponent(v_least) < pf_exponent(v_most) - kTrApartV))
-              sm.redo[it % kTrLists] = 1;
-            sm.note[note_at.i] = make_float4(pow2f(5 - ek), pow2f(-v_exp), pow2f(ek - 5), __int_as_float(v_exp));
+            if (odd || lk < ek - kTrApartK || v_least < v_most - kTrApartV) sm.redo[it % kTrLists] = 1;
+            auto& to = sm.note[note_at.i];
+            to.k = pow2f(k_wide ? 5 - ek : 14 - ek);
+            to.v = pow2f(v_wide ? -v_exp : 24 - v_exp);
+            to.k_wide = k_wide;
+            to.v_wide = v_wide;
+            to.back = pow2f(k_wide ? ek - 5 : ek + 10);
+            to.v_exp = v_exp;
             mbar_arrive(smem_u32(&sm.note_full[note_at.i]));
           }
           __syncwarp();
@@ -621,11 +665,10 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
   } else if (warp >= 8) {
     // ------------------------------------------------------------ conversion
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTrRegsConvert));
-    const bool is_v = warp >= 12;
-    const int ct = tid & 127;
-    TrRing raw_at(kTrRaw), note_at(kTrNotes), op(kTrOps, 1);               // (a wait for operands that nobody reads is over at once)
-    uint64_t* op_free = is_v ? sm.v_free : sm.k_free;
-    uint64_t* op_full = is_v ? sm.v_full : sm.k_full;
+    // warps 8-11 take the even steps, 12-15 the odd ones, K first: scores run ahead of their softmax
+    const int ct = tid & 127, mine = warp >= 12;
+    TrRing raw_at(kTrRaw, 0, mine), note_at(kTrNotes, 0, mine), op(kTrOps, 1, mine);         // (a wait for operands that nobody reads is over at once)
+    int ahead = mine;                                    // steps from the item's first to this warp's next
 #pragma unroll 1
     for (int it = 0;; ++it) {
       const TrItem& l = sm.list[it % kTrLists];
@@ -633,27 +676,39 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       ok = __all_sync(0xffffffffu, ok);
       if (!ok || l.kvh < 0) break;
       const int steps = l.steps;
-      int visible = l.total - l.lo * kTrTok;
+      int visible = l.total - (l.lo + ahead) * kTrTok;
 #pragma unroll 1
-      for (int s = 0; s < steps; ++s, visible -= kTrTok) {
+      for (; ahead < steps; ahead += 2, visible -= 2 * kTrTok) {
         if (ok) ok = mbar_wait_park(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag);
         if (ok) ok = mbar_wait_park(smem_u32(&sm.note_full[note_at.i]), note_at.phase, abort_flag);
-        if (ok) ok = mbar_wait_park(smem_u32(&op_free[op.i]), op.phase, abort_flag);
+        if (ok) ok = mbar_wait_park(smem_u32(&sm.k_free[op.i]), op.phase, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint8_t* pages = raw + raw_at.i * kTrPages * L::stride;
-        if (!is_v) tr_convert_k<KBITS, VBITS>(sm.k[op.i], pages, sm.note[note_at.i].x, ct);
-        else tr_convert_v<KBITS, VBITS>(sm.v[op.i], pages, visible, sm.note[note_at.i].y, ct);
+        const auto& note = sm.note[note_at.i];
+        const float v_mul = note.v;
+        const int v_wide = note.v_wide;
+        if (!note.k_wide) tr_convert_k<KBITS, VBITS, false>(sm.k[op.i], pages, note.k, ct);
+        else tr_convert_k<KBITS, VBITS, true>(sm.k[op.i], pages, note.k, ct);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.k_full[op.i]));
+        ok = mbar_wait_park(smem_u32(&sm.v_free[op.i]), op.phase, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (!v_wide) tr_convert_v<KBITS, VBITS, false>(sm.v[op.i], pages, visible, v_mul, ct);
+        else tr_convert_v<KBITS, VBITS, true>(sm.v[op.i], pages, visible, v_mul, ct);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(smem_u32(&op_full[op.i]));
+          mbar_arrive(smem_u32(&sm.v_full[op.i]));
           mbar_arrive(smem_u32(&sm.raw_free[raw_at.i]));
         }
-        raw_at.advance();
-        note_at.advance();
-        op.advance();
+        raw_at.advance(2);
+        note_at.advance(2);
+        op.advance(2);
       }
+      ahead -= steps;
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sm.list_free[it % kTrLists]));
     }
@@ -685,25 +740,19 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       }
       if (tr_takes_part(l, t)) {
         // a power of two brings the row's largest magnitude to 2^10 .. 2^11; what is not finite stays
-        const uint4* q = reinterpret_cast<const uint4*>(p.q + r.q);
-        uint32_t most = 0;
-        if (r.q >= 0) {
-#pragma unroll 4
-          for (int c = 0; c < 16; ++c) {
-            const uint4 u = q[c];
-            const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+        uint4 q[16];                                     // all loads in flight at once
 #pragma unroll
-            for (int j = 0; j < 4; ++j) most = max(most, max(in[j] & 0x7FFFu, in[j] >> 16 & 0x7FFFu));
-          }
-        }
+        for (int c = 0; c < 16; ++c) q[c] = r.q >= 0 ? reinterpret_cast<const uint4*>(p.q + r.q)[c] : make_uint4(0u, 0u, 0u, 0u);
+        uint32_t most = 0;                               // (two magnitudes a word: the larger of the upper, then of the lower ones)
+#pragma unroll
+        for (int c = 0; c < 16; ++c) most = __vmaxu2(most, __vmaxu2(__vmaxu2(q[c].x & 0x7FFF7FFFu, q[c].y & 0x7FFF7FFFu), __vmaxu2(q[c].z & 0x7FFF7FFFu, q[c].w & 0x7FFF7FFFu)));
+        most = max(most >> 16, most & 0xFFFFu);
         const int e = most >= 0x7F80u || most == 0u ? 0 : max(static_cast<int>(most >> 7) - 127 - 10, -126);
         const float down = pow2f(-e);
         r.mul = pow2f(e) * p.scale * 1.4426950408889634f;
-#pragma unroll 2
+#pragma unroll
         for (int c = 0; c < 16; ++c) {                   // eight channels
-          uint4 u = make_uint4(0u, 0u, 0u, 0u);
-          if (r.q >= 0) u = q[c];
-          const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+          const uint32_t in[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
           uint32_t x[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -773,7 +822,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
             mx = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
           }
           // (there before K was converted; written again after this step's product, which waits for what follows: kTrNotes)
-          const float2 told = *reinterpret_cast<const float2*>(&sm.note[note].z);
+          const float2 told = make_float2(sm.note[note].back, __int_as_float(sm.note[note].v_exp));
           note += split ? 2 : 1;
           if (note >= kTrNotes) note -= kTrNotes;
           const float mul = told.x * cur.mul, top = mx * mul;
@@ -946,23 +995,30 @@ tree_merge_kernel(const CbTreeAttn p, const int part_rows) {
   const float2* part_ml = reinterpret_cast<const float2*>(part_o + static_cast<size_t>(gridDim.x) * 2 * part_rows * kD);
   const TrDesc d = reinterpret_cast<const TrDesc*>(part_ml + static_cast<size_t>(gridDim.x) * 2 * part_rows)[blockIdx.x];
   const int lane = threadIdx.x & 31, G = p.Hq / p.Hkv;
-  for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); d.parts > 0 && row < d.rows; row += gridDim.y * 8) {
-    auto at = [&](int c) { return static_cast<size_t>(2 * (blockIdx.x + c) + (c == 0)) * part_rows + row; };
-    float m = -INFINITY;
-    for (int c = lane; c < d.parts; c += 32) m = fmaxf(m, __ldcg(part_ml + at(c)).x);
-    m = warp_max(m);
-    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < d.parts; ++c) {
-      const float2 ml = __ldcg(part_ml + at(c));
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(part_o + at(c) * kD) + lane);
-      const float f = fast_exp2(ml.x - (m == -INFINITY ? 0.f : m));                    // of a part that saw nothing: zero
-      sum = fmaf(f, ml.y, sum);
-      o[0] = fmaf(f, x.x, o[0]); o[1] = fmaf(f, x.y, o[1]); o[2] = fmaf(f, x.z, o[2]); o[3] = fmaf(f, x.w, o[3]);
+  const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (d.parts <= 0 || row >= d.rows) return;
+  auto at = [&](int c) { return static_cast<size_t>(2 * (blockIdx.x + c) + (c == 0)) * part_rows + row; };
+  float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int c0 = 0; c0 < d.parts; c0 += 32) {             // a lane has a part's maximum and sum
+    const int n = min(32, d.parts - c0);
+    const float2 ml = lane < n ? __ldcg(part_ml + at(c0 + lane)) : make_float2(-INFINITY, 0.f);
+    const float top = fmaxf(m, warp_max(ml.x)), use = top == -INFINITY ? 0.f : top;
+    const float f = fast_exp2(ml.x - use), old = fast_exp2(m - use);                     // of a part that saw nothing: zero
+    m = top;
+    sum = sum * old + warp_sum(f * ml.y);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] *= old;
+#pragma unroll 8
+    for (int c = 0; c < n; ++c) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(part_o + at(c0 + c) * kD) + lane);
+      const float g = __shfl_sync(0xffffffffu, f, c);
+      o[0] = fmaf(g, x.x, o[0]); o[1] = fmaf(g, x.y, o[1]); o[2] = fmaf(g, x.z, o[2]); o[3] = fmaf(g, x.w, o[3]);
     }
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-    const int node = (d.first + row) / G, col = (d.kvh * G + (d.first + row - node * G)) * kD;
-    reinterpret_cast<uint2*>(p.out + (d.row0 + node) * p.ldo + col)[lane] = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
   }
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  const int node = (d.first + row) / G, col = (d.kvh * G + (d.first + row - node * G)) * kD;
+  reinterpret_cast<uint2*>(p.out + (d.row0 + node) * p.ldo + col)[lane] = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
 }
 
 template <int KB, int VB>
@@ -985,7 +1041,7 @@ static int launch_tree(const CbTreeAttn& p, cudaStream_t st) {
   }
   const int rows = tr_rows(p.words, p.rows, p.Hq / p.Hkv);
   cudaError_t e = launch(tree_kernel<KB, VB>, dim3(sms[dev]), dim3(kTrThreads), smem, st, p, rows);
-  if (e == cudaSuccess) e = launch(tree_merge_kernel, dim3(sms[dev], (rows + 15) / 16), dim3(256), 0, st, p, rows);
+  if (e == cudaSuccess) e = launch(tree_merge_kernel, dim3(sms[dev], (rows + 7) / 8), dim3(256), 0, st, p, rows);
   return static_cast<int>(e);
 }
 

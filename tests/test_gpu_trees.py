@@ -73,9 +73,12 @@ class _Round:
     def truth(self, scale=D ** -0.5):
         """(result, how far a kernel may be off), in 64 bits.
 
-        Keys, values and probabilities are rounded to f16 (2^-11 of each), the result to bf16 (2^-8); a score is off by 2^-11 of the sum of
-        its products' magnitudes at most, which moves a probability and its sum by as much; sums in 32 bits, exponentials and
-        the sums of the matrix units add less than 2^-16.
+        Keys and values are products of codes and scales that are rounded to f16 (2^-11 each), probabilities are rounded to f16, the result to bf16 (2^-8);
+        a score is off by 2^-10 of the sum of its products' magnitudes at most, which moves a probability and its sum by as much; sums in 32 bits,
+        exponentials and the sums of the matrix units add less than 2^-16.
+
+        The largest scale lies between 2^-10 and 2^-9 in the unit of the operands, whose smallest steps are 2^-24; a product and the bias in it are each off by
+        half of one at most, so that a key or value may be off by 2^-14 of the largest scale besides.
 
         A probability below 2^-14 has the absolute steps of f16's smallest numbers instead: it is off by half of one, 2^-25, at most, relative to a running
         maximum that is not above the row's own, so that the sum it is divided by is one at least: 2^-25 of the sum of the values' magnitudes."""
@@ -93,14 +96,15 @@ class _Round:
                 k, v = (torch.cat([page[x] for page in pages])[:s + c].double() for x in (0, 1))
                 q = self.q[rows, h * group * D:(h + 1) * group * D].cpu().double().view(c, group, D)
                 z = torch.einsum("cgd,td->cgt", q, k) * scale
-                off = torch.einsum("cgd,td->cgt", q.abs(), k.abs()) * scale * 2.0 ** -11
+                most = [torch.cat([self.scales()[x][p, h].flatten() for p in table[self.slots[i], :-(-(s + c) // 16)].tolist()]).nan_to_num().max().item() for x in (0, 1)]
+                off = torch.einsum("cgd,td->cgt", q.abs(), k.abs()) * scale * 2.0 ** -10 + q.abs().sum(-1, keepdim=True) * scale * 2.0 ** -14 * most[0]
                 z = z.masked_fill(~sees[:, None], -torch.inf)
                 p = torch.where(sees[:, None], torch.exp(z - z.amax(-1, keepdim=True)), 0.0)
                 sums = p.sum(-1, keepdim=True)
                 p = torch.where(sums > 0, p / sums, 0.0)
                 o, a = torch.einsum("cgt,td->cgd", p, v), torch.einsum("cgt,td->cgd", p, v.abs())
                 e = torch.where(sees[:, None], off, 0.0).amax(-1, keepdim=True)
-                t = (torch.expm1(2 * e) + 2 * 2.0 ** -11 + 2.0 ** -16) * a * 1.01 + 2.0 ** -8 * o.abs() + 2.0 ** -25 * torch.einsum("cgt,td->cgd", sees[:, None].double().expand(z.shape), v.abs())
+                t = (torch.expm1(2 * e) + 3 * 2.0 ** -11 + 2.0 ** -16) * a * 1.01 + 2.0 ** -14 * most[1] + 2.0 ** -8 * o.abs() + 2.0 ** -25 * torch.einsum("cgt,td->cgd", sees[:, None].double().expand(z.shape), v.abs())
                 ref[rows, h * group * D:(h + 1) * group * D], tol[rows, h * group * D:(h + 1) * group * D] = o.reshape(c, -1), t.reshape(c, -1)
         return ref, tol
 
