@@ -124,6 +124,11 @@ static constexpr int kTrApartK = 18, kTrApartV = 14;     // ... and the long one
 static constexpr int kTrHalf = kTrTok * 128;             // bytes of 64 channels of a step
 static constexpr uint32_t kTrTmemCols = 512, kTrTmemTile = 256, kTrTmemP = 64, kTrTmemQ = 96, kTrTmemO = 128;
 
+// mbar_wait_park with what follows a wait that is not over at once out of the way of the loops.
+__device__ __forceinline__ bool tr_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
+  return mbar_wait_park(bar, parity, abort_flag);
+}
 // Where a role stands in a ring of n places, and the parity that it waits for there
 struct TrRing {
   int i, n;
@@ -339,9 +344,9 @@ __device__ __forceinline__ uint32_t tr_least(const float4& s) {
 __device__ __forceinline__ void tr_tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
-__device__ __forceinline__ void tr_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
-               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+__device__ __forceinline__ void tr_tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+               "r"(r[6]), "r"(r[7])
                : "memory");
 }
 
@@ -376,7 +381,7 @@ __global__ void __launch_bounds__(kTrThreads, 1)
 tree_kernel(const CbTreeAttn p, const int part_rows) {
   using L = TreeLay<KBITS, VBITS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  TrSmem& sm = *reinterpret_cast<TrSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  TrSmem& sm = *reinterpret_cast<TrSmem*>(smem_raw + (-smem_u32(smem_raw) & 1023u));      // (by way of an integer it would be a generic address)
   uint8_t* raw = reinterpret_cast<uint8_t*>(&sm + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv;
   volatile uint32_t* abort_flag = &sm.abort_word;
@@ -470,7 +475,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       };
       auto publish = [&](int n) {                        // the CTA's n-th item; false: there is none
         TrItem& to = sm.list[n % kTrLists];
-        if (ok && n >= kTrLists) ok = mbar_wait_park(smem_u32(&sm.list_free[n % kTrLists]), (n / kTrLists - 1) & 1, abort_flag);
+        if (ok && n >= kTrLists) ok = tr_wait(smem_u32(&sm.list_free[n % kTrLists]), (n / kTrLists - 1) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return false;
         TrItem l;
@@ -517,7 +522,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           if (s < l.steps) {
             if (s > 0 && s % 8 == 0) ids = ids_later;
             const int b = gs % kTrRaw;
-            if (ok && gs >= kTrRaw) ok = mbar_wait_park(smem_u32(&sm.raw_free[b]), (gs / kTrRaw - 1) & 1, abort_flag);
+            if (ok && gs >= kTrRaw) ok = tr_wait(smem_u32(&sm.raw_free[b]), (gs / kTrRaw - 1) & 1, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int n = min(kTrPages, pages - (l.lo + s) * kTrPages);
@@ -549,7 +554,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
 #pragma unroll 1
       for (int it = 0;; ++it) {
         const TrItem& l = sm.list[it % kTrLists];
-        if (ok) ok = mbar_wait_park(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+        if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok || l.kvh < 0) break;
         const int steps = l.steps;
@@ -557,22 +562,26 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
         bool v_wide = false;
 #pragma unroll 1
         for (int s = 0; s < steps; ++s, visible -= kTrTok) {
-          if (ok) ok = mbar_wait_park(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag);
+          if (ok) ok = tr_wait(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const uint8_t* pages = raw + raw_at.i * kTrPages * L::stride;
-          uint32_t most[2], least[2];
+          uint32_t most[2] = {0u, 0u}, least[2] = {0u, 0u};
           bool odd = false;                              // some are not finite
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
+          const uint8_t* of = pages + L::vScale;
+#pragma unroll 1
+          for (int w = 1; w >= 0; --w) {                 // V, then K
             float4 scale[2];
-            pf_scales(pages + (w == 0 ? L::kScale : L::vScale), L::stride, visible, lane, scale);
-            most[w] = __reduce_max_sync(0xffffffffu, max(pf_most<false>(scale[0]), pf_most<false>(scale[1])));
-            if (most[w] >= 0x7F800000u) {
+            pf_scales(of, L::stride, visible, lane, scale);
+            of = pages + L::kScale;
+            most[1] = most[0];
+            least[1] = least[0];
+            most[0] = __reduce_max_sync(0xffffffffu, max(pf_most<false>(scale[0]), pf_most<false>(scale[1])));
+            if (__builtin_expect(most[0] >= 0x7F800000u, 0)) {
               odd = true;
-              most[w] = __reduce_max_sync(0xffffffffu, max(pf_most<true>(scale[0]), pf_most<true>(scale[1])));
+              most[0] = __reduce_max_sync(0xffffffffu, max(pf_most<true>(scale[0]), pf_most<true>(scale[1])));
             }
-            least[w] = __reduce_min_sync(0xffffffffu, min(tr_least(scale[0]), tr_least(scale[1])));
+            least[0] = __reduce_min_sync(0xffffffffu, min(tr_least(scale[0]), tr_least(scale[1])));
           }
           const int ek = pf_exponent(most[0]), ev = pf_exponent(most[1]), lk = pf_exponent(least[0]);
           const bool k_wide = lk < ek - kTrApart || ek > 100;
@@ -613,7 +622,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       uint32_t q_phase = 0;                              // bit = tile
       for (int it = 0;; ++it) {
         const TrItem& l = sm.list[it % kTrLists];
-        if (ok) ok = mbar_wait_park(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+        if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok || l.kvh < 0) break;
         const int steps = l.steps;
@@ -621,7 +630,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
 #pragma unroll 1
         for (int s = 0; s < steps; ++s, op.advance()) {
           const int b = op.i;
-          if (ok) ok = mbar_wait_park(smem_u32(is_s ? &sm.k_full[b] : &sm.v_full[b]), op.phase, abort_flag);
+          if (ok) ok = tr_wait(smem_u32(is_s ? &sm.k_full[b] : &sm.v_full[b]), op.phase, abort_flag);
 #pragma unroll
           for (int t = 0; t < kTrTiles; ++t) {
             if (split && (s & 1) != t) continue;
@@ -629,12 +638,12 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
             const uint32_t tile = tmem + t * kTrTmemTile;
             if (is_s) {
               if (first) {
-                if (ok) ok = mbar_wait_park(smem_u32(&sm.q_full[t]), q_phase >> t & 1, abort_flag);
+                if (ok) ok = tr_wait(smem_u32(&sm.q_full[t]), q_phase >> t & 1, abort_flag);
                 q_phase ^= 1u << t;
               }
-              if (ok) ok = mbar_wait_park(smem_u32(&sm.s_free[t]), s_phase >> t & 1, abort_flag);
+              if (ok) ok = tr_wait(smem_u32(&sm.s_free[t]), s_phase >> t & 1, abort_flag);
             } else {
-              if (ok) ok = mbar_wait_park(smem_u32(&sm.p_full[t]), s_phase >> t & 1, abort_flag);
+              if (ok) ok = tr_wait(smem_u32(&sm.p_full[t]), s_phase >> t & 1, abort_flag);
             }
             ok = __all_sync(0xffffffffu, ok);
             s_phase ^= 1u << t;
@@ -672,31 +681,31 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
 #pragma unroll 1
     for (int it = 0;; ++it) {
       const TrItem& l = sm.list[it % kTrLists];
-      if (ok) ok = mbar_wait_park(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+      if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok || l.kvh < 0) break;
       const int steps = l.steps;
       int visible = l.total - (l.lo + ahead) * kTrTok;
 #pragma unroll 1
       for (; ahead < steps; ahead += 2, visible -= 2 * kTrTok) {
-        if (ok) ok = mbar_wait_park(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag);
-        if (ok) ok = mbar_wait_park(smem_u32(&sm.note_full[note_at.i]), note_at.phase, abort_flag);
-        if (ok) ok = mbar_wait_park(smem_u32(&sm.k_free[op.i]), op.phase, abort_flag);
+        if (ok) ok = tr_wait(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag);
+        if (ok) ok = tr_wait(smem_u32(&sm.note_full[note_at.i]), note_at.phase, abort_flag);
+        if (ok) ok = tr_wait(smem_u32(&sm.k_free[op.i]), op.phase, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint8_t* pages = raw + raw_at.i * kTrPages * L::stride;
         const auto& note = sm.note[note_at.i];
         const float v_mul = note.v;
         const int v_wide = note.v_wide;
-        if (!note.k_wide) tr_convert_k<KBITS, VBITS, false>(sm.k[op.i], pages, note.k, ct);
+        if (__builtin_expect(!note.k_wide, 1)) tr_convert_k<KBITS, VBITS, false>(sm.k[op.i], pages, note.k, ct);
         else tr_convert_k<KBITS, VBITS, true>(sm.k[op.i], pages, note.k, ct);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sm.k_full[op.i]));
-        ok = mbar_wait_park(smem_u32(&sm.v_free[op.i]), op.phase, abort_flag);
+        ok = tr_wait(smem_u32(&sm.v_free[op.i]), op.phase, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (!v_wide) tr_convert_v<KBITS, VBITS, false>(sm.v[op.i], pages, visible, v_mul, ct);
+        if (__builtin_expect(!v_wide, 1)) tr_convert_v<KBITS, VBITS, false>(sm.v[op.i], pages, visible, v_mul, ct);
         else tr_convert_v<KBITS, VBITS, true>(sm.v[op.i], pages, visible, v_mul, ct);
         fence_proxy_async_smem();
         __syncwarp();
@@ -725,7 +734,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
     // the row of the thread in item `it`, and Q of its tile; false: no more items
     auto begin = [&](int it, Row& r) {
       const TrItem& l = sm.list[it % kTrLists];
-      if (ok) ok = mbar_wait_park(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+      if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       r.q = r.out = -1;
       r.sees = p.masks;
@@ -773,7 +782,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
     int note0 = 0, n = 0, exchanges = 0;                 // note of the item's first step; steps that this tile took part in; items in both tiles
     bool lent = false;                                   // the other tile may still read this one's output
     auto wait_lent = [&]() {
-      if (lent && ok) ok = mbar_wait_park(smem_u32(&sm.exch_free), (exchanges - 1) & 1, abort_flag);
+      if (lent && ok) ok = tr_wait(smem_u32(&sm.exch_free), (exchanges - 1) & 1, abort_flag);
       lent = false;
     };
     Row cur = {-1, -1, p.masks, 0.f};
@@ -792,10 +801,10 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
 #pragma unroll 1
         for (int s = first; s < steps; s += split ? 2 : 1) {
           const int tok0 = (l.lo + s) * kTrTok;
-          if (ok) ok = mbar_wait_park(smem_u32(&sm.s_full[t]), n & 1, abort_flag);
+          if (ok) ok = tr_wait(smem_u32(&sm.s_full[t]), n & 1, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
-          if (tok0 + kTrTok > start) {                   // what a row does not see: -inf in place of its scores
+          if (__builtin_expect(tok0 + kTrTok > start, 0)) {                   // what a row does not see: -inf in place of its scores
             const uint2 see = mine ? tr_visible(cur.sees, p.words, start, total, tok0) : make_uint2(0u, 0u);
 #pragma unroll 1
             for (int c = 0; c < 2; ++c) {
@@ -842,30 +851,30 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           const float use = m == -INFINITY ? 0.f : m;
           const float2 less = make_float2(-use, -use), mul2 = make_float2(mul, mul);
           // the previous product has read the probabilities and written the output
-          if (ok && s > first) ok = mbar_wait_park(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
+          if (ok && s > first) ok = tr_wait(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
           if (s == first) wait_lent();
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
           float2 part_sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t a[32], pr[16];
-            tmem_ld_32x32(tile + c * 32, a);
+          for (int c = 0; c < 4; ++c) {
+            uint32_t a[16], pr[8];
+            tmem_ld_32x16(tile + c * 16, a);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
+            for (int j = 0; j < 8; ++j) {
               const float2 d = __ffma2_rn(make_float2(__uint_as_float(a[2 * j]), __uint_as_float(a[2 * j + 1])), mul2, less);
               const float2 x = make_float2(fast_exp2(d.x), fast_exp2(d.y));
               part_sum[j & 1] = __fadd2_rn(part_sum[j & 1], x);
               pr[j] = pack_f16x2(x.x, x.y);
             }
-            tr_tmem_st16(tile + kTrTmemP + c * 16, pr);
+            tr_tmem_st8(tile + kTrTmemP + c * 8, pr);
           }
           sum += (part_sum[0].x + part_sum[0].y) + (part_sum[1].x + part_sum[1].y);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&sm.s_free[t]));
-          if (s > first && __any_sync(0xffffffffu, grew)) {
+          if (__builtin_expect(s > first && __any_sync(0xffffffffu, grew), 0)) {
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               uint32_t o[32];
@@ -895,7 +904,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           for (int j = 0; j < 16; ++j) reinterpret_cast<uint4*>(p.out + cur.out)[j] = make_uint4(0u, 0u, 0u, 0u);
         }
       } else {
-        if (ok && in) ok = mbar_wait_park(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
+        if (ok && in) ok = tr_wait(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         // what this tile's output and the other's are multiplied with
         float mul[2] = {pow2f(v_exp), 0.f};
@@ -907,7 +916,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&sm.exch_full));
-          if (ok) ok = mbar_wait_park(smem_u32(&sm.exch_full), exchanges & 1, abort_flag);
+          if (ok) ok = tr_wait(smem_u32(&sm.exch_full), exchanges & 1, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           ++exchanges;
           lent = true;
