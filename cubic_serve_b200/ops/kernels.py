@@ -1085,7 +1085,7 @@ def adjust_logits(logits: torch.Tensor, request: torch.Tensor | None, history: t
     packed = native.ADJUST.pack(
         logits.data_ptr(), out.data_ptr(), _vector(request, i32, rows, "request"), history.data_ptr(), _vector(length, i32, n, "length"), _vector(prompt, i32, n, "prompt"),
         _vector(repetition, f32, n, "repetition"), _vector(frequency, f32, n, "frequency"), _vector(presence, f32, n, "presence"), b[0], b[1], b[2],
-        0 if mask is None else mask.data_ptr(), *d, ldl, ldo, ldh, ldm, lds, rows, vocab, n, most, b[3], words, logits.dtype is f32, 0)
+        0 if mask is None else mask.data_ptr(), *d, ldl, ldo, ldh, ldm, lds, rows, vocab, n, most, b[3], words, logits.dtype is f32)
     if rows:
         _call("cb_adjust_logits", (packed,), (logits, out, request, history, length, prompt, repetition, frequency, presence, *(bias or ()), mask, *(drafts or ())))
     return out

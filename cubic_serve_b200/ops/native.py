@@ -573,7 +573,7 @@ VOCABULARY = struct.Struct("@PqPq11P4i")                     # CbVocabulary, csr
 TREE_ATTN = struct.Struct("@11P4q10if4x")                    # CbTreeAttn, csrc/tree_attn.cu
 VERIFY_TREE = struct.Struct("@8P3i4x")                       # CbVerifyTree, csrc/draft_tree.cu
 KEEP_TOKENS = struct.Struct("@7P2q9i4x")                     # CbKeepTokens, csrc/draft_tree.cu
-ADJUST = struct.Struct("@16P5q8i")                           # CbAdjust, csrc/adjust_logits.cu
+ADJUST = struct.Struct("@16P5q7i4x")                           # CbAdjust, csrc/adjust_logits.cu
 
 
 class ReduceNormStruct(ctypes.Structure):
