@@ -36,9 +36,9 @@ namespace cb {
 
 // A token's word: index of its bias + 1 (kAdjustFar: at least that), seen, count
 static constexpr uint32_t kAdjustFar = 2047u, kAdjustSeen = 1u << 11, kAdjustOne = 1u << 12;
-static constexpr int kAdjustThreads = 256, kAdjustVectors = 4, kAdjustBytes = kAdjustThreads * kAdjustVectors * 16;        // of a block's logits
+static constexpr int kAdjustBytes = 16384;               // of a block's logits
 
-static_assert(kAdjustBytes / 2 / 32 <= kAdjustThreads, "a word of marks for every thread");
+static_assert(kAdjustBytes / 2 / 32 <= 256, "a word of marks for every thread");
 static constexpr int kAdjustList = 1024, kAdjustAhead = 2;
 
 __device__ __forceinline__ float adjust_load(float v) { return v; }
@@ -46,10 +46,12 @@ __device__ __forceinline__ float adjust_load(__nv_bfloat16 v) { return __bfloat1
 __device__ __forceinline__ void adjust_store(float& to, float v) { to = v; }
 __device__ __forceinline__ void adjust_store(__nv_bfloat16& to, float v) { to = __float2bfloat16(v); }
 
-template <typename T>
-__global__ void __launch_bounds__(kAdjustThreads, 6)
+// THREADS: 256, so that six blocks of an SM have their latencies at different times, or 1024 where there are no more than two blocks an SM: then the trips through a
+// long history count (9 rows of 50257 behind 20000 tokens: 29 us by blocks of 256).
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1536 / THREADS)
 adjust_kernel(const CbAdjust p) {
-  constexpr int N = 16 / sizeof(T), kRange = kAdjustBytes / sizeof(T);
+  constexpr int N = 16 / sizeof(T), kRange = kAdjustBytes / sizeof(T), kVectors = kAdjustBytes / 16 / THREADS;
   __shared__ uint32_t table[kRange], marked[kRange / 32];
   __shared__ uint16_t list[kAdjustList];
   __shared__ int listed;
@@ -62,11 +64,11 @@ adjust_kernel(const CbAdjust p) {
   const int ahead = static_cast<int>(reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T), lo = blockIdx.x * kRange - ahead;
   if (lo >= p.vocab) return;
   const bool wide = (reinterpret_cast<uintptr_t>(out) & 15) == (reinterpret_cast<uintptr_t>(in) & 15), copies = in != out || p.mask != nullptr;
-  uint4 v[kAdjustVectors];
+  uint4 v[kVectors];
   if (copies) {
 #pragma unroll
-    for (int k = 0; k < kAdjustVectors; ++k) {
-      const int at = lo + (k * kAdjustThreads + tid) * N;
+    for (int k = 0; k < kVectors; ++k) {
+      const int at = lo + (k * THREADS + tid) * N;
       if (at >= 0 && at + N <= p.vocab) v[k] = *reinterpret_cast<const uint4*>(in + at);
     }
   }
@@ -83,7 +85,7 @@ adjust_kernel(const CbAdjust p) {
     if (p.frequency != nullptr) freq = p.frequency[r];
     if (p.presence != nullptr) pres = p.presence[r];
   }
-  for (int i = tid; i < kRange / 32; i += kAdjustThreads) marked[i] = 0;
+  for (int i = tid; i < kRange / 32; i += THREADS) marked[i] = 0;
   if (tid == 0) listed = 0;
   __syncthreads();
   const int* said = known ? p.history + r * p.ldh : p.history;
@@ -99,20 +101,20 @@ adjust_kernel(const CbAdjust p) {
     if (tid < first) one(said[tid], tid >= prompt);
     const int4* four = reinterpret_cast<const int4*>(said + first);
 #pragma unroll 1
-    for (int i0 = tid; i0 < fours; i0 += kAdjustAhead * kAdjustThreads) {
+    for (int i0 = tid; i0 < fours; i0 += kAdjustAhead * THREADS) {
       int4 t[kAdjustAhead];                                // loads in flight together (behind one another's atomics they would not be)
 #pragma unroll
-      for (int k = 0; k < kAdjustAhead; ++k) t[k] = i0 + k * kAdjustThreads < fours ? four[i0 + k * kAdjustThreads] : make_int4(-1, -1, -1, -1);
+      for (int k = 0; k < kAdjustAhead; ++k) t[k] = i0 + k * THREADS < fours ? four[i0 + k * THREADS] : make_int4(-1, -1, -1, -1);
 #pragma unroll
       for (int k = 0; k < kAdjustAhead; ++k) {
-        const int at = first + 4 * (i0 + k * kAdjustThreads);
+        const int at = first + 4 * (i0 + k * THREADS);
         one(t[k].x, at >= prompt); one(t[k].y, at + 1 >= prompt); one(t[k].z, at + 2 >= prompt); one(t[k].w, at + 3 >= prompt);
       }
     }
     const int rest = first + 4 * fours + tid;
     if (rest < length) one(said[rest], rest >= prompt);
     if (row0 >= 0)
-      for (int j = 1 + tid; j < 32 * p.words && j < p.rows - row0; j += kAdjustThreads)
+      for (int j = 1 + tid; j < 32 * p.words && j < p.rows - row0; j += THREADS)
         if (p.sees[row * p.lds + (j >> 5)] >> (j & 31) & 1u) one(p.draft[row0 + j], true);
   };
   auto mark = [&](int at, bool) {
@@ -122,7 +124,7 @@ adjust_kernel(const CbAdjust p) {
     table[at] = 0;
   };
   each(mark);
-  for (int e = b0 + tid; e < b1; e += kAdjustThreads) {
+  for (int e = b0 + tid; e < b1; e += THREADS) {
     const int token = p.bias_id[e];
     if (static_cast<unsigned>(token - from) < tokens) mark(token - lo, false);
   }
@@ -130,8 +132,8 @@ adjust_kernel(const CbAdjust p) {
   auto allowed = [&](int token) { return mask == nullptr || (mask[token >> 5] >> (token & 31) & 1u) != 0; };
   if (copies) {
 #pragma unroll
-    for (int k = 0; k < kAdjustVectors; ++k) {
-      const int at = lo + (k * kAdjustThreads + tid) * N;
+    for (int k = 0; k < kVectors; ++k) {
+      const int at = lo + (k * THREADS + tid) * N;
       if (at >= p.vocab || at + N <= 0) continue;
       if (at >= 0 && at + N <= p.vocab) {
         if (mask != nullptr) {
@@ -163,7 +165,7 @@ adjust_kernel(const CbAdjust p) {
   }
   __syncthreads();
   if (b1 > b0) {
-    for (int e = b0 + tid; e < b1; e += kAdjustThreads) {
+    for (int e = b0 + tid; e < b1; e += THREADS) {
       const int token = p.bias_id[e];
       if (static_cast<unsigned>(token - from) < tokens) atomicMax(table + (token - lo), min(static_cast<uint32_t>(e - b0) + 1u, kAdjustFar));
     }
@@ -207,9 +209,9 @@ adjust_kernel(const CbAdjust p) {
     adjust_store(out[token], x);
   };
   if (listed <= kAdjustList) {
-    for (int i = tid; i < listed; i += kAdjustThreads) adjust(list[i]);
+    for (int i = tid; i < listed; i += THREADS) adjust(list[i]);
   } else {                                                 // more than there is room for: all marked ones, a word a warp
-    for (int i = tid >> 5; i < kRange / 32; i += kAdjustThreads / 32)
+    for (int i = tid >> 5; i < kRange / 32; i += THREADS / 32)
       if (marked[i] >> (tid & 31) & 1u) adjust(32 * i + (tid & 31));
   }
 }
@@ -223,5 +225,16 @@ extern "C" int cb_adjust_logits(const CbAdjust* p, void* stream) {
   const int size = p->f32 ? 4 : 2, range = kAdjustBytes / size;
   const dim3 grid((p->vocab + 16 / size - 1 + range - 1) / range, p->rows);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return static_cast<int>(p->f32 ? launch(adjust_kernel<float>, grid, dim3(kAdjustThreads), 0, st, *p) : launch(adjust_kernel<__nv_bfloat16>, grid, dim3(kAdjustThreads), 0, st, *p));
+  static int sms[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -18;
+  if (!sms[dev]) {
+    int n = 0;
+    const cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    sms[dev] = n;
+  }
+  if (static_cast<long long>(grid.x) * grid.y <= 2 * sms[dev])
+    return static_cast<int>(p->f32 ? launch(adjust_kernel<float, 1024>, grid, dim3(1024), 0, st, *p) : launch(adjust_kernel<__nv_bfloat16, 1024>, grid, dim3(1024), 0, st, *p));
+  return static_cast<int>(p->f32 ? launch(adjust_kernel<float, 256>, grid, dim3(256), 0, st, *p) : launch(adjust_kernel<__nv_bfloat16, 256>, grid, dim3(256), 0, st, *p));
 }
