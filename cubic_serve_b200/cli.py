@@ -25,6 +25,7 @@ class SpeculativeConfig:
     mode: str = "fixed"            # fixed | dynamic
     max_tokens: int = 0
     policy: dict | None = None
+    branches: int = 1              # continuations of an n-gram draft, verified as one tree
 
 
 def parse_speculative_config(text: str | None) -> SpeculativeConfig:
@@ -44,7 +45,10 @@ def parse_speculative_config(text: str | None) -> SpeculativeConfig:
         raise argparse.ArgumentTypeError("mode must be fixed or dynamic")
     if cfg["method"] == "ngram" and mode != "fixed":
         raise argparse.ArgumentTypeError("n-gram drafts have no planned length: a request without a match drafts nothing")
-    return SpeculativeConfig(cfg["method"], n, mode, int(cfg.get("max_tokens", n)), cfg.get("policy"))
+    branches = cfg.get("branches", 1)
+    if not isinstance(branches, int) or isinstance(branches, bool) or not 1 <= branches <= 16 or branches > 1 and cfg["method"] != "ngram":
+        raise argparse.ArgumentTypeError("branches must be an integer in [1, 16], of n-gram drafts")
+    return SpeculativeConfig(cfg["method"], n, mode, int(cfg.get("max_tokens", n)), cfg.get("policy"), branches)
 
 
 def parse_devices(text: str | None) -> list[int]:

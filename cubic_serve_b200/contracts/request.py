@@ -99,6 +99,8 @@ class SamplingMeta:
     top_logprobs: int = 0
     whole_vocabulary: bool = False
     min_p: float = 0.0
+    repetition_penalty: float = 1.0
+    logit_bias: tuple[tuple[int, float], ...] = ()
 
     def __post_init__(self) -> None:
         if not 0.0 <= self.temperature <= 2.0:
@@ -109,6 +111,10 @@ class SamplingMeta:
             raise RequestError("min_p must be in [0, 1]", param="min_p")
         if not 0 <= self.top_k <= (2 ** 31 - 1 if self.whole_vocabulary or self.min_p > 0 else 20):
             raise RequestError("top_k must be between 0 and 20", param="top_k")
+        if not 0.0 < self.repetition_penalty <= 100.0:
+            raise RequestError("repetition_penalty must be in (0, 100]", param="repetition_penalty")
+        if len(self.logit_bias) > 1024 or any(t < 0 or not -100.0 <= v <= 100.0 for t, v in self.logit_bias):
+            raise RequestError("logit_bias must map up to 1024 tokens to numbers in [-100, 100]", param="logit_bias")
         if self.max_tokens is not None and self.max_tokens < 1:
             raise RequestError("max_tokens must be at least 1", param="max_tokens")
 

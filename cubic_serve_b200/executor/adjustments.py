@@ -1,0 +1,66 @@
+"""What requests say about their logits, on the device: token histories by request slot, penalties and biases (``K.adjust_logits``)."""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import numpy as np
+import torch
+
+
+@dataclass
+class Adjustment:
+    """Penalties and biases of one request (``runtime.scheduler.SamplingParams``), and the tokens that they look at."""
+    tokens: list[int]            # prompt and output so far
+    prompt: int                  # how many of them are the prompt's
+    repetition: float = 1.0
+    frequency: float = 0.0
+    presence: float = 0.0
+    bias: tuple[tuple[int, float], ...] = ()
+
+
+class Adjustments:
+    """Histories ``[slots, most]`` that grow with their requests: a step uploads the tokens that are new and a few numbers a slot.
+    ``stage`` is called on the stream of the steps; what it returns holds until the next call."""
+
+    def __init__(self, slots: int, most: int, device) -> None:
+        self.slots, self.most, self.device = slots, most, torch.device(device)
+        self.history = torch.zeros(slots, most, dtype=torch.int32, device=device)
+        self._have: list[tuple[int, int]] = [(-2, 0)] * slots          # whose tokens a row holds, and how many
+
+    def stage(self, segs, rows: list[int] | None = None) -> dict:
+        """Operands of ``K.adjust_logits`` for one row of logits a segment, or ``rows[i]`` neighbouring rows of segment i."""
+        n = self.slots
+        ints = np.zeros((2, n), dtype=np.int32)                        # length, prompt
+        floats = np.zeros((3, n), dtype=np.float32)                    # repetition, frequency, presence
+        floats[0] = 1.0
+        where, what, bias = [], [], {}
+        for s in segs:
+            a = s.adjust
+            if a is None:
+                continue
+            slot, L = s.request_slot, min(len(a.tokens), self.most)
+            uid, have = self._have[slot]
+            if uid != s.uid or s.uid < 0 or have > L:
+                have = 0
+            where.append(np.arange(slot * self.most + have, slot * self.most + L, dtype=np.int64))
+            what.append(np.asarray(a.tokens[have:L], dtype=np.int32))
+            self._have[slot] = (s.uid, L)
+            ints[:, slot] = L, min(a.prompt, L)
+            floats[:, slot] = a.repetition, a.frequency, a.presence
+            if a.bias:
+                bias[slot] = a.bias
+        each = rows or [1] * len(segs)
+        request = np.repeat(np.array([s.request_slot if s.adjust is not None else -1 for s in segs], dtype=np.int32), each)
+        up = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(self.device)             # noqa: E731 - (a copy from pageable memory has left it when the call returns)
+        where = np.concatenate(where) if where else np.zeros(0, dtype=np.int64)
+        if where.size:
+            self.history.view(-1).index_copy_(0, up(where), up(np.concatenate(what)))
+        ints, floats = up(ints), up(floats)
+        out = dict(request=up(request), history=self.history, length=ints[0], prompt=ints[1], repetition=floats[0], frequency=floats[1], presence=floats[2])
+        if bias:
+            count = np.zeros(n + 1, dtype=np.int32)
+            for slot, b in bias.items():
+                count[slot + 1] = len(b)
+            pairs = [p for slot in sorted(bias) for p in bias[slot]]
+            out["bias"] = (up(np.cumsum(count, dtype=np.int32)), up(np.array([t for t, _ in pairs], dtype=np.int32)), up(np.array([v for _, v in pairs], dtype=np.float32)))
+        return out

@@ -22,6 +22,7 @@ import torch
 
 from ..models.decoder import DecoderRunner, StepBatch
 from ..ops import kernels as K
+from .adjustments import Adjustment, Adjustments
 from .graph_runtime import CudaGraphRuntime, GraphState
 
 log = logging.getLogger(__name__)
@@ -60,6 +61,7 @@ class Segment:
     whole: bool = False
     min_p: float = 0.0
     adapter: int = -1            # slot of the request's low-rank adapter, -1 = none
+    adjust: Adjustment | None = None     # penalties and biases of the sampled row's logits
 
 
 class _Staging:
@@ -433,6 +435,9 @@ class GpuExecutor:
         assert self.max_tokens <= runner.max_tokens
         if runner.cfg.is_hybrid and max_rows > runner.max_requests:
             raise ValueError("the runner's recurrent state has fewer rows than the executor has request slots")
+        # penalties and biases likewise: a row's logits on one GPU, and drafts that are verified against them where rounds do that
+        self.accepts_adjustments = self.accepts_vocabulary_draws
+        self._adjustments = None
         # the low-rank adapters that requests may name (speculative rounds compute and verify without)
         self.low_rank = getattr(runner, "low_rank", None) if type(self) is GpuExecutor else None
         self.builder = BatchBuilder(max_rows * rows_per_request, self.max_tokens, max_model_len,
@@ -531,6 +536,21 @@ class GpuExecutor:
         self.stage.d["mask"] = self._mask_dev
         self.h2d_mask_bytes_last = n * words * 4
         return True
+
+    def _stage_adjustments(self, segs: list[Segment]) -> int:
+        """Stage the penalties and biases of this step's sampled rows; returns how many rows have some."""
+        self.stage.d.pop("adjust", None)
+        wanted = [s for s in segs if s.sample]
+        n = sum(s.adjust is not None for s in wanted)
+        if n:
+            with torch.cuda.stream(self.stream):
+                self.stage.d["adjust"] = self._request_adjustments().stage(wanted)
+        return n
+
+    def _request_adjustments(self) -> Adjustments:
+        if self._adjustments is None:
+            self._adjustments = Adjustments(self.max_rows, self.builder.max_pages * K.PAGE_TOKENS, self.device)
+        return self._adjustments
 
     def _stage_whole(self, segs: list[Segment]) -> int:
         """Stage which sampled rows draw from the whole vocabulary; returns how many."""
@@ -684,7 +704,7 @@ class GpuExecutor:
         if self.runner.tp is not None or self.runner.pp is not None:
             raise NotImplementedError("logits of chosen positions are read on one GPU")
         if self.use_graphs and all(len(s.token_ids) == 1 for s in segs) and self.graph_rt.dispatch(len(segs)) is not None:
-            self.collect(self.launch([replace(s, sample=True, temperature=0.0, mask=None) for s in segs]))
+            self.collect(self.launch([replace(s, sample=True, temperature=0.0, mask=None, adjust=None) for s in segs]))
             got = self.logits[:len(segs)].float().cpu().numpy()
             return [got[i:i + 1] if s.logit_offsets else got[:0] for i, s in enumerate(segs)]
         if self._upload_pending:
@@ -727,8 +747,9 @@ class GpuExecutor:
         masked = self._stage_masks(segs)
         whole = True in [s.whole for s in segs]
         decode = (all(len(s.token_ids) == 1 for s in segs) and self.use_graphs and (self.graph_masks or not masked))
+        adjusts = any(s.adjust is not None for s in segs)
         # the budgets' state machine runs on the ids of the draw, inside the step
-        decode = decode and not (whole and self.runner.reasoning is not None)
+        decode = decode and not ((whole or adjusts) and self.runner.reasoning is not None)
         cap = self.graph_rt.dispatch(total) if decode else None
         if self._upload_pending:
             # the pinned staging buffer is rewritten below: the previous launch's upload must have left it
@@ -738,6 +759,7 @@ class GpuExecutor:
         b, rows = self._fill(segs, pad_rows_to=cap, lengths=True) if laid_out else self._fill(segs, pad_rows_to=cap)
         given = self.builder.stage_layout(segs) if laid_out else 0
         whole = self._stage_whole(segs) if whole or "whole" in self.stage.d else 0
+        adjusts = self._stage_adjustments(segs) if adjusts or "adjust" in self.stage.d else 0
         poisoned = cap is not None and getattr(self, "audit_poison_padding", False)
         if poisoned:
             self._poison_padding(total, cap)
@@ -767,6 +789,8 @@ class GpuExecutor:
                 self._ev[k][0].record(self.stream)
             if cap is not None:
                 launches = self.graph_rt.replay(cap, self._leases[k]).launches
+                if adjusts:                    # behind the graph, whose sampler drew from the logits as they are
+                    launches += self.runner.adjust_and_draw(self.stage.d, self.logits, self.out_ids, rows)
                 if whole:                      # behind the graph, whose sampler drew these rows from the 20 best
                     self.runner.draw_whole(self.stage.d, self.logits, self.out_ids, rows)
                     launches += 1

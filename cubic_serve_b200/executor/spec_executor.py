@@ -566,3 +566,115 @@ class NgramSpeculativeGpuExecutor(SpeculativeGpuExecutor):
         self.h2d_bytes_last += R * Kd * 4
         self.d2h_bytes_last = R * (Kd + 2) * 4
         return out
+
+
+class NgramTreeSpeculativeGpuExecutor(NgramSpeculativeGpuExecutor):
+    """Rounds whose drafts branch: up to ``branches`` continuations from the request's own history, merged where they begin alike
+    (``runtime/trees.py``), are reviewed in one target pass -- every draft sees the context and the drafts that lead to it -- and the
+    path that the target agrees with is kept: its keys and values move up behind the context.  Penalties and biases apply to every
+    row with the drafts above it counted as output, so that a round emits what single steps would."""
+
+    def __init__(self, runner, depth: int, branches: int, **kw) -> None:
+        if not 1 <= depth * branches < K.TREE_MAX_NODES:
+            raise ValueError(f"a tree holds up to {K.TREE_MAX_NODES - 1} drafts")
+        if getattr(runner, "tp", None) is not None or getattr(runner, "pp", None) is not None:
+            raise NotImplementedError("drafts in trees are reviewed on one GPU")
+        nodes = 1 + depth * branches
+        kw["max_model_len"] = kw.get("max_model_len", 4096) + nodes          # drafts lie behind a request's last position for the length of a round
+        super().__init__(runner, nodes - 1, **kw)
+        self.draft_depth, self.draft_branches = depth, branches
+        self.accepts_adjustments = True
+        self.words = -(-nodes // 32)
+        self.caches = K.LayerCaches(list(runner.kv), runner.hkv, runner.D, runner.k_bits, runner.v_bits)
+        rows, dev = self.max_rows, self.device
+        # int32 operands of a round, staged together: by row tokens, parents and masks; by request its row of the page table, first row, nodes and context
+        self._tree_sizes = [("tokens", rows * nodes), ("parents", rows * nodes), ("masks", rows * nodes * self.words), ("request", rows), ("row0", rows), ("count", rows), ("start", rows)]
+        total = sum(n for _, n in self._tree_sizes)
+        self._tree_host = torch.zeros(total, dtype=torch.int32, pin_memory=torch.cuda.is_available())
+        self._tree_dev = torch.zeros(total, dtype=torch.int32, device=dev)
+        # target's choices by row, then what the host reads back: accepted drafts, and the choices along the path
+        self._choices = torch.zeros(rows * nodes, dtype=torch.int32, device=dev)
+        self._back = torch.zeros(rows * (depth + 2), dtype=torch.int32, device=dev)
+        self._path = torch.zeros(rows, depth + 1, dtype=torch.int32, device=dev)
+        self._after_current_stream()
+
+    def execute_speculative(self, segs: list[Segment], depths: list[int] | None = None, drafts: list[list[list[int]]] | None = None):
+        """``drafts[i]``: continuations for request ``i``, the likeliest first (possibly none).  Returns per request the emitted tokens."""
+        from ..runtime.trees import merge_drafts, tree_depths, tree_masks
+        R = len(segs)
+        most = min(self.speculative_depth, self.max_tokens // max(R, 1) - 1)              # (rows of a pass)
+        trees = []
+        for i, (s, d) in enumerate(zip(segs, drafts or [[]] * R)):
+            k = self.draft_depth if depths is None else max(0, min(self.draft_depth, int(depths[i])))
+            room = len(s.pages) * K.PAGE_TOKENS - s.start - 1                # slots that the request has pages for
+            trees.append(merge_drafts([c[:k] for c in d], max(0, min(most, room))))
+        counts = [len(t) for t, _ in trees]
+        if max(counts, default=1) == 1:
+            ids = self.execute(segs)
+            self.last_round = {"depth": 0, "accepted": [0] * R, "proposed": [0] * R, "proposal_ms": 0.0,
+                               "target_ms": self.device_ms[-1] if (self.timing and self.device_ms) else 0.0}
+            return [[int(t)] for t in ids]
+        T, W, D = sum(counts), self.words, self.draft_depth
+        if self._upload_pending:
+            self._uploaded.synchronize()                                     # a plain step's staging upload may still be in flight
+            self._upload_pending = False
+        h, at, off = self._tree_host.numpy(), {}, 0
+        for name, _ in self._tree_sizes:                                     # compact: one copy takes what is in use
+            n = R if name in ("request", "row0", "count", "start") else T * W if name == "masks" else T
+            at[name] = (off, off + n)
+            off += -(-n // 4) * 4
+        put = lambda name, v: h.__setitem__(slice(*at[name]), v)             # noqa: E731
+        tokens = np.concatenate([np.array([int(s.token_ids[0])] + t[1:], dtype=np.int32) for s, (t, _) in zip(segs, trees)])
+        put("tokens", tokens)
+        put("parents", np.concatenate([np.array(p, dtype=np.int32) for _, p in trees]))
+        put("masks", np.concatenate([tree_masks(p, W) for _, p in trees]).view(np.int32).reshape(-1))
+        put("request", [s.request_slot for s in segs])
+        row0 = np.concatenate([[0], np.cumsum(counts)[:-1]])
+        put("row0", row0)
+        put("count", counts)
+        put("start", [s.start for s in segs])
+        review = [Segment(s.request_slot, [int(x) for x in tokens[r:r + c]], s.start, s.pages, True, uid=s.uid) for s, r, c in zip(segs, row0, counts)]
+        b, _ = self._fill(review, review=True)
+        self.stage.h["positions"][:T] = np.concatenate([s.start + tree_depths(p) for s, (_, p) in zip(segs, trees)])
+        b.logit_rows, b.num_logit_rows = self.stage.d["logit_rows"], T
+        self.stage.h["logit_rows"][:T] = np.arange(T)
+        with torch.cuda.stream(self.stream):
+            ev0, ev1 = self._ev[0]
+            if self.timing:
+                ev0.record(self.stream)
+            self._tree_dev[:off].copy_(self._tree_host[:off], non_blocking=True)
+            d = {name: self._tree_dev[lo:hi] for name, (lo, hi) in at.items()}
+            masks = d["masks"].view(T, W)
+            self.h2d_bytes_last = self.stage.upload() + 4 * off
+            b.trees = (d["request"], d["row0"], d["count"], d["start"], masks)
+            hidden = self.runner.forward_hidden(b)
+            logits = self.runner.forward_logits(b, hidden, self._review_logits(T))
+            if any(s.adjust is not None for s in segs):
+                wants = self._request_adjustments().stage(segs, counts)
+                first = torch.zeros(self._adjustments.slots, dtype=torch.int32, device=self.device)          # first row, by request slot
+                first.index_copy_(0, d["request"].long(), d["row0"])
+                K.adjust_logits(logits[:T], drafts=(d["tokens"], masks, first), **wants)
+            choices, accepted = self._choices[:T], self._back[:R]
+            emitted, path = self._back[R:R * (D + 2)].view(R, D + 1), self._path[:R]
+            self._sample_greedy(logits, T, choices)
+            K.verify_tree(choices, d["tokens"], d["parents"], d["row0"], d["count"], accepted, path, emitted)
+            K.keep_tokens(self.caches, b.page_table, d["request"], d["start"], accepted, path, ws=self.runner.ws)
+            if self.timing:
+                ev1.record(self.stream)
+            back = self._back[:R * (D + 2)].cpu().numpy()
+            self.stream.synchronize()
+        tgt_ms = 0.0
+        if self.timing:
+            tgt_ms = ev0.elapsed_time(ev1)
+            self.device_ms.append(tgt_ms)
+        acc, em = back[:R], back[R:].reshape(R, D + 1)
+        out = [[int(t) for t in em[i, :acc[i] + 1]] for i in range(R)]
+        proposed = [c - 1 for c in counts]
+        self.stats["accepted"] += int(acc.sum())
+        self.stats["emitted"] += int(acc.sum()) + R
+        self.stats["rounds"] += 1
+        self.stats["proposed"] += sum(proposed)
+        self.last_round = {"depth": D, "accepted": [int(a) for a in acc], "proposed": proposed, "proposal_ms": 0.0, "target_ms": tgt_ms}
+        self.kernel_launches_last = self.runner.launches_per_step + 3
+        self.d2h_bytes_last = R * (D + 2) * 4
+        return out

@@ -27,7 +27,7 @@ from pathlib import Path
 from ..runtime.scheduler import SamplingParams
 
 _SAMPLING_FIELDS = ("temperature", "top_p", "top_k", "seed", "max_tokens", "stop_token_ids", "ignore_eos", "thinking_budget",
-                    "whole_vocabulary", "min_p", "adapter")
+                    "whole_vocabulary", "min_p", "adapter", "repetition_penalty", "frequency_penalty", "presence_penalty", "logit_bias")
 
 
 @dataclass

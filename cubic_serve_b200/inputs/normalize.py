@@ -160,6 +160,17 @@ def _openai_structured(body: dict) -> StructuredOutput:
     raise RequestError(f"unsupported response_format type {rf['type']!r}", param="response_format")
 
 
+def _logit_bias(body) -> tuple[tuple[int, float], ...]:
+    """``logit_bias`` of a request: an object of token ids and numbers."""
+    bias = body.get("logit_bias") or {}
+    _require(isinstance(bias, dict), "logit_bias must be an object", "logit_bias")
+    out = []
+    for t, v in bias.items():
+        _require(isinstance(t, str) and t.isdecimal() and isinstance(v, (int, float)) and not isinstance(v, bool), "logit_bias maps token ids to numbers", "logit_bias")
+        out.append((int(t), float(v)))
+    return tuple(out)
+
+
 def normalize_openai_chat_completions(body: Any, default_model: str | None = None,
                                       sampling_defaults: dict | None = None) -> CanonicalChatRequest:
     _require(isinstance(body, dict), "request body must be a JSON object")
@@ -213,7 +224,7 @@ def normalize_openai_chat_completions(body: Any, default_model: str | None = Non
         presence_penalty=float(_as_number(body, "presence_penalty", 0.0, -2.0, 2.0)),
         frequency_penalty=float(_as_number(body, "frequency_penalty", 0.0, -2.0, 2.0)),
         logprobs=bool(body.get("logprobs", False)), top_logprobs=tlp,
-        whole_vocabulary=whole, min_p=min_p)
+        whole_vocabulary=whole, min_p=min_p, repetition_penalty=float(_as_number(body, "repetition_penalty", 1.0)), logit_bias=_logit_bias(body))
     tools, choice = _openai_tools(body)
     structured = _openai_structured(body)
     _require(not (structured.kind != StructuredKind.NONE and choice.mode in ("required", "named")),

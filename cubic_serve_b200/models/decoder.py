@@ -274,6 +274,7 @@ class StepBatch:
     # the temporal axis) and encoder feature rows ``[(first row, bf16 [n, H])]`` that replace token embeddings
     positions_hw: tuple | None = None
     embeds: list | None = None
+    trees: tuple | None = None   # a pass over trees of drafts: request, row0, count, start, masks of ``K.tree_attention`` in place of row blocks
     row_adapters: torch.Tensor | None = None     # int32 [T] adapter slot of every row, -1 = none (decoders with low-rank adapters)
 
 
@@ -447,6 +448,12 @@ class DecoderRunner(StepRunner):
     def _attend(self, b: StepBatch, q: torch.Tensor, out: torch.Tensor, kv: torch.Tensor, rb0: int, rb1: int) -> int:
         """Attention of the row blocks ``[rb0, rb1)``: portions of prompts in one launch, what is before and after them in
         one each.  Returns the launches."""
+        if b.trees is not None:
+            request, row0, count, start, masks = b.trees
+            rows = q.shape[0]
+            K.tree_attention(q.view(rows, -1), out.view(rows, -1), kv, b.page_table, request, row0, count, start, masks, self.hq, self.hkv, self.D, self.k_bits,
+                             self.v_bits, scale=self.cfg.attention_scale, ws=self.ws)
+            return 2
         lo, hi = max(b.attn_prompts[0], rb0), min(b.attn_prompts[1], rb1)
         if lo >= hi:
             lo = hi = rb1

@@ -40,12 +40,23 @@ class StepRunner:
         """Whole step: layers, final norm, lm_head, sampling (and the cross-rank token agreement under TP), then the
         thinking-budget state machine on the sampled ids when it is enabled."""
         self._run_step(b, d, logits_buf, out_ids)
+        if d.get("adjust") is not None and b.num_logit_rows:
+            self.launches_per_step += self.adjust_and_draw(d, logits_buf, out_ids, b.num_logit_rows)
         if d.get("whole") is not None and b.num_logit_rows:
             self.draw_whole(d, logits_buf, out_ids, b.num_logit_rows)
             self.launches_per_step += 1
         if self.reasoning is not None and b.num_logit_rows:
             self.reasoning.apply(out_ids, d["row_slot"], d["budget_init"], b.num_logit_rows)
             self.launches_per_step += 1
+
+    def adjust_and_draw(self, d: dict, logits_buf: torch.Tensor, out_ids: torch.Tensor, rows: int) -> int:
+        """Adjust the logits of the rows whose requests want it (``d["adjust"]``: the operands of ``K.adjust_logits``) and draw all rows again:
+        the others' come out the same.  Returns the launches."""
+        logits = K.adjust_logits(logits_buf[:rows], **d["adjust"])
+        mask = d.get("mask")
+        K.sample(logits, out_ids[:rows], temperature=d["temperature"][:rows], top_p=d["top_p"][:rows], top_k=d["top_k"][:rows], seeds=d["seeds"][:rows],
+                 counters=d["draws"][:rows], vocab=logits.shape[1], mask=None if mask is None else mask[:rows])
+        return 2
 
     def draw_whole(self, d: dict, logits_buf: torch.Tensor, out_ids: torch.Tensor, rows: int) -> None:
         """Draw the rows ``d["whole"]`` again, from the whole vocabulary, by the stream that the sampler drew them with."""

@@ -144,6 +144,10 @@ class TokenChatBackend:
         sp = SamplingParams(temperature=s.temperature, top_p=s.top_p, top_k=s.top_k, seed=s.seed, max_tokens=max_tokens,
                             stop_token_ids=tuple(s.stop_token_ids) + ((eos,) if eos is not None else ()),
                             matcher=matcher, adapter=req.model if req.model in self.adapter_names else None, whole_vocabulary=s.whole_vocabulary, min_p=s.min_p,
+                            repetition_penalty=s.repetition_penalty, logit_bias=s.logit_bias,
+                            # (executors that do not adjust logits have always left these two aside)
+                            **({"frequency_penalty": s.frequency_penalty, "presence_penalty": s.presence_penalty}
+                               if getattr(self.engine.executor, "accepts_adjustments", False) else {}),
                             thinking_budget=req.reasoning.budget_tokens if prepared.starts_in_reasoning else None)
         with self._lock:
             self._live[req.request_id] = live

@@ -16,6 +16,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
+from ..executor.adjustments import Adjustment
 from ..executor.gpu_executor import Segment
 from .cache.pool import PagePool
 from .cache.prefix import PrefixCache
@@ -92,6 +93,12 @@ class LLMEngine:
                 raise AdmissionError("the media positions do not cover the prompt", status=400)
         if sampling is not None and sampling.draws_whole and not getattr(self.executor, "accepts_vocabulary_draws", False):
             raise AdmissionError("this executor draws from the 20 best tokens only; whole_vocabulary and min_p are not accepted", status=400)
+        if sampling is not None and sampling.adjusts:
+            if not getattr(self.executor, "accepts_adjustments", False):
+                raise AdmissionError("this executor does not adjust logits; penalties and logit_bias are not accepted", status=400)
+            vocab = getattr(getattr(self.executor, "cfg", None), "vocab_size", 0)
+            if any(t >= vocab for t, _ in sampling.logit_bias):
+                raise AdmissionError(f"logit_bias names tokens outside the vocabulary of {vocab}", status=400)
         rid = request_id or f"req-{next(self._ids)}"
         if rid in self.requests:
             raise AdmissionError(f"duplicate request id {rid}")
@@ -204,7 +211,7 @@ class LLMEngine:
             self._ahead_stale = False
             return False
         return bool(plan.segments) and not plan.copies and not plan.finished and not plan.state_restores and all(
-            s.count == 1 and s.sample and s.request.sampling.matcher is None for s in plan.segments)
+            s.count == 1 and s.sample and s.request.sampling.matcher is None and not s.request.sampling.adjusts for s in plan.segments)
 
     def _segments(self, plan: BatchPlan, ahead: bool = False) -> list:
         """Executor segments of a plan.  ``ahead``: the plan is a look-ahead step whose input tokens are not known on
@@ -225,6 +232,8 @@ class LLMEngine:
                                 r.draws + (1 if ahead else 0), (r.arrival << 16) | (r.preemptions & 0xFFFF), mask,
                                 self._budget_init(r) if s.sample and end_id is not None else -2, mask_fn))
             segs[-1].adapter = r.adapter_slot
+            if s.sample and sp.adjusts:
+                segs[-1].adjust = Adjustment(r.tokens, len(r.prompt), sp.repetition_penalty, sp.frequency_penalty, sp.presence_penalty, sp.logit_bias)
             if sp.draws_whole:
                 segs[-1].whole, segs[-1].min_p = True, sp.min_p
             if r.multimodal is not None:
@@ -378,12 +387,14 @@ class LLMEngine:
         token limit still allows."""
         if self.ngram is None:
             from .ngram import NgramProposer
-            self.ngram = NgramProposer()
+            self.ngram = NgramProposer(positions=getattr(self.executor, "draft_branches", 1))
+        max_depth = getattr(self.executor, "draft_depth", max_depth)
         drafts = []
         for s in plan.segments:
             r = s.request
             room = max(0, r.sampling.max_tokens - len(r.output) - 1)
-            drafts.append(self.ngram.propose(r.request_id, r.tokens, min(max_depth, room)))
+            k = min(max_depth, room)
+            drafts.append(self.ngram.propose(r.request_id, r.tokens, k) if self.ngram.positions == 1 else self.ngram.propose_many(r.request_id, r.tokens, k))
         return self.executor.execute_speculative(segs, drafts=drafts)
 
     def generate(self, prompts: list[list[int]], sampling: SamplingParams | None = None) -> list[list[int]]:

@@ -53,12 +53,30 @@ class SamplingParams:
     min_p: float = 0.0
     # the low-rank adapter that the request's tokens are computed with (``models/low_rank.py``); None = the model alone
     adapter: str | None = None
+    # what the logits are before a token is drawn (``ops.kernels.adjust_logits``): those of the prompt's and the output's tokens divided (above
+    # 0) or multiplied (else) by ``repetition_penalty``, those of tokens that the output holds c times lowered by
+    # c * frequency_penalty + presence_penalty, and ``logit_bias``, pairs of a token and what is added to it
+    repetition_penalty: float = 1.0
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+    logit_bias: tuple[tuple[int, float], ...] = ()
 
     @property
     def draws_whole(self) -> bool:
         return self.temperature > 0 and (self.whole_vocabulary or self.min_p > 0)
 
+    @property
+    def adjusts(self) -> bool:
+        """Whether the request's logits are adjusted at all."""
+        return self.repetition_penalty != 1.0 or self.frequency_penalty != 0.0 or self.presence_penalty != 0.0 or bool(self.logit_bias)
+
     def validate(self) -> None:
+        if not 0.0 < self.repetition_penalty <= 100.0:
+            raise ValueError("repetition_penalty must be in (0, 100]")
+        if not (-2.0 <= self.frequency_penalty <= 2.0 and -2.0 <= self.presence_penalty <= 2.0):
+            raise ValueError("frequency_penalty and presence_penalty must be in [-2, 2]")
+        if len(self.logit_bias) > 1024 or any(t < 0 or not -100.0 <= v <= 100.0 for t, v in self.logit_bias):
+            raise ValueError("logit_bias must be up to 1024 pairs of a token and a number in [-100, 100]")
         if not 0.0 <= self.temperature <= 2.0:
             raise ValueError("temperature must be in [0, 2]")
         if not 0.0 < self.top_p <= 1.0:

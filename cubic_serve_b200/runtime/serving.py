@@ -196,9 +196,10 @@ def build_backend(args, devices: list[int], tp: int, spec, k_bits: int, v_bits: 
         depth = getattr(spec, "num_speculative_tokens", 0) if spec is not None else 0
         if depth and getattr(spec, "method", "mtp") == "ngram":
             # prompt-lookup drafts: no draft model; steps without a draft replay the decode graphs
-            from ..executor.spec_executor import NgramSpeculativeGpuExecutor
-            executor = NgramSpeculativeGpuExecutor(runner, depth, max_rows=args.max_running_requests,
-                                                   max_prefill_tokens=args.token_budget, max_model_len=max_len)
+            from ..executor.spec_executor import NgramSpeculativeGpuExecutor, NgramTreeSpeculativeGpuExecutor
+            branches = getattr(spec, "branches", 1)
+            kw = dict(max_rows=args.max_running_requests, max_prefill_tokens=args.token_budget, max_model_len=max_len)
+            executor = NgramSpeculativeGpuExecutor(runner, depth, **kw) if branches == 1 else NgramTreeSpeculativeGpuExecutor(runner, depth, branches, **kw)
             caps = executor.capture_decode_graphs()
             log.info("n-gram speculative decoding: depth %d; decode graphs %s; %d KV pages", depth, caps, pages)
         elif depth:

@@ -402,7 +402,7 @@ class _Wishes:
 
 
 @pytest.mark.parametrize("f32", [False, True])
-@pytest.mark.parametrize("rows,vocab,n,most", [(1, 1000, 1, 50), (5, 33, 3, 40), (3, 1, 2, 9), (9, 50257, 4, 3000), (2, 151936, 2, 700), (40, 8192, 40, 1), (3, 8193, 3, 2000), (2, 100, 2, 0)])
+@pytest.mark.parametrize("rows,vocab,n,most", [(1, 1000, 1, 50), (5, 33, 3, 40), (3, 1, 2, 9), (9, 50257, 4, 3000), (2, 151936, 2, 700), (40, 8192, 40, 1), (3, 8193, 3, 2000), (2, 100, 2, 0), (300, 9000, 50, 60)])
 def test_logits_as_requests_want_them(rows, vocab, n, most, f32):
     _Wishes(rows, vocab, n, most, f32, seed=rows + vocab, bias=30, masked=True).check()
     _Wishes(rows, vocab, n, most, f32, seed=rows + vocab + 1, bias=5).check()

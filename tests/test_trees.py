@@ -114,3 +114,74 @@ def test_keep_tokens_refuses(change):
     a.update(change)
     with pytest.raises(ValueError):
         K.keep_tokens(**a)
+
+
+# ------------------------------------------------------------------------------------------------- what requests say
+def test_requests_say_what_their_logits_are():
+    from cubic_serve_b200.contracts.request import RequestError
+    from cubic_serve_b200.inputs.normalize import normalize_openai_chat_completions
+    body = {"model": "m", "messages": [{"role": "user", "content": "hi"}]}
+    s = normalize_openai_chat_completions({**body, "repetition_penalty": 1.2, "presence_penalty": 0.5, "logit_bias": {"17": -100, "4": 2.5}}).sampling
+    assert (s.repetition_penalty, s.presence_penalty, s.logit_bias) == (1.2, 0.5, ((17, -100.0), (4, 2.5)))
+    s = normalize_openai_chat_completions(body).sampling
+    assert (s.repetition_penalty, s.logit_bias) == (1.0, ())
+    for bad in ({"repetition_penalty": 0}, {"repetition_penalty": -1}, {"logit_bias": [1]}, {"logit_bias": {"a": 1}}, {"logit_bias": {"-3": 1}}, {"logit_bias": {"3": "1"}},
+                {"logit_bias": {"3": 101}}, {"logit_bias": {str(i): 0 for i in range(1025)}}, {"logit_bias": {"3": float("nan")}}):
+        with pytest.raises(RequestError):
+            normalize_openai_chat_completions({**body, **bad})
+
+
+def test_sampling_parameters_of_adjustments():
+    from cubic_serve_b200.runtime.scheduler import SamplingParams
+    assert not SamplingParams().adjusts and SamplingParams(presence_penalty=0.1).adjusts and SamplingParams(logit_bias=((1, 2.0),)).adjusts
+    for bad in (dict(repetition_penalty=0.0), dict(frequency_penalty=2.5), dict(presence_penalty=-3.0), dict(logit_bias=((-1, 0.0),)), dict(logit_bias=((1, 101.0),)),
+                dict(logit_bias=tuple((i, 0.0) for i in range(1025)))):
+        with pytest.raises(ValueError):
+            SamplingParams(**bad).validate()
+
+
+def test_histories_are_staged_as_they_grow():
+    from types import SimpleNamespace as S
+
+    from cubic_serve_b200.executor.adjustments import Adjustment, Adjustments
+    a = Adjustments(4, 10, "cpu")
+    tokens = [5, 6, 7]
+    seg = S(request_slot=2, uid=9, adjust=Adjustment(tokens, 2, 1.5, 0.5, 0.25, ((3, 1.0), (8, -2.0))))
+    none = S(request_slot=1, uid=4, adjust=None)
+    d = a.stage([none, seg])
+    assert d["request"].tolist() == [-1, 2] and d["length"].tolist() == [0, 0, 3, 0] and d["prompt"].tolist() == [0, 0, 2, 0]
+    assert d["history"][2, :3].tolist() == tokens and d["repetition"].tolist() == [1.0, 1.0, 1.5, 1.0] and d["presence"][2].item() == 0.25
+    assert d["bias"][0].tolist() == [0, 0, 0, 2, 2] and d["bias"][1].tolist() == [3, 8] and d["bias"][2].tolist() == [1.0, -2.0]
+    tokens += [8, 9]
+    assert a.stage([seg], [3])["request"].tolist() == [2, 2, 2] and a.history[2, :5].tolist() == tokens
+    other = S(request_slot=2, uid=10, adjust=Adjustment([1], 1))                              # another request in the slot
+    d = a.stage([other])
+    assert d["length"][2].item() == 1 and a.history[2, 0].item() == 1 and "bias" not in d
+    long = S(request_slot=0, uid=11, adjust=Adjustment(list(range(14)), 12))                  # longer than there is room for
+    assert a.stage([long])["length"][0].item() == 10
+
+
+def test_several_continuations_of_a_history():
+    from cubic_serve_b200.runtime.ngram import NgramIndex, NgramProposer
+    x = NgramIndex(3, 1, 4)
+    x.extend([1, 2, 3, 1, 2, 4, 1, 2, 5, 1, 2])
+    assert x.propose(2) == [5, 1] and x.propose_many(2) == [[5, 1], [4, 1], [3, 1]] and x.propose_many(0) == []
+    y = NgramIndex(3, 1, 2)
+    y.extend([1, 2, 3, 1, 2, 4, 1, 2, 5, 1, 2])
+    assert y.propose_many(3) == [[5, 1, 2], [4, 1, 2]]
+    p = NgramProposer(positions=3)
+    assert p.propose_many("a", [1, 2, 9, 1, 2], 2) == [[9, 1]] and p.propose("a", [1, 2, 9, 1, 2], 2) == [9, 1]
+    with pytest.raises(ValueError):
+        NgramIndex(positions=0)
+
+
+def test_branches_on_the_command_line():
+    import argparse
+
+    from cubic_serve_b200.cli import parse_speculative_config
+    assert parse_speculative_config('{"method":"ngram","num_speculative_tokens":4,"branches":3}').branches == 3
+    assert parse_speculative_config('{"method":"ngram","num_speculative_tokens":4}').branches == 1
+    for bad in ('{"method":"ngram","num_speculative_tokens":4,"branches":0}', '{"method":"ngram","num_speculative_tokens":4,"branches":17}',
+                '{"method":"ngram","num_speculative_tokens":4,"branches":true}', '{"method":"mtp","num_speculative_tokens":4,"branches":2}'):
+        with pytest.raises(argparse.ArgumentTypeError):
+            parse_speculative_config(bad)
