@@ -19,13 +19,32 @@ class Adjustment:
 
 
 class Adjustments:
-    """Histories ``[slots, most]`` that grow with their requests: a step uploads the tokens that are new and a few numbers a slot.
-    ``stage`` is called on the stream of the steps; what it returns holds until the next call."""
+    """Histories ``[slots, most]`` that grow with their requests: a step uploads the tokens that are new and a few numbers a slot, in
+    one copy.  ``stage`` is called on the stream of the steps, when that stream has left the copy of the call before; what it
+    returns holds until the next call."""
 
     def __init__(self, slots: int, most: int, device) -> None:
         self.slots, self.most, self.device = slots, most, torch.device(device)
         self.history = torch.zeros(slots, most, dtype=torch.int32, device=device)
         self._have: list[tuple[int, int]] = [(-2, 0)] * slots          # whose tokens a row holds, and how many
+        self._host = self._dev = torch.empty(0, dtype=torch.uint8)
+
+    def _upload(self, arrays: dict) -> dict:
+        """The arrays on the device, by way of one pinned buffer and one copy."""
+        at, end = {}, 0
+        for name, a in arrays.items():
+            at[name], end = end, end + -(-a.nbytes // 16) * 16
+        if end > self._host.numel():
+            size = max(end, 2 * self._host.numel(), 1 << 16)
+            self._host = torch.empty(size, dtype=torch.uint8, pin_memory=self.device.type == "cuda")
+            self._dev = torch.empty(size, dtype=torch.uint8, device=self.device)
+        h, out = self._host.numpy(), {}
+        for name, a in arrays.items():
+            h[at[name]:at[name] + a.nbytes] = np.ascontiguousarray(a).reshape(-1).view(np.uint8)
+        self._dev[:end].copy_(self._host[:end], non_blocking=True)
+        for name, a in arrays.items():
+            out[name] = self._dev[at[name]:at[name] + a.nbytes].view(getattr(torch, a.dtype.name)).view(a.shape)
+        return out
 
     def stage(self, segs, rows: list[int] | None = None) -> dict:
         """Operands of ``K.adjust_logits`` for one row of logits a segment, or ``rows[i]`` neighbouring rows of segment i."""
@@ -49,18 +68,20 @@ class Adjustments:
             floats[:, slot] = a.repetition, a.frequency, a.presence
             if a.bias:
                 bias[slot] = a.bias
-        each = rows or [1] * len(segs)
-        request = np.repeat(np.array([s.request_slot if s.adjust is not None else -1 for s in segs], dtype=np.int32), each)
-        up = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(self.device)             # noqa: E731 - (a copy from pageable memory has left it when the call returns)
-        where = np.concatenate(where) if where else np.zeros(0, dtype=np.int64)
-        if where.size:
-            self.history.view(-1).index_copy_(0, up(where), up(np.concatenate(what)))
-        ints, floats = up(ints), up(floats)
-        out = dict(request=up(request), history=self.history, length=ints[0], prompt=ints[1], repetition=floats[0], frequency=floats[1], presence=floats[2])
+        request = np.repeat(np.array([s.request_slot if s.adjust is not None else -1 for s in segs], dtype=np.int32), rows or [1] * len(segs))
+        arrays = {"where": np.concatenate(where) if where else np.zeros(0, dtype=np.int64), "what": np.concatenate(what) if what else np.zeros(0, dtype=np.int32),
+                  "ints": ints, "floats": floats, "request": request}
         if bias:
             count = np.zeros(n + 1, dtype=np.int32)
             for slot, b in bias.items():
                 count[slot + 1] = len(b)
             pairs = [p for slot in sorted(bias) for p in bias[slot]]
-            out["bias"] = (up(np.cumsum(count, dtype=np.int32)), up(np.array([t for t, _ in pairs], dtype=np.int32)), up(np.array([v for _, v in pairs], dtype=np.float32)))
+            arrays.update(first=np.cumsum(count, dtype=np.int32), ids=np.array([t for t, _ in pairs], dtype=np.int32), values=np.array([v for _, v in pairs], dtype=np.float32))
+        d = self._upload(arrays)
+        if d["where"].numel():
+            self.history.view(-1).index_copy_(0, d["where"], d["what"])
+        out = dict(request=d["request"], history=self.history, length=d["ints"][0], prompt=d["ints"][1], repetition=d["floats"][0], frequency=d["floats"][1],
+                   presence=d["floats"][2])
+        if bias:
+            out["bias"] = (d["first"], d["ids"], d["values"])
         return out
