@@ -113,10 +113,13 @@ static constexpr int kTrThreads = 640;
 static constexpr int kTrRegs = 96, kTrRegsSoftmax = 136, kTrRegsConvert = 72, kTrRegsOther = 64;
 static_assert(2 * kTrRegsSoftmax + 2 * kTrRegsConvert + kTrRegsOther <= 5 * kTrRegs, "five warpgroups");
 static constexpr int kTrLists = 4, kTrRaw = 4;
-static constexpr int kTrOps = 3;                         // steps of operands
-// Steps whose powers of two are kept: the note of step s is written behind raw_full (s) <- raw_free (s - kTrRaw) <- v_free of step s - kTrRaw - kTrOps <- p_full of the
+// Operands: of K of two steps, of V, which waits longer, of four.  A step's places, the four warps that convert it and, of items in both tiles, its tile go by its number in
+// the CTA, so that whoever waits at a place has waited for each of its steps before.
+static constexpr int kTrOpsK = 2, kTrOpsV = 4;
+// Steps whose powers of two are kept: the note of step s is written behind raw_full (s) <- raw_free (s - kTrRaw) <- v_free of step s - kTrRaw - kTrOpsV <- p_full of the
 // tiles that take part in it, which have read theirs by then.
-static constexpr int kTrNotes = kTrRaw + kTrOps;
+static constexpr int kTrNotes = 8;
+static_assert(kTrRaw % 2 == 0 && kTrNotes % 2 == 0 && kTrRaw + kTrOpsV <= kTrNotes, "even and odd steps have their own places");
 static constexpr long long kTrLeast = 1;                       // steps of a CTA, at least
 static constexpr float kTrGrowth = 2.f;
 static constexpr int kTrApart = 9;                       // powers of two that scales are apart: up to here the short conversion, ...
@@ -149,8 +152,8 @@ struct TrItem {
 struct TrDesc { int parts, row0, first, rows, kvh, pad[3]; };
 struct __align__(1024) TrSmem {
   uint8_t q[kTrTiles][kTrRows * 128];                    // f16, channels 64..127: [row][128 B], 16-byte chunk ^ (row & 7)
-  uint8_t k[kTrOps][2 * kTrHalf];                             // f16 [stage][64-channel half][token][128 B]
-  uint8_t v[kTrOps][2 * kTrHalf];                             // likewise
+  uint8_t k[kTrOpsK][2 * kTrHalf];                             // f16 [stage][64-channel half][token][128 B]
+  uint8_t v[kTrOpsV][2 * kTrHalf];                             // likewise
   struct Note {
     float k, v;                                          // of a step: what the scales of K and V are multiplied with, ...
     int k_wide, v_wide;                                  // ... and whether the long conversion takes them
@@ -158,7 +161,7 @@ struct __align__(1024) TrSmem {
     int v_exp;                                           // output is 2^v_exp times ...
   } note[kTrNotes];
   uint32_t redo[kTrLists];                               // of an item's steps: some values are beyond what f16 operands hold
-  uint64_t raw_full[kTrRaw], raw_free[kTrRaw], k_full[kTrOps], k_free[kTrOps], v_full[kTrOps], v_free[kTrOps], note_full[kTrNotes];
+  uint64_t raw_full[kTrRaw], raw_free[kTrRaw], k_full[kTrTiles][kTrOpsK], k_free[kTrOpsK], v_full[kTrTiles][kTrOpsV], v_free[kTrOpsV], note_full[kTrNotes];
   uint64_t list_full[kTrLists], list_free[kTrLists], q_full[kTrTiles], s_full[kTrTiles], s_free[kTrTiles], p_full[kTrTiles], pv_done[kTrTiles];
   uint64_t exch_full, exch_free;
   TrItem list[kTrLists];
@@ -170,7 +173,8 @@ struct __align__(1024) TrSmem {
 
 // Items of one tile's rows have them in both tiles, which take its steps in turn (two warps of a kind on a scheduler where one would wait for itself).
 __device__ __forceinline__ bool tr_split(const TrItem& l) { return l.rows <= kTrRows; }
-__device__ __forceinline__ bool tr_takes_part(const TrItem& l, int t) { return tr_split(l) ? l.steps > t : l.steps > 0; }
+// The first step of an item that tile t takes; `before`: steps of the CTA before the item.
+__device__ __forceinline__ int tr_first(const TrItem& l, int t, int before) { return tr_split(l) ? (before ^ t) & 1 : 0; }
 
 __device__ __forceinline__ long long tr_divide(long long a, long long b) {       // (most numbers have 32 bits)
   return (a | b) >> 32 ? a / b : static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
@@ -367,7 +371,7 @@ __device__ __forceinline__ uint2 tr_visible(const uint32_t* sees, int words, int
 }
 
 // Roles: warps 0-7 own a row a thread (softmax needs no exchange: tensor-memory lane = row); warps 8-11 convert raw pages to the swizzled operands of K
-// and V ([token][channel], f16), by turns with warps 12-15; warps 16 and 18 issue the MMAs of the scores and of the output; warp 17 makes the items and copies pages;
+// and V ([token][channel], f16), by turns with warps 12-15; warps 16 and 18 issue the MMAs of a tile each; warp 17 makes the items and copies pages;
 // warp 19 finds the powers of two that bring a step's values into f16's range.
 // Tensor memory of a tile of 128 rows: scores, probabilities (the A operand of their product), output and the first half of Q's channels; the other half of
 // Q is in shared memory.  The scores of step i + 1 are computed while the softmax of step i runs.  The output is rescaled only when a row's maximum has grown by more
@@ -393,11 +397,13 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       mbar_init(smem_u32(&sm.raw_full[b]), 1);
       mbar_init(smem_u32(&sm.raw_free[b]), 4);
     }
-    for (int b = 0; b < kTrOps; ++b) {
-      mbar_init(smem_u32(&sm.k_full[b]), 4);
-      mbar_init(smem_u32(&sm.k_free[b]), 1);
-      mbar_init(smem_u32(&sm.v_full[b]), 4);
-      mbar_init(smem_u32(&sm.v_free[b]), 1);
+    for (int b = 0; b < kTrOpsV; ++b) {
+      if (b < kTrOpsK) mbar_init(smem_u32(&sm.k_free[b]), 2);            // an MMA warp each, or one of them twice
+      mbar_init(smem_u32(&sm.v_free[b]), 2);
+      for (int t = 0; t < kTrTiles; ++t) {
+        if (b < kTrOpsK) mbar_init(smem_u32(&sm.k_full[t][b]), 4);
+        mbar_init(smem_u32(&sm.v_full[t][b]), 4);
+      }
     }
     for (int b = 0; b < kTrNotes; ++b) {
       mbar_init(smem_u32(&sm.note_full[b]), 1);
@@ -613,61 +619,69 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       }
     } else {
       // ---------------------------------------------------------------- MMAs
-      const bool leader = elect_one(), is_s = warp == 16;
+      const bool leader = elect_one();
+      const int t = warp == 18;
       const uint32_t idesc_s = umma_idesc(kTrRows, kTrTok, 0u, 0u), idesc_o = umma_idesc(kTrRows, kD, 0u, 0u) | 1u << 16;      // V: channels are contiguous
-      const uint64_t dq = umma_desc_sw128(smem_u32(sm.q[0])), dk = umma_desc_sw128(smem_u32(sm.k[0])), dv = umma_desc_sw128_n(smem_u32(sm.v[0]), kTrHalf);
-      TrRing op(kTrOps);
-      uint32_t s_phase = 3;                                // of what each tile lets go or brings, bit = tile (a wait for scores that nobody holds is over at once)
-      if (!is_s) s_phase = 0;
-      uint32_t q_phase = 0;                              // bit = tile
+      const uint64_t dq = umma_desc_sw128(smem_u32(sm.q[t])), dk = umma_desc_sw128(smem_u32(sm.k[0])), dv = umma_desc_sw128_n(smem_u32(sm.v[0]), kTrHalf);
+      const uint32_t tile = tmem + t * kTrTmemTile;
+      int before = 0;                                    // steps of earlier items
+      uint32_t q_phase = 0, k_phase = 0, v_phase = 0, s_phase = 1, p_phase = 0;            // k and v: bit = place; (a wait for scores that nobody holds is over at once)
+#pragma unroll 1
       for (int it = 0;; ++it) {
         const TrItem& l = sm.list[it % kTrLists];
         if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok || l.kvh < 0) break;
-        const int steps = l.steps;
+        const int steps = l.steps, first = tr_first(l, t, before);
         const bool split = tr_split(l);
+        const int by = split ? 2 : 1;
+        if (first < steps) {
+          if (ok) ok = tr_wait(smem_u32(&sm.q_full[t]), q_phase, abort_flag);
+          q_phase ^= 1u;
+        }
+        // scores of step s, then the product of the one before: scores run ahead of their softmax
 #pragma unroll 1
-        for (int s = 0; s < steps; ++s, op.advance()) {
-          const int b = op.i;
-          if (ok) ok = tr_wait(smem_u32(is_s ? &sm.k_full[b] : &sm.v_full[b]), op.phase, abort_flag);
-#pragma unroll
-          for (int t = 0; t < kTrTiles; ++t) {
-            if (split && (s & 1) != t) continue;
-            const bool first = s == (split ? t : 0);
-            const uint32_t tile = tmem + t * kTrTmemTile;
-            if (is_s) {
-              if (first) {
-                if (ok) ok = tr_wait(smem_u32(&sm.q_full[t]), q_phase >> t & 1, abort_flag);
-                q_phase ^= 1u << t;
-              }
-              if (ok) ok = tr_wait(smem_u32(&sm.s_free[t]), s_phase >> t & 1, abort_flag);
-            } else {
-              if (ok) ok = tr_wait(smem_u32(&sm.p_full[t]), s_phase >> t & 1, abort_flag);
-            }
+        for (int s = first; s < steps + by && first < steps; s += by) {
+          if (s < steps) {
+            const int b = (before + s) & (kTrOpsK - 1);
+            if (ok) ok = tr_wait(smem_u32(&sm.k_full[t][b]), k_phase >> b & 1, abort_flag);
+            if (ok) ok = tr_wait(smem_u32(&sm.s_free[t]), s_phase, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
-            s_phase ^= 1u << t;
+            k_phase ^= 1u << b;
+            s_phase ^= 1u;
             tc_fence_after();
             if (ok && leader) {
-              if (is_s) {
-                const uint64_t k0 = dk + (b * (2 * kTrHalf) >> 4);
+              const uint64_t k0 = dk + (b * (2 * kTrHalf) >> 4);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) umma_f16_ts(tile, tile + kTrTmemQ + k * 8, k0 + k * 2, idesc_s, k > 0);
+              for (int k = 0; k < 4; ++k) umma_f16_ts(tile, tile + kTrTmemQ + k * 8, k0 + k * 2, idesc_s, k > 0);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) umma_f16(tile, dq + (t * (kTrRows * 128) >> 4) + k * 2, k0 + (kTrHalf >> 4) + k * 2, idesc_s, 1);
-                tc_commit(smem_u32(&sm.s_full[t]));
-              } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  umma_f16_ts(tile + kTrTmemO, tile + kTrTmemP + k * 8, dv + (b * (2 * kTrHalf) >> 4) + k * (16 * 128 >> 4), idesc_o, !first || k > 0);
-                tc_commit(smem_u32(&sm.pv_done[t]));
-              }
+              for (int k = 0; k < 4; ++k) umma_f16(tile, dq + k * 2, k0 + (kTrHalf >> 4) + k * 2, idesc_s, 1);
+              tc_commit(smem_u32(&sm.s_full[t]));
+              tc_commit(smem_u32(&sm.k_free[b]));
+              if (split) tc_commit(smem_u32(&sm.k_free[b]));
             }
             __syncwarp();
           }
-          if (ok && leader) tc_commit(smem_u32(is_s ? &sm.k_free[b] : &sm.v_free[b]));
-          __syncwarp();
+          if (s > first) {
+            const int b = (before + s - by) & (kTrOpsV - 1);
+            if (ok) ok = tr_wait(smem_u32(&sm.v_full[t][b]), v_phase >> b & 1, abort_flag);
+            if (ok) ok = tr_wait(smem_u32(&sm.p_full[t]), p_phase, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            v_phase ^= 1u << b;
+            p_phase ^= 1u;
+            tc_fence_after();
+            if (ok && leader) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f16_ts(tile + kTrTmemO, tile + kTrTmemP + k * 8, dv + (b * (2 * kTrHalf) >> 4) + k * (16 * 128 >> 4), idesc_o, s - by > first || k > 0);
+              tc_commit(smem_u32(&sm.pv_done[t]));
+              tc_commit(smem_u32(&sm.v_free[b]));
+              if (split) tc_commit(smem_u32(&sm.v_free[b]));
+            }
+            __syncwarp();
+          }
         }
+        before += steps;
         if (lane == 0) mbar_arrive(smem_u32(&sm.list_free[it % kTrLists]));
       }
     }
@@ -676,7 +690,9 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTrRegsConvert));
     // warps 8-11 take the even steps, 12-15 the odd ones, K first: scores run ahead of their softmax
     const int ct = tid & 127, mine = warp >= 12;
-    TrRing raw_at(kTrRaw, 0, mine), note_at(kTrNotes, 0, mine), op(kTrOps, 1, mine);         // (a wait for operands that nobody reads is over at once)
+    TrRing raw_at(kTrRaw, 0, mine), note_at(kTrNotes, 0, mine);
+    uint32_t k_phase = 1, v_phase = 1;                   // (a wait for operands that nobody reads is over at once)
+    int vb = mine;                                       // V's place
     int ahead = mine;                                    // steps from the item's first to this warp's next
 #pragma unroll 1
     for (int it = 0;; ++it) {
@@ -685,37 +701,45 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       ok = __all_sync(0xffffffffu, ok);
       if (!ok || l.kvh < 0) break;
       const int steps = l.steps;
+      const bool split = tr_split(l);
       int visible = l.total - (l.lo + ahead) * kTrTok;
 #pragma unroll 1
       for (; ahead < steps; ahead += 2, visible -= 2 * kTrTok) {
         if (ok) ok = tr_wait(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag);
         if (ok) ok = tr_wait(smem_u32(&sm.note_full[note_at.i]), note_at.phase, abort_flag);
-        if (ok) ok = tr_wait(smem_u32(&sm.k_free[op.i]), op.phase, abort_flag);
+        if (ok) ok = tr_wait(smem_u32(&sm.k_free[mine]), k_phase, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint8_t* pages = raw + raw_at.i * kTrPages * L::stride;
         const auto& note = sm.note[note_at.i];
         const float v_mul = note.v;
         const int v_wide = note.v_wide;
-        if (__builtin_expect(!note.k_wide, 1)) tr_convert_k<KBITS, VBITS, false>(sm.k[op.i], pages, note.k, ct);
-        else tr_convert_k<KBITS, VBITS, true>(sm.k[op.i], pages, note.k, ct);
+        if (__builtin_expect(!note.k_wide, 1)) tr_convert_k<KBITS, VBITS, false>(sm.k[mine], pages, note.k, ct);
+        else tr_convert_k<KBITS, VBITS, true>(sm.k[mine], pages, note.k, ct);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.k_full[op.i]));
-        ok = tr_wait(smem_u32(&sm.v_free[op.i]), op.phase, abort_flag);
+        // (of items in both tiles, the even steps are tile 0's)
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&sm.k_full[mine][mine]));
+          if (!split) mbar_arrive(smem_u32(&sm.k_full[1 - mine][mine]));
+        }
+        ok = tr_wait(smem_u32(&sm.v_free[vb]), v_phase, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (__builtin_expect(!v_wide, 1)) tr_convert_v<KBITS, VBITS, false>(sm.v[op.i], pages, visible, v_mul, ct);
-        else tr_convert_v<KBITS, VBITS, true>(sm.v[op.i], pages, visible, v_mul, ct);
+        if (__builtin_expect(!v_wide, 1)) tr_convert_v<KBITS, VBITS, false>(sm.v[vb], pages, visible, v_mul, ct);
+        else tr_convert_v<KBITS, VBITS, true>(sm.v[vb], pages, visible, v_mul, ct);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(smem_u32(&sm.v_full[op.i]));
+          mbar_arrive(smem_u32(&sm.v_full[mine][vb]));
+          if (!split) mbar_arrive(smem_u32(&sm.v_full[1 - mine][vb]));
           mbar_arrive(smem_u32(&sm.raw_free[raw_at.i]));
         }
         raw_at.advance(2);
         note_at.advance(2);
-        op.advance(2);
+        k_phase ^= 1u;
+        vb ^= 2;
+        v_phase ^= vb == mine;
       }
       ahead -= steps;
       __syncwarp();
@@ -732,7 +756,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       float mul;                                         // what its scores are multiplied with, but for K's power of two
     };
     // the row of the thread in item `it`, and Q of its tile; false: no more items
-    auto begin = [&](int it, Row& r) {
+    auto begin = [&](int it, int before, Row& r) {
       const TrItem& l = sm.list[it % kTrLists];
       if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
@@ -747,7 +771,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
         r.out = (l.row0 + node) * p.ldo + col;
         r.sees = p.masks + (l.row0 + node) * p.ldm;
       }
-      if (tr_takes_part(l, t)) {
+      if (tr_first(l, t, before) < l.steps) {
         // a power of two brings the row's largest magnitude to 2^10 .. 2^11; what is not finite stays
         uint4 q[16];                                     // all loads in flight at once
 #pragma unroll
@@ -779,7 +803,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       }
       return true;
     };
-    int note0 = 0, n = 0, exchanges = 0;                 // note of the item's first step; steps that this tile took part in; items in both tiles
+    int before = 0, n = 0, exchanges = 0;                // steps of earlier items; steps that this tile took part in; items in both tiles
     bool lent = false;                                   // the other tile may still read this one's output
     auto wait_lent = [&]() {
       if (lent && ok) ok = tr_wait(smem_u32(&sm.exch_free), (exchanges - 1) & 1, abort_flag);
@@ -791,16 +815,14 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
     for (int it = -1; more; ++it) {                      // (-1: nothing yet but the first item's Q)
       const TrItem& l = sm.list[max(it, 0) % kTrLists];
       const int steps = it < 0 ? 0 : l.steps, start = l.start, total = l.total;
-      const bool split = it >= 0 && tr_split(l), in = it >= 0 && tr_takes_part(l, t), mine = cur.q >= 0;
+      const int first = it < 0 ? 0 : tr_first(l, t, before);
+      const bool split = it >= 0 && tr_split(l), in = first < steps, mine = cur.q >= 0;
       float m = -INFINITY, sum = 0.f;
       int v_exp = 0;
       {
-        const int first = split ? t : 0;
-        int note = note0 + first;
-        if (note >= kTrNotes) note -= kTrNotes;
 #pragma unroll 1
         for (int s = first; s < steps; s += split ? 2 : 1) {
-          const int tok0 = (l.lo + s) * kTrTok;
+          const int tok0 = (l.lo + s) * kTrTok, note = (before + s) & (kTrNotes - 1);
           if (ok) ok = tr_wait(smem_u32(&sm.s_full[t]), n & 1, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
@@ -832,8 +854,6 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           }
           // (there before K was converted; written again after this step's product, which waits for what follows: kTrNotes)
           const float2 told = make_float2(sm.note[note].back, __int_as_float(sm.note[note].v_exp));
-          note += split ? 2 : 1;
-          if (note >= kTrNotes) note -= kTrNotes;
           const float mul = told.x * cur.mul, top = mx * mul;
           float alpha = 1.f;
           bool grew = top > m + kTrGrowth || (m == -INFINITY && top > m);
@@ -892,10 +912,9 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           ++n;
         }
       }
-      note0 = (note0 + steps) % kTrNotes;
       // the next item's Q while the last product runs (all of this item's scores are there)
       Row next;
-      more = begin(it + 1, next);
+      more = begin(it + 1, before + steps, next);
       const int part = it < 0 ? -1 : l.part;
       const size_t at = static_cast<size_t>(max(part, 0)) * part_rows + (split ? row : t * kTrRows + row);
       if (steps == 0) {                                  // a request that is told wrongly
@@ -908,7 +927,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
         ok = __all_sync(0xffffffffu, ok);
         // what this tile's output and the other's are multiplied with
         float mul[2] = {pow2f(v_exp), 0.f};
-        const bool other = split && steps > 1 - t;       // the other tile has an output
+        const bool other = split && (1 - first) < steps; // the other tile has an output
         if (split) {
           wait_lent();
           sm.exch_ml[t][row] = make_float2(m, sum);
@@ -985,6 +1004,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       }
       __syncwarp();
       if (lane == 0 && it >= 0) mbar_arrive(smem_u32(&sm.list_free[it % kTrLists]));
+      before += steps;
       cur = next;
     }
   }
