@@ -104,9 +104,11 @@ __device__ __forceinline__ void tree_row(const CbTreeAttn& p, const TreeRequest&
 }
 
 // ------------------------------------------------------------------------------------------------- schedule
-// An item is up to 256 rows (node x query head of the group) of a request and key / value head, in steps of 64 tokens.  The steps of all items, one after the
-// other, are dealt out evenly: CTA c takes the steps [c per, (c + 1) per), however uneven the requests are.  An item that several CTAs share leaves a part (its
-// maximum, sum and unnormalised output) of each in the workspace, and tree_merge_kernel joins them in order: no atomics, the same bits every time.
+// An item is up to 256 rows (node x query head of the group) of a request and key / value head, in steps of 64 tokens.  The slots of all items, one after the
+// other, are dealt out evenly: CTA c takes those that begin at the units [c per, (c + 1) per), however uneven the requests are.  An item has a slot for each step, and
+// kTrSwitch before them: its queries and its results take as long as five steps (dealt out by steps alone 32 x 64 behind up to 1500 took 142 us in place of 121, 2 x 64
+// behind 32000 122 in place of 113).  An item that several CTAs share leaves a part (its maximum, sum and unnormalised output) of each in the workspace, and
+// tree_merge_kernel joins them in order: no atomics, the same bits every time.
 static constexpr int kTrTiles = 2, kTrRows = 128, kTrItemRows = kTrTiles * kTrRows;
 static constexpr int kTrPages = 4, kTrTok = kTrPages * kPageTokens;
 static constexpr int kTrThreads = 640;
@@ -120,7 +122,7 @@ static constexpr int kTrOpsK = 2, kTrOpsV = 4;
 // tiles that take part in it, which have read theirs by then.
 static constexpr int kTrNotes = 8;
 static_assert(kTrRaw % 2 == 0 && kTrNotes % 2 == 0 && kTrRaw + kTrOpsV <= kTrNotes, "even and odd steps have their own places");
-static constexpr long long kTrLeast = 1;                       // steps of a CTA, at least
+static constexpr int kTrSwitch = 5;                      // slots that an item takes in the schedule before its steps
 static constexpr float kTrGrowth = 2.f;
 static constexpr int kTrApart = 9;                       // powers of two that scales are apart: up to here the short conversion, ...
 static constexpr int kTrApartK = 18, kTrApartV = 14;     // ... and the long one
@@ -168,7 +170,7 @@ struct __align__(1024) TrSmem {
   float2 exch_ml[kTrTiles][kTrRows];                     // rows in both tiles: maximum and sum, ...
   int exch_exp[kTrTiles][kTrRows];                       // ... and v_exp
   uint32_t tmem, abort_word;
-  long long upto[kTreeMaxRequests + 1];                  // steps of the requests before
+  long long upto[kTreeMaxRequests + 1], items[kTreeMaxRequests + 1];     // units of the requests before; their items' units a slot
 };
 
 // Items of one tile's rows have them in both tiles, which take its steps in turn (two warps of a kind on a scheduler where one would wait for itself).
@@ -180,6 +182,8 @@ __device__ __forceinline__ long long tr_divide(long long a, long long b) {      
   return (a | b) >> 32 ? a / b : static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
 }
 __device__ __forceinline__ int tr_steps(const TreeRequest& r) { return max(1, (r.total + kTrTok - 1) / kTrTok); }
+// Units of the schedule that a step takes: one if its request's items are in both tiles (tr_split), else two.
+__device__ __forceinline__ int tr_slot(const TreeRequest& r, int G) { return r.count * G <= kTrRows ? 1 : 2; }
 __device__ __forceinline__ int tr_groups(const TreeRequest& r, int G) { return (r.count * G + kTrItemRows - 1) / kTrItemRows; }
 static inline int tr_rows(int words, int rows, int G) {
   const long long most = static_cast<long long>(words * 32 < rows ? words * 32 : rows) * G;
@@ -441,37 +445,58 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTrRegsOther));
     if (warp == 17) {
       // ------------------------------------------------------- items and pages
-      // steps of all requests, summed
-      long long all = 0;
-      if (lane == 0) sm.upto[0] = 0;
-#pragma unroll 4
+      // units and items of all requests, summed
+      long long all = 0, items = 0;
+      int unit = 1;                                      // the longest slot
+      TreeRequest r = {0, 0, 0, 0, 0};
+      if (lane == 0) sm.upto[0] = sm.items[0] = 0;
+#pragma unroll 1
       for (int i0 = 0; i0 < p.n; i0 += 32) {
-        long long v = 0;
+        long long v = 0, w = 0;
         if (i0 + lane < p.n) {
-          const TreeRequest r = tree_request(p, i0 + lane, bad);
-          v = static_cast<long long>(tr_steps(r)) * (tr_groups(r, G) * p.Hkv);
+          r = tree_request(p, i0 + lane, bad);
+          const int slot = tr_slot(r, G);
+          unit = max(unit, slot);
+          w = static_cast<long long>(tr_groups(r, G) * p.Hkv) * slot;
+          v = w * tr_steps(r);
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const long long before = __shfl_up_sync(0xffffffffu, v, o);
-          if (lane >= o) v += before;
+          const long long v0 = __shfl_up_sync(0xffffffffu, v, o), w0 = __shfl_up_sync(0xffffffffu, w, o);
+          if (lane >= o) { v += v0; w += w0; }
         }
-        if (i0 + lane < p.n) sm.upto[i0 + lane + 1] = all + v;
+        if (i0 + lane < p.n) {
+          sm.upto[i0 + lane + 1] = all + v;
+          sm.items[i0 + lane + 1] = items + w;
+        }
         all += __shfl_sync(0xffffffffu, v, 31);
+        items += __shfl_sync(0xffffffffu, w, 31);
       }
+      const int longest = __reduce_max_sync(0xffffffffu, unit);
       __syncwarp();
-      const long long per = max(kTrLeast, tr_divide(all + gridDim.x - 1, gridDim.x));
+      const int before = static_cast<int>(min(static_cast<long long>(kTrSwitch), tr_divide(all + gridDim.x - 1, gridDim.x) / 2));       // slots of an item before its steps
+      if (before) {
+        for (int k = lane; k <= p.n; k += 32) sm.upto[k] += before * sm.items[k];
+        all += before * items;
+        __syncwarp();
+      }
+      const long long per = max(static_cast<long long>(longest), tr_divide(all + gridDim.x - 1, gridDim.x));
       long long u = min(all, per * blockIdx.x);
       const long long end = min(all, u + per);
       int i = 0, gs = 0;
-      TreeRequest r = {0, 0, 0, 0, 0};
-      if (u < end) {                                     // the request of the first step
+      auto request_of = [&](int k) {                     // (the lanes have the first 32)
+        if (p.n > 32) return tree_request(p, k, bad);
+        TreeRequest to;
+        to.slot = __shfl_sync(0xffffffffu, r.slot, k); to.row0 = __shfl_sync(0xffffffffu, r.row0, k); to.count = __shfl_sync(0xffffffffu, r.count, k);
+        to.start = __shfl_sync(0xffffffffu, r.start, k); to.total = __shfl_sync(0xffffffffu, r.total, k);
+        return to;
+      };
+      if (u < end) {                                     // the request of the first unit
         int hi = p.n;
         while (hi - i > 1) {
           const int mid = (i + hi) >> 1;
           if (sm.upto[mid] <= u) i = mid; else hi = mid;
         }
-        r = tree_request(p, i, bad);
       }
       TrDesc d = {};
       int ids_next = 0;                                  // pages of the item made last, 32 from its first on
@@ -486,27 +511,37 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
         if (!ok) return false;
         TrItem l;
         l.kvh = -1;
-        if (u < end) {
-          while (u >= sm.upto[i + 1]) {
-            ++i;
-            if (u < sm.upto[i + 1]) r = tree_request(p, i, bad);
-          }
-          const int S = tr_steps(r), groups = tr_groups(r, G);
-          const long long off = u - sm.upto[i];
-          const int k = static_cast<int>(tr_divide(off, S)), s = static_cast<int>(off - static_cast<long long>(k) * S);
-          const int n_steps = static_cast<int>(min(static_cast<long long>(S - s), end - u));
+        while (u < end && l.kvh < 0) {
+          while (u >= sm.upto[i + 1]) ++i;
+          const TreeRequest of = request_of(i);
+          const int S = tr_steps(of), groups = tr_groups(of, G), slot = tr_slot(of, G);
+          const long long long_item = static_cast<long long>(slot) * (before + S), off = u - sm.upto[i];
+          const int k = static_cast<int>(tr_divide(off, long_item));
+          const long long item = u - (off - k * long_item);                              // where the item begins
+          auto step_at = [&](long long at) {             // the first step whose slot begins at `at` or behind it
+            return max(0, static_cast<int>(min((at - item + slot - 1) >> (slot - 1), static_cast<long long>(before + S))) - before);
+          };
+          const int s = step_at(u), n_steps = step_at(end) - s;
+          u = min(end, item + long_item);
+          if (n_steps <= 0) continue;
           l.kvh = k / groups;
-          l.slot = r.slot; l.row0 = r.row0; l.count = r.count; l.start = r.start; l.total = r.total;
+          l.slot = of.slot; l.row0 = of.row0; l.count = of.count; l.start = of.start; l.total = of.total;
           l.first = (k - l.kvh * groups) * kTrItemRows;
-          l.rows = min(kTrItemRows, r.count * G - l.first);
+          l.rows = min(kTrItemRows, of.count * G - l.first);
           l.lo = s;
-          l.steps = r.total > 0 ? n_steps : 0;
+          l.steps = of.total > 0 ? n_steps : 0;
           l.part = n_steps == S ? -1 : 2 * static_cast<int>(blockIdx.x) + (s == 0);
           if (l.part >= 0 && s == 0) {
-            d.parts = static_cast<int>(tr_divide(u + S - 1, per)) - static_cast<int>(blockIdx.x) + 1;
+            d.parts = static_cast<int>(tr_divide(item + slot * static_cast<long long>(before + S - 1), per)) - static_cast<int>(blockIdx.x) + 1;
             d.row0 = l.row0; d.first = l.first; d.rows = l.rows; d.kvh = l.kvh;
           }
-          u += n_steps;
+          if (n > 0)                                     // its queries are on their way into the L2 cache
+            for (int row = lane; row < l.rows; row += 32) {
+              const int node = (l.first + row) / G;
+              const __nv_bfloat16* at = p.q + (l.row0 + node) * p.ldq + (l.kvh * G + (l.first + row - node * G)) * kD;
+              asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+              asm volatile("prefetch.global.L2 [%0];" ::"l"(at + 64));
+            }
         }
         if (lane == 0) {
           to = l;
@@ -773,9 +808,28 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       }
       if (tr_first(l, t, before) < l.steps) {
         // a power of two brings the row's largest magnitude to 2^10 .. 2^11; what is not finite stays
-        uint4 q[16];                                     // all loads in flight at once
+        // All loads in flight at once, eight lanes a row (a row a lane would have 32 lines of memory in a load: 7000 cycles, not 2500); a half at a time goes to the
+        // row's lane by way of the warp's own rows of Q's operand.
+        uint4 q[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) q[c] = r.q >= 0 ? reinterpret_cast<const uint4*>(p.q + r.q)[c] : make_uint4(0u, 0u, 0u, 0u);
+        for (int j = 0; j < 8; ++j) {
+          const long long from = __shfl_sync(0xffffffffu, r.q, 4 * j + (lane >> 3));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) q[8 * h + j] = from >= 0 ? reinterpret_cast<const uint4*>(p.q + from)[8 * h + (lane & 7)] : make_uint4(0u, 0u, 0u, 0u);
+        }
+        uint8_t* rows = sm.q[t] + (warp & 3) * 32 * 128;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int of = 4 * j + (lane >> 3);
+            *reinterpret_cast<uint4*>(rows + of * 128 + (((lane & 7) ^ (of & 7)) << 4)) = q[8 * h + j];
+          }
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) q[8 * h + c] = *reinterpret_cast<const uint4*>(rows + lane * 128 + ((c ^ (lane & 7)) << 4));
+          __syncwarp();
+        }
         uint32_t most = 0;                               // (two magnitudes a word: the larger of the upper, then of the lower ones)
 #pragma unroll
         for (int c = 0; c < 16; ++c) most = __vmaxu2(most, __vmaxu2(__vmaxu2(q[c].x & 0x7FFF7FFFu, q[c].y & 0x7FFF7FFFu), __vmaxu2(q[c].z & 0x7FFF7FFFu, q[c].w & 0x7FFF7FFFu)));
@@ -916,7 +970,9 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       Row next;
       more = begin(it + 1, before + steps, next);
       const int part = it < 0 ? -1 : l.part;
-      const size_t at = static_cast<size_t>(max(part, 0)) * part_rows + (split ? row : t * kTrRows + row);
+      // of a part, [four channels][row]: a warp's rows are neighbours
+      const size_t in_part = split ? row : t * kTrRows + row, at = static_cast<size_t>(max(part, 0)) * part_rows + in_part;
+      float4* const part_to = reinterpret_cast<float4*>(part_o) + static_cast<size_t>(max(part, 0)) * 32 * part_rows + in_part;
       if (steps == 0) {                                  // a request that is told wrongly
         if (mine) {
 #pragma unroll
@@ -949,6 +1005,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
         tc_fence_after();
         if (!*const_cast<volatile uint32_t*>(&sm.redo[it % kTrLists])) {
           const float inv = part >= 0 ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;            // NaN stays
+          const long long beside = __shfl_xor_sync(0xffffffffu, cur.out, 1);                              // the next lane's row
           const int c0 = split ? 4 * t : 0, c1 = split ? 4 * t + 4 : 8;                                  // of 16 channels
 #pragma unroll 1
           for (int c = c0; c < c1; ++c) {
@@ -966,12 +1023,18 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
             }
             if (mine && part >= 0) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(part_o + at * kD + c * 16)[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-            } else if (mine) {
-#pragma unroll
-              for (int j = 0; j < 2; ++j)
-                reinterpret_cast<uint4*>(p.out + cur.out + c * 16)[j] = make_uint4(pack_bf16x2(o[8 * j], o[8 * j + 1]), pack_bf16x2(o[8 * j + 2], o[8 * j + 3]),
-                                                                                  pack_bf16x2(o[8 * j + 4], o[8 * j + 5]), pack_bf16x2(o[8 * j + 6], o[8 * j + 7]));
+              for (int j = 0; j < 4; ++j) part_to[static_cast<size_t>(4 * c + j) * part_rows] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            } else if (part < 0) {
+              // two lanes write a row's 32 bytes, then the next row's
+              const uint4 x = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7])),
+                          y = make_uint4(pack_bf16x2(o[8], o[9]), pack_bf16x2(o[10], o[11]), pack_bf16x2(o[12], o[13]), pack_bf16x2(o[14], o[15]));
+              const bool odd = lane & 1;
+              uint4 z = odd ? x : y;
+              z.x = __shfl_xor_sync(0xffffffffu, z.x, 1); z.y = __shfl_xor_sync(0xffffffffu, z.y, 1);
+              z.z = __shfl_xor_sync(0xffffffffu, z.z, 1); z.w = __shfl_xor_sync(0xffffffffu, z.w, 1);
+              const long long even_row = odd ? beside : cur.out, odd_row = odd ? cur.out : beside;
+              if (even_row >= 0) *reinterpret_cast<uint4*>(p.out + even_row + c * 16 + 8 * odd) = odd ? z : x;
+              if (odd_row >= 0) *reinterpret_cast<uint4*>(p.out + odd_row + c * 16 + 8 * odd) = odd ? y : z;
             }
           }
           if (part >= 0 && mine && c0 == 0) part_ml[at] = make_float2(m, sum);
@@ -987,9 +1050,8 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
             float rm, rs, o[4];
             tree_row<KBITS, VBITS>(p, r, l.kvh, lo, hi, sees, p.q + q, lane, rm, rs, o, bad);
             if (part >= 0) {
-              const size_t to = at - lane + of;
-              reinterpret_cast<float4*>(part_o + to * kD)[lane] = make_float4(o[0], o[1], o[2], o[3]);
-              if (lane == 0) part_ml[to] = make_float2(rm, rs);
+              part_to[static_cast<size_t>(lane) * part_rows - lane + of] = make_float4(o[0], o[1], o[2], o[3]);
+              if (lane == 0) part_ml[at - lane + of] = make_float2(rm, rs);
             } else {
               const float f = rs > 0.f ? 1.f / rs : rs == 0.f ? 0.f : rs;
               reinterpret_cast<uint2*>(p.out + out)[lane] = make_uint2(pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f));
@@ -1015,39 +1077,72 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
   if (tid == 0 && sm.abort_word) atomicExch(p.status, static_cast<uint32_t>(kErrBarrierTimeout));
 }
 
-// Joins the parts of items that several CTAs shared: block x looks after the item that began in CTA x and went on beyond it.  A warp has a row at a time.
+// Joins the parts of items that several CTAs shared: block x looks after the item that began in CTA x and went on beyond it.  A warp's lanes are eight rows times four of
+// the 32 fours of channels, so that both sides are whole sectors; a thread has ROWS rows, eight apart, and PARTS parts of them in flight.  Few rows mean many parts of each
+// and blocks that are all resident at once: one row and eight parts (1 x 8 behind 700: 15.4 us, with two and four 17.8); else two and four (2 x 64 behind 32000: 109.6 us
+// against 110.9, 32 x 64 behind up to 1500: 122.6 against 126.3).
+static constexpr int kTrMergeFew = 40;                   // rows: five blocks fit a multiprocessor
+template <int ROWS, int PARTS>
 __global__ void __launch_bounds__(256)
 tree_merge_kernel(const CbTreeAttn p, const int part_rows) {
   pdl_wait();
   pdl_launch_dependents();
-  const float* part_o = p.partial;
-  const float2* part_ml = reinterpret_cast<const float2*>(part_o + static_cast<size_t>(gridDim.x) * 2 * part_rows * kD);
+  const float4* part_o = reinterpret_cast<const float4*>(p.partial);
+  const float2* part_ml = reinterpret_cast<const float2*>(part_o + static_cast<size_t>(gridDim.x) * 2 * part_rows * (kD / 4));
   const TrDesc d = reinterpret_cast<const TrDesc*>(part_ml + static_cast<size_t>(gridDim.x) * 2 * part_rows)[blockIdx.x];
-  const int lane = threadIdx.x & 31, G = p.Hq / p.Hkv;
-  const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
-  if (d.parts <= 0 || row >= d.rows) return;
-  auto at = [&](int c) { return static_cast<size_t>(2 * (blockIdx.x + c) + (c == 0)) * part_rows + row; };
-  float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-  for (int c0 = 0; c0 < d.parts; c0 += 32) {             // a lane has a part's maximum and sum
-    const int n = min(32, d.parts - c0);
-    const float2 ml = lane < n ? __ldcg(part_ml + at(c0 + lane)) : make_float2(-INFINITY, 0.f);
-    const float top = fmaxf(m, warp_max(ml.x)), use = top == -INFINITY ? 0.f : top;
-    const float f = fast_exp2(ml.x - use), old = fast_exp2(m - use);                     // of a part that saw nothing: zero
-    m = top;
-    sum = sum * old + warp_sum(f * ml.y);
+  const int row0 = blockIdx.y * 8 * ROWS + (threadIdx.x & 7), four = threadIdx.x >> 3, G = p.Hq / p.Hkv;
+  if (d.parts <= 0 || row0 >= d.rows) return;
+  float m[ROWS], sum[ROWS], o[ROWS][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] *= old;
-#pragma unroll 8
-    for (int c = 0; c < n; ++c) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(part_o + at(c0 + c) * kD) + lane);
-      const float g = __shfl_sync(0xffffffffu, f, c);
-      o[0] = fmaf(g, x.x, o[0]); o[1] = fmaf(g, x.y, o[1]); o[2] = fmaf(g, x.z, o[2]); o[3] = fmaf(g, x.w, o[3]);
+  for (int k = 0; k < ROWS; ++k) {
+    m[k] = -INFINITY;
+    sum[k] = o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
+  }
+#pragma unroll 1
+  for (int c = 0; c < d.parts; c += PARTS) {
+    float2 ml[PARTS][ROWS];
+    float4 x[PARTS][ROWS];
+#pragma unroll
+    for (int e = 0; e < PARTS; ++e) {
+      const size_t part = 2 * (blockIdx.x + c + e) + (c + e == 0);
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        const int row = row0 + 8 * k;
+        const bool there = c + e < d.parts && row < d.rows;
+        ml[e][k] = there ? __ldcg(part_ml + part * part_rows + row) : make_float2(-INFINITY, 0.f);
+        x[e][k] = there ? __ldcg(part_o + (part * 32 + four) * part_rows + row) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      float top = m[k];
+#pragma unroll
+      for (int e = 0; e < PARTS; ++e) top = fmaxf(top, ml[e][k].x);
+      const float use = top == -INFINITY ? 0.f : top, old = fast_exp2(m[k] - use);
+      m[k] = top;
+      sum[k] *= old;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[k][j] *= old;
+#pragma unroll
+      for (int e = 0; e < PARTS; ++e) {
+        const float f = fast_exp2(ml[e][k].x - use);     // of a part that saw nothing: zero
+        sum[k] = fmaf(f, ml[e][k].y, sum[k]);
+        o[k][0] = fmaf(f, x[e][k].x, o[k][0]);
+        o[k][1] = fmaf(f, x[e][k].y, o[k][1]);
+        o[k][2] = fmaf(f, x[e][k].z, o[k][2]);
+        o[k][3] = fmaf(f, x[e][k].w, o[k][3]);
+      }
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-  const int node = (d.first + row) / G, col = (d.kvh * G + (d.first + row - node * G)) * kD;
-  reinterpret_cast<uint2*>(p.out + (d.row0 + node) * p.ldo + col)[lane] = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const int row = row0 + 8 * k;
+    if (row >= d.rows) break;
+    const float f = sum[k] > 0.f ? 1.f / sum[k] : sum[k] == 0.f ? 0.f : sum[k];
+    const int node = (d.first + row) / G;
+    const long long to = (d.row0 + node) * p.ldo + (d.kvh * G + (d.first + row - node * G)) * kD + four * 4;
+    *reinterpret_cast<uint2*>(p.out + to) = make_uint2(pack_bf16x2(o[k][0] * f, o[k][1] * f), pack_bf16x2(o[k][2] * f, o[k][3] * f));
+  }
 }
 
 template <int KB, int VB>
@@ -1070,7 +1165,8 @@ static int launch_tree(const CbTreeAttn& p, cudaStream_t st) {
   }
   const int rows = tr_rows(p.words, p.rows, p.Hq / p.Hkv);
   cudaError_t e = launch(tree_kernel<KB, VB>, dim3(sms[dev]), dim3(kTrThreads), smem, st, p, rows);
-  if (e == cudaSuccess) e = launch(tree_merge_kernel, dim3(sms[dev], (rows + 7) / 8), dim3(256), 0, st, p, rows);
+  const int step = rows <= kTrMergeFew ? 8 : 16;
+  if (e == cudaSuccess) e = launch(step == 8 ? tree_merge_kernel<1, 8> : tree_merge_kernel<2, 4>, dim3(sms[dev], (rows + step - 1) / step), dim3(256), 0, st, p, rows);
   return static_cast<int>(e);
 }
 
