@@ -137,6 +137,14 @@ def test_attention_of_many_requests():
     _Round([(int(r.integers(0, 300)), int(r.integers(0, 20))) for _ in range(150)], 8, 2, 8, 8, seed=6).check()
 
 
+@pytest.mark.parametrize("hq,hkv,requests", [(8, 2, 40), (64, 4, 5), (64, 4, 33), (6, 6, 70), (16, 1, 2)])
+def test_attention_of_trees_of_all_sizes_side_by_side(hq, hkv, requests):
+    """Trees of one tile's rows, of more, of many items and of none, behind contexts of no token to many: shares of the multiprocessors begin and end anywhere."""
+    r = np.random.default_rng(requests)
+    counts = [1, 64, 0, 33, 8, 17, 2, 40]
+    _Round([(int(r.integers(0, 4) and r.integers(0, 700)), counts[i % 8]) for i in range(requests)], hq, hkv, 8, 6, seed=requests).check()
+
+
 def test_attention_of_a_long_context_beside_short_ones():
     _Round([(9000, 30), (3, 1), (700, 64), (0, 2)], 16, 2, 4, 8, seed=7).check()
 
