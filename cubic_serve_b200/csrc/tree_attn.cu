@@ -112,7 +112,9 @@ __device__ __forceinline__ void tree_row(const CbTreeAttn& p, const TreeRequest&
 static constexpr int kTrTiles = 2, kTrRows = 128, kTrItemRows = kTrTiles * kTrRows;
 static constexpr int kTrPages = 4, kTrTok = kTrPages * kPageTokens;
 static constexpr int kTrThreads = 640;
-static constexpr int kTrRegs = 96, kTrRegsSoftmax = 136, kTrRegsConvert = 72, kTrRegsOther = 64;
+// Registers go to the softmax, whose loops keep a row's scores (64 x 16 behind 4096: with 128 of them 265 us, 136: 252, 144: 245), as long as the warps of the second line
+// spill nothing in their loops (32 x 64 with 56 and 48 for these: 127 us in place of 121).
+static constexpr int kTrRegs = 96, kTrRegsSoftmax = 144, kTrRegsConvert = 64, kTrRegsOther = 64;
 static_assert(2 * kTrRegsSoftmax + 2 * kTrRegsConvert + kTrRegsOther <= 5 * kTrRegs, "five warpgroups");
 static constexpr int kTrLists = 4, kTrRaw = 4;
 // Operands: of K of two steps, of V, which waits longer, of four.  A step's places, the four warps that convert it and, of items in both tiles, its tile go by its number in
@@ -895,17 +897,18 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
             }
             tmem_st_wait();
           }
-          float mx = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t a[32];
-            tmem_ld_32x32(tile + c * 32, a);
-            tmem_ld_wait();
-            float of[4] = {-INFINITY, -INFINITY, -INFINITY, mx};
+          // all scores into registers: the next step's replace them at once (2 x 64 behind 32000: 101 us; with the scores read again for the exponentials 109)
+          uint32_t a[2][32];
+          tmem_ld_32x32(tile, a[0]);
+          tmem_ld_32x32(tile + 32, a[1]);
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sm.s_free[t]));
+          float of[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) of[j / 2 & 3] = fmaxf(of[j / 2 & 3], fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
-            mx = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
-          }
+          for (int j = 0; j < 64; j += 2) of[j / 2 & 3] = fmaxf(of[j / 2 & 3], fmaxf(__uint_as_float(a[j >> 5][j & 31]), __uint_as_float(a[j >> 5][(j & 31) + 1])));
+          const float mx = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
           // (there before K was converted; written again after this step's product, which waits for what follows: kTrNotes)
           const float2 told = make_float2(sm.note[note].back, __int_as_float(sm.note[note].v_exp));
           const float mul = told.x * cur.mul, top = mx * mul;
@@ -930,14 +933,13 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
           float2 part_sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
+#pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t a[16], pr[8];
-            tmem_ld_32x16(tile + c * 16, a);
-            tmem_ld_wait();
+            uint32_t pr[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float2 d = __ffma2_rn(make_float2(__uint_as_float(a[2 * j]), __uint_as_float(a[2 * j + 1])), mul2, less);
+              const int at = c * 16 + 2 * j;
+              const float2 d = __ffma2_rn(make_float2(__uint_as_float(a[at >> 5][at & 31]), __uint_as_float(a[at >> 5][(at & 31) + 1])), mul2, less);
               const float2 x = make_float2(fast_exp2(d.x), fast_exp2(d.y));
               part_sum[j & 1] = __fadd2_rn(part_sum[j & 1], x);
               pr[j] = pack_f16x2(x.x, x.y);
@@ -945,9 +947,6 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
             tr_tmem_st8(tile + kTrTmemP + c * 8, pr);
           }
           sum += (part_sum[0].x + part_sum[0].y) + (part_sum[1].x + part_sum[1].y);
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sm.s_free[t]));
           if (__builtin_expect(s > first && __any_sync(0xffffffffu, grew), 0)) {
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
