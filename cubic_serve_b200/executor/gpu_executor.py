@@ -573,6 +573,7 @@ class GpuExecutor:
         self.graph_masks = True
         self.stage.d["mask"] = self._mask_dev
         self.stage.d.pop("whole", None)
+        self.stage.d.pop("adjust", None)
         rt = CudaGraphRuntime(resources=(0, 1))
         if isinstance(getattr(self.runner, "attn", None), torch.Tensor):
             with torch.cuda.stream(self.stream):

@@ -97,6 +97,17 @@ def test_biases_force_and_forbid(kind):
     runner.ws.check_status()
 
 
+def test_graphs_captured_behind_an_adjusted_step_hold_none_of_it():
+    eng, ex, runner = _engine()
+    p = _prompts(3)
+    base = _run(eng, [(q, _sampling()) for q in p])
+    assert all(set(o) == {42} for o in _run(eng, [(q, _sampling(logit_bias=((42, 100.0),))) for q in p]))
+    ex.capture_decode_graphs([4, 8])
+    assert _run(eng, [(q, _sampling()) for q in p]) == base
+    assert all(set(o) == {42} for o in _run(eng, [(q, _sampling(logit_bias=((42, 100.0),))) for q in p]))
+    runner.ws.check_status()
+
+
 @pytest.mark.parametrize("kb,vb,rotation", [(8, 8, False), (4, 8, True), (6, 6, False)])
 def test_tree_rounds_match_plain_greedy_and_accept_repetitions(kb, vb, rotation):
     eng, _, r0 = _engine("plain", kb=kb, vb=vb, rotation=rotation)
