@@ -2,8 +2,11 @@
 //
 // verify_tree: from node 0 on, the target's choice at a node is emitted; the first child that holds it is the next node, and without one the walk ends.
 // keep_tokens: the nodes of a path, path[0] = 0 < path[1] < .., lie at the slots start + path[k] of their request; line start + path[k] of every layer and
-// key / value head becomes line start + k.  path[k] >= k, so a line is read before anything is put in its place: all of a warp's lines are
-// loaded first.  A lane has four channels, and no other lane the words that hold them (K words of 4 bits: lanes t and t + 4 exchange their halves).
+// key / value head becomes line start + k.  path[k] >= k, so a line is read before anything is put in its place: a warp
+// loads four lines, puts them down and goes on.  A lane has four channels, and no other lane the words that hold them (K words of 4 bits: lanes t and t + 4 exchange their halves).
+//
+// Bound by latency, a few dependent trips to memory each: a warp walks a request's tree, 32 nodes a look; a warp moves the lines of a request, layer and head, so that
+// these fill the GPU.  Both together for a tree of 8 nodes and 36 layers 5 us, for 64 of 26 nodes 8 us.
 #include "paged_attn.cuh"
 
 // Packed by ops/native.py::VERIFY_TREE.

@@ -385,6 +385,10 @@ __device__ __forceinline__ uint2 tr_visible(const uint32_t* sees, int words, int
 // Powers of two keep operands in the range of f16: a row's for Q (undone with the softmax' scale: its 8 bits stay exact), a step's for K (likewise), one for V that grows
 // with the largest scale (undone with the output).  Items whose scales are further apart than that holds (2^18 in a step of K, 2^14 in a CTA's steps of V), or not finite,
 // are computed in fp32 (tree_row): a hundred times as long, for caches as no model has them.
+// Bound by instructions: 16384 scores and as many codes a step of 256 rows take half of all issue slots, on five warps a scheduler whose programs differ, so that
+// fewer instructions of straight code are worth more than fewer cycles of one role (any role's loops unrolled: 3 to 11 % slower). Matrix units are busy for a quarter of the time, memory
+// for less: 64 x 16 behind 4096 (8 bits, 32 / 8 heads) 250 us, 2.6 TB/s of the cache; 2 x 64 behind 32000 (K 4 bits, 32 / 4) 101 us; 32 x 64 behind up to 1500 (6 bits, 64 / 4) 121 us.
+// One request of 8 nodes behind 700 tokens is a chain of latencies: 15 us, of which the second launch is 4.
 // Every wait is bounded; on a timeout the roles leave, the status word is set and tensor memory is freed.
 template <int KBITS, int VBITS>
 __global__ void __launch_bounds__(kTrThreads, 1)

@@ -1016,7 +1016,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, page
     _require(n <= TREE_MAX_REQUESTS, "a launch takes up to 1024 requests")
     ldq, ldo = _rows(q, "q", torch.bfloat16), _rows(out, "out", torch.bfloat16)
     (rows, width), at = q.shape, q.data_ptr()
-    _require(width == hq * 128 and out.shape == q.shape and rows * (hq // hkv) < 1 << 31, "q and out: a row of all query heads for every node")
+    _require(width == hq * 128 and out.shape == q.shape and rows * (hq // hkv) < (1 << 31) - 256, "q and out: a row of all query heads for every node")
     _require((ldq | ldo) % 8 == 0 and (at | out.data_ptr()) % 16 == 0, "rows of q and out start on 16 bytes")
     ld, ldm, words = _rows(page_table, "page_table", i32), _rows(masks, "masks", i32), masks.shape[1]
     _require(masks.shape[0] >= rows and 1 <= words <= TREE_MAX_NODES // 32, "masks: one to eight words for every row")
