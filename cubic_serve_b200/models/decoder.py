@@ -448,7 +448,7 @@ class DecoderRunner(StepRunner):
     def _attend(self, b: StepBatch, q: torch.Tensor, out: torch.Tensor, kv: torch.Tensor, rb0: int, rb1: int) -> int:
         """Attention of the row blocks ``[rb0, rb1)``: portions of prompts in one launch, what is before and after them in
         one each.  Returns the launches."""
-        if b.trees is not None:
+        if getattr(b, "trees", None) is not None:
             request, row0, count, start, masks = b.trees
             rows = q.shape[0]
             K.tree_attention(q.view(rows, -1), out.view(rows, -1), kv, b.page_table, request, row0, count, start, masks, self.hq, self.hkv, self.D, self.k_bits,
