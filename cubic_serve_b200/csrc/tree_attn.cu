@@ -63,10 +63,11 @@ struct TreeLay {
                        vScale = vCode + kPageTokens * kD * VBITS / 8, bytes = vScale + kBytesOfScales, stride = (bytes + 127) & ~127;
 };
 
-// One row over the tokens [lo, hi) in fp32, by a warp whose lanes have four channels each.  `sees`: the row's words.
+// One row over the tokens [lo, hi) in fp32, by a warp whose lanes have four channels each.  `sees`: the row's words.  `alive` counts every 1024 tokens: the CTA's other
+// warps wait meanwhile, and their limit is one of time without progress.
 template <int KBITS, int VBITS>
 __device__ __forceinline__ void tree_row(const CbTreeAttn& p, const TreeRequest& r, int kvh, int lo, int hi, const uint32_t* sees, const __nv_bfloat16* q,
-                                         int lane, float& m, float& sum, float (&o)[4], bool& bad) {
+                                         int lane, float& m, float& sum, float (&o)[4], bool& bad, uint32_t* alive) {
   using L = TreeLay<KBITS, VBITS>;
   constexpr float kBias = 1 << (KBITS - 1), vBias = 1 << (VBITS - 1);
   const uint2 qw = reinterpret_cast<const uint2*>(q)[lane];
@@ -78,6 +79,7 @@ __device__ __forceinline__ void tree_row(const CbTreeAttn& p, const TreeRequest&
   for (int c = 0; c < 4; ++c) o[c] = 0.f;
 #pragma unroll 1
   for (int t = lo; t < hi; ++t) {
+    if (lane == 0 && (t & 1023) == 0) atomicAdd(alive, 1u);
     const int j = t - r.start;
     if (j >= 0 && !(sees[j >> 5] >> (j & 31) & 1u)) continue;
     const int page = tree_page(p, r.slot, t / kPageTokens, bad), tok = t % kPageTokens;
@@ -131,10 +133,27 @@ static constexpr int kTrApartK = 18, kTrApartV = 14;     // ... and the long one
 static constexpr int kTrHalf = kTrTok * 128;             // bytes of 64 channels of a step
 static constexpr uint32_t kTrTmemCols = 512, kTrTmemTile = 256, kTrTmemP = 64, kTrTmemQ = 96, kTrTmemO = 128;
 
-// mbar_wait_park with what follows a wait that is not over at once out of the way of the loops.
+// A bounded wait with what follows when it is not over at once out of the way of the loops.  The limit starts anew while the word behind the abort flag (TrSmem::abort_flag[1]) counts:
+// rows of the fp32 program take 370 ns a token, so that 32 of them behind 130000 tokens are longer than the limit.
 __device__ __forceinline__ bool tr_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
   if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
-  return mbar_wait_park(bar, parity, abort_flag);
+  long long t0 = 0;
+  uint32_t polls = 0, alive = 0;
+  while (true) {
+    if (mbar_try_wait_hint(bar, parity, 20000u)) return true;
+    if ((++polls & 0xFu) == 0) {
+      if (*abort_flag) return false;
+      const long long now = clock64();
+      const uint32_t counts = abort_flag[1];
+      if (t0 == 0 || counts != alive) {
+        t0 = now;
+        alive = counts;
+      } else if (now - t0 > kWaitBudgetCycles) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
 }
 // Where a role stands in a ring of n places, and the parity that it waits for there
 struct TrRing {
@@ -171,7 +190,7 @@ struct __align__(1024) TrSmem {
   TrItem list[kTrLists];
   float2 exch_ml[kTrTiles][kTrRows];                     // rows in both tiles: maximum and sum, ...
   int exch_exp[kTrTiles][kTrRows];                       // ... and v_exp
-  uint32_t tmem, abort_word;
+  uint32_t tmem, abort_flag[2];                          // [1]: progress of the fp32 program (tr_wait)
   long long upto[kTreeMaxRequests + 1], items[kTreeMaxRequests + 1];     // units of the requests before; their items' units a slot
 };
 
@@ -398,7 +417,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
   TrSmem& sm = *reinterpret_cast<TrSmem*>(smem_raw + (-smem_u32(smem_raw) & 1023u));      // (by way of an integer it would be a generic address)
   uint8_t* raw = reinterpret_cast<uint8_t*>(&sm + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv;
-  volatile uint32_t* abort_flag = &sm.abort_word;
+  volatile uint32_t* abort_flag = sm.abort_flag;
   float* part_o = p.partial;
   float2* part_ml = reinterpret_cast<float2*>(part_o + static_cast<size_t>(gridDim.x) * 2 * part_rows * kD);
   TrDesc* desc = reinterpret_cast<TrDesc*>(part_ml + static_cast<size_t>(gridDim.x) * 2 * part_rows);
@@ -431,7 +450,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
     }
     mbar_init(smem_u32(&sm.exch_full), 8);
     mbar_init(smem_u32(&sm.exch_free), 8);
-    sm.abort_word = 0;
+    sm.abort_flag[0] = sm.abort_flag[1] = 0;
     mbar_fence_init();
   }
   if (warp == 16) {
@@ -1051,7 +1070,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
             const long long q = __shfl_sync(0xffffffffu, cur.q, of), out = __shfl_sync(0xffffffffu, cur.out, of);
             const uint32_t* sees = reinterpret_cast<const uint32_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(cur.sees), of));
             float rm, rs, o[4];
-            tree_row<KBITS, VBITS>(p, r, l.kvh, lo, hi, sees, p.q + q, lane, rm, rs, o, bad);
+            tree_row<KBITS, VBITS>(p, r, l.kvh, lo, hi, sees, p.q + q, lane, rm, rs, o, bad, sm.abort_flag + 1);
             if (part >= 0) {
               part_to[static_cast<size_t>(lane) * part_rows - lane + of] = make_float4(o[0], o[1], o[2], o[3]);
               if (lane == 0) part_ml[at - lane + of] = make_float2(rm, rs);
@@ -1077,7 +1096,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
   __syncthreads();
   if (warp == 16) tmem_dealloc(tmem, kTrTmemCols);
   if (bad) atomicExch(p.status, static_cast<uint32_t>(kErrBadArgument));
-  if (tid == 0 && sm.abort_word) atomicExch(p.status, static_cast<uint32_t>(kErrBarrierTimeout));
+  if (tid == 0 && sm.abort_flag[0]) atomicExch(p.status, static_cast<uint32_t>(kErrBarrierTimeout));
 }
 
 // Joins the parts of items that several CTAs shared: block x looks after the item that began in CTA x and went on beyond it.  A warp's lanes are eight rows times four of

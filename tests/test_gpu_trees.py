@@ -312,6 +312,35 @@ def test_attention_on_a_stream_and_in_a_graph():
     ws.check_status()
 
 
+def test_values_far_apart_behind_a_long_context():
+    """A context of 160000 tokens whose scales take the program in 32 bits: all rows of an item of 256 by one CTA.
+
+    The context is the same 256 tokens over and over, so that each counts as often as it is there.  n products are summed in 32 bits, one after the other: each addition is
+    off by 2^-24 of what is there at most, in the sum and in the output.  A score is off by 2^-24 of the sum of its products' magnitudes for each of 16 roundings
+    at most, exponentials by 2^-20, the result by 2^-8."""
+    times, sms = 625, K.sm_count(torch.device(DEV, 0))
+    rd = _Round([(256, 64)], 4, 1, 8, 8, seed=21)
+    rd.scales()[1][int(rd.table[int(rd.slots[0]), 3])] *= 2.0 ** -24
+    ids = rd.table[int(rd.slots[0]), :20]
+    table = torch.cat([ids[:16].repeat(times), ids[16:]])[None].contiguous()
+    cache, _, _, _, _, _, masks, *rest = rd.args()
+    out, ws = torch.full((64 * sms, 4 * D), 7.0, device=DEV, dtype=torch.bfloat16), K.Workspace(torch.device(DEV, 0), 16, 16, 16)
+    K.tree_attention(rd.q.repeat(sms, 1), out, cache, table, _i32([0] * sms), _i32(np.arange(sms) * 64), _i32([64] * sms), _i32([256 * times] * sms), masks.repeat(sms, 1), *rest, ws=ws)
+    ws.check_status()
+    pages = [eager.decode_cache_page(rd.cache[p, 0].cpu(), D, 8, 8) for p in ids.tolist()]
+    k, v = (torch.cat([page[x] for page in pages]).double() for x in (0, 1))
+    q, n = rd.q.cpu().double().view(64, 4, D), 256 * times + 64
+    z = torch.einsum("cgd,td->cgt", q, k) * D ** -0.5
+    off = (torch.einsum("cgd,td->cgt", q.abs(), k.abs()) * D ** -0.5 * 16 * 2.0 ** -24).amax(-1, keepdim=True)
+    often = torch.full((64, 1, 320), float(times), dtype=torch.float64)
+    often[:, 0, 256:] = torch.from_numpy(((rd.sees[:, :, None] >> np.arange(32, dtype=np.uint32)) & 1).reshape(64, -1).astype(np.float64))
+    p = often * torch.exp(z - z.amax(-1, keepdim=True))
+    p = p / p.sum(-1, keepdim=True)
+    ref, tol = torch.einsum("cgt,td->cgd", p, v), (torch.expm1(2 * off) + 2 * n * 2.0 ** -24 + 2.0 ** -19) * torch.einsum("cgt,td->cgd", p, v.abs())
+    assert bool(((out[:64].cpu().double() - ref.reshape(64, -1)).abs() <= (tol + 2.0 ** -8 * ref.abs()).reshape(64, -1)).all())
+    assert torch.equal(out, out[:64].repeat(sms, 1))
+
+
 def test_no_requests():
     rd = _Round([(30, 5)], 4, 2, 8, 8, seed=17)
     cache, table, slots, row0, count, start, *rest = rd.args()
