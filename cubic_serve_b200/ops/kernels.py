@@ -993,6 +993,17 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> int:
     return ld
 
 
+def _apart_or_same(a: torch.Tensor, b: torch.Tensor, lda: int, ldb: int) -> bool:
+    """Whether two matrices of one shape and type, of neighbouring elements, are the same one or share no element (rows of the one may
+    lie between rows of the other where the row strides are equal)."""
+    rows, cols = a.shape
+    size = a.element_size()
+    apart, lda, ldb = (b.data_ptr() - a.data_ptr()) // size, lda if rows > 1 else cols, ldb if rows > 1 else cols
+    if apart == 0 and lda == ldb or apart >= (rows - 1) * lda + cols or -apart >= (rows - 1) * ldb + cols:
+        return True
+    return rows > 1 and lda == ldb and cols <= apart % lda <= lda - cols
+
+
 @functools.lru_cache(maxsize=256)
 def _tree_floats(device: int, words: int, rows: int, group: int) -> int:
     return native.lib().cb_tree_attn_floats(sm_count(torch.device("cuda", device)), words, rows, group)
@@ -1043,7 +1054,8 @@ def adjust_logits(logits: torch.Tensor, request: torch.Tensor | None, history: t
                   repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None, presence: torch.Tensor | None = None,
                   bias: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None, mask: torch.Tensor | None = None,
                   drafts: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """Logits (bf16 or fp32 ``[rows, vocab]``) as the requests want them (``csrc/adjust_logits.cu``); in place without ``out``.
+    """Logits (bf16 or fp32 ``[rows, vocab]``) as the requests want them (``csrc/adjust_logits.cu``); in place without ``out``,
+    which otherwise shares no element with them.
 
     Row ``r`` belongs to request ``request[r]`` (int32; None: request r; below 0: none, only ``mask`` applies).  ``history`` int32
     ``[n, most]`` holds the requests' tokens, ``length[n]`` of them, the first ``prompt[n]`` (None: none) the prompt's.  A token of the
@@ -1064,6 +1076,7 @@ def adjust_logits(logits: torch.Tensor, request: torch.Tensor | None, history: t
     else:
         ldo = _rows(out, "out", logits.dtype)
         _require(out.shape == logits.shape, "out: as many logits")
+        _require(_apart_or_same(logits, out, ldl, ldo), "out: the logits themselves, or memory apart from theirs")
     ldh = _rows(history, "history", i32)
     n, most = history.shape
     _require(most < (1 << 20) - 256, "a history of less than 2^20 tokens")

@@ -79,6 +79,21 @@ def test_adjust_logits_refuses(change):
         K.adjust_logits(**_adjust_args(**change))
 
 
+@pytest.mark.parametrize("logits,out,fits", [
+    ((0, 100, 100), (400, 100, 100), True), ((400, 100, 100), (0, 100, 100), True), ((0, 100, 100), (0, 100, 100), True),        # beside, and the same
+    ((0, 100, 100), (399, 100, 100), False), ((399, 100, 100), (0, 100, 100), False), ((0, 100, 100), (8, 100, 100), False), ((8, 100, 100), (0, 100, 100), False),
+    ((0, 200, 100), (100, 200, 100), True), ((100, 200, 100), (0, 200, 100), True), ((0, 200, 100), (99, 200, 100), False), ((0, 200, 100), (101, 200, 100), False),
+    ((0, 200, 100), (300, 200, 100), True), ((0, 208, 100), (104, 208, 100), True), ((0, 200, 100), (0, 100, 100), False), ((0, 100, 100), (0, 200, 100), False),
+])
+def test_results_of_adjusted_logits_beside_them_or_in_place(logits, out, fits):
+    """``(first element, row stride, columns)`` of four rows of one buffer; what is accepted reaches the next check, which refuses for the GPU's sake."""
+    buffer = torch.zeros(1200)
+    a, b = (buffer[at:].as_strided((4, cols), (ld, 1), at) for at, ld, cols in (logits, out))
+    with pytest.raises(ValueError) as e:
+        K.adjust_logits(**_adjust_args(logits=a, out=b))
+    assert ("apart" in str(e.value)) != fits
+
+
 @pytest.mark.parametrize("change", [
     dict(tokens=_ints(5)), dict(parents=torch.ones(6)), dict(row0=torch.ones(2)), dict(count=_ints(1)), dict(accepted=_ints(1)), dict(path=torch.zeros(1, 4, dtype=I32)),
     dict(path=torch.zeros(2, 3, dtype=I32)), dict(path=torch.zeros(2, 8, dtype=I32)[:, ::2]), dict(emitted=torch.zeros(2, 4)), dict(path=torch.zeros(2, 0, dtype=I32), emitted=torch.zeros(2, 0, dtype=I32)), dict(),
