@@ -121,7 +121,12 @@ keep_tokens_kernel(const CbKeepTokens p, const KvLayout lay) {
       const int at = t / kPageTokens, page = at < p.width ? table[at] : -1;
       return page >= 0 && page < p.pages ? cache + (static_cast<size_t>(page) * p.Hkv + head) * lay.blob_bytes : nullptr;
     };
-    int before = 0;
+    // the whole path before any line moves: it rises, and all its pages are there
+    for (int k = 1 + lane; k <= accepted; k += 32) {
+      const int at = path[k];
+      bad = bad || at <= (k > 1 ? path[k - 1] : 0) || at > (1 << 30) - start || (at != k && (line(start + at) == nullptr || line(start + k) == nullptr));
+    }
+    bad = __any_sync(0xffffffffu, bad);
     for (int k0 = 1; k0 <= accepted && !bad; k0 += kLines) {
       uint32_t kc[kLines], vc[kLines];
       float ks[kLines], vs[kLines];
@@ -129,20 +134,11 @@ keep_tokens_kernel(const CbKeepTokens p, const KvLayout lay) {
       int tok[kLines];
 #pragma unroll
       for (int l = 0; l < kLines; ++l) {
-        const int k = k0 + l;
+        const int k = k0 + l, at = k <= accepted ? path[k] : k;
         to[l] = nullptr;
-        if (k > accepted || bad) continue;
-        const int at = path[k];
-        bad = at <= before || at > (1 << 30) - start;
-        before = at;
-        if (bad || at == k) continue;
+        if (at == k) continue;
         const uint8_t* from = line(start + at);
         to[l] = line(start + k);
-        if (from == nullptr || to[l] == nullptr) {
-          bad = true;
-          to[l] = nullptr;
-          continue;
-        }
         const int src = (start + at) % kPageTokens;
         tok[l] = (start + k) % kPageTokens;
         kc[l] = pf_codes_k<KBITS>(from, src, lane);

@@ -584,6 +584,24 @@ def test_paths_that_do_not_rise_and_pages_that_are_not_there_move_nothing_and_ar
         assert all(torch.equal(a, b) for a, b in zip(now, caches))
 
 
+@pytest.mark.parametrize("path,page", [([0, 3, 2], None), ([0, 2, 4, 6, 8, 8, 9], None), ([0, 2, 4, 6, 8, 9, -1], None), (list(range(0, 70, 2)) + [60], None),
+                                       ([0, 3, 20], 1), ([0, 3, 4, 9, 20, 21], 1), ([0, 3, 4, 5, 6, 7, 8, 9, 40], 3)])
+def test_paths_that_are_wrong_further_on_move_nothing(path, page):
+    """Lines of a path before the place where it is wrong stay, and other requests' move."""
+    paths = [path, [0, 3, 5]]
+    caches, table, want_path, accepted = _keep_case(2, 10, 2, 8, 8, paths, seed=4)
+    if page is not None:
+        table[0, page] = -1
+    now, only = ([c.clone() for c in caches] for _ in range(2))
+    ws = K.Workspace(torch.device(DEV, 0), 16, 16, 16)
+    K.keep_tokens(K.LayerCaches(now, 2, D, 8, 8), _i32(table), _i32([0, 1]), _i32([10] * 2), _i32(accepted), _i32(want_path), ws=ws)
+    with pytest.raises(NativeLibraryError):
+        ws.check_status()
+    K.keep_tokens(K.LayerCaches(only, 2, D, 8, 8), _i32(table), _i32([1]), _i32([10]), _i32(accepted[1:]), _i32(want_path[1:]), ws=ws)
+    ws.check_status()
+    assert all(torch.equal(a, b) for a, b in zip(now, only)) and not all(torch.equal(a, b) for a, b in zip(now, caches))
+
+
 # ------------------------------------------------------------------------------------------------- together
 @pytest.mark.parametrize("kb,vb", [(8, 8), (4, 8), (6, 6)])
 def test_a_round_leaves_the_cache_of_a_chain(kb, vb):
