@@ -9,6 +9,7 @@ through per-request queues with batched wake-ups (``runtime/token_stream.py:38,2
 from __future__ import annotations
 
 import asyncio
+import logging
 import threading
 import time
 from collections import deque
@@ -20,6 +21,8 @@ from ..generation.output import GenerationOutputPipeline
 from ..inputs.chat import ChatInputProcessor
 from .engine import EnginePoisoned, LLMEngine
 from .scheduler import AdmissionError, FinishReason, SamplingParams
+
+log = logging.getLogger(__name__)
 
 
 class TokenStream:
@@ -88,6 +91,7 @@ class TokenChatBackend:
         self.default_max_tokens = default_max_tokens
         self.model_names: frozenset[str] = frozenset()       # what the model itself is called: no adapter's name
         self.ready = True
+        self._left_aside = False         # whether it was said that penalties and biases are
         self._lock = threading.Lock()
         self._inbox: deque = deque()
         self._live: dict[str, _Live] = {}
@@ -144,11 +148,7 @@ class TokenChatBackend:
         sp = SamplingParams(temperature=s.temperature, top_p=s.top_p, top_k=s.top_k, seed=s.seed, max_tokens=max_tokens,
                             stop_token_ids=tuple(s.stop_token_ids) + ((eos,) if eos is not None else ()),
                             matcher=matcher, adapter=req.model if req.model in self.adapter_names else None, whole_vocabulary=s.whole_vocabulary, min_p=s.min_p,
-                            repetition_penalty=s.repetition_penalty, logit_bias=s.logit_bias,
-                            # (executors that do not adjust logits have always left these two aside)
-                            **({"frequency_penalty": s.frequency_penalty, "presence_penalty": s.presence_penalty}
-                               if getattr(self.engine.executor, "accepts_adjustments", False) else {}),
-                            thinking_budget=req.reasoning.budget_tokens if prepared.starts_in_reasoning else None)
+                            **self._adjustments(s), thinking_budget=req.reasoning.budget_tokens if prepared.starts_in_reasoning else None)
         with self._lock:
             self._live[req.request_id] = live
             if plan is None or not plan.jobs:
@@ -165,6 +165,17 @@ class TokenChatBackend:
             self.processor.submit(plan).add_done_callback(encoded)
         self._wake.set()
         return self._events(live)
+
+    def _adjustments(self, s) -> dict:
+        """The penalties and biases of a request; on an executor that does not adjust logits none, as ever: its requests may carry these
+        fields, and they change nothing."""
+        wanted = {"repetition_penalty": s.repetition_penalty, "frequency_penalty": s.frequency_penalty, "presence_penalty": s.presence_penalty, "logit_bias": s.logit_bias}
+        if getattr(self.engine.executor, "accepts_adjustments", False):
+            return wanted
+        if SamplingParams(**wanted).adjusts and not self._left_aside:
+            self._left_aside = True
+            log.warning("requests ask for penalties or logit_bias, which %s leaves aside", type(self.engine.executor).__name__)
+        return {}
 
     def _reasoning_end_sequence(self) -> list[int]:
         """Token ids of the marker that closes a reasoning block (empty when the tokenizer cannot encode it)."""

@@ -248,6 +248,48 @@ def test_real_backend_end_to_end_on_cpu():
     assert eng.pool.num_used == len(eng.prefix)
 
 
+@pytest.mark.parametrize("adjusts", [False, True])
+def test_penalties_and_biases_of_requests_by_executor(adjusts):
+    """An executor that adjusts logits is told all four; requests to another one run as if they had said nothing."""
+    from cubic_serve_b200.executor.eager_executor import EagerPagedExecutor
+    from cubic_serve_b200.inputs.chat import ByteTokenizer
+    from cubic_serve_b200.models.config import ModelConfig
+    from cubic_serve_b200.models.reference import random_dense_weights
+    from cubic_serve_b200.runtime.async_engine import TokenChatBackend
+    from cubic_serve_b200.runtime.engine import LLMEngine
+    from cubic_serve_b200.runtime.scheduler import SchedulerConfig
+
+    tok = ByteTokenizer()
+    cfg = ModelConfig(num_layers=1, hidden_size=64, num_q_heads=2, num_kv_heads=1, head_dim=32, intermediate_size=128, vocab_size=tok.vocab_size)
+    ex, told = EagerPagedExecutor(cfg, random_dense_weights(cfg, 0), 64), []
+    execute = ex.execute
+
+    def recorded(segs):
+        told.extend(s.adjust for s in segs if s.sample)
+        return execute(segs)
+    ex.execute, ex.accepts_adjustments = recorded, adjusts
+    eng = LLMEngine(ex, 64, SchedulerConfig(max_running_requests=4, max_model_len=512, max_batched_tokens=256))
+    fields = {"repetition_penalty": 1.25, "frequency_penalty": 0.5, "presence_penalty": -0.75, "logit_bias": {"17": 2.5}}
+
+    async def go():
+        backend = TokenChatBackend(eng, tok, default_max_tokens=4)
+        body = {"model": "toy", "messages": [{"role": "user", "content": "hello"}], "max_tokens": 4, "temperature": 0}
+        plain = await _call(CubicASGIApp(backend, "toy"), "POST", "/v1/chat/completions", body)
+        n = len(told)
+        each = [await _call(CubicASGIApp(backend, "toy"), "POST", "/v1/chat/completions", {**body, k: v}) for k, v in fields.items()]
+        backend.close()
+        return plain, each, told[n:]
+
+    (status, text), each, seen = asyncio.run(go())
+    assert [status] + [s for s, _ in each] == [200] * 5
+    if adjusts:
+        got = [(a.repetition, a.frequency, a.presence, a.bias) for a in seen]
+        assert sorted(set(got)) == sorted([(1.25, 0.0, 0.0, ()), (1.0, 0.5, 0.0, ()), (1.0, 0.0, -0.75, ()), (1.0, 0.0, 0.0, ((17, 2.5),))])
+    else:
+        assert set(seen) == {None}
+        assert all(json.loads(t)["choices"][0]["message"] == json.loads(text)["choices"][0]["message"] for _, t in each)
+
+
 def test_sampling_defaults_from_generation_config(tmp_path):
     from cubic_serve_b200.inputs.normalize import (normalize_anthropic_messages, normalize_openai_chat_completions,
                                                    sampling_defaults_from_generation_config)
