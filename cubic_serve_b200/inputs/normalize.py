@@ -166,7 +166,9 @@ def _logit_bias(body) -> tuple[tuple[int, float], ...]:
     _require(isinstance(bias, dict), "logit_bias must be an object", "logit_bias")
     out = []
     for t, v in bias.items():
-        _require(isinstance(t, str) and t.isdecimal() and isinstance(v, (int, float)) and not isinstance(v, bool), "logit_bias maps token ids to numbers", "logit_bias")
+        _require(isinstance(t, str) and len(t) <= 100 and t.isdecimal() and isinstance(v, (int, float)) and not isinstance(v, bool),
+                 "logit_bias maps token ids to numbers", "logit_bias")
+        _require(-100 <= v <= 100, "logit_bias must map tokens to numbers in [-100, 100]", "logit_bias")
         out.append((int(t), float(v)))
     return tuple(out)
 
@@ -224,7 +226,7 @@ def normalize_openai_chat_completions(body: Any, default_model: str | None = Non
         presence_penalty=float(_as_number(body, "presence_penalty", 0.0, -2.0, 2.0)),
         frequency_penalty=float(_as_number(body, "frequency_penalty", 0.0, -2.0, 2.0)),
         logprobs=bool(body.get("logprobs", False)), top_logprobs=tlp,
-        whole_vocabulary=whole, min_p=min_p, repetition_penalty=float(_as_number(body, "repetition_penalty", 1.0)), logit_bias=_logit_bias(body))
+        whole_vocabulary=whole, min_p=min_p, repetition_penalty=float(_as_number(body, "repetition_penalty", 1.0, 0, 100)), logit_bias=_logit_bias(body))
     tools, choice = _openai_tools(body)
     structured = _openai_structured(body)
     _require(not (structured.kind != StructuredKind.NONE and choice.mode in ("required", "named")),

@@ -146,6 +146,16 @@ def test_requests_say_what_their_logits_are():
             normalize_openai_chat_completions({**body, **bad})
 
 
+@pytest.mark.parametrize("bad", [{"logit_bias": {"3": 10 ** 400}}, {"logit_bias": {"3": -10 ** 400}}, {"logit_bias": {"9" * 5000: 1}},
+                                 {"repetition_penalty": 10 ** 400}])
+def test_numbers_of_any_length_are_requests_errors(bad):
+    """Whole numbers in JSON may be longer than what Python turns into a float, or a text into a number."""
+    from cubic_serve_b200.contracts.request import RequestError
+    from cubic_serve_b200.inputs.normalize import normalize_openai_chat_completions
+    with pytest.raises(RequestError):
+        normalize_openai_chat_completions({"model": "m", "messages": [{"role": "user", "content": "hi"}], **bad})
+
+
 def test_sampling_parameters_of_adjustments():
     from cubic_serve_b200.runtime.scheduler import SamplingParams
     assert not SamplingParams().adjusts and SamplingParams(presence_penalty=0.1).adjusts and SamplingParams(logit_bias=((1, 2.0),)).adjusts
