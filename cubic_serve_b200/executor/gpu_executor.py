@@ -435,9 +435,6 @@ class GpuExecutor:
         assert self.max_tokens <= runner.max_tokens
         if runner.cfg.is_hybrid and max_rows > runner.max_requests:
             raise ValueError("the runner's recurrent state has fewer rows than the executor has request slots")
-        # penalties and biases likewise: a row's logits on one GPU, and drafts that are verified against them where rounds do that
-        self.accepts_adjustments = self.accepts_vocabulary_draws
-        self._adjustments = None
         # the low-rank adapters that requests may name (speculative rounds compute and verify without)
         self.low_rank = getattr(runner, "low_rank", None) if type(self) is GpuExecutor else None
         self.builder = BatchBuilder(max_rows * rows_per_request, self.max_tokens, max_model_len,
@@ -445,6 +442,9 @@ class GpuExecutor:
         self.stage = self.builder.stage
         self._fill = self.builder._fill
         self.invalidate_page_rows = self.builder.invalidate_page_rows
+        # penalties and biases likewise: a row's logits on one GPU, and drafts that are verified against them where rounds do that
+        self.accepts_adjustments = self.accepts_vocabulary_draws and self._adjustable()
+        self._adjustments = None
         v_local = runner.w.lm_head.n
         self.logits = torch.empty(max_rows, v_local, dtype=getattr(runner, "logits_dtype", torch.bfloat16), device=self.device)
         # a step's sampled ids, behind what its layout on the device says of it: one copy brings both
@@ -546,6 +546,10 @@ class GpuExecutor:
             with torch.cuda.stream(self.stream):
                 self.stage.d["adjust"] = self._request_adjustments().stage(wanted)
         return n
+
+    def _adjustable(self) -> bool:
+        """Whether ``K.adjust_logits`` takes this model's vocabulary and the longest text of a request."""
+        return self.runner.w.lm_head.n <= K.ADJUST_MAX_VOCAB and self.builder.max_pages * K.PAGE_TOKENS <= K.ADJUST_MAX_HISTORY
 
     def _request_adjustments(self) -> Adjustments:
         if self._adjustments is None:

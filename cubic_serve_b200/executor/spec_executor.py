@@ -583,7 +583,7 @@ class NgramTreeSpeculativeGpuExecutor(NgramSpeculativeGpuExecutor):
         kw["max_model_len"] = kw.get("max_model_len", 4096) + nodes          # drafts lie behind a request's last position for the length of a round
         super().__init__(runner, nodes - 1, **kw)
         self.draft_depth, self.draft_branches = depth, branches
-        self.accepts_adjustments = True
+        self.accepts_adjustments = self._adjustable()
         self.words = -(-nodes // 32)
         self.caches = K.LayerCaches(list(runner.kv), runner.hkv, runner.D, runner.k_bits, runner.v_bits)
         rows, dev = self.max_rows, self.device

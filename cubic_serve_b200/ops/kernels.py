@@ -981,6 +981,7 @@ def sample_vocabulary(logits: torch.Tensor, out_ids: torch.Tensor, temperature: 
 
 # ------------------------------------------------------------------ drafts in trees, and what requests say about their tokens
 TREE_MAX_REQUESTS, TREE_MAX_NODES, TREE_MAX_GROUP = 1024, 256, 128
+ADJUST_MAX_VOCAB, ADJUST_MAX_HISTORY = 1 << 20, (1 << 20) - 257
 
 
 def _rows(t: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> int:
@@ -1069,7 +1070,7 @@ def adjust_logits(logits: torch.Tensor, request: torch.Tensor | None, history: t
     _require(logits.dtype in (torch.bfloat16, f32), "logits are a bf16 or fp32 matrix")
     ldl = _rows(logits, "logits")
     rows, vocab = logits.shape
-    _require(1 <= vocab <= 1 << 20 and rows <= 65535, "up to 65535 rows of one to 2^20 logits")
+    _require(1 <= vocab <= ADJUST_MAX_VOCAB and rows <= 65535, "up to 65535 rows of one to 2^20 logits")
     ldo = ldl
     if out is None:
         out = logits
@@ -1079,7 +1080,7 @@ def adjust_logits(logits: torch.Tensor, request: torch.Tensor | None, history: t
         _require(_apart_or_same(logits, out, ldl, ldo), "out: the logits themselves, or memory apart from theirs")
     ldh = _rows(history, "history", i32)
     n, most = history.shape
-    _require(most < (1 << 20) - 256, "a history of less than 2^20 tokens")
+    _require(most <= ADJUST_MAX_HISTORY, "a history of less than 2^20 tokens")
     _require(request is not None or n >= rows, "request: whose rows they are")
     b = (0, 0, 0, 0)
     if bias is not None:

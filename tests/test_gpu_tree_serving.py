@@ -178,3 +178,25 @@ def test_drafts_near_the_end_of_the_model_length_and_of_requests():
     assert [len(o) for o in out] == [8, 1, 2]
     runner.ws.check_status()
     assert eng.pool.num_used == 0
+
+
+@pytest.mark.parametrize("kind", ["plain", "tree"])
+@pytest.mark.parametrize("length,accepts", [((1 << 20) - 300, True), (1 << 20, False)])
+def test_engines_of_longer_texts_than_penalties_look_at_refuse_them_at_once(kind, length, accepts):
+    from cubic_serve_b200.executor.gpu_executor import GpuExecutor
+    from cubic_serve_b200.executor.spec_executor import NgramTreeSpeculativeGpuExecutor
+    from cubic_serve_b200.runtime.engine import LLMEngine
+    from cubic_serve_b200.runtime.scheduler import AdmissionError, SchedulerConfig
+    _, _, runner = _engine("plain", False)
+    kw = dict(max_rows=2, max_prefill_tokens=64, max_model_len=length)
+    ex = GpuExecutor(runner, use_graphs=False, **kw) if kind == "plain" else NgramTreeSpeculativeGpuExecutor(runner, 3, 4, use_graphs=False, **kw)
+    eng = LLMEngine(ex, 256, SchedulerConfig(max_running_requests=2, max_model_len=length, max_batched_tokens=64, enable_prefix_cache=False))
+    assert ex.accepts_adjustments == accepts
+    wish = _sampling(max_tokens=3, logit_bias=((42, 100.0),))
+    if accepts:
+        assert _run(eng, [([1, 2, 3], wish)]) == [[42] * 3]
+    else:
+        with pytest.raises(AdmissionError):
+            eng.add_request([1, 2, 3], wish)
+    assert len(_run(eng, [([1, 2, 3], _sampling(max_tokens=3))])[0]) == 3
+    runner.ws.check_status()
