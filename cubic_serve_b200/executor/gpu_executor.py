@@ -67,7 +67,8 @@ class Segment:
 class _Staging:
     """Typed views over one pinned host buffer and its device mirror."""
 
-    def __init__(self, max_tokens: int, max_rows: int, max_row_blocks: int, max_pages: int, device, adapters: bool = False) -> None:
+    def __init__(self, max_tokens: int, max_rows: int, max_row_blocks: int, max_pages: int, device, adapters: bool = False, slots: int | None = None) -> None:
+        slots = max_rows if slots is None else slots
         self.max_tokens, self.max_rows, self.max_row_blocks, self.max_pages = max_tokens, max_rows, max_row_blocks, max_pages
         fields = [
             ("token_ids", np.int32, max_tokens),
@@ -85,7 +86,7 @@ class _Staging:
             ("positions", np.int32, max_tokens), ("slots", np.int32, max_tokens),
             ("rb_req", np.int32, max_row_blocks), ("rb_qstart", np.int32, max_row_blocks),
             ("rb_qcount", np.int32, max_row_blocks), ("rb_ctx", np.int32, max_row_blocks),
-            ("page_table", np.int32, max_rows * max_pages),
+            ("page_table", np.int32, slots * max_pages),
             # row- and column-axis rotary positions of multimodal prefill steps (``positions`` is the temporal axis)
             ("positions_h", np.int32, max_tokens), ("positions_w", np.int32, max_tokens),
         ]
@@ -106,8 +107,8 @@ class _Staging:
             size = np.dtype(dt).itemsize * n
             self.h[name] = self.h_np[o:o + size].view(dt)
             self.d[name] = self.dev[o:o + size].view(tmap[dt])
-        self.d["page_table"] = self.d["page_table"].view(max_rows, max_pages)
-        self.h["page_table"] = self.h["page_table"].reshape(max_rows, max_pages)
+        self.d["page_table"] = self.d["page_table"].view(slots, max_pages)
+        self.h["page_table"] = self.h["page_table"].reshape(slots, max_pages)
 
     @property
     def lengths_bytes(self) -> int:
@@ -137,8 +138,11 @@ def capturing(graph: "torch.cuda.CUDAGraph", stream: "torch.cuda.Stream"):
 class BatchBuilder:
     """Host side of a step: turns segments into the staged metadata arrays (no CUDA calls except the upload)."""
 
-    def __init__(self, max_rows: int, max_tokens: int, max_model_len: int, group: int, kv_heads: int, device, adapters: bool = False) -> None:
-        """``adapters``: rows carry the slots of low-rank adapters (``Segment.adapter``)."""
+    def __init__(self, max_rows: int, max_tokens: int, max_model_len: int, group: int, kv_heads: int, device, adapters: bool = False,
+                 slots: int | None = None) -> None:
+        """``max_rows``: sampled rows of a step, as many as request slots; ``slots``: the latter where they are fewer (rounds sample
+        several rows a request).  ``adapters``: rows carry the slots of low-rank adapters (``Segment.adapter``)."""
+        self.slots = slots = max_rows if slots is None else slots
         self.adapters = adapters
         self.qb = 16 // group                                   # query positions per attention row block
         self.kv_heads = kv_heads
@@ -146,11 +150,11 @@ class BatchBuilder:
         self.max_tokens = max_tokens
         self.max_pages = -(-max_model_len // K.PAGE_TOKENS)
         max_rb = max(max_rows, max_tokens // self.qb + max_rows)
-        self.stage = _Staging(max_tokens, max_rows, max_rb, self.max_pages, device, adapters)
+        self.stage = _Staging(max_tokens, max_rows, max_rb, self.max_pages, device, adapters, slots)
         self.device = device
-        self._page_rows: list[tuple[int, int]] = [(-2, 0)] * max_rows
+        self._page_rows: list[tuple[int, int]] = [(-2, 0)] * slots
         # steps that are laid out on the device: whose pages its table holds, and how many; what it is given, as [pages held | new pages]
-        self._device_uid, self._device_held = np.full(max_rows, -2, dtype=np.int64), np.zeros(max_rows, dtype=np.int32)
+        self._device_uid, self._device_held = np.full(slots, -2, dtype=np.int64), np.zeros(slots, dtype=np.int32)
         self.given_host = self.given = None
 
     def _splits(self, row_blocks: int, decode: bool = False) -> int:
@@ -249,7 +253,7 @@ class BatchBuilder:
         """What ``stage_layout`` fills.  An executor makes it before its first step: memory of the caller's stream, that the steps' stream
         is to write, has to be free of what the caller's stream still does with it."""
         if self.given is None:
-            n = self.max_rows * (self.max_pages + 1)
+            n = self.slots * (self.max_pages + 1)
             self.given_host = torch.empty(n, dtype=torch.int32, pin_memory=torch.cuda.is_available())
             self.given = torch.empty(n, dtype=torch.int32, device=self.device)
 
@@ -416,7 +420,7 @@ class BatchBuilder:
 class GpuExecutor:
     def __init__(self, runner: DecoderRunner, max_rows: int = 256, max_prefill_tokens: int = 8192,
                  max_model_len: int = 4096, use_graphs: bool = True, rows_per_request: int = 1, device_layout: bool = False) -> None:
-        """``rows_per_request`` > 1 sizes the sampled-row staging for speculative review (K + 1 rows per request).
+        """``rows_per_request`` > 1 sizes the sampled-row staging for speculative review (K + 1 rows per request, as many as a pass has tokens).
         ``device_layout``: positions, cache slots, row blocks and the block table of a step are made on the GPU from the lengths of its
         requests (``K.step_layout``) and only the lengths, the new pages and the sampling parameters are uploaded; steps with media
         positions and speculative rounds keep the host's."""
@@ -437,8 +441,10 @@ class GpuExecutor:
             raise ValueError("the runner's recurrent state has fewer rows than the executor has request slots")
         # the low-rank adapters that requests may name (speculative rounds compute and verify without)
         self.low_rank = getattr(runner, "low_rank", None) if type(self) is GpuExecutor else None
-        self.builder = BatchBuilder(max_rows * rows_per_request, self.max_tokens, max_model_len,
-                                    runner.hq // runner.hkv, runner.hkv, self.device, adapters=self.low_rank is not None)
+        # every step uploads the block table: a row for each request, and for rounds one that no request has (padding of a captured review)
+        sampled = min(max_rows * rows_per_request, self.max_tokens)
+        self.builder = BatchBuilder(sampled, self.max_tokens, max_model_len, runner.hq // runner.hkv, runner.hkv, self.device,
+                                    adapters=self.low_rank is not None, slots=max_rows + (rows_per_request > 1))
         self.stage = self.builder.stage
         self._fill = self.builder._fill
         self.invalidate_page_rows = self.builder.invalidate_page_rows
@@ -448,7 +454,7 @@ class GpuExecutor:
         v_local = runner.w.lm_head.n
         self.logits = torch.empty(max_rows, v_local, dtype=getattr(runner, "logits_dtype", torch.bfloat16), device=self.device)
         # a step's sampled ids, behind what its layout on the device says of it: one copy brings both
-        self._result = torch.zeros(4 + max_rows * rows_per_request, dtype=torch.int32, device=self.device)
+        self._result = torch.zeros(4 + sampled, dtype=torch.int32, device=self.device)
         self.out_ids = self._result[4:]
         # two result buffers: a step may be launched before the previous step's ids have been read (``launch`` / ``collect``)
         self._result_host = torch.zeros(2, self._result.numel(), dtype=torch.int32, pin_memory=torch.cuda.is_available())
@@ -495,7 +501,7 @@ class GpuExecutor:
     def _mask_buffers(self) -> None:
         if getattr(self, "_mask_host", None) is None:
             words = -(-self.cfg.vocab_size // 32)
-            rows = self.out_ids.numel()
+            rows = self.max_rows                   # (the review rows of rounds have masks of their own)
             self._mask_host = torch.empty(rows, words, dtype=torch.int32, pin_memory=torch.cuda.is_available())
             self._mask_dev = torch.full((rows, words), -1, dtype=torch.int32, device=self.device)     # everything allowed
             self._mask_rows_dirty = 0

@@ -1,5 +1,6 @@
 """Host-side batch staging: decode fast path, prefill row blocks, padding rows, incremental page-table rows."""
 import numpy as np
+import pytest
 
 from cubic_serve_b200.executor.gpu_executor import BatchBuilder, Segment
 
@@ -122,3 +123,16 @@ def test_three_axis_positions_and_feature_rows_are_staged():
     assert b3.positions_hw is None
     b4, _ = bb.fill([Segment(0, [5], 40, [3, 4, 5], positions3=np.full((3, 1), 33, np.int32)), Segment(1, [6], 20, [6, 7])])
     assert h["positions"][:2].tolist() == [33, 20] and h["rb_ctx"][:2].tolist() == [41, 21]
+
+
+def test_rounds_of_many_rows_have_a_block_table_of_their_requests():
+    """What a step uploads does not grow with the rows of a request: 256 requests of 113 rows, 8192 tokens long."""
+    few = BatchBuilder(max_rows=256, max_tokens=8192, max_model_len=8192, group=4, kv_heads=8, device="cpu")
+    many = BatchBuilder(max_rows=8192, max_tokens=8192, max_model_len=8192 + 113, group=4, kv_heads=8, device="cpu", slots=257)
+    assert many.stage.h["page_table"].shape == (257, -(-(8192 + 113) // 16)) and many.stage.nbytes < few.stage.nbytes + (1 << 20)
+    b, rows = many._fill([Segment(256, [1, 2, 3], 20, [4, 5], True, uid=1), Segment(3, [9], 0, [7], True, uid=2)])
+    assert rows == 2 and many.stage.h["page_table"][256, :2].tolist() == [4, 5] and many.stage.h["rb_req"][:2].tolist() == [256, 3]
+    with pytest.raises(IndexError):
+        many._fill([Segment(257, [1], 0, [1], True, uid=3)])
+    many.make_layout_buffers()
+    assert many.given.numel() == 257 * (many.max_pages + 1)

@@ -200,3 +200,16 @@ def test_engines_of_longer_texts_than_penalties_look_at_refuse_them_at_once(kind
             eng.add_request([1, 2, 3], wish)
     assert len(_run(eng, [([1, 2, 3], _sampling(max_tokens=3))])[0]) == 3
     runner.ws.check_status()
+
+
+def test_plain_steps_of_a_tree_executor_upload_no_more_than_others():
+    """The staging of 4 x 4 drafts a request: its plain steps upload a row of pages a request, and masks have a row a request."""
+    from cubic_serve_b200.executor.gpu_executor import GpuExecutor
+    from cubic_serve_b200.executor.spec_executor import NgramTreeSpeculativeGpuExecutor
+    _, _, runner = _engine("plain", False)
+    kw = dict(max_rows=64, max_prefill_tokens=512, max_model_len=4096)
+    plain, tree = GpuExecutor(runner, **kw), NgramTreeSpeculativeGpuExecutor(runner, 4, 4, **kw)
+    tree.capture_decode_graphs([4])
+    assert tree._mask_dev.shape[0] == 64
+    # two more pages a row for the drafts, and a row more; the arrays of sampled rows and of row blocks have 512 and 640 entries, of 68 and 16 bytes
+    assert tree.stage.nbytes <= plain.stage.nbytes + 4 * (65 * 258 - 64 * 256) + 96 * 512
