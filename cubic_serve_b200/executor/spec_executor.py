@@ -596,6 +596,7 @@ class NgramTreeSpeculativeGpuExecutor(NgramSpeculativeGpuExecutor):
         self._choices = torch.zeros(rows * nodes, dtype=torch.int32, device=dev)
         self._back = torch.zeros(rows * (depth + 2), dtype=torch.int32, device=dev)
         self._path = torch.zeros(rows, depth + 1, dtype=torch.int32, device=dev)
+        self._review_logits(min(rows * nodes, self.max_tokens))              # as many rows as a pass can have, before anything else takes the memory
         self._after_current_stream()
 
     def execute_speculative(self, segs: list[Segment], depths: list[int] | None = None, drafts: list[list[list[int]]] | None = None):

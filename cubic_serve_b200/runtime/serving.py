@@ -69,6 +69,15 @@ def plan_kv_pages(free_bytes: int, reserve_bytes: int, cfg, tp: int, k_bits: int
                                                                       state_snapshots)
 
 
+def request_buffers_bytes(max_running: int, max_model_len: int, max_tokens: int, vocab: int, depth: int = 0, branches: int = 1) -> int:
+    """Device memory beside the cache that an executor of one GPU takes for what requests may ask for: the texts that penalties look
+    at, and with drafts in trees (``branches`` > 1) the logits of a round."""
+    if branches <= 1:
+        return 0 if depth else 4 * max_running * (-(-max_model_len // 16) * 16)
+    nodes = 1 + depth * branches
+    return 4 * max_running * (-(-(max_model_len + nodes) // 16) * 16) + 2 * vocab * min(max_running * nodes, max_tokens)
+
+
 def build_backend(args, devices: list[int], tp: int, spec, k_bits: int, v_bits: int):
     import torch
 
@@ -187,6 +196,9 @@ def build_backend(args, devices: list[int], tp: int, spec, k_bits: int, v_bits: 
                 raise SystemExit(f"{adapters[0][0]} low-rank adapters of ranks up to {adapters[0][1]} take {held / 2 ** 30:.1f} GiB; "
                                  f"{max(0, free - reserve) / 2 ** 30:.1f} GiB are left beside weights and reserve (--low-rank-slots, --low-rank-max-rank)")
             reserve += held
+        drafted = spec is not None and getattr(spec, "method", "none") != "none"
+        reserve += request_buffers_bytes(args.max_running_requests, max_len, max(args.token_budget, args.max_running_requests), cfg.vocab_size,
+                                         getattr(spec, "num_speculative_tokens", 0) if drafted else 0, getattr(spec, "branches", 1) if drafted else 1)
         pages = plan_kv_pages(free, reserve, cfg, 1, k_bits, v_bits, max_len,
                               args.max_running_requests, state_snapshots=snapshots)
         runner = defn.build_runner(cfg, weights, num_pages=pages, max_tokens=args.token_budget, k_bits=k_bits, v_bits=v_bits,

@@ -213,3 +213,11 @@ def test_plain_steps_of_a_tree_executor_upload_no_more_than_others():
     assert tree._mask_dev.shape[0] == 64
     # two more pages a row for the drafts, and a row more; the arrays of sampled rows and of row blocks have 512 and 640 entries, of 68 and 16 bytes
     assert tree.stage.nbytes <= plain.stage.nbytes + 4 * (65 * 258 - 64 * 256) + 96 * 512
+
+
+def test_rounds_take_no_memory_of_their_own_for_their_logits():
+    eng, ex, runner = _engine("tree")
+    at = ex._rl.data_ptr()
+    assert ex._rl.shape == (8 * 13, VOCAB)
+    _run(eng, [(q, _sampling(max_tokens=33, logit_bias=((42, 100.0),))) for q in _prompts(8)])
+    assert ex.stats["rounds"] > 0 and ex._rl.data_ptr() == at and ex._rl.shape == (8 * 13, VOCAB)

@@ -210,3 +210,16 @@ def test_branches_on_the_command_line():
                 '{"method":"ngram","num_speculative_tokens":4,"branches":true}', '{"method":"mtp","num_speculative_tokens":4,"branches":2}'):
         with pytest.raises(argparse.ArgumentTypeError):
             parse_speculative_config(bad)
+
+
+def test_memory_of_what_requests_may_ask_for():
+    from cubic_serve_b200.executor.adjustments import Adjustments
+    from cubic_serve_b200.executor.gpu_executor import BatchBuilder
+    from cubic_serve_b200.runtime.serving import request_buffers_bytes
+
+    def histories(running, length):
+        return Adjustments(running, 16 * BatchBuilder(running, 64, length, 4, 2, "cpu").max_pages, "cpu").history.nbytes
+    assert request_buffers_bytes(8, 1000, 512, 2048) == histories(8, 1000)
+    assert request_buffers_bytes(8, 1000, 512, 2048, 4) == 0                                  # chains of drafts: neither
+    assert request_buffers_bytes(8, 1000, 512, 2048, 4, 4) == histories(8, 1017) + 2 * 2048 * 8 * 17
+    assert request_buffers_bytes(256, 8192, 8192, 151936, 7, 16) == histories(256, 8305) + 2 * 151936 * 8192       # a pass of 8192 rows
