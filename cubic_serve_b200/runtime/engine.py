@@ -389,12 +389,13 @@ class LLMEngine:
             from .ngram import NgramProposer
             self.ngram = NgramProposer(positions=getattr(self.executor, "draft_branches", 1))
         max_depth = getattr(self.executor, "draft_depth", max_depth)
+        # (trees take a list of continuations, also where it is at most one)
+        propose = self.ngram.propose_many if hasattr(self.executor, "draft_branches") else self.ngram.propose
         drafts = []
         for s in plan.segments:
             r = s.request
             room = max(0, r.sampling.max_tokens - len(r.output) - 1)
-            k = min(max_depth, room)
-            drafts.append(self.ngram.propose(r.request_id, r.tokens, k) if self.ngram.positions == 1 else self.ngram.propose_many(r.request_id, r.tokens, k))
+            drafts.append(propose(r.request_id, r.tokens, min(max_depth, room)))
         return self.executor.execute_speculative(segs, drafts=drafts)
 
     def generate(self, prompts: list[list[int]], sampling: SamplingParams | None = None) -> list[list[int]]:

@@ -223,3 +223,47 @@ def test_memory_of_what_requests_may_ask_for():
     assert request_buffers_bytes(8, 1000, 512, 2048, 4) == 0                                  # chains of drafts: neither
     assert request_buffers_bytes(8, 1000, 512, 2048, 4, 4) == histories(8, 1017) + 2 * 2048 * 8 * 17
     assert request_buffers_bytes(256, 8192, 8192, 151936, 7, 16) == histories(256, 8305) + 2 * 151936 * 8192       # a pass of 8192 rows
+
+
+class _TreeExecutor:
+    """An executor of rounds with trees without a GPU: the target says 7 over and over, and so every draft of it is accepted."""
+    draft_source, speculative_sampling, speculative_grammar = "ngram", False, False
+
+    def __init__(self, depth, branches):
+        self.draft_depth, self.draft_branches, self.speculative_depth = depth, branches, depth * branches
+        self.rounds, self.forgotten = [], []
+
+    def execute(self, segs):
+        return [7 for s in segs if s.sample]
+
+    def copy_pages(self, pairs):
+        pass
+
+    def invalidate_page_rows(self, slots):
+        self.forgotten += list(slots)
+
+    def execute_speculative(self, segs, depths=None, drafts=None):
+        self.rounds.append([(len(s.pages), s.start, [list(c) for c in d]) for s, d in zip(segs, drafts)])
+        out = []
+        for s, d in zip(segs, drafts):
+            tree = merge_drafts(d, max(0, len(s.pages) * 16 - s.start - 1))[0]
+            n = 0
+            while n < len(tree) - 1 and tree[n + 1] == 7:
+                n += 1
+            out.append([7] * (n + 1))
+        return out
+
+
+def _tree_engine(depth, branches, pages, requests=2, **kw):
+    from cubic_serve_b200.runtime.engine import LLMEngine
+    from cubic_serve_b200.runtime.scheduler import SchedulerConfig
+    ex = _TreeExecutor(depth, branches)
+    return LLMEngine(ex, pages, SchedulerConfig(max_running_requests=requests, max_model_len=512, max_batched_tokens=256, enable_prefix_cache=False)), ex
+
+
+@pytest.mark.parametrize("branches", [1, 4])
+def test_an_executor_of_trees_is_given_lists_of_continuations(branches):
+    from cubic_serve_b200.runtime.scheduler import SamplingParams
+    eng, ex = _tree_engine(3, branches, 64)
+    assert eng.generate([[7] * 9, [1, 2, 3]], SamplingParams(max_tokens=12, ignore_eos=True)) == [[7] * 12] * 2
+    assert any(d == [[7, 7, 7]] for r in ex.rounds for _, _, d in r)
