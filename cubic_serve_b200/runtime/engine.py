@@ -22,6 +22,7 @@ from .cache.pool import PagePool
 from .cache.prefix import PrefixCache
 from .scheduler import (AdmissionError, BatchPlan, ContinuousScheduler, FinishReason, Request, RequestStatus,
                         SamplingParams, SchedulerConfig)
+from .trees import merge_drafts
 
 
 @dataclass
@@ -55,7 +56,9 @@ class LLMEngine:
         self.prefix = PrefixCache(self.pool, enabled=self.cfg.enable_prefix_cache,
                                   checkpoint_slots=self.cfg.state_checkpoint_slots or None)
         self.scheduler = ContinuousScheduler(self.cfg, self.pool, self.prefix)
-        self.scheduler.decode_lookahead = getattr(executor, "speculative_depth", 0)
+        # drafts in trees are lent their pages once they are known, and have less room where there are none
+        self._lends_pages = hasattr(executor, "draft_branches")
+        self.scheduler.decode_lookahead = 0 if self._lends_pages else getattr(executor, "speculative_depth", 0)
         self.eos_token_id = eos_token_id
         # dynamic draft length (reference: runtime/speculative.py DynamicDraftPlanner.plan): per-request acceptance
         # history + measured round costs choose each request's draft length; off = the executor's fixed depth
@@ -327,6 +330,10 @@ class LLMEngine:
             else:
                 self.prefill_tokens += s.count
         finished = {r.request_id: r for r in self.scheduler.commit(plan, sampled, self.eos_token_id)}
+        if self._lends_pages:
+            back = [s.request.slot for s in plan.segments if s.sample and s.request.status is RequestStatus.RUNNING and self.scheduler.return_pages(s.request)]
+            if back:                     # the next pages there are others
+                self.executor.invalidate_page_rows(back)
         if self.scheduler.state_saves:
             # snapshots of the recurrent state at freshly published page boundaries (stream-ordered after the step)
             saves, self.scheduler.state_saves = self.scheduler.state_saves, []
@@ -396,6 +403,8 @@ class LLMEngine:
             r = s.request
             room = max(0, r.sampling.max_tokens - len(r.output) - 1)
             drafts.append(propose(r.request_id, r.tokens, min(max_depth, room)))
+            if self._lends_pages:
+                self.scheduler.lend_pages(r, len(merge_drafts(drafts[-1], self.executor.speculative_depth)[0]) - 1)
         return self.executor.execute_speculative(segs, drafts=drafts)
 
     def generate(self, prompts: list[list[int]], sampling: SamplingParams | None = None) -> list[list[int]]:

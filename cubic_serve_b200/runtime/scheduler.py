@@ -384,6 +384,24 @@ class ContinuousScheduler:
         scheduled.add(r.request_id)
         return True
 
+    # ------------------------------------------------------------- room for drafts
+    def lend_pages(self, r: Request, slots: int) -> None:
+        """Pages for up to ``slots`` drafts behind the request's next token, as many as can be had without preempting anybody."""
+        need = -(-(r.num_computed + 1 + slots) // BLOCK) - len(r.pages)
+        if need > 0:
+            if need > self.pool.num_free:
+                self.prefix.evict(need - self.pool.num_free)
+            r.pages.extend(self.pool.alloc(min(need, self.pool.num_free)))
+
+    def return_pages(self, r: Request) -> bool:
+        """Take back what a request's next token does not need; whether there was any."""
+        keep = -(-(r.num_computed + 1) // BLOCK)
+        spare = r.pages[keep:]
+        if spare:
+            self.pool.release(spare)
+            r.pages = r.pages[:keep]
+        return bool(spare)
+
     # ------------------------------------------------------------- imposed steps
     def imposed_plan(self, entries: list[tuple[Request, int]]) -> BatchPlan:
         """The plan of a step whose batch is given from outside: the next ``n`` tokens of every listed request, which are

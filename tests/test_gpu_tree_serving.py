@@ -221,3 +221,39 @@ def test_rounds_take_no_memory_of_their_own_for_their_logits():
     assert ex._rl.shape == (8 * 13, VOCAB)
     _run(eng, [(q, _sampling(max_tokens=33, logit_bias=((42, 100.0),))) for q in _prompts(8)])
     assert ex.stats["rounds"] > 0 and ex._rl.data_ptr() == at and ex._rl.shape == (8 * 13, VOCAB)
+
+
+@pytest.mark.parametrize("kb,vb,rotation", [(8, 8, False), (4, 8, True)])
+def test_what_rounds_leave_in_the_cache_is_read_on(kb, vb, rotation):
+    """Rounds of a biased token, whose drafts branch: most are wrong, some right ones lie behind wrong ones and move up, pages are lent and change hands.  Requests that
+    then go on from the cached texts without the bias say what logits of a plain pass over the whole text say, to the rounding of codes and logits."""
+    from cubic_serve_b200.executor.gpu_executor import Segment
+    eng, ex, runner = _engine("tree", kb=kb, vb=vb, rotation=rotation, prefix=True)
+    rng, prompts = np.random.default_rng(8), []
+    for i in range(6):
+        x = rng.integers(50, VOCAB, 40).tolist()
+        prompts.append([42] * 5 + x[:9] + [42, 42] + x[9:20] + [42] * 3 + x[20:20 + 3 * i] + [42, 42])
+    moved, keep = [], ex.execute_speculative
+
+    def recorded(segs, **kw):
+        out = keep(segs, **kw)
+        if ex.last_round["depth"]:
+            moved.extend(int(p[k]) != k for p, a in zip(ex._path.cpu().numpy(), ex.last_round["accepted"]) for k in range(1, a + 1))
+        return out
+    ex.execute_speculative = recorded
+    out = _run(eng, [(p, _sampling(max_tokens=30, logit_bias=((42, 100.0),))) for p in prompts])
+    assert all(o == [42] * 30 for o in out) and sum(moved) >= len(prompts) and ex.stats["accepted"] < ex.stats["proposed"]
+    texts = [p + o[:29] for p, o in zip(prompts, out)]
+    ids = [eng.add_request(t, _sampling(max_tokens=12)) for t in texts]
+    reqs = [eng.requests[i] for i in ids]
+    while eng.has_unfinished:
+        eng.step()
+    runner.ws.check_status()
+    _, pex, _ = _engine("plain", False, kb=kb, vb=vb, rotation=rotation)
+    for text, prompt, r in zip(texts, prompts, reqs):
+        assert r.num_cached_prefix == (len(text) - 1) // 16 * 16 > len(prompt) + 8             # lines that rounds wrote and moved
+        seq = text + r.output
+        offs = list(range(len(text) - 1, len(seq) - 1))
+        logits = pex.execute_logits([Segment(0, seq, 0, list(range(-(-len(seq) // 16))), True, uid=-1, logit_offsets=offs)])[0]
+        for x, t in zip(logits, r.output):
+            assert x[t] >= x.max() - np.abs(x).max() / (2 ** (min(kb, vb) - 1) - 1)

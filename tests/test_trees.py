@@ -267,3 +267,39 @@ def test_an_executor_of_trees_is_given_lists_of_continuations(branches):
     eng, ex = _tree_engine(3, branches, 64)
     assert eng.generate([[7] * 9, [1, 2, 3]], SamplingParams(max_tokens=12, ignore_eos=True)) == [[7] * 12] * 2
     assert any(d == [[7, 7, 7]] for r in ex.rounds for _, _, d in r)
+
+
+def test_drafts_in_trees_hold_pages_for_their_round_alone():
+    """Requests without a match hold what plain ones do; those with one are lent pages for what they draft, and give them back."""
+    from cubic_serve_b200.runtime.scheduler import SamplingParams
+    eng, ex = _tree_engine(7, 16, 64)
+    a, b = (eng.add_request(p, SamplingParams(max_tokens=40, ignore_eos=True)) for p in ([1, 2, 3, 4], [7, 7, 1, 2, 3, 4, 5, 6, 7, 7, 11, 12, 13, 14, 15, 16, 7, 7, 21, 22, 23, 24, 25, 26]))
+    a, b = eng.requests[a], eng.requests[b]
+    while eng.has_unfinished:
+        eng.step()
+        for r in (a, b):
+            assert len(r.pages) <= -(-(r.num_computed + 1) // 16)
+        assert eng.pool.num_used == len(a.pages) + len(b.pages)
+    assert a.output == b.output == [7] * 40
+    drafted = [(pages, start, len(merge_drafts(d, 112)[0])) for r in ex.rounds for pages, start, d in r]
+    assert {n > 1 for _, _, n in drafted} == {True, False}
+    assert all(pages == -(-(start + n) // 16) for pages, start, n in drafted), "as many slots as the drafts can take"
+    assert ex.forgotten, "rows of the block table whose pages were given back are written anew"
+
+
+def test_drafts_in_trees_preempt_nobody():
+    """Eight requests that repeat themselves in a pool that just holds their tokens: all drafts have less room, no request loses its place or its last tokens."""
+    from cubic_serve_b200.runtime.scheduler import SamplingParams
+    eng, ex = _tree_engine(7, 16, 1 + 8 * 4, requests=8)
+    reqs = [eng.requests[eng.add_request([7] * 9 + [i], SamplingParams(max_tokens=54, ignore_eos=True))] for i in range(8)]
+    while eng.has_unfinished:
+        eng.step()
+    assert [r.preemptions for r in reqs] == [0] * 8 and [r.output for r in reqs] == [[7] * 54] * 8
+    assert eng.steps < 54 and eng.pool.num_used == 0
+
+
+def test_drafts_in_trees_shorten_no_request():
+    """A request alone in a pool that its last token fills."""
+    from cubic_serve_b200.runtime.scheduler import SamplingParams
+    eng, ex = _tree_engine(7, 16, 1 + 3)
+    assert eng.generate([[7] * 9], SamplingParams(max_tokens=39, ignore_eos=True)) == [[7] * 39]
