@@ -759,8 +759,8 @@ class GpuExecutor:
         whole = True in [s.whole for s in segs]
         decode = (all(len(s.token_ids) == 1 for s in segs) and self.use_graphs and (self.graph_masks or not masked))
         adjusts = any(s.adjust is not None for s in segs)
-        # the budgets' state machine runs on the ids of the draw, inside the step
-        decode = decode and not ((whole or adjusts) and self.runner.reasoning is not None)
+        # the budgets' state machine runs on the ids of the draw from all tokens, inside the step
+        decode = decode and not (whole and self.runner.reasoning is not None)
         cap = self.graph_rt.dispatch(total) if decode else None
         if self._upload_pending:
             # the pinned staging buffer is rewritten below: the previous launch's upload must have left it
@@ -799,9 +799,16 @@ class GpuExecutor:
             if self.timing:
                 self._ev[k][0].record(self.stream)
             if cap is not None:
+                budget = self.runner.reasoning if adjusts else None
+                if budget is not None:
+                    budget.remember()
                 launches = self.graph_rt.replay(cap, self._leases[k]).launches
-                if adjusts:                    # behind the graph, whose sampler drew from the logits as they are
+                if adjusts:                    # behind the graph, whose sampler drew from the logits as they are, ...
                     launches += self.runner.adjust_and_draw(self.stage.d, self.logits, self.out_ids, rows)
+                if budget is not None:         # ... and whose budgets have counted what it drew
+                    budget.undo()
+                    budget.apply(self.out_ids, self.stage.d["row_slot"], self.stage.d["budget_init"], rows)
+                    launches += 1
                 if whole:                      # behind the graph, whose sampler drew these rows from the 20 best
                     self.runner.draw_whole(self.stage.d, self.logits, self.out_ids, rows)
                     launches += 1

@@ -1361,8 +1361,10 @@ class ReasoningBudget:
         self.end_token_id = int(end_token_id)
         self.forced = [int(t) for t in forced_tokens]
         self._seq = (ctypes.c_int * len(self.forced))(*self.forced)
-        self.left = torch.full((slots,), -1, dtype=torch.int32, device=device)
-        self.fpos = torch.zeros(slots, dtype=torch.int32, device=device)
+        self._state = torch.zeros(2, slots, dtype=torch.int32, device=device)
+        self._before = torch.zeros_like(self._state)
+        self.left, self.fpos = self._state
+        self.left.fill_(-1)
 
     def apply(self, ids: torch.Tensor, row_slot: torch.Tensor, init: torch.Tensor, rows: int) -> None:
         """Run the state machine on the step's ``rows`` sampled ids in place."""
@@ -1370,6 +1372,14 @@ class ReasoningBudget:
                                                 self.fpos.data_ptr(), rows, self.end_token_id, self._seq,
                                                 len(self.forced), _stream())
         native.check(code, "cb_reasoning_budget")
+
+    def remember(self) -> None:
+        """Keep the state of now for ``undo``."""
+        self._before.copy_(self._state)
+
+    def undo(self) -> None:
+        """The state of the last ``remember``: what ``apply`` did since, on ids that are drawn again, is done anew."""
+        self._state.copy_(self._before)
 
 
 # ------------------------------------------------------------------ layered decoders (models/layered.py)

@@ -257,3 +257,17 @@ def test_what_rounds_leave_in_the_cache_is_read_on(kb, vb, rotation):
         logits = pex.execute_logits([Segment(0, seq, 0, list(range(-(-len(seq) // 16))), True, uid=-1, logit_offsets=offs)])[0]
         for x, t in zip(logits, r.output):
             assert x[t] >= x.max() - np.abs(x).max() / (2 ** (min(kb, vb) - 1) - 1)
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_steps_with_penalties_and_thinking_budgets_replay_their_graphs(graphs):
+    """A budget counts what is drawn from the adjusted logits, once: tokens that a bias forces, an end that it brings, and neighbours that want nothing."""
+    eng, ex, runner = _engine("plain", graphs, reasoning=(5, [6, 5]))
+    p = _prompts(5)
+    out = _run(eng, [(p[0], _sampling(thinking_budget=7, logit_bias=((42, 100.0),))), (p[1], _sampling(thinking_budget=3)), (p[2], _sampling(thinking_budget=9, logit_bias=((5, 100.0),))),
+                     (p[3], _sampling(thinking_budget=0, logit_bias=((42, 100.0),))), (p[4], _sampling(logit_bias=((43, 100.0),)))])
+    assert out[0] == [42] * 7 + [6, 5] + [42] * 11 and out[1][3:5] == [6, 5]
+    assert out[2] == [5] * 20 and out[3] == [6, 5] + [42] * 18 and out[4] == [43] * 20
+    if graphs:
+        assert sum(s["replays"] for s in ex.graph_rt.stats()["slots"].values()) == 19                 # all but the prompts' step
+    runner.ws.check_status()
