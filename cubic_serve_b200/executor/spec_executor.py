@@ -610,7 +610,7 @@ class NgramTreeSpeculativeGpuExecutor(NgramSpeculativeGpuExecutor):
             room = len(s.pages) * K.PAGE_TOKENS - s.start - 1                # slots that the request has pages for
             trees.append(merge_drafts([c[:k] for c in d], max(0, min(most, room))))
         counts = [len(t) for t, _ in trees]
-        if max(counts, default=1) == 1:
+        if max(counts, default=1) == 1 or R > K.TREE_MAX_REQUESTS:           # (a launch takes no more)
             ids = self.execute(segs)
             self.last_round = {"depth": 0, "accepted": [0] * R, "proposed": [0] * R, "proposal_ms": 0.0,
                                "target_ms": self.device_ms[-1] if (self.timing and self.device_ms) else 0.0}

@@ -271,3 +271,14 @@ def test_steps_with_penalties_and_thinking_budgets_replay_their_graphs(graphs):
     if graphs:
         assert sum(s["replays"] for s in ex.graph_rt.stats()["slots"].values()) == 19                 # all but the prompts' step
     runner.ws.check_status()
+
+
+def test_more_requests_than_a_round_takes_run_plainly(monkeypatch):
+    from cubic_serve_b200.ops import kernels as K
+    monkeypatch.setattr(K, "TREE_MAX_REQUESTS", 4)
+    eng, ex, runner = _engine("tree")
+    p = _prompts(6)
+    wish = [_sampling(max_tokens=n, logit_bias=((42, 100.0),)) for n in (12, 12, 12, 12, 30, 30)]
+    assert _run(eng, list(zip(p, wish))) == [[42] * s.max_tokens for s in wish]
+    assert ex.stats["rounds"] > 0 and eng.steps >= 12 + 2
+    runner.ws.check_status()
