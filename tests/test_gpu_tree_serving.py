@@ -282,3 +282,31 @@ def test_more_requests_than_a_round_takes_run_plainly(monkeypatch):
     assert _run(eng, list(zip(p, wish))) == [[42] * s.max_tokens for s in wish]
     assert ex.stats["rounds"] > 0 and eng.steps >= 12 + 2
     runner.ws.check_status()
+
+
+def test_rounds_wait_for_constrained_and_sampling_requests():
+    """Beside a greedy request that repeats itself: as long as one with a grammar, or one that samples, runs, steps are plain ones, and the grammar holds."""
+    from cubic_serve_b200.generation.constraints import ChoiceMatcher
+
+    class Tok:
+        def encode(self, text, add_special_tokens=False):
+            return [100 + ord(c) for c in text]
+
+    for other in ("grammar", "sampling"):
+        eng, ex, runner = _engine("tree")
+        p, eos = _prompts(2), 3
+        options = ["alpha beta gamma", "alphabet soup, hot"]
+        sampling = _sampling(max_tokens=30, ignore_eos=False, stop_token_ids=(eos,), matcher=ChoiceMatcher(options, Tok(), eos), presence_penalty=0.5) if other == "grammar" \
+            else _sampling(max_tokens=17, temperature=0.9, seed=3)
+        a, b = (eng.requests[eng.add_request(q, s)] for q, s in ((p[0], sampling), (p[1], _sampling(max_tokens=60, logit_bias=((42, 100.0),)))))
+        while a.request_id in eng.requests:
+            assert ex.stats["rounds"] == 0
+            eng.step()
+        assert len(b.output) == len(a.output) >= 16
+        if other == "grammar":
+            assert a.output[-1] == eos and "".join(chr(t - 100) for t in a.output[:-1]) in options
+        steps = eng.steps
+        while eng.has_unfinished:
+            eng.step()
+        assert ex.stats["rounds"] > 0 and b.output == [42] * 60 and eng.steps - steps < 60 - len(a.output)
+        runner.ws.check_status()

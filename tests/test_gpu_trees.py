@@ -312,6 +312,47 @@ def test_attention_on_a_stream_and_in_a_graph():
     ws.check_status()
 
 
+@pytest.mark.parametrize("requests", [1, 90])
+@pytest.mark.parametrize("which,low,high", [(0, 0, 25), (1, 0, 25), (1, 25, 0), (0, 0, -40)])
+def test_scales_far_apart_of_items_of_both_tiles(requests, which, low, high):
+    """129 to 256 rows an item, in parts (one request) and whole: the program in 32 bits, each tile its own rows."""
+    rd = _Round([(200 - i % 3, (64, 40, 33)[i % 3]) for i in range(requests)], 4, 2, 8, 8, seed=22)
+    s = rd.scales()[which]
+    for i, (start, count) in enumerate(rd.sizes):
+        held = -(-(start + count) // 16)
+        for j in range(held):
+            page = int(rd.table[int(rd.slots[i]), j])
+            s[page] = (s[page].double() * 2.0 ** round(low + (high - low) * j / (held - 1))).float()
+    if which == 0:
+        rd.q = (rd.q.double() * 2.0 ** -max(low, high)).bfloat16()
+    rd.check()
+
+
+@pytest.mark.parametrize("which,bad", [(0, float("nan")), (1, float("nan")), (1, float("inf"))])
+def test_values_that_are_not_finite_in_items_of_both_tiles(which, bad):
+    """At a token of one context and at a node of another tree: 256 rows an item, whole ones and parts."""
+    rd = _Round([(70, 64)] * 70 + [(500, 64)], 4, 2, 8, 8, seed=23)
+    want = rd.run()
+    for req, tok in ((3, 33), (68, 70 + 5), (70, 100)):
+        scales = rd.scales()[which]
+        page = int(rd.table[int(rd.slots[req]), tok // 16])
+        old = scales[page, :, tok % 16].clone()
+        scales[page, :, tok % 16] = bad
+        out = rd.run()
+        scales[page, :, tok % 16] = old
+        node = tok - rd.sizes[req][0]
+        rows = np.arange(out.shape[0]) // 64 == req
+        if node >= 0:
+            rows &= (rd.sees[:, node >> 5] >> np.uint32(node & 31) & 1).astype(bool)
+        hit, others = torch.from_numpy(rows).to(DEV), torch.from_numpy(np.arange(out.shape[0]) // 64 != req).to(DEV)
+        assert rows.any() and not torch.isfinite(out[hit].float()).all(-1).any() and torch.isfinite(out[~hit].float()).all()
+        assert torch.equal(out[others], want[others])
+        # rows of the tree that do not see it: the same in 32 bits
+        ref, tol = rd.truth()
+        off = (out.cpu().double() - ref).abs()
+        assert bool((off <= tol + 1e-30)[~torch.from_numpy(rows)].all())
+
+
 def test_values_far_apart_behind_a_long_context():
     """A context of 160000 tokens whose scales take the program in 32 bits: all rows of an item of 256 by one CTA.
 
