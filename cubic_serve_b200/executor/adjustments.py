@@ -52,7 +52,7 @@ class Adjustments:
         ints = np.zeros((2, n), dtype=np.int32)                        # length, prompt
         floats = np.zeros((3, n), dtype=np.float32)                    # repetition, frequency, presence
         floats[0] = 1.0
-        where, what, bias = [], [], {}
+        where, what, bias, held = [], [], {}, {}
         for s in segs:
             a = s.adjust
             if a is None:
@@ -63,7 +63,7 @@ class Adjustments:
                 have = 0
             where.append(np.arange(slot * self.most + have, slot * self.most + L, dtype=np.int64))
             what.append(np.asarray(a.tokens[have:L], dtype=np.int32))
-            self._have[slot] = (s.uid, L)
+            held[slot] = (s.uid, L)
             ints[:, slot] = L, min(a.prompt, L)
             floats[:, slot] = a.repetition, a.frequency, a.presence
             if a.bias:
@@ -80,6 +80,8 @@ class Adjustments:
         d = self._upload(arrays)
         if d["where"].numel():
             self.history.view(-1).index_copy_(0, d["where"], d["what"])
+        for slot, have in held.items():          # (once the tokens are on their way: not if anything above failed)
+            self._have[slot] = have
         out = dict(request=d["request"], history=self.history, length=d["ints"][0], prompt=d["ints"][1], repetition=d["floats"][0], frequency=d["floats"][1],
                    presence=d["floats"][2])
         if bias:

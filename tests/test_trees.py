@@ -303,3 +303,15 @@ def test_drafts_in_trees_shorten_no_request():
     from cubic_serve_b200.runtime.scheduler import SamplingParams
     eng, ex = _tree_engine(7, 16, 1 + 3)
     assert eng.generate([[7] * 9], SamplingParams(max_tokens=39, ignore_eos=True)) == [[7] * 39]
+
+
+def test_tokens_that_could_not_be_staged_are_staged_by_the_next_step():
+    from types import SimpleNamespace as S
+
+    from cubic_serve_b200.executor.adjustments import Adjustment, Adjustments
+    a = Adjustments(2, 10, "cpu")
+    segs = [S(request_slot=0, uid=1, adjust=Adjustment([5, 6], 2)), S(request_slot=1, uid=2, adjust=Adjustment([7], 1, bias=((1 << 40, 1.0),)))]
+    with pytest.raises(OverflowError):
+        a.stage(segs)
+    segs[0].adjust.tokens.append(9)
+    assert a.stage(segs[:1])["length"].tolist() == [3, 0] and a.history[0, :3].tolist() == [5, 6, 9]
