@@ -128,7 +128,7 @@ __device__ __forceinline__ bool mbar_try_wait_hint(uint32_t bar, uint32_t parity
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool mbar_wait_park(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+__device__ __forceinline__ bool mbar_wait_park(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, long long budget = kWaitBudgetCycles) {
   if (mbar_try_wait(bar, parity)) return true;
   long long t0 = 0;
   uint32_t polls = 0;
@@ -139,7 +139,7 @@ __device__ __forceinline__ bool mbar_wait_park(uint32_t bar, uint32_t parity, vo
       const long long now = clock64();
       if (t0 == 0) {
         t0 = now;
-      } else if (now - t0 > kWaitBudgetCycles) {
+      } else if (now - t0 > budget) {
         *abort_flag = 1;
         return false;
       }

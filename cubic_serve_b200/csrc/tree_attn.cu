@@ -63,11 +63,10 @@ struct TreeLay {
                        vScale = vCode + kPageTokens * kD * VBITS / 8, bytes = vScale + kBytesOfScales, stride = (bytes + 127) & ~127;
 };
 
-// One row over the tokens [lo, hi) in fp32, by a warp whose lanes have four channels each.  `sees`: the row's words.  `alive` counts every 1024 tokens: the CTA's other
-// warps wait meanwhile, and their limit is one of time without progress.
+// One row over the tokens [lo, hi) in fp32, by a warp whose lanes have four channels each.  `sees`: the row's words.
 template <int KBITS, int VBITS>
 __device__ __forceinline__ void tree_row(const CbTreeAttn& p, const TreeRequest& r, int kvh, int lo, int hi, const uint32_t* sees, const __nv_bfloat16* q,
-                                         int lane, float& m, float& sum, float (&o)[4], bool& bad, uint32_t* alive) {
+                                         int lane, float& m, float& sum, float (&o)[4], bool& bad) {
   using L = TreeLay<KBITS, VBITS>;
   constexpr float kBias = 1 << (KBITS - 1), vBias = 1 << (VBITS - 1);
   const uint2 qw = reinterpret_cast<const uint2*>(q)[lane];
@@ -79,7 +78,6 @@ __device__ __forceinline__ void tree_row(const CbTreeAttn& p, const TreeRequest&
   for (int c = 0; c < 4; ++c) o[c] = 0.f;
 #pragma unroll 1
   for (int t = lo; t < hi; ++t) {
-    if (lane == 0 && (t & 1023) == 0) atomicAdd(alive, 1u);
     const int j = t - r.start;
     if (j >= 0 && !(sees[j >> 5] >> (j & 31) & 1u)) continue;
     const int page = tree_page(p, r.slot, t / kPageTokens, bad), tok = t % kPageTokens;
@@ -133,28 +131,14 @@ static constexpr int kTrApartK = 18, kTrApartV = 14;     // ... and the long one
 static constexpr int kTrHalf = kTrTok * 128;             // bytes of 64 channels of a step
 static constexpr uint32_t kTrTmemCols = 512, kTrTmemTile = 256, kTrTmemP = 64, kTrTmemQ = 96, kTrTmemO = 128;
 
-// A bounded wait with what follows when it is not over at once out of the way of the loops.  The limit starts anew while the word behind the abort flag (TrSmem::abort_flag[1]) counts:
-// rows of the fp32 program take 370 ns a token, so that 32 of them behind 130000 tokens are longer than the limit.
-__device__ __forceinline__ bool tr_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+// Waits of a launch are bounded by `limit`: a warp's 32 rows of the fp32 program take 720 cycles a row and token (pages in the L2 cache), behind 130000 tokens longer than other kernels' waits
+// may, so that the longest context there can be counts in it (tr_limit).  What follows a wait that is not over at once is out of the way of the loops.
+__device__ __forceinline__ bool tr_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, long long limit) {
   if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
-  long long t0 = 0;
-  uint32_t polls = 0, alive = 0;
-  while (true) {
-    if (mbar_try_wait_hint(bar, parity, 20000u)) return true;
-    if ((++polls & 0xFu) == 0) {
-      if (*abort_flag) return false;
-      const long long now = clock64();
-      const uint32_t counts = abort_flag[1];
-      if (t0 == 0 || counts != alive) {
-        t0 = now;
-        alive = counts;
-      } else if (now - t0 > kWaitBudgetCycles) {
-        *abort_flag = 1;
-        return false;
-      }
-    }
-  }
+  return mbar_wait_park(bar, parity, abort_flag, limit);
 }
+static constexpr long long kTrSlowCycles = 4096;         // of a row and token, with room to spare
+static inline long long tr_limit(const CbTreeAttn& p) { return kWaitBudgetCycles + 32 * kTrSlowCycles * kPageTokens * p.width; }
 // Where a role stands in a ring of n places, and the parity that it waits for there
 struct TrRing {
   int i, n;
@@ -190,7 +174,7 @@ struct __align__(1024) TrSmem {
   TrItem list[kTrLists];
   float2 exch_ml[kTrTiles][kTrRows];                     // rows in both tiles: maximum and sum, ...
   int exch_exp[kTrTiles][kTrRows];                       // ... and v_exp
-  uint32_t tmem, abort_flag[2];                          // [1]: progress of the fp32 program (tr_wait)
+  uint32_t tmem, abort_word;
   long long upto[kTreeMaxRequests + 1], items[kTreeMaxRequests + 1];     // units of the requests before; their items' units a slot
 };
 
@@ -411,13 +395,13 @@ __device__ __forceinline__ uint2 tr_visible(const uint32_t* sees, int words, int
 // Every wait is bounded; on a timeout the roles leave, the status word is set and tensor memory is freed.
 template <int KBITS, int VBITS>
 __global__ void __launch_bounds__(kTrThreads, 1)
-tree_kernel(const CbTreeAttn p, const int part_rows) {
+tree_kernel(const CbTreeAttn p, const int part_rows, const long long limit) {
   using L = TreeLay<KBITS, VBITS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   TrSmem& sm = *reinterpret_cast<TrSmem*>(smem_raw + (-smem_u32(smem_raw) & 1023u));      // (by way of an integer it would be a generic address)
   uint8_t* raw = reinterpret_cast<uint8_t*>(&sm + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv;
-  volatile uint32_t* abort_flag = sm.abort_flag;
+  volatile uint32_t* abort_flag = &sm.abort_word;
   float* part_o = p.partial;
   float2* part_ml = reinterpret_cast<float2*>(part_o + static_cast<size_t>(gridDim.x) * 2 * part_rows * kD);
   TrDesc* desc = reinterpret_cast<TrDesc*>(part_ml + static_cast<size_t>(gridDim.x) * 2 * part_rows);
@@ -450,7 +434,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
     }
     mbar_init(smem_u32(&sm.exch_full), 8);
     mbar_init(smem_u32(&sm.exch_free), 8);
-    sm.abort_flag[0] = sm.abort_flag[1] = 0;
+    sm.abort_word = 0;
     mbar_fence_init();
   }
   if (warp == 16) {
@@ -531,7 +515,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       };
       auto publish = [&](int n) {                        // the CTA's n-th item; false: there is none
         TrItem& to = sm.list[n % kTrLists];
-        if (ok && n >= kTrLists) ok = tr_wait(smem_u32(&sm.list_free[n % kTrLists]), (n / kTrLists - 1) & 1, abort_flag);
+        if (ok && n >= kTrLists) ok = tr_wait(smem_u32(&sm.list_free[n % kTrLists]), (n / kTrLists - 1) & 1, abort_flag, limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return false;
         TrItem l;
@@ -588,7 +572,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           if (s < l.steps) {
             if (s > 0 && s % 8 == 0) ids = ids_later;
             const int b = gs % kTrRaw;
-            if (ok && gs >= kTrRaw) ok = tr_wait(smem_u32(&sm.raw_free[b]), (gs / kTrRaw - 1) & 1, abort_flag);
+            if (ok && gs >= kTrRaw) ok = tr_wait(smem_u32(&sm.raw_free[b]), (gs / kTrRaw - 1) & 1, abort_flag, limit);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int n = min(kTrPages, pages - (l.lo + s) * kTrPages);
@@ -620,7 +604,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
 #pragma unroll 1
       for (int it = 0;; ++it) {
         const TrItem& l = sm.list[it % kTrLists];
-        if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+        if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag, limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok || l.kvh < 0) break;
         const int steps = l.steps;
@@ -628,7 +612,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
         bool v_wide = false;
 #pragma unroll 1
         for (int s = 0; s < steps; ++s, visible -= kTrTok) {
-          if (ok) ok = tr_wait(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag);
+          if (ok) ok = tr_wait(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag, limit);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const uint8_t* pages = raw + raw_at.i * kTrPages * L::stride;
@@ -689,14 +673,14 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
 #pragma unroll 1
       for (int it = 0;; ++it) {
         const TrItem& l = sm.list[it % kTrLists];
-        if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+        if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag, limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok || l.kvh < 0) break;
         const int steps = l.steps, first = tr_first(l, t, before);
         const bool split = tr_split(l);
         const int by = split ? 2 : 1;
         if (first < steps) {
-          if (ok) ok = tr_wait(smem_u32(&sm.q_full[t]), q_phase, abort_flag);
+          if (ok) ok = tr_wait(smem_u32(&sm.q_full[t]), q_phase, abort_flag, limit);
           q_phase ^= 1u;
         }
         // scores of step s, then the product of the one before: scores run ahead of their softmax
@@ -704,8 +688,8 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
         for (int s = first; s < steps + by && first < steps; s += by) {
           if (s < steps) {
             const int b = (before + s) & (kTrOpsK - 1);
-            if (ok) ok = tr_wait(smem_u32(&sm.k_full[t][b]), k_phase >> b & 1, abort_flag);
-            if (ok) ok = tr_wait(smem_u32(&sm.s_free[t]), s_phase, abort_flag);
+            if (ok) ok = tr_wait(smem_u32(&sm.k_full[t][b]), k_phase >> b & 1, abort_flag, limit);
+            if (ok) ok = tr_wait(smem_u32(&sm.s_free[t]), s_phase, abort_flag, limit);
             ok = __all_sync(0xffffffffu, ok);
             k_phase ^= 1u << b;
             s_phase ^= 1u;
@@ -724,8 +708,8 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           }
           if (s > first) {
             const int b = (before + s - by) & (kTrOpsV - 1);
-            if (ok) ok = tr_wait(smem_u32(&sm.v_full[t][b]), v_phase >> b & 1, abort_flag);
-            if (ok) ok = tr_wait(smem_u32(&sm.p_full[t]), p_phase, abort_flag);
+            if (ok) ok = tr_wait(smem_u32(&sm.v_full[t][b]), v_phase >> b & 1, abort_flag, limit);
+            if (ok) ok = tr_wait(smem_u32(&sm.p_full[t]), p_phase, abort_flag, limit);
             ok = __all_sync(0xffffffffu, ok);
             v_phase ^= 1u << b;
             p_phase ^= 1u;
@@ -757,7 +741,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
 #pragma unroll 1
     for (int it = 0;; ++it) {
       const TrItem& l = sm.list[it % kTrLists];
-      if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+      if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag, limit);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok || l.kvh < 0) break;
       const int steps = l.steps;
@@ -765,9 +749,9 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
       int visible = l.total - (l.lo + ahead) * kTrTok;
 #pragma unroll 1
       for (; ahead < steps; ahead += 2, visible -= 2 * kTrTok) {
-        if (ok) ok = tr_wait(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag);
-        if (ok) ok = tr_wait(smem_u32(&sm.note_full[note_at.i]), note_at.phase, abort_flag);
-        if (ok) ok = tr_wait(smem_u32(&sm.k_free[mine]), k_phase, abort_flag);
+        if (ok) ok = tr_wait(smem_u32(&sm.raw_full[raw_at.i]), raw_at.phase, abort_flag, limit);
+        if (ok) ok = tr_wait(smem_u32(&sm.note_full[note_at.i]), note_at.phase, abort_flag, limit);
+        if (ok) ok = tr_wait(smem_u32(&sm.k_free[mine]), k_phase, abort_flag, limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint8_t* pages = raw + raw_at.i * kTrPages * L::stride;
@@ -783,7 +767,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           mbar_arrive(smem_u32(&sm.k_full[mine][mine]));
           if (!split) mbar_arrive(smem_u32(&sm.k_full[1 - mine][mine]));
         }
-        ok = tr_wait(smem_u32(&sm.v_free[vb]), v_phase, abort_flag);
+        ok = tr_wait(smem_u32(&sm.v_free[vb]), v_phase, abort_flag, limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (__builtin_expect(!v_wide, 1)) tr_convert_v<KBITS, VBITS, false>(sm.v[vb], pages, visible, v_mul, ct);
@@ -818,7 +802,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
     // the row of the thread in item `it`, and Q of its tile; false: no more items
     auto begin = [&](int it, int before, Row& r) {
       const TrItem& l = sm.list[it % kTrLists];
-      if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag);
+      if (ok) ok = tr_wait(smem_u32(&sm.list_full[it % kTrLists]), (it / kTrLists) & 1, abort_flag, limit);
       ok = __all_sync(0xffffffffu, ok);
       r.q = r.out = -1;
       r.sees = p.masks;
@@ -885,7 +869,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
     int before = 0, n = 0, exchanges = 0;                // steps of earlier items; steps that this tile took part in; items in both tiles
     bool lent = false;                                   // the other tile may still read this one's output
     auto wait_lent = [&]() {
-      if (lent && ok) ok = tr_wait(smem_u32(&sm.exch_free), (exchanges - 1) & 1, abort_flag);
+      if (lent && ok) ok = tr_wait(smem_u32(&sm.exch_free), (exchanges - 1) & 1, abort_flag, limit);
       lent = false;
     };
     Row cur = {-1, -1, p.masks, 0.f};
@@ -902,7 +886,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
 #pragma unroll 1
         for (int s = first; s < steps; s += split ? 2 : 1) {
           const int tok0 = (l.lo + s) * kTrTok, note = (before + s) & (kTrNotes - 1);
-          if (ok) ok = tr_wait(smem_u32(&sm.s_full[t]), n & 1, abort_flag);
+          if (ok) ok = tr_wait(smem_u32(&sm.s_full[t]), n & 1, abort_flag, limit);
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
           if (__builtin_expect(tok0 + kTrTok > start, 0)) {                   // what a row does not see: -inf in place of its scores
@@ -951,7 +935,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           const float use = m == -INFINITY ? 0.f : m;
           const float2 less = make_float2(-use, -use), mul2 = make_float2(mul, mul);
           // the previous product has read the probabilities and written the output
-          if (ok && s > first) ok = tr_wait(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
+          if (ok && s > first) ok = tr_wait(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag, limit);
           if (s == first) wait_lent();
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
@@ -1001,7 +985,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           for (int j = 0; j < 16; ++j) reinterpret_cast<uint4*>(p.out + cur.out)[j] = make_uint4(0u, 0u, 0u, 0u);
         }
       } else {
-        if (ok && in) ok = tr_wait(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag);
+        if (ok && in) ok = tr_wait(smem_u32(&sm.pv_done[t]), (n - 1) & 1, abort_flag, limit);
         ok = __all_sync(0xffffffffu, ok);
         // what this tile's output and the other's are multiplied with
         float mul[2] = {pow2f(v_exp), 0.f};
@@ -1013,7 +997,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&sm.exch_full));
-          if (ok) ok = tr_wait(smem_u32(&sm.exch_full), exchanges & 1, abort_flag);
+          if (ok) ok = tr_wait(smem_u32(&sm.exch_full), exchanges & 1, abort_flag, limit);
           ok = __all_sync(0xffffffffu, ok);
           ++exchanges;
           lent = true;
@@ -1070,7 +1054,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
             const long long q = __shfl_sync(0xffffffffu, cur.q, of), out = __shfl_sync(0xffffffffu, cur.out, of);
             const uint32_t* sees = reinterpret_cast<const uint32_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(cur.sees), of));
             float rm, rs, o[4];
-            tree_row<KBITS, VBITS>(p, r, l.kvh, lo, hi, sees, p.q + q, lane, rm, rs, o, bad, sm.abort_flag + 1);
+            tree_row<KBITS, VBITS>(p, r, l.kvh, lo, hi, sees, p.q + q, lane, rm, rs, o, bad);
             if (part >= 0) {
               part_to[static_cast<size_t>(lane) * part_rows - lane + of] = make_float4(o[0], o[1], o[2], o[3]);
               if (lane == 0) part_ml[at - lane + of] = make_float2(rm, rs);
@@ -1096,7 +1080,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows) {
   __syncthreads();
   if (warp == 16) tmem_dealloc(tmem, kTrTmemCols);
   if (bad) atomicExch(p.status, static_cast<uint32_t>(kErrBadArgument));
-  if (tid == 0 && sm.abort_flag[0]) atomicExch(p.status, static_cast<uint32_t>(kErrBarrierTimeout));
+  if (tid == 0 && sm.abort_word) atomicExch(p.status, static_cast<uint32_t>(kErrBarrierTimeout));
 }
 
 // Joins the parts of items that several CTAs shared: block x looks after the item that began in CTA x and went on beyond it.  A warp's lanes are eight rows times four of
@@ -1186,7 +1170,7 @@ static int launch_tree(const CbTreeAttn& p, cudaStream_t st) {
     sms[dev] = n;
   }
   const int rows = tr_rows(p.words, p.rows, p.Hq / p.Hkv);
-  cudaError_t e = launch(tree_kernel<KB, VB>, dim3(sms[dev]), dim3(kTrThreads), smem, st, p, rows);
+  cudaError_t e = launch(tree_kernel<KB, VB>, dim3(sms[dev]), dim3(kTrThreads), smem, st, p, rows, tr_limit(p));
   const int step = rows <= kTrMergeFew ? 8 : 16;
   if (e == cudaSuccess) e = launch(step == 8 ? tree_merge_kernel<1, 8> : tree_merge_kernel<2, 4>, dim3(sms[dev], (rows + step - 1) / step), dim3(256), 0, st, p, rows);
   return static_cast<int>(e);
