@@ -117,28 +117,37 @@ keep_tokens_kernel(const CbKeepTokens p, const KvLayout lay) {
     const int layer = unit / p.Hkv, head = unit - layer * p.Hkv;
     uint8_t* cache = reinterpret_cast<uint8_t*>(p.caches[layer]);
     const int* table = p.table + slot * p.ld;
-    auto line = [&](int t) -> uint8_t* {                // blob of token t's page
+    auto page_of = [&](int t) {                          // -1: not there
       const int at = t / kPageTokens, page = at < p.width ? table[at] : -1;
-      return page >= 0 && page < p.pages ? cache + (static_cast<size_t>(page) * p.Hkv + head) * lay.blob_bytes : nullptr;
+      return page < p.pages ? page : -1;
     };
-    // the whole path before any line moves: it rises, and all its pages are there
-    for (int k = 1 + lane; k <= accepted; k += 32) {
-      const int at = path[k];
-      bad = bad || at <= (k > 1 ? path[k - 1] : 0) || at > (1 << 30) - start || (at != k && (line(start + at) == nullptr || line(start + k) == nullptr));
-    }
+    // a lane has a place of the path, and the pages of its line; the whole path is looked at before any line moves: it rises, and all its pages are there
+    int mine = 0, from_page = -1, to_page = -1;
+    auto look = [&](int k) {
+      if (k > accepted) return;
+      mine = path[k];
+      bad = bad || mine <= (k > 1 ? path[k - 1] : 0) || mine > (1 << 30) - start;
+      if (bad || mine == k) return;
+      from_page = page_of(start + mine);
+      to_page = page_of(start + k);
+      bad = from_page < 0 || to_page < 0;
+    };
+    for (int k0 = 1; k0 <= accepted; k0 += 32) look(k0 + lane);
     bad = __any_sync(0xffffffffu, bad);
+    auto blob = [&](int page) { return cache + (static_cast<size_t>(page) * p.Hkv + head) * lay.blob_bytes; };
     for (int k0 = 1; k0 <= accepted && !bad; k0 += kLines) {
+      if (accepted > 32 && k0 % 32 == 1) look(k0 + lane);
       uint32_t kc[kLines], vc[kLines];
       float ks[kLines], vs[kLines];
       uint8_t* to[kLines];
       int tok[kLines];
 #pragma unroll
       for (int l = 0; l < kLines; ++l) {
-        const int k = k0 + l, at = k <= accepted ? path[k] : k;
+        const int k = k0 + l, of = (k - 1) & 31, at = __shfl_sync(0xffffffffu, mine, of), fp = __shfl_sync(0xffffffffu, from_page, of), tp = __shfl_sync(0xffffffffu, to_page, of);
         to[l] = nullptr;
-        if (at == k) continue;
-        const uint8_t* from = line(start + at);
-        to[l] = line(start + k);
+        if (k > accepted || at == k) continue;
+        const uint8_t* from = blob(fp);
+        to[l] = blob(tp);
         const int src = (start + at) % kPageTokens;
         tok[l] = (start + k) % kPageTokens;
         kc[l] = pf_codes_k<KBITS>(from, src, lane);

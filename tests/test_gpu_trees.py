@@ -625,6 +625,25 @@ def test_paths_that_do_not_rise_and_pages_that_are_not_there_move_nothing_and_ar
         assert all(torch.equal(a, b) for a, b in zip(now, caches))
 
 
+@pytest.mark.parametrize("kb,vb", [(8, 8), (4, 6), (6, 4)])
+def test_kept_paths_longer_than_a_warp(kb, vb):
+    """32, 33 and 64 places, some of whose lines move and some stay, beside a short one."""
+    paths = [list(range(30)) + [33, 40, 63], list(range(20)) + list(range(21, 35)), [0] + list(range(30, 62)), [0] + list(range(1, 64)), [0, 2]]
+    n, hkv, start = len(paths), 2, 13
+    caches, table, path, accepted = _keep_case(n, start, hkv, kb, vb, paths, layers=2, seed=30 + kb)
+    before = [c.cpu().clone() for c in caches]
+    K.keep_tokens(K.LayerCaches(caches, hkv, D, kb, vb), _i32(table), _i32(np.arange(n)), _i32(np.full(n, start)), _i32(accepted), _i32(path))
+    K.workspace(torch.device(DEV, 0)).check_status()
+    for c, old in zip(caches, before):
+        for i, p in enumerate(paths):
+            for h in range(hkv):
+                new, was = ([torch.cat(x) for x in zip(*(eager.decode_cache_page(t[pg, h], D, kb, vb) for pg in table[i].tolist()))] for t in (c.cpu(), old))
+                for a, b in zip(new, was):
+                    ref = b.clone()
+                    ref[start:start + len(p)] = b[[start + node for node in p]]
+                    assert torch.equal(a, ref)
+
+
 @pytest.mark.parametrize("path,page", [([0, 3, 2], None), ([0, 2, 4, 6, 8, 8, 9], None), ([0, 2, 4, 6, 8, 9, -1], None), (list(range(0, 70, 2)) + [60], None),
                                        ([0, 3, 20], 1), ([0, 3, 4, 9, 20, 21], 1), ([0, 3, 4, 5, 6, 7, 8, 9, 40], 3)])
 def test_paths_that_are_wrong_further_on_move_nothing(path, page):
