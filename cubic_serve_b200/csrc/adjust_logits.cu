@@ -7,7 +7,8 @@
 // Bound by memory: a row is read and written once, 16 bytes at a time.  A block has a range of a row's tokens (16 KB of logits).  With its logits on their way it reads
 // the request's history, which is in the caches for the row's other blocks, and marks the tokens of its range that are in it; the first to mark one clears its word.
 // Then the logits are copied (in place: left), the words count, and the marked tokens are done by a thread each: few of a range are, but most warps would meet one (all
-// tokens through their words: 223 us for 624 rows of 151936, so 104, 3.6 TB/s).  256 rows of 151936 in place behind 1280 tokens: 53 us, 2.9 TB/s; one row: 5.
+// tokens through their words: 223 us for 624 rows of 151936, so 104, 3.6 TB/s).  256 rows of 151936 behind 1280 tokens, with biases and some masks, from one buffer to
+// another: 53 us, 2.9 TB/s; in place without masks, where only the marked tokens are touched, 30; 624 rows of trees in place 71; one row 5.
 #include "ptx.cuh"
 #include "launch.cuh"
 

@@ -200,6 +200,9 @@ static inline int tr_rows(int words, int rows, int G) {
 // operands hold is below 2^-2 and their scales are no more than 2^9 apart: below 2^-14 f16 has steps of 2^-24.
 // WIDE: the code as f16 (a subtraction) times sh + sl, f16 each: the product with sl, rounded, is 2^-11 of the whole, so that the multiply-add behind it rounds once
 // what 32-bit arithmetic would; values up to 2^15.
+// So keys and values have 10 to 11 bits here, where the prompt kernel keeps pairs of f16 (20 and 18); probabilities are f16 in both, their sum takes them in 32 bits.  On
+// caches as servers fill them the result's own rounding to bf16 is 1.66e-3 of it; what comes before adds 0.75 to 0.9e-3 with the short conversion, 0.46 to 0.6e-3 with the
+// long one throughout, which takes longer (64 x 16 behind 4096 279 us in place of 242, 32 x 64 128 for 122, 2 x 64 behind 32000 103 for 99), pairs of f16 twice the products.
 // What K holds of tokens that no row sees is masked with their scores.
 __device__ __forceinline__ void tr_put(uint32_t to, const uint4& x) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
@@ -387,10 +390,12 @@ __device__ __forceinline__ uint2 tr_visible(const uint32_t* sees, int words, int
 // than a factor of four: until then probabilities relative to the older maximum are at most 4.
 // Powers of two keep operands in the range of f16: a row's for Q (undone with the softmax' scale: its 8 bits stay exact), a step's for K (likewise), one for V that grows
 // with the largest scale (undone with the output).  Items whose scales are further apart than that holds (2^18 in a step of K, 2^14 in a CTA's steps of V), or not finite,
-// are computed in fp32 (tree_row): a hundred times as long, for caches as no model has them.
-// Bound by instructions: 16384 scores and as many codes a step of 256 rows take half of all issue slots, on five warps a scheduler whose programs differ, so that
-// fewer instructions of straight code are worth more than fewer cycles of one role (any role's loops unrolled: 3 to 11 % slower). Matrix units are busy for a quarter of the time, memory
-// for less: 64 x 16 behind 4096 (8 bits, 32 / 8 heads) 250 us, 2.6 TB/s of the cache; 2 x 64 behind 32000 (K 4 bits, 32 / 4) 101 us; 32 x 64 behind up to 1500 (6 bits, 64 / 4) 121 us.
+// are computed in fp32 (tree_row), a row at a time, 370 ns a token: a hundred times as long.  A group of zeros is stored with a scale of one, so that one of them among values
+// whose scales are below 2^-14 is enough for that.
+// Nothing is full: issue slots are half taken (16384 scores and as many codes a step of 256 rows, five warps a scheduler), matrix units for a quarter of the time, memory for as much.
+// What a step waits for is its own chain from role to role, and instructions: warps whose rows a narrow tree does not have run the softmax all the same, items of one
+// request convert the same pages anew, programs that differ share the instruction caches (any role's loops unrolled: 3 to 11 % slower; six more behind every wait: 9 %).
+// 64 x 16 behind 4096 (8 bits, 32 / 8 heads) 242 us, 2.6 TB/s of the cache; 2 x 64 behind 32000 (K 4 bits, 32 / 4) 100 us; 32 x 64 behind up to 1500 (6 bits, 64 / 4) 122 us.
 // One request of 8 nodes behind 700 tokens is a chain of latencies: 15 us, of which the second launch is 4.
 // Every wait is bounded; on a timeout the roles leave, the status word is set and tensor memory is freed.
 template <int KBITS, int VBITS>
@@ -944,7 +949,7 @@ tree_kernel(const CbTreeAttn p, const int part_rows, const long long limit) {
           for (int c = 0; c < 4; ++c) {
             uint32_t pr[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 8; ++j) {                // (f16: off by 2^-11 of itself, below 2^-14 by 2^-25; their sum has them as they are)
               const int at = c * 16 + 2 * j;
               const float2 d = __ffma2_rn(make_float2(__uint_as_float(a[at >> 5][at & 31]), __uint_as_float(a[at >> 5][(at & 31) + 1])), mul2, less);
               const float2 x = make_float2(fast_exp2(d.x), fast_exp2(d.y));

@@ -21,6 +21,7 @@ Optional capabilities (attribute -> meaning):
 * ``accepts_features``: segments may carry encoder feature rows and three-axis positions;
 * ``keeps_request_state``: the executor holds a request's context itself (no pages): the engine keeps prefix sharing off;
 * ``accepts_vocabulary_draws``: segments may draw from the whole vocabulary (``Segment.whole``, any ``top_k``, ``min_p``);
+* ``draft_branches``: rounds draft in trees (``execute_speculative(segments, drafts=)``: lists of continuations), no more than the segments' pages hold;
 * ``accepts_adjustments``: segments may carry penalties and biases of their logits (``Segment.adjust``);
 * ``low_rank`` + ``load_adapter(name, directory) / unload_adapter(name)``: segments may name a low-rank adapter's slot;
 * ``reasoning_end_id``: thinking budgets are enforced by the executor.

@@ -1020,8 +1020,8 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, page
     the whole context, and of its tree the nodes whose bits are set in its row of ``masks`` (int32 ``[rows, up to 8]``, bit ``j % 32`` of
     word ``j / 32``; usually its ancestors and itself: ``runtime.trees.tree_masks``).  A row that sees nothing becomes zeros; rows of no
     request stay.  ``q`` and ``out`` may be views of wider rows.  A request that is told wrongly (more nodes than ``masks`` has bits, a
-    context that its row of ``page_table`` does not hold) gets zeros, a page that is not there is read as page 0, and
-    ``ws.check_status`` raises in both cases.  Launches that may run at the same time need a ``ws`` of their own each."""
+    context that its row of ``page_table`` does not hold) gets zeros, one whose rows ``q`` does not have writes none, a page that is
+    not there is read as page 0, and ``ws.check_status`` raises in all cases.  Launches that may run at the same time need a ``ws`` of their own each."""
     n, i32 = request.numel(), torch.int32
     _require(head_dim == 128, "heads of 128 channels")
     _require(hkv > 0 and hq % hkv == 0 and hq // hkv <= TREE_MAX_GROUP, "query heads share the key / value heads evenly, up to 128 each")
@@ -1147,7 +1147,8 @@ def keep_tokens(caches: LayerCaches, page_table: torch.Tensor, request: torch.Te
 
     Of request ``i`` the line at slot ``start[i] + path[i, k]`` moves to ``start[i] + k``, ``0 < k <= accepted[i]``; ``path`` rises from
     0, as ``verify_tree`` leaves it.  ``request`` int32: rows of ``page_table``, none of them twice; the pages behind ``start`` are
-    the requests' own.  A path that does not rise and pages that are not there move nothing, and ``ws.check_status`` raises."""
+    the requests' own.  A path that does not rise throughout, or one of whose pages is not there, moves nothing, and
+    ``ws.check_status`` raises."""
     n, i32 = request.numel(), torch.int32
     ld, ldp = _rows(page_table, "page_table", i32), _rows(path, "path", i32)
     _require(path.shape[0] >= n and path.shape[1] >= 1, "path: a row of at least one node for every request")
