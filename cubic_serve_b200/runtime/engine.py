@@ -332,7 +332,7 @@ class LLMEngine:
         finished = {r.request_id: r for r in self.scheduler.commit(plan, sampled, self.eos_token_id)}
         if self._lends_pages:
             back = [s.request.slot for s in plan.segments if s.sample and s.request.status is RequestStatus.RUNNING and self.scheduler.return_pages(s.request)]
-            if back:                     # the next pages there are others
+            if back and hasattr(self.executor, "invalidate_page_rows"):              # the next pages there are others
                 self.executor.invalidate_page_rows(back)
         if self.scheduler.state_saves:
             # snapshots of the recurrent state at freshly published page boundaries (stream-ordered after the step)

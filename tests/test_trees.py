@@ -315,3 +315,14 @@ def test_tokens_that_could_not_be_staged_are_staged_by_the_next_step():
         a.stage(segs)
     segs[0].adjust.tokens.append(9)
     assert a.stage(segs[:1])["length"].tolist() == [3, 0] and a.history[0, :3].tolist() == [5, 6, 9]
+
+
+def test_an_executor_of_trees_without_a_block_table_of_its_own():
+    """Executors need not keep rows of pages (``models/protocol.py``)."""
+    from cubic_serve_b200.runtime.scheduler import SamplingParams
+    eng, ex = _tree_engine(7, 16, 64)
+    plain = type("PlainRows", (), {k: getattr(ex, k) for k in ("draft_source", "speculative_sampling", "speculative_grammar", "draft_depth", "draft_branches", "speculative_depth", "execute",
+                                                              "copy_pages", "execute_speculative")})()
+    eng.executor = plain
+    prompt = [7, 7, 1, 2, 3, 4, 5, 6, 7, 7, 11, 12, 13, 14, 15, 16, 7, 7, 21, 22, 23, 24, 25, 26]
+    assert eng.generate([prompt], SamplingParams(max_tokens=20, ignore_eos=True)) == [[7] * 20]
